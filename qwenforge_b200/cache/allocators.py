@@ -47,31 +47,60 @@ class SlotAllocator:
 
 
 class PageAllocator:
-    """Pages 0..n-1 of one group's storage."""
+    """Pages 0..n-1 of one group's storage. A page has one holder when it is taken; `share` adds holders (sequences that
+    begin with the same positions), and it is free again when the last of them has given it back."""
 
     def __init__(self, n_pages: int):
         if n_pages <= 0:
             raise ValueError("a cache group needs at least one page")
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))
-        self._held = [False] * n_pages
+        self._holders = [0] * n_pages
+        self.n_shared = 0   # pages with more than one holder
 
     @property
     def n_free(self) -> int:
         return len(self._free)
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
 
     def take(self, count: int) -> list[int]:
         if count > len(self._free):
             raise CacheFull(f"{count} cache pages wanted, {len(self._free)} of {self.n_pages} free")
         pages = [self._free.pop() for _ in range(count)]
         for p in pages:
-            self._held[p] = True
+            self._holders[p] = 1
         return pages
+
+    def _check_held(self, page: int) -> None:
+        if not (0 <= page < self.n_pages) or not self._holders[page]:
+            raise CacheMisuse(f"page {page} is not held (released twice, or never taken)")
+
+    def share(self, pages, count: int = 1) -> None:
+        """`count` further holders for each of these pages."""
+        for p in pages:
+            self._check_held(p)
+            self.n_shared += self._holders[p] == 1 and count > 0
+            self._holders[p] += count
 
     def give_back(self, pages) -> None:
         pages = list(pages)
+        freed = []
         for p in pages:
-            if not (0 <= p < self.n_pages) or not self._held[p]:
-                raise CacheMisuse(f"page {p} is not held (released twice, or never taken)")
-            self._held[p] = False
-        self._free.extend(sorted(pages, reverse=True))
+            self._check_held(p)
+            self._holders[p] -= 1
+            self.n_shared -= self._holders[p] == 1
+            if not self._holders[p]:
+                freed.append(p)
+        self._free.extend(sorted(freed, reverse=True))
+
+    def compact(self) -> list[tuple[int, int]]:
+        """(from, to) pairs after which the held pages are 0..held-1; the allocator counts them as moved."""
+        held = self.n_pages - len(self._free)
+        behind = [p for p in range(held, self.n_pages) if self._holders[p]]
+        moves = list(zip(behind, sorted(p for p in self._free if p < held)))
+        for old, new in moves:
+            self._holders[new], self._holders[old] = self._holders[old], 0
+        self._free = list(range(self.n_pages - 1, held - 1, -1))
+        return moves

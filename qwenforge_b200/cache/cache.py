@@ -26,6 +26,10 @@ pages, page table and page allocator). A group with a window gives pages back as
 every position on them has left the window, so in steady state a sequence holds about
 window / PAGE_TOKENS + 1 pages there.
 
+A sequence may be forked (`fork`): the new ones hold its whole pages with it (a page counts its holders) and get copies of the page
+that is still being filled and of the fixed-size state. So a page at or behind a sequence's length is always its own, and no write
+reaches a page that two sequences hold. `rewind` drops a sequence's last positions, `compact` moves the held pages to the front.
+
 The state that decoding itself keeps per sequence (latest token, position, step count, budget)
 lives in the decode graph's own device buffers (`engine/graphs.py`); this cache holds only what
 the model's mixers declare.
@@ -37,6 +41,7 @@ from typing import Optional, Sequence
 
 import torch
 
+from .. import ops
 from .allocators import CacheFull, CacheMisuse, PageAllocator, SlotAllocator
 
 PAGE_TOKENS = 64
@@ -199,6 +204,70 @@ class KvGroup:
     def pages_held(self, slot: int) -> int:
         return len(self._held[slot])
 
+    def _put(self, slot: int, logical: int, page: int) -> None:
+        self._held[slot][logical] = page
+        self._host_table[slot, logical] = page
+        self._dirty.add(slot)
+
+    def filling(self, slot: int, length: int) -> Optional[int]:
+        """The logical page that a sequence of `length` positions has begun and not filled (None: there is none, or it is not held)."""
+        rows = self.need.rows(length)
+        return rows // PAGE_TOKENS if rows % PAGE_TOKENS and rows // PAGE_TOKENS in self._held[slot] else None
+
+    def fork(self, slot: int, length: int, forks: Sequence[int]) -> None:
+        """The slots of `forks` (which hold nothing) get the pages that `slot` has filled, and a copy each of the one it is filling."""
+        held, whole = self._held[slot], self.need.rows(length) // PAGE_TOKENS
+        kept = {lp: page for lp, page in held.items() if lp < whole}
+        self.pages.share(kept.values(), len(forks))
+        partial = self.filling(slot, length)
+        copies = self.pages.take(len(forks)) if partial is not None else []
+        for i, fork in enumerate(forks):
+            for lp, page in kept.items():
+                self._put(fork, lp, page)
+            if partial is not None:
+                self._put(fork, partial, copies[i])
+        if copies:
+            ops.copy_pages(self.storage, [(held[partial], page, self.need.rows(length) % PAGE_TOKENS) for page in copies])
+
+    def rewind_missing(self, slot: int, length: int) -> bool:
+        """Whether a page that a sequence of `length` positions still needs has been given back."""
+        first = self.first_needed(length)
+        rows = self.need.rows(length)
+        return rows > first and bool(self.pages_missing(slot, first, rows))
+
+    def shares_filling(self, slot: int, length: int) -> bool:
+        """Whether the page in which `length` ends is one that other sequences hold too."""
+        partial = self.filling(slot, length)
+        return partial is not None and self.pages.holders(self._held[slot][partial]) > 1
+
+    def rewind(self, slot: int, length: int) -> None:
+        """Back to `length` positions: pages behind it are given back, and the one it ends in becomes the slot's own."""
+        held, rows = self._held[slot], self.need.rows(length)
+        if self.shares_filling(slot, length):
+            partial = rows // PAGE_TOKENS
+            old, (new,) = held[partial], self.pages.take(1)
+            ops.copy_pages(self.storage, [(old, new, rows % PAGE_TOKENS)])
+            self.pages.give_back([old])
+            self._put(slot, partial, new)
+        gone = [lp for lp in held if lp * PAGE_TOKENS >= rows]
+        if gone:
+            self.pages.give_back([held.pop(lp) for lp in gone])
+            for lp in gone:
+                self._host_table[slot, lp] = -1
+            self._dirty.add(slot)
+
+    def compact(self) -> int:
+        """Held pages to the front of the storage; returns how many moved."""
+        moves = self.pages.compact()
+        if moves:
+            ops.copy_pages(self.storage, moves)
+            to = dict(moves)
+            for slot, held in enumerate(self._held):
+                for lp, page in held.items():
+                    if page in to:
+                        self._put(slot, lp, to[page])
+        return len(moves)
+
     def flush(self) -> None:
         """Bring the device page table up to date with the host's (rows that changed since the last call)."""
         if not self._dirty:
@@ -223,6 +292,9 @@ class StateGroup:
 
     def reset(self, slot: int) -> None:
         self.storage[:, slot].zero_()
+
+    def fork(self, slot: int, forks: Sequence[int]) -> None:
+        ops.copy_pages(self.storage, [(slot, fork) for fork in forks])
 
 
 class StateSite:
@@ -259,6 +331,7 @@ class SequenceCache:
         pages_per_seq = self.max_len // PAGE_TOKENS
         self.slots = SlotAllocator(self.max_seqs)
         self.lengths = [0] * self.max_seqs
+        self._shared: dict = {}   # batch (slots) -> what its sequences share
 
         # who keeps what: (schedule entry, path of names inside its bundle; () for an entry with one need) per need
         by_need: dict[object, list[tuple]] = {}
@@ -353,6 +426,96 @@ class SequenceCache:
             group.release(slot)
         self.lengths[slot] = 0
         self.slots.give_back(slot)
+        self._shared.clear()
+
+    # ------------------------------------------------------------------ branches
+    def fork(self, slot: int, count: int = 1) -> list[int]:
+        """Start `count` sequences that continue where `slot` stands: its positions (whole pages shared, the begun one copied) and its
+        fixed-size state. Pages that `slot` has reserved ahead stay its own. All or nothing: CacheFull leaves everything as it was."""
+        self._check_held(slot)
+        if count < 0:
+            raise ValueError("fork: count must be >= 0")
+        if count > self.slots.n_free:
+            raise CacheFull(f"{count} sequence slots wanted, {self.slots.n_free} of {self.max_seqs} free")
+        length = self.lengths[slot]
+        for group in self.kv_groups:
+            if group.filling(slot, length) is not None and count > group.pages.n_free:
+                raise CacheFull(f"{count} cache pages wanted, {group.pages.n_free} of {group.pages.n_pages} free")
+        if count == 0:
+            return []
+        forks = [self.slots.take() for _ in range(count)]
+        for group in self.kv_groups:
+            group.fork(slot, length, forks)
+        for group in self.state_groups:
+            group.fork(slot, forks)
+        for fork in forks:
+            self.lengths[fork] = length
+        self._shared.clear()
+        return forks
+
+    def rewind(self, slot: int, length: int) -> None:
+        """Drop the positions of `slot` from `length` on (drafted tokens that were refused); pages behind it become free, those that were
+        reserved ahead among them. Not possible where something cannot go back: a fixed-size state, or positions that a window has
+        given up since. All or nothing."""
+        self._check_held(slot)
+        if not 0 <= length <= self.lengths[slot]:
+            raise ValueError(f"rewind: length {length} outside 0 .. {self.lengths[slot]}")
+        if length < self.lengths[slot]:
+            if self.state_groups:
+                raise CacheMisuse("rewind: a state of fixed size cannot go back")
+            if any(group.rewind_missing(slot, length) for group in self.kv_groups):
+                raise CacheMisuse(f"rewind: positions that a query at {length} sees have left their window and were given up")
+        for group in self.kv_groups:
+            if group.shares_filling(slot, length) and not group.pages.n_free:
+                raise CacheFull(f"1 cache page wanted, 0 of {group.pages.n_pages} free")
+        for group in self.kv_groups:
+            group.rewind(slot, length)
+        self.lengths[slot] = length
+        self._shared.clear()
+
+    def compact(self) -> int:
+        """Move the held pages of every group to the front of its storage, so that all behind them is free; the page tables on the
+        device follow at once. Returns how many pages moved."""
+        moved = sum(group.compact() for group in self.kv_groups)
+        self.flush()
+        return moved
+
+    def pages_used(self) -> list[int]:
+        """Per group of keys and values, the held pages (a shared one counts once)."""
+        return [group.pages.n_pages - group.pages.n_free for group in self.kv_groups]
+
+    def shared_groups(self, slots: Sequence[int]) -> list[tuple]:
+        """Which sequences of a batch begin with the same pages: (batch entries, pages) for every two or more that do, as
+        `ops.SharedPrefix` takes them. Only positions that every later query sees count (keys and values without a window)."""
+        group = next((g for g in self.kv_groups if g.need.window <= 0 and g.need.chunk <= 0 and g.need.every == 1), None)
+        if group is None or not group.pages.n_shared:
+            return []
+        families: dict = {}
+        for entry, slot in enumerate(slots):
+            if slot >= 0 and 0 in group._held[slot]:
+                families.setdefault(group._held[slot][0], []).append(entry)
+        found = []
+        for entries in families.values():
+            if len(entries) < 2:
+                continue
+            whole = min(self.lengths[slots[e]] for e in entries) // PAGE_TOKENS
+            rows = group._host_table[[slots[e] for e in entries], :whole]
+            same = (rows == rows[0]).all(0)
+            pages = whole if bool(same.all()) else int(same.to(torch.int8).argmin())
+            if pages > 0:
+                found.append((entries, pages))
+        return found
+
+    def shared_prefix(self, slots: Sequence[int]):
+        """`ops.SharedPrefix` of a batch whose sequences begin with the same pages, or None. Kept for a batch that comes back, until a
+        sequence is forked, rewound or closed."""
+        key = tuple(slots)
+        if key not in self._shared:
+            if len(self._shared) >= 256:
+                self._shared.clear()
+            groups = self.shared_groups(key)
+            self._shared[key] = ops.SharedPrefix(groups, len(key), self.device) if groups else None
+        return self._shared[key]
 
     def flush(self) -> None:
         for group in self.kv_groups:

@@ -7,24 +7,7 @@
 #include <float.h>
 
 #include "common.cuh"
-
-__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
-    x ^= x >> 16;
-    x *= 0x7FEB352Du;
-    x ^= x >> 15;
-    x *= 0x846CA68Bu;
-    x ^= x >> 16;
-    return x;
-}
-
-__device__ __forceinline__ uint32_t row_key(unsigned long long seed, long long seq_id, int step) {
-    uint32_t key = mix32((uint32_t)seed ^ 0x9E3779B9u);
-    key = mix32(key ^ (uint32_t)(seed >> 32));
-    key = mix32(key ^ (uint32_t)seq_id);
-    key = mix32(key ^ (uint32_t)((unsigned long long)seq_id >> 32) ^ 0x85EBCA6Bu);
-    key = mix32(key ^ (uint32_t)step);
-    return key;
-}
+#include "random.cuh"
 
 // One block scans a chunk of one row's vocabulary; with several chunks per row the blocks leave their best
 // (score, id) in scratch and take a ticket, and the block that draws the row's last ticket picks the row's best
@@ -49,8 +32,7 @@ sample_kernel(const float* __restrict__ logits, int vocab, long long row_stride,
     int bi = 0x7fffffff;
     auto consider = [&](float s, int i) {
         if (sample) {
-            const uint32_t bits = mix32(key ^ mix32((uint32_t)i ^ 0x27D4EB2Fu));
-            const float u = ((float)(bits >> 9) + 0.5f) * (1.0f / 8388608.0f);
+            const float u = ((float)token_bits(key, (uint32_t)i) + 0.5f) * (1.0f / 8388608.0f);
             s = s * inv_t - logf(-logf(u));
         }
         if (s > bv || (s == bv && i < bi)) {
