@@ -49,8 +49,13 @@ class ModelStepper:
     def reserve(self, slot_totals) -> None:
         self.cache.reserve(list(slot_totals))
 
-    def step_and_choose(self, entries, seq_ids, steps) -> list[int]:
+    def fork(self, slot: int, count: int) -> list[int]:
+        return self.cache.fork(slot, count)
+
+    def step_and_choose(self, entries, seq_ids, steps, continuations: int = 1) -> list[int]:
         logits = self.model.step(self.cache, entries)
+        if continuations > 1:
+            logits = logits.repeat_interleave(continuations, 0)
         device = logits.device
         ids = steps_t = None
         if not self.sampler.greedy:
@@ -79,7 +84,8 @@ class _GraphSession:
         self.stepper = stepper
         self.slots = [r[0] for r in rows]
         longest = max(cache.lengths[slot] + (budget - made) for slot, _, _, made, budget in rows)
-        self.graph = stepper.graph_decoder.get(len(rows), longest, stepper.sampler)
+        shared = cache.shared_prefix(self.slots) if hasattr(cache, "shared_prefix") else None
+        self.graph = stepper.graph_decoder.get(len(rows), longest, stepper.sampler, *(() if shared is None else (shared,)))
         cache.flush()
         self.graph.load(self.slots, [r[1] for r in rows], [cache.lengths[r[0]] for r in rows], [r[3] for r in rows],
                         [r[4] for r in rows], [r[2] for r in rows], stop_token_ids)
@@ -127,13 +133,15 @@ class StudentEngine:
         self.last_loop: Optional[GenerationLoop] = None
 
     # ------------------------------------------------------------------ cache sizing
-    def _ensure_cache(self, prompt_lengths: Sequence[int], budgets: Sequence[int], batch_size: int) -> None:
+    def _ensure_cache(self, prompt_lengths: Sequence[int], budgets: Sequence[int], batch_size: int, continuations: int = 1) -> None:
         """A cache that holds the largest batch of this call; kept and reused while it is large enough."""
         need_tokens = need_seqs = 0
         for begin in range(0, len(prompt_lengths), batch_size):
             chunk = range(begin, min(begin + batch_size, len(prompt_lengths)))
             tokens = sum(round_up(max(prompt_lengths[i], 1) + max(budgets[i], 1), PAGE_TOKENS) for i in chunk)
-            need_tokens, need_seqs = max(need_tokens, tokens), max(need_seqs, len(chunk))
+            # (a further continuation holds the pages behind the prompt's whole ones)
+            tokens += (continuations - 1) * sum(round_up(max(prompt_lengths[i], 1) % PAGE_TOKENS + max(budgets[i], 1), PAGE_TOKENS) for i in chunk)
+            need_tokens, need_seqs = max(need_tokens, tokens), max(need_seqs, len(chunk) * continuations)
         if self._max_cache_tokens is not None:
             if need_tokens > self._max_cache_tokens:
                 raise CacheFull(f"a batch of this call needs {need_tokens} cache tokens; "
@@ -153,14 +161,16 @@ class StudentEngine:
     @torch.inference_mode()
     def generate_ids(self, prompts: Sequence[Sequence[int]], max_new_tokens, batch_size: int = 1,
                      temperature: float = 0.0, seed: Optional[int] = None,
-                     stop_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False) -> list[list[int]]:
+                     stop_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False, continuations: int = 1) -> list[list[int]]:
         return [r.tokens for r in self.generate_results(prompts, max_new_tokens, batch_size, temperature, seed,
-                                                        stop_token_ids, ignore_eos)]
+                                                        stop_token_ids, ignore_eos, continuations)]
 
     @torch.inference_mode()
     def generate_results(self, prompts, max_new_tokens, batch_size: int = 1, temperature: float = 0.0,
                          seed: Optional[int] = None, stop_token_ids: Optional[Sequence[int]] = None,
-                         ignore_eos: bool = False) -> list[SequenceResult]:
+                         ignore_eos: bool = False, continuations: int = 1) -> list[SequenceResult]:
+        """`continuations` > 1: so many results per prompt, one after another, each with random numbers of its own; a prompt runs once and
+        its continuations share its cache pages."""
         prompts = [list(p) for p in prompts]
         if not prompts:
             return []
@@ -168,12 +178,12 @@ class StudentEngine:
         budgets = [int(max_new_tokens)] * n if isinstance(max_new_tokens, int) else [int(b) for b in max_new_tokens]
         size = max(int(batch_size), 1)
         stops = self.model.spec.stop_token_ids if stop_token_ids is None else tuple(stop_token_ids)
-        self._ensure_cache([len(p) for p in prompts], budgets, size)
+        self._ensure_cache([len(p) for p in prompts], budgets, size, int(continuations))
         sampler = Sampler(SamplingParams(float(temperature), self.seed if seed is None else int(seed)))
         loop = GenerationLoop(ModelStepper(self.model, self.cache, sampler, self.graph_decoder), stops, ignore_eos,
                               getattr(self.tokenizer, "bos_token_id", None))
         self.last_loop = loop
-        return loop.run(prompts, budgets, size)
+        return loop.run(prompts, budgets, size, int(continuations))
 
     # ------------------------------------------------------------------ strings
     @torch.inference_mode()

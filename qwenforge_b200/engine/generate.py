@@ -33,6 +33,9 @@ class Stepper(Protocol):
     def step_and_choose(self, entries: Sequence[tuple[int, Sequence[int]]], seq_ids: Sequence[int],
                         steps: Sequence[int]) -> list[int]: ...
 
+    # For several continuations of a prompt: `step_and_choose` with a fourth argument n chooses n tokens from each entry's logits
+    # (seq_ids and steps then hold n per entry), and `fork(slot, count)` starts `count` sequences where `slot` stands.
+
     # Optional: a stepper may also offer `open_decode_session(rows, stop_token_ids)`, with rows of
     # (slot, latest token, sequence id, tokens generated so far, budget). It returns None, or an object whose
     # `run(n)` performs up to n single-token steps for all rows without the host in between and returns, per
@@ -68,21 +71,24 @@ class GenerationLoop:
     def _stops(self, token: int) -> bool:
         return not self.ignore_eos and token in self.stop_token_ids
 
-    def run(self, prompts: Sequence[Sequence[int]], max_new_tokens, batch_size: int = 1) -> list[SequenceResult]:
-        """prompts: token ids per request; max_new_tokens: one budget for all or one per request."""
+    def run(self, prompts: Sequence[Sequence[int]], max_new_tokens, batch_size: int = 1, continuations: int = 1) -> list[SequenceResult]:
+        """prompts: token ids per request; max_new_tokens: one budget for all or one per request. `continuations` results per request,
+        in its place one after another: the prompt runs once, and its sequence is forked behind it."""
         n = len(prompts)
+        if continuations < 1:
+            raise ValueError("continuations must be >= 1")
         budgets = [int(max_new_tokens)] * n if isinstance(max_new_tokens, int) else [int(b) for b in max_new_tokens]
         if len(budgets) != n:
             raise ValueError("max_new_tokens must be one number or one per prompt")
-        results = [SequenceResult() for _ in range(n)]
+        results = [SequenceResult() for _ in range(n * continuations)]
         self.steps_run = self.prompt_steps_run = self.decoded_tokens = 0
         self.decode_seconds = 0.0
         size = max(int(batch_size), 1)
         for begin in range(0, n, size):
-            self._run_batch(list(range(begin, min(begin + size, n))), prompts, budgets, results)
+            self._run_batch(list(range(begin, min(begin + size, n))), prompts, budgets, results, continuations)
         return results
 
-    def _run_batch(self, indices, prompts, budgets, results) -> None:
+    def _run_batch(self, indices, prompts, budgets, results, continuations: int = 1) -> None:
         stepper = self.stepper
         batch = []
         for i in indices:
@@ -92,7 +98,8 @@ class GenerationLoop:
                     raise ValueError("Cannot generate from an empty prompt without a BOS token")
                 tokens = [self.bos_token_id]
             if budgets[i] <= 0:
-                results[i].finish_reason = "length"
+                for result in results[i * continuations:(i + 1) * continuations]:
+                    result.finish_reason = "length"
                 continue
             if len(tokens) + budgets[i] > stepper.max_positions:
                 raise ValueError(f"Requested sequence length {len(tokens) + budgets[i]} "
@@ -103,11 +110,21 @@ class GenerationLoop:
         live: list[_Live] = []
         try:
             for i, tokens in batch:
-                live.append(_Live(i, stepper.open(), budgets[i], results[i]))
+                live.append(_Live(i * continuations, stepper.open(), budgets[i], results[i * continuations]))
             # room for every sequence's whole future, so that no later step can run out of cache
             stepper.reserve([(s.slot, len(tokens) + s.budget - 1) for s, (_, tokens) in zip(live, batch)])
-            chosen = stepper.step_and_choose([(s.slot, tokens) for s, (_, tokens) in zip(live, batch)],
-                                             [s.index for s in live], [0] * len(live))
+            if continuations == 1:
+                chosen = stepper.step_and_choose([(s.slot, tokens) for s, (_, tokens) in zip(live, batch)],
+                                                 [s.index for s in live], [0] * len(live))
+            else:   # every continuation draws its own first token from the prompt's one row of logits
+                chosen = stepper.step_and_choose([(s.slot, tokens) for s, (_, tokens) in zip(live, batch)],
+                                                 [s.index + c for s in live for c in range(continuations)],
+                                                 [0] * (len(live) * continuations), continuations)
+                for at, (s, (_, tokens)) in enumerate(list(zip(live, batch))):
+                    forks = [_Live(s.index + c + 1, slot, s.budget, results[s.index + c + 1])
+                             for c, slot in enumerate(stepper.fork(s.slot, continuations - 1))]
+                    live[at * continuations + 1:at * continuations + 1] = forks
+                    stepper.reserve([(f.slot, len(tokens) + f.budget - 1) for f in forks])
             self.prompt_steps_run += 1
             live = self._take(live, chosen)
             started = time.perf_counter()

@@ -58,7 +58,7 @@ def length_bound(n: int) -> int:
 class DecodeGraph:
     """Static buffers and the captured step for `rows` sequences."""
 
-    def __init__(self, model, cache, rows: int, max_len: int, sampler: Sampler):
+    def __init__(self, model, cache, rows: int, max_len: int, sampler: Sampler, shared=None):
         device = model.device
         self.model, self.cache, self.rows, self.sampler = model, cache, rows, sampler
         i32 = dict(dtype=torch.int32, device=device)
@@ -79,6 +79,8 @@ class DecodeGraph:
             tok_seq=arange[:rows].clone(), tok_pos=self.tok_pos, slots=self.slots, cu_q=arange,
             want_rows=arange[:rows].clone(), err=model.err, dtype=model.dtype, attention=model.attention,
             decode_scratch=ops.DecodeScratch(device))  # the graph's own: its addresses are baked into the capture
+        if shared is not None:   # (what is shared is the graph's own too: a later session of the same shape loads it anew)
+            self.ctx.shared, self.ctx.shared_scratch = shared, ops.SharedScratch(device)
         self.sample_scratch = ops.SampleScratch()
         # Where the embedding is a plain lookup, the kernel that advances the rows' state also embeds their next tokens,
         # and a step starts at its first layer.
@@ -177,12 +179,18 @@ class GraphDecoder:
     def supported(model) -> bool:
         return all(getattr(part, "graph_safe", True) for part in model.parts())
 
-    def get(self, rows: int, max_len: int, sampler: Sampler) -> DecodeGraph:
+    def get(self, rows: int, max_len: int, sampler: Sampler, shared=None) -> DecodeGraph:
+        """`shared`: what the rows' sequences share (`SequenceCache.shared_prefix`), if anything."""
         key = (rows, length_bound(max_len), sampler.params.temperature, sampler.params.seed)
+        if shared is not None:
+            shared = ops.SharedPrefix(shared.groups, rows, self.model.device, bound_pages=length_bound(shared.most_pages))
+            key += shared.shape()
         graph = self.graphs.pop(key, None)
         if graph is None:
-            graph = DecodeGraph(self.model, self.cache, rows, key[1], sampler)
+            graph = DecodeGraph(self.model, self.cache, rows, key[1], sampler, shared)
             graph.capture()
+        elif shared is not None:
+            graph.ctx.shared.load(shared)
         self.graphs[key] = graph
         while len(self.graphs) > self.keep:
             self.graphs.pop(next(iter(self.graphs)))

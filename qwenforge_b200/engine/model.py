@@ -41,7 +41,7 @@ class Model:
         self.final_norm = build_part("norm", spec.final_norm)
         self.head = build_part("head", spec.head)
         self.err = None
-        self.decode_scratch = None
+        self.decode_scratch = self.shared_scratch = None
         self.prefill_graphs = None  # engine.graphs.PrefillGraphs once enabled
         # a callable (index, hidden, delta) that is shown the float32 residual stream after the embedding (index 0) and
         # after every schedule entry (index k + 1); the stream's value there is hidden + delta when delta is pending.
@@ -92,6 +92,7 @@ class Model:
             part.bind(tensors, self.dtype, self.device)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.decode_scratch = ops.DecodeScratch(self.device)
+        self.shared_scratch = ops.SharedScratch(self.device)
         self._bound = True
         return self
 
@@ -211,6 +212,8 @@ class Model:
             # from pageable memory the copy is complete when the call returns, so the host array may go
             dev = torch.from_numpy(step.packed).to(self.device)
             ctx = context_of(step, dev, self.err, self.dtype, self.attention, self.decode_scratch)
+            if ctx.is_decode:
+                ctx.shared, ctx.shared_scratch = cache.shared_prefix(step.host_slots), self.shared_scratch
             if extras:
                 ctx.extras = {}
                 for name, per_entry in extras.items():

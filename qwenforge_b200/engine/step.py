@@ -31,6 +31,10 @@ class StepContext:
     dtype: torch.dtype
     attention: str = "auto"          # "auto": fastest kernel that takes the shape; "generic": the SIMT kernel
     decode_scratch: Optional[object] = None   # ops.DecodeScratch shared by the model's attention layers
+    # single tokens of sequences that begin with the same cache pages (`ops.SharedPrefix`), and the workspaces of the attention that reads
+    # those once for all of them; None: every sequence is read by itself
+    shared: Optional[object] = None
+    shared_scratch: Optional[object] = None
     # per-token side inputs named by whoever feeds the step, [T, ...] on the device: what a part needs beyond a
     # token's index in its sequence (positions on several axes, token types). `tok_pos` stays the index that
     # orders the cache and the causal mask.

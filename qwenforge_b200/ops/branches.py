@@ -94,9 +94,10 @@ class SharedPrefix:
     """Which sequences of a batch begin with the same cache pages. groups: (batch entries, pages) each; the entries of a group hold the
     same page ids in the first `pages` places of their page tables, whole pages that none of them writes any more (`SequenceCache.fork`
     makes such sequences, `SequenceCache.shared_groups` finds them). An entry is in one group at most; groups without pages are left
-    out. Stays valid while these pages are shared, however long the sequences get, also where some of them have ended (slot -1)."""
+    out. Stays valid while these pages are shared, however long the sequences get, also where some of them have ended (slot -1).
+    `bound_pages`: the most pages that any group may share when what is shared is replaced later (`load`) under a captured graph."""
 
-    def __init__(self, groups: Sequence[tuple], n_seqs: int, device):
+    def __init__(self, groups: Sequence[tuple], n_seqs: int, device, bound_pages: int = 0):
         self.n_seqs = int(n_seqs)
         if self.n_seqs <= 0:
             raise KernelError("SharedPrefix: a batch has at least one sequence")
@@ -116,13 +117,28 @@ class SharedPrefix:
         pages = [p for _, p in self.groups]
         self.most_members = max((len(e) for e, _ in self.groups), default=0)
         self.most_pages = max(pages, default=0)
-        self.least_pages = min(entry_pages)
+        if 0 < bound_pages < self.most_pages:
+            raise KernelError(f"SharedPrefix: a group shares {self.most_pages} pages, more than the bound of {bound_pages}")
+        self.bound_pages = max(self.most_pages, int(bound_pages))
+        self.least_pages = 0 if bound_pages else min(entry_pages)
         sizes = (len(entry_pages), len(members), len(begin), len(pages))
         packed = torch.tensor(entry_pages + members + begin + pages, dtype=torch.int32).to(device)
         self.entry_pages, self.members, self.begin, self.pages = packed.split(sizes)
 
     def __len__(self) -> int:
         return len(self.groups)
+
+    def shape(self) -> tuple:
+        """What the launches go by: the batch, the groups' members, the bound on their pages."""
+        return (self.n_seqs, tuple(len(entries) for entries, _ in self.groups), self.bound_pages)
+
+    def load(self, other: "SharedPrefix") -> None:
+        """Take over what `other`, of the same members per group and within the bound, says is shared; the addresses stay."""
+        if other.shape()[:2] != self.shape()[:2] or other.most_pages > self.bound_pages:
+            raise KernelError("SharedPrefix: what is loaded has other groups, or more pages than the bound")
+        for mine, theirs in zip((self.entry_pages, self.members, self.begin, self.pages), (other.entry_pages, other.members, other.begin, other.pages)):
+            mine.copy_(theirs)
+        self.groups, self.most_pages = other.groups, other.most_pages
 
 
 class SharedScratch:
@@ -162,10 +178,10 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     own_chunks = -(-group_heads // own_chunk)
     shared_runs = 1
     fewest = 0   # records when nothing is cut
-    for entries, pages in share.groups:
+    for entries, _ in share.groups:
         chunks = -(-len(entries) * group_heads // row_chunk)
         fewest += chunks
-        shared_runs = max(shared_runs, min(-(-pages // least), max(1, slots // chunks)))
+        shared_runs = max(shared_runs, min(-(-share.bound_pages // least), max(1, slots // chunks)))
     fewest += share.n_seqs * own_chunks
     own_runs = max(1, min(-(-own_pages // least), max(1, slots // own_chunks)))
     return most_rows, shared_runs, own_runs, max(fewest, slots)

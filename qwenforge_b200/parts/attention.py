@@ -297,7 +297,8 @@ class GqaAttention(Mixer):
             return self._forward_with_options(x, ctx, site, writes_cache)
         fast = (ctx.attention == "auto" and x.dtype == torch.bfloat16
                 and self.head_dim in ops.FAST_ATTENTION_HEAD_DIMS)
-        plan = self.decode_plan(ctx) if fast and ctx.is_decode else None
+        shares = self.reads_shared(ctx)
+        plan = self.decode_plan(ctx) if fast and ctx.is_decode and not shares else None
         rotary = self.position.fused_rotary() if self.position is not None else None
         inv_freq, rot_dim = rotary if rotary is not None else (None, 0)
         late_bias = self.position is None or rotary is not None  # the kernel that rotates and stores adds the bias
@@ -326,7 +327,9 @@ class GqaAttention(Mixer):
             ops.rope_cache_write(qkv, ctx.tok_seq, ctx.tok_pos, ctx.slots, inv_freq, rot_dim, self.n_heads, q, args,
                                  writes_cache, ctx.err, bias=self.qkv_bias_t if late_bias else None)
         attended = torch.empty_like(q)
-        if fast and ctx.is_decode:
+        if shares:
+            self._attend_shared(q, attended, args, ctx)
+        elif fast and ctx.is_decode:
             ops.attention_decode(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs,
                                  self.scale, self.window, self.decode_splits(ctx), ctx.decode_scratch, ctx.err, plan)
         elif fast:
@@ -458,7 +461,7 @@ class GqaAttention(Mixer):
     def _folds(self, hidden, ctx, o_way) -> bool:
         """Whether the output projection folds the attention's partial results itself."""
         n = hidden.shape[0]
-        return (o_way == "skinny" and n == ctx.n_seqs and ops.fold_project_pays(n, self.o_weight)
+        return (not self.reads_shared(ctx) and o_way == "skinny" and n == ctx.n_seqs and ops.fold_project_pays(n, self.o_weight)
                 and ops.fold_project_takes(n, self.o_weight, hidden, self.n_heads, self.head_dim))
 
     def takes_sums(self, hidden, ctx) -> bool:
@@ -485,7 +488,8 @@ class GqaAttention(Mixer):
         leave = 0
         if folds and ctx.step_memo and ctx.step_memo.get("pre_norm.feed_forward_leaves_sums"):
             leave = ops.fold_project_large_blocks(self.o_weight, self.n_heads, self.head_dim)
-        plan = self.decode_plan(ctx, leave)
+        shares = self.reads_shared(ctx)
+        plan = None if shares else self.decode_plan(ctx, leave)
         inv_freq, rot_dim = self.position.fused_rotary() if self.position is not None else (None, 0)
         args = ops.KvSiteArgs(site.storage, site.table, self.n_kv, self.head_dim)
         q = torch.empty((n, self.q_width), dtype=torch.bfloat16, device=hidden.device)
@@ -514,14 +518,32 @@ class GqaAttention(Mixer):
             ops.fold_project(plan, ctx.decode_scratch, self.o_weight, hidden, self.n_heads, self.head_dim, n_splits, sums, settled=True)
             return
         attended = torch.empty_like(q)
-        ops.attention_decode(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs,
-                             self.scale, self.window, n_splits, ctx.decode_scratch, ctx.err, plan)
+        if shares:
+            self._attend_shared(q, attended, args, ctx)
+        else:
+            ops.attention_decode(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs,
+                                 self.scale, self.window, n_splits, ctx.decode_scratch, ctx.err, plan)
         if o_way == "skinny":
             ops.skinny_gemm(ops.EPI_RESIDUAL, self.o_weight, x=attended, residual=hidden)
         elif o_way == "wide":
             ops.wide_gemm(ops.EPI_RESIDUAL, self.o_weight, x=attended, residual=hidden, err=ctx.err)
         else:
             ops.residual_add(hidden, ops.linear(attended, self.o_weight))
+
+    def reads_shared(self, ctx) -> bool:
+        """Whether this step's sequences begin with the same pages and the layer reads those once for all of them."""
+        return (ctx.shared is not None and ctx.is_decode and ctx.n_tokens == ctx.n_seqs and ctx.attention == "auto" and self.plain
+                and self.window <= 0)
+
+    def _attend_shared(self, q, attended, args, ctx) -> None:
+        memo = ctx.step_memo if ctx.step_memo is not None else {}
+        key = ("gqa_attention.shared_plan", self.n_kv, self.n_heads, self.head_dim)
+        plan = memo.get(key)
+        if plan is None:
+            plan = memo[key] = ops.attention_shared_plan(ctx.cu_q, ctx.tok_pos, ctx.slots, self.n_kv, self.head_dim, self.n_heads, ctx.n_seqs,
+                                                         ctx.shared, ctx.shared_scratch, q.dtype, ctx.max_kv_len)
+        ops.attention_shared(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs, self.scale, ctx.shared,
+                             ctx.shared_scratch, ctx.err, plan=plan)
 
     def decode_plan(self, ctx, leave: int = 0) -> torch.Tensor:
         """Which block of the decode attention takes which run of which sequence: made once per step, by the first

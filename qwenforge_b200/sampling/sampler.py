@@ -39,3 +39,20 @@ class Sampler:
             out = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
         ops.sample(logits, self.params.temperature, self.params.seed, seq_ids, steps, out, scratch)
         return out
+
+    def verify(self, logits: torch.Tensor, drafted: torch.Tensor, first: torch.Tensor, most: int, uniforms: Optional[torch.Tensor] = None,
+               draft_logits: Optional[torch.Tensor] = None, seq_ids: Optional[torch.Tensor] = None,
+               steps: Optional[torch.Tensor] = None, scratch=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Which drafted tokens stay, and the token behind them (`ops.verify_drafts`). logits float32 [rows, vocab]: a row per drafted
+        token and one more per entry, entry s's from first[s] on; drafted int32, uniforms float32 and draft_logits float32 [.., vocab] one
+        after another; seq_ids and steps as when sampling. Returns accepted int32 [entries] and tokens int32 [entries, most + 1]."""
+        n = first.numel() - 1
+        accepted = torch.empty(n, dtype=torch.int32, device=logits.device)
+        tokens = torch.empty((n, most + 1), dtype=torch.int32, device=logits.device)
+        if uniforms is None:
+            if not self.greedy:
+                raise ValueError("verify: sampling needs uniforms")
+            uniforms = torch.empty(0, dtype=torch.float32, device=logits.device)
+        ops.verify_drafts(logits, draft_logits, drafted, first, uniforms, self.params.temperature, self.params.seed, seq_ids, steps,
+                          accepted, tokens, scratch)
+        return accepted, tokens
