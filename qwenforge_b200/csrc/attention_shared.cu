@@ -5,14 +5,13 @@
 // s_ij = q_i k_j scale log2(e). The sums over a sequence's keys fall into parts, each with a maximum m of its own; parts (m, l, o) join as
 //   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
 // The keys of the pages that a group of sequences shares are one part (or, cut into runs, several) of ALL rows of the group at once: they are
-// fetched once for members x heads rows, instead of once for every member. The keys behind them are a sequence's own parts, as in
-// attention_decode.cu. A last kernel joins each row's parts.
+// fetched once for members x heads rows, instead of once for every member. The keys behind them are a sequence's own parts. A last kernel joins
+// each row's parts.
 //
-// Which block takes which run is worked out on the device from the lengths of the step (`shared_plan_kernel`), so that a captured step can be
-// replayed with other lengths; what is shared stands in arrays on the device:
-//   entry_pages [n_seqs]  pages that the sequence shares with its group (0: none)
+// Which block and warp take which run is worked out on the device from the lengths of the step (`shared_plan_kernel`), so that a captured step can
+// be replayed with other lengths; what is shared stands in arrays on the device:
+//   entry_pages [n_seqs]  pages that the sequence shares with its group (0: none);   entry_group [n_seqs]  its group (-1: none)
 //   members     [n_seqs]  batch entries, group after group;   begin [n_groups + 1]  where each group starts there;   pages [n_groups]
-// The plan: header of n_seqs ints (runs of the shared part | runs of the own part << 16), padded to four, then records of eight ints.
 //
 // Everything is held in float32 but the weights, which enter the second product as bf16 (their rounding, 2^-9 of each, is that of the result).
 #include "mma.cuh"
@@ -20,125 +19,172 @@
 #define SH_PREFIX 1   // record kinds
 #define SH_OWN 0
 
-struct SharedRecord {
-    int kind;      // SH_OWN, SH_PREFIX, or -1: no such block
+struct __align__(16) SharedRecord {
+    int kind;      // SH_OWN or SH_PREFIX
     int subject;   // batch entry, or group
-    int chunk;     // which rows of it
+    int chunk;     // which rows of it: chunk * (rows of a tile) ..
     int slot;      // whose page table is read
     int p_begin, p_end;
-    int limit;     // keys below it are seen by every row
-    int part;      // which of a row's parts the block writes
+    int limit;     // keys below it are seen by every row (a sequence's own part: its length)
+    int part;      // which of a row's parts this is
 };
 
-// ---- the plan: one block. A group's pages count once per chunk of its rows, a sequence's own pages once per chunk of its heads; the target is the
-// pages per block at which all of them fill `slots` blocks once (at least `least`: a page per warp), as in attention_decode.cu.
+// The plan: four counts (block records, warp records, tile records, 0), then n_seqs ints (a row's shared parts | its own parts << 16) padded to four,
+// then the block records, the warp records and the tile records.
+__host__ __device__ constexpr long long shared_plan_records(int n_seqs) { return 4 + (n_seqs + 3) / 4 * 4; }   // (where they begin, in ints)
+
+// ---- the plan: one block. An item is a group's pages or a sequence's own, times its tiles of rows. With X pages x tiles x kv heads in all and `warps`
+// warps at once, a warp gets t = max(1, X / warps) pages. Items of up to `team` t pages are cut into warp records of t pages, each a part of its own;
+// longer ones into block records of up to `team` t pages, whose warps bring their sums together. A group of `tile_rows` rows or more with `tile_pages`
+// pages or more goes to the tensor-core tiles instead (attention_shared_tiles.cuh): pairs of tiles of 128 rows, cut into runs of as many turns of two
+// pages as make the records fill the SMs once.
 #define SH_PLAN_THREADS 256
+#define SH_MAX_SEQS 2048
 __global__ void __launch_bounds__(SH_PLAN_THREADS)
-shared_plan_kernel(const int* __restrict__ cu_q, const int* __restrict__ tok_pos, const int* __restrict__ slots, int n_seqs, const int* __restrict__ entry_pages,
-                   const int* __restrict__ members, const int* __restrict__ begin, const int* __restrict__ pages, int n_groups, int kv_heads, int group_heads,
-                   int row_chunk, int own_chunk, float row_cost, int blocks, int least, int most_shared, int most_own, int* __restrict__ plan, int n_records) {
-    __shared__ int scratch[SH_PLAN_THREADS / 32 + 1];
+shared_plan_kernel(const int* __restrict__ tok_pos, const int* __restrict__ slots, int n_seqs, const int* __restrict__ entry_pages,
+                   const int* __restrict__ entry_group, const int* __restrict__ begin, const int* __restrict__ pages, int n_groups, int kv_heads,
+                   int group_heads, int row_tile, int warps, int team, int most_shared, int most_own, int tile_rows, int tile_pages, int sms, int* __restrict__ plan,
+                   int block_records, int warp_records, int tile_records) {
+    extern __shared__ int plan_s[];
+    __shared__ long long sums_s[SH_PLAN_THREADS / 32];
+    const int n_items = n_groups + n_seqs;
+    int* own_s = plan_s;                  // [n_seqs] pages of a sequence's own part
+    int* slot_s = own_s + n_seqs;         // [n_groups] a live member's slot (-1: all have ended)
+    int* least_s = slot_s + n_groups;     // [n_groups] the fewest keys that a live member sees
+    int* first_s = least_s + n_groups;    // [n_items] an item's first record of its kind
+    int* runs_s = first_s + n_items;      // [n_groups] a group's parts
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto block_total = [&](int v) -> int {
+    auto block_total = [&](long long v) -> long long {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         __syncthreads();
-        if (lane == 0) scratch[warp] = v;
+        if (lane == 0) sums_s[warp] = v;
         __syncthreads();
-        int t = 0;
+        long long t = 0;
 #pragma unroll
-        for (int w = 0; w < SH_PLAN_THREADS / 32; ++w) t += scratch[w];
+        for (int w = 0; w < SH_PLAN_THREADS / 32; ++w) t += sums_s[w];
         return t;
     };
+    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS) slot_s[g] = -1, least_s[g] = 0x7fffffff;
+    __syncthreads();
     grid_dependency_wait();
-    const int own_chunks = (group_heads + own_chunk - 1) / own_chunk;
-    auto own_pages = [&](int s) -> int {
-        if (s >= n_seqs || slots[s] < 0) return 0;
-        return max(0, tok_pos[cu_q[s]] / QF_PAGE + 1 - entry_pages[s]);
-    };
-    auto group_slot = [&](int g) -> int {   // the first live member's: its pages are everyone's
-        for (int i = begin[g]; i < begin[g + 1]; ++i)
-            if (slots[members[i]] >= 0) return slots[members[i]];
-        return -1;
-    };
-    auto chunks_of = [&](int g) -> int { return ((begin[g + 1] - begin[g]) * group_heads + row_chunk - 1) / row_chunk; };
-    auto cut = [](int n_pages, float target, int most) -> int {   // runs of equal size, none without a page
-        if (n_pages <= 0) return 0;
-        const int n = min(max((int)ceilf((float)n_pages / target), 1), most);
-        const int each = (n_pages + n - 1) / n;
-        return (n_pages + each - 1) / each;
-    };
-    int cost = 0;
-    for (int s = tid; s < n_seqs; s += SH_PLAN_THREADS) cost += own_pages(s) * own_chunks;
-    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
-        if (group_slot(g) >= 0) cost += (int)(pages[g] * chunks_of(g) * row_cost);
-    cost = block_total(cost);
-    float target = fmaxf((float)least, (float)cost * (float)kv_heads / (float)blocks);
-    for (int round = 0; round < 16; ++round) {
-        int runs = 0;
-        for (int s = tid; s < n_seqs; s += SH_PLAN_THREADS) runs += cut(own_pages(s), target, most_own) * own_chunks;
-        for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
-            if (group_slot(g) >= 0) runs += cut(pages[g], fmaxf((float)least, target / row_cost), most_shared) * chunks_of(g);
-        runs = block_total(runs);
-        if ((long long)runs * kv_heads <= blocks) break;
-        if (round == 14) target = 3.0e38f;   // one run each: always within the grid
-        else target *= fmaxf(1.05f, (float)runs * (float)kv_heads / (float)blocks);
+    const int own_tiles = (group_heads + row_tile - 1) / row_tile;
+    auto group_rows = [&](int g) -> int { return (begin[g + 1] - begin[g]) * group_heads; };
+    auto tiled = [&](int g) -> bool { return group_rows(g) >= tile_rows && pages[g] >= tile_pages; };
+    auto group_tiles = [&](int g) -> int { return tiled(g) ? (group_rows(g) + 255) / 256 : (group_rows(g) + row_tile - 1) / row_tile; };
+    long long cost = 0, turns = 0;   // (turns: of all pairs of tiles, of one kv head)
+    for (int s = tid; s < n_seqs; s += SH_PLAN_THREADS) {
+        const int slot = slots[s], pos = tok_pos[s], g = entry_group[s], n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - entry_pages[s]);
+        own_s[s] = n;
+        cost += (long long)n * own_tiles;
+        if (slot >= 0 && g >= 0) {
+            atomicMax(slot_s + g, slot);
+            atomicMin(least_s + g, pos + 1);
+        }
     }
-    SharedRecord* records = reinterpret_cast<SharedRecord*>(plan + (n_seqs + 3) / 4 * 4);
-    // the records: groups first (their blocks take longest), then sequences, each in rising order
-    int before = 0;
-    auto place = [&](int n) -> int {   // exclusive prefix sum over the block, and the sum added to `before` for everyone
-        int upto = n;
+    __syncthreads();
+    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
+        if (slot_s[g] >= 0) (tiled(g) ? turns : cost) += (long long)(tiled(g) ? (pages[g] + 1) / 2 : pages[g]) * group_tiles(g);
+    cost = block_total(cost) * kv_heads;
+    int stretch = 2;   // turns of a tile record
+    if (tile_records > 0) {
+        turns = block_total(turns) * kv_heads;
+        stretch = (int)max(2ll, (turns + sms - 1) / sms);
+        for (int round = 0; round < 16; ++round) {   // (cutting into whole turns may give more records than SMs)
+            long long records = 0;
+            for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
+                if (slot_s[g] >= 0 && tiled(g)) records += (long long)((pages[g] + 1) / 2 + stretch - 1) / stretch * group_tiles(g);
+            records = block_total(records) * kv_heads;
+            if (records <= sms) break;
+            stretch = round == 14 ? 0x3fffffff : (int)max((long long)stretch + 1, stretch * records / sms);
+        }
+    }
+    const int each = (int)max(1ll, (cost + warps - 1) / warps);
+    // parts of an item (the most that there is room for: longer runs then), and whether they are whole blocks' work
+    auto cut = [&](int n_pages, int most_parts, bool& whole) -> int {
+        whole = n_pages > (long long)team * each;
+        const int want = (int)((n_pages + (whole ? (long long)team : 1ll) * each - 1) / ((whole ? (long long)team : 1ll) * each));
+        const int n = min(max(want, 1), most_parts), run = (n_pages + n - 1) / n;
+        return n_pages > 0 ? (n_pages + run - 1) / run : 0;   // no part without a page
+    };
+    auto cut_tiles = [&](int n_pages) -> int {   // runs of whole turns
+        const int all = (n_pages + 1) / 2, n = min(max((all + stretch - 1) / stretch, 1), most_shared), run = (all + n - 1) / n;
+        return (all + run - 1) / run;
+    };
+    // where every item's records begin: a prefix sum of the three counts at once, 21 bits each
+    constexpr int BLOCKS = 42, TILES = 21, BITS = (1 << 21) - 1;
+    long long before = 0;
+    for (int i0 = 0; i0 < n_items; i0 += SH_PLAN_THREADS) {
+        const int i = i0 + tid;
+        long long n = 0;
+        bool whole = false;
+        if (i < n_groups) {
+            const int parts = slot_s[i] < 0 ? 0 : tiled(i) ? cut_tiles(pages[i]) : cut(pages[i], most_shared, whole);
+            runs_s[i] = parts;
+            n = (long long)parts * group_tiles(i);
+        } else if (i < n_items) {
+            n = (long long)cut(own_s[i - n_groups], most_own, whole) * own_tiles;
+        }
+        const int shift = i < n_groups && tiled(i) ? TILES : whole ? BLOCKS : 0;
+        const long long mine = n << shift;
+        long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, upto, o);
+            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += t;
         }
         __syncthreads();
-        if (lane == 31) scratch[warp] = upto;
+        if (lane == 31) sums_s[warp] = upto;
         __syncthreads();
-        int first = before, all = 0;
+        long long first = before + upto - mine;
 #pragma unroll
         for (int w = 0; w < SH_PLAN_THREADS / 32; ++w) {
-            if (w < warp) first += scratch[w];
-            all += scratch[w];
+            if (w < warp) first += sums_s[w];
+            before += sums_s[w];
         }
-        before += all;
-        return first + upto - n;
-    };
-    for (int g0 = 0; g0 < n_groups; g0 += SH_PLAN_THREADS) {
-        const int g = g0 + tid;
-        const int slot = g < n_groups ? group_slot(g) : -1;
-        const int runs = slot >= 0 ? cut(pages[g], fmaxf((float)least, target / row_cost), most_shared) : 0, chunks = slot >= 0 ? chunks_of(g) : 0;
-        const int first = place(runs * chunks);
-        if (runs <= 0) continue;
-        const int each = (pages[g] + runs - 1) / runs;
-        for (int k = 0; k < runs * chunks; ++k)
-            if (first + k < n_records)
-                records[first + k] = SharedRecord{SH_PREFIX, g, k / runs, slot, k % runs * each, min((k % runs + 1) * each, pages[g]), pages[g] * QF_PAGE, k % runs};
-        for (int i = begin[g]; i < begin[g + 1]; ++i) plan[members[i]] = runs;
+        if (i < n_items) first_s[i] = (int)(first >> shift) & BITS;
     }
-    __syncthreads();   // the header's first halves are written
-    for (int s0 = 0; s0 < n_seqs; s0 += SH_PLAN_THREADS) {
-        const int s = s0 + tid;
-        const int mine = own_pages(s), runs = cut(mine, target, most_own);
-        const int first = place(runs * own_chunks);
-        if (s >= n_seqs) continue;
-        const int shared = entry_pages[s] > 0 && slots[s] >= 0 ? plan[s] : 0;
-        plan[s] = shared | runs << 16;
-        if (runs <= 0) continue;
-        const int each = (mine + runs - 1) / runs, from = entry_pages[s];
-        for (int k = 0; k < runs * own_chunks; ++k)
-            if (first + k < n_records)
-                records[first + k] = SharedRecord{SH_OWN, s, k / runs, slots[s], from + k % runs * each, from + min((k % runs + 1) * each, mine),
-                                                  tok_pos[cu_q[s]] + 1, shared + k % runs};
+    __syncthreads();
+    SharedRecord* blocks = reinterpret_cast<SharedRecord*>(plan + shared_plan_records(n_seqs));
+    if (tid == 0) {
+        plan[0] = min((int)(before >> BLOCKS) & BITS, block_records);
+        plan[1] = min((int)before & BITS, warp_records);
+        plan[2] = min((int)(before >> TILES) & BITS, tile_records);
     }
-    for (int j = before + tid; j < n_records; j += SH_PLAN_THREADS) records[j].kind = -1;
+    for (int i = warp; i < n_items; i += SH_PLAN_THREADS / 32) {   // a warp per item, a lane per record
+        const bool group = i < n_groups, tile = group && tiled(i);
+        const int s = i - n_groups, n_pages = group ? pages[i] : own_s[s];
+        bool whole = false;
+        int parts = tile ? cut_tiles(n_pages) : cut(n_pages, group ? most_shared : most_own, whole), tiles, slot, from, limit, part0 = 0;
+        if (group) {
+            slot = slot_s[i];
+            if (slot < 0) continue;
+            tiles = group_tiles(i);
+            from = 0;
+            limit = min(least_s[i], n_pages * QF_PAGE);
+        } else {
+            const int g = entry_group[s];
+            slot = slots[s];
+            part0 = g >= 0 && slot >= 0 ? runs_s[g] : 0;
+            if (lane == 0) plan[4 + s] = part0 | parts << 16;
+            tiles = own_tiles;
+            from = entry_pages[s];
+            limit = tok_pos[s] + 1;
+        }
+        const int run = parts <= 0 ? 0 : tile ? ((n_pages + 1) / 2 + parts - 1) / parts * 2 : (n_pages + parts - 1) / parts;
+        const int most = tile ? tile_records : whole ? block_records : warp_records;
+        SharedRecord* at = blocks + (tile ? block_records + warp_records : whole ? 0 : block_records);
+        for (int k = lane; k < parts * tiles; k += 32) {
+            const int part = k % parts;
+            if (first_s[i] + k < most)
+                at[first_s[i] + k] = SharedRecord{group ? SH_PREFIX : SH_OWN, group ? i : s, k / parts, slot, from + part * run,
+                                                  from + min((part + 1) * run, n_pages), limit, part0 + part};
+        }
+    }
 }
 
 // ---- what every kernel of the parts needs
 struct SharedArgs {
-    const int* cu_q;
     const int* tok_pos;
     const int* slots;
     const int* members;
@@ -147,294 +193,241 @@ struct SharedArgs {
     float* part_o;    // [n_seqs * n_heads][most_parts][D]
     float* part_ml;   // [n_seqs * n_heads][most_parts][2]
     int* err;
-    int n_seqs, n_heads, most_parts;
+    int n_seqs, n_heads, most_parts, block_records, tile_first;   // (tile_first: where the tile records begin behind the first record)
     float scale_log2;
 };
 
-// Row r of a block: its place in q ([n_seqs * n_heads] rows of D), the keys it sees, or -1 where there is no such row or its entry is padding.
-__device__ __forceinline__ int shared_row(const SharedArgs& a, const SharedRecord& rec, int kv_heads, int kvh, int rows, int r, int& limit) {
+// Row `at` of a record's subject: its place in q ([n_seqs * n_heads] rows of D), or -1 where there is no such row. (The rows of a member that has ended
+// have a place too: nobody reads what is left there.)
+__device__ __forceinline__ int shared_row(const SharedArgs& a, const SharedRecord& rec, int kv_heads, int kvh, int at) {
     const int G = a.n_heads / kv_heads;
-    int entry, head;
-    limit = 0;
-    const int at = rec.chunk * rows + r;
-    if (rec.kind == SH_PREFIX) {
-        const int i = a.begin[rec.subject] + at / G;
-        if (i >= a.begin[rec.subject + 1]) return -1;
-        entry = a.members[i];
-        head = at % G;
-    } else {
-        if (at >= G) return -1;
-        entry = rec.subject;
-        head = at;
-    }
-    if (a.slots[entry] < 0) return -1;
-    limit = a.tok_pos[a.cu_q[entry]] + 1;
-    return entry * a.n_heads + kvh * G + head;
+    if (rec.kind == SH_OWN) return at < G ? rec.subject * a.n_heads + kvh * G + at : -1;
+    const int i = a.begin[rec.subject] + at / G;
+    return i < a.begin[rec.subject + 1] ? a.members[i] * a.n_heads + kvh * G + at % G : -1;
+}
+// The keys that the row at a place sees.
+__device__ __forceinline__ int shared_seen(const SharedArgs& a, int place) {
+    return place < 0 ? 0 : a.tok_pos[place / a.n_heads] + 1;
 }
 
-// ---- bf16 on mma.sync: a block takes one run for up to 16 * MT rows. Each warp works alone on whole pages, in two halves through its own two
-// buffers (16-byte asynchronous copies into padded rows), as in attention_decode.cu; the rows' queries lie in shared memory and every fragment of keys
-// or values that a warp loads serves all of the block's tiles of 16 rows (one of a sequence's own part, up to MT of a group).
+// ---- bf16 on mma.sync, straight from memory to registers. A warp takes 16 rows and a run of pages, 16 keys a step: S = Q K^T, softmax with a running
+// maximum, O += P V. Neither product minds the order of what it sums over, nor the second one the order of its columns, so the fragments are cut to
+// suit 16-byte loads: lane (g, j) = (lane / 4, lane % 4) holds of key g's row the columns 32 u + 8 j .. + 7 (two k-steps of the first product, Q
+// cut alike), and of the values of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 the columns E g .. E g + E - 1, E = D / 8, which make the n-tiles' column g. No shared
+// memory, no barrier: the next step's keys and values are on their way as soon as the current ones have been multiplied.
+// What bounds it: memory latency while a run is short, then the rate at which pages arrive.
+// Warps of a block, and blocks of an SM.
 __host__ __device__ constexpr int shared_warps(int d) { return d <= 64 ? 8 : 4; }
-template <int D> struct SharedShape {
-    static constexpr int WARPS = shared_warps(D), THREADS = 32 * WARPS, LD = D + 8;   // LD: a padded row of keys, values, queries (bf16) or sums (float32)
-    static constexpr int PAGE_BYTES = 2 * QF_PAGE * LD * 2;
-};
+__host__ __device__ constexpr int shared_resident(int d) { return 2; }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(SharedShape<D>::THREADS)
+template <int D>
+__global__ void __launch_bounds__(32 * shared_warps(D), shared_resident(D))
 shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a) {
-    using S = SharedShape<D>;
-    constexpr int WARPS = S::WARPS, LD = S::LD, KS = D / 16, NT = D / 8, HALF = QF_PAGE / 2, STAGE = 2 * HALF * LD, ROWS = 16 * MT, CH = D / 8;
-    extern __shared__ uint4 smem[];
-    unsigned char* pages_s = reinterpret_cast<unsigned char*>(smem);
-    bf16* q_s = reinterpret_cast<bf16*>(pages_s + (size_t)WARPS * S::PAGE_BYTES);
-    __shared__ float m_s[WARPS * ROWS], l_s[WARPS * ROWS];
-    __shared__ int row_at[ROWS], row_limit[ROWS], least_limit;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int SH_WARPS = shared_warps(D), KU = D / 32, E = D / 8, NT = E, LO = D + 4;
+    extern __shared__ float4 merge_s4[];
+    float* merge_s = reinterpret_cast<float*>(merge_s4);   // [SH_WARPS][16][LO]
+    __shared__ float m_s[SH_WARPS][16], l_s[SH_WARPS][16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
     grid_launch_dependents();
     grid_dependency_wait();
-    const int4* records = reinterpret_cast<const int4*>(a.plan + (a.n_seqs + 3) / 4 * 4) + 2 * (blockIdx.x / site.kv_heads);
-    const int4 x = records[0], y = records[1];
-    const SharedRecord rec = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (rec.kind < 0) return;
-    const int kvh = blockIdx.x % site.kv_heads, tiles = rec.kind == SH_PREFIX ? MT : 1;
-
-    bf16* stage0 = reinterpret_cast<bf16*>(pages_s + (size_t)warp * S::PAGE_BYTES);
-    const int* table_row = site.table + (long long)rec.slot * site.table_stride;
-    const int my_pages = rec.p_begin + warp < rec.p_end ? (rec.p_end - rec.p_begin - warp + WARPS - 1) / WARPS : 0;
-    const int n_halves = 2 * my_pages;
-    auto half_live = [&](int i, int& page, int& key0) {
-        if (i >= n_halves) return false;
-        const int p = rec.p_begin + warp + (i >> 1) * WARPS;
-        key0 = p * QF_PAGE + (i & 1) * HALF;
-        page = __ldg(table_row + p);
-        if (page < 0) {
-            if (lane == 0 && (i & 1) == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-            return false;
+    const int kv_heads = site.kv_heads, n_blocks = a.plan[0] * kv_heads, n_tasks = a.plan[1] * kv_heads;
+    const int units = n_blocks + (n_tasks + SH_WARPS - 1) / SH_WARPS;
+    const SharedRecord* records = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs));
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const bool whole = unit < n_blocks;   // a block's record, or one for each of its warps
+        const int task = whole ? unit : (unit - n_blocks) * SH_WARPS + warp;
+        if (!whole && task >= n_tasks) break;
+        const int kvh = task % kv_heads;
+        SharedRecord rec = records[(whole ? 0 : a.block_records) + task / kv_heads];
+        int p0 = rec.p_begin, p1 = rec.p_end;
+        if (whole) {
+            const int per = (p1 - p0 + SH_WARPS - 1) / SH_WARPS;
+            p0 += warp * per;
+            p1 = min(p0 + per, p1);
         }
-        return key0 < rec.limit;
-    };
-    auto issue = [&](int i) {
-        int page, key0;
-        if (half_live(i, page, key0)) {
-            bf16* kb = stage0 + (size_t)(i & 1) * STAGE;
-            bf16* vb = kb + HALF * LD;
-            const bf16* kp = site.base + (long long)page * site.page_elems + ((long long)kvh * QF_PAGE + (i & 1) * HALF) * D;
-            const bf16* vp = kp + (long long)site.kv_heads * QF_PAGE * D;
-#pragma unroll 4
-            for (int j = lane; j < HALF * CH; j += 32) {
-                const int r = j / CH, c = (j % CH) * 8;
-                cp_async_16(kb + (size_t)r * LD + c, kp + (size_t)r * D + c, true);
-                cp_async_16(vb + (size_t)r * LD + c, vp + (size_t)r * D + c, true);
+        const int steps = p0 < p1 ? 4 * (p1 - p0) : 0;
+        const int bound = rec.kind == SH_OWN ? rec.limit : rec.p_end * QF_PAGE;   // no row sees a key from here on
+        const int* table_row = site.table + (long long)rec.slot * site.table_stride;
+        int table = 0;   // a lane each the numbers of 32 pages
+        uint4 k[2][KU];            // n-tile t: key 8 t + g
+        uint32_t v[4][E / 2];      // keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9
+        const bf16* k_at = nullptr;   // the step's 16 keys (null: nothing to see there)
+        auto find = [&](int i) {
+            k_at = nullptr;
+            if (i >= steps) return;
+            const int n = i >> 2;
+            if ((i & 127) == 0) table = p0 + n + lane < p1 ? __ldg(table_row + p0 + n + lane) : 0;
+            const int page = __shfl_sync(0xffffffffu, table, n & 31);
+            if (page < 0) {
+                if (lane == 0 && (i & 3) == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+                return;
             }
-        }
-        cp_async_commit();   // one group per half, empty when there is nothing to fetch
-    };
-    issue(0);
-
-    // ---- the rows and their queries
-    if (threadIdx.x == 0) least_limit = rec.limit;
-    __syncthreads();
-    if (threadIdx.x < ROWS) {
-        int limit;
-        const int place = threadIdx.x < 16 * tiles ? shared_row(a, rec, site.kv_heads, kvh, 16 * tiles, threadIdx.x, limit) : -1;
-        row_at[threadIdx.x] = place;
-        row_limit[threadIdx.x] = place < 0 ? rec.limit : limit;   // (a row that is not there sees what all see; nothing is kept of it)
-        if (place >= 0 && limit < rec.limit) atomicMin(&least_limit, limit);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * CH; i += S::THREADS) {
-        const int r = i / CH, c = i % CH * 8, place = row_at[r];
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (place >= 0) v = *reinterpret_cast<const uint4*>(q + (size_t)place * D + c);
-        *reinterpret_cast<uint4*>(q_s + (size_t)r * LD + c) = v;
-    }
-    __syncthreads();
-
-    float o[MT][NT][4];
-    float m_run[MT][2], l_run[MT][2];
-    int seen[MT][2];   // keys that this lane's rows see
+            if ((p0 + n) * QF_PAGE + 16 * (i & 3) >= bound) return;
+            k_at = site.base + (long long)page * site.page_elems + ((long long)kvh * QF_PAGE + 16 * (i & 3)) * D;
+        };
+        auto load_keys = [&]() {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+                for (int u = 0; u < KU; ++u) k[t][u] = __ldg(reinterpret_cast<const uint4*>(k_at + (8 * t + g) * D + 32 * u + 8 * j));
+        };
+        auto load_values = [&](const bf16* v_at) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            m_run[t][r] = QF_NEG_BIG;
-            l_run[t][r] = 0.f;
-            seen[t][r] = row_limit[16 * t + (lane >> 2) + 8 * r];
-        }
-    }
-    for (int i = 0; i < n_halves; ++i) {
-        issue(i + 1);
-        int page, key0;
-        const bool live = half_live(i, page, key0);
-        cp_async_wait<1>();
-        __syncwarp();   // each lane waited for its own copies; together the half page is complete
-        if (live) {
-            bf16* kb = stage0 + (size_t)(i & 1) * STAGE;
-            bf16* vb = kb + HALF * LD;
-            if (key0 + HALF > rec.limit) {
-                // what lies behind a sequence's last position is nobody's: 0 times a NaN left there is not 0
-                for (int j = lane; j < HALF * CH; j += 32) {
-                    const int r = j / CH, c = (j % CH) * 8;
-                    if (key0 + r >= rec.limit) *reinterpret_cast<uint4*>(vb + (size_t)r * LD + c) = make_uint4(0, 0, 0, 0);
-                }
-                __syncwarp();
-            }
-            const bool full = key0 + HALF <= least_limit;   // every row sees the half whole
-            float s[MT][4][4];
+            for (int r = 0; r < 4; ++r) {
+                const bf16* row = v_at + (2 * j + (r & 1) + 8 * (r >> 1)) * D + E * g;
+                if constexpr (E % 8 == 0) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+                    for (int u = 0; u < E / 8; ++u) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + 8 * u));
+                        v[r][4 * u] = x.x, v[r][4 * u + 1] = x.y, v[r][4 * u + 2] = x.z, v[r][4 * u + 3] = x.w;
+                    }
+                } else {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t kf[2][4];
-#pragma unroll
-                for (int t2 = 0; t2 < 2; ++t2)   // 16 keys each
-                    ldmatrix_x4(kf[t2], kb + (size_t)(16 * t2 + (lane >> 4) * 8 + (lane & 7)) * LD + 16 * ks + ((lane >> 3) & 1) * 8);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if (t >= tiles) break;
-                    uint32_t qa[4];
-                    ldmatrix_x4(qa, q_s + (size_t)(16 * t + (lane & 15)) * LD + 16 * ks + (lane >> 4) * 8);
-#pragma unroll
-                    for (int t2 = 0; t2 < 2; ++t2) {
-                        mma_bf16_16816(s[t][2 * t2], qa, kf[t2][0], kf[t2][1]);
-                        mma_bf16_16816(s[t][2 * t2 + 1], qa, kf[t2][2], kf[t2][3]);
+                    for (int u = 0; u < E / 4; ++u) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + 4 * u));
+                        v[r][2 * u] = x.x, v[r][2 * u + 1] = x.y;
                     }
                 }
             }
-            uint32_t pa[MT][2][4];
+        };
+        const long long to_values = (long long)kv_heads * QF_PAGE * D;
+        find(0);
+        if (k_at) {
+            load_keys();
+            load_values(k_at + to_values);
+        }
+        const int place0 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g), place1 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g + 8);
+        uint4 q0[KU], q1[KU];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                if (t >= tiles) break;
-                float mx[2] = {QF_NEG_BIG, QF_NEG_BIG};
+        for (int u = 0; u < KU; ++u) {
+            q0[u] = place0 < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(q + (size_t)place0 * D + 32 * u + 8 * j);
+            q1[u] = place1 < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(q + (size_t)place1 * D + 32 * u + 8 * j);
+        }
+        float o[NT][4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        float m0 = QF_NEG_BIG, m1 = QF_NEG_BIG, l0 = 0.f, l1 = 0.f;   // rows g and g + 8; the sums are this lane's share
+        for (int i = 0; i < steps; ++i) {
+            const bool live = k_at != nullptr;
+            const int key0 = (p0 + (i >> 2)) * QF_PAGE + 16 * (i & 3);
+            float s[2][4];
+            if (live) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[t][n][e] *= a.scale_log2;
-                        if (!full) {
-                            const int kj = key0 + 8 * n + 2 * (lane & 3) + (e & 1);
-                            if (kj >= seen[t][e >> 1]) s[t][n][e] = QF_NEG_BIG;
-                        }
-                        mx[e >> 1] = fmaxf(mx[e >> 1], s[t][n][e]);
-                    }
-                float corr[2], sum[2] = {0.f, 0.f};
+                for (int t = 0; t < 2; ++t) {
+                    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    const float m_new = fmaxf(m_run[t][r], mx[r]);
-                    corr[r] = fast_exp2(m_run[t][r] - m_new);
-                    m_run[t][r] = m_new;
-                    mx[r] = m_new <= QF_NEG_BIG ? 0.f : m_new;   // a row that has seen no key yet: its weights are 2^(-huge) = 0
-                }
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[t][n][e] = fast_exp2(s[t][n][e] - mx[e >> 1]);
-                        sum[e >> 1] += s[t][n][e];
-                    }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                    l_run[t][r] = l_run[t][r] * corr[r] + sum[r];
-                }
-                if (corr[0] != 1.f || corr[1] != 1.f) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        o[t][nt][0] *= corr[0];
-                        o[t][nt][1] *= corr[0];
-                        o[t][nt][2] *= corr[1];
-                        o[t][nt][3] *= corr[1];
-                    }
-                }
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    pa[t][kk][0] = pack_bf16(s[t][2 * kk][0], s[t][2 * kk][1]);
-                    pa[t][kk][1] = pack_bf16(s[t][2 * kk][2], s[t][2 * kk][3]);
-                    pa[t][kk][2] = pack_bf16(s[t][2 * kk + 1][0], s[t][2 * kk + 1][1]);
-                    pa[t][kk][3] = pack_bf16(s[t][2 * kk + 1][2], s[t][2 * kk + 1][3]);
-                }
-            }
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt += 2) {
-                    uint32_t vf[4];
-                    ldmatrix_x4_trans(vf, vb + (size_t)(16 * kk + ((lane >> 3) & 1) * 8 + (lane & 7)) * LD + 8 * nt + (lane >> 4) * 8);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        if (t >= tiles) break;
-                        mma_bf16_16816(o[t][nt], pa[t][kk], vf[0], vf[1]);
-                        mma_bf16_16816(o[t][nt + 1], pa[t][kk], vf[2], vf[3]);
+                    for (int u = 0; u < KU; ++u) {
+                        const uint32_t lo[4] = {q0[u].x, q1[u].x, q0[u].y, q1[u].y}, hi[4] = {q0[u].z, q1[u].z, q0[u].w, q1[u].w};
+                        mma_bf16_16816(s[t], lo, k[t][u].x, k[t][u].y);
+                        mma_bf16_16816(s[t], hi, k[t][u].z, k[t][u].w);
                     }
                 }
             }
+            find(i + 1);
+            if (k_at) load_keys();   // (on their way while the softmax and the second product run)
+            if (live) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] *= a.scale_log2;
+                if (key0 + 16 > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
+                    const int see0 = min(bound, rec.kind == SH_OWN ? bound : shared_seen(a, place0)), see1 = min(bound, rec.kind == SH_OWN ? bound : shared_seen(a, place1));
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (key0 + 8 * t + 2 * j + (e & 1) >= (e >> 1 ? see1 : see0)) s[t][e] = QF_NEG_BIG;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key0 + 2 * j + (r & 1) + 8 * (r >> 1) >= bound)
+#pragma unroll
+                            for (int u = 0; u < E / 2; ++u) v[r][u] = 0u;
+                }
+                float top0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), top1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
+                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
+                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+                if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1)) {
+                    const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1), c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
+                    m0 = n0, m1 = n1;
+                    l0 *= c0, l1 *= c1;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[t][0] *= c0, o[t][1] *= c0, o[t][2] *= c1, o[t][3] *= c1;
+                }
+                const float from0 = m0 <= QF_NEG_BIG ? 0.f : m0, from1 = m1 <= QF_NEG_BIG ? 0.f : m1;   // (no key seen yet: weights of 2^(-huge) = 0)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[t][0] = fast_exp2(s[t][0] - from0), s[t][1] = fast_exp2(s[t][1] - from0);
+                    s[t][2] = fast_exp2(s[t][2] - from1), s[t][3] = fast_exp2(s[t][3] - from1);
+                    l0 += s[t][0] + s[t][1];
+                    l1 += s[t][2] + s[t][3];
+                }
+                const uint32_t p[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t pick = t & 1 ? 0x7632u : 0x5410u;
+                    mma_bf16_16816(o[t], p, __byte_perm(v[0][t / 2], v[1][t / 2], pick), __byte_perm(v[2][t / 2], v[3][t / 2], pick));
+                }
+            }
+            if (k_at) load_values(k_at + to_values);
         }
-        __syncwarp();   // every lane has read this buffer before the copies of half i + 2 overwrite it
-    }
-    cp_async_wait<0>();
-
-    // ---- the warps' sums come together, 16 rows at a time through the warps' own buffers, in warp order
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-        if ((lane & 3) == 0) {
-            m_s[warp * ROWS + 16 * t + (lane >> 2)] = m_run[t][0];
-            m_s[warp * ROWS + 16 * t + (lane >> 2) + 8] = m_run[t][1];
+        for (int d = 1; d < 4; d <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
         }
-    __syncthreads();
-    float* o_w = reinterpret_cast<float*>(pages_s + (size_t)warp * S::PAGE_BYTES);
+        // o[t][0], o[t][1] are row g's columns 2 j E + t and (2 j + 1) E + t: 2 E columns side by side
+        auto leave = [&](float* row0, float* row1, float f0, float f1) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        if (t >= tiles) break;
-        float f[2];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = 16 * t + (lane >> 2) + 8 * r;
-            float m_all = m_s[row];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) m_all = fmaxf(m_all, m_s[w * ROWS + row]);
-            f[r] = exp2f(m_run[t][r] - m_all);
-            if ((lane & 3) == 0) l_s[warp * ROWS + row] = l_run[t][r] * f[r];
+                for (int t = 0; t < E; t += 4) {
+                    const int c = (2 * j + h) * E + t;
+                    if (row0) *reinterpret_cast<float4*>(row0 + c) = make_float4(o[t][h] * f0, o[t + 1][h] * f0, o[t + 2][h] * f0, o[t + 3][h] * f0);
+                    if (row1) *reinterpret_cast<float4*>(row1 + c) = make_float4(o[t][2 + h] * f1, o[t + 1][2 + h] * f1, o[t + 2][2 + h] * f1, o[t + 3][2 + h] * f1);
+                }
+        };
+        if (!whole) {
+            const size_t at0 = (size_t)place0 * a.most_parts + rec.part, at1 = (size_t)place1 * a.most_parts + rec.part;
+            leave(place0 < 0 ? nullptr : a.part_o + at0 * D, place1 < 0 ? nullptr : a.part_o + at1 * D, 1.f, 1.f);
+            if (j == 0 && place0 >= 0) *reinterpret_cast<float2*>(a.part_ml + at0 * 2) = make_float2(m0, l0);
+            if (j == 0 && place1 >= 0) *reinterpret_cast<float2*>(a.part_ml + at1 * 2) = make_float2(m1, l1);
+            continue;
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = 8 * nt + 2 * (lane & 3), r0 = lane >> 2, r1 = r0 + 8;
-            *reinterpret_cast<float2*>(o_w + r0 * LD + c) = make_float2(o[t][nt][0] * f[0], o[t][nt][1] * f[0]);
-            *reinterpret_cast<float2*>(o_w + r1 * LD + c) = make_float2(o[t][nt][2] * f[1], o[t][nt][3] * f[1]);
-        }
+        // the warps' sums come together in warp order
+        if (j == 0) m_s[warp][g] = m0, m_s[warp][g + 8] = m1;
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * (D / 4); i += S::THREADS) {
-            const int r = i / (D / 4), c = i % (D / 4) * 4, place = row_at[16 * t + r];
+        float top0 = m_s[0][g], top1 = m_s[0][g + 8];
+#pragma unroll
+        for (int w = 1; w < SH_WARPS; ++w) top0 = fmaxf(top0, m_s[w][g]), top1 = fmaxf(top1, m_s[w][g + 8]);
+        const float f0 = fast_exp2(m0 - top0), f1 = fast_exp2(m1 - top1);
+        if (j == 0) l_s[warp][g] = l0 * f0, l_s[warp][g + 8] = l1 * f1;
+        leave(merge_s + (warp * 16 + g) * LO, merge_s + (warp * 16 + g + 8) * LO, f0, f1);
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * (D / 4); i += 32 * SH_WARPS) {
+            const int r = i / (D / 4), c = i % (D / 4) * 4, place = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + r);
             if (place < 0) continue;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(pages_s + (size_t)w * S::PAGE_BYTES) + r * LD + c);
+            for (int w = 0; w < SH_WARPS; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(merge_s + (w * 16 + r) * LO + c);
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
-            *reinterpret_cast<float4*>(a.part_o + ((size_t)place * a.most_parts + rec.part) * D + c) = sum;
+            const size_t at = (size_t)place * a.most_parts + rec.part;
+            *reinterpret_cast<float4*>(a.part_o + at * D + c) = sum;
+            if (c == 0) {
+                float m = m_s[0][r], l = 0.f;
+#pragma unroll
+                for (int w = 0; w < SH_WARPS; ++w) m = fmaxf(m, m_s[w][r]), l += l_s[w][r];
+                *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+            }
         }
-        __syncthreads();
-    }
-    if (threadIdx.x < 16 * tiles) {
-        const int r = threadIdx.x, place = row_at[r];
-        if (place < 0) return;
-        float m = m_s[r], l = 0.f;
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) m = fmaxf(m, m_s[w * ROWS + r]);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) l += l_s[w * ROWS + r];
-        *reinterpret_cast<float2*>(a.part_ml + ((size_t)place * a.most_parts + rec.part) * 2) = make_float2(m, l);
+        __syncthreads();   // (the next unit writes these again)
     }
 }
+
+#include "attention_shared_tiles.cuh"
 
 // ---- any type and head size: float32 arithmetic. A block takes one run for 16 rows; a page's keys, then its values, in shared memory as float32.
 #define SH_ROWS 16
@@ -451,15 +444,15 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     __shared__ float m_s[SH_ROWS], l_s[SH_ROWS], corr_s[SH_ROWS];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int4* records = reinterpret_cast<const int4*>(a.plan + (a.n_seqs + 3) / 4 * 4) + 2 * (blockIdx.x / site.kv_heads);
-    const int4 x = records[0], y = records[1];
-    const SharedRecord rec = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (rec.kind < 0) return;
-    const int kvh = blockIdx.x % site.kv_heads, tid = threadIdx.x;
+    const SharedRecord* records = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs));
+    const int kv_heads = site.kv_heads, n_blocks = a.plan[0] * kv_heads, units = n_blocks + a.plan[1] * kv_heads, tid = threadIdx.x;
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {   // (both kinds of record are a block's work here)
+    const int task = unit < n_blocks ? unit : unit - n_blocks, kvh = task % kv_heads;
+    const SharedRecord rec = records[(unit < n_blocks ? 0 : a.block_records) + task / kv_heads];
+    const int bound = rec.kind == SH_OWN ? rec.limit : rec.p_end * QF_PAGE;
     if (tid < SH_ROWS) {
-        int limit;
-        row_at[tid] = shared_row(a, rec, site.kv_heads, kvh, SH_ROWS, tid, limit);
-        row_limit[tid] = limit;   // (0, and no key, for a row that is not there)
+        row_at[tid] = shared_row(a, rec, kv_heads, kvh, SH_ROWS * rec.chunk + tid);
+        row_limit[tid] = min(bound, shared_seen(a, row_at[tid]));
         m_s[tid] = QF_NEG_BIG;
         l_s[tid] = 0.f;
     }
@@ -486,7 +479,7 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
             if (tid == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
             continue;
         }
-        const int key0 = p * QF_PAGE, n_rows = min(QF_PAGE, rec.limit - key0);
+        const int key0 = p * QF_PAGE, n_rows = min(QF_PAGE, bound - key0);
         const T* keys = site.base + (long long)page * site.page_elems + (long long)kvh * QF_PAGE * D;
         __syncthreads();
         fetch(keys, n_rows);
@@ -542,134 +535,189 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     }
     __syncthreads();
     const int place = row_at[my_row];
-    if (place < 0) return;
-    const size_t part = (size_t)place * a.most_parts + rec.part;
+    if (place >= 0) {
+        const size_t part = (size_t)place * a.most_parts + rec.part;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const float v[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
+        for (int u = 0; u < U; ++u) {
+            const float v[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (64 * u + my_col + e < D) a.part_o[part * D + 64 * u + my_col + e] = v[e];
+            for (int e = 0; e < 4; ++e)
+                if (64 * u + my_col + e < D) a.part_o[part * D + 64 * u + my_col + e] = v[e];
+        }
+        if (tid % 16 == 0) {
+            a.part_ml[part * 2] = m_s[my_row];
+            a.part_ml[part * 2 + 1] = l_s[my_row];
+        }
     }
-    if (tid % 16 == 0) {
-        a.part_ml[part * 2] = m_s[my_row];
-        a.part_ml[part * 2 + 1] = l_s[my_row];
+    __syncthreads();   // (the next unit writes these again)
     }
 }
 
-// ---- the parts of a row come together: a thread per output element
-template <typename T>
+// ---- the parts of a row come together: a thread per V neighbouring output elements, eight parts on their way at once
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __restrict__ sinks) {
     grid_launch_dependents();
     grid_dependency_wait();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)a.n_seqs * a.n_heads * D) return;
-    const int row = (int)(i / D), d = (int)(i % D), entry = row / a.n_heads;
-    const int runs = a.slots[entry] < 0 ? 0 : (a.plan[entry] & 0xffff) + (a.plan[entry] >> 16);
+    const int per = D / V;
+    if (i >= (long long)a.n_seqs * a.n_heads * per) return;
+    const int row = (int)(i / per), d = (int)(i % per) * V, entry = row / a.n_heads;
+    const int packed = a.plan[4 + entry], runs = a.slots[entry] < 0 ? 0 : (packed & 0xffff) + (packed >> 16);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.most_parts;
     const float* po = a.part_o + (size_t)row * a.most_parts * D + d;
-    float top = QF_NEG_BIG, den = 0.f, num = 0.f;
-    for (int k = 0; k < runs; ++k) {
-        const float2 x = ml[k];
-        const float m = fmaxf(top, x.x), keep = exp2f(top - m), w = exp2f(x.x - m);
-        den = den * keep + w * x.y;
-        num = num * keep + w * po[(size_t)k * D];
+    float top = QF_NEG_BIG, den = 0.f, num[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) num[e] = 0.f;
+    for (int k0 = 0; k0 < runs; k0 += 8) {
+        float2 x[8];
+        float o[8][V];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool in = k0 + k < runs;
+            x[k] = in ? ml[k0 + k] : make_float2(QF_NEG_BIG, 0.f);
+            if constexpr (V == 4) {
+                const float4 v = in ? *reinterpret_cast<const float4*>(po + (size_t)(k0 + k) * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+                o[k][0] = v.x, o[k][1] = v.y, o[k][2] = v.z, o[k][3] = v.w;
+            } else {
+                o[k][0] = in ? po[(size_t)(k0 + k) * D] : 0.f;
+            }
+        }
+        float m = top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, x[k].x);
+        const float keep = exp2f(top - m);
+        den *= keep;
+#pragma unroll
+        for (int e = 0; e < V; ++e) num[e] *= keep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float w = exp2f(x[k].x - m);
+            den = fmaf(w, x[k].y, den);
+#pragma unroll
+            for (int e = 0; e < V; ++e) num[e] = fmaf(w, o[k][e], num[e]);
+        }
         top = m;
     }
+    float keep = 1.f;
     if (sinks && runs > 0) {   // a logit that joins the sum of weights once, with no key and no value
-        const float s2 = sinks[row % a.n_heads] * 1.4426950408889634f, m = fmaxf(top, s2), keep = exp2f(top - m);
+        const float s2 = sinks[row % a.n_heads] * 1.4426950408889634f, m = fmaxf(top, s2);
+        keep = exp2f(top - m);
         den = den * keep + exp2f(s2 - m);
-        num *= keep;
     }
-    out[i] = Num<T>::from_f(den > 0.f ? num / den : 0.f);
+    const float inv = den > 0.f ? keep / den : 0.f;
+    T* to = out + (size_t)row * D + d;
+    if constexpr (V == 4 && sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
+    else if constexpr (V == 4)
+        *reinterpret_cast<float4*>(to) = make_float4(num[0] * inv, num[1] * inv, num[2] * inv, num[3] * inv);
+    else
+        to[0] = Num<T>::from_f(num[0] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
 static bool shared_fast(int is_bf16, int d) { return is_bf16 && (d == 32 || d == 64 || d == 96 || d == 128); }
-// Tiles of 16 rows that a block takes of a group's rows: one or two (four at head size 64 do not fit the registers).
-static int shared_tiles(int is_bf16, int d, int most_rows) {
-    if (!shared_fast(is_bf16, d)) return 1;
-    return most_rows <= 16 ? 1 : 2;
-}
-template <int D> constexpr size_t shared_smem(int mt) {
-    return (size_t)SharedShape<D>::WARPS * SharedShape<D>::PAGE_BYTES + (size_t)16 * mt * SharedShape<D>::LD * 2;
-}
+template <int D> constexpr size_t shared_smem() { return (size_t)shared_warps(D) * 16 * (D + 4) * sizeof(float); }
 static size_t shared_generic_smem(int d) {
     const int ld = (d + 3) / 4 * 4 + 4;
     return (size_t)((SH_ROWS + QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4)) * sizeof(float);
 }
 
-// What sizes the plan and the workspaces. sizes[0]: rows of a block for a group; [1]: rows of a block for a sequence's own part; [2]: pages that a
-// run should have at least; [3]: blocks that run at once.
-QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int most_rows, int* sizes) {
+// Where the tiles take over.
+#define SH_TILE_ROWS 65
+#define SH_TILE_PAGES 8
+
+// What sizes the plan and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of a
+// block record; [3]: the most parts of an item; [4], [5]: a group of so many rows and pages goes to the tiles (0: there are none); [6]: SMs.
+QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     const int sms = qf_sm_count();
     if (sms <= 0 || head_dim <= 0 || head_dim > 256) return (int)cudaErrorInvalidValue;
     const bool fast = shared_fast(is_bf16, head_dim);
-    sizes[0] = 16 * shared_tiles(is_bf16, head_dim, most_rows);
-    sizes[1] = 16;
-    sizes[2] = fast ? shared_warps(head_dim) : 2;
-    sizes[3] = fast ? sms : 2 * sms;
+    sizes[0] = 16;
+    sizes[1] = fast ? shared_warps(head_dim) * shared_resident(head_dim) * sms : 2 * sms;
+    sizes[2] = fast ? shared_warps(head_dim) : 1;
+    sizes[3] = 64;
+    sizes[4] = fast && (head_dim == 64 || head_dim == 128) ? SH_TILE_ROWS : 0;
+    sizes[5] = SH_TILE_PAGES;
+    sizes[6] = sms;
     return 0;
 }
 
-QF_EXPORT int qf_attention_shared_plan(const int* cu_q, const int* tok_pos, const int* slots, int n_seqs, const int* entry_pages, const int* members,
-                                       const int* begin, const int* pages, int n_groups, int kv_heads, int n_heads, int is_bf16, int head_dim,
-                                       int most_rows, int most_shared, int most_own, int* plan, int n_records, cudaStream_t stream) {
-    int sizes[4];
-    if (kv_heads <= 0 || n_heads % kv_heads || n_records <= 0 || most_shared > 0xffff || most_own > 0x7fff) return (int)cudaErrorInvalidValue;
-    const int bad = qf_attention_shared_shape(is_bf16, head_dim, most_rows, sizes);
+QF_EXPORT int qf_attention_shared_plan(const int* tok_pos, const int* slots, int n_seqs, const int* entry_pages, const int* entry_group, const int* begin,
+                                       const int* pages, int n_groups, int kv_heads, int n_heads, int is_bf16, int head_dim, int most_shared, int most_own, int* plan,
+                                       int block_records, int warp_records, int tile_records, cudaStream_t stream) {
+    int sizes[7];
+    if (n_seqs <= 0 || n_seqs > SH_MAX_SEQS || n_groups > n_seqs || kv_heads <= 0 || n_heads % kv_heads || most_own <= 0 || most_own > 0x7fff || most_shared > 0xffff ||
+        (n_groups > 0 && most_shared <= 0))
+        return (int)cudaErrorInvalidValue;
+    const int bad = qf_attention_shared_shape(is_bf16, head_dim, sizes);
     if (bad) return bad;
-    const float row_cost = sizes[0] <= 16 ? 1.f : 1.4f;
-    return (int)launch_pdl(shared_plan_kernel, dim3(1), dim3(SH_PLAN_THREADS), 0, stream, cu_q, tok_pos, slots, n_seqs, entry_pages, members, begin, pages,
-                           n_groups, kv_heads, n_heads / kv_heads, sizes[0], sizes[1], row_cost, sizes[3], sizes[2], most_shared, most_own, plan, n_records);
+    const size_t smem = (size_t)(2 * n_seqs + 4 * n_groups) * sizeof(int);
+    static_assert(6 * SH_MAX_SEQS * sizeof(int) <= 48 * 1024, "the plan's shared memory needs no permission");
+    return (int)launch_pdl(shared_plan_kernel, dim3(1), dim3(SH_PLAN_THREADS), smem, stream, tok_pos, slots, n_seqs, entry_pages, entry_group, begin, pages,
+                           n_groups, kv_heads, n_heads / kv_heads, sizes[0], sizes[1], sizes[2], most_shared, most_own,
+                           tile_records > 0 ? sizes[4] : 0x7fffffff, sizes[5], sizes[6], plan, block_records, warp_records, tile_records);
 }
 
-template <int D, int MT>
-static int launch_parts(const void* q, KvSite<bf16> site, const SharedArgs& a, int n_records, cudaStream_t stream) {
-    constexpr size_t smem = shared_smem<D>(MT);
-    static_assert(smem <= 227 * 1024 && (size_t)16 * SharedShape<D>::LD * 4 <= (size_t)SharedShape<D>::PAGE_BYTES, "a block's shared memory");
-    auto kernel = shared_parts_kernel<D, MT>;
+template <int D>
+static int launch_parts(const void* q, KvSite<bf16> site, const SharedArgs& a, int units, cudaStream_t stream) {
+    constexpr size_t smem = shared_smem<D>();
+    static_assert(shared_resident(D) * (smem + 2048) <= 227 * 1024, "the shared memory of an SM's blocks");
+    auto kernel = shared_parts_kernel<D>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(kernel, dim3((unsigned)(n_records * site.kv_heads)), dim3(SharedShape<D>::THREADS), smem, stream, (const bf16*)q, site, a);
+    const int at_once = qf_sm_count() * shared_resident(D);
+    return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(32 * shared_warps(D)), smem, stream, (const bf16*)q, site, a);
 }
 
 template <typename T>
-static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, int n_records, cudaStream_t stream) {
+static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, int units, cudaStream_t stream) {
     const size_t smem = shared_generic_smem(site.head_dim);
     auto kernel = shared_parts_generic_kernel<T>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(kernel, dim3((unsigned)(n_records * site.kv_heads)), dim3(SH_THREADS), smem, stream, (const T*)q, site, a);
+    const int at_once = 2 * qf_sm_count();
+    return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(SH_THREADS), smem, stream, (const T*)q, site, a);
 }
 
-// The parts and their joining. `plan`: of qf_attention_shared_plan with the same shape, n_records records; part_o, part_ml: n_seqs * n_heads *
-// most_parts * head_dim and * 2 floats, most_parts >= most_shared + most_own. `launched` counts the launches.
-QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const int* cu_q, const int* tok_pos, const int* slots, const int* members,
-                                  const int* begin, const int* plan, int n_records, void* base, const int* table, long long page_elems, int table_stride,
-                                  int kv_heads, int head_dim, int n_heads, int n_seqs, float scale, int most_rows, int most_parts, float* part_o,
-                                  float* part_ml, const float* sinks, int* err, cudaStream_t stream) {
+template <typename T>
+static int launch_join(const SharedArgs& a, int head_dim, void* out, const float* sinks, cudaStream_t stream) {
+    const long long items = (long long)a.n_seqs * a.n_heads * head_dim;
+    if (head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
+        return (int)launch_pdl(shared_join_kernel<T, 4>, dim3((unsigned)((items / 4 + 255) / 256)), dim3(256), 0, stream, a, head_dim, (T*)out, sinks);
+    return (int)launch_pdl(shared_join_kernel<T, 1>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a, head_dim, (T*)out, sinks);
+}
+
+// The parts and their joining. `plan`: of qf_attention_shared_plan with the same shape; part_o, part_ml: n_seqs * n_heads * most_parts * head_dim and
+// * 2 floats, most_parts >= the most shared and own parts of a row together.
+QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const int* tok_pos, const int* slots, const int* members, const int* begin,
+                                  const int* plan, int block_records, int warp_records, int tile_records, void* base, const int* table, long long page_elems, int table_stride,
+                                  int kv_heads, int head_dim, int n_heads, int n_seqs, float scale, int most_parts, float* part_o, float* part_ml,
+                                  const float* sinks, int* err, cudaStream_t stream) {
     if (n_seqs <= 0) return 0;
-    if (kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || head_dim > 256 || n_records <= 0) return (int)cudaErrorInvalidValue;
-    const SharedArgs a = {cu_q, tok_pos, slots, members, begin, plan, part_o, part_ml, err, n_seqs, n_heads, most_parts, scale * 1.4426950408889634f};
+    if (kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || head_dim > 256 || block_records < 0 || warp_records < 0 || block_records + warp_records <= 0)
+        return (int)cudaErrorInvalidValue;
+    const SharedArgs a = {tok_pos, slots, members, begin, plan, part_o, part_ml, err, n_seqs, n_heads, most_parts, block_records, block_records + warp_records,
+                          scale * 1.4426950408889634f};
+    const long long tasks = (long long)warp_records * kv_heads, blocks = (long long)block_records * kv_heads;
+    const bool fast = shared_fast(is_bf16, head_dim);
+    const long long most_units = blocks + (fast ? (tasks + shared_warps(head_dim) - 1) / shared_warps(head_dim) : tasks);
+    const int units = (int)(most_units < 0x7fffffff ? most_units : 0x7fffffff);
     int code;
-    if (shared_fast(is_bf16, head_dim)) {
+    if (fast) {
         const KvSite<bf16> site{(bf16*)base, table, page_elems, table_stride, kv_heads, head_dim};
-        const int mt = shared_tiles(is_bf16, head_dim, most_rows);
-#define QF_SH(D, MT) launch_parts<D, MT>(q, site, a, n_records, stream)
-        if (head_dim == 32) code = mt == 1 ? QF_SH(32, 1) : QF_SH(32, 2);
-        else if (head_dim == 64) code = mt == 1 ? QF_SH(64, 1) : QF_SH(64, 2);
-        else if (head_dim == 96) code = mt == 1 ? QF_SH(96, 1) : QF_SH(96, 2);
-        else code = mt == 1 ? QF_SH(128, 1) : QF_SH(128, 2);
-#undef QF_SH
+        if (tile_records > 0) {
+            code = head_dim == 64 ? launch_tiles<64>(q, site, a, tile_records, stream) : head_dim == 128 ? launch_tiles<128>(q, site, a, tile_records, stream)
+                                                                                                         : (int)cudaErrorInvalidValue;
+            if (code) return code;
+        }
+        code = head_dim == 32 ? launch_parts<32>(q, site, a, units, stream) : head_dim == 64 ? launch_parts<64>(q, site, a, units, stream)
+             : head_dim == 96 ? launch_parts<96>(q, site, a, units, stream) : launch_parts<128>(q, site, a, units, stream);
     } else if (is_bf16) {
-        code = launch_generic(q, KvSite<bf16>{(bf16*)base, table, page_elems, table_stride, kv_heads, head_dim}, a, n_records, stream);
+        code = launch_generic(q, KvSite<bf16>{(bf16*)base, table, page_elems, table_stride, kv_heads, head_dim}, a, units, stream);
     } else {
-        code = launch_generic(q, KvSite<float>{(float*)base, table, page_elems, table_stride, kv_heads, head_dim}, a, n_records, stream);
+        code = launch_generic(q, KvSite<float>{(float*)base, table, page_elems, table_stride, kv_heads, head_dim}, a, units, stream);
     }
     if (code) return code;
-    const unsigned blocks = (unsigned)(((long long)n_seqs * n_heads * head_dim + 255) / 256);
-    if (is_bf16) return (int)launch_pdl(shared_join_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, a, head_dim, (bf16*)out, sinks);
-    return (int)launch_pdl(shared_join_kernel<float>, dim3(blocks), dim3(256), 0, stream, a, head_dim, (float*)out, sinks);
+    return is_bf16 ? launch_join<bf16>(a, head_dim, out, sinks, stream) : launch_join<float>(a, head_dim, out, sinks, stream);
 }

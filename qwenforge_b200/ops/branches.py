@@ -88,6 +88,7 @@ def copy_pages(storage: torch.Tensor, moves) -> None:
 
 
 SHARED_MAX_HEAD_DIM = 256
+SHARED_MAX_SEQS = 2048
 
 
 class SharedPrefix:
@@ -108,22 +109,21 @@ class SharedPrefix:
         if len(set(named)) != len(named) or any(not 0 <= e < self.n_seqs for e in named):
             raise KernelError(f"SharedPrefix: an entry is in two groups or outside 0 .. {self.n_seqs - 1}")
         self.groups = [g for g in kept if g[1] > 0]
-        entry_pages, members, begin = [0] * self.n_seqs, [], [0]
-        for entries, pages in self.groups:
+        entry_pages, entry_group, members, begin = [0] * self.n_seqs, [-1] * self.n_seqs, [], [0]
+        for g, (entries, pages) in enumerate(self.groups):
             members += entries
             begin.append(len(members))
             for e in entries:
-                entry_pages[e] = pages
+                entry_pages[e], entry_group[e] = pages, g
         pages = [p for _, p in self.groups]
-        self.most_members = max((len(e) for e, _ in self.groups), default=0)
         self.most_pages = max(pages, default=0)
         if 0 < bound_pages < self.most_pages:
             raise KernelError(f"SharedPrefix: a group shares {self.most_pages} pages, more than the bound of {bound_pages}")
         self.bound_pages = max(self.most_pages, int(bound_pages))
         self.least_pages = 0 if bound_pages else min(entry_pages)
-        sizes = (len(entry_pages), len(members), len(begin), len(pages))
-        packed = torch.tensor(entry_pages + members + begin + pages, dtype=torch.int32).to(device)
-        self.entry_pages, self.members, self.begin, self.pages = packed.split(sizes)
+        sizes = (self.n_seqs, self.n_seqs, len(members), len(begin), len(pages))
+        packed = torch.tensor(entry_pages + entry_group + members + begin + pages, dtype=torch.int32).to(device)
+        self.entry_pages, self.entry_group, self.members, self.begin, self.pages = packed.split(sizes)
 
     def __len__(self) -> int:
         return len(self.groups)
@@ -136,8 +136,8 @@ class SharedPrefix:
         """Take over what `other`, of the same members per group and within the bound, says is shared; the addresses stay."""
         if other.shape()[:2] != self.shape()[:2] or other.most_pages > self.bound_pages:
             raise KernelError("SharedPrefix: what is loaded has other groups, or more pages than the bound")
-        for mine, theirs in zip((self.entry_pages, self.members, self.begin, self.pages), (other.entry_pages, other.members, other.begin, other.pages)):
-            mine.copy_(theirs)
+        for name in ("entry_pages", "entry_group", "members", "begin", "pages"):
+            getattr(self, name).copy_(getattr(other, name))
         self.groups, self.most_pages = other.groups, other.most_pages
 
 
@@ -158,33 +158,37 @@ class SharedScratch:
 
 
 class SharedPlan:
-    """What `attention_shared_plan` made: the tensor (which block takes which run) and the sizes that the attention's launch goes by."""
-    __slots__ = ("tensor", "key", "records", "most_rows", "most_parts")
+    """What `attention_shared_plan` made: the tensor (which block and warp takes which run) and the sizes that the attention's launch goes by."""
+    __slots__ = ("tensor", "key", "records", "most_parts")
 
-    def __init__(self, tensor, key, records, most_rows, most_parts):
-        self.tensor, self.key, self.records, self.most_rows, self.most_parts = tensor, key, records, most_rows, most_parts
+    def __init__(self, tensor, key, records, most_parts):
+        self.tensor, self.key, self.records, self.most_parts = tensor, key, records, most_parts
 
 
 def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: SharedPrefix, own_pages: int) -> tuple:
-    """(most rows of a group, most runs of a group's pages, most runs of a sequence's own, records of the plan)."""
-    sizes = (_I * 4)()
-    most_rows = share.most_members * (n_heads // kv_heads)
-    _checked = library("attention_shared").qf_attention_shared_shape(_I(int(dtype == torch.bfloat16)), _I(head_dim), _I(most_rows), sizes)
-    if _checked:
-        raise KernelError(f"attention_shared: CUDA error {_checked} when asked for its sizes")
-    row_chunk, own_chunk, least, blocks = sizes
+    """((block records, warp records, tile records) of the plan, most shared parts, most own parts of a row): bounds of what the plan kernel
+    can come to, whatever the lengths. It gives a warp at least `pages x tiles x kv heads / warps` pages, so block records cover, up to
+    twice, no more than the warps there are; tile records fill the SMs once, or are the pairs of tiles uncut."""
+    sizes = (_I * 7)()
+    code = library("attention_shared").qf_attention_shared_shape(_I(int(dtype == torch.bfloat16)), _I(head_dim), sizes)
+    if code:
+        raise KernelError(f"attention_shared: CUDA error {code} when asked for its sizes")
+    row_tile, warps, team, most, tile_rows, tile_pages, sms = sizes
     group_heads = n_heads // kv_heads
-    slots = max(1, blocks // kv_heads)
-    own_chunks = -(-group_heads // own_chunk)
-    shared_runs = 1
-    fewest = 0   # records when nothing is cut
-    for entries, _ in share.groups:
-        chunks = -(-len(entries) * group_heads // row_chunk)
-        fewest += chunks
-        shared_runs = max(shared_runs, min(-(-share.bound_pages // least), max(1, slots // chunks)))
-    fewest += share.n_seqs * own_chunks
-    own_runs = max(1, min(-(-own_pages // least), max(1, slots // own_chunks)))
-    return most_rows, shared_runs, own_runs, max(fewest, slots)
+
+    def parts(pages: int, tiles: int) -> int:
+        return max(team, min(most, -(-pages // team), warps // (team * kv_heads * tiles) + 1))
+    own_tiles = -(-group_heads // row_tile)
+    tiles = [-(-len(entries) * group_heads // row_tile) for entries, _ in share.groups]
+    most_shared = max((parts(share.bound_pages, t) for t in tiles), default=0)
+    pairs = [-(-len(entries) * group_heads // 256) for entries, _ in share.groups if len(entries) * group_heads >= tile_rows]
+    if not tile_rows or share.bound_pages < tile_pages:
+        pairs = []
+    for n in pairs:
+        most_shared = max(most_shared, min(most, -(-share.bound_pages // 4), sms // (kv_heads * n) + 1))
+    records = (2 * warps // (team * kv_heads) + 2, warps // kv_heads + 1 + sum(tiles) + share.n_seqs * own_tiles,
+               max(sms // kv_heads, sum(pairs)) if pairs else 0)
+    return records, most_shared, parts(own_pages, own_tiles)
 
 
 def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, kv_heads: int, head_dim: int, n_heads: int,
@@ -200,21 +204,23 @@ def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torc
         raise KernelError(f"attention_shared: head_dim {head_dim} > {SHARED_MAX_HEAD_DIM} is not supported")
     if kv_heads <= 0 or n_heads <= 0 or n_heads % kv_heads:
         raise KernelError(f"attention_shared: {n_heads} heads do not divide into {kv_heads} groups")
+    if not 0 < n_seqs <= SHARED_MAX_SEQS:
+        raise KernelError(f"attention_shared: a batch of {n_seqs} sequences is not supported (1 to {SHARED_MAX_SEQS})")
     if share.n_seqs != n_seqs or slots.numel() != n_seqs or cu_q.numel() != n_seqs + 1 or tok_pos.numel() != n_seqs:
         raise KernelError("attention_shared: wants exactly one token per sequence, and a SharedPrefix of this batch")
     _here("attention_shared", cu_q, tok_pos, slots, share.entry_pages)
     own_pages = max(1, -(-int(max_kv_len) // PAGE_TOKENS) - share.least_pages)
-    most_rows, shared_runs, own_runs, records = _shared_sizes(dtype, head_dim, kv_heads, n_heads, share, own_pages)
+    records, most_shared, most_own = _shared_sizes(dtype, head_dim, kv_heads, n_heads, share, own_pages)
     key = (n_seqs, kv_heads, n_heads, head_dim, dtype)
-    ints = -(-n_seqs // 4) * 4 + records * 8
+    ints = 4 + -(-n_seqs // 4) * 4 + sum(records) * 8
     held = scratch.plans.get(key)
     if held is None or held.numel() < ints:
         held = scratch.plans[key] = torch.empty(ints, dtype=torch.int32, device=cu_q.device)
     _check(library("attention_shared").qf_attention_shared_plan(
-        _ptr(cu_q), _ptr(tok_pos), _ptr(slots), _I(n_seqs), _ptr(share.entry_pages), _ptr(share.members), _ptr(share.begin), _ptr(share.pages),
-        _I(len(share)), _I(kv_heads), _I(n_heads), _I(int(dtype == torch.bfloat16)), _I(head_dim), _I(most_rows), _I(shared_runs), _I(own_runs),
-        _ptr(held), _I(records), _stream()), "attention_shared_plan")
-    return SharedPlan(held, key, records, most_rows, shared_runs + own_runs)
+        _ptr(tok_pos), _ptr(slots), _I(n_seqs), _ptr(share.entry_pages), _ptr(share.entry_group), _ptr(share.begin), _ptr(share.pages), _I(len(share)),
+        _I(kv_heads), _I(n_heads), _I(int(dtype == torch.bfloat16)), _I(head_dim), _I(most_shared), _I(most_own),
+        _ptr(held), *map(_I, records), _stream()), "attention_shared_plan")
+    return SharedPlan(held, key, records, most_shared + most_own)
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site, n_heads: int,
@@ -256,11 +262,11 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
         raise KernelError("attention_shared: the plan was made for another shape")
     scratch.ensure(n_seqs * n_heads * plan.most_parts, d)
     code = library("attention_shared").qf_attention_shared(
-        _I(int(q.dtype == torch.bfloat16)), _ptr(q), _ptr(out), _ptr(cu_q), _ptr(tok_pos), _ptr(slots), _ptr(share.members), _ptr(share.begin),
-        _ptr(plan.tensor), _I(plan.records), _ptr(site.storage), _ptr(site.table), _LL(site.page_elems), _I(site.table_stride), _I(site.kv_heads),
-        _I(d), _I(n_heads), _I(n_seqs), _F(scale), _I(plan.most_rows), _I(plan.most_parts), _ptr(scratch.part_o), _ptr(scratch.part_ml),
-        _ptr(sinks), _ptr(err), _stream())
-    kernels.launches += 1   # (the parts, and their joining)
+        _I(int(q.dtype == torch.bfloat16)), _ptr(q), _ptr(out), _ptr(tok_pos), _ptr(slots), _ptr(share.members), _ptr(share.begin),
+        _ptr(plan.tensor), *map(_I, plan.records), _ptr(site.storage), _ptr(site.table), _LL(site.page_elems),
+        _I(site.table_stride), _I(site.kv_heads), _I(d), _I(n_heads), _I(n_seqs), _F(scale), _I(plan.most_parts), _ptr(scratch.part_o),
+        _ptr(scratch.part_ml), _ptr(sinks), _ptr(err), _stream())
+    kernels.launches += 2 if plan.records[2] else 1   # (the tiles, the parts, and their joining)
     _check(code, "attention_shared")
 
 
