@@ -46,8 +46,8 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     __shared__ uint32_t tmem_base_s;
     grid_dependency_wait();
     const int kv_heads = site.kv_heads, kvh = (int)(blockIdx.x % kv_heads);
-    if ((int)(blockIdx.x / kv_heads) >= a.plan[2]) return;
-    const SharedRecord rec = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs))[a.tile_first + blockIdx.x / kv_heads];
+    if ((int)(blockIdx.x / kv_heads) >= a.plan[1]) return;
+    const SharedRecord rec = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs))[(size_t)a.most_units * SH_TEAM + blockIdx.x / kv_heads];
     const int warp = threadIdx.x >> 5, t = warp < 8 ? warp >> 2 : 0, row = threadIdx.x & 127;   // row threads: tile t, row `row`
     const int rows = (a.begin[rec.subject + 1] - a.begin[rec.subject]) * (a.n_heads / kv_heads) - 2 * ST_BM * rec.chunk;   // from the first tile's on
     const int tiles = rows > ST_BM ? 2 : 1;

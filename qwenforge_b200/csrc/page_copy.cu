@@ -5,6 +5,10 @@
 // No page is both a source and a target, and none is a target twice (the caller has checked), so the moves have no order.
 // The moves travel as kernel arguments: the call costs one launch, with no copy of a table to the device before it.
 // A block takes PC_THREADS x 4 vectors of one (entry, move). What bounds it: memory. Every thread has its four loads in flight before it stores.
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "common.cuh"
 
 #define PC_THREADS 256
@@ -62,11 +66,34 @@ static cudaError_t launch_moves(const PageMove* moves, int n, unsigned char* bas
                       page_bytes, segments, (int)(segment_bytes / (long long)sizeof(V)), (int)(row_bytes / (long long)sizeof(V)));
 }
 
-// moves: [n][3] int32 on the HOST, checked by the caller (pages inside the storage, rows 0 .. rows of a page). `unit`: 16, 4, 2 or 1 bytes, which
-// divides the base address and every distance. Returns a CUDA error code; `*launched` counts the launches.
-QF_EXPORT int qf_copy_pages(void* base, int entries, long long entry_bytes, long long page_bytes, int segments, long long segment_bytes,
-                            long long row_bytes, int unit, const int* moves, int n, int* launched, cudaStream_t stream) {
-    *launched = 0;
+// What is wrong with n moves of pages 0 .. n_pages - 1 of n_rows rows: 0 nothing, -1 a page outside, -2 rows outside, -3 a page that is the target of two
+// moves, -4 one that is both a source and a target, -5 no memory for the check.
+QF_EXPORT int qf_page_moves_check(const int* moves, int n, int n_pages, int n_rows) {
+    const PageMove* m = reinterpret_cast<const PageMove*>(moves);
+    for (int i = 0; i < n; ++i)
+        if (m[i].from < 0 || m[i].from >= n_pages || m[i].to < 0 || m[i].to >= n_pages) return -1;
+    for (int i = 0; i < n; ++i)
+        if (m[i].rows < 0 || m[i].rows > n_rows) return -2;
+    try {
+        std::vector<int> targets(n > 0 ? n : 0);
+        for (int i = 0; i < n; ++i) targets[i] = m[i].to;
+        if (!std::is_sorted(targets.begin(), targets.end())) std::sort(targets.begin(), targets.end());
+        for (int i = 1; i < n; ++i)
+            if (targets[i] == targets[i - 1]) return -3;
+        for (int i = 0; i < n; ++i)
+            if ((i == 0 || m[i].from != m[i - 1].from) && std::binary_search(targets.begin(), targets.end(), m[i].from)) return -4;
+    } catch (const std::bad_alloc&) {
+        return -5;
+    }
+    return 0;
+}
+
+// moves: [n][3] int32 on the HOST. `unit`: 16, 4, 2 or 1 bytes, which divides the base address and every distance. Returns a CUDA error code, or what
+// qf_page_moves_check says.
+QF_EXPORT int qf_copy_pages(void* base, int entries, int pages, int rows, long long entry_bytes, long long page_bytes, int segments,
+                            long long segment_bytes, long long row_bytes, int unit, const int* moves, int n, cudaStream_t stream) {
+    const int wrong = qf_page_moves_check(moves, n, pages, rows);
+    if (wrong) return wrong;
     if (entries <= 0 || n <= 0 || segments <= 0 || segment_bytes <= 0) return 0;
     if (entries > 65535 || segment_bytes / unit > 0x7fffffffll) return (int)cudaErrorInvalidValue;
     const PageMove* m = reinterpret_cast<const PageMove*>(moves);
@@ -84,7 +111,6 @@ QF_EXPORT int qf_copy_pages(void* base, int entries, long long entry_bytes, long
         else if (unit == 1) QF_PC(unsigned char);
 #undef QF_PC
         if (e != cudaSuccess) return (int)e;
-        ++*launched;
         i += here;
     }
     return 0;

@@ -5,13 +5,14 @@
 // running sum over the vocabulary is needed, and a token turns on rounding only where two scores are equal to the last bits.
 // T <= 0: kept while it is the row's argmax (lowest id of equals); the next token is the argmax.
 //
-// Two launches. (1) A block takes VF_CHUNK logits of a row, all of them in registers at once: their maximum, its lowest id, and the sum of the
-// exponentials against it. (2) A block takes VR_CHUNK tokens of an entry: it brings the rows' statistics together (a warp per draft), decides how many
-// drafts stay, and scores its tokens of the row that follows; the block that draws the entry's last ticket picks the best and writes the outputs.
+// Three launches. (1) A block takes VF_CHUNK logits of a row, all of them in registers at once: their maximum, its lowest id, and the sum of the
+// exponentials against it. (2) A block takes an entry: it brings the rows' statistics together (a warp per draft), decides how many drafts stay, and
+// writes all outputs but the token that is drawn. (3) A block takes a chunk of the row that follows and scores its tokens; the block that draws the
+// entry's last ticket picks the best. (At T <= 0 the second launch writes everything.)
+// What bounds it: memory, in (1); in (3), of the same rows out of the second-level cache, the hash and the logarithm of every token.
 //
-// Decisions are whole numbers, so they are made on sums that are good to more than float32: the argument (x - max) log2(e) / T is formed with its
-// rounding errors (two floats), sums over threads and blocks and the comparison u q < p are float64, and of a block's scores, formed in float32,
-// those within the error bound of the best are formed again in float64.
+// Decisions are whole numbers, so they are made on sums that are good to more than float32: sums over threads and blocks and the comparison u q < p are
+// float64, and of a chunk's scores, formed in float32, those within the error bound of the best are formed again in float64.
 #include <float.h>
 #include <math.h>
 
@@ -22,23 +23,21 @@
 #define VF_EACH 32                             // logits of a thread
 #define VF_CHUNK (VF_THREADS * VF_EACH)
 #define VR_THREADS 256
-#define VR_EACH 8
-#define VR_CHUNK (VR_THREADS * VR_EACH)
+#define VR_FEW 8                               // tokens of a thread in (3): few where there are few blocks, many else
+#define VR_MANY 32
 
-// log2(e) / T as two floats.
-struct Rate {
-    float hi, lo;
+// What (2) leaves for (3).
+struct Decision {
+    int kept, row, d_row, without;   // kept -1: nothing to draw; the rows of target and draft logits (-1: none), the token that is ruled out (-1: none)
+    float t_top, d_top;
+    double t_sum, d_sum;
 };
 
-// 2^((x - top) rate) with the errors of the difference and of the product carried along: within 2^-22 of the value plus the hardware exponential's
-// own error, whatever the size of the argument.
-__device__ __forceinline__ float weight_of(float x, float top, Rate r) {
-    const float d = x - top;
-    if (!(d > -FLT_MAX)) return 0.f;             // -infinity: no weight (an infinite difference has no rounding error to carry)
-    const float back = x - d, e = (x - (d + back)) + (back - top);   // d + e = x - top
-    const float y = d * r.hi, low = fmaf(d, r.hi, -y) + fmaf(d, r.lo, e * r.hi);
-    return fast_exp2(y) * fmaf(low, 0.6931471805599453f, 1.f);
-}
+struct RowStats {
+    float top;       // the largest logit, and its lowest id
+    int id;
+    double sum;      // of e^((x - top) / T)
+};
 
 struct VerifyArgs {
     const float* target;
@@ -53,11 +52,13 @@ struct VerifyArgs {
     int* tokens;
     double* sums;            // [rows + draft rows][chunks]
     float2* tops;            // the same: maximum, its id as bits
+    RowStats* stats;         // [rows + draft rows]
+    Decision* decisions;     // [n]
     double2* best;           // [n][race chunks]: score, id
     int* counters;           // [n]
     int rows, total, vocab, n, most, chunks, race_chunks;
     double inv_t;
-    Rate rate;
+    float rate;              // log2(e) / T
     unsigned long long seed;
     int sampling;
 };
@@ -68,7 +69,26 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-// ---- (1) maximum, its lowest id and the sum of exponentials of VF_CHUNK logits of a row
+// EACH logits of a thread from x[begin ..): fours of neighbours, VF_THREADS fours apart; -infinity from `end` on. at(i): the id of the i-th.
+template <int EACH>
+__device__ __forceinline__ void load_logits(const float* x, int begin, int end, float (&v)[EACH]) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(x + begin) & 15) == 0;
+#pragma unroll
+    for (int u = 0; u < EACH / 4; ++u) {
+        const int i = begin + 4 * (threadIdx.x + u * VF_THREADS);
+        if (aligned && i + 4 <= end) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(x + i));
+            v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * u + e] = i + e < end ? __ldg(x + i + e) : -INFINITY;
+        }
+    }
+}
+__device__ __forceinline__ int id_of(int begin, int i) { return begin + 4 * (threadIdx.x + i / 4 * VF_THREADS) + (i & 3); }
+
+// ---- (1) maximum, its lowest id and the sum of exponentials of VF_CHUNK logits of a row. The difference from the maximum, its product with log2(e) / T
+// and that factor itself round by 2^-24 each of an exponent, the hardware's exponential by 2^-22: of single weights, some up and some down.
 __global__ void __launch_bounds__(VF_THREADS)
 verify_rows_kernel(VerifyArgs a) {
     grid_chain_entry();
@@ -79,30 +99,10 @@ verify_rows_kernel(VerifyArgs a) {
     const float* x = row < a.rows ? a.target + row * a.t_stride : a.draft + (row - a.rows) * a.d_stride;
     const int begin = blockIdx.x * VF_CHUNK, end = min(a.vocab, begin + VF_CHUNK);
     float v[VF_EACH];
-    int at[VF_EACH / 4];   // first id of each four
-    if ((reinterpret_cast<uintptr_t>(x + begin) & 15) == 0) {
+    load_logits(x, begin, end, v);
+    float top = v[0];
 #pragma unroll
-        for (int u = 0; u < VF_EACH / 4; ++u) {
-            at[u] = begin + 4 * (threadIdx.x + u * VF_THREADS);
-            if (at[u] + 4 <= end) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(x + at[u]));
-                v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * u + e] = at[u] + e < end ? x[at[u] + e] : -INFINITY;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < VF_EACH / 4; ++u) {
-            at[u] = begin + 4 * (threadIdx.x + u * VF_THREADS);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * u + e] = at[u] + e < end ? x[at[u] + e] : -INFINITY;
-        }
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VF_EACH; ++i) top = fmaxf(top, v[i]);
+    for (int i = 1; i < VF_EACH; ++i) top = fmaxf(top, v[i]);
     float most = warp_max(top);
     if (lane == 0) top_s[warp] = most;
     __syncthreads();
@@ -113,14 +113,15 @@ verify_rows_kernel(VerifyArgs a) {
     if (top == most) {
 #pragma unroll
         for (int i = VF_EACH - 1; i >= 0; --i)
-            if (v[i] == most && at[i / 4] + (i & 3) < end) id = min(id, at[i / 4] + (i & 3));
+            if (v[i] == most && id_of(begin, i) < end) id = id_of(begin, i);   // (ids of a thread rise with i)
     }
     double sum = 0.0;
-    if (a.sampling) {
+    if (a.sampling && most > -INFINITY) {   // (else no token of the chunk has a weight)
 #pragma unroll
-        for (int u = 0; u < VF_EACH / 4; ++u) {
-            const float s = (weight_of(v[4 * u], most, a.rate) + weight_of(v[4 * u + 1], most, a.rate)) +
-                            (weight_of(v[4 * u + 2], most, a.rate) + weight_of(v[4 * u + 3], most, a.rate));
+        for (int u = 0; u < VF_EACH / 8; ++u) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += fast_exp2((v[8 * u + e] - most) * a.rate);   // (-infinity: 0)
             sum += (double)s;
         }
         sum = warp_sum_f64(sum);
@@ -144,16 +145,17 @@ verify_rows_kernel(VerifyArgs a) {
 }
 
 // A row's statistics from its chunks', by one warp: every lane gets them.
-struct RowStats {
-    float top;
-    int id;
-    double sum;
-};
 __device__ __forceinline__ RowStats row_stats(const VerifyArgs& a, int row) {
     const int lane = threadIdx.x & 31;
+    const float2* tops = a.tops + (size_t)row * a.chunks;
+    const double* sums = a.sums + (size_t)row * a.chunks;
     RowStats s = {-INFINITY, 0x7fffffff, 0.0};
-    for (int c = lane; c < a.chunks; c += 32) {
-        const float2 t = a.tops[(size_t)row * a.chunks + c];
+    float2 mine = make_float2(-INFINITY, __int_as_float(0x7fffffff));
+    double part = 0.0;
+    if (lane < a.chunks) mine = tops[lane], part = sums[lane];   // (32 chunks are 262,144 logits: the loop below is for vocabularies beyond)
+    s.top = mine.x, s.id = __float_as_int(mine.y);
+    for (int c = lane + 32; c < a.chunks; c += 32) {
+        const float2 t = tops[c];
         const int id = __float_as_int(t.y);
         if (t.x > s.top || (t.x == s.top && id < s.id)) s.top = t.x, s.id = id;
     }
@@ -164,25 +166,23 @@ __device__ __forceinline__ RowStats row_stats(const VerifyArgs& a, int row) {
         if (top > s.top || (top == s.top && id < s.id)) s.top = top, s.id = id;
     }
     if (a.sampling) {
-        double sum = 0.0;
-        for (int c = lane; c < a.chunks; c += 32) {
-            const float m = a.tops[(size_t)row * a.chunks + c].x;
-            if (m > -INFINITY) sum += a.sums[(size_t)row * a.chunks + c] * exp(((double)m - (double)s.top) * a.inv_t);
+        double sum = mine.x > -INFINITY ? part * exp(((double)mine.x - (double)s.top) * a.inv_t) : 0.0;
+        for (int c = lane + 32; c < a.chunks; c += 32) {
+            const float m = tops[c].x;
+            if (m > -INFINITY) sum += sums[c] * exp(((double)m - (double)s.top) * a.inv_t);
         }
         s.sum = warp_sum_f64(sum);
     }
     return s;
 }
 
-// ---- (2) how many drafts stay, and the token behind them
+// ---- (2) how many drafts of an entry stay
 __global__ void __launch_bounds__(VR_THREADS)
-verify_choose_kernel(VerifyArgs a) {
+verify_decide_kernel(VerifyArgs a) {
     grid_chain_entry();
     constexpr int WARPS = VR_THREADS / 32;
-    __shared__ int kept_s, ticket_s, id_s[WARPS];
-    __shared__ float low_s[WARPS], t_top, d_top;
-    __shared__ double t_sum, d_sum, best_s[WARPS];
-    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ int kept_s;
+    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int before = 0;   // entries with rows in front of this one: each has a row more than it has drafts
     for (int i = 0; i < s; i += VR_THREADS) {
         const int e = i + threadIdx.x;
@@ -190,102 +190,125 @@ verify_choose_kernel(VerifyArgs a) {
     }
     const int row0 = a.first[s], row1 = a.first[s + 1], count = row1 - row0 - 1, draft0 = row0 - before;
     const bool empty = row1 == row0, wrong = !empty && (row0 < 0 || count < 0 || row1 > a.rows || count > a.most || draft0 < 0 || draft0 + count > a.total);
+    int* const tokens = a.tokens + (size_t)s * (a.most + 1);
     if (empty || wrong) {
-        if (blockIdx.x == 0) {
-            if (threadIdx.x == 0) a.accepted[s] = wrong ? -1 : 0;
-            for (int i = threadIdx.x; i <= a.most; i += VR_THREADS) a.tokens[(size_t)s * (a.most + 1) + i] = -1;
+        if (threadIdx.x == 0) {
+            a.accepted[s] = wrong ? -1 : 0;
+            a.decisions[s].kept = -1;
         }
+        for (int i = threadIdx.x; i <= a.most; i += VR_THREADS) tokens[i] = -1;
         return;
     }
     if (threadIdx.x == 0) kept_s = count;
     __syncthreads();
-    for (int j = warp; j < count; j += WARPS) {   // a warp per draft; the first that is refused ends the kept run
-        if (j >= __shfl_sync(0xffffffffu, *(volatile int*)&kept_s, 0)) break;
-        const int d = a.drafted[draft0 + j];
+    for (int j = warp; j <= count; j += WARPS) {   // a warp per draft, and one for the row behind the last; the first that is refused ends the kept run
+        if (j > __shfl_sync(0xffffffffu, *(volatile int*)&kept_s, 0)) break;
+        const int d = j < count ? a.drafted[draft0 + j] : -1;
         const bool known = d >= 0 && d < a.vocab;
+        const double u = a.sampling && j < count ? (double)a.uniforms[draft0 + j] : 0.0;
+        const float t_logit = a.sampling && known ? a.target[(row0 + j) * a.t_stride + d] : 0.f;
+        const float d_logit = a.draft && known ? a.draft[(draft0 + j) * a.d_stride + d] : 0.f;
         const RowStats t = row_stats(a, row0 + j);
-        bool keep;
-        if (!a.sampling) {
-            keep = known && t.id == d;
-        } else {
-            const double p = known ? exp(((double)a.target[(row0 + j) * a.t_stride + d] - (double)t.top) * a.inv_t) / t.sum : 0.0;
-            double q = 1.0;
-            if (a.draft) {
-                const RowStats r = row_stats(a, a.rows + draft0 + j);
-                q = known ? exp(((double)a.draft[(draft0 + j) * a.d_stride + d] - (double)r.top) * a.inv_t) / r.sum : 1.0;
+        RowStats r = {0.f, 0, 1.0};
+        if (a.draft && j < count) r = row_stats(a, a.rows + draft0 + j);
+        bool keep = j == count;
+        if (!keep && known) {
+            if (!a.sampling) {
+                keep = t.id == d;
+            } else {
+                const double p = exp(((double)t_logit - (double)t.top) * a.inv_t) / t.sum;
+                const double q = a.draft ? exp(((double)d_logit - (double)r.top) * a.inv_t) / r.sum : 1.0;
+                keep = u * q < p;
             }
-            keep = known && (double)a.uniforms[draft0 + j] * q < p;
         }
-        if (lane == 0 && !keep) atomicMin(&kept_s, j);
+        if (lane == 0) {
+            a.stats[row0 + j] = t;
+            if (a.draft && j < count) a.stats[a.rows + draft0 + j] = r;
+            if (!keep) atomicMin(&kept_s, j);
+        }
     }
     __syncthreads();
-    const int kept = kept_s, row = row0 + kept;
-    const bool refused = kept < count;
-    const int d_row = draft0 + kept;
-    auto write = [&](int chosen) {
-        for (int i = threadIdx.x; i <= a.most; i += VR_THREADS)
-            a.tokens[(size_t)s * (a.most + 1) + i] = i < kept ? a.drafted[draft0 + i] : i == kept ? chosen : -1;
-        if (threadIdx.x == 0) a.accepted[s] = kept;
-    };
-    if (!a.sampling) {   // (one block an entry)
-        if (warp == 0) {
-            const RowStats t = row_stats(a, row);
-            if (lane == 0) id_s[0] = t.id >= a.vocab ? 0 : t.id;
+    const int kept = kept_s;   // (its row has been worked out: no warp leaves out a row up to the lowest refused one)
+    for (int i = threadIdx.x; i <= a.most; i += VR_THREADS)
+        if (i != kept) tokens[i] = i < kept ? a.drafted[draft0 + i] : -1;
+    if (threadIdx.x == 0) {
+        const RowStats t = a.stats[row0 + kept];
+        const bool refused = kept < count;
+        a.accepted[s] = kept;
+        if (!a.sampling) {
+            tokens[kept] = t.id >= a.vocab ? 0 : t.id;
+            return;
         }
-        __syncthreads();
-        write(id_s[0]);
-        return;
+        RowStats r = {0.f, 0, 1.0};
+        if (refused && a.draft) r = a.stats[a.rows + draft0 + kept];
+        a.decisions[s] = Decision{kept, row0 + kept, refused && a.draft ? draft0 + kept : -1, refused && !a.draft ? a.drafted[draft0 + kept] : -1,
+                                  t.top, r.top, t.sum, r.sum};
     }
-    if (warp == 0) {
-        const RowStats t = row_stats(a, row);
-        if (lane == 0) t_top = t.top, t_sum = t.sum;
-    } else if (warp == 1 && refused && a.draft) {
-        const RowStats r = row_stats(a, a.rows + d_row);
-        if (lane == 0) d_top = r.top, d_sum = r.sum;
-    }
-    __syncthreads();
-    const float* t_row = a.target + row * a.t_stride;
-    const float* d_logits = refused && a.draft ? a.draft + d_row * a.d_stride : nullptr;
-    const int without = refused && !a.draft ? a.drafted[d_row] : -1;
-    const uint32_t key = row_key(a.seed, a.seq_ids[s], a.steps[s] + kept);
-    const float t_inv = (float)(1.0 / t_sum), d_inv = d_logits ? (float)(1.0 / d_sum) : 0.f;
-    // the two best of a thread, by the upper bounds of their scores
+}
+
+// ---- (3) the token behind the kept drafts. A score is r / E. p = 2^((x - top) rate - log2 sum): the difference, the product and the exponent round by
+// 2^-24 each, of numbers that are at most a few tens for any token with a chance, and the hardware's exponential by 2^-22: p is within 6e-6 of its value
+// as a share. E = -ln u: near 1 by its series in w = 1 - u, which is exact in float32, else by the hardware's logarithm, within 6e-6 as well. So a score
+// lies between (p - q - 6e-6 (p + q)) (1 - 6e-6) / E and the same with other signs; of a thread's tokens the two with the highest upper bounds are
+// kept, and whichever of them reach the block's highest lower bound are scored again in float64.
+#define VR_SLACK 6.0e-6f
+template <int EACH>
+__global__ void __launch_bounds__(VR_THREADS)
+verify_draw_kernel(VerifyArgs a) {
+    grid_chain_entry();
+    constexpr int WARPS = VR_THREADS / 32, CHUNK = VR_THREADS * EACH;
+    __shared__ int ticket_s, id_s[WARPS];
+    __shared__ float low_s[WARPS];
+    __shared__ double best_s[WARPS];
+    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Decision made = a.decisions[s];
+    if (made.kept < 0) return;
+    const float* t_row = a.target + made.row * a.t_stride;
+    const float* d_row = made.d_row >= 0 ? a.draft + made.d_row * a.d_stride : nullptr;
+    const int begin = blockIdx.x * CHUNK, end = min(a.vocab, begin + CHUNK);
+    float x[EACH], y[EACH];
+    load_logits(t_row, begin, end, x);
+    if (d_row) load_logits(d_row, begin, end, y);
+    const uint32_t key = row_key(a.seed, a.seq_ids[s], a.steps[s] + made.kept);
+    const float t_log = (float)log2(made.t_sum), d_log = (float)log2(made.d_sum);
     float high[2] = {-1.f, -1.f}, low = -1.f;
-    int high_id[2] = {-1, -1};
-    const int begin = blockIdx.x * VR_CHUNK, end = min(a.vocab, begin + VR_CHUNK);
+    int high_at[2] = {-1, -1};
 #pragma unroll
-    for (int u = 0; u < VR_EACH; ++u) {
-        const int i = begin + threadIdx.x + u * VR_THREADS;
-        if (i >= end || i == without) continue;
-        const float p = weight_of(t_row[i], t_top, a.rate) * t_inv;
-        const float q = d_logits ? weight_of(d_logits[i], d_top, a.rate) * d_inv : 0.f;
-        const float uniform = ((float)token_bits(key, (uint32_t)i) + 0.5f) * (1.0f / 8388608.0f);
-        const float wait = -logf(uniform);
-        // p and q are within 2^-20 of their values, the quotient within 2^-21 more
-        const float slack = (p + q) * 2.0e-6f, sure = fmaxf(p - q - slack, 0.f) / wait, may = fmaxf(p - q + slack, 0.f) / wait;
-        low = fmaxf(low, sure);
+    for (int i = 0; i < EACH; ++i) {
+        const int id = id_of(begin, i);
+        const float p = fast_exp2(fmaf(x[i] - made.t_top, a.rate, -t_log));
+        const float q = d_row ? fast_exp2(fmaf(y[i] - made.d_top, a.rate, -d_log)) : 0.f;
+        const uint32_t bits = token_bits(key, (uint32_t)id);
+        const float u = ((float)bits + 0.5f) * (1.0f / 8388608.0f), w = ((float)(8388607u - bits) + 0.5f) * (1.0f / 8388608.0f);
+        const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(u);
+        const float r = p - q, slack = (p + q) * VR_SLACK, per = __fdividef(1.f, wait);
+        const bool in = id < end && id != made.without;
+        const float may = in ? fmaf(r, VR_SLACK, r + slack) * per : -1.f;
+        if (in) low = fmaxf(low, (r - slack) * (1.f - VR_SLACK) * per);
         if (may > high[0]) {
-            high[1] = high[0], high_id[1] = high_id[0];
-            high[0] = may, high_id[0] = i;
+            high[1] = high[0], high_at[1] = high_at[0];
+            high[0] = may, high_at[0] = i;
         } else if (may > high[1]) {
-            high[1] = may, high_id[1] = i;
+            high[1] = may, high_at[1] = i;
         }
     }
-    low = warp_max(low);
+    low = warp_max(fmaxf(low, 0.f));
     if (lane == 0) low_s[warp] = low;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) low = fmaxf(low, low_s[w]);
     double best = -1.0;
     int best_id = 0x7fffffff;
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-        if (high_id[k] < 0 || !(high[k] >= low)) continue;
-        const int i = high_id[k];
-        double r = exp(((double)t_row[i] - (double)t_top) * a.inv_t) / t_sum;
-        if (d_logits) r = fmax(r - exp(((double)d_logits[i] - (double)d_top) * a.inv_t) / d_sum, 0.0);
-        const double score = r / -log(((double)token_bits(key, (uint32_t)i) + 0.5) / 8388608.0);
-        if (score > best || (score == best && i < best_id)) best = score, best_id = i;
+        const float reach = k ? high[1] : high[0];
+        const int i = k ? high_at[1] : high_at[0];
+        if (i < 0 || !(reach >= low)) continue;
+        const int id = id_of(begin, i);
+        double r = exp(((double)t_row[id] - (double)made.t_top) * a.inv_t) / made.t_sum;
+        if (d_row) r = fmax(r - exp(((double)d_row[id] - (double)made.d_top) * a.inv_t) / made.d_sum, 0.0);
+        const double score = r / -log(((double)token_bits(key, (uint32_t)id) + 0.5) / 8388608.0);
+        if (score > best || (score == best && id < best_id)) best = score, best_id = id;
     }
     auto better = [](double v, int i, double than, int than_i) { return v > than || (v == than && i < than_i); };
     auto warp_best = [&]() {
@@ -299,67 +322,59 @@ verify_choose_kernel(VerifyArgs a) {
     warp_best();
     if (lane == 0) best_s[warp] = best, id_s[warp] = best_id;
     __syncthreads();
-    if (warp == 0) {
-        best = lane < WARPS ? best_s[lane] : -1.0;
-        best_id = lane < WARPS ? id_s[lane] : 0x7fffffff;
-        warp_best();
-        if (lane == 0) {
-            a.best[(size_t)s * a.race_chunks + blockIdx.x] = make_double2(best, (double)best_id);
-            __threadfence();
-            ticket_s = atomicAdd(a.counters + s, 1);
-        }
+    if (warp != 0) return;
+    best = lane < WARPS ? best_s[lane] : -1.0;
+    best_id = lane < WARPS ? id_s[lane] : 0x7fffffff;
+    warp_best();
+    if (lane == 0) {
+        a.best[(size_t)s * a.race_chunks + blockIdx.x] = make_double2(best, (double)best_id);
+        __threadfence();
+        ticket_s = atomicAdd(a.counters + s, 1);
     }
-    __syncthreads();
-    if (ticket_s != a.race_chunks - 1) return;
+    __syncwarp();
+    if (ticket_s != (int)gridDim.x - 1) return;
     __threadfence();
-    if (warp == 0) {
-        best = -1.0;
-        best_id = 0x7fffffff;
-        for (int c = lane; c < a.race_chunks; c += 32) {
-            const double2 b = __ldcg(a.best + (size_t)s * a.race_chunks + c);
-            if (better(b.x, (int)b.y, best, best_id)) best = b.x, best_id = (int)b.y;
-        }
-        warp_best();
-        if (lane == 0) {
-            a.counters[s] = 0;
-            id_s[0] = best_id >= a.vocab ? 0 : best_id;
-        }
+    best = -1.0;
+    best_id = 0x7fffffff;
+    for (int c = lane; c < (int)gridDim.x; c += 32) {
+        const double2 b = __ldcg(a.best + (size_t)s * a.race_chunks + c);
+        if (better(b.x, (int)b.y, best, best_id)) best = b.x, best_id = (int)b.y;
     }
-    __syncthreads();
-    write(id_s[0]);
-}
-
-// Chunks of a row in (1), and of an entry in (2).
-QF_EXPORT int qf_verify_chunks(int vocab, int* sizes) {
-    sizes[0] = (vocab + VF_CHUNK - 1) / VF_CHUNK;
-    sizes[1] = (vocab + VR_CHUNK - 1) / VR_CHUNK;
-    return 0;
+    warp_best();
+    if (lane == 0) {
+        a.counters[s] = 0;
+        a.tokens[(size_t)s * (a.most + 1) + made.kept] = best_id >= a.vocab ? 0 : best_id;
+    }
 }
 
 // target [rows][t_stride >= vocab] and draft [total][d_stride] (or null) float32; drafted, uniforms [total]; first [n + 1]; accepted [n],
-// tokens [n][most + 1]; sums, tops, best, counters: workspaces of (rows + draft rows) x chunks, n x race chunks and n, counters zero before the
-// first call (the kernel leaves them zero).
+// tokens [n][most + 1]. Workspaces: sums (8 bytes) and tops (8) of (rows + draft rows) x chunks of VF_CHUNK, stats (16) of rows + draft rows, decisions
+// (40) of n, best (16) of n x chunks of VR_THREADS * VR_FEW, counters int32 of n, zero before the first call (the kernels leave them zero).
 QF_EXPORT int qf_verify_drafts(const float* target, int rows, int vocab, long long t_stride, const float* draft, long long d_stride, const int* drafted,
                                int total, const int* first, int n, const float* uniforms, float temperature, unsigned long long seed,
-                               const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most, double* sums, void* tops, void* best,
-                               int* counters, cudaStream_t stream) {
+                               const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most, double* sums, void* tops, void* stats,
+                               void* decisions, void* best, int* counters, cudaStream_t stream) {
+    static_assert(sizeof(Decision) == 40 && sizeof(RowStats) == 16, "what the workspaces are sized by");
     if (n <= 0 || vocab <= 0) return 0;
     VerifyArgs a = {};
     a.target = target, a.draft = draft, a.t_stride = t_stride, a.d_stride = d_stride, a.drafted = drafted, a.first = first, a.uniforms = uniforms;
-    a.seq_ids = seq_ids, a.steps = steps, a.accepted = accepted, a.tokens = tokens, a.sums = sums, a.tops = (float2*)tops, a.best = (double2*)best;
-    a.counters = counters, a.rows = rows, a.total = total, a.vocab = vocab, a.n = n, a.most = most, a.seed = seed, a.sampling = temperature > 0.f;
-    a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_CHUNK - 1) / VR_CHUNK;
+    a.seq_ids = seq_ids, a.steps = steps, a.accepted = accepted, a.tokens = tokens, a.sums = sums, a.tops = (float2*)tops, a.stats = (RowStats*)stats;
+    a.decisions = (Decision*)decisions, a.best = (double2*)best, a.counters = counters, a.rows = rows, a.total = total, a.vocab = vocab, a.n = n;
+    a.most = most, a.seed = seed, a.sampling = temperature > 0.f;
+    a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_THREADS * VR_FEW - 1) / (VR_THREADS * VR_FEW);
     if (a.sampling) {
         a.inv_t = 1.0 / (double)temperature;
-        const double rate = 1.4426950408889634 * a.inv_t;
-        a.rate.hi = (float)rate;
-        a.rate.lo = (float)(rate - (double)a.rate.hi);
+        a.rate = (float)(1.4426950408889634 * a.inv_t);
     }
     const long long all = (long long)rows + (draft ? total : 0);
     if (n > 65535 || all > 65535) return (int)cudaErrorInvalidValue;
-    if (all > 0) {
-        const cudaError_t e = launch_pdl(verify_rows_kernel, dim3((unsigned)a.chunks, (unsigned)all), dim3(VF_THREADS), 0, stream, a);
-        if (e != cudaSuccess) return (int)e;
-    }
-    return (int)launch_pdl(verify_choose_kernel, dim3(a.sampling ? (unsigned)a.race_chunks : 1u, (unsigned)n), dim3(VR_THREADS), 0, stream, a);
+    cudaError_t e = cudaSuccess;
+    if (all > 0) e = launch_pdl(verify_rows_kernel, dim3((unsigned)a.chunks, (unsigned)all), dim3(VF_THREADS), 0, stream, a);
+    if (e == cudaSuccess) e = launch_pdl(verify_decide_kernel, dim3((unsigned)n), dim3(VR_THREADS), 0, stream, a);
+    if (e != cudaSuccess || !a.sampling) return (int)e;
+    // Blocks of 2,048 tokens where they all fit the SMs at once (five to an SM), of 8,192 else.
+    const unsigned many = (unsigned)((vocab + VR_THREADS * VR_MANY - 1) / (VR_THREADS * VR_MANY));
+    if ((long long)a.race_chunks * n <= 5ll * qf_sm_count())
+        return (int)launch_pdl(verify_draw_kernel<VR_FEW>, dim3((unsigned)a.race_chunks, (unsigned)n), dim3(VR_THREADS), 0, stream, a);
+    return (int)launch_pdl(verify_draw_kernel<VR_MANY>, dim3(many, (unsigned)n), dim3(VR_THREADS), 0, stream, a);
 }

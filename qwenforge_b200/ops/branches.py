@@ -4,6 +4,8 @@ pointers, the current stream, error codes."""
 from __future__ import annotations
 
 import ctypes
+from array import array
+from itertools import chain
 from typing import Optional, Sequence
 
 import numpy as np
@@ -11,41 +13,75 @@ import torch
 
 from ..csrc import library
 from . import kernels
-from .kernels import _F, _I, _LL, _P, _ULL, KernelError, _check, _dev, _ptr, _stream
-
+from .kernels import KernelError, _check, _dev
 
 PAGE_TOKENS = 64   # positions of a cache page (QF_PAGE of the kernels, and what the cache hands out)
+_P, _I, _LL, _ULL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_float
+_functions: dict = {}   # exported functions with their argument types (numbers are then converted by the call itself)
+
+
+def _function(lib: str, name: str, *types):
+    fn = _functions.get(name)
+    if fn is None:
+        fn = getattr(library(lib), name)
+        fn.argtypes, fn.restype = types, _I
+        _functions[name] = fn
+    return fn
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _here(what: str, *tensors) -> None:
     """The tensors lie on the current device, whose current stream the kernels run on."""
-    current = torch._C._cuda_getDevice()
+    current = -1
     for t in tensors:
-        if t is not None and t.device.index != current:
+        if t is not None and (t.get_device() != current or current < 0):
+            if not t.is_cuda:
+                raise KernelError(f"{what}: a tensor is on {t.device}: the kernels of this library run on CUDA devices only")
+            if current < 0:
+                current = torch._C._cuda_getDevice()
+            if t.get_device() == current:
+                continue
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{current}")
 
 
+# ---------------------------------------------------------------------------------------------------------------- pages
+_MOVES_WRONG = {-1: "a move names a page outside 0 .. {pages}", -2: "a move names rows outside 0 .. {rows}", -3: "a page is the target of two moves",
+                -4: "a page is the source of one move and the target of another", -5: "no memory for checking the moves"}
+
+
+def _flat_moves(moves, n_rows: int) -> array:
+    try:
+        if isinstance(moves, np.ndarray):
+            moves = moves.tolist()
+        widths = set(map(len, moves))
+        if not widths <= {3}:
+            if widths != {2}:
+                raise KernelError("copy_pages: moves are (from, to) or (from, to, rows)")
+            moves = [(source, target, n_rows) for source, target in moves]
+        return array("i", chain.from_iterable(moves))
+    except (TypeError, OverflowError) as exc:
+        raise KernelError(f"copy_pages: moves are (from, to) or (from, to, rows), small whole numbers ({exc})") from None
+
+
+def _moves_error(code: int, n_pages: int, n_rows: int) -> KernelError:
+    return KernelError("copy_pages: " + _MOVES_WRONG[code].format(pages=n_pages - 1, rows=n_rows))
+
+
 def page_moves(moves, n_pages: int, n_rows: int) -> np.ndarray:
-    """`moves` as int32 [n, 3] (from, to, rows), checked: pages 0 .. n_pages - 1, rows 0 .. n_rows (whole pages where a move names
+    """`moves` as int32 [n, 3] (from, to, rows), checked: pages 0 .. n_pages - 1, rows 0 .. n_rows (whole pages where the moves name
     none), no page a target twice, none both a source and a target."""
-    array = np.asarray(moves, dtype=np.int64)
-    if array.size == 0:
-        return np.zeros((0, 3), dtype=np.int32)
-    if array.ndim != 2 or array.shape[1] not in (2, 3):
-        raise KernelError("copy_pages: moves are (from, to) or (from, to, rows)")
-    if array.shape[1] == 2:
-        array = np.concatenate((array, np.full((len(array), 1), n_rows, dtype=np.int64)), axis=1)
-    if array[:, :2].min() < 0 or array[:, :2].max() >= n_pages:
-        raise KernelError(f"copy_pages: a move names a page outside 0 .. {n_pages - 1}")
-    if array[:, 2].min() < 0 or array[:, 2].max() > n_rows:
-        raise KernelError(f"copy_pages: a move names rows outside 0 .. {n_rows}")
-    seen = np.zeros(n_pages, dtype=np.uint8)
-    seen[array[:, 1]] = 1
-    if int(seen.sum()) != len(array):
-        raise KernelError("copy_pages: a page is the target of two moves")
-    if seen[array[:, 0]].any():
-        raise KernelError("copy_pages: a page is the source of one move and the target of another")
-    return np.ascontiguousarray(array, dtype=np.int32)
+    flat = _flat_moves(moves, n_rows)
+    code = _function("page_copy", "qf_page_moves_check", _P, _I, _I, _I)(flat.buffer_info()[0], len(flat) // 3, n_pages, n_rows)
+    if code:
+        raise _moves_error(code, n_pages, n_rows)
+    return np.array(flat, dtype=np.int32).reshape(-1, 3)
 
 
 def copy_pages(storage: torch.Tensor, moves) -> None:
@@ -53,42 +89,44 @@ def copy_pages(storage: torch.Tensor, moves) -> None:
     (a page dense, entries and pages at any distance; a storage of two or three dimensions has pages of one row). moves: (from, to, rows)
     or (from, to) on the host: the first `rows` rows of page `from`, in each of its planes and heads, become those of page `to`; the
     others stay as they are. No page may be the target of two moves, or both a source and a target."""
-    _dev("storage", storage, contiguous=False)
-    if storage.dim() < 2:
+    shape, strides = storage.shape, storage.stride()
+    if len(shape) < 2:
         raise KernelError("copy_pages: storage has entries and pages")
-    entries, pages = storage.shape[:2]
-    inner = tuple(storage.shape[2:])
-    n_rows, width = (inner[-2], inner[-1]) if len(inner) >= 2 else (1, inner[0] if inner else 1)
-    segments = 1
-    for d in inner[:-2]:
-        segments *= d
-    checked = page_moves(moves, pages, n_rows)
-    page = segments * n_rows * width
-    if page == 0 or entries == 0 or len(checked) == 0:
-        return
-    want = 1
-    for size, stride in zip(reversed(inner), reversed(storage.stride()[2:])):
+    entries, pages = shape[0], shape[1]
+    n_rows, width = (shape[-2], shape[-1]) if len(shape) >= 4 else (1, shape[2] if len(shape) == 3 else 1)
+    segments, want = 1, 1
+    for size, stride in zip(shape[:1:-1], strides[:1:-1]):
         if size != 1 and stride != want:
             raise KernelError("copy_pages: a page of the storage is not contiguous")
         want *= size
-    e_stride, p_stride = storage.stride(0), storage.stride(1)
+    for size in shape[2:-2]:
+        segments *= size
+    page = want
+    e_stride, p_stride = strides[0] if entries > 1 else 0, strides[1] if pages > 1 else 0
     if (pages > 1 and p_stride < page) or (entries > 1 and e_stride < page) or (
             entries > 1 and pages > 1 and e_stride < (pages - 1) * p_stride + page and p_stride < (entries - 1) * e_stride + page):
-        raise KernelError("copy_pages: pages of the storage overlap")
+        if page > 0:
+            raise KernelError("copy_pages: pages of the storage overlap")
+    if entries > 65535:
+        raise KernelError(f"copy_pages: {entries} entries are more than a launch takes (65,535)")
     _here("copy_pages", storage)
-    item = storage.element_size()
-    sizes = (storage.data_ptr(), width * item, e_stride * item if entries > 1 else 0, p_stride * item if pages > 1 else 0)
-    unit = next(u for u in (16, 4, 2, 1) if all(s % u == 0 for s in sizes))
-    launched = _I(0)
-    code = library("page_copy").qf_copy_pages(
-        _ptr(storage), _I(entries), _LL(sizes[2]), _LL(sizes[3]), _I(segments), _LL(n_rows * width * item), _LL(width * item), _I(unit),
-        _P(checked.ctypes.data), _I(len(checked)), ctypes.byref(launched), _stream())
-    kernels.launches += launched.value - 1
+    flat, item = _flat_moves(moves, n_rows), storage.element_size()
+    n, base, row = len(flat) // 3, storage.data_ptr(), width * item
+    e_bytes, p_bytes = e_stride * item, p_stride * item
+    low = base | row | e_bytes | p_bytes
+    unit = 16 if not low & 15 else 4 if not low & 3 else 2 if not low & 1 else 1
+    code = _function("page_copy", "qf_copy_pages", _P, _I, _I, _I, _LL, _LL, _I, _LL, _LL, _I, _P, _I, _P)(
+        base, entries, pages, n_rows, e_bytes, p_bytes, segments if page else 0, n_rows * row, row, unit, flat.buffer_info()[0], n, _stream())
+    if code < 0:
+        raise _moves_error(code, pages, n_rows)
+    kernels.launches += -(-n // 1024) - 1 if page and entries else -1
     _check(code, "copy_pages")
 
 
+# ---------------------------------------------------------------------------------------------------------------- attention
 SHARED_MAX_HEAD_DIM = 256
 SHARED_MAX_SEQS = 2048
+SHARED_TEAM = 4   # warps of a block of the parts' kernel (SH_TEAM)
 
 
 class SharedPrefix:
@@ -124,6 +162,7 @@ class SharedPrefix:
         sizes = (self.n_seqs, self.n_seqs, len(members), len(begin), len(pages))
         packed = torch.tensor(entry_pages + entry_group + members + begin + pages, dtype=torch.int32).to(device)
         self.entry_pages, self.entry_group, self.members, self.begin, self.pages = packed.split(sizes)
+        self.sizes: dict = {}   # shape of an attention -> what its plans and workspaces are sized by
 
     def __len__(self) -> int:
         return len(self.groups)
@@ -166,11 +205,15 @@ class SharedPlan:
 
 
 def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: SharedPrefix, own_pages: int) -> tuple:
-    """((block records, warp records, tile records) of the plan, most shared parts, most own parts of a row): bounds of what the plan kernel
-    can come to, whatever the lengths. It gives a warp at least `pages x tiles x kv heads / warps` pages, so block records cover, up to
-    twice, no more than the warps there are; tile records fill the SMs once, or are the pairs of tiles uncut."""
+    """((units, tile records) of the plan, most shared parts, most own parts of a row): bounds of what the plan kernel can come to, whatever the
+    lengths. It gives a warp at least `pages x tiles x kv heads / warps` pages, so units of a block's run cover, up to twice, no more
+    than the warps there are, and so do single warps' records but for one more per item; tile records fill the SMs once, or are the
+    pairs of tiles uncut."""
+    held = share.sizes.get((dtype, head_dim, kv_heads, n_heads, own_pages))
+    if held is not None:
+        return held
     sizes = (_I * 7)()
-    code = library("attention_shared").qf_attention_shared_shape(_I(int(dtype == torch.bfloat16)), _I(head_dim), sizes)
+    code = _function("attention_shared", "qf_attention_shared_shape", _I, _I, _P)(int(dtype == torch.bfloat16), head_dim, sizes)
     if code:
         raise KernelError(f"attention_shared: CUDA error {code} when asked for its sizes")
     row_tile, warps, team, most, tile_rows, tile_pages, sms = sizes
@@ -186,19 +229,21 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
         pairs = []
     for n in pairs:
         most_shared = max(most_shared, min(most, -(-share.bound_pages // 4), sms // (kv_heads * n) + 1))
-    records = (2 * warps // (team * kv_heads) + 2, warps // kv_heads + 1 + sum(tiles) + share.n_seqs * own_tiles,
-               max(sms // kv_heads, sum(pairs)) if pairs else 0)
-    return records, most_shared, parts(own_pages, own_tiles)
+    singles = warps // kv_heads + 1 + sum(tiles) + share.n_seqs * own_tiles
+    records = (2 * warps // (team * kv_heads) + 2 + -(-singles // SHARED_TEAM), max(sms // kv_heads, sum(pairs)) if pairs else 0)
+    if len(share.sizes) >= 64:
+        share.sizes.clear()
+    held = share.sizes[dtype, head_dim, kv_heads, n_heads, own_pages] = (records, most_shared, parts(own_pages, own_tiles))
+    return held
 
 
-def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, kv_heads: int, head_dim: int, n_heads: int,
-                          n_seqs: int, share: SharedPrefix, scratch: SharedScratch, dtype: torch.dtype, max_kv_len: int) -> SharedPlan:
-    """The plan of one step for `attention_shared` of this shape, worked out on the device from the batch's lengths; it serves every
-    layer of the step with this shape. `max_kv_len`: an upper bound of any sequence's length after the step. The tensor belongs to
-    `scratch` and is overwritten by the next plan of the same shape."""
-    for name, t in (("cu_q", cu_q), ("tok_pos", tok_pos), ("slots", slots)):
-        _dev(name, t, torch.int32)
-    if dtype not in (torch.bfloat16, torch.float32):
+def _batch_refused(cu_q, tok_pos, slots, n_seqs: int, kv_heads: int, n_heads: int, head_dim: int, dtype, share: SharedPrefix) -> None:
+    """Raises what is wrong with a batch, its shape or what it shares; returns if nothing is."""
+    i32 = torch.int32
+    if not (cu_q.dtype is i32 and tok_pos.dtype is i32 and slots.dtype is i32 and cu_q.is_contiguous() and tok_pos.is_contiguous() and slots.is_contiguous()):
+        for name, t in (("cu_q", cu_q), ("tok_pos", tok_pos), ("slots", slots)):
+            _dev(name, t, i32)
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise KernelError(f"attention_shared: dtype {dtype} is not supported (bfloat16 or float32)")
     if not 0 < head_dim <= SHARED_MAX_HEAD_DIM:
         raise KernelError(f"attention_shared: head_dim {head_dim} > {SHARED_MAX_HEAD_DIM} is not supported")
@@ -208,18 +253,26 @@ def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torc
         raise KernelError(f"attention_shared: a batch of {n_seqs} sequences is not supported (1 to {SHARED_MAX_SEQS})")
     if share.n_seqs != n_seqs or slots.numel() != n_seqs or cu_q.numel() != n_seqs + 1 or tok_pos.numel() != n_seqs:
         raise KernelError("attention_shared: wants exactly one token per sequence, and a SharedPrefix of this batch")
+
+
+def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, kv_heads: int, head_dim: int, n_heads: int,
+                          n_seqs: int, share: SharedPrefix, scratch: SharedScratch, dtype: torch.dtype, max_kv_len: int) -> SharedPlan:
+    """The plan of one step for `attention_shared` of this shape, worked out on the device from the batch's lengths; it serves every
+    layer of the step with this shape. `max_kv_len`: an upper bound of any sequence's length after the step. The tensor belongs to
+    `scratch` and is overwritten by the next plan of the same shape."""
+    _batch_refused(cu_q, tok_pos, slots, n_seqs, kv_heads, n_heads, head_dim, dtype, share)
     _here("attention_shared", cu_q, tok_pos, slots, share.entry_pages)
     own_pages = max(1, -(-int(max_kv_len) // PAGE_TOKENS) - share.least_pages)
     records, most_shared, most_own = _shared_sizes(dtype, head_dim, kv_heads, n_heads, share, own_pages)
     key = (n_seqs, kv_heads, n_heads, head_dim, dtype)
-    ints = 4 + -(-n_seqs // 4) * 4 + sum(records) * 8
+    ints = 4 + -(-n_seqs // 4) * 4 + (records[0] * SHARED_TEAM + records[1]) * 8
     held = scratch.plans.get(key)
     if held is None or held.numel() < ints:
         held = scratch.plans[key] = torch.empty(ints, dtype=torch.int32, device=cu_q.device)
-    _check(library("attention_shared").qf_attention_shared_plan(
-        _ptr(tok_pos), _ptr(slots), _I(n_seqs), _ptr(share.entry_pages), _ptr(share.entry_group), _ptr(share.begin), _ptr(share.pages), _I(len(share)),
-        _I(kv_heads), _I(n_heads), _I(int(dtype == torch.bfloat16)), _I(head_dim), _I(most_shared), _I(most_own),
-        _ptr(held), *map(_I, records), _stream()), "attention_shared_plan")
+    _check(_function("attention_shared", "qf_attention_shared_plan", _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P)(
+        tok_pos.data_ptr(), slots.data_ptr(), n_seqs, share.entry_pages.data_ptr(), share.entry_group.data_ptr(), share.begin.data_ptr(),
+        share.pages.data_ptr(), len(share.groups), kv_heads, n_heads, dtype is torch.bfloat16, head_dim, most_shared, most_own, held.data_ptr(),
+        records[0], records[1], _stream()), "attention_shared_plan")
     return SharedPlan(held, key, records, most_shared + most_own)
 
 
@@ -232,61 +285,70 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
     entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page table
     has room for). `plan` (`attention_shared_plan` with the same shape, made in this step) is made here when absent. `sinks` (float32
     [n_heads]): a logit per head that joins the softmax's denominator once, with no key and no value."""
-    _dev("q", q)
-    _dev("out", out, q.dtype)
-    _dev("cache", site.storage, q.dtype, contiguous=False)
-    _dev("page table", site.table, torch.int32, contiguous=False)
-    _dev("err", err, torch.int32)
-    d, page = site.head_dim, PAGE_TOKENS
+    storage, table, d, kv_heads, dtype = site.storage, site.table, site.head_dim, site.kv_heads, q.dtype
+    _batch_refused(cu_q, tok_pos, slots, n_seqs, kv_heads, n_heads, d, dtype, share)
+    if not (out.dtype is dtype and storage.dtype is dtype and q.is_contiguous() and out.is_contiguous() and table.dtype is torch.int32
+            and err.dtype is torch.int32):
+        for name, t, of, dense in (("q", q, dtype, True), ("out", out, dtype, True), ("cache", storage, dtype, False), ("page table", table, torch.int32, False),
+                                   ("err", err, torch.int32, True)):
+            _dev(name, t, of, dense)
     if q.shape != (n_seqs, n_heads * d) or out.shape != q.shape:
         raise KernelError("attention_shared: wants exactly one token per sequence, q and out [n_seqs, n_heads * head_dim]")
-    if site.storage.dim() != 5 or tuple(site.storage.shape[1:]) != (2, site.kv_heads, page, d) or not site.storage[:1].is_contiguous() \
-            or site.page_elems < 2 * site.kv_heads * page * d:
-        raise KernelError(f"attention_shared: the cache is [pages, 2, kv_heads, {page}, head_dim], a page dense")
-    if site.table.dim() != 2 or site.table.stride(1) != 1:
+    page, strides = kv_heads * PAGE_TOKENS * d, storage.stride()
+    if len(strides) != 5 or storage.shape[1:] != (2, kv_heads, PAGE_TOKENS, d) or (strides[1:] != (page, PAGE_TOKENS * d, d, 1) and not storage[:1].is_contiguous()) or site.page_elems < 2 * page:
+        raise KernelError(f"attention_shared: the cache is [pages, 2, kv_heads, {PAGE_TOKENS}, head_dim], a page dense")
+    if table.dim() != 2 or table.stride(1) != 1:
         raise KernelError("attention_shared: the page table is [slots, pages] with unit inner stride")
-    if share.most_pages > site.table.shape[1]:
-        raise KernelError(f"attention_shared: a group shares {share.most_pages} pages, the page table has room for {site.table.shape[1]}")
-    fast = q.dtype == torch.bfloat16 and d in kernels.FAST_ATTENTION_HEAD_DIMS
-    if fast and (q.data_ptr() % 16 or site.storage.data_ptr() % 16 or site.page_elems % d):
+    if share.most_pages > table.shape[1]:
+        raise KernelError(f"attention_shared: a group shares {share.most_pages} pages, the page table has room for {table.shape[1]}")
+    q_at, storage_at = q.data_ptr(), storage.data_ptr()
+    if dtype is torch.bfloat16 and d in kernels.FAST_ATTENTION_HEAD_DIMS and (q_at % 16 or storage_at % 16 or site.page_elems % d):
         raise KernelError("attention_shared: q and the cache begin on 16 bytes, and a page holds whole rows")
     if sinks is not None:
         _dev("sinks", sinks, torch.float32)
         if sinks.numel() != n_heads:
             raise KernelError("attention_shared: sinks must hold one float32 per query head")
-    _here("attention_shared", q, out, cu_q, tok_pos, slots, site.storage, site.table, share.entry_pages, err, sinks)
+    _here("attention_shared", q, out, cu_q, tok_pos, slots, storage, table, share.entry_pages, err, sinks)
     if plan is None:
-        longest = site.table.shape[1] * page if max_kv_len is None else int(max_kv_len)
-        plan = attention_shared_plan(cu_q, tok_pos, slots, site.kv_heads, d, n_heads, n_seqs, share, scratch, q.dtype, longest)
-    elif plan.key != (n_seqs, site.kv_heads, n_heads, d, q.dtype):
+        longest = table.shape[1] * PAGE_TOKENS if max_kv_len is None else int(max_kv_len)
+        plan = attention_shared_plan(cu_q, tok_pos, slots, kv_heads, d, n_heads, n_seqs, share, scratch, dtype, longest)
+    elif plan.key != (n_seqs, kv_heads, n_heads, d, dtype):
         raise KernelError("attention_shared: the plan was made for another shape")
     scratch.ensure(n_seqs * n_heads * plan.most_parts, d)
-    code = library("attention_shared").qf_attention_shared(
-        _I(int(q.dtype == torch.bfloat16)), _ptr(q), _ptr(out), _ptr(tok_pos), _ptr(slots), _ptr(share.members), _ptr(share.begin),
-        _ptr(plan.tensor), *map(_I, plan.records), _ptr(site.storage), _ptr(site.table), _LL(site.page_elems),
-        _I(site.table_stride), _I(site.kv_heads), _I(d), _I(n_heads), _I(n_seqs), _F(scale), _I(plan.most_parts), _ptr(scratch.part_o),
-        _ptr(scratch.part_ml), _ptr(sinks), _ptr(err), _stream())
-    kernels.launches += 2 if plan.records[2] else 1   # (the tiles, the parts, and their joining)
+    units, tiles = plan.records
+    code = _function("attention_shared", "qf_attention_shared", _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _LL, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P,
+                     _P)(
+        dtype is torch.bfloat16, q_at, out.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), share.members.data_ptr(), share.begin.data_ptr(),
+        plan.tensor.data_ptr(), units, tiles, storage_at, table.data_ptr(), site.page_elems, site.table_stride, kv_heads, d, n_heads, n_seqs, scale,
+        plan.most_parts, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), _at(sinks), err.data_ptr(), _stream())
+    kernels.launches += 2 if tiles else 1   # (the tiles, the parts, and their joining)
     _check(code, "attention_shared")
 
 
+# ---------------------------------------------------------------------------------------------------------------- drafts
+VERIFY_CHUNK = 8192        # logits of a block, and tokens of one that draws at the least (VF_CHUNK, VR_THREADS * VR_FEW of the kernels)
+VERIFY_RACE_CHUNK = 2048
+
+
 class VerifyScratch:
-    """Workspaces of `verify_drafts`: what the blocks of a row and of an entry leave for one another, and ticket counters (kept zero
-    between calls by the kernel itself). One instance serves calls that run one after another on one stream; what is captured into a
-    graph has one of its own."""
+    """Workspaces of `verify_drafts`: what its kernels leave for one another, and ticket counters (kept zero between calls by the kernel
+    itself). One instance serves calls that run one after another on one stream; what is captured into a graph has one of its own."""
 
     def __init__(self):
-        self.sums = self.tops = self.best = self.counters = None
+        self.held = self.counters = None   # one buffer of 8-byte words for all but the counters
 
-    def ensure(self, row_chunks: int, entry_chunks: int, entries: int, device) -> None:
-        def room(held, count, width, dtype):
-            if held is None or held.numel() < count * width or held.device != device:
-                return torch.zeros(count * width, dtype=dtype, device=device)
-            return held
-        self.sums = room(self.sums, row_chunks, 1, torch.float64)
-        self.tops = room(self.tops, row_chunks, 2, torch.int32)     # (float32 maximum, id)
-        self.best = room(self.best, entry_chunks, 2, torch.float64)  # (score, id)
-        self.counters = room(self.counters, entries, 1, torch.int32)
+    def ensure(self, row_chunks: int, rows: int, entry_chunks: int, entries: int, device) -> tuple:
+        """The addresses of sums, tops, stats, decisions and best."""
+        sizes = (row_chunks, row_chunks, 2 * rows, 5 * entries, 2 * entry_chunks)
+        starts = [0]
+        for size in sizes:
+            starts.append(starts[-1] + (size + 1) // 2 * 2)   # (16-byte boundaries)
+        if self.held is None or self.held.numel() < starts[-1] or self.held.device != device:
+            self.held = torch.empty(starts[-1], dtype=torch.float64, device=device)
+        if self.counters is None or self.counters.numel() < entries or self.counters.device != device:
+            self.counters = torch.zeros(entries, dtype=torch.int32, device=device)
+        base = self.held.data_ptr()
+        return tuple(base + 8 * start for start in starts[:5])
 
 
 _verify_scratch = VerifyScratch()
@@ -310,47 +372,48 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     accepted int32 [n]: drafts kept; tokens int32 [n, most + 1]: kept drafts, the next token, then -1. An entry of no rows gets 0 and
     -1; one whose rows lie outside `target`, or with more drafts than `tokens` has room for, -1 and -1. A drafted id outside the
     vocabulary is refused. Logits are finite or -infinity. `scratch`: as in `sample`."""
-    _dev("target logits", target, torch.float32, contiguous=False)
+    f32, i32 = torch.float32, torch.int32
+    for name, t, dtype in (("target logits", target, f32), ("drafted", drafted, i32), ("first", first, i32), ("uniforms", uniforms, f32), ("accepted", accepted, i32),
+                           ("tokens", tokens, i32)):
+        if t.dtype is not dtype or not (t is target or t.is_contiguous()):
+            _dev(name, t, dtype, contiguous=t is not target)
     if target.dim() != 2 or target.stride(1) != 1 or target.shape[1] <= 0:
         raise KernelError("verify_drafts: logits must be 2-d with unit inner stride")
     rows, vocab = target.shape
-    n = accepted.numel()
-    for name, t, dtype in (("drafted", drafted, torch.int32), ("first", first, torch.int32), ("uniforms", uniforms, torch.float32),
-                           ("accepted", accepted, torch.int32), ("tokens", tokens, torch.int32)):
-        _dev(name, t, dtype)
+    n, total = accepted.numel(), drafted.numel()
     if first.numel() != n + 1 or tokens.dim() != 2 or tokens.shape[0] != n or tokens.shape[1] < 1:
         raise KernelError("verify_drafts: wants first [n + 1], accepted [n] and tokens [n, most drafts + 1]")
     if n == 0:
         return
-    total = drafted.numel()
     if total < rows - n:
         raise KernelError(f"verify_drafts: {rows} rows of {n} entries go with {rows - n} drafted tokens or more, not {total}")
     if max(n, rows + total) > 65535:
         raise KernelError(f"verify_drafts: {n} entries with {rows} rows and {total} drafts are more than a launch takes (65,535)")
-    sampling = temperature > 0
+    used, sampling = None, temperature > 0
     if sampling:
         if uniforms.numel() != total:
             raise KernelError("verify_drafts: uniforms must have one element per drafted token")
-        _dev("seq_ids", seq_ids, torch.int64)
-        _dev("steps", steps, torch.int32)
+        if seq_ids is None or steps is None:
+            raise KernelError("verify_drafts: sampling needs seq_ids and steps")
+        if seq_ids.dtype is not torch.int64 or steps.dtype is not i32 or not seq_ids.is_contiguous() or not steps.is_contiguous():
+            _dev("seq_ids", seq_ids, torch.int64)
+            _dev("steps", steps, i32)
         if seq_ids.numel() != n or steps.numel() != n:
             raise KernelError("verify_drafts: seq_ids and steps must have one element per entry")
+        _here("verify_drafts", target, seq_ids, steps)
         if draft is not None:
-            _dev("draft logits", draft, torch.float32, contiguous=False)
+            _dev("draft logits", draft, f32, contiguous=False)
             if draft.dim() != 2 or draft.shape != (total, vocab) or (total > 0 and draft.stride(1) != 1):
                 raise KernelError("verify_drafts: draft logits must have a row of the same vocabulary per drafted token")
-    used = draft if sampling and total > 0 else None
-    _here("verify_drafts", target, used, drafted, first, uniforms, accepted, tokens, *((seq_ids, steps) if sampling else ()))
-    lib = library("verify_drafts")
-    sizes = (_I * 2)()
-    lib.qf_verify_chunks(_I(vocab), sizes)
+            used = draft if total > 0 else None
+    _here("verify_drafts", target, used, drafted, first, uniforms, accepted, tokens)
     all_rows = rows + (total if used is not None else 0)
     scratch = scratch or _verify_scratch
-    scratch.ensure(max(all_rows, 1) * sizes[0], n * sizes[1], n, target.device)
-    code = lib.qf_verify_drafts(
-        _ptr(target), _I(rows), _I(vocab), _LL(target.stride(0)), _ptr(used), _LL(used.stride(0) if used is not None else 0), _ptr(drafted), _I(total),
-        _ptr(first), _I(n), _ptr(uniforms), _F(max(float(temperature), 0.0)), _ULL(int(seed) & 0xFFFFFFFFFFFFFFFF), _ptr(seq_ids if sampling else None),
-        _ptr(steps if sampling else None), _ptr(accepted), _ptr(tokens), _I(tokens.shape[1] - 1), _ptr(scratch.sums), _ptr(scratch.tops),
-        _ptr(scratch.best), _ptr(scratch.counters), _stream())
-    kernels.launches += 1   # (the rows' statistics, and the choice)
+    places = scratch.ensure(all_rows * -(-vocab // VERIFY_CHUNK), all_rows, n * -(-vocab // VERIFY_RACE_CHUNK), n, target.device)
+    code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P,
+                     _P)(
+        target.data_ptr(), rows, vocab, target.stride(0), _at(used), used.stride(0) if used is not None else 0, drafted.data_ptr(), total,
+        first.data_ptr(), n, uniforms.data_ptr(), max(float(temperature), 0.0), int(seed) & 0xFFFFFFFFFFFFFFFF, seq_ids.data_ptr() if sampling else None,
+        steps.data_ptr() if sampling else None, accepted.data_ptr(), tokens.data_ptr(), tokens.shape[1] - 1, *places, scratch.counters.data_ptr(), _stream())
+    kernels.launches += 2 if sampling else 1   # (the rows' statistics, the decision, the draw)
     _check(code, "verify_drafts")
