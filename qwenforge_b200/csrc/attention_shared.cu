@@ -8,8 +8,9 @@
 // fetched once for members x heads rows, instead of once for every member. The keys behind them are a sequence's own parts. A last kernel joins
 // each row's parts.
 //
-// Which block and warp take which run is worked out on the device from the lengths of the step (`shared_plan_kernel`), so that a captured step can
-// be replayed with other lengths; what is shared stands in arrays on the device:
+// Which block and warp takes which run is worked out on the device from the lengths of the step, so that a captured step can be replayed with other
+// lengths, and by every block for itself (`shared_plan`: a launch of its own for it took 5 of 11 microseconds of a small call); what is shared stands in
+// arrays on the device:
 //   entry_pages [n_seqs]  pages that the sequence shares with its group (0: none);   entry_group [n_seqs]  its group (-1: none)
 //   members     [n_seqs]  batch entries, group after group;   begin [n_groups + 1]  where each group starts there;   pages [n_groups]
 //
@@ -31,36 +32,89 @@ struct __align__(16) SharedRecord {
     int limit;     // keys below it are seen by every row (a sequence's own part: its length)
     int part;      // which of a row's parts this is
 };
+#define SH_TEAM 4            // warps of a block of the parts' kernel
+#define SH_MAX_SEQS 2048
 
-// The plan: four counts (units, tile records, 0, 0), then n_seqs ints (a row's shared parts | its own parts << 16) padded to four, then the units (a record
-// for each of a block's SH_TEAM warps) and the tile records.
-#define SH_TEAM 4
-__host__ __device__ constexpr long long shared_plan_records(int n_seqs) { return 4 + (n_seqs + 3) / 4 * 4; }   // (where they begin, in ints)
+// What every kernel gets.
+struct SharedArgs {
+    const int* tok_pos;
+    const int* slots;
+    const int* entry_pages;
+    const int* entry_group;
+    const int* members;
+    const int* begin;
+    const int* pages;
+    float* part_o;    // [n_seqs * n_heads][most_parts][D]
+    float* part_ml;   // [n_seqs * n_heads][most_parts][2]
+    int* part_n;      // [n_seqs] a row's shared parts | its own parts << 16
+    int* err;
+    int n_seqs, n_groups, n_heads, kv_heads, most_parts, most_shared, most_own;
+    int row_tile, warps, team, tile_rows, tile_pages, sms;   // (see shared_plan; tile_rows 0: no tiles)
+    float scale_log2;
+};
 
-// ---- the plan: one block. An item is a group's pages or a sequence's own, times its tiles of rows. With X pages x tiles x kv heads in all and `warps`
+// ---- the plan. An item is a group's pages or a sequence's own, times its tiles of `row_tile` rows. With X pages x tiles x kv heads in all and `warps`
 // warps at once, a warp gets t = max(1, X / warps) pages. Items of up to SH_TEAM t pages are cut into records of t pages for a warp each, every one a part
 // of its own; longer ones into runs of up to SH_TEAM t pages for a block, whose warps bring their sums together (SH_TOGETHER; not where a record is a
-// whole block's work, `together_warps` 1). A group of `tile_rows`
-// rows or more with `tile_pages` pages or more goes to the tensor-core tiles instead (attention_shared_tiles.cuh): pairs of tiles of 128 rows, cut into
-// runs of as many turns of two pages as make the records fill the SMs once.
-// What bounds it: the latency of a few dependent loads and of the block's barriers; every number is read once and kept in shared memory.
-#define SH_PLAN_THREADS 256
-#define SH_MAX_SEQS 2048
-__global__ void __launch_bounds__(SH_PLAN_THREADS)
-shared_plan_kernel(const int* __restrict__ tok_pos, const int* __restrict__ slots, int n_seqs, const int* __restrict__ entry_pages,
-                   const int* __restrict__ entry_group, const int* __restrict__ begin, const int* __restrict__ pages, int n_groups, int kv_heads,
-                   int group_heads, int row_tile, int warps, int together_warps, int most_shared, int most_own, int tile_rows, int tile_pages, int sms, int* __restrict__ plan,
-                   int most_units, int most_tiles) {
-    extern __shared__ int plan_s[];
-    __shared__ long long sums_s[SH_PLAN_THREADS / 32];
-    int* own_s = plan_s;                  // [n_seqs] pages of a sequence's own part
-    int* slot_s = own_s + n_seqs;         // [n_groups] a live member's slot (-1: all have ended)
-    int* least_s = slot_s + n_groups;     // [n_groups] the fewest keys that a live member sees
-    int* rows_s = least_s + n_groups;     // [n_groups]
-    int* pages_s = rows_s + n_groups;     // [n_groups]
-    int* first_s = pages_s + n_groups;    // [n_groups] the group's first record of its kind
-    int* runs_s = first_s + n_groups;     // [n_groups] its parts
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// whole block's work, `team` 1). A group of `tile_rows` rows or more with `tile_pages` pages or more goes to the tensor-core tiles instead
+// (attention_shared_tiles.cuh): pairs of tiles of 128 rows, cut into runs of as many turns of two pages as make the records fill their share of the SMs
+// once; the other SMs' warps take the records of everything else meanwhile.
+// What bounds it: the latency of one round of loads and of a dozen barriers.
+struct SharedPlan {
+    int* own;        // [n_seqs] pages of a sequence's own part
+    int* own_first;  // [n_seqs] its first record of its kind
+    int* slot;       // [n_groups] a live member's slot (-1: all have ended)
+    int* least;      // [n_groups] the fewest keys that a live member sees
+    int* rows;       // [n_groups]
+    int* pages;      // [n_groups]
+    int* first;      // [n_groups] the group's first record of its kind
+    int* parts;      // [n_groups]
+    int own_tiles, each, together, stretch;   // (together: items of more pages are blocks' runs)
+    int blocks, singles, tiles;               // records of each kind
+};
+__host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 6 * n_groups; }
+// What an SM takes for a turn of a pair of tiles, and, with ten warps at work, for a page of 16 rows and for what a record costs besides, in microseconds
+// as measured.
+__device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.85f : 2.05f; }
+__device__ __forceinline__ float shared_page_time(int d) { return d <= 64 ? 0.2f : 0.4f; }
+#define SH_RECORD_TIME 0.35f
+
+// Parts of an item of n_pages: of up to `unit` pages, no more than there is room for (longer ones then), none without a page; run: the pages of each.
+__device__ __forceinline__ int shared_cut(int n_pages, int unit, int most, int& run) {
+    run = 0;
+    if (n_pages <= 0) return 0;
+    const int n = min((n_pages + unit - 1) / unit, most);
+    run = (n_pages + n - 1) / n;
+    return (n_pages + run - 1) / run;
+}
+__device__ __forceinline__ bool shared_tiled(const SharedArgs& a, const SharedPlan& p, int g) {
+    return a.tile_rows > 0 && p.rows[g] >= a.tile_rows && p.pages[g] >= a.tile_pages;
+}
+__device__ __forceinline__ int shared_tiles_of(const SharedArgs& a, const SharedPlan& p, int g) {
+    return shared_tiled(a, p, g) ? (p.rows[g] + 255) / 256 : (p.rows[g] + a.row_tile - 1) / a.row_tile;
+}
+__device__ __forceinline__ int shared_cut_group(const SharedArgs& a, const SharedPlan& p, int g, int& run) {
+    run = 0;
+    if (p.slot[g] < 0) return 0;
+    if (!shared_tiled(a, p, g)) return shared_cut(p.pages[g], p.pages[g] > p.together ? p.together : p.each, a.most_shared, run);
+    const int n = shared_cut((p.pages[g] + 1) / 2, p.stretch, a.most_shared, run);
+    run *= 2;
+    return n;
+}
+__device__ __forceinline__ int shared_cut_own(const SharedArgs& a, const SharedPlan& p, int s, int& run) {
+    return shared_cut(p.own[s], p.own[s] > p.together ? p.together : p.each, a.most_own, run);
+}
+
+// By all threads of a block; `room`: shared_plan_ints of shared memory.
+template <int THREADS>
+__device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room, int head_dim) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ long long sums_s[WARPS];
+    SharedPlan p;
+    p.own = room, p.own_first = p.own + a.n_seqs;
+    p.slot = p.own_first + a.n_seqs, p.least = p.slot + a.n_groups, p.rows = p.least + a.n_groups, p.pages = p.rows + a.n_groups;
+    p.first = p.pages + a.n_groups, p.parts = p.first + a.n_groups;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group_heads = a.n_heads / a.kv_heads;
     auto block_total = [&](long long v) -> long long {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -69,61 +123,85 @@ shared_plan_kernel(const int* __restrict__ tok_pos, const int* __restrict__ slot
         __syncthreads();
         long long t = 0;
 #pragma unroll
-        for (int w = 0; w < SH_PLAN_THREADS / 32; ++w) t += sums_s[w];
+        for (int w = 0; w < WARPS; ++w) t += sums_s[w];
         return t;
     };
-    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS) slot_s[g] = -1, least_s[g] = 0x7fffffff;
-    __syncthreads();
-    grid_dependency_wait();
-    const int own_tiles = (group_heads + row_tile - 1) / row_tile;
-    auto tiled = [&](int g) -> bool { return rows_s[g] >= tile_rows && pages_s[g] >= tile_pages; };
-    auto group_tiles = [&](int g) -> int { return tiled(g) ? (rows_s[g] + 255) / 256 : (rows_s[g] + row_tile - 1) / row_tile; };
+    p.own_tiles = (group_heads + a.row_tile - 1) / a.row_tile;
     long long sum = 0;   // pages x tiles of this thread's items, and (32 bits up) turns of pairs of tiles
-    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS) rows_s[g] = (begin[g + 1] - begin[g]) * group_heads, pages_s[g] = pages[g];
-    for (int s = tid; s < n_seqs; s += SH_PLAN_THREADS) {
-        const int slot = slots[s], pos = tok_pos[s], g = entry_group[s], n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - entry_pages[s]);
-        own_s[s] = n;
-        sum += n * own_tiles;
-        if (slot >= 0 && g >= 0) {
-            atomicMax(slot_s + g, slot);
-            atomicMin(least_s + g, pos + 1);
+    // (everything is asked for before the first barrier: one round trip)
+    int slot = -1, pos = 0, group = -1, shared = 0, rows = 0, pages = 0;
+    if (tid < a.n_seqs) slot = a.slots[tid], pos = a.tok_pos[tid], group = a.entry_group[tid], shared = a.entry_pages[tid];
+    if (tid < a.n_groups) rows = (a.begin[tid + 1] - a.begin[tid]) * group_heads, pages = a.pages[tid];
+    for (int g = tid; g < a.n_groups; g += THREADS) {
+        if (g != tid) rows = (a.begin[g + 1] - a.begin[g]) * group_heads, pages = a.pages[g];
+        p.slot[g] = -1, p.least[g] = 0x7fffffff, p.rows[g] = rows, p.pages[g] = pages;
+    }
+    if (a.n_groups > 0) __syncthreads();
+    for (int s = tid; s < a.n_seqs; s += THREADS) {
+        if (s != tid) slot = a.slots[s], pos = a.tok_pos[s], group = a.entry_group[s], shared = a.entry_pages[s];
+        const int n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - shared);
+        p.own[s] = n;
+        sum += n * p.own_tiles;
+        if (slot >= 0 && group >= 0) {
+            atomicMax(p.slot + group, slot);
+            atomicMin(p.least + group, pos + 1);
         }
     }
-    __syncthreads();
-    for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
-        if (slot_s[g] >= 0) sum += tiled(g) ? (long long)((pages_s[g] + 1) / 2 * group_tiles(g)) << 32 : (long long)(pages_s[g] * group_tiles(g));
+    if (a.n_groups > 0) __syncthreads();
+    for (int g = tid; g < a.n_groups; g += THREADS)
+        if (p.slot[g] >= 0)
+            sum += shared_tiled(a, p, g) ? (long long)((p.pages[g] + 1) / 2 * shared_tiles_of(a, p, g)) << 32 : (long long)(p.pages[g] * shared_tiles_of(a, p, g));
     sum = block_total(sum);
-    const int each = (int)max(1ll, ((sum & 0xffffffff) * kv_heads + warps - 1) / warps), team = together_warps > 1 ? (int)min((long long)each * SH_TEAM, 0x3fffffffll) : 0x3fffffff;
-    int stretch = 2;   // turns of a tile record
-    if (most_tiles > 0) {
-        stretch = (int)max(2ll, ((sum >> 32) * kv_heads + sms - 1) / sms);
-        for (int round = 0; round < 16; ++round) {   // (cutting into whole turns may give more records than SMs)
-            long long records = 0;
-            for (int g = tid; g < n_groups; g += SH_PLAN_THREADS)
-                if (slot_s[g] >= 0 && tiled(g)) records += ((pages_s[g] + 1) / 2 + stretch - 1) / stretch * group_tiles(g);
-            records = block_total(records) * kv_heads;
-            if (records <= sms) break;
-            stretch = round == 14 ? 0x3fffffff : (int)max((long long)stretch + 1, stretch * records / sms);
+    const unsigned work = (unsigned)sum * (unsigned)a.kv_heads;
+    int warps = a.warps;
+    p.stretch = 2;   // turns of a tile record
+    if (a.tile_rows > 0) {
+        const int turns = (int)(sum >> 32) * a.kv_heads;
+        const float tile_time = (float)turns * shared_turn_time(head_dim);
+        const float page_time = (float)work * shared_page_time(head_dim) + (float)min(a.n_seqs * p.own_tiles * a.kv_heads, (int)work) * SH_RECORD_TIME;
+        const int share = work == 0 ? a.sms : min(max((int)((float)a.sms * tile_time / (tile_time + page_time)), 1), a.sms - 1);
+        int records = 0;
+        if (turns > 0) {
+            p.stretch = max(2, (turns + share - 1) / share);
+            for (int round = 0; round < 16; ++round) {   // (cutting into whole turns may give more records than SMs)
+                long long mine = 0;
+                for (int g = tid; g < a.n_groups; g += THREADS)
+                    if (p.slot[g] >= 0 && shared_tiled(a, p, g)) mine += ((p.pages[g] + 1) / 2 + p.stretch - 1) / p.stretch * shared_tiles_of(a, p, g);
+                records = (int)block_total(mine) * a.kv_heads;
+                if (records <= share) break;
+                p.stretch = round == 14 ? 0x3fffffff : (int)max((long long)p.stretch + 1, (long long)p.stretch * records / share);
+            }
         }
+        warps = max((int)gridDim.x - records, 1) * WARPS;
     }
-    // parts of an item: no more than there is room for (longer runs then), none without a page; and the pages of each
-    auto cut = [&](int n_pages, int unit, int most, int& run) -> int {
-        if (n_pages <= 0) return 0;
-        const int n = min((n_pages + unit - 1) / unit, most);
-        run = (n_pages + n - 1) / n;
-        return (n_pages + run - 1) / run;
-    };
-    auto cut_group = [&](int g, int& run) -> int {
-        if (slot_s[g] < 0) return 0;
-        if (!tiled(g)) return cut(pages_s[g], pages_s[g] > team ? team : each, most_shared, run);
-        const int n = cut((pages_s[g] + 1) / 2, stretch, most_shared, run);
-        run *= 2;
-        return n;
-    };
+    p.each = (int)max(1u, (work + warps - 1) / warps);
+    p.together = a.team > 1 ? p.each * SH_TEAM : 0x3fffffff;
+    for (int round = 0; a.tile_rows > 0 && round < 8; ++round) {   // a few records more than warps would take twice the time
+        long long mine = 0;
+        int run;
+        for (int s = tid; s < a.n_seqs; s += THREADS) mine += shared_cut_own(a, p, s, run) * p.own_tiles;
+        for (int g = tid; g < a.n_groups; g += THREADS)
+            if (!shared_tiled(a, p, g)) mine += shared_cut_group(a, p, g, run) * shared_tiles_of(a, p, g);
+        const long long records = block_total(mine) * a.kv_heads;
+        if (records <= warps || records > 3ll * warps) break;
+        ++p.each;
+    }
     // Where every item's records begin: a prefix sum of three counts at once, 21 bits each: runs for a block, tile records, records for a warp.
     constexpr int BLOCKS = 42, TILES = 21, BITS = (1 << 21) - 1;
     long long before = 0;
-    auto place = [&](long long mine) -> long long {
+    for (int i0 = 0; i0 < a.n_groups + a.n_seqs; i0 += THREADS) {
+        const int i = i0 + tid, s = i - a.n_groups;
+        int parts = 0, run, shift = 0;
+        long long mine = 0;
+        if (s < 0) {
+            parts = shared_cut_group(a, p, i, run);
+            shift = shared_tiled(a, p, i) ? TILES : p.pages[i] > p.together ? BLOCKS : 0;
+            mine = (long long)(parts * shared_tiles_of(a, p, i)) << shift;
+        } else if (s < a.n_seqs) {
+            parts = shared_cut_own(a, p, s, run);
+            shift = p.own[s] > p.together ? BLOCKS : 0;
+            mine = (long long)(parts * p.own_tiles) << shift;
+        }
         long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -133,101 +211,66 @@ shared_plan_kernel(const int* __restrict__ tok_pos, const int* __restrict__ slot
         __syncthreads();
         if (lane == 31) sums_s[warp] = upto;
         __syncthreads();
-        long long first = before + upto - mine;
+        long long at = before + upto - mine;
 #pragma unroll
-        for (int w = 0; w < SH_PLAN_THREADS / 32; ++w) {
-            if (w < warp) first += sums_s[w];
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) at += sums_s[w];
             before += sums_s[w];
         }
-        return first;
-    };
-    for (int g0 = 0; g0 < n_groups; g0 += SH_PLAN_THREADS) {
-        const int g = g0 + tid;
-        int run = 0, parts = 0, shift = 0;
-        if (g < n_groups) {
-            parts = cut_group(g, run);
-            shift = tiled(g) ? TILES : pages_s[g] > team ? BLOCKS : 0;
-        }
-        const long long first = place(g < n_groups ? (long long)(parts * group_tiles(g)) << shift : 0);
-        if (g < n_groups) runs_s[g] = parts, first_s[g] = (int)(first >> shift) & BITS;
+        if (s < 0) p.first[i] = (int)(at >> shift) & BITS, p.parts[i] = parts;
+        else if (s < a.n_seqs) p.own_first[s] = (int)(at >> shift) & BITS;
     }
-    // The sequences' own counts are needed before any warp record can be placed (they lie behind the block's): first the counts, then the records.
-    const long long groups_end = before;
-    for (int s0 = 0; s0 < n_seqs; s0 += SH_PLAN_THREADS) {
-        const int s = s0 + tid;
-        int run = 0;
-        const int n = s < n_seqs ? own_s[s] : 0;
-        const long long parts = cut(n, n > team ? team : each, most_own, run) * own_tiles;
-        place(parts << (n > team ? BLOCKS : 0));
-    }
-    const int blocks = (int)(before >> BLOCKS) & BITS, singles = (int)before & BITS, units = blocks + (singles + SH_TEAM - 1) / SH_TEAM;
-    SharedRecord* const records = reinterpret_cast<SharedRecord*>(plan + shared_plan_records(n_seqs));
-    SharedRecord* const tiles = records + (size_t)most_units * SH_TEAM;
-    if (tid == 0) {
-        plan[0] = min(units, most_units);
-        plan[1] = min((int)(before >> TILES) & BITS, most_tiles);
-    }
-    // a run for a block: its warps' shares of the pages; a record for a warp: its place behind all blocks'
-    auto write = [&](bool together, int index, SharedRecord r) {
-        if (!together) {
-            const int at = blocks * SH_TEAM + index;
-            if (at < most_units * SH_TEAM) records[at] = r;
-            return;
-        }
-        if (index >= most_units) return;
-        const int from = r.p_begin, to = r.p_end, per = (to - from + SH_TEAM - 1) / SH_TEAM;
-        r.kind |= SH_TOGETHER;
+    p.blocks = (int)(before >> BLOCKS) & BITS, p.tiles = (int)(before >> TILES) & BITS, p.singles = (int)before & BITS;
+    __syncthreads();
+    return p;
+}
+
+// Records [index, index + N) of a kind (SH_TOGETHER: blocks' runs; SH_NONE, for want of another name: tile records; 0: warps' records) into to[N]; by
+// THREADS threads, this one the `tid`-th, which then synchronise. Records that there are none of are left as they were.
+template <int THREADS, int N>
+__device__ __forceinline__ void shared_records(const SharedArgs& a, const SharedPlan& p, int tid, int kind, int index, SharedRecord* to) {
+    for (int g = tid; g < a.n_groups; g += THREADS) {
+        const int mine = shared_tiled(a, p, g) ? SH_NONE : p.pages[g] > p.together ? SH_TOGETHER : 0, n = p.parts[g] * shared_tiles_of(a, p, g), first = p.first[g];
+        if (mine != kind || first >= index + N || first + n <= index) continue;
+        int run;
+        shared_cut_group(a, p, g, run);
 #pragma unroll
-        for (int w = 0; w < SH_TEAM; ++w) {
-            r.p_begin = min(from + w * per, to);
-            r.p_end = min(from + (w + 1) * per, to);
-            records[index * SH_TEAM + w] = r;
-        }
-    };
-    if (tid < SH_TEAM && singles % SH_TEAM && tid >= singles % SH_TEAM)   // the last unit's warps without a record
-        write(false, singles / SH_TEAM * SH_TEAM + tid, SharedRecord{SH_NONE, 0, 0, 0, 0, 0, 0, 0});
-    for (int g = 0; g < n_groups; ++g) {   // the whole block at a group's records
-        int run = 0;
-        const int parts = cut_group(g, run), n = parts * group_tiles(g), limit = min(least_s[g], pages_s[g] * QF_PAGE);
-        const bool tile = tiled(g), together = !tile && pages_s[g] > team;
-        for (int k = tid; k < n; k += SH_PLAN_THREADS) {
-            const int part = k % parts;
-            const SharedRecord r = {SH_PREFIX, g, k / parts, slot_s[g], part * run, min((part + 1) * run, pages_s[g]), limit, part};
-            if (!tile) write(together, first_s[g] + k, r);
-            else if (first_s[g] + k < most_tiles) tiles[first_s[g] + k] = r;
+        for (int w = 0; w < N; ++w) {
+            const int k = index + w - first;
+            if (k < 0 || k >= n) continue;
+            const int part = k % p.parts[g];
+            to[w] = SharedRecord{SH_PREFIX | (kind & SH_TOGETHER), g, k / p.parts[g], p.slot[g], part * run, min((part + 1) * run, p.pages[g]),
+                                 min(p.least[g], p.pages[g] * QF_PAGE), part};
         }
     }
-    before = groups_end;
-    for (int s0 = 0; s0 < n_seqs; s0 += SH_PLAN_THREADS) {
-        const int s = s0 + tid;
-        int run = 0;
-        const int n = s < n_seqs ? own_s[s] : 0, parts = cut(n, n > team ? team : each, most_own, run);
-        const bool together = n > team;
-        const long long first = place((long long)(parts * own_tiles) << (together ? BLOCKS : 0));
-        if (s >= n_seqs) continue;
-        const int g = entry_group[s], slot = slots[s], shared = g >= 0 && slot >= 0 ? runs_s[g] : 0, from = entry_pages[s];
-        plan[4 + s] = shared | parts << 16;
-        const int index = (int)(first >> (together ? BLOCKS : 0)) & BITS;
-        for (int k = 0; k < parts * own_tiles; ++k) {
+    if (kind == SH_NONE) return;
+    for (int s = tid; s < a.n_seqs; s += THREADS) {
+        const int mine = p.own[s] > p.together ? SH_TOGETHER : 0, first = p.own_first[s];
+        if (mine != kind || first >= index + N) continue;
+        int run;
+        const int parts = shared_cut_own(a, p, s, run), n = parts * p.own_tiles;
+        if (first + n <= index) continue;
+        const int from = a.entry_pages[s], g = a.entry_group[s], shared = g >= 0 ? p.parts[g] : 0, length = a.tok_pos[s] + 1;
+        const int slot = a.slots[s];
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            const int k = index + w - first;
+            if (k < 0 || k >= n) continue;
             const int part = k % parts;
-            write(together, index + k, SharedRecord{SH_OWN, s, k / parts, slot, from + part * run, from + min((part + 1) * run, n), tok_pos[s] + 1, shared + part});
+            to[w] = SharedRecord{SH_OWN | kind, s, k / parts, slot, from + part * run, from + min((part + 1) * run, p.own[s]), length, shared + part};
         }
     }
 }
 
-// ---- what every kernel of the parts needs
-struct SharedArgs {
-    const int* tok_pos;
-    const int* slots;
-    const int* members;
-    const int* begin;
-    const int* plan;
-    float* part_o;    // [n_seqs * n_heads][most_parts][D]
-    float* part_ml;   // [n_seqs * n_heads][most_parts][2]
-    int* err;
-    int n_seqs, n_heads, most_parts, most_units;
-    float scale_log2;
-};
+// How many parts every row has, for whoever joins them: by the first block of the parts' kernel.
+template <int THREADS>
+__device__ __forceinline__ void shared_count_parts(const SharedArgs& a, const SharedPlan& p) {
+    for (int s = threadIdx.x; s < a.n_seqs; s += THREADS) {
+        int run;
+        const int g = a.entry_group[s], slot = a.slots[s];
+        a.part_n[s] = slot < 0 ? 0 : (g >= 0 ? p.parts[g] : 0) | shared_cut_own(a, p, s, run) << 16;
+    }
+}
 
 // Row `at` of a record's subject: its place in q ([n_seqs * n_heads] rows of D), or -1 where there is no such row. (The rows of a member that has ended
 // have a place too: nobody reads what is left there.)
@@ -255,209 +298,249 @@ __device__ __forceinline__ uint4 load_shared_16(const uint4* p) {
 // cut alike), and of the values of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 the columns E g .. E g + E - 1, E = D / 8, which make the n-tiles' column g. No shared
 // memory, no barrier: all of a step's keys and values are on their way at once, the next step's as soon as the registers are free again.
 // What bounds it: the latency of memory while a run is short (a page at head size 64 is one step), then the rate at which pages arrive.
-__host__ __device__ constexpr int shared_keys(int d) { return d <= 64 ? 64 : 32; }
+template <int D> struct SharedSums {
+    float o[D / 8][4];       // o[t][0], o[t][1]: row g's columns 2 j E + t and (2 j + 1) E + t; o[t][2], o[t][3]: row g + 8's
+    float m0, m1, l0, l1;    // rows g and g + 8: maximum and sum of weights
+    int place0, place1;      // where they lie in q
+    // 2 E columns of either row side by side
+    __device__ __forceinline__ void leave(float* row0, float* row1, float f0, float f1) const {
+        constexpr int E = D / 8;
+        const int j = threadIdx.x & 3;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < E; t += 4) {
+                const int c = (2 * j + h) * E + t;
+                if (row0) *reinterpret_cast<float4*>(row0 + c) = make_float4(o[t][h] * f0, o[t + 1][h] * f0, o[t + 2][h] * f0, o[t + 3][h] * f0);
+                if (row1) *reinterpret_cast<float4*>(row1 + c) = make_float4(o[t][2 + h] * f1, o[t + 1][2 + h] * f1, o[t + 2][2 + h] * f1, o[t + 3][2 + h] * f1);
+            }
+    }
+    // as a part of its own
+    __device__ __forceinline__ void leave_part(const SharedArgs& a, int part) const {
+        const size_t at0 = (size_t)place0 * a.most_parts + part, at1 = (size_t)place1 * a.most_parts + part;
+        leave(place0 < 0 ? nullptr : a.part_o + at0 * D, place1 < 0 ? nullptr : a.part_o + at1 * D, 1.f, 1.f);
+        if ((threadIdx.x & 3) == 0 && place0 >= 0) *reinterpret_cast<float2*>(a.part_ml + at0 * 2) = make_float2(m0, l0);
+        if ((threadIdx.x & 3) == 0 && place1 >= 0) *reinterpret_cast<float2*>(a.part_ml + at1 * 2) = make_float2(m1, l1);
+    }
+};
+// Bytes of shared memory that a warp needs for its queries: none where they are held in registers.
+__host__ __device__ constexpr int shared_query_bytes(int d) { return d <= 64 ? 0 : 16 * d * 2; }
 
+template <int D, int KEYS>
+__device__ __forceinline__ void shared_warp(const bf16* __restrict__ q, const KvSite<bf16>& site, const SharedArgs& a, const SharedRecord& rec, int kvh,
+                                            uint4* query_room, SharedSums<D>& out) {
+    constexpr int SIX = KEYS / 16, STEPS = QF_PAGE / KEYS, KU = D / 32, E = D / 8, NT = E;
+    const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
+    const bool prefix = rec.kind & SH_PREFIX;
+    const int p0 = rec.p_begin, p1 = rec.p_end, steps = STEPS * (p1 - p0);
+    const int bound = prefix ? p1 * QF_PAGE : rec.limit;   // no row sees a key from here on
+    const int* table_row = site.table + (long long)rec.slot * site.table_stride;
+    int table = 0;   // a lane each the numbers of 32 pages
+    uint4 k[2 * SIX][KU];          // n-tile t: key 8 t + g
+    uint32_t v[4 * SIX][E / 2];    // of every 16 keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9
+    const bf16* k_at = nullptr;    // the step's keys (null: nothing to see there)
+    auto find = [&](int i) {
+        k_at = nullptr;
+        if (i >= steps) return;
+        const int n = i / STEPS, part = i % STEPS;
+        if (n % 32 == 0 && part == 0) table = p0 + n + lane < p1 ? __ldg(table_row + p0 + n + lane) : 0;
+        const int page = __shfl_sync(0xffffffffu, table, n & 31);
+        if (page < 0) {
+            if (lane == 0 && part == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+            return;
+        }
+        if ((p0 + n) * QF_PAGE + KEYS * part >= bound) return;
+        k_at = site.base + (long long)page * site.page_elems + ((long long)kvh * QF_PAGE + KEYS * part) * D;
+    };
+    auto load_keys = [&]() {
+#pragma unroll
+        for (int t = 0; t < 2 * SIX; ++t)
+#pragma unroll
+            for (int u = 0; u < KU; ++u) k[t][u] = __ldg(reinterpret_cast<const uint4*>(k_at + (8 * t + g) * D + 32 * u + 8 * j));
+    };
+    auto load_values = [&](const bf16* v_at) {
+#pragma unroll
+        for (int r = 0; r < 4 * SIX; ++r) {
+            const bf16* row = v_at + (r / 4 * 16 + 2 * j + (r & 1) + 8 * (r >> 1 & 1)) * D + E * g;
+            if constexpr (E % 8 == 0) {
+#pragma unroll
+                for (int u = 0; u < E / 8; ++u) {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + 8 * u));
+                    v[r][4 * u] = x.x, v[r][4 * u + 1] = x.y, v[r][4 * u + 2] = x.z, v[r][4 * u + 3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < E / 4; ++u) {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + 4 * u));
+                    v[r][2 * u] = x.x, v[r][2 * u + 1] = x.y;
+                }
+            }
+        }
+    };
+    const long long to_values = (long long)kv_heads * QF_PAGE * D;
+    find(0);
+    if (k_at) {
+        load_keys();
+        load_values(k_at + to_values);
+    }
+    const int place0 = out.place0 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g);
+    const int place1 = out.place1 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g + 8);
+    // the queries' fragments: in registers, or, beyond head size 64, where keys, values and sums fill those, a lane's own 16 bytes at a time out of
+    // shared memory
+    constexpr bool HELD = shared_query_bytes(D) == 0;
+    uint4 q_held[HELD ? KU : 1][2];
+    uint4* const q_s = query_room + lane;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int place = r ? place1 : place0;
+            const uint4 x = place < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(q + (size_t)place * D + 32 * u + 8 * j);
+            if (HELD) q_held[HELD ? u : 0][r] = x;
+            else q_s[(2 * u + r) * 32] = x;
+        }
+    asm volatile("" ::: "memory");   // (the stores stand before the reads below, which the compiler does not see as reads of this)
+    float(&o)[NT][4] = out.o;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    float m0 = QF_NEG_BIG, m1 = QF_NEG_BIG, l0 = 0.f, l1 = 0.f;   // (the sums are this lane's share)
+    for (int i = 0; i < steps; ++i) {
+        const bool live = k_at != nullptr;
+        const int key0 = (p0 + i / STEPS) * QF_PAGE + KEYS * (i % STEPS);
+        float s[2 * SIX][4];
+        if (live) {
+#pragma unroll
+            for (int t = 0; t < 2 * SIX; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                const uint4 x = HELD ? q_held[HELD ? u : 0][0] : load_shared_16(q_s + 2 * u * 32), y = HELD ? q_held[HELD ? u : 0][1] : load_shared_16(q_s + (2 * u + 1) * 32);
+                const uint32_t lo[4] = {x.x, y.x, x.y, y.y}, hi[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+                for (int t = 0; t < 2 * SIX; ++t) {
+                    mma_bf16_16816(s[t], lo, k[t][u].x, k[t][u].y);
+                    mma_bf16_16816(s[t], hi, k[t][u].z, k[t][u].w);
+                }
+            }
+        }
+        find(i + 1);
+        if (k_at) load_keys();   // (on their way while the softmax and the second product run)
+        if (live) {
+            float top0 = QF_NEG_BIG, top1 = QF_NEG_BIG;
+            if (key0 + KEYS > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
+                const int see0 = prefix ? min(bound, shared_seen(a, place0)) : bound, see1 = prefix ? min(bound, shared_seen(a, place1)) : bound;
+#pragma unroll
+                for (int t = 0; t < 2 * SIX; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] = key0 + 8 * t + 2 * j + (e & 1) < (e >> 1 ? see1 : see0) ? s[t][e] * a.scale_log2 : QF_NEG_BIG;
+#pragma unroll
+                for (int r = 0; r < 4 * SIX; ++r)
+                    if (key0 + r / 4 * 16 + 2 * j + (r & 1) + 8 * (r >> 1 & 1) >= bound)
+#pragma unroll
+                        for (int u = 0; u < E / 2; ++u) v[r][u] = 0u;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2 * SIX; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] *= a.scale_log2;
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * SIX; ++t) top0 = fmaxf(top0, fmaxf(s[t][0], s[t][1])), top1 = fmaxf(top1, fmaxf(s[t][2], s[t][3]));
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+            if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1)) {
+                const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1), c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
+                m0 = n0, m1 = n1;
+                l0 *= c0, l1 *= c1;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t][0] *= c0, o[t][1] *= c0, o[t][2] *= c1, o[t][3] *= c1;
+            }
+            const float from0 = m0 <= QF_NEG_BIG ? 0.f : m0, from1 = m1 <= QF_NEG_BIG ? 0.f : m1;   // (no key seen yet: weights of 2^(-huge) = 0)
+#pragma unroll
+            for (int x = 0; x < SIX; ++x) {   // 16 keys at a time
+#pragma unroll
+                for (int t = 2 * x; t < 2 * x + 2; ++t) {
+                    s[t][0] = fast_exp2(s[t][0] - from0), s[t][1] = fast_exp2(s[t][1] - from0);
+                    s[t][2] = fast_exp2(s[t][2] - from1), s[t][3] = fast_exp2(s[t][3] - from1);
+                    l0 += s[t][0] + s[t][1];
+                    l1 += s[t][2] + s[t][3];
+                }
+                const uint32_t p[4] = {pack_bf16(s[2 * x][0], s[2 * x][1]), pack_bf16(s[2 * x][2], s[2 * x][3]),
+                                       pack_bf16(s[2 * x + 1][0], s[2 * x + 1][1]), pack_bf16(s[2 * x + 1][2], s[2 * x + 1][3])};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t pick = t & 1 ? 0x7632u : 0x5410u;
+                    mma_bf16_16816(o[t], p, __byte_perm(v[4 * x][t / 2], v[4 * x + 1][t / 2], pick), __byte_perm(v[4 * x + 2][t / 2], v[4 * x + 3][t / 2], pick));
+                }
+            }
+        }
+        if (k_at) load_values(k_at + to_values);
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    out.m0 = m0, out.m1 = m1, out.l0 = l0, out.l1 = l1;
+}
+
+// Batches without tiles: blocks of SH_TEAM warps, two an SM.
 template <int D>
 __global__ void __launch_bounds__(32 * SH_TEAM, 2)
 shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a) {
-    constexpr int KEYS = shared_keys(D), SIX = KEYS / 16, STEPS = QF_PAGE / KEYS, KU = D / 32, E = D / 8, NT = E, LO = D + 4;
+    constexpr int KEYS = D <= 64 ? 64 : 32, LO = D + 4, THREADS = 32 * SH_TEAM;
     __shared__ __align__(16) float merge_s[SH_TEAM][16][LO];
     __shared__ float m_s[SH_TEAM][16], l_s[SH_TEAM][16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    __shared__ SharedRecord record_s[SH_TEAM];
+    extern __shared__ int plan_s[];
+    static_assert(shared_query_bytes(D) <= (int)sizeof(merge_s[0]), "the queries lie where the sums will");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
     grid_launch_dependents();
     grid_dependency_wait();
-    const int kv_heads = site.kv_heads, units = a.plan[0] * kv_heads;
-    const SharedRecord* records = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs));
+    const SharedPlan plan = shared_plan<THREADS>(a, plan_s, D);
+    if (blockIdx.x == 0) shared_count_parts<THREADS>(a, plan);
+    const int units = (plan.blocks + (plan.singles + SH_TEAM - 1) / SH_TEAM) * kv_heads;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const int kvh = unit % kv_heads;
-        const SharedRecord rec = records[unit / kv_heads * SH_TEAM + warp];
-        if (rec.kind & SH_NONE) break;   // (the last warps of the last unit)
-        const bool prefix = rec.kind & SH_PREFIX;
-        const int p0 = rec.p_begin, p1 = rec.p_end, steps = STEPS * (p1 - p0);
-        const int bound = prefix ? p1 * QF_PAGE : rec.limit;   // no row sees a key from here on
-        const int* table_row = site.table + (long long)rec.slot * site.table_stride;
-        int table = 0;   // a lane each the numbers of 32 pages
-        uint4 k[2 * SIX][KU];          // n-tile t: key 8 t + g
-        uint32_t v[4 * SIX][E / 2];    // of every 16 keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9
-        const bf16* k_at = nullptr;    // the step's keys (null: nothing to see there)
-        auto find = [&](int i) {
-            k_at = nullptr;
-            if (i >= steps) return;
-            const int n = i / STEPS, half = i % STEPS;
-            if (n % 32 == 0 && half == 0) table = p0 + n + lane < p1 ? __ldg(table_row + p0 + n + lane) : 0;
-            const int page = __shfl_sync(0xffffffffu, table, n & 31);
-            if (page < 0) {
-                if (lane == 0 && half == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-                return;
-            }
-            if ((p0 + n) * QF_PAGE + KEYS * half >= bound) return;
-            k_at = site.base + (long long)page * site.page_elems + ((long long)kvh * QF_PAGE + KEYS * half) * D;
-        };
-        auto load_keys = [&]() {
-#pragma unroll
-            for (int t = 0; t < 2 * SIX; ++t)
-#pragma unroll
-                for (int u = 0; u < KU; ++u) k[t][u] = __ldg(reinterpret_cast<const uint4*>(k_at + (8 * t + g) * D + 32 * u + 8 * j));
-        };
-        auto load_values = [&](const bf16* v_at) {
-#pragma unroll
-            for (int r = 0; r < 4 * SIX; ++r) {
-                const bf16* row = v_at + (r / 4 * 16 + 2 * j + (r & 1) + 8 * (r >> 1 & 1)) * D + E * g;
-                if constexpr (E % 8 == 0) {
-#pragma unroll
-                    for (int u = 0; u < E / 8; ++u) {
-                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + 8 * u));
-                        v[r][4 * u] = x.x, v[r][4 * u + 1] = x.y, v[r][4 * u + 2] = x.z, v[r][4 * u + 3] = x.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < E / 4; ++u) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + 4 * u));
-                        v[r][2 * u] = x.x, v[r][2 * u + 1] = x.y;
-                    }
-                }
-            }
-        };
-        const long long to_values = (long long)kv_heads * QF_PAGE * D;
-        find(0);
-        if (k_at) {
-            load_keys();
-            load_values(k_at + to_values);
+        const int kvh = unit % kv_heads, index = unit / kv_heads;
+        const bool whole = index < plan.blocks;   // a block's run, or a record for each of its warps
+        if (threadIdx.x < SH_TEAM) record_s[threadIdx.x].kind = SH_NONE;
+        __syncthreads();
+        if (whole) shared_records<THREADS, 1>(a, plan, threadIdx.x, SH_TOGETHER, index, record_s);
+        else shared_records<THREADS, SH_TEAM>(a, plan, threadIdx.x, 0, (index - plan.blocks) * SH_TEAM, record_s);
+        __syncthreads();
+        SharedRecord rec = record_s[whole ? 0 : warp];
+        __syncthreads();   // (the next unit writes these again)
+        if (rec.kind & SH_NONE) continue;   // (the last warps of the last unit)
+        if (whole) {   // this warp's share of the pages
+            const int from = rec.p_begin, to = rec.p_end, per = (to - from + SH_TEAM - 1) / SH_TEAM;
+            rec.p_begin = min(from + warp * per, to);
+            rec.p_end = min(rec.p_begin + per, to);
         }
-        const int place0 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g), place1 = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + g + 8);
-        // the queries' fragments: in registers, or, beyond head size 64, where keys, values and sums fill those, a lane's own 16 bytes at a time out of
-        // shared memory (the room that the warp's sums take at the end)
-        constexpr bool HELD = D <= 64;
-        uint4 q_held[HELD ? KU : 1][2];
-        uint4* const q_s = reinterpret_cast<uint4*>(&merge_s[warp][0][0]) + lane;
-#pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int place = r ? place1 : place0;
-                const uint4 x = place < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(q + (size_t)place * D + 32 * u + 8 * j);
-                if (HELD) q_held[HELD ? u : 0][r] = x;
-                else q_s[(2 * u + r) * 32] = x;
-            }
-        asm volatile("" ::: "memory");   // (the stores stand before the reads below, which the compiler does not see as reads of this)
-        float o[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-        float m0 = QF_NEG_BIG, m1 = QF_NEG_BIG, l0 = 0.f, l1 = 0.f;   // rows g and g + 8; the sums are this lane's share
-        for (int i = 0; i < steps; ++i) {
-            const bool live = k_at != nullptr;
-            const int key0 = (p0 + i / STEPS) * QF_PAGE + KEYS * (i % STEPS);
-            float s[2 * SIX][4];
-            if (live) {
-#pragma unroll
-                for (int t = 0; t < 2 * SIX; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-                for (int u = 0; u < KU; ++u) {
-                    const uint4 x = HELD ? q_held[HELD ? u : 0][0] : load_shared_16(q_s + 2 * u * 32), y = HELD ? q_held[HELD ? u : 0][1] : load_shared_16(q_s + (2 * u + 1) * 32);
-                    const uint32_t lo[4] = {x.x, y.x, x.y, y.y}, hi[4] = {x.z, y.z, x.w, y.w};
-#pragma unroll
-                    for (int t = 0; t < 2 * SIX; ++t) {
-                        mma_bf16_16816(s[t], lo, k[t][u].x, k[t][u].y);
-                        mma_bf16_16816(s[t], hi, k[t][u].z, k[t][u].w);
-                    }
-                }
-            }
-            find(i + 1);
-            if (k_at) load_keys();   // (on their way while the softmax and the second product run)
-            if (live) {
-                float top0 = QF_NEG_BIG, top1 = QF_NEG_BIG;
-                if (key0 + KEYS > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
-                    const int see0 = prefix ? min(bound, shared_seen(a, place0)) : bound, see1 = prefix ? min(bound, shared_seen(a, place1)) : bound;
-#pragma unroll
-                    for (int t = 0; t < 2 * SIX; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][e] = key0 + 8 * t + 2 * j + (e & 1) < (e >> 1 ? see1 : see0) ? s[t][e] * a.scale_log2 : QF_NEG_BIG;
-#pragma unroll
-                    for (int r = 0; r < 4 * SIX; ++r)
-                        if (key0 + r / 4 * 16 + 2 * j + (r & 1) + 8 * (r >> 1 & 1) >= bound)
-#pragma unroll
-                            for (int u = 0; u < E / 2; ++u) v[r][u] = 0u;
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 2 * SIX; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][e] *= a.scale_log2;
-                }
-#pragma unroll
-                for (int t = 0; t < 2 * SIX; ++t) top0 = fmaxf(top0, fmaxf(s[t][0], s[t][1])), top1 = fmaxf(top1, fmaxf(s[t][2], s[t][3]));
-                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
-                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
-                top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
-                top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
-                if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1)) {
-                    const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1), c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
-                    m0 = n0, m1 = n1;
-                    l0 *= c0, l1 *= c1;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) o[t][0] *= c0, o[t][1] *= c0, o[t][2] *= c1, o[t][3] *= c1;
-                }
-                const float from0 = m0 <= QF_NEG_BIG ? 0.f : m0, from1 = m1 <= QF_NEG_BIG ? 0.f : m1;   // (no key seen yet: weights of 2^(-huge) = 0)
-#pragma unroll
-                for (int x = 0; x < SIX; ++x) {   // 16 keys at a time
-#pragma unroll
-                    for (int t = 2 * x; t < 2 * x + 2; ++t) {
-                        s[t][0] = fast_exp2(s[t][0] - from0), s[t][1] = fast_exp2(s[t][1] - from0);
-                        s[t][2] = fast_exp2(s[t][2] - from1), s[t][3] = fast_exp2(s[t][3] - from1);
-                        l0 += s[t][0] + s[t][1];
-                        l1 += s[t][2] + s[t][3];
-                    }
-                    const uint32_t p[4] = {pack_bf16(s[2 * x][0], s[2 * x][1]), pack_bf16(s[2 * x][2], s[2 * x][3]),
-                                           pack_bf16(s[2 * x + 1][0], s[2 * x + 1][1]), pack_bf16(s[2 * x + 1][2], s[2 * x + 1][3])};
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const uint32_t pick = t & 1 ? 0x7632u : 0x5410u;
-                        mma_bf16_16816(o[t], p, __byte_perm(v[4 * x][t / 2], v[4 * x + 1][t / 2], pick), __byte_perm(v[4 * x + 2][t / 2], v[4 * x + 3][t / 2], pick));
-                    }
-                }
-            }
-            if (k_at) load_values(k_at + to_values);
-        }
-#pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-        }
-        // o[t][0], o[t][1] are row g's columns 2 j E + t and (2 j + 1) E + t: 2 E columns side by side
-        auto leave = [&](float* row0, float* row1, float f0, float f1) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < E; t += 4) {
-                    const int c = (2 * j + h) * E + t;
-                    if (row0) *reinterpret_cast<float4*>(row0 + c) = make_float4(o[t][h] * f0, o[t + 1][h] * f0, o[t + 2][h] * f0, o[t + 3][h] * f0);
-                    if (row1) *reinterpret_cast<float4*>(row1 + c) = make_float4(o[t][2 + h] * f1, o[t + 1][2 + h] * f1, o[t + 2][2 + h] * f1, o[t + 3][2 + h] * f1);
-                }
-        };
-        if (!(rec.kind & SH_TOGETHER)) {
-            const size_t at0 = (size_t)place0 * a.most_parts + rec.part, at1 = (size_t)place1 * a.most_parts + rec.part;
-            leave(place0 < 0 ? nullptr : a.part_o + at0 * D, place1 < 0 ? nullptr : a.part_o + at1 * D, 1.f, 1.f);
-            if (j == 0 && place0 >= 0) *reinterpret_cast<float2*>(a.part_ml + at0 * 2) = make_float2(m0, l0);
-            if (j == 0 && place1 >= 0) *reinterpret_cast<float2*>(a.part_ml + at1 * 2) = make_float2(m1, l1);
+        SharedSums<D> x;
+        shared_warp<D, KEYS>(q, site, a, rec, kvh, reinterpret_cast<uint4*>(&merge_s[warp][0][0]), x);
+        if (!whole) {
+            x.leave_part(a, rec.part);
             continue;
         }
         // the warps' sums come together in warp order
-        if (j == 0) m_s[warp][g] = m0, m_s[warp][g + 8] = m1;
+        if (j == 0) m_s[warp][g] = x.m0, m_s[warp][g + 8] = x.m1;
         __syncthreads();
         float top0 = m_s[0][g], top1 = m_s[0][g + 8];
 #pragma unroll
         for (int w = 1; w < SH_TEAM; ++w) top0 = fmaxf(top0, m_s[w][g]), top1 = fmaxf(top1, m_s[w][g + 8]);
-        const float f0 = fast_exp2(m0 - top0), f1 = fast_exp2(m1 - top1);
-        if (j == 0) l_s[warp][g] = l0 * f0, l_s[warp][g + 8] = l1 * f1;
-        leave(merge_s[warp][g], merge_s[warp][g + 8], f0, f1);
+        const float f0 = fast_exp2(x.m0 - top0), f1 = fast_exp2(x.m1 - top1);
+        if (j == 0) l_s[warp][g] = x.l0 * f0, l_s[warp][g + 8] = x.l1 * f1;
+        x.leave(merge_s[warp][g], merge_s[warp][g + 8], f0, f1);
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * (D / 4); i += 32 * SH_TEAM) {
+        for (int i = threadIdx.x; i < 16 * (D / 4); i += THREADS) {
             const int r = i / (D / 4), c = i % (D / 4) * 4, place = shared_row(a, rec, kv_heads, kvh, 16 * rec.chunk + r);
             if (place < 0) continue;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < SH_TEAM; ++w) {
-                const float4 x = *reinterpret_cast<const float4*>(&merge_s[w][r][c]);
-                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                const float4 v = *reinterpret_cast<const float4*>(&merge_s[w][r][c]);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
             const size_t at = (size_t)place * a.most_parts + rec.part;
             *reinterpret_cast<float4*>(a.part_o + at * D + c) = sum;
@@ -489,12 +572,15 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     __shared__ float m_s[SH_ROWS], l_s[SH_ROWS], corr_s[SH_ROWS];
     grid_launch_dependents();
     grid_dependency_wait();
-    const SharedRecord* records = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs));
-    const int kv_heads = site.kv_heads, units = a.plan[0] * SH_TEAM * kv_heads, tid = threadIdx.x;
+    __shared__ SharedRecord record_s;
+    const SharedPlan plan = shared_plan<SH_THREADS>(a, reinterpret_cast<int*>(p_s + SH_ROWS * (QF_PAGE + 4)), D);
+    if (blockIdx.x == 0) shared_count_parts<SH_THREADS>(a, plan);
+    const int kv_heads = site.kv_heads, units = plan.singles * kv_heads, tid = threadIdx.x;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {   // (a record is a block's work here)
     const int kvh = unit % kv_heads;
-    const SharedRecord rec = records[unit / kv_heads];
-    if (rec.kind & SH_NONE) break;
+    shared_records<SH_THREADS, 1>(a, plan, threadIdx.x, 0, unit / kv_heads, &record_s);
+    __syncthreads();
+    const SharedRecord rec = record_s;
     const int bound = rec.kind & SH_PREFIX ? rec.p_end * QF_PAGE : rec.limit;
     if (tid < SH_ROWS) {
         row_at[tid] = shared_row(a, rec, kv_heads, kvh, SH_ROWS * rec.chunk + tid);
@@ -609,7 +695,7 @@ shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __rest
     const int per = D / V;
     if (i >= (long long)a.n_seqs * a.n_heads * per) return;
     const int row = (int)(i / per), d = (int)(i % per) * V, entry = row / a.n_heads;
-    const int packed = a.plan[4 + entry], runs = a.slots[entry] < 0 ? 0 : (packed & 0xffff) + (packed >> 16);
+    const int packed = a.part_n[entry], runs = (packed & 0xffff) + (packed >> 16);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.most_parts;
     const float* po = a.part_o + (size_t)row * a.most_parts * D + d;
     float top = QF_NEG_BIG, den = 0.f, num[V];
@@ -663,17 +749,18 @@ shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __rest
 
 // ---------------------------------------------------------------------------------------------------------------- host
 static bool shared_fast(int is_bf16, int d) { return is_bf16 && (d == 32 || d == 64 || d == 96 || d == 128); }
-static size_t shared_generic_smem(int d) {
+static size_t shared_generic_smem(int d, int plan_ints) {
     const int ld = (d + 3) / 4 * 4 + 4;
-    return (size_t)((SH_ROWS + QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4)) * sizeof(float);
+    return (size_t)((SH_ROWS + QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4) + plan_ints) * sizeof(float);
 }
 
 // Where the tiles take over.
 #define SH_TILE_ROWS 65
 #define SH_TILE_PAGES 8
 
-// What sizes the plan and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of a
-// block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows and pages goes to the tiles (0: there are none); [6]: SMs.
+// What sizes the launches and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of
+// a block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows and pages goes to the tiles (0: there are
+// none); [6]: SMs.
 QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     const int sms = qf_sm_count();
     if (sms <= 0 || head_dim <= 0 || head_dim > 256) return (int)cudaErrorInvalidValue;
@@ -688,34 +775,23 @@ QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     return 0;
 }
 
-QF_EXPORT int qf_attention_shared_plan(const int* tok_pos, const int* slots, int n_seqs, const int* entry_pages, const int* entry_group, const int* begin,
-                                       const int* pages, int n_groups, int kv_heads, int n_heads, int is_bf16, int head_dim, int most_shared, int most_own,
-                                       int* plan, int most_units, int most_tiles, cudaStream_t stream) {
-    int sizes[7];
-    if (n_seqs <= 0 || n_seqs > SH_MAX_SEQS || n_groups > n_seqs || kv_heads <= 0 || n_heads % kv_heads || most_own <= 0 || most_own > 0x7fff || most_shared > 0xffff ||
-        (n_groups > 0 && most_shared <= 0) || most_units <= 0)
-        return (int)cudaErrorInvalidValue;
-    const int bad = qf_attention_shared_shape(is_bf16, head_dim, sizes);
-    if (bad) return bad;
-    const size_t smem = (size_t)(n_seqs + 6 * n_groups) * sizeof(int);
-    const cudaError_t e = cudaFuncSetAttribute(shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 7 * SH_MAX_SEQS * (int)sizeof(int));
-    if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(shared_plan_kernel, dim3(1), dim3(SH_PLAN_THREADS), smem, stream, tok_pos, slots, n_seqs, entry_pages, entry_group, begin, pages,
-                           n_groups, kv_heads, n_heads / kv_heads, sizes[0], sizes[1], sizes[2], most_shared, most_own,
-                           most_tiles > 0 ? sizes[4] : 0x7fffffff, sizes[5], sizes[6], plan, most_units, most_tiles);
-}
-
 template <int D>
 static int launch_parts(const void* q, KvSite<bf16> site, const SharedArgs& a, int units, cudaStream_t stream) {
-    const int at_once = 2 * qf_sm_count();
-    return (int)launch_pdl(shared_parts_kernel<D>, dim3((unsigned)(units < at_once ? units : at_once)), dim3(32 * SH_TEAM), 0, stream, (const bf16*)q, site, a);
+    const int at_once = 2 * qf_sm_count(), smem = shared_plan_ints(a.n_seqs, a.n_groups) * (int)sizeof(int);
+    auto kernel = shared_parts_kernel<D>;
+    if (smem > 8 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_plan_ints(SH_MAX_SEQS, SH_MAX_SEQS) * (int)sizeof(int));
+        if (e != cudaSuccess) return (int)e;
+    }
+    return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(32 * SH_TEAM), (size_t)smem, stream, (const bf16*)q, site, a);
 }
 
 template <typename T>
 static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, int units, cudaStream_t stream) {
-    const size_t smem = shared_generic_smem(site.head_dim);
+    const size_t smem = shared_generic_smem(site.head_dim, shared_plan_ints(a.n_seqs, a.n_groups));
     auto kernel = shared_parts_generic_kernel<T>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)shared_generic_smem(256, shared_plan_ints(SH_MAX_SEQS, SH_MAX_SEQS)));
     if (e != cudaSuccess) return (int)e;
     const int at_once = 2 * qf_sm_count();
     return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(SH_THREADS), smem, stream, (const T*)q, site, a);
@@ -729,29 +805,35 @@ static int launch_join(const SharedArgs& a, int head_dim, void* out, const float
     return (int)launch_pdl(shared_join_kernel<T, 1>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a, head_dim, (T*)out, sinks);
 }
 
-// The parts and their joining. `plan`: of qf_attention_shared_plan with the same shape; part_o, part_ml: n_seqs * n_heads * most_parts * head_dim and
-// * 2 floats, most_parts >= the most shared and own parts of a row together.
-QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const int* tok_pos, const int* slots, const int* members, const int* begin,
-                                  const int* plan, int most_units, int most_tiles, void* base, const int* table, long long page_elems, int table_stride,
-                                  int kv_heads, int head_dim, int n_heads, int n_seqs, float scale, int most_parts, float* part_o, float* part_ml,
+// `most_units`, `most_tiles`: bounds of the blocks' runs with the groups of SH_TEAM warps' records, and of the tile records that cannot be cut into fewer, of
+// one kv head (0: no group is given to the tiles); `most_shared`, `most_own`: the most parts that a row has room for of each; part_o, part_ml: n_seqs * n_heads * (most_shared +
+// most_own) * head_dim and * 2 floats; part_n: n_seqs ints.
+QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const int* tok_pos, const int* slots, const int* entry_pages,
+                                  const int* entry_group, const int* members, const int* begin, const int* pages, int n_groups, int most_units,
+                                  int most_tiles, int most_shared, int most_own, void* base, const int* table, long long page_elems, int table_stride,
+                                  int kv_heads, int head_dim, int n_heads, int n_seqs, float scale, float* part_o, float* part_ml, int* part_n,
                                   const float* sinks, int* err, cudaStream_t stream) {
-    if (n_seqs <= 0) return 0;
-    if (kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || head_dim > 256 || most_units <= 0)
+    int sizes[7];
+    if (n_seqs <= 0 || n_seqs > SH_MAX_SEQS || n_groups > n_seqs || kv_heads <= 0 || n_heads % kv_heads || most_units <= 0 || most_own <= 0 || most_own > 0x7fff ||
+        most_shared > 0xffff || (n_groups > 0 && most_shared <= 0))
         return (int)cudaErrorInvalidValue;
-    const SharedArgs a = {tok_pos, slots, members, begin, plan, part_o, part_ml, err, n_seqs, n_heads, most_parts, most_units, scale * 1.4426950408889634f};
+    const int bad = qf_attention_shared_shape(is_bf16, head_dim, sizes);
+    if (bad) return bad;
+    const SharedArgs a = {tok_pos, slots, entry_pages, entry_group, members, begin, pages, part_o, part_ml, part_n, err, n_seqs, n_groups, n_heads, kv_heads,
+                          most_shared + most_own, most_shared, most_own, sizes[0], sizes[1], most_tiles > 0 ? 1 : sizes[2], most_tiles > 0 ? sizes[4] : 0, sizes[5], sizes[6],
+                          scale * 1.4426950408889634f};
     const bool fast = shared_fast(is_bf16, head_dim);
     const long long all = (long long)most_units * kv_heads * (fast ? 1 : SH_TEAM);
     const int units = (int)(all < 0x7fffffff ? all : 0x7fffffff);
     int code;
     if (fast) {
         const KvSite<bf16> site{(bf16*)base, table, page_elems, table_stride, kv_heads, head_dim};
-        if (most_tiles > 0) {
+        if (most_tiles > 0)
             code = head_dim == 64 ? launch_tiles<64>(q, site, a, most_tiles, stream) : head_dim == 128 ? launch_tiles<128>(q, site, a, most_tiles, stream)
-                                                                                                         : (int)cudaErrorInvalidValue;
-            if (code) return code;
-        }
-        code = head_dim == 32 ? launch_parts<32>(q, site, a, units, stream) : head_dim == 64 ? launch_parts<64>(q, site, a, units, stream)
-             : head_dim == 96 ? launch_parts<96>(q, site, a, units, stream) : launch_parts<128>(q, site, a, units, stream);
+                                                                                                       : (int)cudaErrorInvalidValue;
+        else
+            code = head_dim == 32 ? launch_parts<32>(q, site, a, units, stream) : head_dim == 64 ? launch_parts<64>(q, site, a, units, stream)
+                 : head_dim == 96 ? launch_parts<96>(q, site, a, units, stream) : launch_parts<128>(q, site, a, units, stream);
     } else if (is_bf16) {
         code = launch_generic(q, KvSite<bf16>{(bf16*)base, table, page_elems, table_stride, kv_heads, head_dim}, a, units, stream);
     } else {

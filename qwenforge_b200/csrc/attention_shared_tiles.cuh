@@ -8,7 +8,9 @@
 //   warp 8           issues the products: O += P V of a tile as soon as its weights are written, then S = Q K^T of its next turn
 //   warp 9           issues the copies
 // There is no causal mask: a row sees every key of the run, but for a member that stands inside the shared pages and for the half turn behind an odd
-// page count. At the end every row leaves its sums, unnormalised and in float32, with its reference maximum and its sum of weights.
+// page count. At the end every row leaves its sums, unnormalised and in float32, with its reference maximum and its sum of weights; a warp's rows go
+// through the room that their queries had, so that they are written 128 bytes or more at a time.
+// Blocks without a tile record give their ten warps the records of everything else, at the same time: sequences' own pages and small groups'.
 // What bounds it: 16,384 exponentials a tile and turn on the SM's special-function units, beside as many cycles of products at D = 128.
 // Every wait is bounded: one that runs out sets QF_ERR_COPY_TIMEOUT and ends the thread's loop, and the block still frees its tensor memory and returns.
 #pragma once
@@ -30,6 +32,7 @@ __device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.asy
 template <int D>
 __global__ void __launch_bounds__(ST_THREADS, 1)
 shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a) {
+    constexpr int WARPS = ST_THREADS / 32;
     constexpr int CB = D / 64;                    // blocks of 64 columns in a row of Q, K or V
     constexpr int Q_BLOCK = ST_BM * 128;          // bytes of one [128][64] block of Q
     constexpr int KV_BLOCK = ST_BK * 128;         // bytes of one [128][64] block of two pages' keys or values
@@ -37,7 +40,7 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     constexpr int Q_BYTES = CB * Q_BLOCK, KV_BYTES = CB * KV_BLOCK;
     constexpr uint32_t TMEM_COLS = 512, O_COL = 256;   // S (and P) of tile t in columns 128 t .., O behind them
     constexpr int PRODUCTS = 8, COPIES = 9;            // the issuing warps
-    extern __shared__ unsigned char tc_smem[];
+    extern __shared__ __align__(16) unsigned char tc_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tc_smem) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_s = smem;                          // [2][CB][128][64]
     unsigned char* k_s = q_s + 2 * Q_BYTES;             // [2][CB][128][64]
@@ -46,10 +49,31 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     __shared__ uint32_t tmem_base_s;
     grid_dependency_wait();
     const int kv_heads = site.kv_heads, kvh = (int)(blockIdx.x % kv_heads);
-    if ((int)(blockIdx.x / kv_heads) >= a.plan[1]) return;
-    const SharedRecord rec = reinterpret_cast<const SharedRecord*>(a.plan + shared_plan_records(a.n_seqs))[(size_t)a.most_units * SH_TEAM + blockIdx.x / kv_heads];
+    __shared__ SharedRecord record_s[WARPS];
+    const SharedPlan plan = shared_plan<ST_THREADS>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
+    if (blockIdx.x == 0) shared_count_parts<ST_THREADS>(a, plan);
+    const int tile_blocks = plan.tiles * kv_heads;
+    if ((int)blockIdx.x >= tile_blocks) {
+        // ---- the other records, a warp each
+        grid_launch_dependents();
+        const int me = threadIdx.x >> 5, all = ((int)gridDim.x - tile_blocks) * WARPS;
+        uint4* const room = reinterpret_cast<uint4*>(tc_smem + (shared_plan_ints(a.n_seqs, a.n_groups) * 4 + 15) / 16 * 16 + me * shared_query_bytes(D));
+        for (int task = me * ((int)gridDim.x - tile_blocks) + (int)blockIdx.x - tile_blocks; task < plan.singles * kv_heads; task += all) {
+            shared_records<32, 1>(a, plan, threadIdx.x & 31, 0, task / kv_heads, record_s + me);
+            __syncwarp();
+            const SharedRecord rec = record_s[me];
+            __syncwarp();
+            SharedSums<D> x;
+            shared_warp<D, (D <= 64 ? 32 : 16)>(q, site, a, rec, task % kv_heads, room, x);
+            x.leave_part(a, rec.part);
+        }
+        return;
+    }
+    shared_records<ST_THREADS, 1>(a, plan, threadIdx.x, SH_NONE, blockIdx.x / kv_heads, record_s);
+    __syncthreads();
+    const SharedRecord rec = record_s[0];
     const int warp = threadIdx.x >> 5, t = warp < 8 ? warp >> 2 : 0, row = threadIdx.x & 127;   // row threads: tile t, row `row`
-    const int rows = (a.begin[rec.subject + 1] - a.begin[rec.subject]) * (a.n_heads / kv_heads) - 2 * ST_BM * rec.chunk;   // from the first tile's on
+    const int rows = plan.rows[rec.subject] - 2 * ST_BM * rec.chunk;   // from the first tile's on
     const int tiles = rows > ST_BM ? 2 : 1;
     const int turns = (rec.p_end - rec.p_begin + 1) / 2, end = rec.p_end * QF_PAGE;   // no key of this run from `end` on
 
@@ -71,8 +95,9 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
+    fence_to_async();   // (the plan's room is the copies' from here on)
     tc_fence_before();
-    __syncthreads();
+    __syncthreads();   // (also: everyone has read what it wants of the plan)
     tc_fence_after();
     grid_launch_dependents();   // (the block has its tensor memory)
     const uint32_t tmem = tmem_base_s;
@@ -268,17 +293,29 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
         if (!timed_out && !wait_all(&bar_pv[t], (turns - 1) & 1)) timed_out = true;
         tc_fence_after();
         if (!timed_out) {   // (the loads are collective: every lane takes part, rows that are not there store nothing)
-            const size_t at = (size_t)(place < 0 ? 0 : place) * a.most_parts + rec.part;
-            if (place >= 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref, l_run);
+            constexpr int HALF = D / 2, C4 = HALF / 4, AT_ONCE = 32 / C4;   // a row's 16-byte pieces of half its columns, and rows that a warp writes at once
+            const int lane = threadIdx.x & 31;
+            if (place >= 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)place * a.most_parts + rec.part) * 2) = make_float2(m_ref, l_run);
+            float4* const room = reinterpret_cast<float4*>(q_s + t * Q_BYTES) + (warp & 3) * 32 * C4;   // the warp's 32 rows of [128][HALF] floats
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t raw[32];
-                tmem_load_32(o_at + c0, raw);
-                if (place >= 0) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<uint4*>(a.part_o + at * D + c0 + c) = make_uint4(raw[c], raw[c + 1], raw[c + 2], raw[c + 3]);
+                for (int c0 = 0; c0 < HALF; c0 += 32) {
+                    uint32_t raw[32];
+                    tmem_load_32(o_at + h * HALF + c0, raw);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)   // piece c of a row lies at c XOR (row modulo 8): neither side meets a bank twice
+                        room[lane * C4 + ((c0 / 4 + c) ^ (lane & 7))] = make_float4(__uint_as_float(raw[4 * c]), __uint_as_float(raw[4 * c + 1]),
+                                                                                     __uint_as_float(raw[4 * c + 2]), __uint_as_float(raw[4 * c + 3]));
                 }
+                __syncwarp();
+#pragma unroll 4
+                for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                    const int r = r0 + lane / C4, c = lane % C4, to = __shfl_sync(0xffffffffu, place, r);
+                    if (to >= 0)
+                        *reinterpret_cast<float4*>(a.part_o + ((size_t)to * a.most_parts + rec.part) * D + h * HALF + 4 * c) = room[r * C4 + (c ^ (r & 7))];
+                }
+                __syncwarp();
             }
         }
     }
@@ -290,7 +327,7 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
 }
 
 template <int D>
-static int launch_tiles(const void* q, KvSite<bf16> site, const SharedArgs& a, int tile_records, cudaStream_t stream) {
+static int launch_tiles(const void* q, KvSite<bf16> site, const SharedArgs& a, int most_tiles, cudaStream_t stream) {
     CUtensorMap map = {};
     if (site.page_elems % D) return (int)cudaErrorInvalidValue;
     // The cache of this entry as one matrix of rows of D elements. The map is given more rows than any cache has (its extent only bounds what a copy may
@@ -298,9 +335,12 @@ static int launch_tiles(const void* q, KvSite<bf16> site, const SharedArgs& a, i
     if (!qf_make_map_bf16(&map, site.base, 1ll << 31, D, D, QF_PAGE)) return (int)cudaErrorNotSupported;
     constexpr size_t stages = (size_t)(D / 64) * (2 * ST_BM + 4 * ST_BK) * 128 + 1024;
     constexpr size_t smem = stages > QF_TMEM_SMEM_ALONE ? stages : (size_t)QF_TMEM_SMEM_ALONE;
+    static_assert(shared_plan_ints(SH_MAX_SEQS, SH_MAX_SEQS) * sizeof(int) + 16 + ST_THREADS / 32 * shared_query_bytes(D) <= smem, "the plan's room, and the queries'");
     static_assert(qf_tmem_fits(512, smem) && smem <= 227 * 1024, "the rule of tcgen05.cuh");
     auto kernel = shared_tiles_kernel<D>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(kernel, dim3((unsigned)(tile_records * site.kv_heads)), dim3(ST_THREADS), smem, stream, map, (const bf16*)q, site, a);
+    // a block to an SM, and no fewer than the records that cannot be cut into fewer, with a few blocks for everything else
+    const int least = most_tiles * site.kv_heads + 4, blocks = least > a.sms ? least : a.sms;
+    return (int)launch_pdl(kernel, dim3((unsigned)blocks), dim3(ST_THREADS), smem, stream, map, (const bf16*)q, site, a);
 }

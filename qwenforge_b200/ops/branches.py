@@ -167,6 +167,9 @@ class SharedPrefix:
     def __len__(self) -> int:
         return len(self.groups)
 
+    def addresses(self) -> tuple:
+        return tuple(t.data_ptr() for t in (self.entry_pages, self.entry_group, self.members, self.begin, self.pages))
+
     def shape(self) -> tuple:
         """What the launches go by: the batch, the groups' members, the bound on their pages."""
         return (self.n_seqs, tuple(len(entries) for entries, _ in self.groups), self.bound_pages)
@@ -181,34 +184,26 @@ class SharedPrefix:
 
 
 class SharedScratch:
-    """Workspaces of `attention_shared`: the parts' sums with their maxima, and the plans. One instance serves calls that run one after
-    another on one stream; what is captured into a graph has one of its own."""
+    """Workspaces of `attention_shared`: the parts' sums with their maxima, and how many parts a row has. One instance serves calls that run
+    one after another on one stream; what is captured into a graph has one of its own."""
 
     def __init__(self, device):
         self.device = torch.device(device)
-        self.part_o = self.part_ml = None
-        self.plans: dict = {}
+        self.part_o = self.part_ml = self.part_n = None
 
-    def ensure(self, parts: int, head_dim: int) -> None:
+    def ensure(self, n_seqs: int, parts: int, head_dim: int) -> None:
         if self.part_o is None or self.part_o.numel() < parts * head_dim:
             self.part_o = torch.empty(parts * head_dim, dtype=torch.float32, device=self.device)
         if self.part_ml is None or self.part_ml.numel() < parts * 2:
             self.part_ml = torch.empty(parts * 2, dtype=torch.float32, device=self.device)
-
-
-class SharedPlan:
-    """What `attention_shared_plan` made: the tensor (which block and warp takes which run) and the sizes that the attention's launch goes by."""
-    __slots__ = ("tensor", "key", "records", "most_parts")
-
-    def __init__(self, tensor, key, records, most_parts):
-        self.tensor, self.key, self.records, self.most_parts = tensor, key, records, most_parts
+        if self.part_n is None or self.part_n.numel() < n_seqs:
+            self.part_n = torch.empty(n_seqs, dtype=torch.int32, device=self.device)
 
 
 def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: SharedPrefix, own_pages: int) -> tuple:
-    """((units, tile records) of the plan, most shared parts, most own parts of a row): bounds of what the plan kernel can come to, whatever the
+    """(units, tile records, most shared parts, most own parts of a row): bounds of what the device's plan can come to, whatever the
     lengths. It gives a warp at least `pages x tiles x kv heads / warps` pages, so units of a block's run cover, up to twice, no more
-    than the warps there are, and so do single warps' records but for one more per item; tile records fill the SMs once, or are the
-    pairs of tiles uncut."""
+    than the warps there are, and so do single warps' records but for one more per item. Tile records: the pairs of tiles, uncut."""
     held = share.sizes.get((dtype, head_dim, kv_heads, n_heads, own_pages))
     if held is not None:
         return held
@@ -227,13 +222,16 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     pairs = [-(-len(entries) * group_heads // 256) for entries, _ in share.groups if len(entries) * group_heads >= tile_rows]
     if not tile_rows or share.bound_pages < tile_pages:
         pairs = []
+    if pairs:   # (everything else is cut for single warps then)
+        most_shared = max(most_shared, min(most // 4, share.bound_pages))
     for n in pairs:
         most_shared = max(most_shared, min(most, -(-share.bound_pages // 4), sms // (kv_heads * n) + 1))
     singles = warps // kv_heads + 1 + sum(tiles) + share.n_seqs * own_tiles
-    records = (2 * warps // (team * kv_heads) + 2 + -(-singles // SHARED_TEAM), max(sms // kv_heads, sum(pairs)) if pairs else 0)
+    units = 2 * warps // (team * kv_heads) + 2 + -(-singles // SHARED_TEAM)
     if len(share.sizes) >= 64:
         share.sizes.clear()
-    held = share.sizes[dtype, head_dim, kv_heads, n_heads, own_pages] = (records, most_shared, parts(own_pages, own_tiles))
+    held = share.sizes[dtype, head_dim, kv_heads, n_heads, own_pages] = (
+        units, sum(pairs), most_shared, min(most // 2, own_pages) if pairs else parts(own_pages, own_tiles))
     return held
 
 
@@ -255,36 +253,15 @@ def _batch_refused(cu_q, tok_pos, slots, n_seqs: int, kv_heads: int, n_heads: in
         raise KernelError("attention_shared: wants exactly one token per sequence, and a SharedPrefix of this batch")
 
 
-def attention_shared_plan(cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, kv_heads: int, head_dim: int, n_heads: int,
-                          n_seqs: int, share: SharedPrefix, scratch: SharedScratch, dtype: torch.dtype, max_kv_len: int) -> SharedPlan:
-    """The plan of one step for `attention_shared` of this shape, worked out on the device from the batch's lengths; it serves every
-    layer of the step with this shape. `max_kv_len`: an upper bound of any sequence's length after the step. The tensor belongs to
-    `scratch` and is overwritten by the next plan of the same shape."""
-    _batch_refused(cu_q, tok_pos, slots, n_seqs, kv_heads, n_heads, head_dim, dtype, share)
-    _here("attention_shared", cu_q, tok_pos, slots, share.entry_pages)
-    own_pages = max(1, -(-int(max_kv_len) // PAGE_TOKENS) - share.least_pages)
-    records, most_shared, most_own = _shared_sizes(dtype, head_dim, kv_heads, n_heads, share, own_pages)
-    key = (n_seqs, kv_heads, n_heads, head_dim, dtype)
-    ints = 4 + -(-n_seqs // 4) * 4 + (records[0] * SHARED_TEAM + records[1]) * 8
-    held = scratch.plans.get(key)
-    if held is None or held.numel() < ints:
-        held = scratch.plans[key] = torch.empty(ints, dtype=torch.int32, device=cu_q.device)
-    _check(_function("attention_shared", "qf_attention_shared_plan", _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P)(
-        tok_pos.data_ptr(), slots.data_ptr(), n_seqs, share.entry_pages.data_ptr(), share.entry_group.data_ptr(), share.begin.data_ptr(),
-        share.pages.data_ptr(), len(share.groups), kv_heads, n_heads, dtype is torch.bfloat16, head_dim, most_shared, most_own, held.data_ptr(),
-        records[0], records[1], _stream()), "attention_shared_plan")
-    return SharedPlan(held, key, records, most_shared + most_own)
-
-
 def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site, n_heads: int,
                      n_seqs: int, scale: float, share: SharedPrefix, scratch: SharedScratch, err: torch.Tensor,
-                     max_kv_len: Optional[int] = None, plan: Optional[SharedPlan] = None, sinks: Optional[torch.Tensor] = None) -> None:
+                     max_kv_len: Optional[int] = None, sinks: Optional[torch.Tensor] = None) -> None:
     """Attention of ONE new token per sequence over its cache, where sequences share their first pages (`share`): what they share is read
     once for all of them. The result is that of `attention_decode`: query head i reads kv head i // (n_heads / kv_heads), key j is visible
     iff j <= the token's position. bfloat16 or float32, head sizes up to 256 (bfloat16 of 32, 64, 96 and 128 on tensor cores). A padding
     entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page table
-    has room for). `plan` (`attention_shared_plan` with the same shape, made in this step) is made here when absent. `sinks` (float32
-    [n_heads]): a logit per head that joins the softmax's denominator once, with no key and no value."""
+    has room for); it sizes the workspaces and the launch. `sinks` (float32 [n_heads]): a logit per head that joins the softmax's denominator
+    once, with no key and no value."""
     storage, table, d, kv_heads, dtype = site.storage, site.table, site.head_dim, site.kv_heads, q.dtype
     _batch_refused(cu_q, tok_pos, slots, n_seqs, kv_heads, n_heads, d, dtype, share)
     if not (out.dtype is dtype and storage.dtype is dtype and q.is_contiguous() and out.is_contiguous() and table.dtype is torch.int32
@@ -309,19 +286,16 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
         if sinks.numel() != n_heads:
             raise KernelError("attention_shared: sinks must hold one float32 per query head")
     _here("attention_shared", q, out, cu_q, tok_pos, slots, storage, table, share.entry_pages, err, sinks)
-    if plan is None:
-        longest = table.shape[1] * PAGE_TOKENS if max_kv_len is None else int(max_kv_len)
-        plan = attention_shared_plan(cu_q, tok_pos, slots, kv_heads, d, n_heads, n_seqs, share, scratch, dtype, longest)
-    elif plan.key != (n_seqs, kv_heads, n_heads, d, dtype):
-        raise KernelError("attention_shared: the plan was made for another shape")
-    scratch.ensure(n_seqs * n_heads * plan.most_parts, d)
-    units, tiles = plan.records
-    code = _function("attention_shared", "qf_attention_shared", _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _LL, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P,
-                     _P)(
-        dtype is torch.bfloat16, q_at, out.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), share.members.data_ptr(), share.begin.data_ptr(),
-        plan.tensor.data_ptr(), units, tiles, storage_at, table.data_ptr(), site.page_elems, site.table_stride, kv_heads, d, n_heads, n_seqs, scale,
-        plan.most_parts, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), _at(sinks), err.data_ptr(), _stream())
-    kernels.launches += 2 if tiles else 1   # (the tiles, the parts, and their joining)
+    longest = table.shape[1] * PAGE_TOKENS if max_kv_len is None else int(max_kv_len)
+    own_pages = max(1, -(-longest // PAGE_TOKENS) - share.least_pages)
+    units, tiles, most_shared, most_own = _shared_sizes(dtype, d, kv_heads, n_heads, share, own_pages)
+    scratch.ensure(n_seqs, n_seqs * n_heads * (most_shared + most_own), d)
+    code = _function("attention_shared", "qf_attention_shared", _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _LL, _I, _I, _I, _I, _I, _F, _P,
+                     _P, _P, _P, _P, _P)(
+        dtype is torch.bfloat16, q_at, out.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *share.addresses(), len(share.groups), units, tiles, most_shared,
+        most_own, storage_at, table.data_ptr(), site.page_elems, site.table_stride, kv_heads, d, n_heads, n_seqs, scale, scratch.part_o.data_ptr(),
+        scratch.part_ml.data_ptr(), scratch.part_n.data_ptr(), _at(sinks), err.data_ptr(), _stream())
+    kernels.launches += 1   # (the parts, and their joining)
     _check(code, "attention_shared")
 
 

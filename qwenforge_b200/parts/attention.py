@@ -536,14 +536,8 @@ class GqaAttention(Mixer):
                 and self.window <= 0)
 
     def _attend_shared(self, q, attended, args, ctx) -> None:
-        memo = ctx.step_memo if ctx.step_memo is not None else {}
-        key = ("gqa_attention.shared_plan", self.n_kv, self.n_heads, self.head_dim)
-        plan = memo.get(key)
-        if plan is None:
-            plan = memo[key] = ops.attention_shared_plan(ctx.cu_q, ctx.tok_pos, ctx.slots, self.n_kv, self.head_dim, self.n_heads, ctx.n_seqs,
-                                                         ctx.shared, ctx.shared_scratch, q.dtype, ctx.max_kv_len)
         ops.attention_shared(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs, self.scale, ctx.shared,
-                             ctx.shared_scratch, ctx.err, plan=plan)
+                             ctx.shared_scratch, ctx.err, max_kv_len=ctx.max_kv_len)
 
     def decode_plan(self, ctx, leave: int = 0) -> torch.Tensor:
         """Which block of the decode attention takes which run of which sequence: made once per step, by the first
