@@ -31,9 +31,15 @@ struct __align__(16) SharedRecord {
     int p_begin, p_end;
     int limit;     // keys below it are seen by every row (a sequence's own part: its length)
     int part;      // which of a row's parts this is
+    int begin, rows;   // of a group: its first member's place, and members x heads
+    int pad[2];
 };
 #define SH_TEAM 4            // warps of a block of the parts' kernel
 #define SH_MAX_SEQS 2048
+#define SH_TILE_PLAN_INTS 12288
+#define SH_PAGE_TIME_64 0.24f
+#define SH_PAGE_TIME_128 0.4f
+#define SH_RECORD_TIME 0.35f
 
 // What every kernel gets.
 struct SharedArgs {
@@ -49,99 +55,105 @@ struct SharedArgs {
     int* part_n;      // [n_seqs] a row's shared parts | its own parts << 16
     int* err;
     int n_seqs, n_groups, n_heads, kv_heads, most_parts, most_shared, most_own;
-    int row_tile, warps, team, tile_rows, tile_pages, sms;   // (see shared_plan; tile_rows 0: no tiles)
+    int warps, team, tile_rows, tile_pages, sms;   // (see shared_plan; tile_rows 0: no tiles)
     float scale_log2;
 };
 
-// ---- the plan. An item is a group's pages or a sequence's own, times its tiles of `row_tile` rows. With X pages x tiles x kv heads in all and `warps`
-// warps at once, a warp gets t = max(1, X / warps) pages. Items of up to SH_TEAM t pages are cut into records of t pages for a warp each, every one a part
-// of its own; longer ones into runs of up to SH_TEAM t pages for a block, whose warps bring their sums together (SH_TOGETHER; not where a record is a
-// whole block's work, `team` 1). A group of `tile_rows` rows or more with `tile_pages` pages or more goes to the tensor-core tiles instead
-// (attention_shared_tiles.cuh): pairs of tiles of 128 rows, cut into runs of as many turns of two pages as make the records fill their share of the SMs
-// once; the other SMs' warps take the records of everything else meanwhile.
-// What bounds it: the latency of one round of loads and of a dozen barriers.
+// n / d rounded down, and up, for 0 <= n < 2^20 and 0 < d: the quotient in float32 is off by one at most.
+__device__ __forceinline__ int shared_div(int n, int d) {
+    int q = (int)__fdividef((float)n, (float)d);
+    const int r = n - q * d;
+    return q + (r < 0 ? -1 : r >= d ? 1 : 0);
+}
+__device__ __forceinline__ int shared_div_up(int n, int d) {
+    const int q = shared_div(n, d);
+    return q + (q * d < n);
+}
+
+// ---- the plan. An item is a group's pages or a sequence's own, times its tiles of 16 rows. A group of `tile_rows` rows or more with `tile_pages` pages
+// or more goes to the tensor-core tiles (attention_shared_tiles.cuh): pairs of tiles of 128 rows, every group's pages cut into runs by its share of the
+// work, no more records than the SMs that the tiles get by theirs. Everything else is cut into records of t pages for a warp each, every one a part of its
+// own: t = max(1, pages x tiles x kv heads / warps), beside tiles the next larger t that gives no more records than the other SMs have warps (two records
+// in a row take a warp twice the time); without tiles an item of more than SH_TEAM t pages goes in runs of up to SH_TEAM t to blocks, whose warps bring
+// their sums together (SH_TOGETHER).
+// What bounds it: the latency of one round of loads and of half a dozen barriers.
+#define SH_ROW_TILE 16
 struct SharedPlan {
     int* own;        // [n_seqs] pages of a sequence's own part
     int* own_first;  // [n_seqs] its first record of its kind
     int* slot;       // [n_groups] a live member's slot (-1: all have ended)
     int* least;      // [n_groups] the fewest keys that a live member sees
     int* rows;       // [n_groups]
+    int* begin;      // [n_groups]
     int* pages;      // [n_groups]
     int* first;      // [n_groups] the group's first record of its kind
     int* parts;      // [n_groups]
-    int own_tiles, each, together, stretch;   // (together: items of more pages are blocks' runs)
-    int blocks, singles, tiles;               // records of each kind
+    int own_tiles, each, together;    // (together: items of more pages are blocks' runs)
+    float tile_share;                 // parts of a tiled group beyond its first, for every turn
+    int blocks, singles, tiles;       // records of each kind
 };
-__host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 6 * n_groups; }
+__host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 7 * n_groups; }
 // What an SM takes for a turn of a pair of tiles, and, with ten warps at work, for a page of 16 rows and for what a record costs besides, in microseconds
 // as measured.
-__device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.85f : 2.05f; }
-__device__ __forceinline__ float shared_page_time(int d) { return d <= 64 ? 0.2f : 0.4f; }
-#define SH_RECORD_TIME 0.35f
+__device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.8f : 2.1f; }
+__device__ __forceinline__ float shared_page_time(int d) { return d <= 64 ? SH_PAGE_TIME_64 : SH_PAGE_TIME_128; }
 
-// Parts of an item of n_pages: of up to `unit` pages, no more than there is room for (longer ones then), none without a page; run: the pages of each.
-__device__ __forceinline__ int shared_cut(int n_pages, int unit, int most, int& run) {
+// An item of n pages in `want` parts: no more than there is room for, none without a page; run: the pages of each.
+__device__ __forceinline__ int shared_cut(int n, int want, int most, int& run) {
     run = 0;
-    if (n_pages <= 0) return 0;
-    const int n = min((n_pages + unit - 1) / unit, most);
-    run = (n_pages + n - 1) / n;
-    return (n_pages + run - 1) / run;
+    if (n <= 0) return 0;
+    run = shared_div_up(n, max(1, min(want, min(n, most))));
+    return shared_div_up(n, run);
+}
+__device__ __forceinline__ int shared_want(const SharedPlan& p, int n) {
+    return shared_div_up(n, n > p.together ? p.together : p.each);
 }
 __device__ __forceinline__ bool shared_tiled(const SharedArgs& a, const SharedPlan& p, int g) {
     return a.tile_rows > 0 && p.rows[g] >= a.tile_rows && p.pages[g] >= a.tile_pages;
 }
 __device__ __forceinline__ int shared_tiles_of(const SharedArgs& a, const SharedPlan& p, int g) {
-    return shared_tiled(a, p, g) ? (p.rows[g] + 255) / 256 : (p.rows[g] + a.row_tile - 1) / a.row_tile;
+    return shared_tiled(a, p, g) ? (p.rows[g] + 255) / 256 : (p.rows[g] + SH_ROW_TILE - 1) / SH_ROW_TILE;
 }
 __device__ __forceinline__ int shared_cut_group(const SharedArgs& a, const SharedPlan& p, int g, int& run) {
     run = 0;
     if (p.slot[g] < 0) return 0;
-    if (!shared_tiled(a, p, g)) return shared_cut(p.pages[g], p.pages[g] > p.together ? p.together : p.each, a.most_shared, run);
-    const int n = shared_cut((p.pages[g] + 1) / 2, p.stretch, a.most_shared, run);
+    const int n = p.pages[g];
+    if (!shared_tiled(a, p, g)) return shared_cut(n, shared_want(p, n), a.most_shared, run);
+    const int turns = (n + 1) / 2, parts = shared_cut(turns, 1 + (int)((float)turns * p.tile_share), a.most_shared, run);
     run *= 2;
-    return n;
+    return parts;
 }
 __device__ __forceinline__ int shared_cut_own(const SharedArgs& a, const SharedPlan& p, int s, int& run) {
-    return shared_cut(p.own[s], p.own[s] > p.together ? p.together : p.each, a.most_own, run);
+    return shared_cut(p.own[s], shared_want(p, p.own[s]), a.most_own, run);
 }
 
 // By all threads of a block; `room`: shared_plan_ints of shared memory.
 template <int THREADS>
 __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room, int head_dim) {
     constexpr int WARPS = THREADS / 32;
-    __shared__ long long sums_s[WARPS];
+    __shared__ long long sums_s[2][WARPS];
     SharedPlan p;
     p.own = room, p.own_first = p.own + a.n_seqs;
-    p.slot = p.own_first + a.n_seqs, p.least = p.slot + a.n_groups, p.rows = p.least + a.n_groups, p.pages = p.rows + a.n_groups;
-    p.first = p.pages + a.n_groups, p.parts = p.first + a.n_groups;
+    p.slot = p.own_first + a.n_seqs, p.least = p.slot + a.n_groups, p.rows = p.least + a.n_groups, p.begin = p.rows + a.n_groups;
+    p.pages = p.begin + a.n_groups, p.first = p.pages + a.n_groups, p.parts = p.first + a.n_groups;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group_heads = a.n_heads / a.kv_heads;
-    auto block_total = [&](long long v) -> long long {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        __syncthreads();
-        if (lane == 0) sums_s[warp] = v;
-        __syncthreads();
-        long long t = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) t += sums_s[w];
-        return t;
-    };
-    p.own_tiles = (group_heads + a.row_tile - 1) / a.row_tile;
-    long long sum = 0;   // pages x tiles of this thread's items, and (32 bits up) turns of pairs of tiles
+    p.own_tiles = (group_heads + SH_ROW_TILE - 1) / SH_ROW_TILE;
     // (everything is asked for before the first barrier: one round trip)
-    int slot = -1, pos = 0, group = -1, shared = 0, rows = 0, pages = 0;
+    int slot = -1, pos = 0, group = -1, shared = 0, begin = 0, end = 0, pages = 0;
     if (tid < a.n_seqs) slot = a.slots[tid], pos = a.tok_pos[tid], group = a.entry_group[tid], shared = a.entry_pages[tid];
-    if (tid < a.n_groups) rows = (a.begin[tid + 1] - a.begin[tid]) * group_heads, pages = a.pages[tid];
+    if (tid < a.n_groups) begin = a.begin[tid], end = a.begin[tid + 1], pages = a.pages[tid];
     for (int g = tid; g < a.n_groups; g += THREADS) {
-        if (g != tid) rows = (a.begin[g + 1] - a.begin[g]) * group_heads, pages = a.pages[g];
-        p.slot[g] = -1, p.least[g] = 0x7fffffff, p.rows[g] = rows, p.pages[g] = pages;
+        if (g != tid) begin = a.begin[g], end = a.begin[g + 1], pages = a.pages[g];
+        p.slot[g] = -1, p.least[g] = 0x7fffffff, p.rows[g] = (end - begin) * group_heads, p.begin[g] = begin, p.pages[g] = pages;
     }
     if (a.n_groups > 0) __syncthreads();
+    // of this thread's items: pages x tiles, and tiles (32 bits up); turns of pairs of tiles, and pairs
+    long long sum = 0, tile_sum = 0;
     for (int s = tid; s < a.n_seqs; s += THREADS) {
         if (s != tid) slot = a.slots[s], pos = a.tok_pos[s], group = a.entry_group[s], shared = a.entry_pages[s];
         const int n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - shared);
         p.own[s] = n;
-        sum += n * p.own_tiles;
+        sum += n * p.own_tiles + ((long long)(n > 0 ? p.own_tiles : 0) << 32);
         if (slot >= 0 && group >= 0) {
             atomicMax(p.slot + group, slot);
             atomicMin(p.least + group, pos + 1);
@@ -149,42 +161,53 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     }
     if (a.n_groups > 0) __syncthreads();
     for (int g = tid; g < a.n_groups; g += THREADS)
-        if (p.slot[g] >= 0)
-            sum += shared_tiled(a, p, g) ? (long long)((p.pages[g] + 1) / 2 * shared_tiles_of(a, p, g)) << 32 : (long long)(p.pages[g] * shared_tiles_of(a, p, g));
-    sum = block_total(sum);
-    const unsigned work = (unsigned)sum * (unsigned)a.kv_heads;
-    int warps = a.warps;
-    p.stretch = 2;   // turns of a tile record
-    if (a.tile_rows > 0) {
-        const int turns = (int)(sum >> 32) * a.kv_heads;
-        const float tile_time = (float)turns * shared_turn_time(head_dim);
-        const float page_time = (float)work * shared_page_time(head_dim) + (float)min(a.n_seqs * p.own_tiles * a.kv_heads, (int)work) * SH_RECORD_TIME;
-        const int share = work == 0 ? a.sms : min(max((int)((float)a.sms * tile_time / (tile_time + page_time)), 1), a.sms - 1);
-        int records = 0;
-        if (turns > 0) {
-            p.stretch = max(2, (turns + share - 1) / share);
-            for (int round = 0; round < 16; ++round) {   // (cutting into whole turns may give more records than SMs)
-                long long mine = 0;
-                for (int g = tid; g < a.n_groups; g += THREADS)
-                    if (p.slot[g] >= 0 && shared_tiled(a, p, g)) mine += ((p.pages[g] + 1) / 2 + p.stretch - 1) / p.stretch * shared_tiles_of(a, p, g);
-                records = (int)block_total(mine) * a.kv_heads;
-                if (records <= share) break;
-                p.stretch = round == 14 ? 0x3fffffff : (int)max((long long)p.stretch + 1, (long long)p.stretch * records / share);
-            }
+        if (p.slot[g] >= 0 && p.pages[g] > 0) {
+            const int tiles = shared_tiles_of(a, p, g);
+            if (shared_tiled(a, p, g)) tile_sum += (p.pages[g] + 1) / 2 * tiles + ((long long)tiles << 32);
+            else sum += p.pages[g] * tiles + ((long long)tiles << 32);
         }
-        warps = max((int)gridDim.x - records, 1) * WARPS;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), tile_sum += __shfl_xor_sync(0xffffffffu, tile_sum, o);
+    if (lane == 0) sums_s[0][warp] = sum, sums_s[1][warp] = tile_sum;
+    __syncthreads();
+    sum = tile_sum = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += sums_s[0][w], tile_sum += sums_s[1][w];
+    const float work = (float)(unsigned)sum * a.kv_heads, items = (float)(sum >> 32) * a.kv_heads;
+    int warps = a.warps;
+    p.together = 0x3fffffff, p.tile_share = 0.f;
+    if (a.tile_rows > 0) {
+        const float turns = (float)(unsigned)tile_sum * a.kv_heads, pairs = (float)(tile_sum >> 32) * a.kv_heads;
+        const float tile_time = turns * shared_turn_time(head_dim), page_time = work * shared_page_time(head_dim) + items * SH_RECORD_TIME;
+        // (by a little less than the quotient, so that no rounding makes it one record more)
+        const float sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(a.sms * tile_time / (tile_time + page_time)), 1.f), a.sms - 1.f);
+        if (turns > 0.f) p.tile_share = fmaxf(sms - pairs, 0.f) / turns * 0.9999f;
+        warps = (int)fmaxf((float)gridDim.x - fmaxf(sms, pairs), 1.f) * WARPS;
     }
-    p.each = (int)max(1u, (work + warps - 1) / warps);
-    p.together = a.team > 1 ? p.each * SH_TEAM : 0x3fffffff;
-    for (int round = 0; a.tile_rows > 0 && round < 8; ++round) {   // a few records more than warps would take twice the time
-        long long mine = 0;
-        int run;
-        for (int s = tid; s < a.n_seqs; s += THREADS) mine += shared_cut_own(a, p, s, run) * p.own_tiles;
+    p.each = max(1, (int)ceilf(work / (float)warps));
+    if (a.team > 1) p.together = p.each * SH_TEAM;
+    if (a.tile_rows > 0 && items <= (float)warps) {   // records for six sizes at once
+        long long three[2] = {0, 0};
+        auto count = [&](int n, int tiles) {
+#pragma unroll
+            for (int c = 0; c < 6; ++c) three[c / 3] += (long long)(shared_div_up(n, p.each + c) * tiles) << (21 * (c % 3));
+        };
+        for (int s = tid; s < a.n_seqs; s += THREADS) count(p.own[s], p.own_tiles);
         for (int g = tid; g < a.n_groups; g += THREADS)
-            if (!shared_tiled(a, p, g)) mine += shared_cut_group(a, p, g, run) * shared_tiles_of(a, p, g);
-        const long long records = block_total(mine) * a.kv_heads;
-        if (records <= warps || records > 3ll * warps) break;
-        ++p.each;
+            if (p.slot[g] >= 0 && !shared_tiled(a, p, g)) count(p.pages[g], shared_tiles_of(a, p, g));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) three[0] += __shfl_xor_sync(0xffffffffu, three[0], o), three[1] += __shfl_xor_sync(0xffffffffu, three[1], o);
+        __syncthreads();
+        if (lane == 0) sums_s[0][warp] = three[0], sums_s[1][warp] = three[1];
+        __syncthreads();
+        three[0] = three[1] = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) three[0] += sums_s[0][w], three[1] += sums_s[1][w];
+        int larger = 5;
+#pragma unroll
+        for (int c = 4; c >= 0; --c)
+            if ((int)(three[c / 3] >> (21 * (c % 3)) & 0x1fffff) * a.kv_heads <= warps) larger = c;
+        p.each += larger;
     }
     // Where every item's records begin: a prefix sum of three counts at once, 21 bits each: runs for a block, tile records, records for a warp.
     constexpr int BLOCKS = 42, TILES = 21, BITS = (1 << 21) - 1;
@@ -209,13 +232,13 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
             if (lane >= o) upto += t;
         }
         __syncthreads();
-        if (lane == 31) sums_s[warp] = upto;
+        if (lane == 31) sums_s[0][warp] = upto;
         __syncthreads();
         long long at = before + upto - mine;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) at += sums_s[w];
-            before += sums_s[w];
+            if (w < warp) at += sums_s[0][w];
+            before += sums_s[0][w];
         }
         if (s < 0) p.first[i] = (int)(at >> shift) & BITS, p.parts[i] = parts;
         else if (s < a.n_seqs) p.own_first[s] = (int)(at >> shift) & BITS;
@@ -225,25 +248,32 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     return p;
 }
 
-// Records [index, index + N) of a kind (SH_TOGETHER: blocks' runs; SH_NONE, for want of another name: tile records; 0: warps' records) into to[N]; by
-// THREADS threads, this one the `tid`-th, which then synchronise. Records that there are none of are left as they were.
+// A record of a group's, the k-th.
+__device__ __forceinline__ SharedRecord shared_group_record(const SharedArgs& a, const SharedPlan& p, int g, int k, int kind) {
+    int run;
+    shared_cut_group(a, p, g, run);
+    const int chunk = shared_div(k, p.parts[g]), part = k - chunk * p.parts[g];
+    return SharedRecord{SH_PREFIX | kind, g, chunk, p.slot[g], part * run, min((part + 1) * run, p.pages[g]), min(p.least[g], p.pages[g] * QF_PAGE), part,
+                        p.begin[g], p.rows[g], {0, 0}};
+}
+// Tile record `index`, which there is.
+__device__ __forceinline__ SharedRecord shared_tile_record(const SharedArgs& a, const SharedPlan& p, int index) {
+    int g = 0;
+    while (g < a.n_groups - 1 && !(shared_tiled(a, p, g) && index >= p.first[g] && index < p.first[g] + p.parts[g] * shared_tiles_of(a, p, g))) ++g;
+    return shared_group_record(a, p, g, index - p.first[g], 0);
+}
+// Records [index, index + N) of a kind (SH_TOGETHER: blocks' runs; 0: warps' records) into to[N]; by THREADS threads, this one the `tid`-th, which then
+// synchronise. Records that there are none of are left as they were.
 template <int THREADS, int N>
 __device__ __forceinline__ void shared_records(const SharedArgs& a, const SharedPlan& p, int tid, int kind, int index, SharedRecord* to) {
     for (int g = tid; g < a.n_groups; g += THREADS) {
-        const int mine = shared_tiled(a, p, g) ? SH_NONE : p.pages[g] > p.together ? SH_TOGETHER : 0, n = p.parts[g] * shared_tiles_of(a, p, g), first = p.first[g];
+        if (shared_tiled(a, p, g)) continue;
+        const int mine = p.pages[g] > p.together ? SH_TOGETHER : 0, n = p.parts[g] * shared_tiles_of(a, p, g), first = p.first[g];
         if (mine != kind || first >= index + N || first + n <= index) continue;
-        int run;
-        shared_cut_group(a, p, g, run);
 #pragma unroll
-        for (int w = 0; w < N; ++w) {
-            const int k = index + w - first;
-            if (k < 0 || k >= n) continue;
-            const int part = k % p.parts[g];
-            to[w] = SharedRecord{SH_PREFIX | (kind & SH_TOGETHER), g, k / p.parts[g], p.slot[g], part * run, min((part + 1) * run, p.pages[g]),
-                                 min(p.least[g], p.pages[g] * QF_PAGE), part};
-        }
+        for (int w = 0; w < N; ++w)
+            if (index + w >= first && index + w < first + n) to[w] = shared_group_record(a, p, g, index + w - first, kind & SH_TOGETHER);
     }
-    if (kind == SH_NONE) return;
     for (int s = tid; s < a.n_seqs; s += THREADS) {
         const int mine = p.own[s] > p.together ? SH_TOGETHER : 0, first = p.own_first[s];
         if (mine != kind || first >= index + N) continue;
@@ -256,8 +286,8 @@ __device__ __forceinline__ void shared_records(const SharedArgs& a, const Shared
         for (int w = 0; w < N; ++w) {
             const int k = index + w - first;
             if (k < 0 || k >= n) continue;
-            const int part = k % parts;
-            to[w] = SharedRecord{SH_OWN | kind, s, k / parts, slot, from + part * run, from + min((part + 1) * run, p.own[s]), length, shared + part};
+            const int chunk = shared_div(k, parts), part = k - chunk * parts;
+            to[w] = SharedRecord{SH_OWN | kind, s, chunk, slot, from + part * run, from + min((part + 1) * run, p.own[s]), length, shared + part, 0, 0, {0, 0}};
         }
     }
 }
@@ -277,8 +307,8 @@ __device__ __forceinline__ void shared_count_parts(const SharedArgs& a, const Sh
 __device__ __forceinline__ int shared_row(const SharedArgs& a, const SharedRecord& rec, int kv_heads, int kvh, int at) {
     const int G = a.n_heads / kv_heads;
     if (!(rec.kind & SH_PREFIX)) return at < G ? rec.subject * a.n_heads + kvh * G + at : -1;
-    const int i = a.begin[rec.subject] + at / G;
-    return i < a.begin[rec.subject + 1] ? a.members[i] * a.n_heads + kvh * G + at % G : -1;
+    const int i = shared_div(at, G);
+    return at < rec.rows ? a.members[rec.begin + i] * a.n_heads + kvh * G + at - i * G : -1;
 }
 // The keys that the row at a place sees.
 __device__ __forceinline__ int shared_seen(const SharedArgs& a, int place) {
@@ -302,10 +332,19 @@ template <int D> struct SharedSums {
     float o[D / 8][4];       // o[t][0], o[t][1]: row g's columns 2 j E + t and (2 j + 1) E + t; o[t][2], o[t][3]: row g + 8's
     float m0, m1, l0, l1;    // rows g and g + 8: maximum and sum of weights
     int place0, place1;      // where they lie in q
+    bool by_fragment;        // o[t] holds columns 8 t + 2 j and the next of both rows instead
     // 2 E columns of either row side by side
     __device__ __forceinline__ void leave(float* row0, float* row1, float f0, float f1) const {
         constexpr int E = D / 8;
         const int j = threadIdx.x & 3;
+        if (by_fragment) {
+#pragma unroll
+            for (int t = 0; t < E; ++t) {
+                if (row0) *reinterpret_cast<float2*>(row0 + 8 * t + 2 * j) = make_float2(o[t][0] * f0, o[t][1] * f0);
+                if (row1) *reinterpret_cast<float2*>(row1 + 8 * t + 2 * j) = make_float2(o[t][2] * f1, o[t][3] * f1);
+            }
+            return;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -483,6 +522,129 @@ __device__ __forceinline__ void shared_warp(const bf16* __restrict__ q, const Kv
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
     }
     out.m0 = m0, out.m1 = m1, out.l0 = l0, out.l1 = l1;
+    out.by_fragment = false;
+}
+
+// ---- the same work through shared memory, for the warps beside the tiles, of which an SM holds ten with half the registers: stages of 16 keys by 16-byte
+// asynchronous copies, so that what is on its way does not take registers. A row's 16-byte pieces are stored at c XOR (row modulo 8): neither the copies
+// nor ldmatrix meet a bank twice. Fragments as ldmatrix gives them.
+__host__ __device__ constexpr int shared_stages(int d) { return d <= 64 ? 4 : 2; }
+__host__ __device__ constexpr int shared_stage_bytes(int d) { return 2 * 16 * d * 2; }
+
+template <int D>
+__device__ __forceinline__ void shared_warp_staged(const bf16* __restrict__ q, const KvSite<bf16>& site, const SharedArgs& a, const SharedRecord& rec, int kvh,
+                                                   unsigned char* room, SharedSums<D>& out) {
+    constexpr int STAGES = shared_stages(D), BYTES = shared_stage_bytes(D), C = D / 8, KS = D / 16, NT = D / 8, STEPS = QF_PAGE / 16;
+    const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
+    const bool prefix = rec.kind & SH_PREFIX;
+    const int p0 = rec.p_begin, p1 = rec.p_end, bound = prefix ? p1 * QF_PAGE : rec.limit, steps = (min(bound, p1 * QF_PAGE) - p0 * QF_PAGE + 15) / 16;
+    const int* table_row = site.table + (long long)rec.slot * site.table_stride;
+    int table = 0;
+    auto piece = [&](unsigned char* base, int r, int c) { return base + (r * C + (c ^ (r & 7))) * 16; };
+    auto issue = [&](int i) {
+        if (i < steps) {
+            const int n = i / STEPS;
+            if (i % (32 * STEPS) == 0) table = p0 + n + lane < p1 ? __ldg(table_row + p0 + n + lane) : 0;
+            const int page = __shfl_sync(0xffffffffu, table, n & 31);
+            unsigned char* keys = room + i % STAGES * BYTES;
+            if (page < 0 && lane == 0 && i % STEPS == 0) atomicOr(a.err, QF_ERR_NO_PAGE);   // (reported; some held memory is read instead)
+            const bf16* from = site.base + (long long)max(page, 0) * site.page_elems + ((long long)kvh * QF_PAGE + 16 * (i % STEPS)) * D;
+            const bf16* values = from + (long long)kv_heads * QF_PAGE * D;
+#pragma unroll
+            for (int x = lane; x < 16 * C; x += 32) {
+                cp_async_16(piece(keys, x / C, x % C), from + x * 8, true);
+                cp_async_16(piece(keys + BYTES / 2, x / C, x % C), values + x * 8, true);
+            }
+        }
+        cp_async_commit();   // one group per step, empty when there is nothing to fetch
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    const int place0 = out.place0 = shared_row(a, rec, kv_heads, kvh, SH_ROW_TILE * rec.chunk + g);
+    const int place1 = out.place1 = shared_row(a, rec, kv_heads, kvh, SH_ROW_TILE * rec.chunk + g + 8);
+    uint32_t qa[KS][4];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int place = e & 1 ? place1 : place0;
+            qa[ks][e] = place < 0 ? 0u : *reinterpret_cast<const uint32_t*>(q + (size_t)place * D + 16 * ks + 8 * (e >> 1) + 2 * j);
+        }
+    float(&o)[NT][4] = out.o;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    float m0 = QF_NEG_BIG, m1 = QF_NEG_BIG, l0 = 0.f, l1 = 0.f;
+    for (int i = 0; i < steps; ++i) {
+        issue(i + STAGES - 1);
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();   // each lane waited for its own copies; together the stage is complete
+        unsigned char* keys = room + i % STAGES * BYTES;
+        unsigned char* values = keys + BYTES / 2;
+        const int key0 = p0 * QF_PAGE + 16 * i;
+        float s[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint32_t kf[4];
+            ldmatrix_x4(kf, piece(keys, (lane >> 4) * 8 + (lane & 7), 2 * ks + ((lane >> 3) & 1)));
+            mma_bf16_16816(s[0], qa[ks], kf[0], kf[1]);
+            mma_bf16_16816(s[1], qa[ks], kf[2], kf[3]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] *= a.scale_log2;
+        if (key0 + 16 > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
+            const int see0 = prefix ? min(bound, shared_seen(a, place0)) : bound, see1 = prefix ? min(bound, shared_seen(a, place1)) : bound;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key0 + 8 * t + 2 * j + (e & 1) >= (e >> 1 ? see1 : see0)) s[t][e] = QF_NEG_BIG;
+            for (int x = lane; x < 16 * C; x += 32)
+                if (key0 + x / C >= bound) *reinterpret_cast<uint4*>(piece(values, x / C, x % C)) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
+        float top0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), top1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
+        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
+        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+        if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1)) {
+            const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1), c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
+            m0 = n0, m1 = n1;
+            l0 *= c0, l1 *= c1;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t][0] *= c0, o[t][1] *= c0, o[t][2] *= c1, o[t][3] *= c1;
+        }
+        const float from0 = m0 <= QF_NEG_BIG ? 0.f : m0, from1 = m1 <= QF_NEG_BIG ? 0.f : m1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t][0] = fast_exp2(s[t][0] - from0), s[t][1] = fast_exp2(s[t][1] - from0);
+            s[t][2] = fast_exp2(s[t][2] - from1), s[t][3] = fast_exp2(s[t][3] - from1);
+            l0 += s[t][0] + s[t][1];
+            l1 += s[t][2] + s[t][3];
+        }
+        const uint32_t p[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+            uint32_t vf[4];
+            ldmatrix_x4_trans(vf, piece(values, ((lane >> 3) & 1) * 8 + (lane & 7), t + (lane >> 4)));
+            mma_bf16_16816(o[t], p, vf[0], vf[1]);
+            mma_bf16_16816(o[t + 1], p, vf[2], vf[3]);
+        }
+        __syncwarp();   // every lane has read this stage before the copies that come next overwrite it
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    out.m0 = m0, out.m1 = m1, out.l0 = l0, out.l1 = l1;
+    out.by_fragment = true;
 }
 
 // Batches without tiles: blocks of SH_TEAM warps, two an SM.
@@ -754,24 +916,25 @@ static size_t shared_generic_smem(int d, int plan_ints) {
     return (size_t)((SH_ROWS + QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4) + plan_ints) * sizeof(float);
 }
 
-// Where the tiles take over.
+// Where the tiles take over, unless the plan takes more shared memory than the warps beside them leave.
 #define SH_TILE_ROWS 65
 #define SH_TILE_PAGES 8
 
 // What sizes the launches and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of
 // a block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows and pages goes to the tiles (0: there are
-// none); [6]: SMs.
+// none), [7] if the plan takes no more than so many ints (2 a sequence, 7 a group); [6]: SMs.
 QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     const int sms = qf_sm_count();
     if (sms <= 0 || head_dim <= 0 || head_dim > 256) return (int)cudaErrorInvalidValue;
     const bool fast = shared_fast(is_bf16, head_dim);
-    sizes[0] = 16;
+    sizes[0] = SH_ROW_TILE;
     sizes[1] = fast ? 2 * SH_TEAM * sms : 2 * sms;
     sizes[2] = fast ? SH_TEAM : 1;
     sizes[3] = 64;
     sizes[4] = fast && (head_dim == 64 || head_dim == 128) ? SH_TILE_ROWS : 0;
     sizes[5] = SH_TILE_PAGES;
     sizes[6] = sms;
+    sizes[7] = SH_TILE_PLAN_INTS;
     return 0;
 }
 
@@ -813,16 +976,17 @@ QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const i
                                   int most_tiles, int most_shared, int most_own, void* base, const int* table, long long page_elems, int table_stride,
                                   int kv_heads, int head_dim, int n_heads, int n_seqs, float scale, float* part_o, float* part_ml, int* part_n,
                                   const float* sinks, int* err, cudaStream_t stream) {
-    int sizes[7];
+    int sizes[8];
     if (n_seqs <= 0 || n_seqs > SH_MAX_SEQS || n_groups > n_seqs || kv_heads <= 0 || n_heads % kv_heads || most_units <= 0 || most_own <= 0 || most_own > 0x7fff ||
         most_shared > 0xffff || (n_groups > 0 && most_shared <= 0))
         return (int)cudaErrorInvalidValue;
     const int bad = qf_attention_shared_shape(is_bf16, head_dim, sizes);
     if (bad) return bad;
     const SharedArgs a = {tok_pos, slots, entry_pages, entry_group, members, begin, pages, part_o, part_ml, part_n, err, n_seqs, n_groups, n_heads, kv_heads,
-                          most_shared + most_own, most_shared, most_own, sizes[0], sizes[1], most_tiles > 0 ? 1 : sizes[2], most_tiles > 0 ? sizes[4] : 0, sizes[5], sizes[6],
+                          most_shared + most_own, most_shared, most_own, sizes[1], most_tiles > 0 ? 1 : sizes[2], most_tiles > 0 ? sizes[4] : 0, sizes[5], sizes[6],
                           scale * 1.4426950408889634f};
     const bool fast = shared_fast(is_bf16, head_dim);
+    if (most_tiles > 0 && (!fast || shared_plan_ints(n_seqs, n_groups) > SH_TILE_PLAN_INTS)) return (int)cudaErrorInvalidValue;
     const long long all = (long long)most_units * kv_heads * (fast ? 1 : SH_TEAM);
     const int units = (int)(all < 0x7fffffff ? all : 0x7fffffff);
     int code;

@@ -40,45 +40,19 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     constexpr int Q_BYTES = CB * Q_BLOCK, KV_BYTES = CB * KV_BLOCK;
     constexpr uint32_t TMEM_COLS = 512, O_COL = 256;   // S (and P) of tile t in columns 128 t .., O behind them
     constexpr int PRODUCTS = 8, COPIES = 9;            // the issuing warps
-    extern __shared__ __align__(16) unsigned char tc_smem[];
+    extern __shared__ __align__(128) unsigned char tc_smem[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tc_smem) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_s = smem;                          // [2][CB][128][64]
     unsigned char* k_s = q_s + 2 * Q_BYTES;             // [2][CB][128][64]
     unsigned char* v_s = k_s + 2 * KV_BYTES;            // [2][CB][128][64]
     __shared__ __align__(8) uint64_t bar_q, bar_k[2], bar_v[2], bar_k_free[2], bar_v_free[2], bar_s[2], bar_p[2], bar_pv[2], bar_end;
     __shared__ uint32_t tmem_base_s;
-    grid_dependency_wait();
-    const int kv_heads = site.kv_heads, kvh = (int)(blockIdx.x % kv_heads);
     __shared__ SharedRecord record_s[WARPS];
-    const SharedPlan plan = shared_plan<ST_THREADS>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
-    if (blockIdx.x == 0) shared_count_parts<ST_THREADS>(a, plan);
-    const int tile_blocks = plan.tiles * kv_heads;
-    if ((int)blockIdx.x >= tile_blocks) {
-        // ---- the other records, a warp each
-        grid_launch_dependents();
-        const int me = threadIdx.x >> 5, all = ((int)gridDim.x - tile_blocks) * WARPS;
-        uint4* const room = reinterpret_cast<uint4*>(tc_smem + (shared_plan_ints(a.n_seqs, a.n_groups) * 4 + 15) / 16 * 16 + me * shared_query_bytes(D));
-        for (int task = me * ((int)gridDim.x - tile_blocks) + (int)blockIdx.x - tile_blocks; task < plan.singles * kv_heads; task += all) {
-            shared_records<32, 1>(a, plan, threadIdx.x & 31, 0, task / kv_heads, record_s + me);
-            __syncwarp();
-            const SharedRecord rec = record_s[me];
-            __syncwarp();
-            SharedSums<D> x;
-            shared_warp<D, (D <= 64 ? 32 : 16)>(q, site, a, rec, task % kv_heads, room, x);
-            x.leave_part(a, rec.part);
-        }
-        return;
-    }
-    shared_records<ST_THREADS, 1>(a, plan, threadIdx.x, SH_NONE, blockIdx.x / kv_heads, record_s);
-    __syncthreads();
-    const SharedRecord rec = record_s[0];
     const int warp = threadIdx.x >> 5, t = warp < 8 ? warp >> 2 : 0, row = threadIdx.x & 127;   // row threads: tile t, row `row`
-    const int rows = plan.rows[rec.subject] - 2 * ST_BM * rec.chunk;   // from the first tile's on
-    const int tiles = rows > ST_BM ? 2 : 1;
-    const int turns = (rec.p_end - rec.p_begin + 1) / 2, end = rec.p_end * QF_PAGE;   // no key of this run from `end` on
-
+    // Barriers and tensor memory before anything else: beside the end of the kernel before this one. (A block that turns out to have no tile record gives
+    // its tensor memory back unused.)
     if (threadIdx.x == 0) {
-        mbar_init(&bar_q, 4 * tiles);
+        mbar_init(&bar_q, 8);
         mbar_init(&bar_end, 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -95,12 +69,49 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_s)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    fence_to_async();   // (the plan's room is the copies' from here on)
     tc_fence_before();
-    __syncthreads();   // (also: everyone has read what it wants of the plan)
+    __syncthreads();
     tc_fence_after();
-    grid_launch_dependents();   // (the block has its tensor memory)
     const uint32_t tmem = tmem_base_s;
+    grid_launch_dependents();   // (the block has its tensor memory)
+    grid_dependency_wait();
+    const int kv_heads = site.kv_heads, kvh = (int)(blockIdx.x % kv_heads);
+    const SharedPlan plan = shared_plan<ST_THREADS>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
+    if (blockIdx.x == 0) shared_count_parts<ST_THREADS>(a, plan);
+    const int tile_blocks = plan.tiles * kv_heads;
+    if ((int)blockIdx.x >= tile_blocks) {
+        // ---- the other records, a warp each
+        const int all = ((int)gridDim.x - tile_blocks) * WARPS;
+        unsigned char* const room = tc_smem + (shared_plan_ints(a.n_seqs, a.n_groups) * 4 + 127) / 128 * 128 + warp * (shared_stages(D) * shared_stage_bytes(D));
+        for (int task = warp * ((int)gridDim.x - tile_blocks) + (int)blockIdx.x - tile_blocks; task < plan.singles * kv_heads; task += all) {
+            shared_records<32, 1>(a, plan, threadIdx.x & 31, 0, task / kv_heads, record_s + warp);
+            __syncwarp();
+            const SharedRecord rec = record_s[warp];
+            __syncwarp();
+            SharedSums<D> x;
+            shared_warp_staged<D>(q, site, a, rec, task % kv_heads, room, x);
+            x.leave_part(a, rec.part);
+        }
+        tc_fence_before();
+        __syncthreads();
+        if (warp == PRODUCTS)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32  %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+        return;
+    }
+    const SharedRecord rec = shared_tile_record(a, plan, blockIdx.x / kv_heads);
+    const int rows = rec.rows - 2 * ST_BM * rec.chunk;   // from the first tile's on
+    const int tiles = rows > ST_BM ? 2 : 1;
+    const int turns = (rec.p_end - rec.p_begin + 1) / 2, end = rec.p_end * QF_PAGE;   // no key of this run from `end` on
+    // the rows' queries, on their way while the block comes together
+    int place = -1;
+    uint4 query[D / 8];
+    if (warp < PRODUCTS) {
+        if (t < tiles) place = shared_row(a, rec, kv_heads, kvh, 2 * ST_BM * rec.chunk + ST_BM * t + row);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) query[c] = place < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(q + (size_t)place * D)[c];
+    }
+    fence_to_async();   // (the plan's room is the copies' from here on)
+    __syncthreads();    // (everyone has read what it wants of the plan)
     bool timed_out = false;
     // A warp waits as one: the loads and stores of tensor memory and the choice of the issuing lane are collective.
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
@@ -204,19 +215,18 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
         if (leader) umma_commit(&bar_end);   // the block ends when no product of its is at work
         __syncwarp();
         timed_out |= !wait_all(&bar_end, 0);
-    } else if (t < tiles) {
+    } else {
         // ---- the row threads
-        const int place = shared_row(a, rec, kv_heads, kvh, 2 * ST_BM * rec.chunk + ST_BM * t + row);
         {
             unsigned char* to = q_s + t * Q_BYTES + row * 128;
-            const uint4* from = reinterpret_cast<const uint4*>(q + (size_t)(place < 0 ? 0 : place) * D);
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)   // the 128-byte swizzle: 16-byte chunk c of a row of 64 columns lies at c XOR (row modulo 8)
-                *reinterpret_cast<uint4*>(to + c / 8 * Q_BLOCK + ((c % 8) ^ (row & 7)) * 16) = place < 0 ? make_uint4(0, 0, 0, 0) : from[c];
+                *reinterpret_cast<uint4*>(to + c / 8 * Q_BLOCK + ((c % 8) ^ (row & 7)) * 16) = query[c];
             fence_to_async();
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_q);
         }
+        if (t < tiles) {
         const int see = rec.limit >= end ? end : min(end, shared_seen(a, place)), all_see = min(end, rec.limit);
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * t, o_at = lanes + O_COL + 128 * t;
         const float folded = a.scale_log2 > 0.f ? a.scale_log2 : 1.f;
@@ -318,6 +328,7 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
                 __syncwarp();
             }
         }
+        }
     }
     if (timed_out) atomicOr(a.err, QF_ERR_COPY_TIMEOUT);
     tc_fence_before();
@@ -334,9 +345,10 @@ static int launch_tiles(const void* q, KvSite<bf16> site, const SharedArgs& a, i
     // address; copies address rows of held pages only).
     if (!qf_make_map_bf16(&map, site.base, 1ll << 31, D, D, QF_PAGE)) return (int)cudaErrorNotSupported;
     constexpr size_t stages = (size_t)(D / 64) * (2 * ST_BM + 4 * ST_BK) * 128 + 1024;
-    constexpr size_t smem = stages > QF_TMEM_SMEM_ALONE ? stages : (size_t)QF_TMEM_SMEM_ALONE;
-    static_assert(shared_plan_ints(SH_MAX_SEQS, SH_MAX_SEQS) * sizeof(int) + 16 + ST_THREADS / 32 * shared_query_bytes(D) <= smem, "the plan's room, and the queries'");
-    static_assert(qf_tmem_fits(512, smem) && smem <= 227 * 1024, "the rule of tcgen05.cuh");
+    constexpr size_t smem = 226 * 1024;   // (one block an SM in any case)
+    static_assert(SH_TILE_PLAN_INTS * sizeof(int) + 128 + ST_THREADS / 32 * shared_stages(D) * shared_stage_bytes(D) <= smem,
+                  "the plan's room, and the stages of the other records' warps");
+    static_assert(qf_tmem_fits(512, smem) && stages <= smem && smem <= 227 * 1024, "the rule of tcgen05.cuh");
     auto kernel = shared_tiles_kernel<D>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;

@@ -207,11 +207,11 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     held = share.sizes.get((dtype, head_dim, kv_heads, n_heads, own_pages))
     if held is not None:
         return held
-    sizes = (_I * 7)()
+    sizes = (_I * 8)()
     code = _function("attention_shared", "qf_attention_shared_shape", _I, _I, _P)(int(dtype == torch.bfloat16), head_dim, sizes)
     if code:
         raise KernelError(f"attention_shared: CUDA error {code} when asked for its sizes")
-    row_tile, warps, team, most, tile_rows, tile_pages, sms = sizes
+    row_tile, warps, team, most, tile_rows, tile_pages, sms, tile_ints = sizes
     group_heads = n_heads // kv_heads
 
     def parts(pages: int, tiles: int) -> int:
@@ -220,7 +220,7 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     tiles = [-(-len(entries) * group_heads // row_tile) for entries, _ in share.groups]
     most_shared = max((parts(share.bound_pages, t) for t in tiles), default=0)
     pairs = [-(-len(entries) * group_heads // 256) for entries, _ in share.groups if len(entries) * group_heads >= tile_rows]
-    if not tile_rows or share.bound_pages < tile_pages:
+    if not tile_rows or share.bound_pages < tile_pages or 2 * share.n_seqs + 7 * len(share) > tile_ints:
         pairs = []
     if pairs:   # (everything else is cut for single warps then)
         most_shared = max(most_shared, min(most // 4, share.bound_pages))
