@@ -5,14 +5,16 @@
 // running sum over the vocabulary is needed, and a token turns on rounding only where two scores are equal to the last bits.
 // T <= 0: kept while it is the row's argmax (lowest id of equals); the next token is the argmax.
 //
-// Three launches. (1) A block takes VF_CHUNK logits of a row, all of them in registers at once: their maximum, its lowest id, and the sum of the
-// exponentials against it. (2) A block takes an entry: it brings the rows' statistics together (a warp per draft), decides how many drafts stay, and
-// writes all outputs but the token that is drawn. (3) A block takes a chunk of the row that follows and scores its tokens; the block that draws the
-// entry's last ticket picks the best. (At T <= 0 the second launch writes everything.)
-// What bounds it: memory, in (1); in (3), of the same rows out of the second-level cache, the hash and the logarithm of every token.
+// Two launches. (1) A block takes VF_CHUNK logits of a row, all of them in registers at once: their maximum, its lowest id, and the sum of the
+// exponentials against it. (2) Every block of an entry brings its rows' statistics together (a warp per draft) and decides how many drafts stay; one writes
+// what follows. Then they score the tokens of the row behind the kept drafts, chunk after chunk, and the block that draws the entry's last ticket
+// picks the best. (That every block decides for itself costs less than a launch between, and than tickets in (1), which hold its blocks up: 48 entries, 346
+// rows of 151,936: (1) 32 microseconds, with tickets 49.)
+// What bounds it: memory, in (1); in (2), latency, and of the same rows out of the second-level cache the hash and the logarithm of the tokens that may
+// still win.
 //
 // Decisions are whole numbers, so they are made on sums that are good to more than float32: sums over threads and blocks and the comparison u q < p are
-// float64, and of a chunk's scores, formed in float32, those within the error bound of the best are formed again in float64.
+// float64, and of a chunk's scores, formed in float32, those that may be the best by their error bounds are formed again in float64 where there are two or more.
 #include <float.h>
 #include <math.h>
 
@@ -22,15 +24,22 @@
 #define VF_THREADS 256
 #define VF_EACH 32                             // logits of a thread
 #define VF_CHUNK (VF_THREADS * VF_EACH)
-#define VR_THREADS 256
-#define VR_FEW 8                               // tokens of a thread in (3): few where there are few blocks, many else
-#define VR_MANY 32
+#define VR_EACH 8                              // tokens of a thread and chunk in (2)
+#define VR_CHUNK (VF_THREADS * VR_EACH)
+#define VR_BLOCKS 4                            // of an SM at once
 
-// What (2) leaves for (3).
+// What a block has decided.
 struct Decision {
-    int kept, row, d_row, without;   // kept -1: nothing to draw; the rows of target and draft logits (-1: none), the token that is ruled out (-1: none)
-    float t_top, d_top;
+    int kept, row, d_row, without;   // the rows of target and draft logits that a token is drawn from (-1: none), the token that is ruled out (-1: none)
+    float t_top, d_top, t_log, d_log;   // the rows' maxima, and the base-2 logarithms of their sums
     double t_sum, d_sum;
+};
+// The two best of some tokens by the upper bounds of their scores (0x7fffffff: none), and the highest lower bound; none of the bounds is negative.
+struct __align__(16) Contenders {
+    float high[2];
+    int id[2];
+    float low;
+    int pad[3];
 };
 
 struct RowStats {
@@ -52,9 +61,7 @@ struct VerifyArgs {
     int* tokens;
     double* sums;            // [rows + draft rows][chunks]
     float2* tops;            // the same: maximum, its id as bits
-    RowStats* stats;         // [rows + draft rows]
-    Decision* decisions;     // [n]
-    double2* best;           // [n][race chunks]: score, id
+    Contenders* best;        // [n][chunks of (2)]
     int* counters;           // [n]
     int rows, total, vocab, n, most, chunks, race_chunks;
     double inv_t;
@@ -87,9 +94,55 @@ __device__ __forceinline__ void load_logits(const float* x, int begin, int end, 
 }
 __device__ __forceinline__ int id_of(int begin, int i) { return begin + 4 * (threadIdx.x + i / 4 * VF_THREADS) + (i & 3); }
 
+// The statistics of a target row and of the draft row beside it (-1: none, a sum of 1) from their chunks', by one warp: every lane gets them. What the
+// chunks leave is asked for at once; a chunk's factor 2^((its maximum - the row's) rate) is the hardware's, within 2^-22.
+__device__ __forceinline__ void row_stats(const VerifyArgs& a, int row, int d_row, RowStats& t, RowStats& r) {
+    const int lane = threadIdx.x & 31, rows[2] = {row, d_row};
+    float2 mine[2];
+    double part[2] = {0.0, 0.0};
+    RowStats s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const bool in = rows[k] >= 0 && lane < a.chunks;
+        mine[k] = in ? __ldcg(a.tops + (size_t)rows[k] * a.chunks + lane) : make_float2(-INFINITY, __int_as_float(0x7fffffff));
+        if (in && a.sampling) part[k] = __ldcg(a.sums + (size_t)rows[k] * a.chunks + lane);
+        s[k].top = mine[k].x, s[k].id = __float_as_int(mine[k].y);
+        for (int c = lane + 32; rows[k] >= 0 && c < a.chunks; c += 32) {   // (32 chunks are 262,144 logits)
+            const float2 x = __ldcg(a.tops + (size_t)rows[k] * a.chunks + c);
+            if (x.x > s[k].top || (x.x == s[k].top && __float_as_int(x.y) < s[k].id)) s[k].top = x.x, s[k].id = __float_as_int(x.y);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float top = __shfl_xor_sync(0xffffffffu, s[k].top, o);
+            const int id = __shfl_xor_sync(0xffffffffu, s[k].id, o);
+            if (top > s[k].top || (top == s[k].top && id < s[k].id)) s[k].top = top, s[k].id = id;
+        }
+    if (a.sampling) {
+        double sum[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            sum[k] = mine[k].x > -INFINITY ? part[k] * (double)fast_exp2((mine[k].x - s[k].top) * a.rate) : 0.0;
+            for (int c = lane + 32; rows[k] >= 0 && c < a.chunks; c += 32) {
+                const float m = __ldcg(a.tops + (size_t)rows[k] * a.chunks + c).x;
+                if (m > -INFINITY) sum[k] += __ldcg(a.sums + (size_t)rows[k] * a.chunks + c) * (double)fast_exp2((m - s[k].top) * a.rate);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+        s[0].sum = sum[0], s[1].sum = sum[1];
+    }
+    if (d_row < 0) s[1] = RowStats{0.f, 0, 1.0};
+    t = s[0], r = s[1];
+}
+
 // ---- (1) maximum, its lowest id and the sum of exponentials of VF_CHUNK logits of a row. The difference from the maximum, its product with log2(e) / T
 // and that factor itself round by 2^-24 each of an exponent, the hardware's exponential by 2^-22: of single weights, some up and some down.
-__global__ void __launch_bounds__(VF_THREADS)
+__global__ void __launch_bounds__(VF_THREADS, 4)
 verify_rows_kernel(VerifyArgs a) {
     grid_chain_entry();
     __shared__ float top_s[VF_THREADS / 32];
@@ -144,47 +197,14 @@ verify_rows_kernel(VerifyArgs a) {
     }
 }
 
-// A row's statistics from its chunks', by one warp: every lane gets them.
-__device__ __forceinline__ RowStats row_stats(const VerifyArgs& a, int row) {
-    const int lane = threadIdx.x & 31;
-    const float2* tops = a.tops + (size_t)row * a.chunks;
-    const double* sums = a.sums + (size_t)row * a.chunks;
-    RowStats s = {-INFINITY, 0x7fffffff, 0.0};
-    float2 mine = make_float2(-INFINITY, __int_as_float(0x7fffffff));
-    double part = 0.0;
-    if (lane < a.chunks) mine = tops[lane], part = sums[lane];   // (32 chunks are 262,144 logits: the loop below is for vocabularies beyond)
-    s.top = mine.x, s.id = __float_as_int(mine.y);
-    for (int c = lane + 32; c < a.chunks; c += 32) {
-        const float2 t = tops[c];
-        const int id = __float_as_int(t.y);
-        if (t.x > s.top || (t.x == s.top && id < s.id)) s.top = t.x, s.id = id;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float top = __shfl_xor_sync(0xffffffffu, s.top, o);
-        const int id = __shfl_xor_sync(0xffffffffu, s.id, o);
-        if (top > s.top || (top == s.top && id < s.id)) s.top = top, s.id = id;
-    }
-    if (a.sampling) {
-        double sum = mine.x > -INFINITY ? part * exp(((double)mine.x - (double)s.top) * a.inv_t) : 0.0;
-        for (int c = lane + 32; c < a.chunks; c += 32) {
-            const float m = tops[c].x;
-            if (m > -INFINITY) sum += sums[c] * exp(((double)m - (double)s.top) * a.inv_t);
-        }
-        s.sum = warp_sum_f64(sum);
-    }
-    return s;
-}
-
-// ---- (2) how many drafts of an entry stay
-__global__ void __launch_bounds__(VR_THREADS)
-verify_decide_kernel(VerifyArgs a) {
-    grid_chain_entry();
-    constexpr int WARPS = VR_THREADS / 32;
+// ---- (2) how many drafts of an entry stay, by all threads of a block; false: there is nothing to draw.
+__device__ __forceinline__ bool decide(const VerifyArgs& a, int s, bool writes, Decision& made) {
+    constexpr int WARPS = VF_THREADS / 32, CACHE = 32;
     __shared__ int kept_s;
-    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ RowStats t_s[CACHE], r_s[CACHE], last_s[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int before = 0;   // entries with rows in front of this one: each has a row more than it has drafts
-    for (int i = 0; i < s; i += VR_THREADS) {
+    for (int i = 0; i < s; i += VF_THREADS) {
         const int e = i + threadIdx.x;
         before += __syncthreads_count(e < s && a.first[e + 1] > a.first[e]);
     }
@@ -192,12 +212,11 @@ verify_decide_kernel(VerifyArgs a) {
     const bool empty = row1 == row0, wrong = !empty && (row0 < 0 || count < 0 || row1 > a.rows || count > a.most || draft0 < 0 || draft0 + count > a.total);
     int* const tokens = a.tokens + (size_t)s * (a.most + 1);
     if (empty || wrong) {
-        if (threadIdx.x == 0) {
-            a.accepted[s] = wrong ? -1 : 0;
-            a.decisions[s].kept = -1;
+        if (writes) {
+            if (threadIdx.x == 0) a.accepted[s] = wrong ? -1 : 0;
+            for (int i = threadIdx.x; i <= a.most; i += VF_THREADS) tokens[i] = -1;
         }
-        for (int i = threadIdx.x; i <= a.most; i += VR_THREADS) tokens[i] = -1;
-        return;
+        return false;
     }
     if (threadIdx.x == 0) kept_s = count;
     __syncthreads();
@@ -208,9 +227,8 @@ verify_decide_kernel(VerifyArgs a) {
         const double u = a.sampling && j < count ? (double)a.uniforms[draft0 + j] : 0.0;
         const float t_logit = a.sampling && known ? a.target[(row0 + j) * a.t_stride + d] : 0.f;
         const float d_logit = a.draft && known ? a.draft[(draft0 + j) * a.d_stride + d] : 0.f;
-        const RowStats t = row_stats(a, row0 + j);
-        RowStats r = {0.f, 0, 1.0};
-        if (a.draft && j < count) r = row_stats(a, a.rows + draft0 + j);
+        RowStats t, r;
+        row_stats(a, row0 + j, a.draft && j < count ? a.rows + draft0 + j : -1, t, r);
         bool keep = j == count;
         if (!keep && known) {
             if (!a.sampling) {
@@ -222,159 +240,206 @@ verify_decide_kernel(VerifyArgs a) {
             }
         }
         if (lane == 0) {
-            a.stats[row0 + j] = t;
-            if (a.draft && j < count) a.stats[a.rows + draft0 + j] = r;
+            if (j < CACHE) t_s[j] = t, r_s[j] = r;
             if (!keep) atomicMin(&kept_s, j);
         }
     }
     __syncthreads();
     const int kept = kept_s;   // (its row has been worked out: no warp leaves out a row up to the lowest refused one)
-    for (int i = threadIdx.x; i <= a.most; i += VR_THREADS)
-        if (i != kept) tokens[i] = i < kept ? a.drafted[draft0 + i] : -1;
-    if (threadIdx.x == 0) {
-        const RowStats t = a.stats[row0 + kept];
-        const bool refused = kept < count;
-        a.accepted[s] = kept;
-        if (!a.sampling) {
-            tokens[kept] = t.id >= a.vocab ? 0 : t.id;
-            return;
+    const bool refused = kept < count;
+    if (kept >= CACHE) {
+        if (warp == 0) {
+            RowStats t, r;
+            row_stats(a, row0 + kept, refused && a.draft ? a.rows + draft0 + kept : -1, t, r);
+            if (lane == 0) last_s[0] = t, last_s[1] = r;
         }
-        RowStats r = {0.f, 0, 1.0};
-        if (refused && a.draft) r = a.stats[a.rows + draft0 + kept];
-        a.decisions[s] = Decision{kept, row0 + kept, refused && a.draft ? draft0 + kept : -1, refused && !a.draft ? a.drafted[draft0 + kept] : -1,
-                                  t.top, r.top, t.sum, r.sum};
+        __syncthreads();
     }
+    const RowStats t = kept < CACHE ? t_s[kept] : last_s[0], r = kept < CACHE ? r_s[kept] : last_s[1];
+    if (writes) {
+        for (int i = threadIdx.x; i <= a.most; i += VF_THREADS)
+            if (i != kept) tokens[i] = i < kept ? a.drafted[draft0 + i] : -1;
+        if (threadIdx.x == 0) {
+            a.accepted[s] = kept;
+            if (!a.sampling) tokens[kept] = t.id >= a.vocab ? 0 : t.id;
+        }
+    }
+    made = Decision{kept, row0 + kept, refused && a.draft ? draft0 + kept : -1, refused && !a.draft ? a.drafted[draft0 + kept] : -1,
+                    t.top, r.top, __log2f((float)t.sum), __log2f((float)r.sum), t.sum, r.sum};
+    return a.sampling;
 }
 
-// ---- (3) the token behind the kept drafts. A score is r / E. p = 2^((x - top) rate - log2 sum): the difference, the product and the exponent round by
-// 2^-24 each, of numbers that are at most a few tens for any token with a chance, and the hardware's exponential by 2^-22: p is within 6e-6 of its value
-// as a share. E = -ln u: near 1 by its series in w = 1 - u, which is exact in float32, else by the hardware's logarithm, within 6e-6 as well. So a score
-// lies between (p - q - 6e-6 (p + q)) (1 - 6e-6) / E and the same with other signs; of a thread's tokens the two with the highest upper bounds are
-// kept, and whichever of them reach the block's highest lower bound are scored again in float64.
+// ---- (2) the token behind the kept drafts. A score is r / E. p = 2^((x - top) rate - log2 sum): the difference, the product, the logarithm and the
+// exponent round by 2^-24 to 2^-22 each, of numbers that are at most a few tens for any token with a chance, and the hardware's exponential by 2^-22: p is
+// within 6e-6 of its value as a share. E = -ln u: near 1 by its series in w = 1 - u, which is exact in float32, else by the hardware's logarithm, within
+// 6e-6 as well. So a score lies between (p - q - 6e-6 (p + q)) (1 - 6e-6) / E and the same with other signs. A thread, a warp, a block keeps the two
+// tokens with the highest upper bounds, and the highest lower bound of all; of what the blocks leave, the tokens whose upper bound reaches the highest
+// lower bound of all may be the best: mostly one, else they are scored again in float64. (A third token of one block's within 1e-5 of the best is not
+// looked at.) Since E >= w, a token whose upper bound on p - q is below w times the lower bound so far cannot win: most need neither logarithm nor
+// division, and most of the rest no hash.
 #define VR_SLACK 6.0e-6f
-template <int EACH>
-__global__ void __launch_bounds__(VR_THREADS)
+__device__ __forceinline__ void keep_two(Contenders& x, float high, int id) {
+    if (high > x.high[0] || (high == x.high[0] && id < x.id[0])) {
+        x.high[1] = x.high[0], x.id[1] = x.id[0];
+        x.high[0] = high, x.id[0] = id;
+    } else if (high > x.high[1] || (high == x.high[1] && id < x.id[1])) {
+        x.high[1] = high, x.id[1] = id;
+    }
+}
+// Of all threads of a block, to all of them: bounds that are not negative compare as their bits do, which a warp reduces in one instruction.
+__device__ __forceinline__ Contenders of_warp(const Contenders& x) {
+    Contenders y;
+    const unsigned high = __float_as_uint(x.high[0]), most = __reduce_max_sync(0xffffffffu, high);
+    y.high[0] = __uint_as_float(most);
+    y.id[0] = __reduce_min_sync(0xffffffffu, high == most ? x.id[0] : 0x7fffffff);
+    const bool gone = x.id[0] == y.id[0];   // (a lane whose best is the warp's best stands in with its second)
+    const unsigned other = __float_as_uint(gone ? x.high[1] : x.high[0]), second = __reduce_max_sync(0xffffffffu, other);
+    y.high[1] = __uint_as_float(second);
+    y.id[1] = __reduce_min_sync(0xffffffffu, other == second ? (gone ? x.id[1] : x.id[0]) : 0x7fffffff);
+    y.low = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x.low)));
+    return y;
+}
+__device__ __forceinline__ Contenders of_block(const Contenders& x, Contenders* room) {
+    constexpr int WARPS = VF_THREADS / 32;
+    const int lane = threadIdx.x & 31;
+    const Contenders mine = of_warp(x);
+    __syncthreads();
+    if (lane == 0) room[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    Contenders y = {{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    if (lane < WARPS) y = room[lane];
+    return of_warp(y);
+}
+
+__global__ void __launch_bounds__(VF_THREADS, VR_BLOCKS)
 verify_draw_kernel(VerifyArgs a) {
     grid_chain_entry();
-    constexpr int WARPS = VR_THREADS / 32, CHUNK = VR_THREADS * EACH;
-    __shared__ int ticket_s, id_s[WARPS];
-    __shared__ float low_s[WARPS];
-    __shared__ double best_s[WARPS];
+    constexpr int WARPS = VF_THREADS / 32;
+    __shared__ int low_s, ticket_s;
+    __shared__ Contenders best_s[WARPS];
     const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Decision made = a.decisions[s];
-    if (made.kept < 0) return;
+    const long long seq_id = a.sampling ? a.seq_ids[s] : 0;
+    const int step = a.sampling ? a.steps[s] : 0;
+    Decision made;
+    if (!decide(a, s, blockIdx.x == 0, made)) return;
     const float* t_row = a.target + made.row * a.t_stride;
     const float* d_row = made.d_row >= 0 ? a.draft + made.d_row * a.d_stride : nullptr;
-    const int begin = blockIdx.x * CHUNK, end = min(a.vocab, begin + CHUNK);
-    float x[EACH], y[EACH];
-    load_logits(t_row, begin, end, x);
-    if (d_row) load_logits(d_row, begin, end, y);
-    const uint32_t key = row_key(a.seed, a.seq_ids[s], a.steps[s] + made.kept);
-    const float t_log = (float)log2(made.t_sum), d_log = (float)log2(made.d_sum);
-    float high[2] = {-1.f, -1.f}, low = -1.f;
-    int high_at[2] = {-1, -1};
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int id = id_of(begin, i);
-        const float p = fast_exp2(fmaf(x[i] - made.t_top, a.rate, -t_log));
-        const float q = d_row ? fast_exp2(fmaf(y[i] - made.d_top, a.rate, -d_log)) : 0.f;
-        const uint32_t bits = token_bits(key, (uint32_t)id);
-        const float u = ((float)bits + 0.5f) * (1.0f / 8388608.0f), w = ((float)(8388607u - bits) + 0.5f) * (1.0f / 8388608.0f);
-        const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(u);
-        const float r = p - q, slack = (p + q) * VR_SLACK, per = __fdividef(1.f, wait);
-        const bool in = id < end && id != made.without;
-        const float may = in ? fmaf(r, VR_SLACK, r + slack) * per : -1.f;
-        if (in) low = fmaxf(low, (r - slack) * (1.f - VR_SLACK) * per);
-        if (may > high[0]) {
-            high[1] = high[0], high_at[1] = high_at[0];
-            high[0] = may, high_at[0] = i;
-        } else if (may > high[1]) {
-            high[1] = may, high_at[1] = i;
-        }
-    }
-    low = warp_max(fmaxf(low, 0.f));
-    if (lane == 0) low_s[warp] = low;
+    const uint32_t key = row_key(a.seed, seq_id, step + made.kept);
+    if (threadIdx.x == 0) low_s = 0;   // the highest lower bound that a thread has found, as bits of a float32 that is not negative
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) low = fmaxf(low, low_s[w]);
-    double best = -1.0;
-    int best_id = 0x7fffffff;
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-        const float reach = k ? high[1] : high[0];
-        const int i = k ? high_at[1] : high_at[0];
-        if (i < 0 || !(reach >= low)) continue;
-        const int id = id_of(begin, i);
-        double r = exp(((double)t_row[id] - (double)made.t_top) * a.inv_t) / made.t_sum;
-        if (d_row) r = fmax(r - exp(((double)d_row[id] - (double)made.d_top) * a.inv_t) / made.d_sum, 0.0);
-        const double score = r / -log(((double)token_bits(key, (uint32_t)id) + 0.5) / 8388608.0);
-        if (score > best || (score == best && id < best_id)) best = score, best_id = id;
-    }
-    auto better = [](double v, int i, double than, int than_i) { return v > than || (v == than && i < than_i); };
-    auto warp_best = [&]() {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(0xffffffffu, best, o);
-            const int i = __shfl_xor_sync(0xffffffffu, best_id, o);
-            if (better(v, i, best, best_id)) best = v, best_id = i;
-        }
+    Contenders mine = {{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    float x[VR_EACH], y[VR_EACH], x_next[VR_EACH], y_next[VR_EACH];   // (the next chunk's are on their way while this one's are scored)
+    auto load = [&](int begin) {
+        const int end = min(a.vocab, begin + VR_CHUNK);
+        if (begin >= end) return;
+        load_logits(t_row, begin, end, x_next);
+        if (d_row) load_logits(d_row, begin, end, y_next);
     };
-    warp_best();
-    if (lane == 0) best_s[warp] = best, id_s[warp] = best_id;
-    __syncthreads();
-    if (warp != 0) return;
-    best = lane < WARPS ? best_s[lane] : -1.0;
-    best_id = lane < WARPS ? id_s[lane] : 0x7fffffff;
-    warp_best();
-    if (lane == 0) {
-        a.best[(size_t)s * a.race_chunks + blockIdx.x] = make_double2(best, (double)best_id);
+    load(blockIdx.x * VR_CHUNK);
+    for (int begin = blockIdx.x * VR_CHUNK; begin < a.vocab; begin += gridDim.x * VR_CHUNK) {
+        const int end = min(a.vocab, begin + VR_CHUNK);
+#pragma unroll
+        for (int i = 0; i < VR_EACH; ++i) x[i] = x_next[i], y[i] = y_next[i];
+        load(begin + gridDim.x * VR_CHUNK);
+        float low = fmaxf(mine.low, __int_as_float(*(volatile int*)&low_s));
+        const float before = low;
+#pragma unroll
+        for (int i = 0; i < VR_EACH; ++i) {
+            const int id = id_of(begin, i);
+            const float p = fast_exp2(fmaf(x[i] - made.t_top, a.rate, -made.t_log));
+            const float q = d_row ? fast_exp2(fmaf(y[i] - made.d_top, a.rate, -made.d_log)) : 0.f;
+            const float r = p - q, slack = (p + q) * VR_SLACK;
+            if (!(r + slack > low * 5.9e-8f) || id >= end || id == made.without) continue;   // (w is 2^-24 at the least)
+            const uint32_t bits = token_bits(key, (uint32_t)id);
+            const float w = ((float)(8388607u - bits) + 0.5f) * (1.0f / 8388608.0f);
+            if (!(r + slack > low * w)) continue;
+            const float u = ((float)bits + 0.5f) * (1.0f / 8388608.0f);
+            const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(u);
+            const float per = __fdividef(1.f, wait);
+            low = fmaxf(low, (r - slack) * (1.f - VR_SLACK) * per);
+            keep_two(mine, fmaxf(fmaf(r, VR_SLACK, r + slack) * per, 0.f), id);
+        }
+        mine.low = low;
+        if (begin + (int)gridDim.x * VR_CHUNK < a.vocab && __any_sync(0xffffffffu, low > before)) {
+            const float most = warp_max(low);
+            if (lane == 0) atomicMax(&low_s, __float_as_int(most));
+        }
+    }
+    mine = of_block(mine, best_s);
+    Contenders* all = a.best + (size_t)s * a.race_chunks;
+    if (threadIdx.x == 0) {
+        all[blockIdx.x] = mine;
         __threadfence();
         ticket_s = atomicAdd(a.counters + s, 1);
     }
-    __syncwarp();
+    __syncthreads();
     if (ticket_s != (int)gridDim.x - 1) return;
     __threadfence();
-    best = -1.0;
-    best_id = 0x7fffffff;
-    for (int c = lane; c < (int)gridDim.x; c += 32) {
-        const double2 b = __ldcg(a.best + (size_t)s * a.race_chunks + c);
-        if (better(b.x, (int)b.y, best, best_id)) best = b.x, best_id = (int)b.y;
+    // the entry's last block: what the others have left
+    mine = Contenders{{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    for (int c = threadIdx.x; c < (int)gridDim.x; c += VF_THREADS) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(all + c));
+        const float low = __ldcg(&all[c].low);
+        keep_two(mine, x.x, __float_as_int(x.z));
+        keep_two(mine, x.y, __float_as_int(x.w));
+        mine.low = fmaxf(mine.low, low);
     }
-    warp_best();
+    mine = of_block(mine, best_s);
+    if (warp != 0) return;
+    int chosen = mine.id[0];
+    const float low = mine.low;
+    if (mine.high[1] >= low) {   // two or more may be the best
+        double best = -1.0;
+        chosen = 0x7fffffff;
+        for (int c = lane; c < (int)gridDim.x; c += 32)
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+                const int id = __ldcg(&all[c].id[k]);
+                if (!(__ldcg(&all[c].high[k]) >= low) || id >= a.vocab) continue;
+                double r = exp(((double)t_row[id] - (double)made.t_top) * a.inv_t) / made.t_sum;
+                if (d_row) r = fmax(r - exp(((double)d_row[id] - (double)made.d_top) * a.inv_t) / made.d_sum, 0.0);
+                const double score = r / -log(((double)token_bits(key, (uint32_t)id) + 0.5) / 8388608.0);
+                if (score > best || (score == best && id < chosen)) best = score, chosen = id;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const double v = __shfl_xor_sync(0xffffffffu, best, o);
+            const int i = __shfl_xor_sync(0xffffffffu, chosen, o);
+            if (v > best || (v == best && i < chosen)) best = v, chosen = i;
+        }
+    }
     if (lane == 0) {
         a.counters[s] = 0;
-        a.tokens[(size_t)s * (a.most + 1) + made.kept] = best_id >= a.vocab ? 0 : best_id;
+        a.tokens[(size_t)s * (a.most + 1) + made.kept] = chosen >= a.vocab ? 0 : chosen;
     }
 }
 
 // target [rows][t_stride >= vocab] and draft [total][d_stride] (or null) float32; drafted, uniforms [total]; first [n + 1]; accepted [n],
-// tokens [n][most + 1]. Workspaces: sums (8 bytes) and tops (8) of (rows + draft rows) x chunks of VF_CHUNK, stats (16) of rows + draft rows, decisions
-// (40) of n, best (16) of n x chunks of VR_THREADS * VR_FEW, counters int32 of n, zero before the first call (the kernels leave them zero).
+// tokens [n][most + 1]. Workspaces: sums (8 bytes) and tops (8) of (rows + draft rows) x chunks of VF_CHUNK, best (32) of n x chunks of VR_CHUNK,
+// counters int32 of n, zero before the first call (the kernels leave them zero).
 QF_EXPORT int qf_verify_drafts(const float* target, int rows, int vocab, long long t_stride, const float* draft, long long d_stride, const int* drafted,
                                int total, const int* first, int n, const float* uniforms, float temperature, unsigned long long seed,
-                               const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most, double* sums, void* tops, void* stats,
-                               void* decisions, void* best, int* counters, cudaStream_t stream) {
-    static_assert(sizeof(Decision) == 40 && sizeof(RowStats) == 16, "what the workspaces are sized by");
+                               const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most, double* sums, void* tops, void* best,
+                               int* counters, cudaStream_t stream) {
+    static_assert(sizeof(Contenders) == 32, "what the workspaces are sized by");
     if (n <= 0 || vocab <= 0) return 0;
     VerifyArgs a = {};
     a.target = target, a.draft = draft, a.t_stride = t_stride, a.d_stride = d_stride, a.drafted = drafted, a.first = first, a.uniforms = uniforms;
-    a.seq_ids = seq_ids, a.steps = steps, a.accepted = accepted, a.tokens = tokens, a.sums = sums, a.tops = (float2*)tops, a.stats = (RowStats*)stats;
-    a.decisions = (Decision*)decisions, a.best = (double2*)best, a.counters = counters, a.rows = rows, a.total = total, a.vocab = vocab, a.n = n;
+    a.seq_ids = seq_ids, a.steps = steps, a.accepted = accepted, a.tokens = tokens, a.sums = sums, a.tops = (float2*)tops;
+    a.best = (Contenders*)best, a.counters = counters, a.rows = rows, a.total = total, a.vocab = vocab, a.n = n;
     a.most = most, a.seed = seed, a.sampling = temperature > 0.f;
-    a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_THREADS * VR_FEW - 1) / (VR_THREADS * VR_FEW);
+    a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_CHUNK - 1) / VR_CHUNK;
     if (a.sampling) {
         a.inv_t = 1.0 / (double)temperature;
         a.rate = (float)(1.4426950408889634 * a.inv_t);
     }
     const long long all = (long long)rows + (draft ? total : 0);
     if (n > 65535 || all > 65535) return (int)cudaErrorInvalidValue;
-    cudaError_t e = cudaSuccess;
-    if (all > 0) e = launch_pdl(verify_rows_kernel, dim3((unsigned)a.chunks, (unsigned)all), dim3(VF_THREADS), 0, stream, a);
-    if (e == cudaSuccess) e = launch_pdl(verify_decide_kernel, dim3((unsigned)n), dim3(VR_THREADS), 0, stream, a);
-    if (e != cudaSuccess || !a.sampling) return (int)e;
-    // Blocks of 2,048 tokens where they all fit the SMs at once (five to an SM), of 8,192 else.
-    const unsigned many = (unsigned)((vocab + VR_THREADS * VR_MANY - 1) / (VR_THREADS * VR_MANY));
-    if ((long long)a.race_chunks * n <= 5ll * qf_sm_count())
-        return (int)launch_pdl(verify_draw_kernel<VR_FEW>, dim3((unsigned)a.race_chunks, (unsigned)n), dim3(VR_THREADS), 0, stream, a);
-    return (int)launch_pdl(verify_draw_kernel<VR_MANY>, dim3(many, (unsigned)n), dim3(VR_THREADS), 0, stream, a);
+    if (all > 0) {
+        const cudaError_t e = launch_pdl(verify_rows_kernel, dim3((unsigned)a.chunks, (unsigned)all), dim3(VF_THREADS), 0, stream, a);
+        if (e != cudaSuccess) return (int)e;
+    }
+    // as many blocks to an entry as make all of them run at once
+    const int each = a.sampling ? VR_BLOCKS * qf_sm_count() / n : 1;
+    return (int)launch_pdl(verify_draw_kernel, dim3((unsigned)(each < 1 ? 1 : each < a.race_chunks ? each : a.race_chunks), (unsigned)n), dim3(VF_THREADS), 0, stream, a);
 }

@@ -300,7 +300,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
 
 
 # ---------------------------------------------------------------------------------------------------------------- drafts
-VERIFY_CHUNK = 8192        # logits of a block, and tokens of one that draws at the least (VF_CHUNK, VR_THREADS * VR_FEW of the kernels)
+VERIFY_CHUNK = 8192        # logits of a block, and tokens of one that draws at the least (VF_CHUNK, VR_CHUNK of the kernels)
 VERIFY_RACE_CHUNK = 2048
 
 
@@ -311,18 +311,16 @@ class VerifyScratch:
     def __init__(self):
         self.held = self.counters = None   # one buffer of 8-byte words for all but the counters
 
-    def ensure(self, row_chunks: int, rows: int, entry_chunks: int, entries: int, device) -> tuple:
-        """The addresses of sums, tops, stats, decisions and best."""
-        sizes = (row_chunks, row_chunks, 2 * rows, 5 * entries, 2 * entry_chunks)
-        starts = [0]
-        for size in sizes:
-            starts.append(starts[-1] + (size + 1) // 2 * 2)   # (16-byte boundaries)
-        if self.held is None or self.held.numel() < starts[-1] or self.held.device != device:
-            self.held = torch.empty(starts[-1], dtype=torch.float64, device=device)
+    def ensure(self, row_chunks: int, entry_chunks: int, entries: int, device) -> tuple:
+        """The addresses of sums, tops and best."""
+        starts = (0, row_chunks, 2 * row_chunks)   # (sums of 8 bytes, tops of 8; what blocks leave, of 32, begins on 16)
+        need = starts[2] + 4 * entry_chunks
+        if self.held is None or self.held.numel() < need or self.held.device != device:
+            self.held = torch.empty(need, dtype=torch.float64, device=device)
         if self.counters is None or self.counters.numel() < entries or self.counters.device != device:
             self.counters = torch.zeros(entries, dtype=torch.int32, device=device)
         base = self.held.data_ptr()
-        return tuple(base + 8 * start for start in starts[:5])
+        return base, base + 8 * starts[1], base + 8 * starts[2]
 
 
 _verify_scratch = VerifyScratch()
@@ -383,11 +381,10 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     _here("verify_drafts", target, used, drafted, first, uniforms, accepted, tokens)
     all_rows = rows + (total if used is not None else 0)
     scratch = scratch or _verify_scratch
-    places = scratch.ensure(all_rows * -(-vocab // VERIFY_CHUNK), all_rows, n * -(-vocab // VERIFY_RACE_CHUNK), n, target.device)
-    code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P,
-                     _P)(
+    places = scratch.ensure(all_rows * -(-vocab // VERIFY_CHUNK), n * -(-vocab // VERIFY_RACE_CHUNK), n, target.device)
+    code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P)(
         target.data_ptr(), rows, vocab, target.stride(0), _at(used), used.stride(0) if used is not None else 0, drafted.data_ptr(), total,
         first.data_ptr(), n, uniforms.data_ptr(), max(float(temperature), 0.0), int(seed) & 0xFFFFFFFFFFFFFFFF, seq_ids.data_ptr() if sampling else None,
         steps.data_ptr() if sampling else None, accepted.data_ptr(), tokens.data_ptr(), tokens.shape[1] - 1, *places, scratch.counters.data_ptr(), _stream())
-    kernels.launches += 2 if sampling else 1   # (the rows' statistics, the decision, the draw)
+    kernels.launches += all_rows > 0   # (the rows' statistics, and the decision with the draw)
     _check(code, "verify_drafts")
