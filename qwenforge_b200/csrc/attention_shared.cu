@@ -719,131 +719,178 @@ shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a)
 
 #include "attention_shared_tiles.cuh"
 
-// ---- any type and head size: float32 arithmetic. A block takes one run for 16 rows; a page's keys, then its values, in shared memory as float32.
-#define SH_ROWS 16
+// ---- any type and head size: float32 arithmetic. A block takes a record: 16 rows, a page at a time. Keys and values come in registers, all of a page's in
+// flight at once and the next page's while this one's are at work, and go to shared memory as float32 (padded rows: eight keys' 16 bytes meet no bank
+// twice). Thread = (key, every fourth row) for the scores, (row, 4 columns of every 64) for the sums.
+// What bounds it: shared memory's reads, 5 of 16 bytes for 16 multiply-adds in the first product and 5 for 16 in the second; a short run, latency.
+// Measured with the join, float32, head size 64, 14 heads over 2, 12 sequences behind 24 shared pages and one of their own with up to 200 tokens: 20.7 us;
+// with loads a page late and a key's row read once per query instead, 36.6.
+#define SH_ROWS SH_ROW_TILE
 #define SH_THREADS 256
+// 4 columns from c of a row of D as float32: 16 bytes at once where `wide`, zeros behind the row's end.
 template <typename T>
+__device__ __forceinline__ float4 shared_four(const T* row, int c, int D, bool wide) {
+    if constexpr (sizeof(T) == 4)
+        if (wide) return c < D ? __ldg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(c < D ? Num<T>::to_f(row[c]) : 0.f, c + 1 < D ? Num<T>::to_f(row[c + 1]) : 0.f, c + 2 < D ? Num<T>::to_f(row[c + 2]) : 0.f,
+                       c + 3 < D ? Num<T>::to_f(row[c + 3]) : 0.f);
+}
+
+// UNITS: head sizes up to 64 UNITS.
+template <typename T, int UNITS>
 __global__ void __launch_bounds__(SH_THREADS)
-shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs a) {
-    extern __shared__ float fs[];
+shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs a, int wide) {
+    extern __shared__ float4 fs[];
+    constexpr int EACH = 4 * UNITS;               // fours of a row that a thread brings: columns 4 (tid % 4) + 16 i
+    constexpr bool AHEAD = UNITS <= 2;            // beyond, there are no registers for a second page's values
     const int D = site.head_dim, LD = (D + 3) / 4 * 4 + 4;
-    float* q_s = fs;                              // [16][LD]
-    float* kv_s = q_s + SH_ROWS * LD;             // [64][LD]
-    float* p_s = kv_s + QF_PAGE * LD;             // [16][64 + 4]
+    float* q_s = reinterpret_cast<float*>(fs);    // [16][LD]
+    float* k_s = q_s + SH_ROWS * LD;              // [64][LD]
+    float* v_s = k_s + QF_PAGE * LD;              // [64][LD]
+    float* p_s = v_s + QF_PAGE * LD;              // [16][64 + 4]
     __shared__ int row_at[SH_ROWS], row_limit[SH_ROWS];
     __shared__ float m_s[SH_ROWS], l_s[SH_ROWS], corr_s[SH_ROWS];
+    __shared__ SharedRecord record_s;
     grid_launch_dependents();
     grid_dependency_wait();
-    __shared__ SharedRecord record_s;
     const SharedPlan plan = shared_plan<SH_THREADS>(a, reinterpret_cast<int*>(p_s + SH_ROWS * (QF_PAGE + 4)), D);
     if (blockIdx.x == 0) shared_count_parts<SH_THREADS>(a, plan);
     const int kv_heads = site.kv_heads, units = plan.singles * kv_heads, tid = threadIdx.x;
+    const int their_row = tid / 4, their_col = tid % 4 * 4;   // what this thread brings of a page
+    const int key = tid % 64, r0 = tid / 64;                  // its scores: rows r0 + 4 i
+    const int my_row = tid / 16, my_col = tid % 16 * 4;       // its sums: columns my_col + 64 u
+    const long long to_values = (long long)kv_heads * QF_PAGE * D;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {   // (a record is a block's work here)
-    const int kvh = unit % kv_heads;
-    shared_records<SH_THREADS, 1>(a, plan, threadIdx.x, 0, unit / kv_heads, &record_s);
-    __syncthreads();
-    const SharedRecord rec = record_s;
-    const int bound = rec.kind & SH_PREFIX ? rec.p_end * QF_PAGE : rec.limit;
-    if (tid < SH_ROWS) {
-        row_at[tid] = shared_row(a, rec, kv_heads, kvh, SH_ROWS * rec.chunk + tid);
-        row_limit[tid] = min(bound, shared_seen(a, row_at[tid]));
-        m_s[tid] = QF_NEG_BIG;
-        l_s[tid] = 0.f;
-    }
-    __syncthreads();
-    for (int i = tid; i < SH_ROWS * LD; i += SH_THREADS) {
-        const int r = i / LD, c = i % LD;
-        q_s[i] = c < D && row_at[r] >= 0 ? Num<T>::to_f(q[(size_t)row_at[r] * D + c]) : 0.f;
-    }
-    // a thread's outputs: row tid / 16, columns 4 (tid % 16) + 64 u .. + 3
-    constexpr int U = 4;   // head sizes up to 256
-    float4 o[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int my_row = tid / 16, my_col = tid % 16 * 4;
-    auto fetch = [&](const T* from, int n_rows) {   // rows of D into kv_s, zeros behind row n_rows and column D
-        for (int i = tid; i < QF_PAGE * LD; i += SH_THREADS) {
-            const int r = i / LD, c = i % LD;
-            kv_s[i] = r < n_rows && c < D ? Num<T>::to_f(from[(size_t)r * D + c]) : 0.f;
-        }
-    };
-    for (int p = rec.p_begin; p < rec.p_end; ++p) {
-        const int page = site.table[(long long)rec.slot * site.table_stride + p];
-        if (page < 0) {
-            if (tid == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-            continue;
-        }
-        const int key0 = p * QF_PAGE, n_rows = min(QF_PAGE, bound - key0);
-        const T* keys = site.base + (long long)page * site.page_elems + (long long)kvh * QF_PAGE * D;
+        const int kvh = unit % kv_heads;
+        shared_records<SH_THREADS, 1>(a, plan, tid, 0, unit / kv_heads, &record_s);
         __syncthreads();
-        fetch(keys, n_rows);
-        __syncthreads();
-        {   // scores: thread = key tid % 64, rows tid / 64 + 4 i
-            const int key = tid % 64, r0 = tid / 64;
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int c = 0; c < LD - 4; c += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(kv_s + key * LD + c);
+        const SharedRecord rec = record_s;
+        const int bound = rec.kind & SH_PREFIX ? rec.p_end * QF_PAGE : rec.limit;
+        const int* table_row = site.table + (long long)rec.slot * site.table_stride;
+        float4 keys[EACH], values[AHEAD ? EACH : 1];
+        // A row of a page: null where there is none to read (zeros then): behind the run, behind its last key, a page that is not held.
+        auto row_of = [&](int p) -> const T* {
+            if (p >= rec.p_end || p * QF_PAGE + their_row >= bound) return nullptr;
+            const int page = table_row[p];
+            return page < 0 ? nullptr : site.base + (long long)page * site.page_elems + ((long long)kvh * QF_PAGE + their_row) * D;
+        };
+        auto bring = [&](const T* row, float4* to) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 q4 = *reinterpret_cast<const float4*>(q_s + (r0 + 4 * i) * LD + c);
-                    s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+            for (int i = 0; i < EACH; ++i) to[i] = row ? shared_four(row, their_col + 16 * i, D, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        auto put = [&](const float4* from, float* to) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                if (their_col + 16 * i < LD - 4) *reinterpret_cast<float4*>(to + their_row * LD + their_col + 16 * i) = from[i];
+        };
+        const T* row = row_of(rec.p_begin);
+        bring(row, keys);
+        if (AHEAD) bring(row ? row + to_values : nullptr, values);
+        if (tid < SH_ROWS) {
+            row_at[tid] = shared_row(a, rec, kv_heads, kvh, SH_ROWS * rec.chunk + tid);
+            row_limit[tid] = min(bound, shared_seen(a, row_at[tid]));
+            m_s[tid] = QF_NEG_BIG;
+            l_s[tid] = 0.f;
+        }
+        __syncthreads();
+        {
+            const int place = row_at[my_row];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+                if (64 * u + my_col < LD - 4)
+                    *reinterpret_cast<float4*>(q_s + my_row * LD + 64 * u + my_col) =
+                        place < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : shared_four(q + (size_t)place * D, 64 * u + my_col, D, wide);
+        }
+        float4 o[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = rec.p_begin; p < rec.p_end; ++p) {
+            const T* here = row;
+            const bool missing = table_row[p] < 0;
+            if (missing && tid == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+            put(keys, k_s);
+            __syncthreads();
+            row = row_of(p + 1);
+            bring(row, keys);
+            {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < LD - 4; c += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(k_s + key * LD + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 q4 = *reinterpret_cast<const float4*>(q_s + (r0 + 4 * i) * LD + c);
+                        s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    p_s[(r0 + 4 * i) * (QF_PAGE + 4) + key] = !missing && p * QF_PAGE + key < row_limit[r0 + 4 * i] ? s[i] * a.scale_log2 : QF_NEG_BIG;
             }
+            if (AHEAD) put(values, v_s);
+            else {
+                float4 now[AHEAD ? 1 : EACH];
+                bring(here ? here + to_values : nullptr, now);
+                put(now, v_s);
+            }
+            __syncthreads();
+            if (AHEAD) bring(row ? row + to_values : nullptr, values);
+            {   // softmax: 16 lanes a row, four keys each
+                float* p4 = p_s + my_row * (QF_PAGE + 4) + my_col;
+                float4 v = *reinterpret_cast<float4*>(p4);
+                float mx = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p_s[(r0 + 4 * i) * (QF_PAGE + 4) + key] = key0 + key < row_limit[r0 + 4 * i] ? s[i] * a.scale_log2 : QF_NEG_BIG;
+                for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                const float m_old = m_s[my_row], m_new = fmaxf(m_old, mx), from = m_new <= QF_NEG_BIG ? 0.f : m_new;
+                v.x = exp2f(v.x - from), v.y = exp2f(v.y - from), v.z = exp2f(v.z - from), v.w = exp2f(v.w - from);
+                float sum = (v.x + v.y) + (v.z + v.w);
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                *reinterpret_cast<float4*>(p4) = v;
+                __syncwarp();   // (a row's 16 threads are half a warp: nobody else writes or reads its weights)
+                if (tid % 16 == 0) {
+                    const float corr = exp2f(m_old - m_new);
+                    corr_s[my_row] = corr;
+                    m_s[my_row] = m_new;
+                    l_s[my_row] = l_s[my_row] * corr + sum;
+                }
+                __syncwarp();
+            }
+            const float corr = corr_s[my_row];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) o[u].x *= corr, o[u].y *= corr, o[u].z *= corr, o[u].w *= corr;
+#pragma unroll 4
+            for (int k0 = 0; k0 < QF_PAGE; k0 += 4) {   // (rows behind the last key are zeros, and so are their weights)
+                const float4 w4 = *reinterpret_cast<const float4*>(p_s + my_row * (QF_PAGE + 4) + k0);
+                const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u)
+                        if (64 * u + my_col < LD - 4) {
+                            const float4 v = *reinterpret_cast<const float4*>(v_s + (k0 + e) * LD + 64 * u + my_col);
+                            o[u].x = fmaf(w[e], v.x, o[u].x), o[u].y = fmaf(w[e], v.y, o[u].y), o[u].z = fmaf(w[e], v.z, o[u].z), o[u].w = fmaf(w[e], v.w, o[u].w);
+                        }
+            }
         }
-        __syncthreads();
-        fetch(keys + (long long)site.kv_heads * QF_PAGE * D, n_rows);
-        {   // softmax: 16 lanes a row, four keys each
-            float* p4 = p_s + my_row * (QF_PAGE + 4) + my_col;
-            float4 v = *reinterpret_cast<float4*>(p4);
-            float mx = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+        const int place = row_at[my_row];
+        if (place >= 0) {
+            const size_t part = (size_t)place * a.most_parts + rec.part;
 #pragma unroll
-            for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float m_old = m_s[my_row], m_new = fmaxf(m_old, mx), from = m_new <= QF_NEG_BIG ? 0.f : m_new;
-            v.x = exp2f(v.x - from), v.y = exp2f(v.y - from), v.z = exp2f(v.z - from), v.w = exp2f(v.w - from);
-            float sum = (v.x + v.y) + (v.z + v.w);
+            for (int u = 0; u < UNITS; ++u) {
+                const float v[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
+                const int c = 64 * u + my_col;
+                if (D % 4 == 0 && c < D) *reinterpret_cast<float4*>(a.part_o + part * D + c) = o[u];
+                else
 #pragma unroll
-            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            *reinterpret_cast<float4*>(p4) = v;
-            __syncwarp();
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < D) a.part_o[part * D + c + e] = v[e];
+            }
             if (tid % 16 == 0) {
-                const float corr = exp2f(m_old - m_new);
-                corr_s[my_row] = corr;
-                m_s[my_row] = m_new;
-                l_s[my_row] = l_s[my_row] * corr + sum;
+                a.part_ml[part * 2] = m_s[my_row];
+                a.part_ml[part * 2 + 1] = l_s[my_row];
             }
         }
-        __syncthreads();
-        const float corr = corr_s[my_row];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (64 * u + my_col < D) {
-                o[u].x *= corr, o[u].y *= corr, o[u].z *= corr, o[u].w *= corr;
-                for (int k = 0; k < n_rows; ++k) {
-                    const float w = p_s[my_row * (QF_PAGE + 4) + k];
-                    const float4 v = *reinterpret_cast<const float4*>(kv_s + k * LD + 64 * u + my_col);
-                    o[u].x = fmaf(w, v.x, o[u].x), o[u].y = fmaf(w, v.y, o[u].y), o[u].z = fmaf(w, v.z, o[u].z), o[u].w = fmaf(w, v.w, o[u].w);
-                }
-            }
-    }
-    __syncthreads();
-    const int place = row_at[my_row];
-    if (place >= 0) {
-        const size_t part = (size_t)place * a.most_parts + rec.part;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float v[4] = {o[u].x, o[u].y, o[u].z, o[u].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (64 * u + my_col + e < D) a.part_o[part * D + 64 * u + my_col + e] = v[e];
-        }
-        if (tid % 16 == 0) {
-            a.part_ml[part * 2] = m_s[my_row];
-            a.part_ml[part * 2 + 1] = l_s[my_row];
-        }
-    }
-    __syncthreads();   // (the next unit writes these again)
+        __syncthreads();   // (the next unit writes these again)
     }
 }
 
@@ -913,7 +960,7 @@ shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __rest
 static bool shared_fast(int is_bf16, int d) { return is_bf16 && (d == 32 || d == 64 || d == 96 || d == 128); }
 static size_t shared_generic_smem(int d, int plan_ints) {
     const int ld = (d + 3) / 4 * 4 + 4;
-    return (size_t)((SH_ROWS + QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4) + plan_ints) * sizeof(float);
+    return (size_t)((SH_ROWS + 2 * QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4) + plan_ints) * sizeof(float);
 }
 
 // Where the tiles take over, unless the plan takes more shared memory than the warps beside them leave.
@@ -949,15 +996,22 @@ static int launch_parts(const void* q, KvSite<bf16> site, const SharedArgs& a, i
     return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(32 * SH_TEAM), (size_t)smem, stream, (const bf16*)q, site, a);
 }
 
-template <typename T>
+template <typename T, int UNITS>
 static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, int units, cudaStream_t stream) {
     const size_t smem = shared_generic_smem(site.head_dim, shared_plan_ints(a.n_seqs, a.n_groups));
-    auto kernel = shared_parts_generic_kernel<T>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)shared_generic_smem(256, shared_plan_ints(SH_MAX_SEQS, SH_MAX_SEQS)));
+    if (smem > 227 * 1024) return (int)cudaErrorInvalidValue;
+    auto kernel = shared_parts_generic_kernel<T, UNITS>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
     if (e != cudaSuccess) return (int)e;
     const int at_once = 2 * qf_sm_count();
-    return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(SH_THREADS), smem, stream, (const T*)q, site, a);
+    const bool wide = sizeof(T) == 4 && site.head_dim % 4 == 0 && site.page_elems % 4 == 0 && reinterpret_cast<uintptr_t>(site.base) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    return (int)launch_pdl(kernel, dim3((unsigned)(units < at_once ? units : at_once)), dim3(SH_THREADS), smem, stream, (const T*)q, site, a, (int)wide);
+}
+template <typename T>
+static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, int units, cudaStream_t stream) {
+    return site.head_dim <= 64 ? launch_generic<T, 1>(q, site, a, units, stream) : site.head_dim <= 128 ? launch_generic<T, 2>(q, site, a, units, stream)
+                                                                                                        : launch_generic<T, 4>(q, site, a, units, stream);
 }
 
 template <typename T>
