@@ -1,5 +1,5 @@
 // The launches of a prompt step's longest stretches, issued from native code: a norm; queries, keys and values, attention and output
-// projection; gate, up and down; three recurrent mixers whole. The kernels and the library products are those that the Python entries of
+// projection; gate, up and down; three recurrent mixers whole; and the launches for several continuations of one prompt (ops/branches.py). The kernels and the library products are those that the Python entries of
 // ops/kernels.py launch one by one, where a layer of few microseconds a kernel waits for its arguments to be made (a launch 4 to 5
 // microseconds of host time beside 2 to 3 of the driver's own, a buffer 3 to 5; here 3 and 1).
 // Every function looks at its tensors as those entries do and answers None, having done nothing, for what it does not take: the caller then
@@ -10,6 +10,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <climits>
+#include <vector>
 
 namespace {
 
@@ -47,6 +50,11 @@ int (*causal_conv)(int, const void*, int, const float*, const float*, const int*
                    void*, int, int, Stream);
 int (*row_chunks)(const void*, int, const void*, int, const void*, int, const float*, const float*, int, float, const float*, const int*, const int*, int, int,
                   float*, long long, long long, int, int, int, float, float*, long long, int, float*, Stream);
+int (*attention_shared)(int, const void*, void*, const int*, const int*, const int*, const int*, const int*, const int*, const int*, int, int, int, int, int,
+                        void*, const int*, long long, int, int, int, int, int, float, float*, float*, int*, const float*, int*, Stream);
+int (*copy_pages)(void*, int, int, int, long long, long long, int, long long, long long, int, const int*, int, Stream);
+int (*verify_drafts)(const float*, int, int, long long, const float*, long long, const int*, int, const int*, int, const float*, float, unsigned long long,
+                     const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
 PyObject* kernel_error = nullptr;
 
 const struct {
@@ -57,7 +65,8 @@ const struct {
                {"qf_tc_gemm_is_persistent", (void**)&tc_is_persistent}, {"qf_tc_gemm", (void**)&tc_gemm}, {"qf_tc_gemm_tail", (void**)&tc_gemm_tail},
                {"qf_stabilized_gates", (void**)&stabilized_gates}, {"qf_state_chunks", (void**)&state_chunks},
                {"qf_gated_group_norm", (void**)&gated_group_norm}, {"qf_rope_cache_write", (void**)&rope_cache_write}, {"qf_swiglu", (void**)&swiglu},
-               {"qf_causal_conv", (void**)&causal_conv}, {"qf_row_chunks", (void**)&row_chunks}};
+               {"qf_causal_conv", (void**)&causal_conv}, {"qf_row_chunks", (void**)&row_chunks},
+               {"qf_attention_shared", (void**)&attention_shared}, {"qf_copy_pages", (void**)&copy_pages}, {"qf_verify_drafts", (void**)&verify_drafts}};
 
 // setup(KernelError, {name: address}): some of the entries, or more of them later.
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -351,6 +360,145 @@ PyObject* gated_linear_attention(PyObject*, PyObject* const* args, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- several continuations of one prompt: the launches of ops/branches.py, whose checks stand there. These answer the entry's code, None for what they do
+// not take (the caller then checks and launches itself). Host time of a call, microseconds, there / here: attention of two sequences 17 / 7.8, four
+// drafts of one 16 / 6.3, a page forked seven times 10 / 4.1.
+bool on(const at::Tensor* t, at::ScalarType type, int device) { return t && t->is_cuda() && t->scalar_type() == type && t->get_device() == device; }
+bool dense(const at::Tensor* t, at::ScalarType type, int device) { return on(t, type, device) && t->is_contiguous(); }
+template <typename Launch> PyObject* code_of(Launch launch) {
+    int code;
+    {
+        Unlocked without;
+        code = launch();
+    }
+    return PyLong_FromLong(code);
+}
+
+// attention_shared(q, out, cu_q, tok_pos, slots, storage, table, share (five tensors), part_o, part_ml, part_n, sinks or None, err, page_elems, kv_heads,
+//                  head_dim, n_heads, n_seqs, scale, groups, most_pages, units, tiles, most_shared, most_own)
+PyObject* shared_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 29) return PyErr_Format(PyExc_TypeError, "attention_shared: 29 arguments");
+    const at::Tensor* t[17];
+    for (int i = 0; i < 17; ++i) t[i] = tensor(args[i]);
+    const at::Tensor *q = t[0], *out = t[1], *cu = t[2], *pos = t[3], *slots = t[4], *storage = t[5], *table = t[6], *sinks = t[15], *err = t[16];
+    const long long page = number(args[17]), kv = number(args[18]), d = number(args[19]), heads = number(args[20]), seqs = number(args[21]);
+    const double scale = PyFloat_AsDouble(args[22]);
+    const long long groups = number(args[23]), most_pages = number(args[24]), units = number(args[25]), tiles = number(args[26]);
+    const long long shared = number(args[27]), own = number(args[28]);
+    if (PyErr_Occurred()) return nullptr;
+    const int device = c10::cuda::current_device();
+    const at::ScalarType type = q ? q->scalar_type() : at::kInt;
+    bool takes = attention_shared && (type == at::kBFloat16 || type == at::kFloat) && dense(q, type, device) && dense(out, type, device) &&
+                 dense(cu, at::kInt, device) && dense(pos, at::kInt, device) && dense(slots, at::kInt, device) && on(storage, type, device) &&
+                 on(table, at::kInt, device) && dense(err, at::kInt, device) && (args[15] == Py_None || dense(sinks, at::kFloat, device)) &&
+                 on(t[12], at::kFloat, device) && on(t[13], at::kFloat, device) && on(t[14], at::kInt, device);
+    for (int i = 7; takes && i < 12; ++i) takes = on(t[i], at::kInt, device);
+    if (!takes || d <= 0 || d > 256 || kv <= 0 || heads <= 0 || heads % kv || seqs <= 0 || seqs > 2048 || t[7]->numel() != seqs || slots->numel() != seqs ||
+        cu->numel() != seqs + 1 || pos->numel() != seqs || q->dim() != 2 || q->size(0) != seqs || q->size(1) != heads * d || out->sizes() != q->sizes() ||
+        storage->dim() != 5 || storage->size(1) != 2 || storage->size(2) != kv || storage->size(3) != 64 || storage->size(4) != d || page < 2 * kv * 64 * d ||
+        storage->stride(1) != kv * 64 * d || storage->stride(2) != 64 * d || storage->stride(3) != d || storage->stride(4) != 1 || table->dim() != 2 ||
+        table->stride(1) != 1 || most_pages > table->size(1) || (sinks && sinks->numel() != heads) || shared < 0 || own <= 0 || units <= 0 || tiles < 0 ||
+        t[12]->numel() < seqs * heads * (shared + own) * d || t[13]->numel() < seqs * heads * (shared + own) * 2 || t[14]->numel() < seqs ||
+        (type == at::kBFloat16 && (!on16(*q) || !on16(*storage) || page % d)))
+        Py_RETURN_NONE;
+    return code_of([&] {
+        return attention_shared(type == at::kBFloat16, q->data_ptr(), out->data_ptr(), ints(pos), ints(slots), ints(t[7]), ints(t[8]), ints(t[9]), ints(t[10]),
+                                ints(t[11]), (int)groups, (int)units, (int)tiles, (int)shared, (int)own, storage->data_ptr(), ints(table), page,
+                                (int)table->stride(0), (int)kv, (int)d, (int)heads, (int)seqs, (float)scale, at_ptr<float>(*t[12]), at_ptr<float>(*t[13]),
+                                at_ptr<int>(*t[14]), sinks ? sinks->const_data_ptr<float>() : nullptr, at_ptr<int>(*err), stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(target, draft or None, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held, counters, temperature, seed, row_chunks,
+//               entry_chunks): positive temperatures. Chunks: those of a row's statistics, and of a row's race.
+PyObject* drafts_verified(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 15) return PyErr_Format(PyExc_TypeError, "verify_drafts: 15 arguments");
+    const at::Tensor* t[11];
+    for (int i = 0; i < 11; ++i) t[i] = tensor(args[i]);
+    const at::Tensor *target = t[0], *draft = t[1], *drafted = t[2], *first = t[3], *uniforms = t[4], *ids = t[5], *steps = t[6], *accepted = t[7], *tokens = t[8];
+    const double temperature = PyFloat_AsDouble(args[11]);
+    const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[12]);
+    const long long row_chunk = number(args[13]), race_chunk = number(args[14]);
+    if (PyErr_Occurred()) return nullptr;
+    const int device = c10::cuda::current_device();
+    const bool draws = temperature > 0;
+    if (!verify_drafts || !on(target, at::kFloat, device) || (!draft && args[1] != Py_None) || !dense(drafted, at::kInt, device) || !dense(first, at::kInt, device) ||
+        !dense(uniforms, at::kFloat, device) || !dense(accepted, at::kInt, device) || !dense(tokens, at::kInt, device) || !on(t[9], at::kDouble, device) ||
+        !on(t[10], at::kInt, device) || target->dim() != 2 || target->stride(1) != 1 || target->size(1) <= 0 || tokens->dim() != 2 || row_chunk <= 0 || race_chunk <= 0 ||
+        (draws && (!dense(ids, at::kLong, device) || !dense(steps, at::kInt, device))))
+        Py_RETURN_NONE;
+    const long long rows = target->size(0), vocab = target->size(1), entries = accepted->numel(), total = drafted->numel();
+    const bool used = draws && draft && total > 0;
+    if (rows <= 0 || entries <= 0 || first->numel() != entries + 1 || tokens->size(0) != entries || tokens->size(1) < 1 || total < rows - entries ||
+        entries > 65535 || rows + total > 65535 || (draws && (uniforms->numel() != total || ids->numel() != entries || steps->numel() != entries)) ||
+        (draws && draft && (!on(draft, at::kFloat, device) || draft->dim() != 2 || draft->size(0) != total || draft->size(1) != vocab)) ||
+        (used && draft->stride(1) != 1))
+        Py_RETURN_NONE;
+    const long long row_chunks = (rows + (used ? total : 0)) * ((vocab + row_chunk - 1) / row_chunk), races = entries * ((vocab + race_chunk - 1) / race_chunk);
+    if (t[9]->numel() < 2 * row_chunks + 4 * races || t[10]->numel() < entries) Py_RETURN_NONE;
+    double* held = at_ptr<double>(*t[9]);
+    return code_of([&] {
+        return verify_drafts(target->const_data_ptr<float>(), (int)rows, (int)vocab, target->stride(0), used ? draft->const_data_ptr<float>() : nullptr,
+                             used ? draft->stride(0) : 0, ints(drafted), (int)total, ints(first), (int)entries, uniforms->const_data_ptr<float>(),
+                             draws ? (float)temperature : 0.f, seed, draws ? reinterpret_cast<const long long*>(ids->const_data_ptr<int64_t>()) : nullptr,
+                             draws ? ints(steps) : nullptr, at_ptr<int>(*accepted), at_ptr<int>(*tokens), (int)tokens->size(1) - 1, held, held + row_chunks,
+                             held + 2 * row_chunks, at_ptr<int>(*t[10]), stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// copy_pages(storage, moves): a list of tuples of three or two whole numbers.
+PyObject* pages_copied(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) return PyErr_Format(PyExc_TypeError, "copy_pages: 2 arguments");
+    const at::Tensor* storage = tensor(args[0]);
+    if (!copy_pages || !storage || !storage->is_cuda() || storage->get_device() != c10::cuda::current_device() || !PyList_CheckExact(args[1])) Py_RETURN_NONE;
+    const int dims = (int)storage->dim();
+    if (dims < 2) Py_RETURN_NONE;
+    const long long entries = storage->size(0), pages = storage->size(1), item = (long long)storage->element_size();
+    const long long rows = dims >= 4 ? storage->size(dims - 2) : 1, width = dims >= 4 ? storage->size(dims - 1) : dims == 3 ? storage->size(2) : 1;
+    long long page = 1, segments = 1;
+    for (int i = dims - 1; i >= 2; --i) {
+        if (storage->size(i) != 1 && storage->stride(i) != page) Py_RETURN_NONE;
+        page *= storage->size(i);
+        if (i < dims - 2) segments *= storage->size(i);
+    }
+    const long long apart = entries > 1 ? storage->stride(0) : 0, step = pages > 1 ? storage->stride(1) : 0;
+    if (page <= 0 || entries <= 0 || entries > 65535 || pages <= 0 || pages > INT_MAX || rows > INT_MAX || segments > INT_MAX || (pages > 1 && step < page) ||
+        (entries > 1 && apart < page) || (entries > 1 && pages > 1 && apart < (pages - 1) * step + page && step < (entries - 1) * apart + page))
+        Py_RETURN_NONE;
+    const Py_ssize_t count = PyList_GET_SIZE(args[1]);
+    if (count <= 0 || count > 1 << 20) Py_RETURN_NONE;
+    std::vector<int> moves((size_t)count * 3);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        PyObject* move = PyList_GET_ITEM(args[1], i);
+        if (!PyTuple_CheckExact(move)) Py_RETURN_NONE;
+        const Py_ssize_t size = PyTuple_GET_SIZE(move);
+        if ((size != 2 && size != 3) || size != PyTuple_GET_SIZE(PyList_GET_ITEM(args[1], 0))) Py_RETURN_NONE;
+        for (int e = 0; e < 3; ++e) {
+            long long v = rows;
+            int over = 0;
+            if (e < size) {
+                PyObject* o = PyTuple_GET_ITEM(move, e);
+                if (!PyLong_CheckExact(o)) Py_RETURN_NONE;
+                v = PyLong_AsLongLongAndOverflow(o, &over);
+            }
+            if (over || v < INT_MIN || v > INT_MAX) Py_RETURN_NONE;
+            moves[i * 3 + e] = (int)v;
+        }
+    }
+    unsigned char* base = at_ptr<unsigned char>(*storage);
+    const long long row = width * item, low = (long long)reinterpret_cast<uintptr_t>(base) | row | apart * item | step * item;
+    const int unit = !(low & 15) ? 16 : !(low & 3) ? 4 : !(low & 1) ? 2 : 1;
+    return code_of([&] {
+        return copy_pages(base, (int)entries, (int)pages, (int)rows, apart * item, step * item, (int)segments, rows * row, row, unit, moves.data(), (int)count, stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {{"setup", (PyCFunction)(void (*)())setup, METH_FASTCALL, nullptr},
                          {"rms_norm", (PyCFunction)(void (*)())rms_norm, METH_FASTCALL, nullptr},
                          {"prompt_attention", (PyCFunction)(void (*)())prompt_attention, METH_FASTCALL, nullptr},
@@ -358,6 +506,9 @@ PyMethodDef methods[] = {{"setup", (PyCFunction)(void (*)())setup, METH_FASTCALL
                          {"matrix_memory", (PyCFunction)(void (*)())matrix_memory, METH_FASTCALL, nullptr},
                          {"state_space", (PyCFunction)(void (*)())state_space, METH_FASTCALL, nullptr},
                          {"gated_linear_attention", (PyCFunction)(void (*)())gated_linear_attention, METH_FASTCALL, nullptr},
+                         {"attention_shared", (PyCFunction)(void (*)())shared_attention, METH_FASTCALL, nullptr},
+                         {"verify_drafts", (PyCFunction)(void (*)())drafts_verified, METH_FASTCALL, nullptr},
+                         {"copy_pages", (PyCFunction)(void (*)())pages_copied, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

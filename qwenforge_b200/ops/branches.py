@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from ..csrc import library
-from . import kernels
+from . import host, kernels
 from .kernels import KernelError, _check, _dev
 
 PAGE_TOKENS = 64   # positions of a cache page (QF_PAGE of the kernels, and what the cache hands out)
@@ -26,6 +26,15 @@ def _function(lib: str, name: str, *types):
         fn = getattr(library(lib), name)
         fn.argtypes, fn.restype = types, _I
         _functions[name] = fn
+    return fn
+
+
+def _native(name: str, lib: str):
+    """The native function of an entry below. It checks and launches where everything is in order; what it answers None for, the entry checks and launches
+    itself, in Python."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = host.entry(name, lib)
     return fn
 
 
@@ -89,6 +98,13 @@ def copy_pages(storage: torch.Tensor, moves) -> None:
     (a page dense, entries and pages at any distance; a storage of two or three dimensions has pages of one row). moves: (from, to, rows)
     or (from, to) on the host: the first `rows` rows of page `from`, in each of its planes and heads, become those of page `to`; the
     others stay as they are. No page may be the target of two moves, or both a source and a target."""
+    if storage.is_cuda:
+        code = _native("copy_pages", "page_copy")(storage, moves)
+        if code is not None:
+            if code < 0:
+                raise _moves_error(code, storage.shape[1], storage.shape[-2] if storage.dim() >= 4 else 1)
+            kernels.launches += -(-len(moves) // 1024) - 1
+            return _check(code, "copy_pages")
     shape, strides = storage.shape, storage.stride()
     if len(shape) < 2:
         raise KernelError("copy_pages: storage has entries and pages")
@@ -235,6 +251,11 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     return held
 
 
+def _own_pages(max_kv_len: Optional[int], table: torch.Tensor, share: SharedPrefix) -> int:
+    """The most pages that a sequence has to itself."""
+    return max(1, (table.shape[1] if max_kv_len is None else -(-int(max_kv_len) // PAGE_TOKENS)) - share.least_pages)
+
+
 def _batch_refused(cu_q, tok_pos, slots, n_seqs: int, kv_heads: int, n_heads: int, head_dim: int, dtype, share: SharedPrefix) -> None:
     """Raises what is wrong with a batch, its shape or what it shares; returns if nothing is."""
     i32 = torch.int32
@@ -263,6 +284,15 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
     has room for); it sizes the workspaces and the launch. `sinks` (float32 [n_heads]): a logit per head that joins the softmax's denominator
     once, with no key and no value."""
     storage, table, d, kv_heads, dtype = site.storage, site.table, site.head_dim, site.kv_heads, q.dtype
+    if q.is_cuda and table.dim() == 2:
+        sizes = share.sizes.get((dtype, d, kv_heads, n_heads, _own_pages(max_kv_len, table, share)))   # (there from the second call on)
+        if sizes is not None:
+            code = _native("attention_shared", "attention_shared")(
+                q, out, cu_q, tok_pos, slots, storage, table, share.entry_pages, share.entry_group, share.members, share.begin, share.pages, scratch.part_o,
+                scratch.part_ml, scratch.part_n, sinks, err, site.page_elems, kv_heads, d, n_heads, n_seqs, scale, len(share.groups), share.most_pages, *sizes)
+            if code is not None:
+                kernels.launches += 1
+                return _check(code, "attention_shared")
     _batch_refused(cu_q, tok_pos, slots, n_seqs, kv_heads, n_heads, d, dtype, share)
     if not (out.dtype is dtype and storage.dtype is dtype and q.is_contiguous() and out.is_contiguous() and table.dtype is torch.int32
             and err.dtype is torch.int32):
@@ -286,9 +316,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
         if sinks.numel() != n_heads:
             raise KernelError("attention_shared: sinks must hold one float32 per query head")
     _here("attention_shared", q, out, cu_q, tok_pos, slots, storage, table, share.entry_pages, err, sinks)
-    longest = table.shape[1] * PAGE_TOKENS if max_kv_len is None else int(max_kv_len)
-    own_pages = max(1, -(-longest // PAGE_TOKENS) - share.least_pages)
-    units, tiles, most_shared, most_own = _shared_sizes(dtype, d, kv_heads, n_heads, share, own_pages)
+    units, tiles, most_shared, most_own = _shared_sizes(dtype, d, kv_heads, n_heads, share, _own_pages(max_kv_len, table, share))
     scratch.ensure(n_seqs, n_seqs * n_heads * (most_shared + most_own), d)
     code = _function("attention_shared", "qf_attention_shared", _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _LL, _I, _I, _I, _I, _I, _F, _P,
                      _P, _P, _P, _P, _P)(
@@ -344,6 +372,13 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     accepted int32 [n]: drafts kept; tokens int32 [n, most + 1]: kept drafts, the next token, then -1. An entry of no rows gets 0 and
     -1; one whose rows lie outside `target`, or with more drafts than `tokens` has room for, -1 and -1. A drafted id outside the
     vocabulary is refused. Logits are finite or -infinity. `scratch`: as in `sample`."""
+    if target.is_cuda:
+        held = scratch or _verify_scratch
+        code = _native("verify_drafts", "verify_drafts")(target, draft, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held.held, held.counters,
+                                                         temperature, int(seed), VERIFY_CHUNK, VERIFY_RACE_CHUNK)
+        if code is not None:
+            kernels.launches += 1
+            return _check(code, "verify_drafts")
     f32, i32 = torch.float32, torch.int32
     for name, t, dtype in (("target logits", target, f32), ("drafted", drafted, i32), ("first", first, i32), ("uniforms", uniforms, f32), ("accepted", accepted, i32),
                            ("tokens", tokens, i32)):

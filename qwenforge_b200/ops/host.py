@@ -19,7 +19,8 @@ from .linear import linear, linear_rows, own_tensor_core_products, tail_rides
 _ENTRIES = {"norm": ("qf_add_rms_norm",),
             "tc_gemm": ("qf_tc_gemm_qkv_pairs_pays", "qf_tc_gemm_qkv_pairs", "qf_tc_gemm_is_persistent", "qf_tc_gemm", "qf_tc_gemm_tail"),
             "attention_prefill_tc": ("qf_attention_prefill_tc_ex",), "rope_cache": ("qf_rope_cache_write",), "activation": ("qf_swiglu",), "recurrent": ("qf_stabilized_gates", "qf_gated_group_norm", "qf_causal_conv"),
-            "state_chunks": ("qf_state_chunks",), "row_chunks": ("qf_row_chunks",)}
+            "state_chunks": ("qf_state_chunks",), "row_chunks": ("qf_row_chunks",), "attention_shared": ("qf_attention_shared",),
+            "verify_drafts": ("qf_verify_drafts",), "page_copy": ("qf_copy_pages",)}
 _known: set = set()   # libraries whose entries the module has been told
 _module = None
 _OWN = {"linear_rows": linear_rows, "tail_rides": tail_rides}   # (of `ops.linear`'s file)
@@ -54,6 +55,13 @@ def _launch(name: str, launches: int, libraries: tuple, *args) -> Optional[torch
     if out is not None:
         kernels.launches += launches
     return out
+
+
+def entry(name: str, library_name: str):
+    """The native module's function `name`, which launches a kernel of this library and answers its code, or None for what it does not take;
+    a function that takes nothing where the module cannot be had."""
+    module = _host(library_name)
+    return (lambda *args: None) if module is None else getattr(module, name)
 
 
 def rms_norm(hidden: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> Optional[torch.Tensor]:
