@@ -26,7 +26,9 @@
 #define VF_CHUNK (VF_THREADS * VF_EACH)
 #define VR_EACH 8                              // tokens of a thread and chunk in (2)
 #define VR_CHUNK (VF_THREADS * VR_EACH)
-#define VR_BLOCKS 4                            // of an SM at once
+// Blocks of an SM at once. Tokens of a thread / blocks, one entry of four drafts and 48 of up to seven (the kernel's and (1)'s microseconds, vocabulary of
+// 151,936): 8 / 3 11.1 and 53.4; 8 / 4 11.5 and 55.1 (registers spill); 8 / 5 12.0 and 56.9; 4 / 6 11.0 and 57.9; 4 / 8 17.1 and 71.7; 16 / 2 11.8 and 54.0.
+#define VR_BLOCKS 3
 
 // What a block has decided.
 struct Decision {
@@ -275,8 +277,8 @@ __device__ __forceinline__ bool decide(const VerifyArgs& a, int s, bool writes, 
 // 6e-6 as well. So a score lies between (p - q - 6e-6 (p + q)) (1 - 6e-6) / E and the same with other signs. A thread, a warp, a block keeps the two
 // tokens with the highest upper bounds, and the highest lower bound of all; of what the blocks leave, the tokens whose upper bound reaches the highest
 // lower bound of all may be the best: mostly one, else they are scored again in float64. (A third token of one block's within 1e-5 of the best is not
-// looked at.) Since E >= w, a token whose upper bound on p - q is below w times the lower bound so far cannot win: most need neither logarithm nor
-// division, and most of the rest no hash.
+// looked at.) Since E >= w, a token whose upper bound on p - q is below w times the lower bound so far cannot win: nearly none needs a logarithm or a
+// division. The bound goes round a warp after every four tokens of its threads, and round the block after every chunk.
 #define VR_SLACK 6.0e-6f
 __device__ __forceinline__ void keep_two(Contenders& x, float high, int id) {
     if (high > x.high[0] || (high == x.high[0] && id < x.id[0])) {
@@ -344,26 +346,38 @@ verify_draw_kernel(VerifyArgs a) {
         float low = fmaxf(mine.low, __int_as_float(*(volatile int*)&low_s));
         const float before = low;
 #pragma unroll
-        for (int i = 0; i < VR_EACH; ++i) {
-            const int id = id_of(begin, i);
-            const float p = fast_exp2(fmaf(x[i] - made.t_top, a.rate, -made.t_log));
-            const float q = d_row ? fast_exp2(fmaf(y[i] - made.d_top, a.rate, -made.d_log)) : 0.f;
-            const float r = p - q, slack = (p + q) * VR_SLACK;
-            if (!(r + slack > low * 5.9e-8f) || id >= end || id == made.without) continue;   // (w is 2^-24 at the least)
-            const uint32_t bits = token_bits(key, (uint32_t)id);
-            const float w = ((float)(8388607u - bits) + 0.5f) * (1.0f / 8388608.0f);
-            if (!(r + slack > low * w)) continue;
-            const float u = ((float)bits + 0.5f) * (1.0f / 8388608.0f);
-            const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(u);
-            const float per = __fdividef(1.f, wait);
-            low = fmaxf(low, (r - slack) * (1.f - VR_SLACK) * per);
-            keep_two(mine, fmaxf(fmaf(r, VR_SLACK, r + slack) * per, 0.f), id);
+        for (int u = 0; u < VR_EACH; u += 4) {
+            const float reach = __fdividef(8388608.f * 1.000001f, low);   // (of the quotient's rounding, upwards; infinite as long as there is no bound)
+            float r[4], slack[4];
+            uint32_t bits[4];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = fast_exp2(fmaf(x[u + e] - made.t_top, a.rate, -made.t_log));
+                const float q = d_row ? fast_exp2(fmaf(y[u + e] - made.d_top, a.rate, -made.d_log)) : 0.f;
+                r[e] = p - q, slack[e] = (p + q) * VR_SLACK;
+                bits[e] = token_bits(key, (uint32_t)id_of(begin, u + e));
+                // 2^23 w: 23 bits under the exponent of 2^23 are that number more than themselves. (Behind the vocabulary's end: 0 < 0, or a NaN.)
+                r[e] = __uint_as_float(0x4b000000u | (8388607u - bits[e])) - 8388607.5f < (r[e] + slack[e]) * reach ? r[e] : -1.f;
+                any |= r[e] > -1.f;
+            }
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int id = id_of(begin, u + e);
+                    if (!(r[e] > -1.f) || id == made.without) continue;
+                    const float w = ((float)(8388607u - bits[e]) + 0.5f) * (1.0f / 8388608.0f);
+                    const float v = ((float)bits[e] + 0.5f) * (1.0f / 8388608.0f);
+                    const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(v);
+                    const float per = __fdividef(1.f, wait);
+                    low = fmaxf(low, (r[e] - slack[e]) * (1.f - VR_SLACK) * per);
+                    keep_two(mine, fmaxf(fmaf(r[e], VR_SLACK, r[e] + slack[e]) * per, 0.f), id);
+                }
+            }
+            low = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(low)));
         }
         mine.low = low;
-        if (begin + (int)gridDim.x * VR_CHUNK < a.vocab && __any_sync(0xffffffffu, low > before)) {
-            const float most = warp_max(low);
-            if (lane == 0) atomicMax(&low_s, __float_as_int(most));
-        }
+        if (begin + (int)gridDim.x * VR_CHUNK < a.vocab && lane == 0 && low > before) atomicMax(&low_s, __float_as_int(low));
     }
     mine = of_block(mine, best_s);
     Contenders* all = a.best + (size_t)s * a.race_chunks;
