@@ -59,16 +59,18 @@ struct SharedArgs {
     float scale_log2;
 };
 
-// n / d rounded down, and up, for 0 <= n < 2^20 and 0 < d: the quotient in float32 is off by one at most.
-__device__ __forceinline__ int shared_div(int n, int d) {
-    int q = (int)__fdividef((float)n, (float)d);
+// n / d rounded down, and up, for 0 <= n < 2^20 and 0 < d, with one = 1 / d in float32: the product is off by one at most.
+__device__ __forceinline__ int shared_div(int n, int d, float one) {
+    int q = (int)((float)n * one);
     const int r = n - q * d;
     return q + (r < 0 ? -1 : r >= d ? 1 : 0);
 }
-__device__ __forceinline__ int shared_div_up(int n, int d) {
-    const int q = shared_div(n, d);
+__device__ __forceinline__ int shared_div(int n, int d) { return shared_div(n, d, __fdividef(1.f, (float)d)); }
+__device__ __forceinline__ int shared_div_up(int n, int d, float one) {
+    const int q = shared_div(n, d, one);
     return q + (q * d < n);
 }
+__device__ __forceinline__ int shared_div_up(int n, int d) { return shared_div_up(n, d, __fdividef(1.f, (float)d)); }
 
 // ---- the plan. An item is a group's pages or a sequence's own, times its tiles of 16 rows. A group of `tile_rows` rows or more with `tile_pages` pages
 // or more goes to the tensor-core tiles (attention_shared_tiles.cuh): pairs of tiles of 128 rows, every group's pages cut into runs by its share of the
@@ -89,6 +91,7 @@ struct SharedPlan {
     int* first;      // [n_groups] the group's first record of its kind
     int* parts;      // [n_groups]
     int own_tiles, each, together;    // (together: items of more pages are blocks' runs)
+    float one_each;                   // 1 / each
     float tile_share;                 // parts of a tiled group beyond its first, for every turn
     int blocks, singles, tiles;       // records of each kind
 };
@@ -98,15 +101,18 @@ __host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { r
 __device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.8f : 2.1f; }
 __device__ __forceinline__ float shared_page_time(int d) { return d <= 64 ? SH_PAGE_TIME_64 : SH_PAGE_TIME_128; }
 
-// An item of n pages in `want` parts: no more than there is room for, none without a page; run: the pages of each.
-__device__ __forceinline__ int shared_cut(int n, int want, int most, int& run) {
+// An item of n pages: how many parts it is cut into, no more than there is room for, none without a page; run: the pages of each but the last.
+__device__ __forceinline__ int shared_cut(const SharedPlan& p, int n, int most, int& run) {
     run = 0;
     if (n <= 0) return 0;
-    run = shared_div_up(n, max(1, min(want, min(n, most))));
-    return shared_div_up(n, run);
-}
-__device__ __forceinline__ int shared_want(const SharedPlan& p, int n) {
-    return shared_div_up(n, n > p.together ? p.together : p.each);
+    const bool whole = n > p.together;
+    run = whole ? p.together : p.each;
+    int parts = shared_div_up(n, run, whole ? p.one_each * (1.f / SH_TEAM) : p.one_each);
+    if (parts > most) {
+        run = shared_div_up(n, most);
+        parts = shared_div_up(n, run);
+    }
+    return parts;
 }
 __device__ __forceinline__ bool shared_tiled(const SharedArgs& a, const SharedPlan& p, int g) {
     return a.tile_rows > 0 && p.rows[g] >= a.tile_rows && p.pages[g] >= a.tile_pages;
@@ -118,20 +124,23 @@ __device__ __forceinline__ int shared_cut_group(const SharedArgs& a, const Share
     run = 0;
     if (p.slot[g] < 0) return 0;
     const int n = p.pages[g];
-    if (!shared_tiled(a, p, g)) return shared_cut(n, shared_want(p, n), a.most_shared, run);
-    const int turns = (n + 1) / 2, parts = shared_cut(turns, 1 + (int)((float)turns * p.tile_share), a.most_shared, run);
-    run *= 2;
-    return parts;
+    if (!shared_tiled(a, p, g)) return shared_cut(p, n, a.most_shared, run);
+    const int turns = (n + 1) / 2, each = shared_div_up(turns, min(1 + (int)((float)turns * p.tile_share), min(turns, a.most_shared)));
+    run = 2 * each;
+    return shared_div_up(turns, each);
 }
 __device__ __forceinline__ int shared_cut_own(const SharedArgs& a, const SharedPlan& p, int s, int& run) {
-    return shared_cut(p.own[s], shared_want(p, p.own[s]), a.most_own, run);
+    return shared_cut(p, p.own[s], a.most_own, run);
 }
 
 // By all threads of a block; `room`: shared_plan_ints of shared memory.
 template <int THREADS>
 __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room, int head_dim) {
-    constexpr int WARPS = THREADS / 32;
-    __shared__ long long sums_s[2][WARPS];
+    constexpr int WARPS = THREADS / 32, SIZES = 6;
+    constexpr unsigned ALL = 0xffffffffu;
+    __shared__ uint4 sums_s[WARPS];
+    __shared__ int2 counts_s[2][WARPS];
+    __shared__ int records_s[SIZES];
     SharedPlan p;
     p.own = room, p.own_first = p.own + a.n_seqs;
     p.slot = p.own_first + a.n_seqs, p.least = p.slot + a.n_groups, p.rows = p.least + a.n_groups, p.begin = p.rows + a.n_groups;
@@ -147,14 +156,27 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
         p.slot[g] = -1, p.least[g] = 0x7fffffff, p.rows[g] = (end - begin) * group_heads, p.begin[g] = begin, p.pages[g] = pages;
     }
     if (a.n_groups > 0) __syncthreads();
-    // of this thread's items: pages x tiles, and tiles (32 bits up); turns of pairs of tiles, and pairs
-    long long sum = 0, tile_sum = 0;
-    for (int s = tid; s < a.n_seqs; s += THREADS) {
-        if (s != tid) slot = a.slots[s], pos = a.tok_pos[s], group = a.entry_group[s], shared = a.entry_pages[s];
+    uint4 sum = make_uint4(0, 0, 0, 0);   // of this thread's items: pages x tiles, and tiles; turns of pairs of tiles, and pairs
+    for (int s0 = 0; s0 < a.n_seqs; s0 += THREADS) {
+        const int s = s0 + tid;
+        if (s0 > 0) {
+            slot = -1;
+            if (s < a.n_seqs) slot = a.slots[s], pos = a.tok_pos[s], group = a.entry_group[s], shared = a.entry_pages[s];
+        }
         const int n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - shared);
-        p.own[s] = n;
-        sum += n * p.own_tiles + ((long long)(n > 0 ? p.own_tiles : 0) << 32);
-        if (slot >= 0 && group >= 0) {
+        if (s < a.n_seqs) p.own[s] = n;
+        sum.x += n * p.own_tiles, sum.y += n > 0 ? p.own_tiles : 0;
+        const bool member = slot >= 0 && group >= 0;
+        const unsigned members = __ballot_sync(ALL, member);
+        if (members == 0) continue;
+        const int teller = __ffs(members) - 1, first = __shfl_sync(ALL, group, teller);
+        if (__all_sync(ALL, !member || group == first)) {   // (mostly: a warp's members are of one group)
+            const int a_slot = __reduce_max_sync(ALL, member ? slot : -1), least = __reduce_min_sync(ALL, member ? pos + 1 : 0x7fffffff);
+            if (lane == teller) {
+                atomicMax(p.slot + first, a_slot);
+                atomicMin(p.least + first, least);
+            }
+        } else if (member) {
             atomicMax(p.slot + group, slot);
             atomicMin(p.least + group, pos + 1);
         }
@@ -163,21 +185,23 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     for (int g = tid; g < a.n_groups; g += THREADS)
         if (p.slot[g] >= 0 && p.pages[g] > 0) {
             const int tiles = shared_tiles_of(a, p, g);
-            if (shared_tiled(a, p, g)) tile_sum += (p.pages[g] + 1) / 2 * tiles + ((long long)tiles << 32);
-            else sum += p.pages[g] * tiles + ((long long)tiles << 32);
+            if (shared_tiled(a, p, g)) sum.z += (p.pages[g] + 1) / 2 * tiles, sum.w += tiles;
+            else sum.x += p.pages[g] * tiles, sum.y += tiles;
         }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), tile_sum += __shfl_xor_sync(0xffffffffu, tile_sum, o);
-    if (lane == 0) sums_s[0][warp] = sum, sums_s[1][warp] = tile_sum;
+    sum = make_uint4(__reduce_add_sync(ALL, sum.x), __reduce_add_sync(ALL, sum.y), __reduce_add_sync(ALL, sum.z), __reduce_add_sync(ALL, sum.w));
+    if (lane == 0) sums_s[warp] = sum;
     __syncthreads();
-    sum = tile_sum = 0;
+    sum = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) sum += sums_s[0][w], tile_sum += sums_s[1][w];
-    const float work = (float)(unsigned)sum * a.kv_heads, items = (float)(sum >> 32) * a.kv_heads;
+    for (int w = 0; w < WARPS; ++w) {
+        const uint4 x = sums_s[w];
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    const float work = (float)sum.x * a.kv_heads, items = (float)sum.y * a.kv_heads;
     int warps = a.warps;
     p.together = 0x3fffffff, p.tile_share = 0.f;
     if (a.tile_rows > 0) {
-        const float turns = (float)(unsigned)tile_sum * a.kv_heads, pairs = (float)(tile_sum >> 32) * a.kv_heads;
+        const float turns = (float)sum.z * a.kv_heads, pairs = (float)sum.w * a.kv_heads;
         const float tile_time = turns * shared_turn_time(head_dim), page_time = work * shared_page_time(head_dim) + items * SH_RECORD_TIME;
         // (by a little less than the quotient, so that no rounding makes it one record more)
         const float sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(a.sms * tile_time / (tile_time + page_time)), 1.f), a.sms - 1.f);
@@ -186,64 +210,59 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     }
     p.each = max(1, (int)ceilf(work / (float)warps));
     if (a.team > 1) p.together = p.each * SH_TEAM;
-    if (a.tile_rows > 0 && items <= (float)warps) {   // records for six sizes at once
-        long long three[2] = {0, 0};
-        auto count = [&](int n, int tiles) {
-#pragma unroll
-            for (int c = 0; c < 6; ++c) three[c / 3] += (long long)(shared_div_up(n, p.each + c) * tiles) << (21 * (c % 3));
-        };
-        for (int s = tid; s < a.n_seqs; s += THREADS) count(p.own[s], p.own_tiles);
-        for (int g = tid; g < a.n_groups; g += THREADS)
-            if (p.slot[g] >= 0 && !shared_tiled(a, p, g)) count(p.pages[g], shared_tiles_of(a, p, g));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) three[0] += __shfl_xor_sync(0xffffffffu, three[0], o), three[1] += __shfl_xor_sync(0xffffffffu, three[1], o);
+    if (a.tile_rows > 0 && items <= (float)warps) {   // records for some sizes, a warp for each: the first that gives every record a warp
+        for (int c = warp; c < SIZES; c += WARPS) {
+            const int each = p.each + c;
+            const float one = __fdividef(1.f, (float)each);
+            int n = 0;
+            for (int s = lane; s < a.n_seqs; s += 32) n += shared_div_up(p.own[s], each, one) * p.own_tiles;
+            for (int g = lane; g < a.n_groups; g += 32)
+                if (p.slot[g] >= 0 && !shared_tiled(a, p, g)) n += shared_div_up(p.pages[g], each, one) * shared_tiles_of(a, p, g);
+            n = __reduce_add_sync(ALL, n);
+            if (lane == 0) records_s[c] = n;
+        }
         __syncthreads();
-        if (lane == 0) sums_s[0][warp] = three[0], sums_s[1][warp] = three[1];
-        __syncthreads();
-        three[0] = three[1] = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) three[0] += sums_s[0][w], three[1] += sums_s[1][w];
-        int larger = 5;
-#pragma unroll
-        for (int c = 4; c >= 0; --c)
-            if ((int)(three[c / 3] >> (21 * (c % 3)) & 0x1fffff) * a.kv_heads <= warps) larger = c;
+        int larger = 0;
+        while (larger < SIZES - 1 && records_s[larger] * a.kv_heads > warps) ++larger;
         p.each += larger;
     }
-    // Where every item's records begin: a prefix sum of three counts at once, 21 bits each: runs for a block, tile records, records for a warp.
-    constexpr int BLOCKS = 42, TILES = 21, BITS = (1 << 21) - 1;
-    long long before = 0;
+    p.one_each = __fdividef(1.f, (float)p.each);
+    // Where every item's records begin: prefix sums of two counts, records for a warp, and tile records or (there are none of one or the other) blocks' runs.
+    int2 before = make_int2(0, 0);
     for (int i0 = 0; i0 < a.n_groups + a.n_seqs; i0 += THREADS) {
         const int i = i0 + tid, s = i - a.n_groups;
-        int parts = 0, run, shift = 0;
-        long long mine = 0;
+        int run, parts = 0;
+        int2 mine = make_int2(0, 0);
+        bool single = false;
         if (s < 0) {
             parts = shared_cut_group(a, p, i, run);
-            shift = shared_tiled(a, p, i) ? TILES : p.pages[i] > p.together ? BLOCKS : 0;
-            mine = (long long)(parts * shared_tiles_of(a, p, i)) << shift;
+            single = !shared_tiled(a, p, i) && p.pages[i] <= p.together;
+            mine.x = parts * shared_tiles_of(a, p, i);
         } else if (s < a.n_seqs) {
-            parts = shared_cut_own(a, p, s, run);
-            shift = p.own[s] > p.together ? BLOCKS : 0;
-            mine = (long long)(parts * p.own_tiles) << shift;
+            mine.x = shared_cut_own(a, p, s, run) * p.own_tiles;
+            single = p.own[s] <= p.together;
         }
-        long long upto = mine;
+        if (!single) mine = make_int2(0, mine.x);
+        int2 upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += t;
+            const int x = __shfl_up_sync(ALL, upto.x, o), y = __shfl_up_sync(ALL, upto.y, o);
+            if (lane >= o) upto.x += x, upto.y += y;
         }
+        int2* const sums = counts_s[i0 / THREADS & 1];   // (the other half may still be read)
+        if (lane == 31) sums[warp] = upto;
         __syncthreads();
-        if (lane == 31) sums_s[0][warp] = upto;
-        __syncthreads();
-        long long at = before + upto - mine;
+        int2 at = make_int2(before.x + upto.x - mine.x, before.y + upto.y - mine.y);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) at += sums_s[0][w];
-            before += sums_s[0][w];
+            const int2 x = sums[w];
+            if (w < warp) at.x += x.x, at.y += x.y;
+            before.x += x.x, before.y += x.y;
         }
-        if (s < 0) p.first[i] = (int)(at >> shift) & BITS, p.parts[i] = parts;
-        else if (s < a.n_seqs) p.own_first[s] = (int)(at >> shift) & BITS;
+        if (s < 0) p.first[i] = single ? at.x : at.y, p.parts[i] = parts;
+        else if (s < a.n_seqs) p.own_first[s] = single ? at.x : at.y;
     }
-    p.blocks = (int)(before >> BLOCKS) & BITS, p.tiles = (int)(before >> TILES) & BITS, p.singles = (int)before & BITS;
+    p.singles = before.x, p.tiles = a.tile_rows > 0 ? before.y : 0, p.blocks = before.y - p.tiles;
     __syncthreads();
     return p;
 }
