@@ -38,8 +38,9 @@ struct __align__(16) SharedRecord {
 #define SH_MAX_SEQS 2048
 #define SH_TILE_PLAN_INTS 12288
 #define SH_PAGE_TIME_64 0.24f
-#define SH_PAGE_TIME_128 0.4f
+#define SH_PAGE_TIME_128 0.5f
 #define SH_RECORD_TIME 0.35f
+#define SH_TILE_LAG 4.5f
 
 // What every kernel gets.
 struct SharedArgs {
@@ -133,8 +134,9 @@ __device__ __forceinline__ int shared_cut_own(const SharedArgs& a, const SharedP
     return shared_cut(p, p.own[s], a.most_own, run);
 }
 
-// By all threads of a block; `room`: shared_plan_ints of shared memory.
-template <int THREADS>
+// By all threads of a block; `room`: shared_plan_ints of shared memory. TILES: of the kernel with tiles, where a block that gets a tile record needs, and
+// works out, the tile records only (the grid's last block works out everything).
+template <int THREADS, bool TILES>
 __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room, int head_dim) {
     constexpr int WARPS = THREADS / 32, SIZES = 6;
     constexpr unsigned ALL = 0xffffffffu;
@@ -200,17 +202,38 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     const float work = (float)sum.x * a.kv_heads, items = (float)sum.y * a.kv_heads;
     int warps = a.warps;
     p.together = 0x3fffffff, p.tile_share = 0.f;
-    if (a.tile_rows > 0) {
+    p.tiles = 0;
+    if constexpr (TILES) {
         const float turns = (float)sum.z * a.kv_heads, pairs = (float)sum.w * a.kv_heads;
+        // x SMs for the tiles, so that they end with the others: lag + tile_time / x = page_time / (sms - x)
         const float tile_time = turns * shared_turn_time(head_dim), page_time = work * shared_page_time(head_dim) + items * SH_RECORD_TIME;
+        const float half = SH_TILE_LAG * a.sms - tile_time - page_time, x = (half + sqrtf(half * half + 4.f * SH_TILE_LAG * tile_time * a.sms)) / (2.f * SH_TILE_LAG);
         // (by a little less than the quotient, so that no rounding makes it one record more)
-        const float sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(a.sms * tile_time / (tile_time + page_time)), 1.f), a.sms - 1.f);
+        const float sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(x), 1.f), a.sms - 1.f);
         if (turns > 0.f) p.tile_share = fmaxf(sms - pairs, 0.f) / turns * 0.9999f;
         warps = (int)fmaxf((float)gridDim.x - fmaxf(sms, pairs), 1.f) * WARPS;
+        for (int g0 = 0; g0 < a.n_groups; g0 += 32) {   // every warp counts for itself
+            const int g = g0 + lane;
+            int run, parts = 0, mine = 0;
+            const bool tiled = g < a.n_groups && shared_tiled(a, p, g);
+            if (tiled) parts = shared_cut_group(a, p, g, run), mine = parts * shared_tiles_of(a, p, g);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(ALL, upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (tiled && warp == 0) p.first[g] = p.tiles + upto - mine, p.parts[g] = parts;
+            p.tiles += __shfl_sync(ALL, upto, 31);
+        }
+        if ((int)blockIdx.x < p.tiles * a.kv_heads && blockIdx.x != gridDim.x - 1) {
+            __syncthreads();
+            return p;
+        }
     }
     p.each = max(1, (int)ceilf(work / (float)warps));
     if (a.team > 1) p.together = p.each * SH_TEAM;
-    if (a.tile_rows > 0 && items <= (float)warps) {   // records for some sizes, a warp for each: the first that gives every record a warp
+    if (TILES && items <= (float)warps) {   // records for some sizes, a warp for each: the first that gives every record a warp
         for (int c = warp; c < SIZES; c += WARPS) {
             const int each = p.each + c;
             const float one = __fdividef(1.f, (float)each);
@@ -227,17 +250,20 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
         p.each += larger;
     }
     p.one_each = __fdividef(1.f, (float)p.each);
-    // Where every item's records begin: prefix sums of two counts, records for a warp, and tile records or (there are none of one or the other) blocks' runs.
+    // Where the other items' records begin: prefix sums of two counts, records for a warp and blocks' runs.
     int2 before = make_int2(0, 0);
     for (int i0 = 0; i0 < a.n_groups + a.n_seqs; i0 += THREADS) {
         const int i = i0 + tid, s = i - a.n_groups;
         int run, parts = 0;
         int2 mine = make_int2(0, 0);
         bool single = false;
+        const bool tiled = TILES && s < 0 && shared_tiled(a, p, i);
         if (s < 0) {
-            parts = shared_cut_group(a, p, i, run);
-            single = !shared_tiled(a, p, i) && p.pages[i] <= p.together;
-            mine.x = parts * shared_tiles_of(a, p, i);
+            if (!tiled) {
+                parts = shared_cut_group(a, p, i, run);
+                single = p.pages[i] <= p.together;
+                mine.x = parts * ((p.rows[i] + SH_ROW_TILE - 1) / SH_ROW_TILE);
+            }
         } else if (s < a.n_seqs) {
             mine.x = shared_cut_own(a, p, s, run) * p.own_tiles;
             single = p.own[s] <= p.together;
@@ -259,10 +285,11 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
             if (w < warp) at.x += x.x, at.y += x.y;
             before.x += x.x, before.y += x.y;
         }
-        if (s < 0) p.first[i] = single ? at.x : at.y, p.parts[i] = parts;
-        else if (s < a.n_seqs) p.own_first[s] = single ? at.x : at.y;
+        if (s < 0) {
+            if (!tiled) p.first[i] = single ? at.x : at.y, p.parts[i] = parts;
+        } else if (s < a.n_seqs) p.own_first[s] = single ? at.x : at.y;
     }
-    p.singles = before.x, p.tiles = a.tile_rows > 0 ? before.y : 0, p.blocks = before.y - p.tiles;
+    p.singles = before.x, p.blocks = before.y;
     __syncthreads();
     return p;
 }
@@ -311,7 +338,7 @@ __device__ __forceinline__ void shared_records(const SharedArgs& a, const Shared
     }
 }
 
-// How many parts every row has, for whoever joins them: by the first block of the parts' kernel.
+// How many parts every row has, for whoever joins them: by one block of the parts' kernel.
 template <int THREADS>
 __device__ __forceinline__ void shared_count_parts(const SharedArgs& a, const SharedPlan& p) {
     for (int s = threadIdx.x; s < a.n_seqs; s += THREADS) {
@@ -679,7 +706,7 @@ shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
     grid_launch_dependents();
     grid_dependency_wait();
-    const SharedPlan plan = shared_plan<THREADS>(a, plan_s, D);
+    const SharedPlan plan = shared_plan<THREADS, false>(a, plan_s, D);
     if (blockIdx.x == 0) shared_count_parts<THREADS>(a, plan);
     const int units = (plan.blocks + (plan.singles + SH_TEAM - 1) / SH_TEAM) * kv_heads;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -772,7 +799,7 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     __shared__ SharedRecord record_s;
     grid_launch_dependents();
     grid_dependency_wait();
-    const SharedPlan plan = shared_plan<SH_THREADS>(a, reinterpret_cast<int*>(p_s + SH_ROWS * (QF_PAGE + 4)), D);
+    const SharedPlan plan = shared_plan<SH_THREADS, false>(a, reinterpret_cast<int*>(p_s + SH_ROWS * (QF_PAGE + 4)), D);
     if (blockIdx.x == 0) shared_count_parts<SH_THREADS>(a, plan);
     const int kv_heads = site.kv_heads, units = plan.singles * kv_heads, tid = threadIdx.x;
     const int their_row = tid / 4, their_col = tid % 4 * 4;   // what this thread brings of a page
@@ -913,59 +940,75 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     }
 }
 
-// ---- the parts of a row come together: a thread per V neighbouring output elements, eight parts on their way at once
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
+// ---- the parts of a row come together: V neighbouring output elements are a lane's, and of their parts every SPLIT-th, eight on their way at once.
+// (No shared memory: the tiles' kernel behind, which wants all of it, may start its blocks beside these.)
+// SPLIT 4 up to 256 elements' lanes an SM, else 2. The operator with 4 / 2 / 1, microseconds: 8 sequences, 14 heads of 64 11.2 / 12.2 / 12.8; 48, 16 heads of
+// 128 18.2 / 19.6 / 22.0; beyond that, 64, 28 heads of 128 28.4 / 27.2 / 28.8; 250, 14 heads of 64 37.4 / 36.4 / 38.1 (the next call's blocks find room later).
+// What bounds it: the latency of three dependent loads and a launch behind the parts; beyond some thousand rows, their bytes.
+#define SH_JOIN 128   // threads of a block
+template <typename T, int V, int SPLIT>
+__global__ void __launch_bounds__(SH_JOIN)
 shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __restrict__ sinks) {
+    constexpr int COLUMNS = 32 / SPLIT;
     grid_launch_dependents();
+    const int split = (threadIdx.x & 31) / COLUMNS, entry = blockIdx.y, per = D / V, i = blockIdx.x * (SH_JOIN / SPLIT) + threadIdx.x / 32 * COLUMNS + threadIdx.x % COLUMNS;
+    const int head = (int)((unsigned)i / (unsigned)per), d = (i - head * per) * V, row = entry * a.n_heads + head;
+    const bool there = head < a.n_heads;
     grid_dependency_wait();
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int per = D / V;
-    if (i >= (long long)a.n_seqs * a.n_heads * per) return;
-    const int row = (int)(i / per), d = (int)(i % per) * V, entry = row / a.n_heads;
-    const int packed = a.part_n[entry], runs = (packed & 0xffff) + (packed >> 16);
+    const int packed = there ? a.part_n[entry] : 0, runs = (packed & 0xffff) + (packed >> 16);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.most_parts;
     const float* po = a.part_o + (size_t)row * a.most_parts * D + d;
     float top = QF_NEG_BIG, den = 0.f, num[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) num[e] = 0.f;
-    for (int k0 = 0; k0 < runs; k0 += 8) {
+    for (int k0 = split; k0 < runs; k0 += 8 * SPLIT) {
         float2 x[8];
         float o[8][V];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const bool in = k0 + k < runs;
-            x[k] = in ? ml[k0 + k] : make_float2(QF_NEG_BIG, 0.f);
+            const int part = k0 + k * SPLIT;
+            const bool in = part < runs;
+            x[k] = in ? ml[part] : make_float2(QF_NEG_BIG, 0.f);
             if constexpr (V == 4) {
-                const float4 v = in ? *reinterpret_cast<const float4*>(po + (size_t)(k0 + k) * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 v = in ? *reinterpret_cast<const float4*>(po + (size_t)part * D) : make_float4(0.f, 0.f, 0.f, 0.f);
                 o[k][0] = v.x, o[k][1] = v.y, o[k][2] = v.z, o[k][3] = v.w;
             } else {
-                o[k][0] = in ? po[(size_t)(k0 + k) * D] : 0.f;
+                o[k][0] = in ? po[(size_t)part * D] : 0.f;
             }
         }
         float m = top;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, x[k].x);
-        const float keep = exp2f(top - m);
+        const float keep = fast_exp2(top - m);
         den *= keep;
 #pragma unroll
         for (int e = 0; e < V; ++e) num[e] *= keep;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float w = exp2f(x[k].x - m);
+            const float w = fast_exp2(x[k].x - m);
             den = fmaf(w, x[k].y, den);
 #pragma unroll
             for (int e = 0; e < V; ++e) num[e] = fmaf(w, o[k][e], num[e]);
         }
         top = m;
     }
-    float keep = 1.f;
-    if (sinks && runs > 0) {   // a logit that joins the sum of weights once, with no key and no value
-        const float s2 = sinks[row % a.n_heads] * 1.4426950408889634f, m = fmaxf(top, s2);
-        keep = exp2f(top - m);
-        den = den * keep + exp2f(s2 - m);
+    const float s2 = sinks && runs > 0 ? sinks[head] * 1.4426950408889634f : -INFINITY;   // a logit that joins the sum of weights once, with no key and no value
+    float all = fmaxf(top, s2);
+#pragma unroll
+    for (int o = COLUMNS; o < 32; o <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    const float f = fast_exp2(top - all);
+    den *= f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) num[e] *= f;
+#pragma unroll
+    for (int o = COLUMNS; o < 32; o <<= 1) {
+        den += __shfl_xor_sync(0xffffffffu, den, o);
+#pragma unroll
+        for (int e = 0; e < V; ++e) num[e] += __shfl_xor_sync(0xffffffffu, num[e], o);
     }
-    const float inv = den > 0.f ? keep / den : 0.f;
+    if (split != 0 || !there) return;
+    den += fast_exp2(s2 - all);
+    const float inv = den > 0.f ? 1.f / den : 0.f;
     T* to = out + (size_t)row * D + d;
     if constexpr (V == 4 && sizeof(T) == 2)
         *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
@@ -1033,12 +1076,17 @@ static int launch_generic(const void* q, KvSite<T> site, const SharedArgs& a, in
                                                                                                         : launch_generic<T, 4>(q, site, a, units, stream);
 }
 
+template <typename T, int V, int SPLIT>
+static int launch_join(const SharedArgs& a, int head_dim, void* out, const float* sinks, cudaStream_t stream) {
+    const long long items = (long long)a.n_heads * (head_dim / V);
+    const dim3 grid((unsigned)((items * SPLIT + SH_JOIN - 1) / SH_JOIN), (unsigned)a.n_seqs);
+    return (int)launch_pdl(shared_join_kernel<T, V, SPLIT>, grid, dim3(SH_JOIN), 0, stream, a, head_dim, (T*)out, sinks);
+}
 template <typename T>
 static int launch_join(const SharedArgs& a, int head_dim, void* out, const float* sinks, cudaStream_t stream) {
-    const long long items = (long long)a.n_seqs * a.n_heads * head_dim;
-    if (head_dim % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
-        return (int)launch_pdl(shared_join_kernel<T, 4>, dim3((unsigned)((items / 4 + 255) / 256)), dim3(256), 0, stream, a, head_dim, (T*)out, sinks);
-    return (int)launch_pdl(shared_join_kernel<T, 1>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a, head_dim, (T*)out, sinks);
+    if (head_dim % 4 || (reinterpret_cast<uintptr_t>(out) & 15)) return launch_join<T, 1, 1>(a, head_dim, out, sinks, stream);
+    const bool few = (long long)a.n_seqs * a.n_heads * head_dim / 4 <= 256ll * a.sms;
+    return few ? launch_join<T, 4, 4>(a, head_dim, out, sinks, stream) : launch_join<T, 4, 2>(a, head_dim, out, sinks, stream);
 }
 
 // `most_units`, `most_tiles`: bounds of the blocks' runs with the groups of SH_TEAM warps' records, and of the tile records that cannot be cut into fewer, of

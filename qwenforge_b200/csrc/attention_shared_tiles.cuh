@@ -76,8 +76,8 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     grid_launch_dependents();   // (the block has its tensor memory)
     grid_dependency_wait();
     const int kv_heads = site.kv_heads, kvh = (int)(blockIdx.x % kv_heads);
-    const SharedPlan plan = shared_plan<ST_THREADS>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
-    if (blockIdx.x == 0) shared_count_parts<ST_THREADS>(a, plan);
+    const SharedPlan plan = shared_plan<ST_THREADS, true>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
+    if (blockIdx.x == gridDim.x - 1) shared_count_parts<ST_THREADS>(a, plan);
     const int tile_blocks = plan.tiles * kv_heads;
     if ((int)blockIdx.x >= tile_blocks) {
         // ---- the other records, a warp each
@@ -108,7 +108,10 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     if (warp < PRODUCTS) {
         if (t < tiles) place = shared_row(a, rec, kv_heads, kvh, 2 * ST_BM * rec.chunk + ST_BM * t + row);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) query[c] = place < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(q + (size_t)place * D)[c];
+        for (int i = 0; i < D / 8; ++i) {   // a warp's 32 rows, whole rows at a time: piece c of row r
+            const int r = (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8), from = __shfl_sync(0xffffffffu, place, r);
+            query[i] = from < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(q + (size_t)from * D)[c];
+        }
     }
     fence_to_async();   // (the plan's room is the copies' from here on)
     __syncthreads();    // (everyone has read what it wants of the plan)
@@ -218,10 +221,11 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     } else {
         // ---- the row threads
         {
-            unsigned char* to = q_s + t * Q_BYTES + row * 128;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c)   // the 128-byte swizzle: 16-byte chunk c of a row of 64 columns lies at c XOR (row modulo 8)
-                *reinterpret_cast<uint4*>(to + c / 8 * Q_BLOCK + ((c % 8) ^ (row & 7)) * 16) = query[c];
+            for (int i = 0; i < D / 8; ++i) {   // the 128-byte swizzle: 16-byte chunk c of a row of 64 columns lies at c XOR (row modulo 8)
+                const int r = (warp & 3) * 32 + (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8);
+                *reinterpret_cast<uint4*>(q_s + t * Q_BYTES + c / 8 * Q_BLOCK + r * 128 + ((c % 8) ^ (r & 7)) * 16) = query[i];
+            }
             fence_to_async();
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_q);
