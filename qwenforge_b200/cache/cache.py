@@ -517,6 +517,13 @@ class SequenceCache:
             self._shared[key] = ops.SharedPrefix(groups, len(key), self.device) if groups else None
         return self._shared[key]
 
+    def shared_worth_reading(self, slots: Sequence[int]):
+        """`shared_prefix`, where an attention layer is faster for reading it once (`ops.attention_shared_pays`); else None."""
+        share = self.shared_prefix(slots)
+        if share is None or any(ops.attention_shared_pays(share, g.storage.dtype, g.need.kv_heads, g.need.head_dim) for g in self.kv_groups):
+            return share
+        return None
+
     def flush(self) -> None:
         for group in self.kv_groups:
             group.flush()

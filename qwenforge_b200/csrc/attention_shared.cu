@@ -56,7 +56,7 @@ struct SharedArgs {
     int* part_n;      // [n_seqs] a row's shared parts | its own parts << 16
     int* err;
     int n_seqs, n_groups, n_heads, kv_heads, most_parts, most_shared, most_own;
-    int warps, team, tile_rows, tile_pages, sms;   // (see shared_plan; tile_rows 0: no tiles)
+    int warps, team, tile_rows, tile_work, sms;   // (see shared_plan; tile_rows 0: no tiles)
     float scale_log2;
 };
 
@@ -73,8 +73,8 @@ __device__ __forceinline__ int shared_div_up(int n, int d, float one) {
 }
 __device__ __forceinline__ int shared_div_up(int n, int d) { return shared_div_up(n, d, __fdividef(1.f, (float)d)); }
 
-// ---- the plan. An item is a group's pages or a sequence's own, times its tiles of 16 rows. A group of `tile_rows` rows or more with `tile_pages` pages
-// or more goes to the tensor-core tiles (attention_shared_tiles.cuh): pairs of tiles of 128 rows, every group's pages cut into runs by its share of the
+// ---- the plan. An item is a group's pages or a sequence's own, times its tiles of 16 rows. A group of `tile_rows` rows or more, and `tile_work` rows x
+// pages or more, goes to the tensor-core tiles (attention_shared_tiles.cuh): pairs of tiles of 128 rows, every group's pages cut into runs by its share of the
 // work, no more records than the SMs that the tiles get by theirs. Everything else is cut into records of t pages for a warp each, every one a part of its
 // own: t = max(1, pages x tiles x kv heads / warps), beside tiles the next larger t that gives no more records than the other SMs have warps (two records
 // in a row take a warp twice the time); without tiles an item of more than SH_TEAM t pages goes in runs of up to SH_TEAM t to blocks, whose warps bring
@@ -116,7 +116,7 @@ __device__ __forceinline__ int shared_cut(const SharedPlan& p, int n, int most, 
     return parts;
 }
 __device__ __forceinline__ bool shared_tiled(const SharedArgs& a, const SharedPlan& p, int g) {
-    return a.tile_rows > 0 && p.rows[g] >= a.tile_rows && p.pages[g] >= a.tile_pages;
+    return a.tile_rows > 0 && p.rows[g] >= a.tile_rows && (float)p.rows[g] * p.pages[g] >= (float)a.tile_work;
 }
 __device__ __forceinline__ int shared_tiles_of(const SharedArgs& a, const SharedPlan& p, int g) {
     return shared_tiled(a, p, g) ? (p.rows[g] + 255) / 256 : (p.rows[g] + SH_ROW_TILE - 1) / SH_ROW_TILE;
@@ -697,7 +697,9 @@ __device__ __forceinline__ void shared_warp_staged(const bf16* __restrict__ q, c
 template <int D>
 __global__ void __launch_bounds__(32 * SH_TEAM, 2)
 shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a) {
-    constexpr int KEYS = D <= 64 ? 64 : 32, LO = D + 4, THREADS = 32 * SH_TEAM;
+    // Keys a step: 64 of head size 32, else 32. The operator with 64 / 32, one group of 8 sequences behind 64 pages, 70 tokens each of their own, microseconds:
+    // head size 32 8.4 / 9.0, 64 11.4 / 10.4, 96 13.1 / 11.0 (two sequences behind one page: 8.0 / 8.1, 9.1 / 8.6, 12.0 / 9.8, 128 16.1 / 11.9).
+    constexpr int KEYS = D <= 32 ? 64 : 32, LO = D + 4, THREADS = 32 * SH_TEAM;
     __shared__ __align__(16) float merge_s[SH_TEAM][16][LO];
     __shared__ float m_s[SH_TEAM][16], l_s[SH_TEAM][16];
     __shared__ SharedRecord record_s[SH_TEAM];
@@ -1025,12 +1027,15 @@ static size_t shared_generic_smem(int d, int plan_ints) {
     return (size_t)((SH_ROWS + 2 * QF_PAGE) * ld + SH_ROWS * (QF_PAGE + 4) + plan_ints) * sizeof(float);
 }
 
-// Where the tiles take over, unless the plan takes more shared memory than the warps beside them leave.
-#define SH_TILE_ROWS 65
-#define SH_TILE_PAGES 8
+// Where the tiles take over, unless the plan takes more shared memory than the warps beside them leave. Rows x pages, single warps / tiles, microseconds (one
+// group, and 70 tokens of each sequence's own): head size 64, 448 x 16 12.1 / 12.6, 112 x 64 11.2 / 12.8, 168 x 64 14.1 / 14.5, 448 x 64 19.1 / 15.0, 1,792 x 8
+// 17.6 / 14.1; head size 128, 70 x 8 13.6 / 13.7, 448 x 2 16.1 / 15.2, 112 x 8 15.6 / 13.8, 56 x 64 16.4 / 15.4, 448 x 16 21.1 / 15.7; 32 x 64 12.9 / 14.9.
+#define SH_TILE_ROWS 48
+#define SH_TILE_WORK_64 8192
+#define SH_TILE_WORK_128 896
 
 // What sizes the launches and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of
-// a block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows and pages goes to the tiles (0: there are
+// a block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows, and rows x pages, goes to the tiles (0: there are
 // none), [7] if the plan takes no more than so many ints (2 a sequence, 7 a group); [6]: SMs.
 QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     const int sms = qf_sm_count();
@@ -1041,7 +1046,7 @@ QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     sizes[2] = fast ? SH_TEAM : 1;
     sizes[3] = 64;
     sizes[4] = fast && (head_dim == 64 || head_dim == 128) ? SH_TILE_ROWS : 0;
-    sizes[5] = SH_TILE_PAGES;
+    sizes[5] = head_dim == 64 ? SH_TILE_WORK_64 : SH_TILE_WORK_128;
     sizes[6] = sms;
     sizes[7] = SH_TILE_PLAN_INTS;
     return 0;

@@ -84,7 +84,7 @@ class _GraphSession:
         self.stepper = stepper
         self.slots = [r[0] for r in rows]
         longest = max(cache.lengths[slot] + (budget - made) for slot, _, _, made, budget in rows)
-        shared = cache.shared_prefix(self.slots) if hasattr(cache, "shared_prefix") else None
+        shared = cache.shared_worth_reading(self.slots) if hasattr(cache, "shared_worth_reading") else None
         self.graph = stepper.graph_decoder.get(len(rows), longest, stepper.sampler, *(() if shared is None else (shared,)))
         cache.flush()
         self.graph.load(self.slots, [r[1] for r in rows], [cache.lengths[r[0]] for r in rows], [r[3] for r in rows],

@@ -180,7 +180,7 @@ class GraphDecoder:
         return all(getattr(part, "graph_safe", True) for part in model.parts())
 
     def get(self, rows: int, max_len: int, sampler: Sampler, shared=None) -> DecodeGraph:
-        """`shared`: what the rows' sequences share (`SequenceCache.shared_prefix`), if anything."""
+        """`shared`: what the rows' sequences share (`SequenceCache.shared_worth_reading`), if anything."""
         key = (rows, length_bound(max_len), sampler.params.temperature, sampler.params.seed)
         if shared is not None:
             shared = ops.SharedPrefix(shared.groups, rows, self.model.device, bound_pages=length_bound(shared.most_pages))

@@ -213,7 +213,7 @@ class Model:
             dev = torch.from_numpy(step.packed).to(self.device)
             ctx = context_of(step, dev, self.err, self.dtype, self.attention, self.decode_scratch)
             if ctx.is_decode:
-                ctx.shared, ctx.shared_scratch = cache.shared_prefix(step.host_slots), self.shared_scratch
+                ctx.shared, ctx.shared_scratch = cache.shared_worth_reading(step.host_slots), self.shared_scratch
             if extras:
                 ctx.extras = {}
                 for name, per_entry in extras.items():

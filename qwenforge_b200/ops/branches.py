@@ -174,6 +174,7 @@ class SharedPrefix:
         if 0 < bound_pages < self.most_pages:
             raise KernelError(f"SharedPrefix: a group shares {self.most_pages} pages, more than the bound of {bound_pages}")
         self.bound_pages = max(self.most_pages, int(bound_pages))
+        self.saved_pages = self._saved()
         self.least_pages = 0 if bound_pages else min(entry_pages)
         sizes = (self.n_seqs, self.n_seqs, len(members), len(begin), len(pages))
         packed = torch.tensor(entry_pages + entry_group + members + begin + pages, dtype=torch.int32).to(device)
@@ -182,6 +183,10 @@ class SharedPrefix:
 
     def __len__(self) -> int:
         return len(self.groups)
+
+    def _saved(self) -> int:
+        """Pages that the batch's sequences read for themselves where nothing is shared, and need not."""
+        return sum((len(entries) - 1) * pages for entries, pages in self.groups)
 
     def addresses(self) -> tuple:
         return tuple(t.data_ptr() for t in (self.entry_pages, self.entry_group, self.members, self.begin, self.pages))
@@ -196,7 +201,25 @@ class SharedPrefix:
             raise KernelError("SharedPrefix: what is loaded has other groups, or more pages than the bound")
         for name in ("entry_pages", "entry_group", "members", "begin", "pages"):
             getattr(self, name).copy_(getattr(other, name))
-        self.groups, self.most_pages = other.groups, other.most_pages
+        self.groups, self.most_pages, self.saved_pages = other.groups, other.most_pages, other.saved_pages
+
+
+# A call costs more than `attention_decode` with its plan made before (two launches and a plan of its own: 9 to 13 microseconds against 4 to 7), which what it
+# does not read has to make up for. Microseconds, one group with 70 tokens each of their own, decode / shared (saved bytes): 14 heads over 2 of 64, 64
+# sequences x 64 pages 21.0 / 15.0 (132 MB), 24 x 64 11.4 / 14.1 (48 MB), 256 x 8 24.6 / 14.1 (67 MB); 28 over 4 of 128, 8 x 64 17.0 / 15.4 (57 MB), 16 x 16
+# 12.2 / 13.7 (31 MB), 64 x 8 20.4 / 15.4 (64 MB), 256 x 64 305 / 41. The kernels for other sizes and float32 take as long as the longest sequence:
+# `attention_generic` / shared, float32, 14 over 2 of 64, 8 x 1 page 9.6 / 10.5, 8 x 4 17.4 / 10.7, 2 x 64 171 / 14; 32 x 4, 16 over 2 of 128, 27.8 / 24.5.
+SHARED_PAYS_BYTES = 56_000_000
+SHARED_PAYS_PAGES = 4
+
+
+def attention_shared_pays(share: SharedPrefix, dtype, kv_heads: int, head_dim: int) -> bool:
+    """Whether `attention_shared` takes this shape, and is faster than the attention that reads every sequence's pages for itself."""
+    if share.n_seqs > SHARED_MAX_SEQS or head_dim > SHARED_MAX_HEAD_DIM:
+        return False
+    if dtype is torch.bfloat16 and head_dim in kernels.FAST_ATTENTION_HEAD_DIMS:
+        return share.saved_pages * kv_heads * head_dim * 4 * PAGE_TOKENS >= SHARED_PAYS_BYTES
+    return share.most_pages >= SHARED_PAYS_PAGES
 
 
 class SharedScratch:
@@ -227,7 +250,7 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     code = _function("attention_shared", "qf_attention_shared_shape", _I, _I, _P)(int(dtype == torch.bfloat16), head_dim, sizes)
     if code:
         raise KernelError(f"attention_shared: CUDA error {code} when asked for its sizes")
-    row_tile, warps, team, most, tile_rows, tile_pages, sms, tile_ints = sizes
+    row_tile, warps, team, most, tile_rows, tile_work, sms, tile_ints = sizes
     group_heads = n_heads // kv_heads
 
     def parts(pages: int, tiles: int) -> int:
@@ -235,8 +258,9 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     own_tiles = -(-group_heads // row_tile)
     tiles = [-(-len(entries) * group_heads // row_tile) for entries, _ in share.groups]
     most_shared = max((parts(share.bound_pages, t) for t in tiles), default=0)
-    pairs = [-(-len(entries) * group_heads // 256) for entries, _ in share.groups if len(entries) * group_heads >= tile_rows]
-    if not tile_rows or share.bound_pages < tile_pages or 2 * share.n_seqs + 7 * len(share) > tile_ints:
+    rows = [len(entries) * group_heads for entries, _ in share.groups]
+    pairs = [-(-r // 256) for r in rows if r >= tile_rows and r * share.bound_pages >= tile_work]
+    if not tile_rows or 2 * share.n_seqs + 7 * len(share) > tile_ints:
         pairs = []
     if pairs:   # (everything else is cut for single warps then)
         most_shared = max(most_shared, min(most // 4, share.bound_pages))

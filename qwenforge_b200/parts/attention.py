@@ -533,7 +533,7 @@ class GqaAttention(Mixer):
     def reads_shared(self, ctx) -> bool:
         """Whether this step's sequences begin with the same pages and the layer reads those once for all of them."""
         return (ctx.shared is not None and ctx.is_decode and ctx.n_tokens == ctx.n_seqs and ctx.attention == "auto" and self.plain
-                and self.window <= 0)
+                and self.window <= 0 and ops.attention_shared_pays(ctx.shared, ctx.dtype, self.n_kv, self.head_dim))
 
     def _attend_shared(self, q, attended, args, ctx) -> None:
         ops.attention_shared(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs, self.scale, ctx.shared,

@@ -243,3 +243,13 @@ def test_tensors_off_the_gpu_are_refused():
         ops.attention_shared(torch.zeros(2, 32), torch.zeros(2, 32), i32, i32[:2], i32[:2], site, 1, 2, 1.0, share, ops.SharedScratch("cpu"), i32[:1])
     with pytest.raises(ops.KernelError, match="CUDA"):
         ops.verify_drafts(torch.zeros(2, 8), None, i32[:1], i32[:2], torch.zeros(1), 1.0, 0, torch.zeros(1, dtype=torch.int64), i32[:1], i32[:1], i32[:2].view(1, 2))
+
+
+def test_when_shared_reading_pays():
+    many = ops.SharedPrefix([(range(64), 64)], 64, "cpu")
+    assert many.saved_pages == 63 * 64
+    assert ops.attention_shared_pays(many, torch.bfloat16, 2, 64) and not ops.attention_shared_pays(many, torch.bfloat16, 2, 300)
+    few = ops.SharedPrefix([([0, 2], 64)], 3, "cpu")
+    assert not ops.attention_shared_pays(few, torch.bfloat16, 2, 64) and ops.attention_shared_pays(few, torch.float32, 2, 64)
+    assert ops.attention_shared_pays(few, torch.bfloat16, 2, 80) and not ops.attention_shared_pays(ops.SharedPrefix([([0, 2], 3)], 3, "cpu"), torch.float32, 2, 64)
+    assert not ops.attention_shared_pays(ops.SharedPrefix([(range(2049), 640)], 2049, "cpu"), torch.bfloat16, 2, 64)

@@ -13,6 +13,13 @@ from tests.helpers import CONFIGS, SMALL_64, SMALL_128, assert_logits_close, mak
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def always_shared(monkeypatch):
+    """These batches are small: they would mostly be faster apart."""
+    monkeypatch.setattr(ops.branches, "SHARED_PAYS_BYTES", 0)
+    monkeypatch.setattr(ops.branches, "SHARED_PAYS_PAGES", 0)
+
+
 def model_of(config, dtype, seed=1):
     folder, _ = make_model_dir(config, seed)
     return Model.from_dir(folder, dtype, "cuda"), folder
@@ -61,6 +68,9 @@ def test_the_layers_run_the_shared_kernel(monkeypatch):
     model.step(cache, [(s, [6]) for s in [slot] + forks])
     assert len(calls) == SMALL_64["num_hidden_layers"]
     model.step(cache, [(forks[0], [7])])   # alone it shares nothing with the batch
+    assert len(calls) == SMALL_64["num_hidden_layers"]
+    monkeypatch.setattr(ops.branches, "SHARED_PAYS_BYTES", 10 ** 9)
+    model.step(cache, [(s, [8]) for s in forks])
     assert len(calls) == SMALL_64["num_hidden_layers"]
 
 
