@@ -79,6 +79,7 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
     const SharedPlan plan = shared_plan<ST_THREADS, true>(a, reinterpret_cast<int*>(tc_smem), D);   // (room that nothing else needs yet)
     if (blockIdx.x == gridDim.x - 1) shared_count_parts<ST_THREADS>(a, plan);
     const int tile_blocks = plan.tiles * kv_heads;
+    bool timed_out = false;
     if ((int)blockIdx.x >= tile_blocks) {
         // ---- the other records, a warp each
         const int all = ((int)gridDim.x - tile_blocks) * WARPS;
@@ -92,246 +93,241 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
             shared_warp_staged<D>(q, site, a, rec, task % kv_heads, room, x);
             x.leave_part(a, rec.part);
         }
-        tc_fence_before();
-        __syncthreads();
-        if (warp == PRODUCTS)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32  %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
-        return;
-    }
-    const SharedRecord rec = shared_tile_record(a, plan, blockIdx.x / kv_heads);
-    const int rows = rec.rows - 2 * ST_BM * rec.chunk;   // from the first tile's on
-    const int tiles = rows > ST_BM ? 2 : 1;
-    const int turns = (rec.p_end - rec.p_begin + 1) / 2, end = rec.p_end * QF_PAGE;   // no key of this run from `end` on
-    // the rows' queries, on their way while the block comes together
-    int place = -1;
-    uint4 query[D / 8];
-    if (warp < PRODUCTS) {
-        if (t < tiles) place = shared_row(a, rec, kv_heads, kvh, 2 * ST_BM * rec.chunk + ST_BM * t + row);
+    } else {
+        const SharedRecord rec = shared_tile_record(a, plan, blockIdx.x / kv_heads);
+        const int rows = rec.rows - 2 * ST_BM * rec.chunk;   // from the first tile's on
+        const int tiles = rows > ST_BM ? 2 : 1;
+        const int turns = (rec.p_end - rec.p_begin + 1) / 2, end = rec.p_end * QF_PAGE;   // no key of this run from `end` on
+        // the rows' queries, on their way while the block comes together
+        int place = -1;
+        uint4 query[D / 8];
+        if (warp < PRODUCTS) {
+            if (t < tiles) place = shared_row(a, rec, kv_heads, kvh, 2 * ST_BM * rec.chunk + ST_BM * t + row);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {   // a warp's 32 rows, whole rows at a time: piece c of row r
-            const int r = (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8), from = __shfl_sync(0xffffffffu, place, r);
-            query[i] = from < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(q + (size_t)from * D)[c];
+            for (int i = 0; i < D / 8; ++i) {   // a warp's 32 rows, whole rows at a time: piece c of row r
+                const int r = (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8), from = __shfl_sync(0xffffffffu, place, r);
+                query[i] = from < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(q + (size_t)from * D)[c];
+            }
         }
-    }
-    fence_to_async();   // (the plan's room is the copies' from here on)
-    __syncthreads();    // (everyone has read what it wants of the plan)
-    bool timed_out = false;
-    // A warp waits as one: the loads and stores of tensor memory and the choice of the issuing lane are collective.
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+        fence_to_async();   // (the plan's room is the copies' from here on)
+        __syncthreads();    // (everyone has read what it wants of the plan)
+        // A warp waits as one: the loads and stores of tensor memory and the choice of the issuing lane are collective.
+        auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
 
-    if (warp == COPIES) {
-        const bool leader = elect_one();
-        const int* table_row = site.table + (long long)rec.slot * site.table_stride;
-        int keys = 0, values = 0;   // turns whose copies have been asked for
-        for (int j = 0; j < turns; ++j) {
-            const int stage = j & 1, first = rec.p_begin + 2 * j;
-            const uint32_t freed = ((j >> 1) + 1) & 1;   // the turn before last has been read
-            int page[2];
+        if (warp == COPIES) {
+            const bool leader = elect_one();
+            const int* table_row = site.table + (long long)rec.slot * site.table_stride;
+            int keys = 0, values = 0;   // turns whose copies have been asked for
+            for (int j = 0; j < turns; ++j) {
+                const int stage = j & 1, first = rec.p_begin + 2 * j;
+                const uint32_t freed = ((j >> 1) + 1) & 1;   // the turn before last has been read
+                int page[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                page[h] = table_row[min(first + h, rec.p_end - 1)];   // (beyond the last page: masked keys, values that nothing reads)
-                if (page[h] < 0) {  // a page that is not held: reported; some held memory is read instead
-                    if (leader) atomicOr(a.err, QF_ERR_NO_PAGE);
-                    page[h] = 0;
+                for (int h = 0; h < 2; ++h) {
+                    page[h] = table_row[min(first + h, rec.p_end - 1)];   // (beyond the last page: masked keys, values that nothing reads)
+                    if (page[h] < 0) {  // a page that is not held: reported; some held memory is read instead
+                        if (leader) atomicOr(a.err, QF_ERR_NO_PAGE);
+                        page[h] = 0;
+                    }
+                }
+                if (j >= 2 && !wait_all(&bar_k_free[stage], freed)) {
+                    timed_out = true;
+                    break;
+                }
+                // row of the cache seen as one matrix [rows][D]; pages may lie at any distance that is whole rows
+                ++keys;
+                if (leader) {
+                    mbar_expect_tx(&bar_k[stage], KV_BYTES);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb)
+                            tma_load_2d(k_s + stage * KV_BYTES + cb * KV_BLOCK + h * PAGE_BYTES, &kv_map, cb * 64,
+                                        (int)((long long)page[h] * (site.page_elems / D) + kvh * QF_PAGE), &bar_k[stage]);
+                }
+                __syncwarp();
+                if (j >= 2 && !wait_all(&bar_v_free[stage], freed)) {
+                    timed_out = true;
+                    break;
+                }
+                ++values;
+                if (leader) {
+                    mbar_expect_tx(&bar_v[stage], KV_BYTES);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb)
+                            tma_load_2d(v_s + stage * KV_BYTES + cb * KV_BLOCK + h * PAGE_BYTES, &kv_map, cb * 64,
+                                        (int)((long long)page[h] * (site.page_elems / D) + (kv_heads + kvh) * QF_PAGE), &bar_v[stage]);
+                }
+                __syncwarp();
+            }
+            // The block ends, also after a wait that ran out, only when nothing is on its way to its shared memory (long arrived otherwise).
+            for (int j = max(keys - 2, 0); j < keys; ++j) timed_out |= !wait_all(&bar_k[j & 1], (j >> 1) & 1);
+            for (int j = max(values - 2, 0); j < values; ++j) timed_out |= !wait_all(&bar_v[j & 1], (j >> 1) & 1);
+        } else if (warp == PRODUCTS) {
+            const bool leader = elect_one();
+            // descriptors: an address field counts 16 bytes, so 16 columns of a K-major row (32 bytes) are 2 units
+            const uint64_t desc_q = smem_desc_sw128(q_s), desc_k = smem_desc_sw128(k_s), desc_v = smem_desc_mn_sw128(v_s, KV_BLOCK);
+            constexpr uint32_t idesc_s = umma_idesc_bf16(ST_BM, ST_BK, false), idesc_pv = umma_idesc_bf16(ST_BM, D, true);
+            // S of tile i, turn j; the last tile that reads a turn's keys hands their stage back
+            auto issue_s = [&](int i, int j) {
+                if (!wait_all(&bar_k[j & 1], (j >> 1) & 1)) return false;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t dq = desc_q + (uint64_t)(i * (Q_BYTES >> 4)), dk = desc_k + (uint64_t)((j & 1) * (KV_BYTES >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks)
+                        umma_bf16(tmem + 128 * i, dq + (uint64_t)((ks / 4) * (Q_BLOCK >> 4) + 2 * (ks % 4)),
+                                  dk + (uint64_t)((ks / 4) * (KV_BLOCK >> 4) + 2 * (ks % 4)), idesc_s, ks > 0 ? 1u : 0u);
+                    umma_commit(&bar_s[i]);
+                    if (i == tiles - 1) umma_commit(&bar_k_free[j & 1]);
+                }
+                __syncwarp();
+                return true;
+            };
+            timed_out = !wait_all(&bar_q, 0);
+            for (int i = 0; i < tiles && !timed_out; ++i) timed_out = !issue_s(i, 0);
+            for (int j = 0; j < turns && !timed_out; ++j) {
+                for (int i = 0; i < tiles && !timed_out; ++i) {
+                    if (!wait_all(&bar_v[j & 1], (j >> 1) & 1) || !wait_all(&bar_p[i], j & 1)) {   // every row has written its weights
+                        timed_out = true;
+                        break;
+                    }
+                    tc_fence_after();
+                    if (leader) {   // values [128 keys][D] as they lie (MN-major), 16 keys are two groups of 8 rows (2048 bytes)
+                        const uint64_t dv = desc_v + (uint64_t)((j & 1) * (KV_BYTES >> 4));
+                        const int k1 = rec.p_begin + 2 * j + 1 < rec.p_end ? ST_BK / 16 : ST_BK / 32;
+#pragma unroll
+                        for (int kk = 0; kk < ST_BK / 16; ++kk)
+                            if (kk < k1)
+                                umma_bf16_tmem_a(tmem + O_COL + 128 * i, tmem + 128 * i + 8 * kk, dv + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
+                                                 (j > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit(&bar_pv[i]);
+                        if (i == tiles - 1) umma_commit(&bar_v_free[j & 1]);
+                    }
+                    __syncwarp();
+                    if (j + 1 < turns && (!wait_all(&bar_pv[i], j & 1) || !issue_s(i, j + 1))) timed_out = true;
                 }
             }
-            if (j >= 2 && !wait_all(&bar_k_free[stage], freed)) {
-                timed_out = true;
-                break;
-            }
-            // row of the cache seen as one matrix [rows][D]; pages may lie at any distance that is whole rows
-            ++keys;
-            if (leader) {
-                mbar_expect_tx(&bar_k[stage], KV_BYTES);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        tma_load_2d(k_s + stage * KV_BYTES + cb * KV_BLOCK + h * PAGE_BYTES, &kv_map, cb * 64,
-                                    (int)((long long)page[h] * (site.page_elems / D) + kvh * QF_PAGE), &bar_k[stage]);
-            }
+            if (leader) umma_commit(&bar_end);   // the block ends when no product of its is at work
             __syncwarp();
-            if (j >= 2 && !wait_all(&bar_v_free[stage], freed)) {
-                timed_out = true;
-                break;
-            }
-            ++values;
-            if (leader) {
-                mbar_expect_tx(&bar_v[stage], KV_BYTES);
+            timed_out |= !wait_all(&bar_end, 0);
+        } else {
+            // ---- the row threads
+            {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        tma_load_2d(v_s + stage * KV_BYTES + cb * KV_BLOCK + h * PAGE_BYTES, &kv_map, cb * 64,
-                                    (int)((long long)page[h] * (site.page_elems / D) + (kv_heads + kvh) * QF_PAGE), &bar_v[stage]);
+                for (int i = 0; i < D / 8; ++i) {   // the 128-byte swizzle: 16-byte chunk c of a row of 64 columns lies at c XOR (row modulo 8)
+                    const int r = (warp & 3) * 32 + (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8);
+                    *reinterpret_cast<uint4*>(q_s + t * Q_BYTES + c / 8 * Q_BLOCK + r * 128 + ((c % 8) ^ (r & 7)) * 16) = query[i];
+                }
+                fence_to_async();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_q);
             }
-            __syncwarp();
-        }
-        // The block ends, also after a wait that ran out, only when nothing is on its way to its shared memory (long arrived otherwise).
-        for (int j = max(keys - 2, 0); j < keys; ++j) timed_out |= !wait_all(&bar_k[j & 1], (j >> 1) & 1);
-        for (int j = max(values - 2, 0); j < values; ++j) timed_out |= !wait_all(&bar_v[j & 1], (j >> 1) & 1);
-    } else if (warp == PRODUCTS) {
-        const bool leader = elect_one();
-        // descriptors: an address field counts 16 bytes, so 16 columns of a K-major row (32 bytes) are 2 units
-        const uint64_t desc_q = smem_desc_sw128(q_s), desc_k = smem_desc_sw128(k_s), desc_v = smem_desc_mn_sw128(v_s, KV_BLOCK);
-        constexpr uint32_t idesc_s = umma_idesc_bf16(ST_BM, ST_BK, false), idesc_pv = umma_idesc_bf16(ST_BM, D, true);
-        // S of tile i, turn j; the last tile that reads a turn's keys hands their stage back
-        auto issue_s = [&](int i, int j) {
-            if (!wait_all(&bar_k[j & 1], (j >> 1) & 1)) return false;
-            tc_fence_after();
-            if (leader) {
-                const uint64_t dq = desc_q + (uint64_t)(i * (Q_BYTES >> 4)), dk = desc_k + (uint64_t)((j & 1) * (KV_BYTES >> 4));
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    umma_bf16(tmem + 128 * i, dq + (uint64_t)((ks / 4) * (Q_BLOCK >> 4) + 2 * (ks % 4)),
-                              dk + (uint64_t)((ks / 4) * (KV_BLOCK >> 4) + 2 * (ks % 4)), idesc_s, ks > 0 ? 1u : 0u);
-                umma_commit(&bar_s[i]);
-                if (i == tiles - 1) umma_commit(&bar_k_free[j & 1]);
-            }
-            __syncwarp();
-            return true;
-        };
-        timed_out = !wait_all(&bar_q, 0);
-        for (int i = 0; i < tiles && !timed_out; ++i) timed_out = !issue_s(i, 0);
-        for (int j = 0; j < turns && !timed_out; ++j) {
-            for (int i = 0; i < tiles && !timed_out; ++i) {
-                if (!wait_all(&bar_v[j & 1], (j >> 1) & 1) || !wait_all(&bar_p[i], j & 1)) {   // every row has written its weights
+            if (t < tiles) {
+            const int see = rec.limit >= end ? end : min(end, shared_seen(a, place)), all_see = min(end, rec.limit);
+            const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * t, o_at = lanes + O_COL + 128 * t;
+            const float folded = a.scale_log2 > 0.f ? a.scale_log2 : 1.f;
+            float m_ref = QF_NEG_BIG, l_run = 0.f;   // the reference maximum of the exponentials, and their sum
+            for (int j = 0; j < turns; ++j) {
+                if (!wait_all(&bar_s[t], j & 1)) {   // (the product of the turn before is done too: S was issued after it)
                     timed_out = true;
                     break;
                 }
                 tc_fence_after();
-                if (leader) {   // values [128 keys][D] as they lie (MN-major), 16 keys are two groups of 8 rows (2048 bytes)
-                    const uint64_t dv = desc_v + (uint64_t)((j & 1) * (KV_BYTES >> 4));
-                    const int k1 = rec.p_begin + 2 * j + 1 < rec.p_end ? ST_BK / 16 : ST_BK / 32;
+                float s[ST_BK];
+                tmem_load_row_128(s_at, s);
+                if (!(a.scale_log2 > 0.f)) {   // below, the scale is folded into the exponent, behind the maximum and the mask: above zero only
 #pragma unroll
-                    for (int kk = 0; kk < ST_BK / 16; ++kk)
-                        if (kk < k1)
-                            umma_bf16_tmem_a(tmem + O_COL + 128 * i, tmem + 128 * i + 8 * kk, dv + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
-                                             (j > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&bar_pv[i]);
-                    if (i == tiles - 1) umma_commit(&bar_v_free[j & 1]);
+                    for (int i = 0; i < ST_BK; ++i) s[i] *= a.scale_log2;
                 }
-                __syncwarp();
-                if (j + 1 < turns && (!wait_all(&bar_pv[i], j & 1) || !issue_s(i, j + 1))) timed_out = true;
-            }
-        }
-        if (leader) umma_commit(&bar_end);   // the block ends when no product of its is at work
-        __syncwarp();
-        timed_out |= !wait_all(&bar_end, 0);
-    } else {
-        // ---- the row threads
-        {
+                const int key0 = (rec.p_begin + 2 * j) * QF_PAGE;
+                if (key0 + ST_BK > all_see) {   // a key that the row does not see gets the weight 2^-inf = 0
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {   // the 128-byte swizzle: 16-byte chunk c of a row of 64 columns lies at c XOR (row modulo 8)
-                const int r = (warp & 3) * 32 + (32 * i + (threadIdx.x & 31)) / (D / 8), c = threadIdx.x % (D / 8);
-                *reinterpret_cast<uint4*>(q_s + t * Q_BYTES + c / 8 * Q_BLOCK + r * 128 + ((c % 8) ^ (r & 7)) * 16) = query[i];
+                    for (int i = 0; i < ST_BK; ++i) s[i] = key0 + i < see ? s[i] : -INFINITY;
+                }
+                float mx[4];  // four chains instead of one: the comparisons do not wait for each other
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i] = s[i];
+#pragma unroll
+                for (int i = 4; i < ST_BK - 4; i += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx[c] = shared_max3(mx[c], s[i + c], s[i + 4 + c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[ST_BK - 4 + c]);
+                // (the scores stay unscaled; the scale is folded into the exponent)
+                const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * folded);
+                float f_o = 1.0f;
+                bool moved = false;
+                if (j == 0) {
+                    m_ref = m_true;  // nothing to rescale yet: the first products overwrite O
+                } else if (m_true - m_ref > 8.0f) {   // (weights stay below 2^8, well inside bf16 and float32)
+                    moved = true;
+                    f_o = fast_exp2(m_ref - m_true);
+                    m_ref = m_true;
+                    l_run *= f_o;
+                }
+                if (__any_sync(0xffffffffu, moved)) {  // the warp's 32 rows of O are loaded and stored together
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 16) {
+                        uint32_t raw[16];
+                        tmem_load_16(o_at + c0, raw);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f_o);
+                        tmem_store_16(o_at + c0, raw);
+                    }
+                }
+                // two neighbouring weights an instruction where the pipes allow it: s * scale - reference, and the sums
+                const float2 by = make_float2(folded, folded), less = make_float2(-m_ref, -m_ref);
+                float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {   // half of the weights at a time: the first are stored while the others are formed
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        float2 p = __ffma2_rn(make_float2(s[64 * h + i], s[64 * h + i + 1]), by, less);
+                        p.x = fast_exp2(p.x), p.y = fast_exp2(p.y);
+                        part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], p);
+                        packed[i / 2] = pack_bf16(p.x, p.y);
+                    }
+                    tmem_store_32(s_at + 32 * h, packed);
+                }
+                l_run += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                tmem_store_wait();
+                tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_p[t]);
             }
-            fence_to_async();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_q);
-        }
-        if (t < tiles) {
-        const int see = rec.limit >= end ? end : min(end, shared_seen(a, place)), all_see = min(end, rec.limit);
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * t, o_at = lanes + O_COL + 128 * t;
-        const float folded = a.scale_log2 > 0.f ? a.scale_log2 : 1.f;
-        float m_ref = QF_NEG_BIG, l_run = 0.f;   // the reference maximum of the exponentials, and their sum
-        for (int j = 0; j < turns; ++j) {
-            if (!wait_all(&bar_s[t], j & 1)) {   // (the product of the turn before is done too: S was issued after it)
-                timed_out = true;
-                break;
-            }
+            if (!timed_out && !wait_all(&bar_pv[t], (turns - 1) & 1)) timed_out = true;
             tc_fence_after();
-            float s[ST_BK];
-            tmem_load_row_128(s_at, s);
-            if (!(a.scale_log2 > 0.f)) {   // below, the scale is folded into the exponent, behind the maximum and the mask: above zero only
-#pragma unroll
-                for (int i = 0; i < ST_BK; ++i) s[i] *= a.scale_log2;
-            }
-            const int key0 = (rec.p_begin + 2 * j) * QF_PAGE;
-            if (key0 + ST_BK > all_see) {   // a key that the row does not see gets the weight 2^-inf = 0
-#pragma unroll
-                for (int i = 0; i < ST_BK; ++i) s[i] = key0 + i < see ? s[i] : -INFINITY;
-            }
-            float mx[4];  // four chains instead of one: the comparisons do not wait for each other
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = s[i];
-#pragma unroll
-            for (int i = 4; i < ST_BK - 4; i += 8)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) mx[c] = shared_max3(mx[c], s[i + c], s[i + 4 + c]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[ST_BK - 4 + c]);
-            // (the scores stay unscaled; the scale is folded into the exponent)
-            const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * folded);
-            float f_o = 1.0f;
-            bool moved = false;
-            if (j == 0) {
-                m_ref = m_true;  // nothing to rescale yet: the first products overwrite O
-            } else if (m_true - m_ref > 8.0f) {   // (weights stay below 2^8, well inside bf16 and float32)
-                moved = true;
-                f_o = fast_exp2(m_ref - m_true);
-                m_ref = m_true;
-                l_run *= f_o;
-            }
-            if (__any_sync(0xffffffffu, moved)) {  // the warp's 32 rows of O are loaded and stored together
+            if (!timed_out) {   // (the loads are collective: every lane takes part, rows that are not there store nothing)
+                constexpr int HALF = D / 2, C4 = HALF / 4, AT_ONCE = 32 / C4;   // a row's 16-byte pieces of half its columns, and rows that a warp writes at once
+                const int lane = threadIdx.x & 31;
+                if (place >= 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)place * a.most_parts + rec.part) * 2) = make_float2(m_ref, l_run);
+                float4* const room = reinterpret_cast<float4*>(q_s + t * Q_BYTES) + (warp & 3) * 32 * C4;   // the warp's 32 rows of [128][HALF] floats
 #pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 16) {
-                    uint32_t raw[16];
-                    tmem_load_16(o_at + c0, raw);
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f_o);
-                    tmem_store_16(o_at + c0, raw);
-                }
-            }
-            // two neighbouring weights an instruction where the pipes allow it: s * scale - reference, and the sums
-            const float2 by = make_float2(folded, folded), less = make_float2(-m_ref, -m_ref);
-            float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    for (int c0 = 0; c0 < HALF; c0 += 32) {
+                        uint32_t raw[32];
+                        tmem_load_32(o_at + h * HALF + c0, raw);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {   // half of the weights at a time: the first are stored while the others are formed
-                uint32_t packed[32];
-#pragma unroll
-                for (int i = 0; i < 64; i += 2) {
-                    float2 p = __ffma2_rn(make_float2(s[64 * h + i], s[64 * h + i + 1]), by, less);
-                    p.x = fast_exp2(p.x), p.y = fast_exp2(p.y);
-                    part[(i >> 1) & 1] = __fadd2_rn(part[(i >> 1) & 1], p);
-                    packed[i / 2] = pack_bf16(p.x, p.y);
-                }
-                tmem_store_32(s_at + 32 * h, packed);
-            }
-            l_run += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-            tmem_store_wait();
-            tc_fence_before();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_p[t]);
-        }
-        if (!timed_out && !wait_all(&bar_pv[t], (turns - 1) & 1)) timed_out = true;
-        tc_fence_after();
-        if (!timed_out) {   // (the loads are collective: every lane takes part, rows that are not there store nothing)
-            constexpr int HALF = D / 2, C4 = HALF / 4, AT_ONCE = 32 / C4;   // a row's 16-byte pieces of half its columns, and rows that a warp writes at once
-            const int lane = threadIdx.x & 31;
-            if (place >= 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)place * a.most_parts + rec.part) * 2) = make_float2(m_ref, l_run);
-            float4* const room = reinterpret_cast<float4*>(q_s + t * Q_BYTES) + (warp & 3) * 32 * C4;   // the warp's 32 rows of [128][HALF] floats
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int c0 = 0; c0 < HALF; c0 += 32) {
-                    uint32_t raw[32];
-                    tmem_load_32(o_at + h * HALF + c0, raw);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)   // piece c of a row lies at c XOR (row modulo 8): neither side meets a bank twice
-                        room[lane * C4 + ((c0 / 4 + c) ^ (lane & 7))] = make_float4(__uint_as_float(raw[4 * c]), __uint_as_float(raw[4 * c + 1]),
-                                                                                     __uint_as_float(raw[4 * c + 2]), __uint_as_float(raw[4 * c + 3]));
-                }
-                __syncwarp();
+                        for (int c = 0; c < 8; ++c)   // piece c of a row lies at c XOR (row modulo 8): neither side meets a bank twice
+                            room[lane * C4 + ((c0 / 4 + c) ^ (lane & 7))] = make_float4(__uint_as_float(raw[4 * c]), __uint_as_float(raw[4 * c + 1]),
+                                                                                         __uint_as_float(raw[4 * c + 2]), __uint_as_float(raw[4 * c + 3]));
+                    }
+                    __syncwarp();
 #pragma unroll 4
-                for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
-                    const int r = r0 + lane / C4, c = lane % C4, to = __shfl_sync(0xffffffffu, place, r);
-                    if (to >= 0)
-                        *reinterpret_cast<float4*>(a.part_o + ((size_t)to * a.most_parts + rec.part) * D + h * HALF + 4 * c) = room[r * C4 + (c ^ (r & 7))];
+                    for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                        const int r = r0 + lane / C4, c = lane % C4, to = __shfl_sync(0xffffffffu, place, r);
+                        if (to >= 0)
+                            *reinterpret_cast<float4*>(a.part_o + ((size_t)to * a.most_parts + rec.part) * D + h * HALF + 4 * c) = room[r * C4 + (c ^ (r & 7))];
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-        }
+            }
         }
     }
     if (timed_out) atomicOr(a.err, QF_ERR_COPY_TIMEOUT);

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from qwenforge_b200 import ops
+from qwenforge_b200.ops import branches
 
 pytestmark = pytest.mark.gpu
 PAGE = 64
@@ -77,7 +78,7 @@ class Batch:
             k, v = (x.repeat_interleave(group, 0) for x in kv)
             q = self.q[e].view(self.heads, 1, self.dim).double()
             score = (q * k).sum(-1) * self.scale
-            spread = float((q * k).abs().sum(-1).max()) * self.scale
+            spread = float((q * k).abs().sum(-1).max()) * abs(self.scale)
             if sinks is not None:
                 score = torch.cat((score, sinks.double()[:, None]), 1)
                 v = torch.cat((v, torch.zeros_like(v[:, :1])), 1)
@@ -298,3 +299,143 @@ def test_offsets_beyond_32_bits():
     b.site = ops.KvSiteArgs(storage, b.table, kv_heads, dim)
     b.run()
     b.check()
+
+
+TILED = [(32, 1, 64), (32, 2, 128)]   # shapes whose groups of nine sequences behind 33 pages go to the tensor-core tiles
+
+
+def tiled(shape, groups=None, own=None, **kw):
+    """Two groups on tiles (288 and 160 or 320 rows, odd and even page counts), a small one on warps, and sequences that share nothing."""
+    groups = groups or [([0, 2, 3, 4, 5, 8, 9, 10, 11], 33), ([1, 6, 7, 12, 13], 52), ([14, 15], 2)]
+    own = own or [1, 63, 64, 65, 130, 7, 200, 31, 500, 2, 33, 64, 128, 129, 70, 1, 300]
+    b = Batch(groups, own, *shape, torch.bfloat16, **kw)
+    tiles = branches._shared_sizes(torch.bfloat16, b.dim, b.kv_heads, b.heads, b.share, branches._own_pages(max(b.lengths), b.table, b.share))[1]
+    assert tiles > 0
+    return b
+
+
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("gap", [0, 128])
+def test_tiles(shape, gap):
+    b = tiled(shape, gap=gap)
+    b.run()
+    b.check()
+    first = b.out.clone()
+    b.run(max_kv_len=None)
+    b.check()
+    b.run()
+    assert torch.equal(b.out, first)
+
+
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("idle", [(0, 4), (1, 6, 7, 12, 13), tuple(range(14)), tuple(range(17))])
+def test_tiles_of_ended_sequences(shape, idle):
+    b = tiled(shape, idle=idle)
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("shape", TILED)
+def test_tiles_of_members_inside_the_shared_pages(shape):
+    b = tiled(shape)
+    b.tok_pos[torch.tensor([0, 3, 12, 14])] = torch.tensor([0, 5 * PAGE + 3, 51 * PAGE, 64], dtype=torch.int32, device="cuda")
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("shape", TILED)
+def test_tiles_with_nothing_beside_them(shape):
+    """Every sequence stands inside what it shares: there are no other records."""
+    b = tiled(shape, [(list(range(10)), 40)], [1] * 10)
+    b.tok_pos.copy_(torch.tensor([40 * PAGE - 1 - 97 * e for e in range(10)], dtype=torch.int32))
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.5])
+def test_tiles_with_sinks_and_any_scale(shape, scale):
+    b = tiled(shape)
+    b.scale = scale
+    sinks = torch.linspace(-5, 9, shape[0], device="cuda")
+    b.run(sinks=sinks)
+    b.check(sinks=sinks)
+
+
+@pytest.mark.parametrize("shape", TILED)
+def test_tiles_read_nothing_behind_the_last_position(shape):
+    b = tiled(shape)
+    for e in range(b.n):
+        length = b.lengths[e]
+        page = int(b.table_cpu[b.slots_cpu[e], (length - 1) // PAGE])
+        if length % PAGE:
+            b.storage[page, 0, :, length % PAGE:] = math.nan
+            b.storage[page, 1, :, length % PAGE:] = math.inf
+    free = set(range(b.storage.shape[0])) - set(b.table_cpu.flatten().tolist())
+    b.storage[list(free)] = math.nan
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("shape", TILED)
+def test_tiles_report_a_page_that_is_not_held(shape):
+    b = tiled(shape)
+    b.table[b.slots.long()[[1, 6, 7, 12, 13]], 3] = -1
+    b.run()
+    assert int(b.err) == ops.ERR_NO_PAGE
+    b.err.zero_()
+    b.idle = {1, 6, 7, 12, 13}   # (their rows are not compared; the others' are whole)
+    b.out[list(b.idle)] = 0
+    b.check()
+
+
+@pytest.mark.parametrize("shape", TILED)
+def test_what_is_shared_is_replaced_under_a_graph(shape):
+    """Within the bound it was captured with: fewer pages are shared, too few for the tiles, then as many as there may be."""
+    b = tiled(shape)
+    share = ops.SharedPrefix(b.groups, b.n, "cuda", bound_pages=64)
+    b.run(share=share)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        b.run(share=share)
+    for pages in (1, 20, None):
+        share.load(ops.SharedPrefix([(e, min(p, pages) if pages else p) for e, p in b.groups], b.n, "cuda"))
+        b.out.fill_(3.0)
+        graph.replay()
+        b.check()
+    with pytest.raises(ops.KernelError):
+        share.load(ops.SharedPrefix([(e, 65) for e, _ in b.groups], b.n, "cuda"))
+    with pytest.raises(ops.KernelError):
+        share.load(ops.SharedPrefix(b.groups[:2], b.n, "cuda"))
+
+
+@pytest.mark.parametrize("shape,groups", [((4, 1, 32), [(range(0, 1000), 2)] + [(range(1000 + 5 * i, 1005 + 5 * i), 3) for i in range(200)]),
+                                          ((8, 1, 64), [(range(3, 2048), 2)]), ((2, 1, 20), [(range(0, 2048, 2), 1)])])
+def test_the_largest_batch(shape, groups):
+    b = Batch([(list(e), p) for e, p in groups], [1 + i % 67 for i in range(2048)], *shape, torch.bfloat16)
+    b.run()
+    b.check()
+
+
+def test_two_graphs_on_two_streams():
+    """With workspaces of their own."""
+    runs = []
+    for seed, shape in ((1, (14, 2, 64)), (2, (16, 2, 128)), (3, (32, 1, 64))):
+        b = Batch(*CASES["many"], *shape, torch.bfloat16, seed=seed)
+        b.run()
+        torch.cuda.synchronize()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            b.run()
+        b.out.fill_(3.0)
+        runs.append((b, graph, stream))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _, graph, stream in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for b, _, _ in runs:
+        b.check()
