@@ -14,7 +14,7 @@
 //   entry_pages [n_seqs]  pages that the sequence shares with its group (0: none);   entry_group [n_seqs]  its group (-1: none)
 //   members     [n_seqs]  batch entries, group after group;   begin [n_groups + 1]  where each group starts there;   pages [n_groups]
 //
-// Everything is held in float32 but the weights, which enter the second product as bf16 (their rounding, 2^-9 of each, is that of the result).
+// Everything is held in float32 but the weights, which enter the second product as bf16 (their rounding, up to 2^-8 of each, is that of the result).
 #include "mma.cuh"
 
 // Record kinds: a sequence's own pages or a group's; with SH_TOGETHER, one of a block's that bring their sums together; none.
@@ -79,7 +79,8 @@ __device__ __forceinline__ int shared_div_up(int n, int d) { return shared_div_u
 // own: t = max(1, pages x tiles x kv heads / warps), beside tiles the next larger t that gives no more records than the other SMs have warps (two records
 // in a row take a warp twice the time); without tiles an item of more than SH_TEAM t pages goes in runs of up to SH_TEAM t to blocks, whose warps bring
 // their sums together (SH_TOGETHER).
-// What bounds it: the latency of one round of loads and of half a dozen barriers.
+// What bounds it: the latency of one round of loads (0.4 us), then of divisions, reductions and half a dozen barriers. Measured from a block's start: with
+// two sequences 2.2 us, beside tiles 3.0 to 3.6 (250 and 64 sequences), a tile's block 2.1 to 2.5.
 #define SH_ROW_TILE 16
 struct SharedPlan {
     int* own;        // [n_seqs] pages of a sequence's own part
@@ -373,7 +374,9 @@ __device__ __forceinline__ uint4 load_shared_16(const uint4* p) {
 // suit 16-byte loads: lane (g, j) = (lane / 4, lane % 4) holds of key g's row the columns 32 u + 8 j .. + 7 (two k-steps of the first product, Q
 // cut alike), and of the values of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 the columns E g .. E g + E - 1, E = D / 8, which make the n-tiles' column g. No shared
 // memory, no barrier: all of a step's keys and values are on their way at once, the next step's as soon as the registers are free again.
-// What bounds it: the latency of memory while a run is short (a page at head size 64 is one step), then the rate at which pages arrive.
+// What bounds it: the latency of memory while a run is short (a page at head size 64 is two steps), then the rate at which pages arrive.
+// Measured, the operator with plan and join: two sequences, 14 heads of 64 over 2, behind 16 pages 9.2 us; 8 behind 64 pages, up to 300 tokens of their
+// own, 10.4 us (its 2.8 MB alone 0.43).
 template <int D> struct SharedSums {
     float o[D / 8][4];       // o[t][0], o[t][1]: row g's columns 2 j E + t and (2 j + 1) E + t; o[t][2], o[t][3]: row g + 8's
     float m0, m1, l0, l1;    // rows g and g + 8: maximum and sum of weights
@@ -574,6 +577,8 @@ __device__ __forceinline__ void shared_warp(const bf16* __restrict__ q, const Kv
 // ---- the same work through shared memory, for the warps beside the tiles, of which an SM holds ten with half the registers: stages of 16 keys by 16-byte
 // asynchronous copies, so that what is on its way does not take registers. A row's 16-byte pieces are stored at c XOR (row modulo 8): neither the copies
 // nor ldmatrix meet a bank twice. Fragments as ldmatrix gives them.
+// What bounds it: the latency of a warp's few stages, ten warps an SM. Measured: the own pages of 64 sequences, 28 heads of 128 over 4, 37 MB, on the 60 SMs
+// that 88 tile records leave, 17 us, 2.1 TB/s.
 __host__ __device__ constexpr int shared_stages(int d) { return d <= 64 ? 4 : 2; }
 __host__ __device__ constexpr int shared_stage_bytes(int d) { return 2 * 16 * d * 2; }
 
@@ -771,7 +776,7 @@ shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a)
 // flight at once and the next page's while this one's are at work, and go to shared memory as float32 (padded rows: eight keys' 16 bytes meet no bank
 // twice). Thread = (key, every fourth row) for the scores, (row, 4 columns of every 64) for the sums.
 // What bounds it: shared memory's reads, 5 of 16 bytes for 16 multiply-adds in the first product and 5 for 16 in the second; a short run, latency.
-// Measured with the join, float32, head size 64, 14 heads over 2, 12 sequences behind 24 shared pages and one of their own with up to 200 tokens: 20.7 us;
+// Measured with the join, float32, head size 64, 14 heads over 2, 12 sequences behind 24 shared pages, each with up to 200 tokens of its own, and one alone: 20.0 us;
 // with loads a page late and a key's row read once per query instead, 36.6.
 #define SH_ROWS SH_ROW_TILE
 #define SH_THREADS 256

@@ -10,6 +10,8 @@
 // what follows. Then they score the tokens of the row behind the kept drafts, chunk after chunk, and the block that draws the entry's last ticket
 // picks the best. (That every block decides for itself costs less than a launch between, and than tickets in (1), which hold its blocks up: 48 entries, 346
 // rows of 151,936: (1) 32 microseconds, with tickets 49.)
+// Measured: those 48 entries 53.5 us: (1) 32, 210 MB at 6.6 TB/s, (2) 21, of which the decision 3.7; one entry of four drafts 11.2; argmaxes of 48 rows
+// of 152,064, 7.4.
 // What bounds it: memory, in (1); in (2), latency, and of the same rows out of the second-level cache the hash and the logarithm of the tokens that may
 // still win.
 //
