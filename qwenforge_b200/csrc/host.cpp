@@ -54,7 +54,7 @@ int (*attention_shared)(int, const void*, void*, const int*, const int*, const i
                         void*, const int*, long long, int, int, int, int, int, float, float*, float*, int*, const float*, int*, Stream);
 int (*copy_pages)(void*, int, int, int, long long, long long, int, long long, long long, int, const int*, int, Stream);
 int (*verify_drafts)(const float*, int, int, long long, const float*, long long, const int*, int, const int*, int, const float*, float, unsigned long long,
-                     const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
+                     unsigned long long, const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
 PyObject* kernel_error = nullptr;
 
 const struct {
@@ -411,17 +411,17 @@ PyObject* shared_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// verify_drafts(target, draft or None, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held, counters, temperature, seed, row_chunks,
-//               entry_chunks): positive temperatures. Chunks: those of a row's statistics, and of a row's race.
+// verify_drafts(target, draft or None, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held, counters, temperature, seed, redraw_seed,
+//               row_chunk, race_chunk): draws, and the greedy choice at a temperature of 0 or less. Chunks: those of a row's statistics, and of a row's race.
 PyObject* drafts_verified(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 15) return PyErr_Format(PyExc_TypeError, "verify_drafts: 15 arguments");
+    if (n != 16) return PyErr_Format(PyExc_TypeError, "verify_drafts: 16 arguments");
     const at::Tensor* t[11];
     for (int i = 0; i < 11; ++i) t[i] = tensor(args[i]);
     const at::Tensor *target = t[0], *draft = t[1], *drafted = t[2], *first = t[3], *uniforms = t[4], *ids = t[5], *steps = t[6], *accepted = t[7], *tokens = t[8];
     const double temperature = PyFloat_AsDouble(args[11]);
-    const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[12]);
-    const long long row_chunk = number(args[13]), race_chunk = number(args[14]);
+    const unsigned long long seed = PyLong_AsUnsignedLongLongMask(args[12]), redraw_seed = PyLong_AsUnsignedLongLongMask(args[13]);
+    const long long row_chunk = number(args[14]), race_chunk = number(args[15]);
     if (PyErr_Occurred()) return nullptr;
     const int device = c10::cuda::current_device();
     const bool draws = temperature > 0;
@@ -443,7 +443,7 @@ PyObject* drafts_verified(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return code_of([&] {
         return verify_drafts(target->const_data_ptr<float>(), (int)rows, (int)vocab, target->stride(0), used ? draft->const_data_ptr<float>() : nullptr,
                              used ? draft->stride(0) : 0, ints(drafted), (int)total, ints(first), (int)entries, uniforms->const_data_ptr<float>(),
-                             draws ? (float)temperature : 0.f, seed, draws ? reinterpret_cast<const long long*>(ids->const_data_ptr<int64_t>()) : nullptr,
+                             draws ? (float)temperature : 0.f, seed, redraw_seed, draws ? reinterpret_cast<const long long*>(ids->const_data_ptr<int64_t>()) : nullptr,
                              draws ? ints(steps) : nullptr, at_ptr<int>(*accepted), at_ptr<int>(*tokens), (int)tokens->size(1) - 1, held, held + row_chunks,
                              held + 2 * row_chunks, at_ptr<int>(*t[10]), stream());
     });

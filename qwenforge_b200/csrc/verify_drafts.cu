@@ -1,6 +1,7 @@
 // Verification of drafted tokens against a model's logits (float32). With p = softmax(target / T), q = softmax(draft / T):
 //   draft d_j is kept while  u_j q_j(d_j) < p_j(d_j);  the token behind the last kept one is  argmax_i r_i / E_i,  r = max(0, p - q) at a refusal
-//   (p without d where there are no draft logits) and r = p behind the last draft,  E_i = -ln u_i, u_i the sampler's number for token i of that step.
+//   (p without d where there are no draft logits) and r = p behind the last draft,  E_i = -ln u_i, u_i the sampler's number for token i of that step,
+//   under a seed of its own at a refusal with draft logits: given that d was refused, numbers that d was drawn with are no longer what they were.
 // argmax_i r_i / E_i draws i with probability r_i / sum r (independent exponential times of rate r_i: the first to go), so neither r's sum nor a
 // running sum over the vocabulary is needed, and a token turns on rounding only where two scores are equal to the last bits.
 // T <= 0: kept while it is the row's argmax (lowest id of equals); the next token is the argmax.
@@ -70,7 +71,7 @@ struct VerifyArgs {
     int rows, total, vocab, n, most, chunks, race_chunks;
     double inv_t;
     float rate;              // log2(e) / T
-    unsigned long long seed;
+    unsigned long long seed, redraw_seed;   // redraw_seed: of draws behind a refused draft that has logits
     int sampling;
 };
 
@@ -328,7 +329,8 @@ verify_draw_kernel(VerifyArgs a) {
     if (!decide(a, s, blockIdx.x == 0, made)) return;
     const float* t_row = a.target + made.row * a.t_stride;
     const float* d_row = made.d_row >= 0 ? a.draft + made.d_row * a.d_stride : nullptr;
-    const uint32_t key = row_key(a.seed, seq_id, step + made.kept);
+    // (A refused draft may have been drawn with this step's numbers under `seed`: the draw behind it must not depend on those.)
+    const uint32_t key = row_key(made.d_row >= 0 ? a.redraw_seed : a.seed, seq_id, step + made.kept);
     if (threadIdx.x == 0) low_s = 0;   // the highest lower bound that a thread has found, as bits of a float32 that is not negative
     __syncthreads();
     Contenders mine = {{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
@@ -435,15 +437,15 @@ verify_draw_kernel(VerifyArgs a) {
 // counters int32 of n, zero before the first call (the kernels leave them zero).
 QF_EXPORT int qf_verify_drafts(const float* target, int rows, int vocab, long long t_stride, const float* draft, long long d_stride, const int* drafted,
                                int total, const int* first, int n, const float* uniforms, float temperature, unsigned long long seed,
-                               const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most, double* sums, void* tops, void* best,
-                               int* counters, cudaStream_t stream) {
+                               unsigned long long redraw_seed, const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most,
+                               double* sums, void* tops, void* best, int* counters, cudaStream_t stream) {
     static_assert(sizeof(Contenders) == 32, "what the workspaces are sized by");
     if (n <= 0 || vocab <= 0) return 0;
     VerifyArgs a = {};
     a.target = target, a.draft = draft, a.t_stride = t_stride, a.d_stride = d_stride, a.drafted = drafted, a.first = first, a.uniforms = uniforms;
     a.seq_ids = seq_ids, a.steps = steps, a.accepted = accepted, a.tokens = tokens, a.sums = sums, a.tops = (float2*)tops;
     a.best = (Contenders*)best, a.counters = counters, a.rows = rows, a.total = total, a.vocab = vocab, a.n = n;
-    a.most = most, a.seed = seed, a.sampling = temperature > 0.f;
+    a.most = most, a.seed = seed, a.redraw_seed = redraw_seed, a.sampling = temperature > 0.f;
     a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_CHUNK - 1) / VR_CHUNK;
     if (a.sampling) {
         a.inv_t = 1.0 / (double)temperature;

@@ -380,7 +380,7 @@ _verify_scratch = VerifyScratch()
 
 def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: torch.Tensor, first: torch.Tensor, uniforms: torch.Tensor,
                   temperature: float, seed: int, seq_ids: torch.Tensor, steps: torch.Tensor, accepted: torch.Tensor, tokens: torch.Tensor,
-                  scratch: Optional[VerifyScratch] = None) -> None:
+                  scratch: Optional[VerifyScratch] = None, redraw_seed: Optional[int] = None) -> None:
     """Which drafted tokens a model keeps, and the token that follows them. Entry s has the rows first[s] .. first[s + 1] - 1 of
     `target` (float32 logits of the model that decides): one behind each of its drafted tokens' contexts and one behind all of them, so
     one row more than it has drafts (none at all for a padding entry). Its drafts, the rows of `draft` (float32 logits of the model that
@@ -391,7 +391,10 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     behind the last kept one is drawn from max(0, p - q), or p without d, if a draft was refused, and from p behind the last:
     the token with the largest r / E, E = -ln of the sampler's own random number for (seed, seq_ids[s], steps[s] + kept, token), where
     steps[s] counts the tokens that the sequence has generated. So kept and drawn tokens together are distributed as the model's own
-    draws. temperature <= 0: a draft is kept while it is the row's argmax (the lowest id of equals), and the next token is the argmax.
+    draws, if the uniforms, each draft and the numbers of the draw are independent. Drafts that `sample` drew for the same sequences and steps
+    are independent of them under another seed only: `redraw_seed` is the seed of draws behind a refused draft with draft logits (None:
+    `seed`, for drafts that were drawn with other numbers; `Sampler.verify` sets it). temperature <= 0: a draft is kept while it is the row's argmax (the lowest
+    id of equals), and the next token is the argmax.
 
     accepted int32 [n]: drafts kept; tokens int32 [n, most + 1]: kept drafts, the next token, then -1. An entry of no rows gets 0 and
     -1; one whose rows lie outside `target`, or with more drafts than `tokens` has room for, -1 and -1. A drafted id outside the
@@ -399,7 +402,7 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     if target.is_cuda:
         held = scratch or _verify_scratch
         code = _native("verify_drafts", "verify_drafts")(target, draft, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held.held, held.counters,
-                                                         temperature, int(seed), VERIFY_CHUNK, VERIFY_RACE_CHUNK)
+                                                         temperature, int(seed), int(seed) if redraw_seed is None else int(redraw_seed), VERIFY_CHUNK, VERIFY_RACE_CHUNK)
         if code is not None:
             kernels.launches += 1
             return _check(code, "verify_drafts")
@@ -441,9 +444,10 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
     all_rows = rows + (total if used is not None else 0)
     scratch = scratch or _verify_scratch
     places = scratch.ensure(all_rows * -(-vocab // VERIFY_CHUNK), n * -(-vocab // VERIFY_RACE_CHUNK), n, target.device)
-    code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P)(
+    code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P)(
         target.data_ptr(), rows, vocab, target.stride(0), _at(used), used.stride(0) if used is not None else 0, drafted.data_ptr(), total,
-        first.data_ptr(), n, uniforms.data_ptr(), max(float(temperature), 0.0), int(seed) & 0xFFFFFFFFFFFFFFFF, seq_ids.data_ptr() if sampling else None,
+        first.data_ptr(), n, uniforms.data_ptr(), max(float(temperature), 0.0), int(seed) & 0xFFFFFFFFFFFFFFFF,
+        int(seed if redraw_seed is None else redraw_seed) & 0xFFFFFFFFFFFFFFFF, seq_ids.data_ptr() if sampling else None,
         steps.data_ptr() if sampling else None, accepted.data_ptr(), tokens.data_ptr(), tokens.shape[1] - 1, *places, scratch.counters.data_ptr(), _stream())
     kernels.launches += all_rows > 0   # (the rows' statistics, and the decision with the draw)
     _check(code, "verify_drafts")

@@ -14,6 +14,10 @@ import torch
 from .. import ops
 
 
+# `verify` draws behind a refused draft under another seed than `__call__`, which may have drawn the draft: its own with these bits changed.
+REDRAW_BITS = 0x9E3779B97F4A7C15
+
+
 @dataclass(frozen=True)
 class SamplingParams:
     temperature: float = 0.0
@@ -45,7 +49,10 @@ class Sampler:
                steps: Optional[torch.Tensor] = None, scratch=None) -> tuple[torch.Tensor, torch.Tensor]:
         """Which drafted tokens stay, and the token behind them (`ops.verify_drafts`). logits float32 [rows, vocab]: a row per drafted
         token and one more per entry, entry s's from first[s] on; drafted int32, uniforms float32 and draft_logits float32 [.., vocab] one
-        after another; seq_ids and steps as when sampling. Returns accepted int32 [entries] and tokens int32 [entries, most + 1]."""
+        after another; seq_ids and steps as when sampling. Returns accepted int32 [entries] and tokens int32 [entries, most + 1].
+
+        Drafts that come with draft_logits may be this sampler's own draws from them, for the same seq_ids and steps, or any other's; without, they
+        must not be draws at random. The uniforms are independent of either, and new ones every time."""
         n = first.numel() - 1
         accepted = torch.empty(n, dtype=torch.int32, device=logits.device)
         tokens = torch.empty((n, most + 1), dtype=torch.int32, device=logits.device)
@@ -54,5 +61,5 @@ class Sampler:
                 raise ValueError("verify: sampling needs uniforms")
             uniforms = torch.empty(0, dtype=torch.float32, device=logits.device)
         ops.verify_drafts(logits, draft_logits, drafted, first, uniforms, self.params.temperature, self.params.seed, seq_ids, steps,
-                          accepted, tokens, scratch)
+                          accepted, tokens, scratch, redraw_seed=self.params.seed ^ REDRAW_BITS)
         return accepted, tokens
