@@ -438,7 +438,7 @@ PyObject* drafts_verified(PyObject*, PyObject* const* args, Py_ssize_t n) {
         (used && draft->stride(1) != 1))
         Py_RETURN_NONE;
     const long long row_chunks = (rows + (used ? total : 0)) * ((vocab + row_chunk - 1) / row_chunk), races = entries * ((vocab + race_chunk - 1) / race_chunk);
-    if (t[9]->numel() < 2 * row_chunks + 4 * races || t[10]->numel() < entries) Py_RETURN_NONE;
+    if (t[9]->numel() < 2 * (row_chunks + races) || t[10]->numel() < entries) Py_RETURN_NONE;
     double* held = at_ptr<double>(*t[9]);
     return code_of([&] {
         return verify_drafts(target->const_data_ptr<float>(), (int)rows, (int)vocab, target->stride(0), used ? draft->const_data_ptr<float>() : nullptr,

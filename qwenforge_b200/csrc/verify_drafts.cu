@@ -17,7 +17,8 @@
 // still win.
 //
 // Decisions are whole numbers, so they are made on sums that are good to more than float32: sums over threads and blocks and the comparison u q < p are
-// float64, and of a chunk's scores, formed in float32, those that may be the best by their error bounds are formed again in float64 where there are two or more.
+// float64 (of exponentials of 2^-20 or better, so a draft whose u q and p are closer than that may go either way). Scores are formed in float32 with bounds of
+// their errors; where two or more tokens may be the best by those, one block forms the row's sums and those tokens' scores again in float64.
 #include <float.h>
 #include <math.h>
 
@@ -39,12 +40,11 @@ struct Decision {
     float t_top, d_top, t_log, d_log;   // the rows' maxima, and the base-2 logarithms of their sums
     double t_sum, d_sum;
 };
-// The two best of some tokens by the upper bounds of their scores (0x7fffffff: none), and the highest lower bound; none of the bounds is negative.
+// Of some tokens, the best by the upper bounds of their scores (id 0x7fffffff: none), the next highest upper bound, and the highest lower bound; none of the
+// bounds is negative.
 struct __align__(16) Contenders {
-    float high[2];
-    int id[2];
-    float low;
-    int pad[3];
+    float high, second, low;
+    int id;
 };
 
 struct RowStats {
@@ -274,33 +274,33 @@ __device__ __forceinline__ bool decide(const VerifyArgs& a, int s, bool writes, 
     return a.sampling;
 }
 
-// ---- (2) the token behind the kept drafts. A score is r / E. p = 2^((x - top) rate - log2 sum): the difference, the product, the logarithm and the
-// exponent round by 2^-24 to 2^-22 each, of numbers that are at most a few tens for any token with a chance, and the hardware's exponential by 2^-22: p is
-// within 6e-6 of its value as a share. E = -ln u: near 1 by its series in w = 1 - u, which is exact in float32, else by the hardware's logarithm, within
-// 6e-6 as well. So a score lies between (p - q - 6e-6 (p + q)) (1 - 6e-6) / E and the same with other signs. A thread, a warp, a block keeps the two
-// tokens with the highest upper bounds, and the highest lower bound of all; of what the blocks leave, the tokens whose upper bound reaches the highest
-// lower bound of all may be the best: mostly one, else they are scored again in float64. (A third token of one block's within 1e-5 of the best is not
-// looked at.) Since E >= w, a token whose upper bound on p - q is below w times the lower bound so far cannot win: nearly none needs a logarithm or a
-// division. The bound goes round a warp after every four tokens of its threads, and round the block after every chunk.
-#define VR_SLACK 6.0e-6f
-__device__ __forceinline__ void keep_two(Contenders& x, float high, int id) {
-    if (high > x.high[0] || (high == x.high[0] && id < x.id[0])) {
-        x.high[1] = x.high[0], x.id[1] = x.id[0];
-        x.high[0] = high, x.id[0] = id;
-    } else if (high > x.high[1] || (high == x.high[1] && id < x.id[1])) {
-        x.high[1] = high, x.id[1] = id;
+// ---- (2) the token behind the kept drafts. A score is r / E. p = 2^((x - top) rate - log2 sum): the difference, the product and the exponent round by 2^-24
+// each of a number of bits, 1.3e-7 of p per bit; the sum is good to 2.7e-6 (weights' errors of 1.3e-7 per bit below the maximum, of which a mean has 14 at
+// most, the hardware's exponentials, eight additions in float32), its logarithm to 1e-6, the hardware's exponential to 2.4e-7. So p is within 1e-5 of its value, as a
+// share, for every token down to 2^-45 of the largest, and none below that has a chance (E is 2^-24 at the least). E = -ln u: near 1 by its series in
+// w = 1 - u, which is exact in float32, else by the hardware's logarithm, within 6e-6. So a score lies between (p - q - 1e-5 (p + q)) (1 - 1e-5) / E and the
+// same with other signs. A thread, a warp, a block keeps the token with the highest upper bound, the next highest upper bound, and the highest lower bound.
+// Where the entry's next highest upper bound is below its highest lower bound, the token with the highest is the best: nearly always, but for models so
+// close that what is left of p - q is lost in the slack; else `rescore`. Since E >= w, a token whose upper bound on p - q is below w times the lower bound
+// so far cannot win: nearly none needs a logarithm or a division. The bound goes round a warp after every four tokens of its threads, and round the
+// block after every chunk.
+#define VR_SLACK 1.0e-5f
+__device__ __forceinline__ void keep_best(Contenders& x, float high, int id) {
+    if (high > x.high || (high == x.high && id < x.id)) {
+        x.second = x.high;
+        x.high = high, x.id = id;
+    } else {
+        x.second = fmaxf(x.second, high);
     }
 }
 // Of all threads of a block, to all of them: bounds that are not negative compare as their bits do, which a warp reduces in one instruction.
 __device__ __forceinline__ Contenders of_warp(const Contenders& x) {
     Contenders y;
-    const unsigned high = __float_as_uint(x.high[0]), most = __reduce_max_sync(0xffffffffu, high);
-    y.high[0] = __uint_as_float(most);
-    y.id[0] = __reduce_min_sync(0xffffffffu, high == most ? x.id[0] : 0x7fffffff);
-    const bool gone = x.id[0] == y.id[0];   // (a lane whose best is the warp's best stands in with its second)
-    const unsigned other = __float_as_uint(gone ? x.high[1] : x.high[0]), second = __reduce_max_sync(0xffffffffu, other);
-    y.high[1] = __uint_as_float(second);
-    y.id[1] = __reduce_min_sync(0xffffffffu, other == second ? (gone ? x.id[1] : x.id[0]) : 0x7fffffff);
+    const unsigned high = __float_as_uint(x.high), most = __reduce_max_sync(0xffffffffu, high);
+    y.high = __uint_as_float(most);
+    y.id = __reduce_min_sync(0xffffffffu, high == most ? x.id : 0x7fffffff);
+    // (a lane whose best is the warp's best stands in with its second)
+    y.second = __uint_as_float(__reduce_max_sync(0xffffffffu, x.id == y.id ? __float_as_uint(x.second) : high));
     y.low = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x.low)));
     return y;
 }
@@ -311,18 +311,80 @@ __device__ __forceinline__ Contenders of_block(const Contenders& x, Contenders* 
     __syncthreads();
     if (lane == 0) room[threadIdx.x >> 5] = mine;
     __syncthreads();
-    Contenders y = {{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    Contenders y = {0.f, 0.f, 0.f, 0x7fffffff};
     if (lane < WARPS) y = room[lane];
     return of_warp(y);
 }
 
+// r and its slack for one token, r = -1 where its upper bound does not reach: reach = 2^23 / (the highest lower bound so far).
+__device__ __forceinline__ bool may_win(const VerifyArgs& a, const Decision& made, bool with_draft, float x, float y, uint32_t bits, float reach, float& r, float& slack) {
+    const float p = fast_exp2(fmaf(x - made.t_top, a.rate, -made.t_log));
+    const float q = with_draft ? fast_exp2(fmaf(y - made.d_top, a.rate, -made.d_log)) : 0.f;
+    r = p - q, slack = (p + q) * VR_SLACK;
+    // 2^23 w: 23 bits under the exponent of 2^23 are that number more than themselves. (Behind the vocabulary's end: 0 < 0, or a NaN.)
+    return __uint_as_float(0x4b000000u | (8388607u - bits)) - 8388607.5f < (r + slack) * reach;
+}
+__device__ __forceinline__ float reach_of(float low) {
+    return __fdividef(8388608.f * 1.000001f, low);   // (of the quotient's rounding, upwards; infinite as long as there is no bound)
+}
+
+// The entry's best token in float64, by all threads of a block: the rows' sums (without a draft row, scores p / E compare without them), then the scores of the
+// tokens whose upper bounds reach `low`. The lowest id of equals; 0x7fffffff where no token has a score above 0. 0.35 ms for rows of
+// 151,936: of ordinary models about one draw in 10^5 comes here, of models whose logits differ by 10^-4 or less most that follow a refusal (of which there are
+// as few as the models are close). Not inlined, so that its registers are not the others'.
+__device__ __noinline__ int rescore(const VerifyArgs& a, const Decision& made, const float* t_row, const float* d_row, uint32_t key, float low) {
+    constexpr int WARPS = VF_THREADS / 32;
+    __shared__ double part_s[2][WARPS];
+    __shared__ int id_s[WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double sum[2] = {0.0, 0.0};
+    if (d_row) {
+        for (int i = threadIdx.x; i < a.vocab; i += VF_THREADS) {
+            sum[0] += exp(((double)t_row[i] - (double)made.t_top) * a.inv_t);
+            sum[1] += exp(((double)d_row[i] - (double)made.d_top) * a.inv_t);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            sum[k] = warp_sum_f64(sum[k]);
+            if (lane == 0) part_s[k][warp] = sum[k];
+        }
+        __syncthreads();
+        sum[0] = sum[1] = 0.0;
+        for (int w = 0; w < WARPS; ++w) sum[0] += part_s[0][w], sum[1] += part_s[1][w];
+        __syncthreads();
+    }
+    const float reach = reach_of(low);
+    double best = 0.0;
+    int chosen = 0x7fffffff;
+    for (int i = threadIdx.x; i < a.vocab; i += VF_THREADS) {
+        float r32, slack;
+        const uint32_t bits = token_bits(key, (uint32_t)i);
+        if (i == made.without || !may_win(a, made, d_row != nullptr, t_row[i], d_row ? d_row[i] : 0.f, bits, reach, r32, slack)) continue;
+        double r = exp(((double)t_row[i] - (double)made.t_top) * a.inv_t);
+        if (d_row) r = r / sum[0] - exp(((double)d_row[i] - (double)made.d_top) * a.inv_t) / sum[1];
+        const double score = r / -log(((double)bits + 0.5) / 8388608.0);
+        if (score > best) best = score, chosen = i;   // (ids of a thread rise)
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const double v = __shfl_xor_sync(0xffffffffu, best, o);
+        const int i = __shfl_xor_sync(0xffffffffu, chosen, o);
+        if (v > best || (v == best && i < chosen)) best = v, chosen = i;
+    }
+    if (lane == 0) part_s[0][warp] = best, id_s[warp] = chosen;
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w)
+        if (part_s[0][w] > best || (part_s[0][w] == best && id_s[w] < chosen)) best = part_s[0][w], chosen = id_s[w];
+    return chosen;
+}
+
 __global__ void __launch_bounds__(VF_THREADS, VR_BLOCKS)
-verify_draw_kernel(VerifyArgs a) {
+verify_draw_kernel(const __grid_constant__ VerifyArgs a) {
     grid_chain_entry();
     constexpr int WARPS = VF_THREADS / 32;
     __shared__ int low_s, ticket_s;
     __shared__ Contenders best_s[WARPS];
-    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int s = blockIdx.y, lane = threadIdx.x & 31;
     const long long seq_id = a.sampling ? a.seq_ids[s] : 0;
     const int step = a.sampling ? a.steps[s] : 0;
     Decision made;
@@ -333,7 +395,7 @@ verify_draw_kernel(VerifyArgs a) {
     const uint32_t key = row_key(made.d_row >= 0 ? a.redraw_seed : a.seed, seq_id, step + made.kept);
     if (threadIdx.x == 0) low_s = 0;   // the highest lower bound that a thread has found, as bits of a float32 that is not negative
     __syncthreads();
-    Contenders mine = {{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    Contenders mine = {0.f, 0.f, 0.f, 0x7fffffff};
     float x[VR_EACH], y[VR_EACH], x_next[VR_EACH], y_next[VR_EACH];   // (the next chunk's are on their way while this one's are scored)
     auto load = [&](int begin) {
         const int end = min(a.vocab, begin + VR_CHUNK);
@@ -343,7 +405,6 @@ verify_draw_kernel(VerifyArgs a) {
     };
     load(blockIdx.x * VR_CHUNK);
     for (int begin = blockIdx.x * VR_CHUNK; begin < a.vocab; begin += gridDim.x * VR_CHUNK) {
-        const int end = min(a.vocab, begin + VR_CHUNK);
 #pragma unroll
         for (int i = 0; i < VR_EACH; ++i) x[i] = x_next[i], y[i] = y_next[i];
         load(begin + gridDim.x * VR_CHUNK);
@@ -351,18 +412,14 @@ verify_draw_kernel(VerifyArgs a) {
         const float before = low;
 #pragma unroll
         for (int u = 0; u < VR_EACH; u += 4) {
-            const float reach = __fdividef(8388608.f * 1.000001f, low);   // (of the quotient's rounding, upwards; infinite as long as there is no bound)
+            const float reach = reach_of(low);
             float r[4], slack[4];
             uint32_t bits[4];
             bool any = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = fast_exp2(fmaf(x[u + e] - made.t_top, a.rate, -made.t_log));
-                const float q = d_row ? fast_exp2(fmaf(y[u + e] - made.d_top, a.rate, -made.d_log)) : 0.f;
-                r[e] = p - q, slack[e] = (p + q) * VR_SLACK;
                 bits[e] = token_bits(key, (uint32_t)id_of(begin, u + e));
-                // 2^23 w: 23 bits under the exponent of 2^23 are that number more than themselves. (Behind the vocabulary's end: 0 < 0, or a NaN.)
-                r[e] = __uint_as_float(0x4b000000u | (8388607u - bits[e])) - 8388607.5f < (r[e] + slack[e]) * reach ? r[e] : -1.f;
+                if (!may_win(a, made, d_row != nullptr, x[u + e], y[u + e], bits[e], reach, r[e], slack[e])) r[e] = -1.f;
                 any |= r[e] > -1.f;
             }
             if (any) {
@@ -375,7 +432,7 @@ verify_draw_kernel(VerifyArgs a) {
                     const float wait = w < 0.03125f ? w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.2f, 0.25f), 0.33333333f), 0.5f), 1.f) : -0.69314718f * __log2f(v);
                     const float per = __fdividef(1.f, wait);
                     low = fmaxf(low, (r[e] - slack[e]) * (1.f - VR_SLACK) * per);
-                    keep_two(mine, fmaxf(fmaf(r[e], VR_SLACK, r[e] + slack[e]) * per, 0.f), id);
+                    keep_best(mine, fmaxf(fmaf(r[e], VR_SLACK, r[e] + slack[e]) * per, 0.f), id);
                 }
             }
             low = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(low)));
@@ -394,52 +451,30 @@ verify_draw_kernel(VerifyArgs a) {
     if (ticket_s != (int)gridDim.x - 1) return;
     __threadfence();
     // the entry's last block: what the others have left
-    mine = Contenders{{0.f, 0.f}, {0x7fffffff, 0x7fffffff}, 0.f};
+    mine = Contenders{0.f, 0.f, 0.f, 0x7fffffff};
     for (int c = threadIdx.x; c < (int)gridDim.x; c += VF_THREADS) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(all + c));
-        const float low = __ldcg(&all[c].low);
-        keep_two(mine, x.x, __float_as_int(x.z));
-        keep_two(mine, x.y, __float_as_int(x.w));
-        mine.low = fmaxf(mine.low, low);
+        const float4 other = __ldcg(reinterpret_cast<const float4*>(all + c));
+        keep_best(mine, other.x, __float_as_int(other.w));
+        mine.second = fmaxf(mine.second, other.y);
+        mine.low = fmaxf(mine.low, other.z);
     }
     mine = of_block(mine, best_s);
-    if (warp != 0) return;
-    int chosen = mine.id[0];
-    const float low = mine.low;
-    if (mine.high[1] >= low) {   // two or more may be the best
-        double best = -1.0;
-        chosen = 0x7fffffff;
-        for (int c = lane; c < (int)gridDim.x; c += 32)
-#pragma unroll 1
-            for (int k = 0; k < 2; ++k) {
-                const int id = __ldcg(&all[c].id[k]);
-                if (!(__ldcg(&all[c].high[k]) >= low) || id >= a.vocab) continue;
-                double r = exp(((double)t_row[id] - (double)made.t_top) * a.inv_t) / made.t_sum;
-                if (d_row) r = fmax(r - exp(((double)d_row[id] - (double)made.d_top) * a.inv_t) / made.d_sum, 0.0);
-                const double score = r / -log(((double)token_bits(key, (uint32_t)id) + 0.5) / 8388608.0);
-                if (score > best || (score == best && id < chosen)) best = score, chosen = id;
-            }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(0xffffffffu, best, o);
-            const int i = __shfl_xor_sync(0xffffffffu, chosen, o);
-            if (v > best || (v == best && i < chosen)) best = v, chosen = i;
-        }
-    }
-    if (lane == 0) {
+    int chosen = mine.id;
+    if (mine.second >= mine.low) chosen = rescore(a, made, t_row, d_row, key, mine.low);   // two or more may be the best
+    if (threadIdx.x == 0) {
         a.counters[s] = 0;
         a.tokens[(size_t)s * (a.most + 1) + made.kept] = chosen >= a.vocab ? 0 : chosen;
     }
 }
 
 // target [rows][t_stride >= vocab] and draft [total][d_stride] (or null) float32; drafted, uniforms [total]; first [n + 1]; accepted [n],
-// tokens [n][most + 1]. Workspaces: sums (8 bytes) and tops (8) of (rows + draft rows) x chunks of VF_CHUNK, best (32) of n x chunks of VR_CHUNK,
+// tokens [n][most + 1]. Workspaces: sums (8 bytes) and tops (8) of (rows + draft rows) x chunks of VF_CHUNK, best (16) of n x chunks of VR_CHUNK,
 // counters int32 of n, zero before the first call (the kernels leave them zero).
 QF_EXPORT int qf_verify_drafts(const float* target, int rows, int vocab, long long t_stride, const float* draft, long long d_stride, const int* drafted,
                                int total, const int* first, int n, const float* uniforms, float temperature, unsigned long long seed,
                                unsigned long long redraw_seed, const long long* seq_ids, const int* steps, int* accepted, int* tokens, int most,
                                double* sums, void* tops, void* best, int* counters, cudaStream_t stream) {
-    static_assert(sizeof(Contenders) == 32, "what the workspaces are sized by");
+    static_assert(sizeof(Contenders) == 16, "what the workspaces are sized by");
     if (n <= 0 || vocab <= 0) return 0;
     VerifyArgs a = {};
     a.target = target, a.draft = draft, a.t_stride = t_stride, a.d_stride = d_stride, a.drafted = drafted, a.first = first, a.uniforms = uniforms;

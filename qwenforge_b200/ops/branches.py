@@ -365,8 +365,8 @@ class VerifyScratch:
 
     def ensure(self, row_chunks: int, entry_chunks: int, entries: int, device) -> tuple:
         """The addresses of sums, tops and best."""
-        starts = (0, row_chunks, 2 * row_chunks)   # (sums of 8 bytes, tops of 8; what blocks leave, of 32, begins on 16)
-        need = starts[2] + 4 * entry_chunks
+        starts = (0, row_chunks, 2 * row_chunks)   # (sums of 8 bytes, tops of 8; what blocks leave, of 16, begins on 16)
+        need = starts[2] + 2 * entry_chunks
         if self.held is None or self.held.numel() < need or self.held.device != device:
             self.held = torch.empty(need, dtype=torch.float64, device=device)
         if self.counters is None or self.counters.numel() < entries or self.counters.device != device:
