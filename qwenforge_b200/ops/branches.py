@@ -4,6 +4,7 @@ pointers, the current stream, error codes."""
 from __future__ import annotations
 
 import ctypes
+import threading
 from array import array
 from itertools import chain
 from typing import Optional, Sequence
@@ -375,7 +376,30 @@ class VerifyScratch:
         return base, base + 8 * starts[1], base + 8 * starts[2]
 
 
-_verify_scratch = VerifyScratch()
+class _StreamScratches(threading.local):
+    """Of callers that bring none: one per thread and stream, since calls on two streams run at once, and two threads may launch in between each other."""
+
+    MOST = 64   # (what goes was allocated on its own stream, behind whose work its memory is used again)
+
+    def __init__(self):
+        self.held: dict = {}
+
+    def get(self, device: int, stream: int) -> VerifyScratch:
+        scratch = self.held.get((device, stream))
+        if scratch is None:
+            while len(self.held) >= self.MOST:
+                self.held.pop(next(iter(self.held)))
+            scratch = self.held[device, stream] = VerifyScratch()
+        return scratch
+
+
+_verify_scratches = _StreamScratches()
+
+
+def _callers_scratch() -> VerifyScratch:
+    if torch._C._cuda_isCurrentStreamCapturing():
+        raise KernelError("verify_drafts: a call that is captured into a graph wants a scratch of its own, which lives as long as the graph")
+    return _verify_scratches.get(torch._C._cuda_getDevice(), _stream())
 
 
 def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: torch.Tensor, first: torch.Tensor, uniforms: torch.Tensor,
@@ -398,10 +422,11 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
 
     accepted int32 [n]: drafts kept; tokens int32 [n, most + 1]: kept drafts, the next token, then -1. An entry of no rows gets 0 and
     -1; one whose rows lie outside `target`, or with more drafts than `tokens` has room for, -1 and -1. A drafted id outside the
-    vocabulary is refused. Logits are finite or -infinity. `scratch`: as in `sample`."""
+    vocabulary is refused. Logits are finite or -infinity. `scratch`: whoever captures the call into a CUDA graph passes one of
+    its own, which then lives as long as the graph; None is one that the thread's calls on the current stream share."""
     if target.is_cuda:
-        held = scratch or _verify_scratch
-        code = _native("verify_drafts", "verify_drafts")(target, draft, drafted, first, uniforms, seq_ids, steps, accepted, tokens, held.held, held.counters,
+        scratch = scratch or _callers_scratch()
+        code = _native("verify_drafts", "verify_drafts")(target, draft, drafted, first, uniforms, seq_ids, steps, accepted, tokens, scratch.held, scratch.counters,
                                                          temperature, int(seed), int(seed) if redraw_seed is None else int(redraw_seed), VERIFY_CHUNK, VERIFY_RACE_CHUNK)
         if code is not None:
             kernels.launches += 1
@@ -442,7 +467,6 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], drafted: 
             used = draft if total > 0 else None
     _here("verify_drafts", target, used, drafted, first, uniforms, accepted, tokens)
     all_rows = rows + (total if used is not None else 0)
-    scratch = scratch or _verify_scratch
     places = scratch.ensure(all_rows * -(-vocab // VERIFY_CHUNK), n * -(-vocab // VERIFY_RACE_CHUNK), n, target.device)
     code = _function("verify_drafts", "qf_verify_drafts", _P, _I, _I, _LL, _P, _LL, _P, _I, _P, _I, _P, _F, _ULL, _ULL, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P)(
         target.data_ptr(), rows, vocab, target.stride(0), _at(used), used.stride(0) if used is not None else 0, drafted.data_ptr(), total,
