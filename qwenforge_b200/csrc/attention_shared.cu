@@ -6,7 +6,9 @@
 //   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
 // The keys of the pages that a group of sequences shares are one part (or, cut into runs, several) of ALL rows of the group at once: they are
 // fetched once for members x heads rows, instead of once for every member. The keys behind them are a sequence's own parts. A last kernel joins
-// each row's parts.
+// each row's parts. A member that stands inside the shared pages does not see all of their keys. No mask would do for it in a product of all rows: what lies
+// behind its position may be anything, and a weight of 0 times a NaN is a NaN. So it takes no part in its group, and reads all of its pages as its own; the
+// group's records leave sums at its rows' places too, which the join passes over.
 //
 // Which block and warp takes which run is worked out on the device from the lengths of the step, so that a captured step can be replayed with other
 // lengths, and by every block for itself (`shared_plan`: a launch of its own for it took 5 of 11 microseconds of a small call); what is shared stands in
@@ -29,7 +31,7 @@ struct __align__(16) SharedRecord {
     int chunk;     // which rows of it: chunk * (rows of a tile) ..
     int slot;      // whose page table is read
     int p_begin, p_end;
-    int limit;     // keys below it are seen by every row (a sequence's own part: its length)
+    int limit;     // no key from here on is seen (a sequence's own part: its length); all rows see every key below
     int part;      // which of a row's parts this is
     int begin, rows;   // of a group: its first member's place, and members x heads
     int pad[2];
@@ -53,7 +55,7 @@ struct SharedArgs {
     const int* pages;
     float* part_o;    // [n_seqs * n_heads][most_parts][D]
     float* part_ml;   // [n_seqs * n_heads][most_parts][2]
-    int* part_n;      // [n_seqs] a row's shared parts | its own parts << 16
+    int* part_n;      // [n_seqs] a row's first part | how many there are << 16
     int* err;
     int n_seqs, n_groups, n_heads, kv_heads, most_parts, most_shared, most_own;
     int warps, team, tile_rows, tile_work, sms;   // (see shared_plan; tile_rows 0: no tiles)
@@ -85,8 +87,7 @@ __device__ __forceinline__ int shared_div_up(int n, int d) { return shared_div_u
 struct SharedPlan {
     int* own;        // [n_seqs] pages of a sequence's own part
     int* own_first;  // [n_seqs] its first record of its kind
-    int* slot;       // [n_groups] a live member's slot (-1: all have ended)
-    int* least;      // [n_groups] the fewest keys that a live member sees
+    int* slot;       // [n_groups] the slot of a live member that sees all that is shared (-1: there is none)
     int* rows;       // [n_groups]
     int* begin;      // [n_groups]
     int* pages;      // [n_groups]
@@ -97,7 +98,9 @@ struct SharedPlan {
     float tile_share;                 // parts of a tiled group beyond its first, for every turn
     int blocks, singles, tiles;       // records of each kind
 };
-__host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 7 * n_groups; }
+__host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 6 * n_groups; }
+// Whether a sequence at `pos` sees all of the pages that it shares.
+__device__ __forceinline__ bool shared_whole(int pos, int shared) { return pos + 1 >= shared * QF_PAGE; }
 // What an SM takes for a turn of a pair of tiles, and, with ten warps at work, for a page of 16 rows and for what a record costs besides, in microseconds
 // as measured.
 __device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.8f : 2.1f; }
@@ -146,7 +149,7 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     __shared__ int records_s[SIZES];
     SharedPlan p;
     p.own = room, p.own_first = p.own + a.n_seqs;
-    p.slot = p.own_first + a.n_seqs, p.least = p.slot + a.n_groups, p.rows = p.least + a.n_groups, p.begin = p.rows + a.n_groups;
+    p.slot = p.own_first + a.n_seqs, p.rows = p.slot + a.n_groups, p.begin = p.rows + a.n_groups;
     p.pages = p.begin + a.n_groups, p.first = p.pages + a.n_groups, p.parts = p.first + a.n_groups;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group_heads = a.n_heads / a.kv_heads;
     p.own_tiles = (group_heads + SH_ROW_TILE - 1) / SH_ROW_TILE;
@@ -156,7 +159,7 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
     if (tid < a.n_groups) begin = a.begin[tid], end = a.begin[tid + 1], pages = a.pages[tid];
     for (int g = tid; g < a.n_groups; g += THREADS) {
         if (g != tid) begin = a.begin[g], end = a.begin[g + 1], pages = a.pages[g];
-        p.slot[g] = -1, p.least[g] = 0x7fffffff, p.rows[g] = (end - begin) * group_heads, p.begin[g] = begin, p.pages[g] = pages;
+        p.slot[g] = -1, p.rows[g] = (end - begin) * group_heads, p.begin[g] = begin, p.pages[g] = pages;
     }
     if (a.n_groups > 0) __syncthreads();
     uint4 sum = make_uint4(0, 0, 0, 0);   // of this thread's items: pages x tiles, and tiles; turns of pairs of tiles, and pairs
@@ -166,22 +169,19 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
             slot = -1;
             if (s < a.n_seqs) slot = a.slots[s], pos = a.tok_pos[s], group = a.entry_group[s], shared = a.entry_pages[s];
         }
-        const int n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - shared);
+        const bool whole = shared_whole(pos, shared);
+        const int n = slot < 0 ? 0 : max(0, pos / QF_PAGE + 1 - (whole ? shared : 0));
         if (s < a.n_seqs) p.own[s] = n;
         sum.x += n * p.own_tiles, sum.y += n > 0 ? p.own_tiles : 0;
-        const bool member = slot >= 0 && group >= 0;
+        const bool member = slot >= 0 && group >= 0 && whole;
         const unsigned members = __ballot_sync(ALL, member);
         if (members == 0) continue;
         const int teller = __ffs(members) - 1, first = __shfl_sync(ALL, group, teller);
         if (__all_sync(ALL, !member || group == first)) {   // (mostly: a warp's members are of one group)
-            const int a_slot = __reduce_max_sync(ALL, member ? slot : -1), least = __reduce_min_sync(ALL, member ? pos + 1 : 0x7fffffff);
-            if (lane == teller) {
-                atomicMax(p.slot + first, a_slot);
-                atomicMin(p.least + first, least);
-            }
+            const int a_slot = __reduce_max_sync(ALL, member ? slot : -1);
+            if (lane == teller) atomicMax(p.slot + first, a_slot);
         } else if (member) {
             atomicMax(p.slot + group, slot);
-            atomicMin(p.least + group, pos + 1);
         }
     }
     if (a.n_groups > 0) __syncthreads();
@@ -300,8 +300,8 @@ __device__ __forceinline__ SharedRecord shared_group_record(const SharedArgs& a,
     int run;
     shared_cut_group(a, p, g, run);
     const int chunk = shared_div(k, p.parts[g]), part = k - chunk * p.parts[g];
-    return SharedRecord{SH_PREFIX | kind, g, chunk, p.slot[g], part * run, min((part + 1) * run, p.pages[g]), min(p.least[g], p.pages[g] * QF_PAGE), part,
-                        p.begin[g], p.rows[g], {0, 0}};
+    const int end = min((part + 1) * run, p.pages[g]);
+    return SharedRecord{SH_PREFIX | kind, g, chunk, p.slot[g], part * run, end, end * QF_PAGE, part, p.begin[g], p.rows[g], {0, 0}};
 }
 // Tile record `index`, which there is.
 __device__ __forceinline__ SharedRecord shared_tile_record(const SharedArgs& a, const SharedPlan& p, int index) {
@@ -327,39 +327,35 @@ __device__ __forceinline__ void shared_records(const SharedArgs& a, const Shared
         int run;
         const int parts = shared_cut_own(a, p, s, run), n = parts * p.own_tiles;
         if (first + n <= index) continue;
-        const int from = a.entry_pages[s], g = a.entry_group[s], shared = g >= 0 ? p.parts[g] : 0, length = a.tok_pos[s] + 1;
-        const int slot = a.slots[s];
+        const int pages = a.entry_pages[s], g = a.entry_group[s], shared = g >= 0 ? p.parts[g] : 0, pos = a.tok_pos[s];
+        const int slot = a.slots[s], from = shared_whole(pos, pages) ? pages : 0;
 #pragma unroll
         for (int w = 0; w < N; ++w) {
             const int k = index + w - first;
             if (k < 0 || k >= n) continue;
             const int chunk = shared_div(k, parts), part = k - chunk * parts;
-            to[w] = SharedRecord{SH_OWN | kind, s, chunk, slot, from + part * run, from + min((part + 1) * run, p.own[s]), length, shared + part, 0, 0, {0, 0}};
+            to[w] = SharedRecord{SH_OWN | kind, s, chunk, slot, from + part * run, from + min((part + 1) * run, p.own[s]), pos + 1, shared + part, 0, 0, {0, 0}};
         }
     }
 }
 
-// How many parts every row has, for whoever joins them: by one block of the parts' kernel.
+// Which parts every row has, for whoever joins them: by one block of the parts' kernel.
 template <int THREADS>
 __device__ __forceinline__ void shared_count_parts(const SharedArgs& a, const SharedPlan& p) {
     for (int s = threadIdx.x; s < a.n_seqs; s += THREADS) {
         int run;
-        const int g = a.entry_group[s], slot = a.slots[s];
-        a.part_n[s] = slot < 0 ? 0 : (g >= 0 ? p.parts[g] : 0) | shared_cut_own(a, p, s, run) << 16;
+        const int g = a.entry_group[s], slot = a.slots[s], shared = g >= 0 ? p.parts[g] : 0, own = shared_cut_own(a, p, s, run);
+        a.part_n[s] = slot < 0 ? 0 : shared_whole(a.tok_pos[s], a.entry_pages[s]) ? (shared + own) << 16 : shared | own << 16;
     }
 }
 
-// Row `at` of a record's subject: its place in q ([n_seqs * n_heads] rows of D), or -1 where there is no such row. (The rows of a member that has ended
-// have a place too: nobody reads what is left there.)
+// Row `at` of a record's subject: its place in q ([n_seqs * n_heads] rows of D), or -1 where there is no such row. (The rows of a member that has ended, or
+// stands inside the shared pages, have a place too: nobody reads what is left there.)
 __device__ __forceinline__ int shared_row(const SharedArgs& a, const SharedRecord& rec, int kv_heads, int kvh, int at) {
     const int G = a.n_heads / kv_heads;
     if (!(rec.kind & SH_PREFIX)) return at < G ? rec.subject * a.n_heads + kvh * G + at : -1;
     const int i = shared_div(at, G);
     return at < rec.rows ? a.members[rec.begin + i] * a.n_heads + kvh * G + at - i * G : -1;
-}
-// The keys that the row at a place sees.
-__device__ __forceinline__ int shared_seen(const SharedArgs& a, int place) {
-    return place < 0 ? 0 : a.tok_pos[place / a.n_heads] + 1;
 }
 
 // 16 bytes of shared memory, read where it says so (the compiler would read them once, ahead of the loop, into registers).
@@ -419,9 +415,7 @@ __device__ __forceinline__ void shared_warp(const bf16* __restrict__ q, const Kv
                                             uint4* query_room, SharedSums<D>& out) {
     constexpr int SIX = KEYS / 16, STEPS = QF_PAGE / KEYS, KU = D / 32, E = D / 8, NT = E;
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
-    const bool prefix = rec.kind & SH_PREFIX;
-    const int p0 = rec.p_begin, p1 = rec.p_end, steps = STEPS * (p1 - p0);
-    const int bound = prefix ? p1 * QF_PAGE : rec.limit;   // no row sees a key from here on
+    const int p0 = rec.p_begin, p1 = rec.p_end, steps = STEPS * (p1 - p0), bound = rec.limit;
     const int* table_row = site.table + (long long)rec.slot * site.table_stride;
     int table = 0;   // a lane each the numbers of 32 pages
     uint4 k[2 * SIX][KU];          // n-tile t: key 8 t + g
@@ -514,12 +508,11 @@ __device__ __forceinline__ void shared_warp(const bf16* __restrict__ q, const Kv
         if (k_at) load_keys();   // (on their way while the softmax and the second product run)
         if (live) {
             float top0 = QF_NEG_BIG, top1 = QF_NEG_BIG;
-            if (key0 + KEYS > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
-                const int see0 = prefix ? min(bound, shared_seen(a, place0)) : bound, see1 = prefix ? min(bound, shared_seen(a, place1)) : bound;
+            if (key0 + KEYS > bound) {   // values behind the last key are nobody's (0 times a NaN is not 0)
 #pragma unroll
                 for (int t = 0; t < 2 * SIX; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][e] = key0 + 8 * t + 2 * j + (e & 1) < (e >> 1 ? see1 : see0) ? s[t][e] * a.scale_log2 : QF_NEG_BIG;
+                    for (int e = 0; e < 4; ++e) s[t][e] = key0 + 8 * t + 2 * j + (e & 1) < bound ? s[t][e] * a.scale_log2 : QF_NEG_BIG;
 #pragma unroll
                 for (int r = 0; r < 4 * SIX; ++r)
                     if (key0 + r / 4 * 16 + 2 * j + (r & 1) + 8 * (r >> 1 & 1) >= bound)
@@ -587,8 +580,7 @@ __device__ __forceinline__ void shared_warp_staged(const bf16* __restrict__ q, c
                                                    unsigned char* room, SharedSums<D>& out) {
     constexpr int STAGES = shared_stages(D), BYTES = shared_stage_bytes(D), C = D / 8, KS = D / 16, NT = D / 8, STEPS = QF_PAGE / 16;
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, kv_heads = site.kv_heads;
-    const bool prefix = rec.kind & SH_PREFIX;
-    const int p0 = rec.p_begin, p1 = rec.p_end, bound = prefix ? p1 * QF_PAGE : rec.limit, steps = (min(bound, p1 * QF_PAGE) - p0 * QF_PAGE + 15) / 16;
+    const int p0 = rec.p_begin, p1 = rec.p_end, bound = rec.limit, steps = (min(bound, p1 * QF_PAGE) - p0 * QF_PAGE + 15) / 16;
     const int* table_row = site.table + (long long)rec.slot * site.table_stride;
     int table = 0;
     auto piece = [&](unsigned char* base, int r, int c) { return base + (r * C + (c ^ (r & 7))) * 16; };
@@ -646,13 +638,12 @@ __device__ __forceinline__ void shared_warp_staged(const bf16* __restrict__ q, c
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[t][e] *= a.scale_log2;
-        if (key0 + 16 > rec.limit) {   // some row may not see some key; values behind the last one are nobody's (0 times a NaN is not 0)
-            const int see0 = prefix ? min(bound, shared_seen(a, place0)) : bound, see1 = prefix ? min(bound, shared_seen(a, place1)) : bound;
+        if (key0 + 16 > bound) {   // values behind the last key are nobody's (0 times a NaN is not 0)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (key0 + 8 * t + 2 * j + (e & 1) >= (e >> 1 ? see1 : see0)) s[t][e] = QF_NEG_BIG;
+                    if (key0 + 8 * t + 2 * j + (e & 1) >= bound) s[t][e] = QF_NEG_BIG;
             for (int x = lane; x < 16 * C; x += 32)
                 if (key0 + x / C >= bound) *reinterpret_cast<uint4*>(piece(values, x / C, x % C)) = make_uint4(0, 0, 0, 0);
             __syncwarp();
@@ -801,7 +792,7 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
     float* k_s = q_s + SH_ROWS * LD;              // [64][LD]
     float* v_s = k_s + QF_PAGE * LD;              // [64][LD]
     float* p_s = v_s + QF_PAGE * LD;              // [16][64 + 4]
-    __shared__ int row_at[SH_ROWS], row_limit[SH_ROWS];
+    __shared__ int row_at[SH_ROWS];
     __shared__ float m_s[SH_ROWS], l_s[SH_ROWS], corr_s[SH_ROWS];
     __shared__ SharedRecord record_s;
     grid_launch_dependents();
@@ -818,7 +809,7 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
         shared_records<SH_THREADS, 1>(a, plan, tid, 0, unit / kv_heads, &record_s);
         __syncthreads();
         const SharedRecord rec = record_s;
-        const int bound = rec.kind & SH_PREFIX ? rec.p_end * QF_PAGE : rec.limit;
+        const int bound = rec.limit;
         const int* table_row = site.table + (long long)rec.slot * site.table_stride;
         float4 keys[EACH], values[AHEAD ? EACH : 1];
         // A row of a page: null where there is none to read (zeros then): behind the run, behind its last key, a page that is not held.
@@ -841,7 +832,6 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
         if (AHEAD) bring(row ? row + to_values : nullptr, values);
         if (tid < SH_ROWS) {
             row_at[tid] = shared_row(a, rec, kv_heads, kvh, SH_ROWS * rec.chunk + tid);
-            row_limit[tid] = min(bound, shared_seen(a, row_at[tid]));
             m_s[tid] = QF_NEG_BIG;
             l_s[tid] = 0.f;
         }
@@ -877,7 +867,7 @@ shared_parts_generic_kernel(const T* __restrict__ q, KvSite<T> site, SharedArgs 
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    p_s[(r0 + 4 * i) * (QF_PAGE + 4) + key] = !missing && p * QF_PAGE + key < row_limit[r0 + 4 * i] ? s[i] * a.scale_log2 : QF_NEG_BIG;
+                    p_s[(r0 + 4 * i) * (QF_PAGE + 4) + key] = !missing && p * QF_PAGE + key < bound ? s[i] * a.scale_log2 : QF_NEG_BIG;
             }
             if (AHEAD) put(values, v_s);
             else {
@@ -962,9 +952,10 @@ shared_join_kernel(SharedArgs a, int D, T* __restrict__ out, const float* __rest
     const int head = (int)((unsigned)i / (unsigned)per), d = (i - head * per) * V, row = entry * a.n_heads + head;
     const bool there = head < a.n_heads;
     grid_dependency_wait();
-    const int packed = there ? a.part_n[entry] : 0, runs = (packed & 0xffff) + (packed >> 16);
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.most_parts;
-    const float* po = a.part_o + (size_t)row * a.most_parts * D + d;
+    const int packed = there ? a.part_n[entry] : 0, runs = packed >> 16;
+    const size_t first = (size_t)row * a.most_parts + (packed & 0xffff);
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
+    const float* po = a.part_o + first * D + d;
     float top = QF_NEG_BIG, den = 0.f, num[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) num[e] = 0.f;
@@ -1041,7 +1032,7 @@ static size_t shared_generic_smem(int d, int plan_ints) {
 
 // What sizes the launches and the workspaces. sizes[0]: rows of a tile; [1]: warps (or blocks, of the kernel for any type) that run at once; [2]: warps of
 // a block that bring their sums together; [3]: the most parts of an item; [4], [5]: a group of so many rows, and rows x pages, goes to the tiles (0: there are
-// none), [7] if the plan takes no more than so many ints (2 a sequence, 7 a group); [6]: SMs.
+// none), [7] if the plan takes no more than so many ints (2 a sequence, 6 a group); [6]: SMs.
 QF_EXPORT int qf_attention_shared_shape(int is_bf16, int head_dim, int* sizes) {
     const int sms = qf_sm_count();
     if (sms <= 0 || head_dim <= 0 || head_dim > 256) return (int)cudaErrorInvalidValue;
@@ -1109,7 +1100,7 @@ QF_EXPORT int qf_attention_shared(int is_bf16, const void* q, void* out, const i
                                   const float* sinks, int* err, cudaStream_t stream) {
     int sizes[8];
     if (n_seqs <= 0 || n_seqs > SH_MAX_SEQS || n_groups > n_seqs || kv_heads <= 0 || n_heads % kv_heads || most_units <= 0 || most_own <= 0 || most_own > 0x7fff ||
-        most_shared > 0xffff || (n_groups > 0 && most_shared <= 0))
+        most_shared > 0x7fff - most_own || (n_groups > 0 && most_shared <= 0))
         return (int)cudaErrorInvalidValue;
     const int bad = qf_attention_shared_shape(is_bf16, head_dim, sizes);
     if (bad) return bad;

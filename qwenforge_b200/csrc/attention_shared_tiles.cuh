@@ -7,9 +7,9 @@
 //                    sum; the weights go back over the scores as bf16, the left operand of the second product
 //   warp 8           issues the products: O += P V of a tile as soon as its weights are written, then S = Q K^T of its next turn
 //   warp 9           issues the copies
-// There is no causal mask: a row sees every key of the run, but for a member that stands inside the shared pages and for the half turn behind an odd
-// page count. At the end every row leaves its sums, unnormalised and in float32, with its reference maximum and its sum of weights; a warp's rows go
-// through the room that their queries had, so that they are written 128 bytes or more at a time.
+// There is no causal mask: a row sees every key of the run, and only the half turn behind an odd page count is masked. At the end every row leaves its sums,
+// unnormalised and in float32, with its reference maximum and its sum of weights; a warp's rows go through the room that their queries had, so that they
+// are written 128 bytes or more at a time.
 // Blocks without a tile record give their ten warps the records of everything else, at the same time: sequences' own pages and small groups'.
 // What bounds it: 16,384 exponentials a tile and turn on the SM's special-function units, beside as many cycles of products at D = 128, and the chain scores,
 // exponentials, product of a tile, of which two overlap; a short run, the way to its first scores (plan, queries: 4 to 5 us) and its sums' way out (2.7 us).
@@ -230,7 +230,6 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
                 if ((threadIdx.x & 31) == 0) mbar_arrive(&bar_q);
             }
             if (t < tiles) {
-            const int see = rec.limit >= end ? end : min(end, shared_seen(a, place)), all_see = min(end, rec.limit);
             const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + 128 * t, o_at = lanes + O_COL + 128 * t;
             const float folded = a.scale_log2 > 0.f ? a.scale_log2 : 1.f;
             float m_ref = QF_NEG_BIG, l_run = 0.f;   // the reference maximum of the exponentials, and their sum
@@ -247,9 +246,9 @@ shared_tiles_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* __re
                     for (int i = 0; i < ST_BK; ++i) s[i] *= a.scale_log2;
                 }
                 const int key0 = (rec.p_begin + 2 * j) * QF_PAGE;
-                if (key0 + ST_BK > all_see) {   // a key that the row does not see gets the weight 2^-inf = 0
+                if (key0 + ST_BK > end) {   // the second page is none: weights of 2^-inf = 0, and the products leave it out
 #pragma unroll
-                    for (int i = 0; i < ST_BK; ++i) s[i] = key0 + i < see ? s[i] : -INFINITY;
+                    for (int i = QF_PAGE; i < ST_BK; ++i) s[i] = -INFINITY;
                 }
                 float mx[4];  // four chains instead of one: the comparisons do not wait for each other
 #pragma unroll

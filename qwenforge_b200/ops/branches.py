@@ -261,7 +261,7 @@ def _shared_sizes(dtype, head_dim: int, kv_heads: int, n_heads: int, share: Shar
     most_shared = max((parts(share.bound_pages, t) for t in tiles), default=0)
     rows = [len(entries) * group_heads for entries, _ in share.groups]
     pairs = [-(-r // 256) for r in rows if r >= tile_rows and r * share.bound_pages >= tile_work]
-    if not tile_rows or 2 * share.n_seqs + 7 * len(share) > tile_ints:
+    if not tile_rows or 2 * share.n_seqs + 6 * len(share) > tile_ints:
         pairs = []
     if pairs:   # (everything else is cut for single warps then)
         most_shared = max(most_shared, min(most // 4, share.bound_pages))
@@ -304,7 +304,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
                      max_kv_len: Optional[int] = None, sinks: Optional[torch.Tensor] = None) -> None:
     """Attention of ONE new token per sequence over its cache, where sequences share their first pages (`share`): what they share is read
     once for all of them. The result is that of `attention_decode`: query head i reads kv head i // (n_heads / kv_heads), key j is visible
-    iff j <= the token's position. bfloat16 or float32, head sizes up to 256 (bfloat16 of 32, 64, 96 and 128 on tensor cores). A padding
+    iff j <= the token's position (a token that stands inside the pages that it shares has them read for itself alone). bfloat16 or float32, head sizes up to 256 (bfloat16 of 32, 64, 96 and 128 on tensor cores). A padding
     entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page table
     has room for); it sizes the workspaces and the launch. `sinks` (float32 [n_heads]): a logit per head that joins the softmax's denominator
     once, with no key and no value."""
