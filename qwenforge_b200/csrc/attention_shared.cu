@@ -210,7 +210,8 @@ __device__ __forceinline__ SharedPlan shared_plan(const SharedArgs& a, int* room
         const float tile_time = turns * shared_turn_time(head_dim), page_time = work * shared_page_time(head_dim) + items * SH_RECORD_TIME;
         const float half = SH_TILE_LAG * a.sms - tile_time - page_time, x = (half + sqrtf(half * half + 4.f * SH_TILE_LAG * tile_time * a.sms)) / (2.f * SH_TILE_LAG);
         // (by a little less than the quotient, so that no rounding makes it one record more)
-        const float sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(x), 1.f), a.sms - 1.f);
+        const float shared_sms = work == 0.f ? (float)a.sms : fminf(fmaxf(floorf(x), 1.f), a.sms - 1.f);
+        const float sms = turns == 0.f ? 0.f : shared_sms;   // (no tiles this time: what a graph's groups share now may be too little, or they have ended)
         if (turns > 0.f) p.tile_share = fmaxf(sms - pairs, 0.f) / turns * 0.9999f;
         warps = (int)fmaxf((float)gridDim.x - fmaxf(sms, pairs), 1.f) * WARPS;
         for (int g0 = 0; g0 < a.n_groups; g0 += 32) {   // every warp counts for itself
