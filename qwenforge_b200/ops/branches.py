@@ -175,6 +175,7 @@ class SharedPrefix:
         if 0 < bound_pages < self.most_pages:
             raise KernelError(f"SharedPrefix: a group shares {self.most_pages} pages, more than the bound of {bound_pages}")
         self.bound_pages = max(self.most_pages, int(bound_pages))
+        self.columns = 1 << 30   # the fewest that a page table of its calls has had
         self.saved_pages = self._saved()
         self.least_pages = 0 if bound_pages else min(entry_pages)
         sizes = (self.n_seqs, self.n_seqs, len(members), len(begin), len(pages))
@@ -198,8 +199,8 @@ class SharedPrefix:
 
     def load(self, other: "SharedPrefix") -> None:
         """Take over what `other`, of the same members per group and within the bound, says is shared; the addresses stay."""
-        if other.shape()[:2] != self.shape()[:2] or other.most_pages > self.bound_pages:
-            raise KernelError("SharedPrefix: what is loaded has other groups, or more pages than the bound")
+        if other.shape()[:2] != self.shape()[:2] or other.most_pages > min(self.bound_pages, self.columns):
+            raise KernelError("SharedPrefix: what is loaded has other groups, or more pages than the bound or the page table has room for")
         for name in ("entry_pages", "entry_group", "members", "begin", "pages"):
             getattr(self, name).copy_(getattr(other, name))
         self.groups, self.most_pages, self.saved_pages = other.groups, other.most_pages, other.saved_pages
@@ -309,6 +310,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok
     has room for); it sizes the workspaces and the launch. `sinks` (float32 [n_heads]): a logit per head that joins the softmax's denominator
     once, with no key and no value."""
     storage, table, d, kv_heads, dtype = site.storage, site.table, site.head_dim, site.kv_heads, q.dtype
+    if table.dim() == 2 and table.shape[1] < share.columns:
+        share.columns = table.shape[1]   # (a graph of this call reads no further, whatever is loaded later)
     if q.is_cuda and table.dim() == 2:
         sizes = share.sizes.get((dtype, d, kv_heads, n_heads, _own_pages(max_kv_len, table, share)))   # (there from the second call on)
         if sizes is not None:
