@@ -484,7 +484,7 @@ QF_EXPORT int qf_verify_drafts(const float* target, int rows, int vocab, long lo
     a.chunks = (vocab + VF_CHUNK - 1) / VF_CHUNK, a.race_chunks = (vocab + VR_CHUNK - 1) / VR_CHUNK;
     if (a.sampling) {
         a.inv_t = 1.0 / (double)temperature;
-        a.rate = (float)(1.4426950408889634 * a.inv_t);
+        a.rate = (float)fmin(1.4426950408889634 * a.inv_t, (double)FLT_MAX);   // (an infinite one times a difference of 0 would be no number)
     }
     const long long all = (long long)rows + (draft ? total : 0);
     if (n > 65535 || all > 65535) return (int)cudaErrorInvalidValue;
