@@ -109,6 +109,21 @@ class BundleNeed:
                 yield prefix + (name,), need
 
 
+def tokens_for_continuations(needs: Sequence[Optional[object]], sequences: Sequence[tuple[int, int]], continuations: int, max_seqs: int) -> int:
+    """Cache tokens that the groups of one row per several positions ask for where every sequence, (prompt length, longest length), is continued
+    `continuations` times: such a group has its share of the cache's pages and one more per sequence, while each continuation holds a copy of the page
+    that its prompt has begun and those behind it."""
+    flat = [inner for need in needs for inner in ([n for _, n in need.flat()] if isinstance(need, BundleNeed) else [need])]
+    tokens = 0
+    for every in {need.every for need in flat if isinstance(need, KvNeed) and need.every > 1}:
+        pages = 0
+        for prompt, total in sequences:
+            rows, begun = total // every, prompt // every // PAGE_TOKENS * PAGE_TOKENS
+            pages += round_up(rows, PAGE_TOKENS) // PAGE_TOKENS + (continuations - 1) * (round_up(rows - begun, PAGE_TOKENS) // PAGE_TOKENS)
+        tokens = max(tokens, PAGE_TOKENS * max(pages, every * (pages - max_seqs)))
+    return tokens
+
+
 class BundleSite:
     """The sites of a schedule entry that keeps several things, by the names its `BundleNeed` gave them."""
 

@@ -19,7 +19,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from ..cache import PAGE_TOKENS, CacheFull, round_up
+from ..cache import PAGE_TOKENS, CacheFull, round_up, tokens_for_continuations
 from ..sampling import Sampler, SamplingParams
 from ..weights.resolve import resolve_model_dir
 from .generate import GenerationLoop, SequenceResult
@@ -141,6 +141,9 @@ class StudentEngine:
             tokens = sum(round_up(max(prompt_lengths[i], 1) + max(budgets[i], 1), PAGE_TOKENS) for i in chunk)
             # (a further continuation holds the pages behind the prompt's whole ones)
             tokens += (continuations - 1) * sum(round_up(max(prompt_lengths[i], 1) % PAGE_TOKENS + max(budgets[i], 1), PAGE_TOKENS) for i in chunk)
+            if continuations > 1:
+                totals = [(max(prompt_lengths[i], 1), max(prompt_lengths[i], 1) + max(budgets[i], 1)) for i in chunk]
+                tokens = max(tokens, tokens_for_continuations(self.model.cache_needs(), totals, continuations, len(chunk) * continuations))
             need_tokens, need_seqs = max(need_tokens, tokens), max(need_seqs, len(chunk) * continuations)
         if self._max_cache_tokens is not None:
             if need_tokens > self._max_cache_tokens:
