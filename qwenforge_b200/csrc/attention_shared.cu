@@ -39,6 +39,9 @@ struct __align__(16) SharedRecord {
 #define SH_TEAM 4            // warps of a block of the parts' kernel
 #define SH_MAX_SEQS 2048
 #define SH_TILE_PLAN_INTS 12288
+// Beside tiles, microseconds (`shared_plan`): a page of 16 rows at head sizes 64 and 128 with ten warps of an SM at work, what a record costs besides, and how
+// much longer than the others' blocks a tile's takes to and from its turns. Fitted to the blocks' times of two cases (attention_shared_tiles.cuh): the own pages
+// of 250 sequences on 22 SMs 21 to 23 (estimate with the lag: 21), of 64 sequences on 60 SMs 17 (15).
 #define SH_PAGE_TIME_64 0.24f
 #define SH_PAGE_TIME_128 0.5f
 #define SH_RECORD_TIME 0.35f
@@ -101,8 +104,7 @@ struct SharedPlan {
 __host__ __device__ constexpr int shared_plan_ints(int n_seqs, int n_groups) { return 2 * n_seqs + 6 * n_groups; }
 // Whether a sequence at `pos` sees all of the pages that it shares.
 __device__ __forceinline__ bool shared_whole(int pos, int shared) { return pos + 1 >= shared * QF_PAGE; }
-// What an SM takes for a turn of a pair of tiles, and, with ten warps at work, for a page of 16 rows and for what a record costs besides, in microseconds
-// as measured.
+// What an SM takes for a turn of a pair of tiles, microseconds (126 blocks of 14 turns 26 at head size 64, 88 of 6 13 at 128), and for a page.
 __device__ __forceinline__ float shared_turn_time(int d) { return d <= 64 ? 1.8f : 2.1f; }
 __device__ __forceinline__ float shared_page_time(int d) { return d <= 64 ? SH_PAGE_TIME_64 : SH_PAGE_TIME_128; }
 
@@ -372,7 +374,7 @@ __device__ __forceinline__ uint4 load_shared_16(const uint4* p) {
 // cut alike), and of the values of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 the columns E g .. E g + E - 1, E = D / 8, which make the n-tiles' column g. No shared
 // memory, no barrier: all of a step's keys and values are on their way at once, the next step's as soon as the registers are free again.
 // What bounds it: the latency of memory while a run is short (a page at head size 64 is two steps), then the rate at which pages arrive.
-// Measured, the operator with plan and join: two sequences, 14 heads of 64 over 2, behind 16 pages 9.2 us; 8 behind 64 pages, up to 300 tokens of their
+// Measured, the operator with plan and join: two sequences, 14 heads of 64 over 2, behind 16 pages 9.4 us; 8 behind 64 pages, up to 300 tokens of their
 // own, 10.4 us (its 2.8 MB alone 0.43).
 template <int D> struct SharedSums {
     float o[D / 8][4];       // o[t][0], o[t][1]: row g's columns 2 j E + t and (2 j + 1) E + t; o[t][2], o[t][3]: row g + 8's
@@ -768,7 +770,7 @@ shared_parts_kernel(const bf16* __restrict__ q, KvSite<bf16> site, SharedArgs a)
 // flight at once and the next page's while this one's are at work, and go to shared memory as float32 (padded rows: eight keys' 16 bytes meet no bank
 // twice). Thread = (key, every fourth row) for the scores, (row, 4 columns of every 64) for the sums.
 // What bounds it: shared memory's reads, 5 of 16 bytes for 16 multiply-adds in the first product and 5 for 16 in the second; a short run, latency.
-// Measured with the join, float32, head size 64, 14 heads over 2, 12 sequences behind 24 shared pages, each with up to 200 tokens of its own, and one alone: 20.0 us;
+// Measured with the join, float32, head size 64, 14 heads over 2, 12 sequences behind 24 shared pages, each with up to 200 tokens of its own, and one alone: 19.0 us;
 // with loads a page late and a key's row read once per query instead, 36.6.
 #define SH_ROWS SH_ROW_TILE
 #define SH_THREADS 256

@@ -13,8 +13,8 @@
 // Blocks without a tile record give their ten warps the records of everything else, at the same time: sequences' own pages and small groups'.
 // What bounds it: 16,384 exponentials a tile and turn on the SM's special-function units, beside as many cycles of products at D = 128, and the chain scores,
 // exponentials, product of a tile, of which two overlap; a short run, the way to its first scores (plan, queries: 4 to 5 us) and its sums' way out (2.7 us).
-// Measured: 250 sequences, 14 heads of 64 over 2, behind 250 pages: the turns of 126 blocks 26 us, 550 TFLOP/s, the operator 36.4; 64 sequences, 28 heads of
-// 128 over 4, behind 128 pages, 88 blocks: turns 13 us, the operator 27.3. Tried with the first of them, at 38.4 us then: a warp for each tile's products
+// Measured: 250 sequences, 14 heads of 64 over 2, behind 250 pages: the turns of 126 blocks 26 us, 550 TFLOP/s, the operator 35.6; 64 sequences, 28 heads of
+// 128 over 4, behind 128 pages, 88 blocks: turns 13 us, the operator 27.0. Tried with the first of them, at 38.4 us then: a warp for each tile's products
 // 43.6; that with a page a turn and the next page's scores formed meanwhile 40.4; the tiles' exponentials strictly in turn 39.9.
 // Every wait is bounded: one that runs out sets QF_ERR_COPY_TIMEOUT and ends the thread's loop, and the block still frees its tensor memory and returns.
 #pragma once

@@ -11,8 +11,8 @@
 // what follows. Then they score the tokens of the row behind the kept drafts, chunk after chunk, and the block that draws the entry's last ticket
 // picks the best. (That every block decides for itself costs less than a launch between, and than tickets in (1), which hold its blocks up: 48 entries, 346
 // rows of 151,936: (1) 32 microseconds, with tickets 49.)
-// Measured: those 48 entries 53.5 us: (1) 32, 210 MB at 6.6 TB/s, (2) 21, of which the decision 3.7; one entry of four drafts 11.2; argmaxes of 48 rows
-// of 152,064, 7.4.
+// Measured: those 48 entries 53.3 us: (1) 32, 210 MB at 6.6 TB/s, (2) 21, of which the decision 3.7; one entry of four drafts 10.0; argmaxes of 48 rows
+// of 152,064, 7.1.
 // What bounds it: memory, in (1); in (2), latency, and of the same rows out of the second-level cache the hash and the logarithm of the tokens that may
 // still win.
 //
@@ -31,7 +31,7 @@
 #define VR_EACH 8                              // tokens of a thread and chunk in (2)
 #define VR_CHUNK (VF_THREADS * VR_EACH)
 // Blocks of an SM at once. Tokens of a thread / blocks, one entry of four drafts and 48 of up to seven (the kernel's and (1)'s microseconds, vocabulary of
-// 151,936): 8 / 3 11.1 and 53.4; 8 / 4 11.5 and 55.1 (registers spill); 8 / 5 12.0 and 56.9; 4 / 6 11.0 and 57.9; 4 / 8 17.1 and 71.7; 16 / 2 11.8 and 54.0.
+// 151,936): 8 / 3 10.0 and 53.4; 8 / 4 11.0 and 54.3; 8 / 5 11.6 and 57.0; 4 / 6 11.7 and 58.9; 4 / 8 16.0 and 63.8 (registers spill); 16 / 2 11.2 and 53.3.
 #define VR_BLOCKS 3
 
 // What a block has decided.

@@ -8,7 +8,9 @@ sequence's whole budget, so a replay needs no host work at all and the host read
 per chunk of steps.
 
 A captured graph is keyed by (rows, bound on the longest sequence, sampling temperature and seed): the bound fixes
-how the decode attention splits its key range, the sampling scalars are arguments of the sampling kernel. Graphs
+how the decode attention splits its key range, the sampling scalars are arguments of the sampling kernel. Where rows'
+sequences begin with the same pages and reading those once pays, the groups' member counts and a bound on their pages are in
+the key too, and which rows and pages they are is loaded anew for every batch. Graphs
 are kept and replayed by later batches of the same key (the reference's registry, :1081-1118). Rows that end early
 stay in the launch as padding entries (slot -1), which touch no cache and change no result.
 """
