@@ -1,0 +1,196 @@
+"""Python entries of the kernels for a sequence cache in 8 bits: written with the rotation, read back, attended over. The same manner as
+`kernels.py`: checks on the host, raw device pointers, the current stream, error codes.
+
+The cache holds an e4m3 code per element (`torch.float8_e4m3fn`) and a float32 power of two per page of 64 positions, plane (keys,
+values) and kv head; an element stands for code * scale."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import kernels
+from .branches import PAGE_TOKENS, _F, _I, _LL, _P, _at, _function, _here, _stream
+from .kernels import KernelError, _check, _dev
+
+E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128)
+E4M3_ROWS = 16     # query rows of a block of the attention (EA_ROWS)
+E4M3_WARPS = 4     # pages that a block has at work, and takes at the least where a sequence is cut (EA_WARPS)
+
+
+class E4m3SiteArgs:
+    """What the kernels need to address one schedule entry's keys and values in 8 bits. storage: float8_e4m3fn [pages, 2, kv_heads, 64,
+    head_dim], scales: float32 [pages, 2, kv_heads] (a page of each dense, pages at any distance of 16 bytes' multiple), table: int32 [slots, columns]."""
+    __slots__ = ("storage", "scales", "table", "kv_heads", "head_dim")
+
+    def __init__(self, storage: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, kv_heads: int, head_dim: int):
+        _dev("cache", storage, torch.float8_e4m3fn, contiguous=False)
+        _dev("scales", scales, torch.float32, contiguous=False)
+        _dev("page table", table, torch.int32, contiguous=False)
+        page = kv_heads * PAGE_TOKENS * head_dim
+        if head_dim not in E4M3_HEAD_DIMS:
+            raise KernelError(f"a cache in 8 bits has head sizes {', '.join(map(str, E4M3_HEAD_DIMS))}, not {head_dim}")
+        if kv_heads <= 0 or storage.dim() != 5 or storage.shape[1:] != (2, kv_heads, PAGE_TOKENS, head_dim) or not storage[:1].is_contiguous():
+            raise KernelError(f"a cache in 8 bits is [pages, 2, kv_heads, {PAGE_TOKENS}, head_dim], a page dense")
+        if scales.shape != (storage.shape[0], 2, kv_heads) or not scales[:1].is_contiguous():
+            raise KernelError("the scales of a cache in 8 bits are [pages, 2, kv_heads], a page dense")
+        if storage.shape[0] > 1 and (storage.stride(0) < 2 * page or storage.stride(0) % 16 or scales.stride(0) < 2 * kv_heads):
+            raise KernelError("the pages of a cache in 8 bits overlap, or do not begin on 16 bytes")
+        if storage.data_ptr() % 16:
+            raise KernelError("a cache in 8 bits begins on 16 bytes")
+        if table.dim() != 2 or table.stride(1) != 1 or table.shape[0] < 1 or table.shape[1] < 1:
+            raise KernelError("the page table is [slots, pages] with unit inner stride")
+        self.storage, self.scales, self.table, self.kv_heads, self.head_dim = storage, scales, table, kv_heads, head_dim
+
+    def address(self) -> tuple:
+        """codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim"""
+        s, c, t = self.storage, self.scales, self.table
+        one = s.shape[0] == 1
+        return (s.data_ptr(), c.data_ptr(), t.data_ptr(), 2 * self.kv_heads * PAGE_TOKENS * self.head_dim if one else s.stride(0),
+                2 * self.kv_heads if one else c.stride(0), t.stride(0), t.shape[1], t.shape[0], self.kv_heads, self.head_dim)
+
+
+_SITE = (_P, _P, _P, _LL, _LL, _I, _I, _I, _I, _I)
+
+
+def _batch(what: str, cu_q, tok_pos, slots, err) -> None:
+    for name, t in (("cu_q", cu_q), ("tok_pos", tok_pos), ("slots", slots), ("err", err)):
+        _dev(name, t, torch.int32)
+    if cu_q.numel() != slots.numel() + 1:
+        raise KernelError(f"{what}: cu_q has one element more than slots")
+
+
+def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor,
+                          inv_freq: Optional[torch.Tensor], rot_dim: int, n_heads: int, q_out: torch.Tensor, site: E4m3SiteArgs, max_q_len: int,
+                          err: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+    """`rope_cache_write` into a cache in 8 bits: qkv [T, (NH + 2 KVH) D] (bfloat16 or float32; perhaps the first columns of wider rows) with its bias, q and
+    k heads rotated by position (split halves of the first rot_dim components; inv_freq None: not at all), q to q_out [T, NH D], k and v
+    as codes. Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at most max_q_len, at consecutive positions; a slot is in one entry at
+    most, and no other sequence holds a page that it writes.
+
+    A page that gets rows takes, per plane and head, the least power of two under which all their finite elements lie within +-448 (of 2^-112
+    to 2^119), and no less than it has if it held rows before the new ones; those rows' codes are then rounded to the larger unit. Rounding is
+    to nearest even, once, from float32. Infinities become +-448, NaN stays. Rows behind the new ones stay as they are; a padding
+    entry (slot -1) writes its queries only."""
+    dtype = qkv.dtype
+    is_bf16 = kernels._is_bf16(dtype)
+    kernels._rows("qkv", qkv)
+    _dev("q_out", q_out, dtype)
+    _dev("tok_seq", tok_seq, torch.int32)
+    _batch("rope_cache_write_e4m3", cu_q, tok_pos, slots, err)
+    n, d, kv_heads = qkv.shape[0], site.head_dim, site.kv_heads
+    width = (n_heads + 2 * kv_heads) * d
+    if n_heads <= 0 or qkv.shape[1] < width or q_out.shape != (n, n_heads * d):
+        raise KernelError("rope_cache_write_e4m3: qkv/q_out widths do not match the head counts")
+    if tok_seq.numel() != n or tok_pos.numel() != n:
+        raise KernelError("rope_cache_write_e4m3: tok_seq and tok_pos have one element per token")
+    if bias is not None:
+        _dev("bias", bias, dtype)
+        if bias.numel() != width:
+            raise KernelError("rope_cache_write_e4m3: bias must have one element per projection column")
+    if inv_freq is not None:
+        _dev("inv_freq", inv_freq, torch.float32)
+        if not 0 <= rot_dim <= d or inv_freq.numel() * 2 != rot_dim:
+            raise KernelError("rope_cache_write_e4m3: inv_freq must hold rot_dim / 2 frequencies, rot_dim at most head_dim")
+    if n and max_q_len <= 0:
+        raise KernelError("rope_cache_write_e4m3: max_q_len is the most tokens of an entry")
+    _here("rope_cache_write_e4m3", qkv, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, site.storage, site.scales, site.table, err, bias)
+    if n == 0:
+        return
+    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _P, _P)(
+        is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
+        n_heads, q_out.data_ptr(), *site.address(), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
+
+
+def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_seqs: int, max_kv_len: int,
+                    err: torch.Tensor, window: int = 0) -> None:
+    """The rows that a batch's sequences hold, back as values: out [pages, 2, kv_heads, 64, head_dim] (bfloat16 or float32, exact in both), at the
+    page numbers of the cache, so that its page table serves both. Of entry s the rows up to its last new token's, from the first that a
+    window of `window` positions (0: all) leaves its first one; every other row of `out` stays as it is. `max_kv_len`: an upper bound of any
+    sequence's length."""
+    is_bf16 = kernels._is_bf16(out.dtype)
+    _dev("out", out, contiguous=False)
+    _batch("cache_read_e4m3", cu_q, tok_pos, slots, err)
+    storage, kv_heads, d = site.storage, site.kv_heads, site.head_dim
+    if out.shape != storage.shape or not out[:1].is_contiguous() or (out.shape[0] > 1 and (out.stride(0) < 2 * kv_heads * PAGE_TOKENS * d or out.stride(0) % 8)):
+        raise KernelError("cache_read_e4m3: out has the cache's shape, a page dense")
+    if out.data_ptr() % 16:
+        raise KernelError("cache_read_e4m3: out begins on 16 bytes")
+    if slots.numel() != n_seqs or window < 0 or (n_seqs and max_kv_len <= 0):
+        raise KernelError("cache_read_e4m3: wants n_seqs slots, a window of 0 or more and a bound on the lengths")
+    _here("cache_read_e4m3", out, cu_q, tok_pos, slots, storage, site.scales, site.table, err)
+    if n_seqs == 0:
+        return
+    pages = min(-(-int(max_kv_len) // PAGE_TOKENS), site.table.shape[1])
+    _check(_function("cache_e4m3", "qf_cache_read_e4m3", _I, _P, _LL, _P, _P, _P, *_SITE, _I, _I, _I, _P, _P)(
+        is_bf16, out.data_ptr(), 2 * kv_heads * PAGE_TOKENS * d if out.shape[0] == 1 else out.stride(0), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(),
+        *site.address(), n_seqs, pages, window, err.data_ptr(), _stream()), "cache_read_e4m3")
+
+
+class E4m3Scratch:
+    """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). One
+    instance serves calls that run one after another on one stream; what is captured into a graph has one of its own."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        self.part_o = self.part_ml = self.tickets = None
+
+    def ensure(self, records: int, pairs: int, head_dim: int) -> None:
+        if self.part_o is None or self.part_o.numel() < records * E4M3_ROWS * head_dim:
+            self.part_o = torch.empty(records * E4M3_ROWS * head_dim, dtype=torch.float32, device=self.device)
+        if self.part_ml is None or self.part_ml.numel() < records * E4M3_ROWS * 2:
+            self.part_ml = torch.empty(records * E4M3_ROWS * 2, dtype=torch.float32, device=self.device)
+        if self.tickets is None or self.tickets.numel() < pairs:
+            self.tickets = torch.zeros(pairs, dtype=torch.int32, device=self.device)
+
+
+_block_slots: dict = {}
+
+
+def _slots_of(is_bf16: int, head_dim: int) -> int:
+    key = (torch._C._cuda_getDevice(), is_bf16, head_dim)
+    n = _block_slots.get(key)
+    if n is None:
+        n = _function("attention_e4m3", "qf_attention_e4m3_slots", _I, _I)(is_bf16, head_dim)
+        if n <= 0:
+            raise KernelError(f"attention_e4m3: the device has no room for a block of head size {head_dim}")
+        _block_slots[key] = n
+    return n
+
+
+def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_heads: int,
+                   n_seqs: int, max_q_len: int, scale: float, window: int, scratch: E4m3Scratch, err: torch.Tensor, max_kv_len: Optional[int] = None) -> None:
+    """Causal grouped-query attention of a step's tokens over a cache in 8 bits: single tokens, and short spans (every 16 rows of tokens times the heads of
+    a group read the cache anew, so a prompt goes by `cache_read_e4m3` and the kernels for many rows). q, out [T, n_heads * head_dim], bfloat16 or
+    float32; query head i reads kv head i // (n_heads / kv_heads); key j is visible to a token at p iff max(0, p - window + 1) <= j <= p
+    (window 0: all up to p). Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at consecutive positions, at most max_q_len; an entry may have none, and a
+    padding entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page
+    table has room for)."""
+    dtype, d, kv_heads = q.dtype, site.head_dim, site.kv_heads
+    is_bf16 = kernels._is_bf16(dtype)
+    _dev("q", q)
+    _dev("out", out, dtype)
+    _batch("attention_e4m3", cu_q, tok_pos, slots, err)
+    if n_heads <= 0 or n_heads % kv_heads:
+        raise KernelError(f"attention_e4m3: {n_heads} heads do not divide into {kv_heads} groups")
+    if q.dim() != 2 or q.shape[1] != n_heads * d or out.shape != q.shape:
+        raise KernelError("attention_e4m3: q/out widths do not match the head count")
+    if slots.numel() != n_seqs or tok_pos.numel() != q.shape[0] or window < 0:
+        raise KernelError("attention_e4m3: wants n_seqs slots, a position per token and a window of 0 or more")
+    if n_seqs and (max_q_len <= 0 or (max_kv_len is not None and max_kv_len <= 0)):
+        raise KernelError("attention_e4m3: max_q_len and max_kv_len bound an entry's tokens and its sequence's length")
+    _here("attention_e4m3", q, out, cu_q, tok_pos, slots, site.storage, site.scales, site.table, err)
+    if q.shape[0] == 0:
+        return
+    columns = site.table.shape[1]
+    most = columns if max_kv_len is None else min(columns, -(-int(max_kv_len) // PAGE_TOKENS))
+    if window > 0:
+        most = min(most, -(-(window + max_q_len - 1) // PAGE_TOKENS) + 1)
+    chunks = -(-min(max_q_len, q.shape[0]) * (n_heads // kv_heads) // E4M3_ROWS)
+    pairs = n_seqs * kv_heads * chunks
+    records = min(pairs + _slots_of(is_bf16, d), pairs * -(-most // E4M3_WARPS))
+    scratch.ensure(records, pairs, d)
+    _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
+    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _LL, _F, _I, _P, _P, _P, _P, _P)(
+        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.address(), n_heads, n_seqs, chunks, most, records,
+        scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
