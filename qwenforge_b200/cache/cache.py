@@ -30,6 +30,11 @@ A sequence may be forked (`fork`): the new ones hold its whole pages with it (a 
 that is still being filled and of the fixed-size state. So a page at or behind a sequence's length is always its own, and no write
 reaches a page that two sequences hold. `rewind` drops a sequence's last positions, `compact` moves the held pages to the front.
 
+Keys and values may be kept in 8 bits (`kv_dtype`): a page then holds e4m3 codes, and the group a power of two for each page, plane and
+head beside them. They travel together: a copied page takes its scales with it. A group has one more storage there, of the model's own
+dtype and one entry's size: the values that a prompt's attention reads back, under the same page numbers, one schedule entry after
+another.
+
 The state that decoding itself keeps per sequence (latest token, position, step count, budget)
 lives in the decode graph's own device buffers (`engine/graphs.py`); this cache holds only what
 the model's mixers declare.
@@ -75,6 +80,11 @@ class KvNeed:
     def rows(self, length: int) -> int:
         """Rows that a sequence of `length` positions holds."""
         return length // self.every
+
+    def fits(self, dtype: torch.dtype) -> bool:
+        """Whether a cache of this dtype (8 bits) has a form for these rows: keys and values, one row of each per position."""
+        return (dtype == torch.float8_e4m3fn and self.planes == 2 and self.chunk == 0 and self.every == 1 and self.pool == 0
+                and self.head_dim in ops.E4M3_HEAD_DIMS)
 
     def merged(self, other: "KvNeed") -> "KvNeed":
         """What serves this need and a reader with a mask of its own over the same rows: where the masks differ, every
@@ -152,22 +162,34 @@ class KvSite:
     def __init__(self, group: "KvGroup", index: int):
         self.group = group
         self.storage = group.storage[index]  # [pages, planes, kv_heads, PAGE_TOKENS, head_dim]
+        self.scales = None if group.scales is None else group.scales[index]  # [pages, planes, kv_heads], of a cache in 8 bits
         self.table = group.table
         self.kv_heads = group.need.kv_heads
         self.head_dim = group.need.head_dim
         self.window = group.need.window
+        self._codes = None
+
+    def codes(self):
+        """What the kernels of a cache in 8 bits address it by (checked once)."""
+        if self._codes is None:
+            self._codes = ops.E4m3SiteArgs(self.storage, self.scales, self.table, self.kv_heads, self.head_dim)
+        return self._codes
 
 
 class KvGroup:
     def __init__(self, need: KvNeed, entries: Sequence[int], n_pages: int, n_slots: int, pages_per_seq: int,
-                 dtype: torch.dtype, device):
+                 dtype: torch.dtype, device, kv_dtype: Optional[torch.dtype] = None):
         self.need = need
         self.entries = list(entries)
         self.pages = PageAllocator(n_pages)
         self.pages_per_seq = pages_per_seq
         # zeroed once: no kernel reads beyond a sequence's length, stale data is finite anyway
-        self.storage = torch.zeros((len(self.entries), n_pages, need.planes, need.kv_heads, PAGE_TOKENS, need.head_dim),
-                                   dtype=dtype, device=device)
+        shape = (len(self.entries), n_pages, need.planes, need.kv_heads, PAGE_TOKENS, need.head_dim)
+        self.storage = torch.zeros(shape, dtype=dtype if kv_dtype is None else kv_dtype, device=device)
+        self.scales = self.values = None
+        if kv_dtype is not None:
+            self.scales = torch.zeros(shape[:4], dtype=torch.float32, device=device)
+            self.values = torch.zeros(shape[1:], dtype=dtype, device=device)
         self.table = torch.full((n_slots, pages_per_seq), -1, dtype=torch.int32, device=device)
         self._host_table = torch.full((n_slots, pages_per_seq), -1, dtype=torch.int32)
         self._held: list[dict[int, int]] = [dict() for _ in range(n_slots)]  # slot -> {logical page: page id}
@@ -242,7 +264,13 @@ class KvGroup:
             if partial is not None:
                 self._put(fork, partial, copies[i])
         if copies:
-            ops.copy_pages(self.storage, [(held[partial], page, self.need.rows(length) % PAGE_TOKENS) for page in copies])
+            self._copy([(held[partial], page, self.need.rows(length) % PAGE_TOKENS) for page in copies])
+
+    def _copy(self, moves: list) -> None:
+        """Rows of pages to other pages, with their pages' scales: (from, to, rows) or (from, to)."""
+        ops.copy_pages(self.storage, moves)
+        if self.scales is not None:
+            ops.copy_pages(self.scales, [move[:2] for move in moves])
 
     def rewind_missing(self, slot: int, length: int) -> bool:
         """Whether a page that a sequence of `length` positions still needs has been given back."""
@@ -261,7 +289,7 @@ class KvGroup:
         if self.shares_filling(slot, length):
             partial = rows // PAGE_TOKENS
             old, (new,) = held[partial], self.pages.take(1)
-            ops.copy_pages(self.storage, [(old, new, rows % PAGE_TOKENS)])
+            self._copy([(old, new, rows % PAGE_TOKENS)])
             self.pages.give_back([old])
             self._put(slot, partial, new)
         gone = [lp for lp in held if lp * PAGE_TOKENS >= rows]
@@ -275,7 +303,7 @@ class KvGroup:
         """Held pages to the front of the storage; returns how many moved."""
         moves = self.pages.compact()
         if moves:
-            ops.copy_pages(self.storage, moves)
+            self._copy(moves)
             to = dict(moves)
             for slot, held in enumerate(self._held):
                 for lp, page in held.items():
@@ -329,14 +357,17 @@ class SequenceCache:
                  rounded up to PAGE_TOKENS; sizes every KV group
     max_seqs     number of slots
     max_len      the longest sequence a slot can hold (sizes the page tables)
+    kv_dtype     None: keys and values in `dtype`; torch.float8_e4m3fn: in 8 bits (every position's own keys and values, of head
+                 sizes that the kernels have)
     """
 
     _serials = 0
 
     def __init__(self, needs: Sequence[Optional[object]], max_tokens: int, max_seqs: int, max_len: int,
-                 dtype: torch.dtype, device):
+                 dtype: torch.dtype, device, kv_dtype: Optional[torch.dtype] = None):
         self.device = torch.device(device)
         self.dtype = dtype
+        self.kv_dtype = kv_dtype
         SequenceCache._serials += 1
         self.serial = SequenceCache._serials  # tells caches apart for whoever keeps things per cache (captured graphs)
         n_pages = max(1, round_up(max_tokens, PAGE_TOKENS) // PAGE_TOKENS)
@@ -368,9 +399,11 @@ class SequenceCache:
 
         for need, keepers in by_need.items():
             if isinstance(need, KvNeed):
+                if kv_dtype is not None and not need.fits(kv_dtype):
+                    raise ValueError(f"a cache in {kv_dtype} does not hold {need}")
                 # a group of one row per `every` positions is sized by rows: fewer pages, each sequence's last one partly empty
                 pages = n_pages if need.every <= 1 else min(n_pages, n_pages // need.every + self.max_seqs)
-                group = KvGroup(need, keepers, pages, self.max_seqs, pages_per_seq, dtype, self.device)
+                group = KvGroup(need, keepers, pages, self.max_seqs, pages_per_seq, dtype, self.device, kv_dtype)
                 self.kv_groups.append(group)
                 for i, (entry, path) in enumerate(keepers):
                     place(entry, path, KvSite(group, i))
@@ -533,7 +566,10 @@ class SequenceCache:
         return self._shared[key]
 
     def shared_worth_reading(self, slots: Sequence[int]):
-        """`shared_prefix`, where an attention layer is faster for reading it once (`ops.attention_shared_pays`); else None."""
+        """`shared_prefix`, where an attention layer is faster for reading it once (`ops.attention_shared_pays`); else None. (A cache in
+        8 bits is read by every sequence for itself.)"""
+        if self.kv_dtype is not None:
+            return None
         share = self.shared_prefix(slots)
         if share is None or any(ops.attention_shared_pays(share, g.storage.dtype, g.need.kv_heads, g.need.head_dim) for g in self.kv_groups):
             return share
@@ -564,6 +600,6 @@ class SequenceCache:
         return total
 
     def storage_bytes(self) -> int:
-        total = sum(g.storage.numel() * g.storage.element_size() for g in self.kv_groups)
+        total = sum(t.numel() * t.element_size() for g in self.kv_groups for t in (g.storage, g.scales, g.values) if t is not None)
         total += sum(g.storage.numel() * g.storage.element_size() for g in self.state_groups)
         return total

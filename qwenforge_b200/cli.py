@@ -40,6 +40,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--device", default=os.environ.get("HF_DEVICE", "cuda"))
     p.add_argument("--dtype", choices=["auto", "float16", "bfloat16", "float32"], default="bfloat16",
                    help="float16 (the reference's default) is served by the bfloat16 path")
+    p.add_argument("--cache-dtype", choices=["auto", "float8_e4m3"], default="auto",
+                   help="what the sequence cache keeps keys and values in: the compute dtype, or 8 bits")
     p.add_argument("--attn-implementation", default="sdpa",
                    help="'sdpa': the fastest attention kernels that take the shapes; anything else: the plain SIMT kernel")
     p.add_argument("--local-files-only", action="store_true")
@@ -153,7 +155,7 @@ def main(argv=None) -> int:
     try:
         engine = StudentEngine(model_path, device=args.device, dtype=args.dtype,
                                attn_implementation=args.attn_implementation, local_files_only=args.local_files_only,
-                               seed=args.seed, cuda_graphs=not (args.no_graphs or args.time_kernels))
+                               seed=args.seed, cuda_graphs=not (args.no_graphs or args.time_kernels), cache_dtype=args.cache_dtype)
         peaks = json.loads(Path(args.peaks).read_text()) if args.peaks else None
         if args.prompt:
             for text in engine.generate(list(args.prompt), args.max_new_tokens_decode, batch_size=len(args.prompt)):

@@ -18,6 +18,20 @@ _NAMES = {
 }
 
 
+_CACHE_NAMES = {"auto": None, "float8_e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+
+
+def resolve_cache_dtype(dtype) -> torch.dtype | None:
+    """What the sequence cache keeps keys and values in: None ("auto": the model's own dtype), or torch.float8_e4m3fn ("float8_e4m3"): 8 bits
+    and a power of two per page of 64 positions and head."""
+    if dtype is None or dtype is torch.float8_e4m3fn:
+        return dtype
+    name = str(dtype).lower()
+    if isinstance(dtype, torch.dtype) or name not in _CACHE_NAMES:
+        raise ValueError(f"Unsupported cache dtype: {dtype} (auto or float8_e4m3)")
+    return _CACHE_NAMES[name]
+
+
 def resolve_dtype(dtype, config_torch_dtype: str | None = None) -> torch.dtype:
     """'auto' takes config.json's torch_dtype; anything else is looked up by name. float16 resolves to bfloat16."""
     asked_for_half = False

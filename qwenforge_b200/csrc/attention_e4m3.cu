@@ -17,11 +17,14 @@
 // of it, and byte t of them is its element of the t-th product: a byte permutation puts two positions side by side for the conversion.
 // A tile's values are on their way while its scores are formed, the next tile's keys from then on.
 //
-// Runs are cut on the device, from the lengths (a captured graph replays this launch with others): every warp works out for itself how
-// many pages a block takes if the batch is to fill the SMs once. A pair with several runs leaves partial results (maximum, sum, output);
-// the block that ends last, by a ticket, joins them in the order of the runs.
+// Work is shared out on the device, from the lengths (a captured graph replays this launch with others): all pages of all (sequence, kv head,
+// 16 rows) in a row, `target` of them to a block, so that one round of blocks does it all. Where every pair's pages can be rounded up to
+// whole blocks within that round, they are, and a block has one pair; else blocks begin and end anywhere, and lengths that
+// differ leave no SM idle. A pair of several blocks leaves partial results (maximum, sum, output); the block that ends last, by a
+// ticket, joins them in their order, sixteen at a time, and the last of those the sixteens.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "e4m3.cuh"
@@ -94,18 +97,6 @@ template <int D> __device__ __forceinline__ int value_component(int t, int n) {
     t -= 4 * P::v32, base += 32 * P::v32;
     return base + 2 * n + t;
 }
-// ... and where component d stands: 8 * product + column.
-template <int D> __device__ __forceinline__ int value_place(int d) {
-    using P = Parts<D>;
-    int t = 0;
-    if (d < 128 * P::v128) return 8 * (d % 16) + d / 16;
-    d -= 128 * P::v128, t += 16 * P::v128;
-    if (d < 64 * P::v64) return 8 * (t + d % 8) + d / 8;
-    d -= 64 * P::v64, t += 8 * P::v64;
-    if (d < 32 * P::v32) return 8 * (t + d % 4) + d / 4;
-    d -= 32 * P::v32, t += 4 * P::v32;
-    return 8 * (t + d % 2) + d / 2;
-}
 template <int D> __device__ __forceinline__ void load_key(uint32_t (&w)[D / 16], const unsigned char* row, int c) {
     using P = Parts<D>;
 #pragma unroll
@@ -144,77 +135,54 @@ template <typename T, int D> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
     static constexpr int TILE = D <= 64 ? (TWO ? 32 : 64) : (TWO && D > 96 ? 16 : 32);   // positions of a step
     static constexpr int BLOCKS = D <= 32 ? 4 : D <= 64 ? 3 : 2;      // of an SM
-    static constexpr int LD = D + 8;                                  // floats from a row to the next where warps leave their outputs
+    // floats from a row to the next where warps leave their outputs: product t's column n at 8 t + 8 (t / 4) + n, so that four products of 32 lanes
+    // meet 32 banks; rows 8 or 24 banks apart, for the warps' own stores
+    static constexpr int ROW = D + 8 * ((D / 8 + 3) / 4), LD = ROW % 32 == 8 || ROW % 32 == 24 ? ROW : ROW + 8;
     static constexpr int SMEM = EA_WARPS * EA_ROWS * LD * 4;
+    static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result
 };
 
 struct AttendArgs {
     const int *cu_q, *tok_pos, *slots;
     E4m3Site site;
-    int n_heads, n_seqs, chunks, most_pages, block_slots, window;
+    int n_heads, n_seqs, single, chunks, most_pages, block_slots, window;
     float scale_log2;
-    float *part_o, *part_ml;
-    int *tickets, *err;
+    float *part_o, *part_ml;   // [2 * blocks][16][PART], [2 * blocks][16][2]
+    int *tickets, *err;        // [4 * blocks]
 };
 
-// What a block does: a run of pages of a sequence. `record` counts (sequence, run), in order.
-struct Run {
-    int seq, run, runs, slot, begin, tokens, first_pos, last_pos, page0, pages;
+struct Sequence {
+    int slot, begin, tokens, first_pos, last_pos, page0, pages;
 };
-__device__ __forceinline__ void sequence_of(const AttendArgs& a, int s, Run& r) {
-    r.begin = a.cu_q[s];
-    r.tokens = a.cu_q[s + 1] - r.begin;
+__device__ __forceinline__ Sequence sequence_of(const AttendArgs& a, int s) {
+    Sequence r;
+    r.begin = a.single ? s : a.cu_q[s];   // (single: every entry has one token)
+    r.tokens = a.single ? 1 : a.cu_q[s + 1] - r.begin;
     r.slot = r.tokens > 0 ? a.slots[s] : -1;
     r.first_pos = r.last_pos = r.page0 = r.pages = 0;
-    if (r.slot >= 0) {
+    if (r.tokens > 0) {
         r.first_pos = a.tok_pos[r.begin];
-        r.last_pos = a.tok_pos[r.begin + r.tokens - 1];
+        r.last_pos = a.single ? r.first_pos : a.tok_pos[r.begin + r.tokens - 1];
+    }
+    if (r.slot >= 0) {
         r.page0 = a.window > 0 ? max(0, r.first_pos - a.window + 1) / QF_PAGE : 0;
-        r.pages = min(r.last_pos / QF_PAGE - r.page0 + 1, a.most_pages);   // (more than the call has said: cut, and reported)
+        r.pages = min(max(r.last_pos / QF_PAGE - r.page0 + 1, 0), a.most_pages);   // (more than the call has said: cut, and reported)
+    }
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* to, const float (&v)[4], int n) {
+    if constexpr (sizeof(T) == 4) {
+        if (n == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+    } else {
+        if (n == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        else *reinterpret_cast<uint32_t*>(to) = pack_bf16(v[0], v[1]);
     }
 }
-__device__ __forceinline__ bool find_run(const AttendArgs& a, int record, int pairs_each, Run& r) {
-    const int lane = threadIdx.x & 31;
-    int total = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        Run x;
-        x.pages = 0;
-        if (s0 + lane < a.n_seqs) sequence_of(a, s0 + lane, x);
-        total += x.pages;
-    }
-    total = (int)warp_sum_u32((uint32_t)total);
-    // pages of a block: the batch's over the block slots that are left when every sequence has rounded up once
-    const int room = max(a.block_slots - a.n_seqs * pairs_each, a.block_slots / 2);
-    const int target = max(EA_WARPS, (int)(((long long)total * pairs_each + room - 1) / room));
-    int before = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        Run x;
-        int runs = 0;
-        if (s0 + lane < a.n_seqs) {
-            sequence_of(a, s0 + lane, x);
-            runs = max(1, (x.pages + target - 1) / target);
-            const int each = (x.pages + runs - 1) / runs;
-            runs = each > 0 ? (x.pages + each - 1) / each : 1;   // (none without a page)
-        }
-        int upto = runs;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const int all = __shfl_sync(0xffffffffu, upto, 31);
-        if (record < before + all) {
-            const int who = __ffs(__ballot_sync(0xffffffffu, before + upto > record)) - 1;
-            r.seq = s0 + who;
-            r.runs = __shfl_sync(0xffffffffu, runs, who);
-            r.run = record - (before + __shfl_sync(0xffffffffu, upto, who) - r.runs);
-            sequence_of(a, r.seq, r);
-            return true;
-        }
-        before += all;
-    }
-    return false;
-}
+
+#define EA_GROUP 16        // partial results that a block joins at once
+#define EA_MOST_GROUPS 64  // ... and groups of them: enough for 1,024 blocks
 
 template <typename T, int D>
 __global__ void __launch_bounds__(EA_WARPS * 32, Shape<T, D>::BLOCKS)
@@ -222,311 +190,421 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
     using S = Shape<T, D>;
     using P = Parts<D>;
     constexpr bool TWO = S::TWO;
-    constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, OT = D / 8, KW = P::k_words, VW = P::v_words, LD = S::LD;
+    constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, OT = D / 8, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART;
+    constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32;
     grid_chain_entry();
     extern __shared__ float shared_o[];   // [warps][rows][LD]
-    __shared__ float m_s[EA_WARPS][EA_ROWS], l_s[EA_WARPS][EA_ROWS];
+    __shared__ float m_s[EA_WARPS][EA_ROWS], l_s[EA_WARPS][EA_ROWS], total_s[EA_ROWS], factor_s[EA_MOST_GROUPS][EA_ROWS];
     __shared__ int ticket_s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const E4m3Site& site = a.site;
-    const int KVH = site.kv_heads, G = a.n_heads / KVH;
-    const int pairs_each = KVH * a.chunks, record = blockIdx.x / pairs_each, y = blockIdx.x % pairs_each;
-    const int kvh = y / a.chunks, chunk = y % a.chunks;
-    Run r;
-    if (!find_run(a, record, pairs_each, r)) return;
-    const int row0 = chunk * EA_ROWS, n_rows = min(EA_ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
-    if (n_rows <= 0) return;
-    const int q_width = a.n_heads * D;
-    // element 0 of a row's query (and output)
-    auto row_at = [&](int row) -> long long {
-        const int i = row0 + row;
-        return (long long)(r.begin + i / G) * q_width + (long long)(kvh * G + i % G) * D;
-    };
-    if (r.slot < 0) {   // a padding entry: zeros
-        for (int i = threadIdx.x; i < n_rows * D; i += EA_WARPS * 32) out[row_at(i / D) + i % D] = Num<T>::from_f(0.f);
-        return;
-    }
-    if (r.run == 0 && threadIdx.x == 0 && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
-    const int each = (r.pages + r.runs - 1) / r.runs;
-    const int p_begin = r.page0 + r.run * each, p_end = min(p_begin + each, r.page0 + r.pages);
-    const int my_pages = p_begin + warp < p_end ? (p_end - p_begin - warp + EA_WARPS - 1) / EA_WARPS : 0;
-    const int length = r.last_pos + 1;
-    // what this lane's two rows see: lo .. hi - 1
-    int lo[2], hi[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int row = g + 8 * e;
-        hi[e] = row < n_rows ? a.tok_pos[r.begin + (row0 + row) / G] + 1 : 0;
-        lo[e] = a.window > 0 ? max(0, hi[e] - a.window) : 0;
-    }
-    const int lo_first = a.window > 0 ? max(0, r.first_pos - a.window + 1) : 0;                 // below: seen by no row
-    const int lo_last = a.window > 0 ? max(0, r.last_pos - a.window + 1) : 0, hi_first = r.first_pos + 1;   // in between: seen by every row
+    const int KVH = site.kv_heads, G = a.n_heads / KVH, pairs_each = KVH * a.chunks;
+    const int q_width = a.n_heads * D, n_blocks = gridDim.x;
 
-    // ---- the queries' fragments
-    uint32_t qa[TWO ? 2 : 1][KW][4];
-    float by[2];   // scores of a row in base-2 units: product * key scale * by
-    {
-        float2 x[2][KW][2];
-        float top[2] = {0.f, 0.f};
+    // ---- this block's share (every warp works it out for itself)
+    int total = 0, whole = 0, target = EA_WARPS;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) total += s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0;
+    total = (int)warp_sum_u32((uint32_t)total) * pairs_each;
+    target = max(target, (total + a.block_slots - 1) / a.block_slots);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) whole += s0 + lane < a.n_seqs ? (sequence_of(a, s0 + lane).pages + target - 1) / target : 0;
+    whole = (int)warp_sum_u32((uint32_t)whole) * pairs_each;
+    const int unit = whole <= a.block_slots ? target : 1;   // pages of a pair are rounded up to whole units
+    if (unit == target) total = whole * target;
+    // padding entries: zeros
+    for (int s = blockIdx.x; s < a.n_seqs; s += n_blocks) {
+        const Sequence r = sequence_of(a, s);
+        if (r.slot < 0)
+            for (int i = threadIdx.x; i < r.tokens * q_width; i += THREADS) out[(long long)r.begin * q_width + i] = Num<T>::from_f(0.f);
+    }
+    const int range_begin = blockIdx.x * target, range_end = min(range_begin + target, total);
+    if (range_begin >= range_end) return;
+    // the sequence in whose pages it begins
+    int seq = 0, base = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const int mine = s0 + lane < a.n_seqs ? (sequence_of(a, s0 + lane).pages + unit - 1) / unit * unit * pairs_each : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > range_begin);
+        if (beyond) {
+            const int who = __ffs(beyond) - 1;
+            seq = s0 + who;
+            base += __shfl_sync(0xffffffffu, upto - mine, who);
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+
+    Sequence r = sequence_of(a, seq);
+    int padded = (r.pages + unit - 1) / unit * unit;
+    for (int at = range_begin; at < range_end;) {
+        while (at >= base + padded * pairs_each) {   // (sequences without pages are passed over)
+            base += padded * pairs_each;
+            r = sequence_of(a, ++seq);
+            padded = (r.pages + unit - 1) / unit * unit;
+        }
+        const int y = (at - base) / padded, pair_begin = base + y * padded, kvh = y / a.chunks, chunk = y % a.chunks;
+        const int p_begin = r.page0 + at - pair_begin, p_end = r.page0 + min(min(padded, range_end - pair_begin), r.pages);
+        const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin;
+        at = min(pair_begin + padded, range_end);
+        if (reports && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
+        const int row0 = chunk * EA_ROWS, n_rows = min(EA_ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
+        if (n_rows <= 0 || p_begin >= p_end) continue;
+        // element 0 of a row's query (and output)
+        auto row_at = [&](int row) -> long long {
+            const int i = row0 + row;
+            return (long long)(r.begin + i / G) * q_width + (long long)(kvh * G + i % G) * D;
+        };
+        const int my_pages = p_begin + warp < p_end ? (p_end - p_begin - warp + EA_WARPS - 1) / EA_WARPS : 0;
+        // what the rows see, lo .. hi - 1: this lane's two, all of them together, every one of them
+        const int t_first = row0 / G, t_last = (row0 + n_rows - 1) / G;
+        const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (a.single ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
+        const int some_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, all_lo = a.window > 0 ? max(0, some_hi - a.window) : 0;
+        int lo[2], hi[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = g + 8 * e;
-            const T* src = q + (row < n_rows ? row_at(row) : 0);
-#pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                const int d = key_component<D>(w, c);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[e][w][i] = row < n_rows ? make_float2(Num<T>::to_f(src[d + 2 * i]), Num<T>::to_f(src[d + 2 * i + 1])) : make_float2(0.f, 0.f);
-                    top[e] = fmaxf(top[e], fmaxf(fabsf(x[e][w][i].x), fabsf(x[e][w][i].y)));
+            hi[e] = row >= n_rows ? 0 : t_first == t_last ? first_hi : a.tok_pos[r.begin + (row0 + row) / G] + 1;
+            lo[e] = a.window > 0 ? max(0, hi[e] - a.window) : 0;
+        }
+
+        // ---- keys of a step: pages p_begin + warp, + EA_WARPS, ..., a tile of one at a time
+        const int steps = my_pages * PER_PAGE;
+        const long long plane = (long long)KVH * QF_PAGE * D;
+        int page_next = -1;          // of the step whose keys are loaded
+        float ks_next = 0.f, vs_next = 0.f;
+        uint32_t kw[NT][KW];
+        auto key0_of = [&](int step) { return (p_begin + warp + step / PER_PAGE * EA_WARPS) * QF_PAGE + step % PER_PAGE * TILE; };
+        auto load_keys = [&](int step) {
+            const int key0 = key0_of(step);
+            if (step % PER_PAGE == 0) {
+                page_next = e4m3_page(site, r.slot, key0);
+                if (page_next < 0) {
+                    if (lane == 0 && y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+                } else {
+                    const float* scales = site.scales + (long long)page_next * site.page_scales + kvh;
+                    ks_next = scales[0];
+                    vs_next = scales[KVH];
                 }
             }
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-            const int up = min(max(exponent_of(top[e]) - 7, -119), 120);
-            by[e] = pow2(up) * a.scale_log2;
-            const float down = pow2(-up);
+            if (page_next < 0 || key0 >= some_hi || key0 + TILE <= some_lo) return;
+            const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + g) * D;
 #pragma unroll
-            for (int w = 0; w < KW; ++w)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float u = x[e][w][i].x * down, v = x[e][w][i].y * down;
-                    qa[0][w][2 * i + e] = pack_half(u, v);
-                    if constexpr (TWO) qa[1][w][2 * i + e] = pack_rest(u, v, qa[0][w][2 * i + e]);
-                }
-        }
-    }
+            for (int t = 0; t < NT; ++t) load_key<D>(kw[t], k + t * 8 * D, c);
+        };
+        if (steps > 0) load_keys(0);
 
-    float o[OT][4];
-#pragma unroll
-    for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m_run[2] = {EA_NONE, EA_NONE}, l_run[2] = {0.f, 0.f};   // (l: this lane's columns only)
-
-    // ---- pages p_begin + warp, + EA_WARPS, ...: a step is a tile of one
-    constexpr int PER_PAGE = QF_PAGE / TILE;
-    const int steps = my_pages * PER_PAGE;
-    const long long plane = (long long)KVH * QF_PAGE * D;
-    int page_next = -1;          // of the step whose keys are loaded
-    float ks_next = 0.f, vs_next = 0.f;
-    uint32_t kw[NT][KW];
-    auto load_keys = [&](int step) {
-        if (step % PER_PAGE == 0) {
-            const int p = p_begin + warp + step / PER_PAGE * EA_WARPS;
-            page_next = e4m3_page(site, r.slot, p * QF_PAGE);
-            if (page_next < 0) {
-                if (lane == 0 && y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-            } else {
-                const float* scales = site.scales + (long long)page_next * site.page_scales + kvh;
-                ks_next = scales[0];
-                vs_next = scales[KVH];
-            }
-        }
-        if (page_next < 0) return;
-        const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + g) * D;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) load_key<D>(kw[t], k + t * 8 * D, c);
-    };
-    if (steps > 0) load_keys(0);
-    for (int step = 0; step < steps; ++step) {
-        const int page = page_next;
-        const int key0 = (p_begin + warp + step / PER_PAGE * EA_WARPS) * QF_PAGE + step % PER_PAGE * TILE;
-        const bool live = page >= 0 && key0 < length && key0 + TILE > lo_first;
-        if (!live) {
-            if (step + 1 < steps) load_keys(step + 1);
-            continue;
-        }
-        const float ks = ks_next, vs = vs_next;
-        const bool inside = key0 >= lo_first && key0 + TILE <= length;   // every position is held and seen by some row
-        // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
-        uint32_t vw[KT][4][VW];
+        // ---- the queries' fragments
+        uint32_t qa[TWO ? 2 : 1][KW][4];
+        float by[2];   // scores of a row in base-2 units: product * key scale * by
         {
-            const unsigned char* v = site.codes + (long long)page * site.page_bytes + plane + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + 2 * c) * D;
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = 16 * kt + (i & 1) + 8 * (i >> 1);
-                    if (inside || (key0 + at + 2 * c >= lo_first && key0 + at + 2 * c < length)) load_value<D>(vw[kt][i], v + (long long)at * D, g);
-                    else
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies there is nobody's, NaN perhaps)
-                }
-        }
-        // ---- scores
-        float s[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                const uint32_t b0 = half2_of_low(kw[t][w]), b1 = half2_of_high(kw[t][w]);
-                if constexpr (TWO) mma_f16_16816(s[t], qa[1][w], b0, b1);
-                mma_f16_16816(s[t], qa[0][w], b0, b1);
-            }
-        }
-        if (step + 1 < steps) load_keys(step + 1);
-        const float by0 = by[0] * ks, by1 = by[1] * ks;
-        float mx[2] = {EA_NONE, EA_NONE};
-        const bool full = key0 >= lo_last && key0 + TILE <= hi_first;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] *= e < 2 ? by0 : by1;
-                if (!full) {
-                    const int key = key0 + 8 * t + 2 * c + (e & 1);
-                    if (key < lo[e >> 1] || key >= hi[e >> 1]) s[t][e] = -INFINITY;
-                }
-                mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
-            }
-        float corr[2], shift[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-            const float m = fmaxf(m_run[e], mx[e]);
-            corr[e] = fast_exp2(m_run[e] - m);
-            m_run[e] = m;
-            shift[e] = m - 14.f;
-            l_run[e] *= corr[e];
-        }
-        uint32_t pa[TWO ? 2 : 1][KT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] = fast_exp2(s[t][e] - shift[e >> 1]);
-                l_run[e >> 1] += s[t][e];
-            }
+            float2 x[2][KW][2];
+            float top[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                pa[0][t / 2][2 * (t % 2) + e] = pack_half(s[t][2 * e], s[t][2 * e + 1]);
-                if constexpr (TWO) pa[1][t / 2][2 * (t % 2) + e] = pack_rest(s[t][2 * e], s[t][2 * e + 1], pa[0][t / 2][2 * (t % 2) + e]);
-            }
-        }
-        // ---- values: four products from a word of each of four positions
-        auto add_values = [&](auto masked, int from, int upto, bool first, bool mine0, bool mine1) {
+                const int row = g + 8 * e;
+                const T* src = q + (row < n_rows ? row_at(row) : 0);
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                constexpr bool M = decltype(masked)::value;
-                const int n = P::v16 != 0 && w == VW - 1 ? 2 : 4;   // products of this word
-                float acc[4][4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    uint32_t x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = vw[kt][i][w];
-                        if constexpr (M) {
-                            const int key = key0 + 16 * kt + 2 * c + (i & 1) + 8 * (i >> 1);
-                            if (key < from || key >= upto) x[i] = 0u;
+                for (int w = 0; w < KW; ++w) {
+                    const int d = key_component<D>(w, c);
+                    x[e][w][0] = x[e][w][1] = make_float2(0.f, 0.f);
+                    if (row < n_rows) {
+                        if constexpr (TWO) {
+                            const float4 v = *reinterpret_cast<const float4*>(src + d);
+                            x[e][w][0] = make_float2(v.x, v.y), x[e][w][1] = make_float2(v.z, v.w);
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(src + d);
+                            x[e][w][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
+                            x[e][w][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
                         }
                     }
-                    const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), b01 = __byte_perm(x[2], x[3], 0x5140);
-                    const uint32_t a23 = __byte_perm(x[0], x[1], 0x7362), b23 = __byte_perm(x[2], x[3], 0x7362);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) top[e] = fmaxf(top[e], fmaxf(fabsf(x[e][w][i].x), fabsf(x[e][w][i].y)));
+                }
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+                const int up = min(max(exponent_of(top[e]) - 7, -119), 120);
+                by[e] = pow2(up) * a.scale_log2;
+                const float down = pow2(-up);
+#pragma unroll
+                for (int w = 0; w < KW; ++w)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float u = x[e][w][i].x * down, v = x[e][w][i].y * down;
+                        qa[0][w][2 * i + e] = pack_half(u, v);
+                        if constexpr (TWO) qa[1][w][2 * i + e] = pack_rest(u, v, qa[0][w][2 * i + e]);
+                    }
+            }
+        }
+
+        float o[OT][4];
+#pragma unroll
+        for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m_run[2] = {EA_NONE, EA_NONE}, l_run[2] = {0.f, 0.f};   // (l: this lane's columns only)
+
+        for (int step = 0; step < steps; ++step) {
+            const int page = page_next;
+            const int key0 = key0_of(step);
+            const bool live = page >= 0 && key0 < some_hi && key0 + TILE > some_lo;
+            if (!live) {
+                if (step + 1 < steps) load_keys(step + 1);
+                continue;
+            }
+            const float ks = ks_next, vs = vs_next;
+            const bool inside = key0 >= some_lo && key0 + TILE <= some_hi;   // every position is held and seen by some row
+            // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
+            uint32_t vw[KT][4][VW];
+            {
+                const unsigned char* v = site.codes + (long long)page * site.page_bytes + plane + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + 2 * c) * D;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 16 * kt + (i & 1) + 8 * (i >> 1);
+                        if (inside || (key0 + at + 2 * c >= some_lo && key0 + at + 2 * c < some_hi)) load_value<D>(vw[kt][i], v + (long long)at * D, g);
+                        else
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies there is nobody's, NaN perhaps)
+                    }
+            }
+            // ---- scores
+            float s[NT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    const uint32_t b0 = half2_of_low(kw[t][w]), b1 = half2_of_high(kw[t][w]);
+                    if constexpr (TWO) mma_f16_16816(s[t], qa[1][w], b0, b1);
+                    mma_f16_16816(s[t], qa[0][w], b0, b1);
+                }
+            }
+            if (step + 1 < steps) load_keys(step + 1);
+            const float by0 = by[0] * ks, by1 = by[1] * ks;
+            float mx[2] = {EA_NONE, EA_NONE};
+            const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[t][e] *= e < 2 ? by0 : by1;
+                    if (!full) {
+                        const int key = key0 + 8 * t + 2 * c + (e & 1);
+                        if (key < lo[e >> 1] || key >= hi[e >> 1]) s[t][e] = -INFINITY;
+                    }
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+                }
+            float corr[2], shift[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                const float m = fmaxf(m_run[e], mx[e]);
+                corr[e] = fast_exp2(m_run[e] - m);
+                m_run[e] = m;
+                shift[e] = m - 14.f;
+                l_run[e] *= corr[e];
+            }
+            uint32_t pa[TWO ? 2 : 1][KT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[t][e] = fast_exp2(s[t][e] - shift[e >> 1]);
+                    l_run[e >> 1] += s[t][e];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    pa[0][t / 2][2 * (t % 2) + e] = pack_half(s[t][2 * e], s[t][2 * e + 1]);
+                    if constexpr (TWO) pa[1][t / 2][2 * (t % 2) + e] = pack_rest(s[t][2 * e], s[t][2 * e + 1], pa[0][t / 2][2 * (t % 2) + e]);
+                }
+            }
+            // ---- values: four products from a word of each of four positions
+            auto add_values = [&](auto masked, int from, int upto, bool first, bool mine0, bool mine1) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    constexpr bool M = decltype(masked)::value;
+                    const int n = P::v16 != 0 && w == VW - 1 ? 2 : 4;   // products of this word
+                    float acc[4][4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = vw[kt][i][w];
+                            if constexpr (M) {
+                                const int key = key0 + 16 * kt + 2 * c + (i & 1) + 8 * (i >> 1);
+                                if (key < from || key >= upto) x[i] = 0u;
+                            }
+                        }
+                        const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), b01 = __byte_perm(x[2], x[3], 0x5140);
+                        const uint32_t a23 = __byte_perm(x[0], x[1], 0x7362), b23 = __byte_perm(x[2], x[3], 0x7362);
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            if (t >= n) break;
+                            const uint32_t u = t < 2 ? a01 : a23, v = t < 2 ? b01 : b23;
+                            const uint32_t b0 = t & 1 ? half2_of_high(u) : half2_of_low(u), b1 = t & 1 ? half2_of_high(v) : half2_of_low(v);
+                            if constexpr (TWO) mma_f16_16816(acc[t], pa[1][kt], b0, b1);
+                            mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                        }
+                    }
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         if (t >= n) break;
-                        const uint32_t u = t < 2 ? a01 : a23, v = t < 2 ? b01 : b23;
-                        const uint32_t b0 = t & 1 ? half2_of_high(u) : half2_of_low(u), b1 = t & 1 ? half2_of_high(v) : half2_of_low(v);
-                        if constexpr (TWO) mma_f16_16816(acc[t], pa[1][kt], b0, b1);
-                        mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                        float(&x)[4] = o[4 * w + t];
+                        if constexpr (M) {
+                            if (first) x[0] *= corr[0], x[1] *= corr[0], x[2] *= corr[1], x[3] *= corr[1];
+                            if (mine0) x[0] = fmaf(acc[t][0], vs, x[0]), x[1] = fmaf(acc[t][1], vs, x[1]);
+                            if (mine1) x[2] = fmaf(acc[t][2], vs, x[2]), x[3] = fmaf(acc[t][3], vs, x[3]);
+                        } else {
+                            x[0] = fmaf(acc[t][0], vs, x[0] * corr[0]);
+                            x[1] = fmaf(acc[t][1], vs, x[1] * corr[0]);
+                            x[2] = fmaf(acc[t][2], vs, x[2] * corr[1]);
+                            x[3] = fmaf(acc[t][3], vs, x[3] * corr[1]);
+                        }
                     }
                 }
+            };
+            bool apart = false;
+            if (!full && t_first != t_last) {   // a NaN that some of the rows do not see must not reach them: 0 * NaN
+                bool nan = false;
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (t >= n) break;
-                    float(&x)[4] = o[4 * w + t];
-                    if constexpr (M) {
-                        if (first) x[0] *= corr[0], x[1] *= corr[0], x[2] *= corr[1], x[3] *= corr[1];
-                        if (mine0) x[0] = fmaf(acc[t][0], vs, x[0]), x[1] = fmaf(acc[t][1], vs, x[1]);
-                        if (mine1) x[2] = fmaf(acc[t][2], vs, x[2]), x[3] = fmaf(acc[t][3], vs, x[3]);
-                    } else {
-                        x[0] = fmaf(acc[t][0], vs, x[0] * corr[0]);
-                        x[1] = fmaf(acc[t][1], vs, x[1] * corr[0]);
-                        x[2] = fmaf(acc[t][2], vs, x[2] * corr[1]);
-                        x[3] = fmaf(acc[t][3], vs, x[3] * corr[1]);
-                    }
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) nan |= holds_nan(vw[kt][i][w]);
+                apart = __any_sync(0xffffffffu, nan);
+            }
+            if (!apart) {
+                add_values(std::false_type{}, 0, 0, true, true, true);
+            } else {   // token by token, each with the positions that it sees
+                for (int t = t_first; t <= t_last; ++t) {
+                    const int upto = a.tok_pos[r.begin + t] + 1;
+                    add_values(std::true_type{}, a.window > 0 ? upto - a.window : 0, upto, t == t_first, (row0 + g) / G == t, (row0 + g + 8) / G == t);
                 }
+            }
+        }
+
+        // ---- the warps' results together
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+            if (c == 0) {
+                m_s[warp][g + 8 * e] = m_run[e];
+                l_s[warp][g + 8 * e] = l_run[e];
+            }
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+                *reinterpret_cast<float2*>(&shared_o[(warp * EA_ROWS + g + 8 * e) * LD + 8 * t + 8 * (t / 4) + 2 * c]) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+        }
+        __syncthreads();
+        const int live_warps = min(EA_WARPS, p_end - p_begin);   // (the others have seen nothing)
+        if (threadIdx.x < EA_ROWS) {
+            float m = EA_NONE, l = 0.f;
+            for (int w = 0; w < live_warps; ++w) m = fmaxf(m, m_s[w][threadIdx.x]);
+            for (int w = 0; w < live_warps; ++w) {
+                const float f = fast_exp2(m_s[w][threadIdx.x] - m);
+                factor_s[w][threadIdx.x] = f;
+                l = fmaf(f, l_s[w][threadIdx.x], l);
+            }
+            m_s[0][threadIdx.x] = m;
+            total_s[threadIdx.x] = l;
+        }
+        __syncthreads();
+        const int first_block = pair_begin / target, runs = (pair_begin + r.pages - 1) / target - first_block + 1, run = (int)blockIdx.x - first_block;
+        // where run k of this pair leaves its results: a block's first pair in the first of its two places
+        auto place_of = [&](int k) { return 2 * (first_block + k) + (pair_begin > (first_block + k) * target ? 1 : 0); };
+        // an item: four products' elements of one column and row, neighbours in the output
+        auto each_item = [&](auto work) {
+            for (int i = threadIdx.x; i < n_rows * VW * 8; i += THREADS) {
+                const int row = i / (VW * 8), w = i / 8 % VW, n = i % 8;
+                work(i, row, w, n, P::v16 != 0 && w == VW - 1 ? 2 : 4);
             }
         };
-        bool apart = false;
-        if (!full && r.tokens > 1) {   // a NaN that some of the rows do not see must not reach them: 0 * NaN
-            bool nan = false;
+        auto give_out = [&](const float (&v)[4], int row, int w, int n, int count) {
+            const float l = total_s[row], inv = l != 0.f ? 1.f / l : 0.f;
+            const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+            store4(out + row_at(row) + value_component<D>(4 * w, n), u, count);
+        };
+        each_item([&](int i, int row, int w, int n, int count) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < live_warps; ++k) {
+                const float f = factor_s[k][row];
+                const float* from = shared_o + (k * EA_ROWS + row) * LD + 40 * w + n;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) nan |= holds_nan(vw[kt][i][w]);
-            apart = __any_sync(0xffffffffu, nan);
-        }
-        if (!apart) {
-            add_values(std::false_type{}, 0, 0, true, true, true);
-        } else {   // token by token, each with the positions that it sees
-            const int t0 = row0 / G, t1 = (row0 + n_rows - 1) / G;
-            for (int t = t0; t <= t1; ++t) {
-                const int upto = a.tok_pos[r.begin + t] + 1;
-                add_values(std::true_type{}, a.window > 0 ? upto - a.window : 0, upto, t == t0, (row0 + g) / G == t, (row0 + g + 8) / G == t);
+                for (int j = 0; j < 4; ++j)
+                    if (j < count) v[j] = fmaf(f, from[8 * j], v[j]);
+            }
+            if (runs == 1) give_out(v, row, w, n, count);
+            else *reinterpret_cast<float4*>(a.part_o + (long long)place_of(run) * EA_ROWS * PART + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        });
+        if (runs > 1) {
+            // joins the results in `count` places (the k-th: place(k)): their sums in total_s, the output by `done`
+            auto join = [&](int count, auto place, auto done) {
+                __threadfence();
+                if (threadIdx.x < EA_ROWS) {
+                    const int row = threadIdx.x;
+                    float m = EA_NONE, l = 0.f;
+                    for (int k = 0; k < count; ++k) m = fmaxf(m, __ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2));
+                    for (int k = 0; k < count; ++k) {
+                        const float f = fast_exp2(__ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2) - m);
+                        factor_s[k][row] = f;
+                        l = fmaf(f, __ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2 + 1), l);
+                    }
+                    m_s[0][row] = m;
+                    total_s[row] = l;
+                }
+                __syncthreads();
+                each_item([&](int i, int row, int w, int n, int items) {
+                    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+                    for (int k = 0; k < count; ++k) {
+                        const float f = factor_s[k][row];
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + (long long)place(k) * EA_ROWS * PART + i * 4));
+                        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+                    }
+                    done(v, i, row, w, n, items);
+                });
+            };
+            auto leave = [&](int place) {   // maximum and sum
+                if (threadIdx.x < n_rows) *reinterpret_cast<float2*>(a.part_ml + (place * EA_ROWS + threadIdx.x) * 2) = make_float2(m_s[0][threadIdx.x], total_s[threadIdx.x]);
+            };
+            auto last_of = [&](int* ticket, int count) {   // whether all others have left theirs; the counter is then as the next call wants it
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    ticket_s = atomicAdd(ticket, 1);
+                    if (ticket_s == count - 1) *ticket = 0;
+                }
+                __syncthreads();
+                return ticket_s == count - 1;
+            };
+            leave(place_of(run));
+            const int group = run / EA_GROUP, groups = (runs + EA_GROUP - 1) / EA_GROUP, members = min(EA_GROUP, runs - group * EA_GROUP);
+            const int home = place_of(group * EA_GROUP);
+            if (last_of(a.tickets + home, members)) {
+                auto member = [&](int k) { return place_of(group * EA_GROUP + k); };
+                if (groups == 1) {
+                    join(members, member, [&](const float (&v)[4], int, int row, int w, int n, int count) { give_out(v, row, w, n, count); });
+                } else {
+                    join(members, member, [&](const float (&v)[4], int i, int, int, int, int) {
+                        *reinterpret_cast<float4*>(a.part_o + (long long)home * EA_ROWS * PART + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                    });
+                    leave(home);
+                    if (last_of(a.tickets + 2 * n_blocks + place_of(0), groups))
+                        join(groups, [&](int k) { return place_of(k * EA_GROUP); },
+                             [&](const float (&v)[4], int, int row, int w, int n, int count) { give_out(v, row, w, n, count); });
+                }
             }
         }
-    }
-
-    // ---- the warps' results together
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
-        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
-        if (c == 0) {
-            m_s[warp][g + 8 * e] = m_run[e];
-            l_s[warp][g + 8 * e] = l_run[e];
-        }
-#pragma unroll
-        for (int t = 0; t < OT; ++t)
-            *reinterpret_cast<float2*>(&shared_o[(warp * EA_ROWS + g + 8 * e) * LD + 8 * t + 2 * c]) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
-    }
-    __syncthreads();
-    const int live_warps = min(EA_WARPS, p_end - p_begin);   // (the others have seen nothing)
-    float* my_o = a.part_o + (long long)blockIdx.x * EA_ROWS * D;
-    float* my_ml = a.part_ml + (long long)blockIdx.x * EA_ROWS * 2;
-    for (int i = threadIdx.x; i < n_rows * D; i += EA_WARPS * 32) {
-        const int row = i / D, d = i % D, at = value_place<D>(d);
-        float m = EA_NONE, l = 0.f, sum = 0.f;
-        for (int w = 0; w < live_warps; ++w) m = fmaxf(m, m_s[w][row]);
-        for (int w = 0; w < live_warps; ++w) {
-            const float f = fast_exp2(m_s[w][row] - m);
-            l = fmaf(f, l_s[w][row], l);
-            sum = fmaf(f, shared_o[(w * EA_ROWS + row) * LD + at], sum);
-        }
-        if (r.runs == 1) {
-            out[row_at(row) + d] = Num<T>::from_f(l != 0.f ? sum / l : 0.f);
-        } else {
-            my_o[i] = sum;
-            if (d == 0) my_ml[2 * row] = m, my_ml[2 * row + 1] = l;
-        }
-    }
-    if (r.runs == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) ticket_s = atomicAdd(a.tickets + r.seq * pairs_each + y, 1);
-    __syncthreads();
-    if (ticket_s != r.runs - 1) return;
-    __threadfence();
-    if (threadIdx.x == 0) a.tickets[r.seq * pairs_each + y] = 0;   // as the next call wants it
-    const long long first = (long long)blockIdx.x - (long long)r.run * pairs_each;
-    for (int i = threadIdx.x; i < n_rows * D; i += EA_WARPS * 32) {
-        const int row = i / D;
-        float m = EA_NONE, l = 0.f, sum = 0.f;
-        for (int k = 0; k < r.runs; ++k) m = fmaxf(m, __ldcg(a.part_ml + ((first + (long long)k * pairs_each) * EA_ROWS + row) * 2));
-        for (int k = 0; k < r.runs; ++k) {
-            const long long part = first + (long long)k * pairs_each;
-            const float f = fast_exp2(__ldcg(a.part_ml + (part * EA_ROWS + row) * 2) - m);
-            l = fmaf(f, __ldcg(a.part_ml + (part * EA_ROWS + row) * 2 + 1), l);
-            sum = fmaf(f, __ldcg(a.part_o + part * EA_ROWS * D + i), sum);
-        }
-        out[row_at(row) + i % D] = Num<T>::from_f(l != 0.f ? sum / l : 0.f);
+        __syncthreads();   // (the next pair takes the same shared memory)
     }
 }
 
@@ -540,14 +618,13 @@ template <typename T, int D> static int slots_of() {
         if (cudaFuncSetAttribute(attend_e4m3_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D>::SMEM) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_e4m3_kernel<T, D>, EA_WARPS * 32, Shape<T, D>::SMEM) != cudaSuccess)
             return 0;
-        cached[device] = n * qf_sm_count();
+        cached[device] = std::min(n * qf_sm_count(), EA_GROUP * EA_MOST_GROUPS);
     }
     return cached[device];
 }
-template <typename T, int D> static int attend(const void* q, void* out, AttendArgs& a, long long records, cudaStream_t stream) {
-    a.block_slots = slots_of<T, D>();
-    if (a.block_slots <= 0) return (int)cudaErrorInvalidDeviceFunction;
-    return (int)launch_pdl(attend_e4m3_kernel<T, D>, dim3((unsigned)records), dim3(EA_WARPS * 32), Shape<T, D>::SMEM, stream, (const T*)q, (T*)out, a);
+template <typename T, int D> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
+    if (a.block_slots <= 0 || a.block_slots != slots_of<T, D>()) return (int)cudaErrorInvalidValue;
+    return (int)launch_pdl(attend_e4m3_kernel<T, D>, dim3(blocks), dim3(EA_WARPS * 32), Shape<T, D>::SMEM, stream, (const T*)q, (T*)out, a);
 }
 
 #define EA_EVERY(T, CALL)               \
@@ -573,21 +650,22 @@ QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim) {
     return 0;
 }
 
-// q, out [tokens][n_heads * head_dim]; chunks: rows of 16 of the longest span, ceil(tokens * n_heads / kv_heads / 16); most_pages: the most pages that a
-// sequence reads. part_o [records][16][head_dim], part_ml [records][16][2] with records = (n_seqs * kv_heads * chunks + slots), or that many pairs times
-// ceil(most_pages / 4) if fewer; tickets [n_seqs * kv_heads * chunks], zero before the first call and after every call.
+// q, out [tokens][n_heads * head_dim], on 16 bytes; single: every entry has one token; chunks: rows of 16 of the longest span, ceil(tokens * n_heads /
+// kv_heads / 16); most_pages: the most pages that a sequence reads; blocks: n_seqs * kv_heads * chunks * ceil(most_pages / 4), block_slots (of
+// qf_attention_e4m3_slots) at most. part_o [2 * blocks][16][32 * ceil(head_dim / 32)], part_ml [2 * blocks][16][2]; tickets [4 * blocks], zero before the
+// first call and after every call.
 QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int* cu_q, const int* tok_pos, const int* slots, void* codes, float* scales,
                                 const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots, int kv_heads,
-                                int head_dim, int n_heads, int n_seqs, int chunks, int most_pages, long long records, float scale, int window, float* part_o,
-                                float* part_ml, int* tickets, int* err, cudaStream_t stream) {
+                                int head_dim, int n_heads, int n_seqs, int single, int chunks, int most_pages, int blocks, int block_slots, float scale, int window,
+                                float* part_o, float* part_ml, int* tickets, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (head_dim <= 0 || head_dim % 16 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads || chunks <= 0 || most_pages <= 0 || columns <= 0 || n_slots <= 0 ||
-        page_bytes % 16 || (uintptr_t)codes % 16 || page_bytes < 2ll * kv_heads * QF_PAGE * head_dim || page_scales < 2ll * kv_heads || records <= 0 ||
-        records > 0x7fffffffll || window < 0 || (long long)n_seqs * kv_heads * chunks > 0x7fffffffll)
+        page_bytes % 16 || ((uintptr_t)codes | (uintptr_t)q | (uintptr_t)out) % 16 || page_bytes < 2ll * kv_heads * QF_PAGE * head_dim || page_scales < 2ll * kv_heads ||
+        blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
     if (n_seqs <= 0) return 0;
-    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_seqs, chunks, most_pages, 0, window, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
-#define EA_ATTEND(T, D) attend<T, D>(q, out, a, records, stream)
+    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_seqs, single, chunks, most_pages, block_slots, window, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
+#define EA_ATTEND(T, D) attend<T, D>(q, out, a, blocks, stream)
     if (is_bf16) {
         EA_EVERY(bf16, EA_ATTEND)
     } else {

@@ -64,7 +64,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(EW_WARPS * 32)
 write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                   const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
-                  T* __restrict__ q_out, E4m3Site site, int n_tokens, int share, int most_rows, int* err) {
+                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_tokens, int share, int most_rows, int* err) {
     grid_chain_entry();
     extern __shared__ float2 turn[];   // [rows of a run][rot_dim / 2] cosine, sine
     const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2, pass = D - rot_dim;
@@ -75,7 +75,7 @@ write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     for (int t = t_begin; t < t_end; ++t) {
         const int seq = tok_seq[t], first_pos = tok_pos[t];
         if (t != cu_q[seq] && first_pos % QF_PAGE != 0) continue;   // (the run began at an earlier token)
-        const int slot = slots[seq], at = first_pos % QF_PAGE;
+        const int slot = write_cache ? slots[seq] : -1, at = first_pos % QF_PAGE;
         int rows = min(cu_q[seq + 1] - t, QF_PAGE - at);
         if (rows > most_rows) {   // (an entry longer than the call has said: there is no room for its angles)
             if (threadIdx.x == 0) atomicOr(err, QF_ERR_ROW_RANGE);
@@ -182,7 +182,7 @@ write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
 
 template <typename T>
 static int write_launch(const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq, const int* tok_pos, const int* slots,
-                        const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int n_tokens, int max_q_len, int* err,
+                        const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int write_cache, int n_tokens, int max_q_len, int* err,
                         cudaStream_t stream) {
     const int heads = n_heads + 2 * site.kv_heads, slices = (heads + EW_WARPS - 1) / EW_WARPS;
     const int share = max_q_len > 1 ? 16 : 1;
@@ -191,9 +191,9 @@ static int write_launch(const void* qkv, const void* bias, long long qkv_stride,
     const bool wide = rot_dim % 16 == 0 && qkv_stride % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias) % 16 == 0;
     const dim3 grid((n_tokens + share - 1) / share, slices);
     return (int)(wide ? launch_pdl(write_e4m3_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
-                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, n_tokens, share, most_rows, err)
+                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err)
                       : launch_pdl(write_e4m3_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
-                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, n_tokens, share, most_rows, err));
+                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err));
 }
 
 static bool site_fits(const E4m3Site& s) {
@@ -206,13 +206,13 @@ static bool site_fits(const E4m3Site& s) {
 QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq,
                                        const int* tok_pos, const int* slots, const float* inv_freq, int rot_dim, int n_heads, void* q_out, void* codes,
                                        float* scales, const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots,
-                                       int kv_heads, int head_dim, int n_tokens, int max_q_len, int* err, cudaStream_t stream) {
+                                       int kv_heads, int head_dim, int write_cache, int n_tokens, int max_q_len, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (!inv_freq) rot_dim = 0;
     if (!site_fits(site) || head_dim > 128 || rot_dim < 0 || rot_dim > head_dim || (rot_dim & 1) || n_heads <= 0 || max_q_len <= 0) return (int)cudaErrorInvalidValue;
     if (n_tokens <= 0) return 0;
-    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, n_tokens, max_q_len, err, stream)
-                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, n_tokens, max_q_len, err, stream);
+    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, max_q_len, err, stream)
+                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, max_q_len, err, stream);
 }
 
 // ---- Read back: the rows that a batch's sequences hold (from the first that a window of `window` positions leaves the first new token, 0:

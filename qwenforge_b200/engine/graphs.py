@@ -81,6 +81,8 @@ class DecodeGraph:
             tok_seq=arange[:rows].clone(), tok_pos=self.tok_pos, slots=self.slots, cu_q=arange,
             want_rows=arange[:rows].clone(), err=model.err, dtype=model.dtype, attention=model.attention,
             decode_scratch=ops.DecodeScratch(device))  # the graph's own: its addresses are baked into the capture
+        if model.cache_dtype is not None:
+            self.ctx.codes_scratch = ops.E4m3Scratch(device)
         if shared is not None:   # (what is shared is the graph's own too: a later session of the same shape loads it anew)
             self.ctx.shared, self.ctx.shared_scratch = shared, ops.SharedScratch(device)
         self.sample_scratch = ops.SampleScratch()
@@ -281,12 +283,15 @@ class PrefillGraphs:
         integers = torch.zeros(step.packed.size, dtype=torch.int32, device=model.device)
         integers.copy_(torch.from_numpy(step.packed))
         ctx = context_of(step, integers, model.err, model.dtype, model.attention, model.decode_scratch)
+        if model.cache_dtype is not None:
+            ctx.codes_scratch = ops.E4m3Scratch(model.device)
         ctx.host_slots = ctx.host_starts = ctx.host_q_lens = None  # a replay's differ: no part may plan on them
         stream = torch.cuda.Stream(device=model.device)
         stream.wait_stream(torch.cuda.current_stream())
         torch.cuda.synchronize()
         before = ops.kernels.launches
         graph = torch.cuda.CUDAGraph()
+        graph.codes_scratch = ctx.codes_scratch   # (its addresses are baked into the capture: it lives as long)
         with capturing(graph, stream, self.pool):
             logits = model.forward(ctx, cache)
         if self.pool is None:

@@ -13,11 +13,11 @@ from typing import Optional, Sequence
 import torch
 
 from .. import ops
-from ..cache import SequenceCache
-from ..config import ModelConfig, ModelSpec, load_config, resolve_dtype
+from ..cache import BundleNeed, KvNeed, SequenceCache
+from ..config import ModelConfig, ModelSpec, load_config, resolve_cache_dtype, resolve_dtype
 from ..csrc import prepare
 from ..parts import build_block, build_part
-from ..parts.base import Pending, PendingNormed, PendingStreams
+from ..parts.base import Mixer, Pending, PendingNormed, PendingStreams
 from ..weights import load_weights, random_state_on_device
 from .step import StepContext, context_of, pack_step
 
@@ -29,7 +29,9 @@ def _walk(part):
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, attention: str = "auto"):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, attention: str = "auto", cache_dtype=None):
+        """`cache_dtype`: None or "auto" (keys and values in `dtype`), or "float8_e4m3" (in 8 bits; every mixer that keeps keys and values
+        must have that form)."""
         spec.validate()
         self.spec = spec
         self.dtype = resolve_dtype(dtype)
@@ -41,7 +43,10 @@ class Model:
         self.final_norm = build_part("norm", spec.final_norm)
         self.head = build_part("head", spec.head)
         self.err = None
-        self.decode_scratch = self.shared_scratch = None
+        self.decode_scratch = self.shared_scratch = self.codes_scratch = None
+        self.cache_dtype = resolve_cache_dtype(cache_dtype)
+        if self.cache_dtype is not None:
+            self._refuse_other_caches()
         self.prefill_graphs = None  # engine.graphs.PrefillGraphs once enabled
         # a callable (index, hidden, delta) that is shown the float32 residual stream after the embedding (index 0) and
         # after every schedule entry (index k + 1); the stream's value there is hidden + delta when delta is pending.
@@ -79,6 +84,15 @@ class Model:
                 needs[e.cache_from] = needs[e.cache_from].merged(own)
         return needs
 
+    def _refuse_other_caches(self) -> None:
+        """A cache in 8 bits is for mixers that say so; a state of fixed size stays as it is."""
+        for index, block in enumerate(self.blocks):
+            for mixer in (part for part in _walk(block) if isinstance(part, Mixer)):
+                need = mixer.cache_need()
+                flat = [n for _, n in need.flat()] if isinstance(need, BundleNeed) else [need]
+                if any(isinstance(n, KvNeed) for n in flat) and not mixer.takes_cache_dtype(self.cache_dtype):
+                    raise ValueError(f"layer {index}: its {mixer.kind or 'mixer'} has no form for a cache in {self.cache_dtype}")
+
     # ------------------------------------------------------------------ weights
     def bind(self, tensors) -> "Model":
         ops.require_cuda(self.device, "the model")
@@ -87,35 +101,38 @@ class Model:
         libraries = {"embed", "norm", "host"}
         for part in self.parts():
             libraries |= part.kernel_libraries(self.dtype)
+        if self.cache_dtype is not None:
+            libraries |= {"cache_e4m3", "attention_e4m3", "page_copy"}
         prepare(libraries)
         for part in self.parts():
             part.bind(tensors, self.dtype, self.device)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.decode_scratch = ops.DecodeScratch(self.device)
         self.shared_scratch = ops.SharedScratch(self.device)
+        self.codes_scratch = None if self.cache_dtype is None else ops.E4m3Scratch(self.device)
         self._bound = True
         return self
 
     @classmethod
-    def from_dir(cls, model_dir, dtype="auto", device="cuda", attention: str = "auto") -> "Model":
+    def from_dir(cls, model_dir, dtype="auto", device="cuda", attention: str = "auto", cache_dtype=None) -> "Model":
         config = load_config(model_dir)
-        return cls.from_config(config, model_dir, dtype, device, attention)
+        return cls.from_config(config, model_dir, dtype, device, attention, cache_dtype)
 
     @classmethod
-    def from_config(cls, config: ModelConfig, model_dir, dtype="auto", device="cuda", attention: str = "auto") -> "Model":
+    def from_config(cls, config: ModelConfig, model_dir, dtype="auto", device="cuda", attention: str = "auto", cache_dtype=None) -> "Model":
         resolved = resolve_dtype(dtype, getattr(config, "torch_dtype", None))
-        model = cls(config.model_spec(), resolved, device, attention)
+        model = cls(config.model_spec(), resolved, device, attention, cache_dtype)
         model.config = config
         tensors = load_weights(model_dir, model.tensor_specs(), resolved, model.device, model.spec.redundant_tensors,
                                model.spec.ignored_tensors)
         return model.bind(tensors)
 
     @classmethod
-    def from_random(cls, config: ModelConfig, seed: int = 0, dtype="bfloat16", device="cuda", attention: str = "auto") -> "Model":
+    def from_random(cls, config: ModelConfig, seed: int = 0, dtype="bfloat16", device="cuda", attention: str = "auto", cache_dtype=None) -> "Model":
         """A model of `config` whose weights are drawn on the device (no model folder): for measurements at sizes of
         tens of GB. `write_random_model` + `from_dir` is the mode whose weights a plain implementation can read."""
         resolved = resolve_dtype(dtype, getattr(config, "torch_dtype", None))
-        model = cls(config.model_spec(), resolved, device, attention)
+        model = cls(config.model_spec(), resolved, device, attention, cache_dtype)
         model.config = config
         ops.require_cuda(model.device, "the model")
         return model.bind(random_state_on_device(model.tensor_specs(), seed, resolved, model.device))
@@ -123,12 +140,13 @@ class Model:
     # ------------------------------------------------------------------ cache
     def new_cache(self, max_tokens: int, max_seqs: int = 256, max_len: Optional[int] = None) -> SequenceCache:
         limit = self.spec.max_positions if max_len is None else min(max_len, self.spec.max_positions)
-        return SequenceCache(self.cache_needs(), max_tokens, max_seqs, limit, self.dtype, self.device)
+        return SequenceCache(self.cache_needs(), max_tokens, max_seqs, limit, self.dtype, self.device, self.cache_dtype)
 
     # ------------------------------------------------------------------ the step
     def forward(self, ctx: StepContext, cache: SequenceCache) -> Optional[torch.Tensor]:
         """Run the schedule over the context's tokens; logits of ctx.want_rows (None if nothing is wanted)."""
         ctx.step_memo = {"model.resolves_sums": True}   # (below)
+        ctx.cache_dtype = getattr(cache, "kv_dtype", None)
         hidden = ctx.embedded if ctx.embedded is not None else self.embedding.forward(ctx.token_ids, ctx)
         delta = None
         # the embedding's output as it is, for stream parts that mix it in again later (the stream itself is updated in place)
@@ -211,7 +229,7 @@ class Model:
         if not replayed:
             # from pageable memory the copy is complete when the call returns, so the host array may go
             dev = torch.from_numpy(step.packed).to(self.device)
-            ctx = context_of(step, dev, self.err, self.dtype, self.attention, self.decode_scratch)
+            ctx = context_of(step, dev, self.err, self.dtype, self.attention, self.decode_scratch, self.codes_scratch)
             if ctx.is_decode:
                 ctx.shared, ctx.shared_scratch = cache.shared_worth_reading(step.host_slots), self.shared_scratch
             if extras:

@@ -43,6 +43,7 @@ def parse_args(argv=None):
                    help="most tokens live requests hold at any time")
     p.add_argument("--dump-layers", default=None, metavar="DIR",
                    help="also write the residual stream after the embedding and after every schedule entry")
+    p.add_argument("--cache-dtype", default="auto", choices=["auto", "float8_e4m3"], help="what the sequence cache keeps keys and values in")
     p.add_argument("--device", default="cuda")
     p.add_argument("--attn-implementation", default="sdpa",
                    help="'sdpa': fastest attention kernels that take the shapes; anything else: the plain SIMT kernel")
@@ -97,7 +98,7 @@ def main(argv=None) -> int:
     out_dir.mkdir(parents=True, exist_ok=True)
     attention = "auto" if args.attn_implementation.lower() in ("sdpa", "flash", "auto") else "generic"
     with torch.inference_mode():
-        model = Model.from_dir(args.model, args.dtype, args.device, attention)
+        model = Model.from_dir(args.model, args.dtype, args.device, attention, args.cache_dtype)
         # every live request may leave its last page partly empty: one page more per slot
         max_seqs = min(max(args.max_tokens, 1), 1024)
         n_tokens = round_up(max(args.max_tokens, 1), PAGE_TOKENS) + max_seqs * PAGE_TOKENS

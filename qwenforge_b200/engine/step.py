@@ -35,6 +35,10 @@ class StepContext:
     # those once for all of them; None: every sequence is read by itself
     shared: Optional[object] = None
     shared_scratch: Optional[object] = None
+    # a cache in 8 bits: its dtype (the model sets it before every run of its schedule; None: keys and values in the model's own), and the workspaces
+    # of the attention over it
+    cache_dtype: Optional[torch.dtype] = None
+    codes_scratch: Optional[object] = None
     # per-token side inputs named by whoever feeds the step, [T, ...] on the device: what a part needs beyond a
     # token's index in its sequence (positions on several axes, token types). `tok_pos` stays the index that
     # orders the cache and the causal mask.
@@ -108,7 +112,7 @@ def pack_step(entries: Sequence[tuple[int, int, Sequence[int]]], want: Optional[
 
 
 def context_of(step: PackedStep, dev: torch.Tensor, err: torch.Tensor, dtype: torch.dtype, attention: str = "auto",
-               decode_scratch=None) -> StepContext:
+               decode_scratch=None, codes_scratch=None) -> StepContext:
     """The context whose tensors are views of `dev`, a device copy of `step.packed` (or a buffer that will hold one)."""
     o = 0
 
@@ -123,7 +127,7 @@ def context_of(step: PackedStep, dev: torch.Tensor, err: torch.Tensor, dtype: to
         n_seqs=n, n_tokens=total, max_q_len=step.max_q_len, max_kv_len=step.max_kv_len,
         token_ids=take(total), tok_seq=take(total), tok_pos=take(total), slots=take(n), cu_q=take(n + 1),
         want_rows=take(step.n_rows) if step.n_rows else None, err=err, dtype=dtype, attention=attention,
-        decode_scratch=decode_scratch,
+        decode_scratch=decode_scratch, codes_scratch=codes_scratch,
         host_slots=step.host_slots, host_starts=step.host_starts, host_q_lens=step.host_q_lens,
     )
 

@@ -62,7 +62,7 @@ def _batch(what: str, cu_q, tok_pos, slots, err) -> None:
 
 def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor,
                           inv_freq: Optional[torch.Tensor], rot_dim: int, n_heads: int, q_out: torch.Tensor, site: E4m3SiteArgs, max_q_len: int,
-                          err: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+                          err: torch.Tensor, bias: Optional[torch.Tensor] = None, write_cache: bool = True) -> None:
     """`rope_cache_write` into a cache in 8 bits: qkv [T, (NH + 2 KVH) D] (bfloat16 or float32; perhaps the first columns of wider rows) with its bias, q and
     k heads rotated by position (split halves of the first rot_dim components; inv_freq None: not at all), q to q_out [T, NH D], k and v
     as codes. Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at most max_q_len, at consecutive positions; a slot is in one entry at
@@ -71,7 +71,7 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     A page that gets rows takes, per plane and head, the least power of two under which all their finite elements lie within +-448 (of 2^-112
     to 2^119), and no less than it has if it held rows before the new ones; those rows' codes are then rounded to the larger unit. Rounding is
     to nearest even, once, from float32. Infinities become +-448, NaN stays. Rows behind the new ones stay as they are; a padding
-    entry (slot -1) writes its queries only."""
+    entry (slot -1) writes its queries only, as does every entry with `write_cache` false."""
     dtype = qkv.dtype
     is_bf16 = kernels._is_bf16(dtype)
     kernels._rows("qkv", qkv)
@@ -97,9 +97,9 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     _here("rope_cache_write_e4m3", qkv, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, site.storage, site.scales, site.table, err, bias)
     if n == 0:
         return
-    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _P, _P)(
+    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _P, _P)(
         is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
-        n_heads, q_out.data_ptr(), *site.address(), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
+        n_heads, q_out.data_ptr(), *site.address(), bool(write_cache), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
 
 
 def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_seqs: int, max_kv_len: int,
@@ -127,6 +127,11 @@ def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor
         *site.address(), n_seqs, pages, window, err.data_ptr(), _stream()), "cache_read_e4m3")
 
 
+def attention_e4m3_pays(max_q_len: int, group: int) -> bool:
+    """Whether a step of up to `max_q_len` tokens per sequence, `group` query heads to a kv head, attends over the codes: its rows fill few tiles."""
+    return max_q_len * group <= 4 * E4M3_ROWS
+
+
 class E4m3Scratch:
     """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). One
     instance serves calls that run one after another on one stream; what is captured into a graph has one of its own."""
@@ -135,13 +140,14 @@ class E4m3Scratch:
         self.device = torch.device(device)
         self.part_o = self.part_ml = self.tickets = None
 
-    def ensure(self, records: int, pairs: int, head_dim: int) -> None:
-        if self.part_o is None or self.part_o.numel() < records * E4M3_ROWS * head_dim:
-            self.part_o = torch.empty(records * E4M3_ROWS * head_dim, dtype=torch.float32, device=self.device)
-        if self.part_ml is None or self.part_ml.numel() < records * E4M3_ROWS * 2:
-            self.part_ml = torch.empty(records * E4M3_ROWS * 2, dtype=torch.float32, device=self.device)
-        if self.tickets is None or self.tickets.numel() < pairs:
-            self.tickets = torch.zeros(pairs, dtype=torch.int32, device=self.device)
+    def ensure(self, blocks: int, head_dim: int) -> None:
+        rows = 2 * blocks * E4M3_ROWS
+        if self.part_o is None or self.part_o.numel() < rows * -(-head_dim // 32) * 32:
+            self.part_o = torch.empty(rows * -(-head_dim // 32) * 32, dtype=torch.float32, device=self.device)
+        if self.part_ml is None or self.part_ml.numel() < 2 * rows:
+            self.part_ml = torch.empty(2 * rows, dtype=torch.float32, device=self.device)
+        if self.tickets is None or self.tickets.numel() < 4 * blocks:
+            self.tickets = torch.zeros(4 * blocks, dtype=torch.int32, device=self.device)
 
 
 _block_slots: dict = {}
@@ -175,6 +181,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
         raise KernelError(f"attention_e4m3: {n_heads} heads do not divide into {kv_heads} groups")
     if q.dim() != 2 or q.shape[1] != n_heads * d or out.shape != q.shape:
         raise KernelError("attention_e4m3: q/out widths do not match the head count")
+    if q.data_ptr() % 16 or out.data_ptr() % 16:
+        raise KernelError("attention_e4m3: q and out begin on 16 bytes")
     if slots.numel() != n_seqs or tok_pos.numel() != q.shape[0] or window < 0:
         raise KernelError("attention_e4m3: wants n_seqs slots, a position per token and a window of 0 or more")
     if n_seqs and (max_q_len <= 0 or (max_kv_len is not None and max_kv_len <= 0)):
@@ -187,10 +195,10 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     if window > 0:
         most = min(most, -(-(window + max_q_len - 1) // PAGE_TOKENS) + 1)
     chunks = -(-min(max_q_len, q.shape[0]) * (n_heads // kv_heads) // E4M3_ROWS)
-    pairs = n_seqs * kv_heads * chunks
-    records = min(pairs + _slots_of(is_bf16, d), pairs * -(-most // E4M3_WARPS))
-    scratch.ensure(records, pairs, d)
+    block_slots = _slots_of(is_bf16, d)
+    blocks = min(block_slots, n_seqs * kv_heads * chunks * -(-most // E4M3_WARPS))
+    scratch.ensure(blocks, d)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
-    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _LL, _F, _I, _P, _P, _P, _P, _P)(
-        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.address(), n_heads, n_seqs, chunks, most, records,
-        scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
+    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P)(
+        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.address(), n_heads, n_seqs,
+        max_q_len == 1 and q.shape[0] == n_seqs, chunks, most, blocks, block_slots, scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")

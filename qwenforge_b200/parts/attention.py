@@ -42,6 +42,8 @@ Options that other designs switch on, each a parameter of the spec (all off for 
                  weight files (`bias_scale`, `bias_rate`)
   out_gate       the concatenated heads are multiplied element by element with sigmoid(G h), a projection [heads * value_dim,
                  hidden] of the same input whose columns follow those of q, k, v in the one product
+A cache in 8 bits (`ctx.cache_dtype`) is taken by the plain form, at the head sizes of its kernels: keys and values are written as codes,
+single tokens and short spans attend over the codes, longer spans over the values that are read back into the group's storage for them.
 The position part may pair components 2j and 2j + 1 (`rotary_interleaved`) instead of j and j + R/2.
 """
 from __future__ import annotations
@@ -295,6 +297,8 @@ class GqaAttention(Mixer):
         n = x.shape[0]
         if not self.plain:
             return self._forward_with_options(x, ctx, site, writes_cache)
+        if site.scales is not None:
+            return self._forward_codes(x, ctx, site, writes_cache)
         fast = (ctx.attention == "auto" and x.dtype == torch.bfloat16
                 and self.head_dim in ops.FAST_ATTENTION_HEAD_DIMS)
         shares = self.reads_shared(ctx)
@@ -450,6 +454,10 @@ class GqaAttention(Mixer):
         return qkv, ops.residual_product_way(rows, self.o_weight)
 
     def fused_takes(self, ctx) -> bool:
+        if ctx.cache_dtype is not None:   # the output projection adds in place; what writes codes is a kernel behind the product
+            return (self.plain and ctx.attention == "auto" and ctx.is_decode and ctx.dtype == torch.bfloat16 and ctx.n_tokens <= ops.WIDE_MAX_ROWS
+                    and not self.out_bias and (self.position is None or self.position.fused_rotary() is not None)
+                    and ops.residual_product_way(ctx.n_tokens, self.o_weight) != "unfused")
         if not (self.plain and ctx.attention == "auto" and ctx.is_decode and ctx.dtype == torch.bfloat16
                 and ctx.n_tokens <= ops.WIDE_MAX_ROWS and self.head_dim in ops.FAST_ATTENTION_HEAD_DIMS and not self.out_bias):
             return False
@@ -467,7 +475,7 @@ class GqaAttention(Mixer):
     def takes_sums(self, hidden, ctx) -> bool:
         """Whether `fused_forward` will be run on this step and takes a `PendingSums`: the QKV product reads it beside the stream, the
         projection moves it there."""
-        if not self.fused_takes(ctx):
+        if ctx.cache_dtype is not None or not self.fused_takes(ctx):
             return False
         qkv_way, o_way = self._ways(ctx)
         rotary = self.position.fused_rotary() if self.position is not None else None
@@ -476,6 +484,8 @@ class GqaAttention(Mixer):
 
     def fused_forward(self, hidden, rms, ctx, site, writes_cache, delta=None):
         n = hidden.shape[0]
+        if site.scales is not None:
+            return self._fused_forward_codes(hidden, rms, ctx, site, writes_cache, delta)
         qkv_way, o_way = self._ways(ctx)
         sums = None
         if isinstance(delta, PendingSums):   # (`takes_sums` has said yes)
@@ -523,12 +533,69 @@ class GqaAttention(Mixer):
         else:
             ops.attention_decode(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs,
                                  self.scale, self.window, n_splits, ctx.decode_scratch, ctx.err, plan)
+        self._project_into(hidden, attended, o_way, ctx)
+
+    def _project_into(self, hidden, attended, o_way, ctx) -> None:
         if o_way == "skinny":
             ops.skinny_gemm(ops.EPI_RESIDUAL, self.o_weight, x=attended, residual=hidden)
         elif o_way == "wide":
             ops.wide_gemm(ops.EPI_RESIDUAL, self.o_weight, x=attended, residual=hidden, err=ctx.err)
         else:
             ops.residual_add(hidden, ops.linear(attended, self.o_weight))
+
+    # ---- a cache in 8 bits
+    def takes_cache_dtype(self, dtype) -> bool:
+        return self.plain and self.cache_need().fits(dtype)
+
+    def _queries_over_codes(self, qkv, ctx, site, writes_cache, rotary, bias):
+        """Rows of the projection -> the attended heads: queries out, keys and values into the cache, attention over it."""
+        n = qkv.shape[0]
+        inv_freq, rot_dim = rotary if rotary is not None else (None, 0)
+        q = torch.empty((n, self.q_width), dtype=qkv.dtype, device=qkv.device)
+        ops.rope_cache_write_e4m3(qkv, ctx.cu_q, ctx.tok_seq, ctx.tok_pos, ctx.slots, inv_freq, rot_dim, self.n_heads, q, site.codes(), ctx.max_q_len, ctx.err,
+                                  bias=bias, write_cache=writes_cache)
+        attended = torch.empty_like(q)
+        if ctx.attention == "auto" and ops.attention_e4m3_pays(ctx.max_q_len, self.n_heads // self.n_kv):
+            ops.attention_e4m3(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window,
+                               ctx.codes_scratch, ctx.err, ctx.max_kv_len)
+            return attended
+        values = site.group.values
+        ops.cache_read_e4m3(values, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), ctx.n_seqs, ctx.max_kv_len, ctx.err, window=self.window)
+        args = ops.KvSiteArgs(values, site.table, self.n_kv, self.head_dim)
+        if ctx.attention == "auto" and qkv.dtype == torch.bfloat16 and self.head_dim in ops.FAST_ATTENTION_HEAD_DIMS:
+            prefill = prefill_attention(self.head_dim, n, ctx.max_kv_len, self.window, max_q_len=ctx.max_q_len, n_seqs=ctx.n_seqs, n_heads=self.n_heads,
+                                        kv_heads=self.n_kv)
+            prefill(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window, ctx.err,
+                    max_kv_len=ctx.max_kv_len)
+        else:
+            ops.attention_generic(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, args, self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window, ctx.err,
+                                  scratch=ctx.decode_scratch, max_kv_len=ctx.max_kv_len)
+        return attended
+
+    def _forward_codes(self, x, ctx, site, writes_cache):
+        n = x.shape[0]
+        rotary = self.position.fused_rotary() if self.position is not None else None
+        late_bias = self.position is None or rotary is not None
+        qkv = ops.linear(x, self.qkv_weight, None if late_bias else self.qkv_bias_t)
+        if not late_bias:
+            self.position.apply(qkv[:, :self.q_width].view(n, self.n_heads, self.head_dim),
+                                qkv[:, self.q_width:self.q_width + self.kv_width].view(n, self.n_kv, self.head_dim), ctx)
+        attended = self._queries_over_codes(qkv, ctx, site, writes_cache, rotary, self.qkv_bias_t if late_bias else None)
+        return ops.linear(attended, self.o_weight, self.o_bias_t)
+
+    def _fused_forward_codes(self, hidden, rms, ctx, site, writes_cache, delta) -> None:
+        n = hidden.shape[0]
+        if ops.skinny_gemm_takes(n, self.qkv_weight, ops.EPI_PLAIN, True) and ops.skinny_gemm_pays(n, self.qkv_weight):
+            if delta is not None:
+                ops.residual_add(hidden, delta)
+            qkv = torch.empty((n, self.qkv_width), dtype=torch.bfloat16, device=hidden.device)
+            ops.skinny_gemm(ops.EPI_PLAIN, self.qkv_weight, hidden=hidden, norm_weight=rms[0], eps=rms[1], out=qkv, constants=True)
+        else:
+            x = torch.empty(hidden.shape, dtype=torch.bfloat16, device=hidden.device)
+            ops.add_rms_norm(hidden, delta, rms[0], rms[1], x, constant_weight=True)
+            qkv = ops.linear(x, self.qkv_weight)
+        attended = self._queries_over_codes(qkv, ctx, site, writes_cache, self.position.fused_rotary() if self.position is not None else None, self.qkv_bias_t)
+        self._project_into(hidden, attended, ops.residual_product_way(n, self.o_weight), ctx)
 
     def reads_shared(self, ctx) -> bool:
         """Whether this step's sequences begin with the same pages and the layer reads those once for all of them."""

@@ -357,6 +357,10 @@ class Mixer(Part):
     def cache_need(self):
         return None
 
+    def takes_cache_dtype(self, dtype) -> bool:
+        """Whether the part runs on a cache that keeps keys and values in this dtype instead of the model's own."""
+        return False
+
     def forward(self, x: torch.Tensor, ctx, site, writes_cache: bool) -> torch.Tensor:
         raise NotImplementedError
 

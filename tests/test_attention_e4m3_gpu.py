@@ -283,7 +283,7 @@ def test_refusals():
         ops.attention_e4m3(**a)
     for change in (dict(q=q.half()), dict(q=q.cpu()), dict(q=q[:, :-64]), dict(q=q.t().contiguous().t()), dict(out=out.float()), dict(out=out[:2]), dict(n_heads=3),
                    dict(n_heads=0), dict(n_heads=8), dict(n_seqs=2), dict(max_q_len=0), dict(max_kv_len=0), dict(window=-1), dict(cu_q=d["cu_q"].long()),
-                   dict(tok_pos=d["tok_pos"][:2]), dict(slots=d["slots"].cpu()), dict(err=c.err.long())):
+                   dict(tok_pos=d["tok_pos"][:2]), dict(q=torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")[1:].view(q.shape)), dict(slots=d["slots"].cpu()), dict(err=c.err.long())):
         with pytest.raises(KernelError):
             attend(**change)
     attend()
