@@ -2,14 +2,14 @@
 //
 //   o = softmax_j(q k_j^T scale) v_j over the keys j that the token sees: max(0, p - window + 1) <= j <= p
 //
-// The codes are multiplied as float16, in which they are exact, with float32 sums; a page's two powers of two enter behind the products:
-// that of the keys as a factor of the scores, that of the values as a factor of the page's share of the output. Queries become
-// float16 behind a power of two per row that brings their largest element to 2^7 .. 2^8: bfloat16 queries lose nothing but what lies 2^-31
-// below that, float32 queries are two such numbers (22 bits) and take two products. Weights are 2^(s - m + 14), at most 2^14 for
-// the running maximum m: rounded to float16 (2^-12 of each weight, less than the output's own rounding) where the output is bfloat16, two
-// numbers where it is float32. Maxima, sums and outputs are float32.
+// The codes are multiplied as float16, in which they are exact, with float32 sums. A page's power of two for the keys is a factor of its scores; that
+// for the values is the unit in which a row's sum of outputs is kept while the page adds to it (an exact shift where the next page's differs).
+// Queries become float16 behind a power of two per row that brings their largest element to 2^7 .. 2^8: bfloat16 queries lose nothing but
+// what lies 2^-31 below that, float32 queries are two such numbers (22 bits) and take two products. Weights are 2^(s - m + 14), at most 2^14
+// for the running maximum m: rounded to float16 (2^-12 of each weight, less than the output's own rounding) where the output is bfloat16, two
+// numbers where it is float32. Maxima, sums and outputs are float32; for float32 outputs the tensor cores' sums end with a tile (they cut bits off).
 //
-// A block takes a run of pages of one (sequence, kv head, 16 rows), its warps a page each in turn. A row is a query head of the kv head's
+// A block takes pages of a (sequence, kv head, 16 rows), its warps a page each in turn; a warp looks its next 32 pages and their scales up at once. A row is a query head of the kv head's
 // group and a token of the span; 16 of them are the rows of m16n8k16 products, whose columns are keys, then components. No shared memory
 // lies on the way of the codes: a lane loads what its fragments hold. For the keys, columns are 8 positions and a lane takes D / 4
 // components of one of them, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
@@ -34,7 +34,7 @@
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -134,7 +134,7 @@ __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(cod
 template <typename T, int D> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
     static constexpr int TILE = D <= 64 ? (TWO ? 32 : 64) : (TWO && D > 96 ? 16 : 32);   // positions of a step
-    static constexpr int BLOCKS = D <= 32 ? 4 : D <= 64 ? 3 : 2;      // of an SM
+    static constexpr int BLOCKS = D <= 32 ? 3 : 2;                    // of an SM
     // floats from a row to the next where warps leave their outputs: product t's column n at 8 t + 8 (t / 4) + n, so that four products of 32 lanes
     // meet 32 banks; rows 8 or 24 banks apart, for the warps' own stores
     static constexpr int ROW = D + 8 * ((D / 8 + 3) / 4), LD = ROW % 32 == 8 || ROW % 32 == 24 ? ROW : ROW + 8;
@@ -181,7 +181,12 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     }
 }
 
+// x * 2^e, e of any size that the result has room for
+__device__ __forceinline__ float scaled(float x, int e) { return x * pow2(e / 2) * pow2(e - e / 2); }
+
+#define EA_PAIR_COST 8     // pages whose time a pair's beginning and end take
 #define EA_GROUP 16        // partial results that a block joins at once
+#define EA_SHARE (EA_WARPS * 32 / EA_ROWS)
 #define EA_MOST_GROUPS 64  // ... and groups of them: enough for 1,024 blocks
 
 template <typename T, int D>
@@ -202,14 +207,27 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
     const int q_width = a.n_heads * D, n_blocks = gridDim.x;
 
     // ---- this block's share (every warp works it out for itself)
-    int total = 0, whole = 0, target = EA_WARPS;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) total += s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0;
+    int total = 0, pairs = 0, whole = 0, target = EA_WARPS;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const int pages = s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0;
+        total += pages;
+        pairs += pages > 0;
+    }
     total = (int)warp_sum_u32((uint32_t)total) * pairs_each;
+    pairs = (int)warp_sum_u32((uint32_t)pairs) * pairs_each;
     target = max(target, (total + a.block_slots - 1) / a.block_slots);
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) whole += s0 + lane < a.n_seqs ? (sequence_of(a, s0 + lane).pages + target - 1) / target : 0;
     whole = (int)warp_sum_u32((uint32_t)whole) * pairs_each;
-    const int unit = whole <= a.block_slots ? target : 1;   // pages of a pair are rounded up to whole units
-    if (unit == target) total = whole * target;
+    // pages of a pair are rounded up to whole units; where blocks may have several pairs, each counts EA_PAIR_COST pages more
+    const bool aligned = whole <= a.block_slots;
+    const int ahead = aligned ? 0 : EA_PAIR_COST;
+    if (aligned) {
+        total = whole * target;
+    } else {
+        total += pairs * ahead;
+        target = max(target, (total + a.block_slots - 1) / a.block_slots);
+    }
+    auto places_of = [&](int pages) { return pages == 0 ? 0 : aligned ? (pages + target - 1) / target * target : pages + ahead; };
     // padding entries: zeros
     for (int s = blockIdx.x; s < a.n_seqs; s += n_blocks) {
         const Sequence r = sequence_of(a, s);
@@ -221,7 +239,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
     // the sequence in whose pages it begins
     int seq = 0, base = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const int mine = s0 + lane < a.n_seqs ? (sequence_of(a, s0 + lane).pages + unit - 1) / unit * unit * pairs_each : 0;
+        const int mine = s0 + lane < a.n_seqs ? places_of(sequence_of(a, s0 + lane).pages) * pairs_each : 0;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -239,15 +257,15 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
     }
 
     Sequence r = sequence_of(a, seq);
-    int padded = (r.pages + unit - 1) / unit * unit;
+    int padded = places_of(r.pages);
     for (int at = range_begin; at < range_end;) {
         while (at >= base + padded * pairs_each) {   // (sequences without pages are passed over)
             base += padded * pairs_each;
             r = sequence_of(a, ++seq);
-            padded = (r.pages + unit - 1) / unit * unit;
+            padded = places_of(r.pages);
         }
         const int y = (at - base) / padded, pair_begin = base + y * padded, kvh = y / a.chunks, chunk = y % a.chunks;
-        const int p_begin = r.page0 + at - pair_begin, p_end = r.page0 + min(min(padded, range_end - pair_begin), r.pages);
+        const int p_begin = r.page0 + max(at - pair_begin - ahead, 0), p_end = r.page0 + min(min(padded, range_end - pair_begin) - ahead, r.pages);
         const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin;
         at = min(pair_begin + padded, range_end);
         if (reports && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
@@ -274,21 +292,33 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
         // ---- keys of a step: pages p_begin + warp, + EA_WARPS, ..., a tile of one at a time
         const int steps = my_pages * PER_PAGE;
         const long long plane = (long long)KVH * QF_PAGE * D;
-        int page_next = -1;          // of the step whose keys are loaded
-        float ks_next = 0.f, vs_next = 0.f;
+        int lane_page = -1, lane_unit = 0;   // of 32 of the warp's pages, one a lane: its number, its scales
+        float lane_scale = 0.f;
+        int page_next = -1, unit_next = 0;   // of the step whose keys are loaded
+        float ks_next = 0.f;
         uint32_t kw[NT][KW];
         auto key0_of = [&](int step) { return (p_begin + warp + step / PER_PAGE * EA_WARPS) * QF_PAGE + step % PER_PAGE * TILE; };
+        auto look_up = [&](int from) {   // pages from .. from + 31 of the warp's
+            lane_page = -1;
+            if (from + lane < my_pages) {
+                lane_page = e4m3_page(site, r.slot, (p_begin + warp + (from + lane) * EA_WARPS) * QF_PAGE);
+                if (lane_page < 0) {
+                    if (y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+                } else {
+                    const float* scales = site.scales + (long long)lane_page * site.page_scales + kvh;
+                    lane_scale = scales[0];
+                    lane_unit = exponent_of(scales[KVH]);
+                }
+            }
+        };
         auto load_keys = [&](int step) {
             const int key0 = key0_of(step);
             if (step % PER_PAGE == 0) {
-                page_next = e4m3_page(site, r.slot, key0);
-                if (page_next < 0) {
-                    if (lane == 0 && y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-                } else {
-                    const float* scales = site.scales + (long long)page_next * site.page_scales + kvh;
-                    ks_next = scales[0];
-                    vs_next = scales[KVH];
-                }
+                const int i = step / PER_PAGE;
+                if (i % 32 == 0) look_up(i);
+                page_next = __shfl_sync(0xffffffffu, lane_page, i % 32);
+                ks_next = __shfl_sync(0xffffffffu, lane_scale, i % 32);
+                unit_next = __shfl_sync(0xffffffffu, lane_unit, i % 32);
             }
             if (page_next < 0 || key0 >= some_hi || key0 + TILE <= some_lo) return;
             const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + g) * D;
@@ -327,8 +357,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                 top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
                 top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
                 const int up = min(max(exponent_of(top[e]) - 7, -119), 120);
-                by[e] = pow2(up) * a.scale_log2;
-                const float down = pow2(-up);
+                by[e] = pow2(up) * fabsf(a.scale_log2);
+                const float down = copysignf(pow2(-up), a.scale_log2);
 #pragma unroll
                 for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -344,68 +374,82 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
 #pragma unroll
         for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m_run[2] = {EA_NONE, EA_NONE}, l_run[2] = {0.f, 0.f};   // (l: this lane's columns only)
+        int unit_run[2] = {0, 0};                                      // o stands for o * 2^unit_run
+        bool begun = false;
 
         for (int step = 0; step < steps; ++step) {
-            const int page = page_next;
-            const int key0 = key0_of(step);
-            const bool live = page >= 0 && key0 < some_hi && key0 + TILE > some_lo;
-            if (!live) {
+            const int page = page_next, key0 = key0_of(step), unit_v = unit_next;
+            const float ks = ks_next;
+            if (page < 0 || key0 >= some_hi || key0 + TILE <= some_lo) {
                 if (step + 1 < steps) load_keys(step + 1);
                 continue;
             }
-            const float ks = ks_next, vs = vs_next;
-            const bool inside = key0 >= some_lo && key0 + TILE <= some_hi;   // every position is held and seen by some row
+            if (!begun) unit_run[0] = unit_run[1] = unit_v;
+            begun = true;
             // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
             uint32_t vw[KT][4][VW];
             {
                 const unsigned char* v = site.codes + (long long)page * site.page_bytes + plane + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + 2 * c) * D;
+                if (key0 >= some_lo && key0 + TILE <= some_hi) {   // every position is held, and seen by some row
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = 16 * kt + (i & 1) + 8 * (i >> 1);
-                        if (inside || (key0 + at + 2 * c >= some_lo && key0 + at + 2 * c < some_hi)) load_value<D>(vw[kt][i], v + (long long)at * D, g);
-                        else
+                        for (int i = 0; i < 4; ++i) load_value<D>(vw[kt][i], v + (16 * kt + (i & 1) + 8 * (i >> 1)) * D, g);
+                } else {
 #pragma unroll
-                            for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies there is nobody's, NaN perhaps)
-                    }
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = 16 * kt + (i & 1) + 8 * (i >> 1), key = key0 + at + 2 * c;
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies elsewhere is nobody's, NaN perhaps)
+                            if (key >= some_lo && key < some_hi) load_value<D>(vw[kt][i], v + at * D, g);
+                        }
+                }
             }
             // ---- scores
             float s[NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
+            for (int w = 0; w < KW; ++w)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
                     const uint32_t b0 = half2_of_low(kw[t][w]), b1 = half2_of_high(kw[t][w]);
                     if constexpr (TWO) mma_f16_16816(s[t], qa[1][w], b0, b1);
                     mma_f16_16816(s[t], qa[0][w], b0, b1);
                 }
-            }
             if (step + 1 < steps) load_keys(step + 1);
-            const float by0 = by[0] * ks, by1 = by[1] * ks;
-            float mx[2] = {EA_NONE, EA_NONE};
+            // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none
+            const float by_k[2] = {by[0] * ks, by[1] * ks};
             const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
+            auto seen = [&](int t, int e) {
+                const int key = key0 + 8 * t + 2 * c + (e & 1);
+                return key >= lo[e >> 1] && key < hi[e >> 1];
+            };
+            float top[2] = {EA_NONE, EA_NONE}, corr[2], shift[2];
+            if (full) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[t][e] *= e < 2 ? by0 : by1;
-                    if (!full) {
-                        const int key = key0 + 8 * t + 2 * c + (e & 1);
-                        if (key < lo[e >> 1] || key >= hi[e >> 1]) s[t][e] = -INFINITY;
-                    }
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
-                }
-            float corr[2], shift[2];
+                    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (seen(t, e)) top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
+            }
+            float m_tile[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                const float m = fmaxf(m_run[e], mx[e]);
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+                m_tile[e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
+                const float m = fmaxf(m_run[e], m_tile[e]);
                 corr[e] = fast_exp2(m_run[e] - m);
                 m_run[e] = m;
-                shift[e] = m - 14.f;
+                shift[e] = 14.f - m;
                 l_run[e] *= corr[e];
             }
             uint32_t pa[TWO ? 2 : 1][KT][4];
@@ -413,7 +457,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[t][e] = fast_exp2(s[t][e] - shift[e >> 1]);
+                    s[t][e] = fast_exp2(fmaf(s[t][e], by_k[e >> 1], shift[e >> 1]));
+                    if (!full && !seen(t, e)) s[t][e] = 0.f;
                     l_run[e >> 1] += s[t][e];
                 }
 #pragma unroll
@@ -422,52 +467,17 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                     if constexpr (TWO) pa[1][t / 2][2 * (t % 2) + e] = pack_rest(s[t][2 * e], s[t][2 * e + 1], pa[0][t / 2][2 * (t % 2) + e]);
                 }
             }
-            // ---- values: four products from a word of each of four positions
-            auto add_values = [&](auto masked, int from, int upto, bool first, bool mine0, bool mine1) {
+            // ---- values. Word w of the four positions of a step holds their elements of the products 4 w .. 4 w + 3
+            auto word_products = [&](int kt, int w, auto take, auto add) {
+                uint32_t x[4];
 #pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    constexpr bool M = decltype(masked)::value;
-                    const int n = P::v16 != 0 && w == VW - 1 ? 2 : 4;   // products of this word
-                    float acc[4][4];
+                for (int i = 0; i < 4; ++i) x[i] = take(vw[kt][i][w], 16 * kt + 2 * c + (i & 1) + 8 * (i >> 1));
+                const uint32_t u[2] = {__byte_perm(x[0], x[1], 0x5140), __byte_perm(x[0], x[1], 0x7362)};
+                const uint32_t v[2] = {__byte_perm(x[2], x[3], 0x5140), __byte_perm(x[2], x[3], 0x7362)};
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        uint32_t x[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = vw[kt][i][w];
-                            if constexpr (M) {
-                                const int key = key0 + 16 * kt + 2 * c + (i & 1) + 8 * (i >> 1);
-                                if (key < from || key >= upto) x[i] = 0u;
-                            }
-                        }
-                        const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), b01 = __byte_perm(x[2], x[3], 0x5140);
-                        const uint32_t a23 = __byte_perm(x[0], x[1], 0x7362), b23 = __byte_perm(x[2], x[3], 0x7362);
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            if (t >= n) break;
-                            const uint32_t u = t < 2 ? a01 : a23, v = t < 2 ? b01 : b23;
-                            const uint32_t b0 = t & 1 ? half2_of_high(u) : half2_of_low(u), b1 = t & 1 ? half2_of_high(v) : half2_of_low(v);
-                            if constexpr (TWO) mma_f16_16816(acc[t], pa[1][kt], b0, b1);
-                            mma_f16_16816(acc[t], pa[0][kt], b0, b1);
-                        }
-                    }
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if (t >= n) break;
-                        float(&x)[4] = o[4 * w + t];
-                        if constexpr (M) {
-                            if (first) x[0] *= corr[0], x[1] *= corr[0], x[2] *= corr[1], x[3] *= corr[1];
-                            if (mine0) x[0] = fmaf(acc[t][0], vs, x[0]), x[1] = fmaf(acc[t][1], vs, x[1]);
-                            if (mine1) x[2] = fmaf(acc[t][2], vs, x[2]), x[3] = fmaf(acc[t][3], vs, x[3]);
-                        } else {
-                            x[0] = fmaf(acc[t][0], vs, x[0] * corr[0]);
-                            x[1] = fmaf(acc[t][1], vs, x[1] * corr[0]);
-                            x[2] = fmaf(acc[t][2], vs, x[2] * corr[1]);
-                            x[3] = fmaf(acc[t][3], vs, x[3] * corr[1]);
-                        }
-                    }
+                for (int t = 0; t < 4; ++t) {
+                    if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
+                    add(t, t & 1 ? half2_of_high(u[t / 2]) : half2_of_low(u[t / 2]), t & 1 ? half2_of_high(v[t / 2]) : half2_of_low(v[t / 2]));
                 }
             };
             bool apart = false;
@@ -479,19 +489,91 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int w = 0; w < VW; ++w) nan |= holds_nan(vw[kt][i][w]);
-                apart = __any_sync(0xffffffffu, nan);
+                apart = nan;
             }
-            if (!apart) {
-                add_values(std::false_type{}, 0, 0, true, true, true);
-            } else {   // token by token, each with the positions that it sees
-                for (int t = t_first; t <= t_last; ++t) {
-                    const int upto = a.tok_pos[r.begin + t] + 1;
-                    add_values(std::true_type{}, a.window > 0 ? upto - a.window : 0, upto, t == t_first, (row0 + g) / G == t, (row0 + g + 8) / G == t);
+            const int up0 = unit_run[0] - unit_v, up1 = unit_run[1] - unit_v;
+            const bool far = apart || abs(up0) > 30 || abs(up1) > 30;   // (an output is within 2^40 units: 2^14 weights, 448, some thousand pages)
+            if (!__any_sync(0xffffffffu, far)) {
+                const float f0 = corr[0] * pow2(up0), f1 = corr[1] * pow2(up1);
+                unit_run[0] = unit_run[1] = unit_v;
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        float acc[4][4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int t, uint32_t b0, uint32_t b1) {
+                                mma_f16_16816(acc[t], pa[1][kt], b0, b1);
+                                mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                            });
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
+                            float(&x)[4] = o[4 * w + t];
+                            x[0] = fmaf(x[0], f0, acc[t][0]), x[1] = fmaf(x[1], f0, acc[t][1]), x[2] = fmaf(x[2], f1, acc[t][2]), x[3] = fmaf(x[3], f1, acc[t][3]);
+                        }
+                    }
+                } else {
+                    if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
+#pragma unroll
+                        for (int t = 0; t < OT; ++t) o[t][0] *= f0, o[t][1] *= f0, o[t][2] *= f1, o[t][3] *= f1;
+                    }
+#pragma unroll
+                    for (int w = 0; w < VW; ++w)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int t, uint32_t b0, uint32_t b1) { mma_f16_16816(o[4 * w + t], pa[0][kt], b0, b1); });
+                }
+            } else {
+                // scales far apart, or a NaN: a unit in which what was there (2^had at most) and what comes (2^comes) both have room, and token by
+                // token, each with the positions that it sees
+                int shift_old[2], shift_new[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int t = 0; t < OT; ++t) most = fmaxf(most, fmaxf(fabsf(o[t][2 * e]), fabsf(o[t][2 * e + 1])));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)) * corr[e];
+                    const int had = most > 0.f ? unit_run[e] + exponent_of(most) : -1000;
+                    const int comes = unit_v + 30 + (int)fmaxf(m_tile[e] - m_run[e], -800.f);
+                    const int unit_both = max(max(had, comes) - 30, -150);
+                    shift_old[e] = unit_run[e] - unit_both, shift_new[e] = unit_v - unit_both;
+                    unit_run[e] = unit_both;
+                }
+#pragma unroll
+                for (int t = 0; t < OT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[t][e] = ldexpf(o[t][e] * corr[e >> 1], shift_old[e >> 1]);
+                for (int token = t_first; token <= t_last; ++token) {
+                    const int upto = t_first == t_last ? first_hi : a.tok_pos[r.begin + token] + 1, from = a.window > 0 ? upto - a.window : 0;
+                    const bool mine[2] = {(row0 + g) / G == token, (row0 + g + 8) / G == token};
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        float acc[4][4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+                            word_products(kt, w, [&](uint32_t x, int at) { return key0 + at >= from && key0 + at < upto ? x : 0u; }, [&](int t, uint32_t b0, uint32_t b1) {
+                                if constexpr (TWO) mma_f16_16816(acc[t], pa[1][kt], b0, b1);
+                                mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                            });
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (mine[e >> 1]) o[4 * w + t][e] += ldexpf(acc[t][e], shift_new[e >> 1]);
+                        }
+                    }
                 }
             }
         }
 
-        // ---- the warps' results together
+        // ---- the warps' results together: the outputs of each alone, under shares of the whole weight
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
@@ -500,25 +582,31 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                 m_s[warp][g + 8 * e] = m_run[e];
                 l_s[warp][g + 8 * e] = l_run[e];
             }
+            // (l is 2^14 or more: the division comes first, so that nothing leaves float32's range before the result does)
+            const float inv = l_run[e] != 0.f ? 1.f / l_run[e] : 0.f;
 #pragma unroll
             for (int t = 0; t < OT; ++t)
-                *reinterpret_cast<float2*>(&shared_o[(warp * EA_ROWS + g + 8 * e) * LD + 8 * t + 8 * (t / 4) + 2 * c]) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+                *reinterpret_cast<float2*>(&shared_o[(warp * EA_ROWS + g + 8 * e) * LD + 8 * t + 8 * (t / 4) + 2 * c]) =
+                    make_float2(scaled(o[t][2 * e] * inv, unit_run[e]), scaled(o[t][2 * e + 1] * inv, unit_run[e]));
         }
         __syncthreads();
         const int live_warps = min(EA_WARPS, p_end - p_begin);   // (the others have seen nothing)
         if (threadIdx.x < EA_ROWS) {
-            float m = EA_NONE, l = 0.f;
+            float m = EA_NONE, l = 0.f, part[EA_WARPS];
             for (int w = 0; w < live_warps; ++w) m = fmaxf(m, m_s[w][threadIdx.x]);
-            for (int w = 0; w < live_warps; ++w) {
-                const float f = fast_exp2(m_s[w][threadIdx.x] - m);
-                factor_s[w][threadIdx.x] = f;
-                l = fmaf(f, l_s[w][threadIdx.x], l);
+#pragma unroll
+            for (int w = 0; w < EA_WARPS; ++w) {
+                part[w] = w < live_warps ? fast_exp2(m_s[w][threadIdx.x] - m) * l_s[w][threadIdx.x] : 0.f;
+                l += part[w];
             }
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int w = 0; w < EA_WARPS; ++w) factor_s[w][threadIdx.x] = part[w] * inv;
             m_s[0][threadIdx.x] = m;
             total_s[threadIdx.x] = l;
         }
         __syncthreads();
-        const int first_block = pair_begin / target, runs = (pair_begin + r.pages - 1) / target - first_block + 1, run = (int)blockIdx.x - first_block;
+        const int first_block = (pair_begin + ahead) / target, runs = (pair_begin + ahead + r.pages - 1) / target - first_block + 1, run = (int)blockIdx.x - first_block;
         // where run k of this pair leaves its results: a block's first pair in the first of its two places
         auto place_of = [&](int k) { return 2 * (first_block + k) + (pair_begin > (first_block + k) * target ? 1 : 0); };
         // an item: four products' elements of one column and row, neighbours in the output
@@ -529,9 +617,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
             }
         };
         auto give_out = [&](const float (&v)[4], int row, int w, int n, int count) {
-            const float l = total_s[row], inv = l != 0.f ? 1.f / l : 0.f;
-            const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-            store4(out + row_at(row) + value_component<D>(4 * w, n), u, count);
+            store4(out + row_at(row) + value_component<D>(4 * w, n), v, count);
         };
         each_item([&](int i, int row, int w, int n, int count) {
             float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -549,18 +635,26 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
             // joins the results in `count` places (the k-th: place(k)): their sums in total_s, the output by `done`
             auto join = [&](int count, auto place, auto done) {
                 __threadfence();
-                if (threadIdx.x < EA_ROWS) {
-                    const int row = threadIdx.x;
-                    float m = EA_NONE, l = 0.f;
-                    for (int k = 0; k < count; ++k) m = fmaxf(m, __ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2));
-                    for (int k = 0; k < count; ++k) {
-                        const float f = fast_exp2(__ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2) - m);
-                        factor_s[k][row] = f;
-                        l = fmaf(f, __ldcg(a.part_ml + (place(k) * EA_ROWS + row) * 2 + 1), l);
-                    }
-                    m_s[0][row] = m;
-                    total_s[row] = l;
+                const int row = threadIdx.x / EA_SHARE, sub = threadIdx.x % EA_SHARE;   // EA_SHARE lanes a row
+                float2 x[EA_MOST_GROUPS / EA_SHARE];
+                float m = EA_NONE, l = 0.f;
+#pragma unroll
+                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i) {
+                    const int k = sub + i * EA_SHARE;
+                    x[i] = k < count && row < n_rows ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (place(k) * EA_ROWS + row) * 2)) : make_float2(EA_NONE, 0.f);
+                    m = fmaxf(m, x[i].x);
                 }
+#pragma unroll
+                for (int s = 1; s < EA_SHARE; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+#pragma unroll
+                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i) l += x[i].y = fast_exp2(x[i].x - m) * x[i].y;
+#pragma unroll
+                for (int s = 1; s < EA_SHARE; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i)
+                    if (sub + i * EA_SHARE < count) factor_s[sub + i * EA_SHARE][row] = x[i].y * inv;
+                if (sub == 0) m_s[0][row] = m, total_s[row] = l;
                 __syncthreads();
                 each_item([&](int i, int row, int w, int n, int items) {
                     float v[4] = {0.f, 0.f, 0.f, 0.f};
