@@ -9,16 +9,19 @@
 // for the running maximum m: rounded to float16 (2^-12 of each weight, less than the output's own rounding) where the output is bfloat16, two
 // numbers where it is float32. Maxima, sums and outputs are float32; for float32 outputs the tensor cores' sums end with a tile (they cut bits off).
 //
-// A block takes pages of a (sequence, kv head, 16 rows), its warps a page each in turn; a warp looks its next 32 pages and their scales up at once. A row is a query head of the kv head's
-// group and a token of the span; 16 of them are the rows of m16n8k16 products, whose columns are keys, then components. No shared memory
-// lies on the way of the codes: a lane loads what its fragments hold. For the keys, columns are 8 positions and a lane takes D / 4
-// components of one of them, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
+// A block takes pages of a (sequence, kv head, 8 or 16 rows), its warps a page each in turn; a warp looks its next 32 pages and their scales up
+// at once. A row is a query head of the kv head's group and a token of the span. Both products are taken with the cache on the left, whose
+// tiles are the tall side of m16n8k16: S^T = K Q^T (16 positions by 8 rows), O^T = V^T P^T (16 components by 8 rows), so that seven or eight heads
+// of a group fill a tile, where they would be half of one the other way round, with half the products, exponentials and sums to keep.
+// P^T comes out of the first with positions where the second wants rows: eight by eight, the warp transposes it (movmatrix).
+// No shared memory lies on the way of the codes: a lane loads what its fragments hold. For the keys a lane takes D / 4 components of one
+// position in eight, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
 // fragments go through the same). For the values a lane takes D / 8 neighbouring components of the four positions that a step wants
-// of it, and byte t of them is its element of the t-th product: a byte permutation puts two positions side by side for the conversion.
+// of it, and byte t of them is its element of component column t: a byte permutation puts two positions side by side for the conversion.
 // A tile's values are on their way while its scores are formed, the next tile's keys from then on.
 //
 // Work is shared out on the device, from the lengths (a captured graph replays this launch with others): all pages of all (sequence, kv head,
-// 16 rows) in a row, `target` of them to a block, so that one round of blocks does it all. Where every pair's pages can be rounded up to
+// rows) in a row, `target` of them to a block, so that one round of blocks does it all. Where every pair's pages can be rounded up to
 // whole blocks within that round, they are, and a block has one pair; else blocks begin and end anywhere, and lengths that
 // differ leave no SM idle. A pair of several blocks leaves partial results (maximum, sum, output); the block that ends last, by a
 // ticket, joins them in their order, sixteen at a time, and the last of those the sixteens.
@@ -30,7 +33,6 @@
 #include "e4m3.cuh"
 
 #define EA_WARPS 4
-#define EA_ROWS 16
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -42,6 +44,12 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// An 8 x 8 matrix of float16, a row's two neighbours to a lane, with rows and columns exchanged.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // what float16 leaves over of two numbers
 __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t taken) {
@@ -131,15 +139,16 @@ template <int D> __device__ __forceinline__ void load_value(uint32_t (&w)[Parts<
 }
 __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 
-template <typename T, int D> struct Shape {
+// NR: eights of rows of a block.
+template <typename T, int D, int NR> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
-    static constexpr int TILE = D <= 64 ? (TWO ? 32 : 64) : (TWO && D > 96 ? 16 : 32);   // positions of a step
-    static constexpr int BLOCKS = D <= 32 ? 3 : 2;                    // of an SM
-    // floats from a row to the next where warps leave their outputs: product t's column n at 8 t + 8 (t / 4) + n, so that four products of 32 lanes
-    // meet 32 banks; rows 8 or 24 banks apart, for the warps' own stores
-    static constexpr int ROW = D + 8 * ((D / 8 + 3) / 4), LD = ROW % 32 == 8 || ROW % 32 == 24 ? ROW : ROW + 8;
-    static constexpr int SMEM = EA_WARPS * EA_ROWS * LD * 4;
-    static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result
+    static constexpr int ROWS = 8 * NR;
+    static constexpr int TILE = D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
+    static constexpr int BLOCKS = NR > 1 ? 2 : 3;                     // of an SM
+    static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result: items of four
+    static constexpr int LD = PART + 4;                               // and where warps leave theirs: rows four banks apart
+    static constexpr int SMEM = EA_WARPS * ROWS * LD * 4;
+    static constexpr int SHARE = EA_WARPS * 32 / ROWS;                // lanes that join a row's maxima and sums
 };
 
 struct AttendArgs {
@@ -147,7 +156,7 @@ struct AttendArgs {
     E4m3Site site;
     int n_heads, n_seqs, single, chunks, most_pages, block_slots, window;
     float scale_log2;
-    float *part_o, *part_ml;   // [2 * blocks][16][PART], [2 * blocks][16][2]
+    float *part_o, *part_ml;   // [2 * blocks][ROWS][PART], [2 * blocks][ROWS][2]
     int *tickets, *err;        // [4 * blocks]
 };
 
@@ -181,43 +190,115 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     }
 }
 
-// x * 2^e, e of any size that the result has room for
-__device__ __forceinline__ float scaled(float x, int e) { return x * pow2(e / 2) * pow2(e - e / 2); }
-
 #define EA_PAIR_COST 8     // pages whose time a pair's beginning and end take
 #define EA_GROUP 16        // partial results that a block joins at once
-#define EA_SHARE (EA_WARPS * 32 / EA_ROWS)
 #define EA_MOST_GROUPS 64  // ... and groups of them: enough for 1,024 blocks
 
-template <typename T, int D>
-__global__ void __launch_bounds__(EA_WARPS * 32, Shape<T, D>::BLOCKS)
-attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArgs a) {
-    using S = Shape<T, D>;
+// Where the results of a pair that begins at pair_begin lie that block `block` leaves: a block's first pair has the first of its two places.
+__device__ __forceinline__ int place_in(int pair_begin, int block, int target) { return 2 * block + (pair_begin > block * target ? 1 : 0); }
+// Element 0 of the query (and output) of row i (token * group + head of the group) of the kv head kvh.
+template <int D> __device__ __forceinline__ long long row_offset(const AttendArgs& a, int begin, int kvh, int i) {
+    const int G = a.n_heads / a.site.kv_heads, token = a.single ? 0 : i / G;
+    return (long long)(begin + token) * a.n_heads * D + (long long)(kvh * G + i - token * G) * D;
+}
+// Item i of a row, four neighbouring components (two of a part of 16), to its row of the output.
+template <typename T, int D> __device__ __forceinline__ void give_out(T* row, const float4& v, int i) {
+    const float u[4] = {v.x, v.y, v.z, v.w};
+    store4(row + value_component<D>(i / 8 * 4, i % 8), u, Parts<D>::v16 != 0 && i / 8 == Parts<D>::v_words - 1 ? 2 : 4);
+}
+
+struct Pair {
+    int begin, first_block, runs, n_rows, row0, kvh, token0;
+};
+// Joins the results of `count` runs of a pair, run0, run0 + apart, ..., in this order: to the output, or, home >= 0, to the place `home` as one more result.
+template <typename T, int D, int NR>
+__device__ __forceinline__ void join_parts(T* out, const AttendArgs& a, const Pair& pair, int target, int run0, int apart, int count, int home, float* factor_s) {
+    using S = Shape<T, D, NR>;
+    constexpr int VW = Parts<D>::v_words, PART = S::PART, ROWS = S::ROWS, THREADS = EA_WARPS * 32, EACH = EA_MOST_GROUPS / S::SHARE;
+    auto place = [&](int k) { return place_in(pair.begin, pair.first_block + run0 + k * apart, target); };
+    auto part_of = [&](int k, int i) { return __ldcg(reinterpret_cast<const float4*>(a.part_o + (long long)place(k) * ROWS * PART + i * 4)); };
+    const int items = pair.n_rows * VW * 8;
+    float4 ready[EA_GROUP];   // the first sixteen parts of this thread's first item, on their way beside the statistics
+#pragma unroll
+    for (int k = 0; k < EA_GROUP; ++k)
+        if (k < count && (int)threadIdx.x < items) ready[k] = part_of(k, threadIdx.x);
+    const int row = threadIdx.x / S::SHARE, sub = threadIdx.x % S::SHARE;
+    float2 x[EACH];
+    float m = EA_NONE, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int k = sub + i * S::SHARE;
+        x[i] = k < count && row < pair.n_rows ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (place(k) * ROWS + row) * 2)) : make_float2(EA_NONE, 0.f);
+        m = fmaxf(m, x[i].x);
+    }
+#pragma unroll
+    for (int i = 1; i < S::SHARE; i <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) l += x[i].y = fast_exp2(x[i].x - m) * x[i].y;
+#pragma unroll
+    for (int i = 1; i < S::SHARE; i <<= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (sub + i * S::SHARE < count) factor_s[(sub + i * S::SHARE) * ROWS + row] = x[i].y * inv;
+    __syncthreads();   // (every result's maximum and sum have been read, and its factor is there)
+    if (home >= 0 && sub == 0 && row < pair.n_rows) *reinterpret_cast<float2*>(a.part_ml + (home * ROWS + row) * 2) = make_float2(m, l);
+    for (int i = threadIdx.x; i < items; i += THREADS) {
+        const int at_row = i / (VW * 8);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < count; k0 += EA_GROUP) {
+            if (k0 > 0 || i >= THREADS) {
+#pragma unroll
+                for (int k = 0; k < EA_GROUP; ++k)
+                    if (k0 + k < count) ready[k] = part_of(k0 + k, i);
+            }
+#pragma unroll
+            for (int k = 0; k < EA_GROUP; ++k)
+                if (k0 + k < count) {
+                    const float f = factor_s[(k0 + k) * ROWS + at_row];
+                    v.x = fmaf(f, ready[k].x, v.x), v.y = fmaf(f, ready[k].y, v.y), v.z = fmaf(f, ready[k].z, v.z), v.w = fmaf(f, ready[k].w, v.w);
+                }
+        }
+        if (home >= 0) *reinterpret_cast<float4*>(a.part_o + (long long)home * ROWS * PART + i * 4) = v;
+        else give_out<T, D>(out + row_offset<D>(a, pair.token0, pair.kvh, pair.row0 + at_row), v, i % (VW * 8));
+    }
+}
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(EA_WARPS * 32, Shape<T, D, NR>::BLOCKS)
+attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ AttendArgs a) {
+    using S = Shape<T, D, NR>;
     using P = Parts<D>;
     constexpr bool TWO = S::TWO;
-    constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, OT = D / 8, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART;
-    constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32;
+    constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, DT = D / 16, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS;
+    constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32, TERMS = TWO ? 2 : 1;
     grid_chain_entry();
-    extern __shared__ float shared_o[];   // [warps][rows][LD]
-    __shared__ float m_s[EA_WARPS][EA_ROWS], l_s[EA_WARPS][EA_ROWS], total_s[EA_ROWS], factor_s[EA_MOST_GROUPS][EA_ROWS];
+    extern __shared__ __align__(16) float shared_o[];   // [warps][rows][LD]
+    __shared__ float m_s[EA_WARPS][ROWS], l_s[EA_WARPS][ROWS], factor_s[EA_MOST_GROUPS * ROWS];
     __shared__ int ticket_s;
+    __shared__ Pair left_s[2];
+    int n_left = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const E4m3Site& site = a.site;
     const int KVH = site.kv_heads, G = a.n_heads / KVH, pairs_each = KVH * a.chunks;
     const int q_width = a.n_heads * D, n_blocks = gridDim.x;
 
-    // ---- this block's share (every warp works it out for itself)
+    // ---- this block's share (every warp works it out for itself; a lane keeps its one of the first 32 sequences)
+    Sequence first;
+    first.pages = 0;
+    if (lane < a.n_seqs) first = sequence_of(a, lane);
+    auto pages_of = [&](int s0) { return s0 == 0 ? first.pages : s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0; };
     int total = 0, pairs = 0, whole = 0, target = EA_WARPS;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const int pages = s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0;
+        const int pages = pages_of(s0);
         total += pages;
         pairs += pages > 0;
     }
-    total = (int)warp_sum_u32((uint32_t)total) * pairs_each;
-    pairs = (int)warp_sum_u32((uint32_t)pairs) * pairs_each;
-    target = max(target, (total + a.block_slots - 1) / a.block_slots);
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) whole += s0 + lane < a.n_seqs ? (sequence_of(a, s0 + lane).pages + target - 1) / target : 0;
-    whole = (int)warp_sum_u32((uint32_t)whole) * pairs_each;
+    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total) * pairs_each;
+    pairs = (int)__reduce_add_sync(0xffffffffu, (unsigned)pairs) * pairs_each;
+    if (total > target * a.block_slots) target = (total + a.block_slots - 1) / a.block_slots;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) whole += (pages_of(s0) + target - 1) / target;
+    whole = (int)__reduce_add_sync(0xffffffffu, (unsigned)whole) * pairs_each;
     // pages of a pair are rounded up to whole units; where blocks may have several pairs, each counts EA_PAIR_COST pages more
     const bool aligned = whole <= a.block_slots;
     const int ahead = aligned ? 0 : EA_PAIR_COST;
@@ -228,35 +309,38 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
         target = max(target, (total + a.block_slots - 1) / a.block_slots);
     }
     auto places_of = [&](int pages) { return pages == 0 ? 0 : aligned ? (pages + target - 1) / target * target : pages + ahead; };
-    // padding entries: zeros
-    for (int s = blockIdx.x; s < a.n_seqs; s += n_blocks) {
-        const Sequence r = sequence_of(a, s);
-        if (r.slot < 0)
-            for (int i = threadIdx.x; i < r.tokens * q_width; i += THREADS) out[(long long)r.begin * q_width + i] = Num<T>::from_f(0.f);
-    }
     const int range_begin = blockIdx.x * target, range_end = min(range_begin + target, total);
-    if (range_begin >= range_end) return;
     // the sequence in whose pages it begins
     int seq = 0, base = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const int mine = s0 + lane < a.n_seqs ? places_of(sequence_of(a, s0 + lane).pages) * pairs_each : 0;
-        int upto = mine;
+    Sequence r = first;
+    if (range_begin < range_end) {
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const int mine = places_of(pages_of(s0)) * pairs_each;
+            int upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > range_begin);
+            if (beyond) {
+                const int who = __ffs(beyond) - 1;
+                seq = s0 + who;
+                base += __shfl_sync(0xffffffffu, upto - mine, who);
+                if (s0 == 0) {
+                    r.slot = __shfl_sync(0xffffffffu, first.slot, who), r.begin = __shfl_sync(0xffffffffu, first.begin, who);
+                    r.tokens = __shfl_sync(0xffffffffu, first.tokens, who), r.first_pos = __shfl_sync(0xffffffffu, first.first_pos, who);
+                    r.last_pos = __shfl_sync(0xffffffffu, first.last_pos, who), r.page0 = __shfl_sync(0xffffffffu, first.page0, who);
+                    r.pages = __shfl_sync(0xffffffffu, first.pages, who);
+                } else {
+                    r = sequence_of(a, seq);
+                }
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > range_begin);
-        if (beyond) {
-            const int who = __ffs(beyond) - 1;
-            seq = s0 + who;
-            base += __shfl_sync(0xffffffffu, upto - mine, who);
-            break;
-        }
-        base += __shfl_sync(0xffffffffu, upto, 31);
     }
 
-    Sequence r = sequence_of(a, seq);
     int padded = places_of(r.pages);
     for (int at = range_begin; at < range_end;) {
         while (at >= base + padded * pairs_each) {   // (sequences without pages are passed over)
@@ -269,25 +353,23 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
         const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin;
         at = min(pair_begin + padded, range_end);
         if (reports && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
-        const int row0 = chunk * EA_ROWS, n_rows = min(EA_ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
+        const int row0 = chunk * ROWS, n_rows = min(ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
         if (n_rows <= 0 || p_begin >= p_end) continue;
-        // element 0 of a row's query (and output)
-        auto row_at = [&](int row) -> long long {
-            const int i = row0 + row;
-            return (long long)(r.begin + i / G) * q_width + (long long)(kvh * G + i % G) * D;
-        };
+        auto row_at = [&](int row) { return row_offset<D>(a, r.begin, kvh, row0 + row); };
         const int my_pages = p_begin + warp < p_end ? (p_end - p_begin - warp + EA_WARPS - 1) / EA_WARPS : 0;
-        // what the rows see, lo .. hi - 1: this lane's two, all of them together, every one of them
-        const int t_first = row0 / G, t_last = (row0 + n_rows - 1) / G;
+        // what the rows see, lo .. hi - 1: this lane's (8 n + 2 c and + 1), all of them together, every one of them
+        const int t_first = a.single ? 0 : row0 / G, t_last = a.single ? 0 : (row0 + n_rows - 1) / G;
         const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (a.single ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
         const int some_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, all_lo = a.window > 0 ? max(0, some_hi - a.window) : 0;
-        int lo[2], hi[2];
+        int lo[NR][2], hi[NR][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int row = g + 8 * e;
-            hi[e] = row >= n_rows ? 0 : t_first == t_last ? first_hi : a.tok_pos[r.begin + (row0 + row) / G] + 1;
-            lo[e] = a.window > 0 ? max(0, hi[e] - a.window) : 0;
-        }
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * n + 2 * c + e;
+                hi[n][e] = row >= n_rows ? 0 : t_first == t_last ? first_hi : a.tok_pos[r.begin + (row0 + row) / G] + 1;
+                lo[n][e] = a.window > 0 ? max(0, hi[n][e] - a.window) : 0;
+            }
 
         // ---- keys of a step: pages p_begin + warp, + EA_WARPS, ..., a tile of one at a time
         const int steps = my_pages * PER_PAGE;
@@ -327,54 +409,57 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
         };
         if (steps > 0) load_keys(0);
 
-        // ---- the queries' fragments
-        uint32_t qa[TWO ? 2 : 1][KW][4];
-        float by[2];   // scores of a row in base-2 units: product * key scale * by
-        {
-            float2 x[2][KW][2];
-            float top[2] = {0.f, 0.f};
+        // ---- the queries' fragments: lane (g, c) has row g's components of its column
+        uint32_t qb[TERMS][NR][KW][2];
+        float by[NR][2];   // scores of rows 8 n + 2 c + e in base-2 units: product * key scale * by
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = g + 8 * e;
-                const T* src = q + (row < n_rows ? row_at(row) : 0);
+        for (int n = 0; n < NR; ++n) {
+            float2 x[KW][2];
+            float top = 0.f;
+            const int row = 8 * n + g;
+            const T* src = q + (row < n_rows ? row_at(row) : 0);
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    const int d = key_component<D>(w, c);
-                    x[e][w][0] = x[e][w][1] = make_float2(0.f, 0.f);
-                    if (row < n_rows) {
-                        if constexpr (TWO) {
-                            const float4 v = *reinterpret_cast<const float4*>(src + d);
-                            x[e][w][0] = make_float2(v.x, v.y), x[e][w][1] = make_float2(v.z, v.w);
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(src + d);
-                            x[e][w][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
-                            x[e][w][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
-                        }
+            for (int w = 0; w < KW; ++w) {
+                const int d = key_component<D>(w, c);
+                x[w][0] = x[w][1] = make_float2(0.f, 0.f);
+                if (row < n_rows) {
+                    if constexpr (TWO) {
+                        const float4 v = *reinterpret_cast<const float4*>(src + d);
+                        x[w][0] = make_float2(v.x, v.y), x[w][1] = make_float2(v.z, v.w);
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(src + d);
+                        x[w][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
+                        x[w][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) top[e] = fmaxf(top[e], fmaxf(fabsf(x[e][w][i].x), fabsf(x[e][w][i].y)));
                 }
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-                const int up = min(max(exponent_of(top[e]) - 7, -119), 120);
-                by[e] = pow2(up) * fabsf(a.scale_log2);
-                const float down = copysignf(pow2(-up), a.scale_log2);
 #pragma unroll
-                for (int w = 0; w < KW; ++w)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float u = x[e][w][i].x * down, v = x[e][w][i].y * down;
-                        qa[0][w][2 * i + e] = pack_half(u, v);
-                        if constexpr (TWO) qa[1][w][2 * i + e] = pack_rest(u, v, qa[0][w][2 * i + e]);
-                    }
+                for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(x[w][i].x), fabsf(x[w][i].y)));
             }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = min(max(exponent_of(top) - 7, -119), 120);
+            const float mine = pow2(up) * fabsf(a.scale_log2), down = copysignf(pow2(-up), a.scale_log2);
+            by[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
+            by[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+#pragma unroll
+            for (int w = 0; w < KW; ++w)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float u = x[w][i].x * down, v = x[w][i].y * down;
+                    qb[0][n][w][i] = pack_half(u, v);
+                    if constexpr (TWO) qb[TERMS - 1][n][w][i] = pack_rest(u, v, qb[0][n][w][i]);
+                }
         }
 
-        float o[OT][4];
+        float o[DT][NR][4];   // components of columns 2 d (0, 1) and 2 d + 1 (2, 3) by rows 2 c, 2 c + 1
 #pragma unroll
-        for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m_run[2] = {EA_NONE, EA_NONE}, l_run[2] = {0.f, 0.f};   // (l: this lane's columns only)
-        int unit_run[2] = {0, 0};                                      // o stands for o * 2^unit_run
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.f;
+        float m_run[NR][2], l_run[NR][2];   // (l: this lane's positions only)
+        int unit_run[NR][2];                // o stands for o * 2^unit_run
+#pragma unroll
+        for (int n = 0; n < NR; ++n) m_run[n][0] = m_run[n][1] = EA_NONE, l_run[n][0] = l_run[n][1] = 0.f, unit_run[n][0] = unit_run[n][1] = 0;
         bool begun = false;
 
         for (int step = 0; step < steps; ++step) {
@@ -384,8 +469,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                 if (step + 1 < steps) load_keys(step + 1);
                 continue;
             }
-            if (!begun) unit_run[0] = unit_run[1] = unit_v;
-            begun = true;
+            if (!begun) {
+#pragma unroll
+                for (int n = 0; n < NR; ++n) unit_run[n][0] = unit_run[n][1] = unit_v;
+                begun = true;
+            }
             // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
             uint32_t vw[KT][4][VW];
             {
@@ -400,357 +488,354 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const AttendArg
                     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int at = 16 * kt + (i & 1) + 8 * (i >> 1), key = key0 + at + 2 * c;
+                            const int at_key = 16 * kt + (i & 1) + 8 * (i >> 1), key = key0 + at_key + 2 * c;
 #pragma unroll
                             for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies elsewhere is nobody's, NaN perhaps)
-                            if (key >= some_lo && key < some_hi) load_value<D>(vw[kt][i], v + at * D, g);
+                            if (key >= some_lo && key < some_hi) load_value<D>(vw[kt][i], v + at_key * D, g);
                         }
                 }
             }
-            // ---- scores
-            float s[NT][4];
+            // ---- scores: positions 16 t + g (0, 1) and 16 t + 8 + g (2, 3) by rows 2 c, 2 c + 1
+            float s[KT][NR][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int n = 0; n < NR; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
 #pragma unroll
             for (int w = 0; w < KW; ++w)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint32_t b0 = half2_of_low(kw[t][w]), b1 = half2_of_high(kw[t][w]);
-                    if constexpr (TWO) mma_f16_16816(s[t], qa[1][w], b0, b1);
-                    mma_f16_16816(s[t], qa[0][w], b0, b1);
+                for (int t = 0; t < KT; ++t) {
+                    const uint32_t x = kw[2 * t][w], z = kw[2 * t + 1][w], k[4] = {half2_of_low(x), half2_of_low(z), half2_of_high(x), half2_of_high(z)};
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        if constexpr (TWO) mma_f16_16816(s[t][n], k, qb[TERMS - 1][n][w][0], qb[TERMS - 1][n][w][1]);
+                        mma_f16_16816(s[t][n], k, qb[0][n][w][0], qb[0][n][w][1]);
+                    }
                 }
             if (step + 1 < steps) load_keys(step + 1);
             // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none
-            const float by_k[2] = {by[0] * ks, by[1] * ks};
             const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
-            auto seen = [&](int t, int e) {
-                const int key = key0 + 8 * t + 2 * c + (e & 1);
-                return key >= lo[e >> 1] && key < hi[e >> 1];
+            auto seen = [&](int t, int n, int e) {
+                const int key = key0 + 16 * t + 8 * (e >> 1) + g;
+                return key >= lo[n][e & 1] && key < hi[n][e & 1];
             };
-            float top[2] = {EA_NONE, EA_NONE}, corr[2], shift[2];
-            if (full) {
+            float corr[NR][2], m_tile[NR][2];
+            uint32_t pb[TERMS][KT][NR][2];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int n = 0; n < NR; ++n) {
+                float top[2] = {EA_NONE, EA_NONE}, shift[2], by_k[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
-            } else {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < KT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (seen(t, e)) top[e >> 1] = fmaxf(top[e >> 1], s[t][e]);
-            }
-            float m_tile[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-                m_tile[e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
-                const float m = fmaxf(m_run[e], m_tile[e]);
-                corr[e] = fast_exp2(m_run[e] - m);
-                m_run[e] = m;
-                shift[e] = 14.f - m;
-                l_run[e] *= corr[e];
-            }
-            uint32_t pa[TWO ? 2 : 1][KT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[t][e] = fast_exp2(fmaf(s[t][e], by_k[e >> 1], shift[e >> 1]));
-                    if (!full && !seen(t, e)) s[t][e] = 0.f;
-                    l_run[e >> 1] += s[t][e];
-                }
+                        if (full || seen(t, n, e)) top[e & 1] = fmaxf(top[e & 1], s[t][n][e]);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    pa[0][t / 2][2 * (t % 2) + e] = pack_half(s[t][2 * e], s[t][2 * e + 1]);
-                    if constexpr (TWO) pa[1][t / 2][2 * (t % 2) + e] = pack_rest(s[t][2 * e], s[t][2 * e + 1], pa[0][t / 2][2 * (t % 2) + e]);
+                    by_k[e] = by[n][e] * ks;
+#pragma unroll
+                    for (int i = 4; i < 32; i <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], i));
+                    m_tile[n][e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
+                    const float m = fmaxf(m_run[n][e], m_tile[n][e]);
+                    corr[n][e] = fast_exp2(m_run[n][e] - m);
+                    m_run[n][e] = m;
+                    shift[e] = 14.f - m;
+                    l_run[n][e] *= corr[n][e];
+                }
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    float(&x)[4] = s[t][n];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = fast_exp2(fmaf(x[e], by_k[e & 1], shift[e & 1]));
+                        if (!full && !seen(t, n, e)) x[e] = 0.f;
+                        l_run[n][e & 1] += x[e];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t most = pack_half(x[2 * h], x[2 * h + 1]);
+                        pb[0][t][n][h] = transposed(most);
+                        if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
+                    }
                 }
             }
-            // ---- values. Word w of the four positions of a step holds their elements of the products 4 w .. 4 w + 3
+            // ---- values. Word w of the four positions of a step holds their elements of the component columns 4 w .. 4 w + 3
             auto word_products = [&](int kt, int w, auto take, auto add) {
                 uint32_t x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = take(vw[kt][i][w], 16 * kt + 2 * c + (i & 1) + 8 * (i >> 1));
-                const uint32_t u[2] = {__byte_perm(x[0], x[1], 0x5140), __byte_perm(x[0], x[1], 0x7362)};
-                const uint32_t v[2] = {__byte_perm(x[2], x[3], 0x5140), __byte_perm(x[2], x[3], 0x7362)};
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
-                    add(t, t & 1 ? half2_of_high(u[t / 2]) : half2_of_low(u[t / 2]), t & 1 ? half2_of_high(v[t / 2]) : half2_of_low(v[t / 2]));
+                for (int d = 0; d < 2; ++d) {
+                    if (P::v16 != 0 && w == VW - 1 && d >= 1) break;
+                    const uint32_t u = __byte_perm(x[0], x[1], d ? 0x7362 : 0x5140), v = __byte_perm(x[2], x[3], d ? 0x7362 : 0x5140);
+                    const uint32_t f[4] = {half2_of_low(u), half2_of_high(u), half2_of_low(v), half2_of_high(v)};
+                    add(2 * w + d, f);
                 }
             };
-            bool apart = false;
+            bool far = false;   // an output is within 2^40 units (2^14 weights, 448, some thousand pages): there is room for 2^30 more
+            int up[NR][2];
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    up[n][e] = unit_run[n][e] - unit_v;
+                    far |= abs(up[n][e]) > 30;
+                }
             if (!full && t_first != t_last) {   // a NaN that some of the rows do not see must not reach them: 0 * NaN
-                bool nan = false;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) nan |= holds_nan(vw[kt][i][w]);
-                apart = nan;
+                        for (int w = 0; w < VW; ++w) far |= holds_nan(vw[kt][i][w]);
             }
-            const int up0 = unit_run[0] - unit_v, up1 = unit_run[1] - unit_v;
-            const bool far = apart || abs(up0) > 30 || abs(up1) > 30;   // (an output is within 2^40 units: 2^14 weights, 448, some thousand pages)
             if (!__any_sync(0xffffffffu, far)) {
-                const float f0 = corr[0] * pow2(up0), f1 = corr[1] * pow2(up1);
-                unit_run[0] = unit_run[1] = unit_v;
+                float f[NR][2];
+                bool moved = false;
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        f[n][e] = corr[n][e] * pow2(up[n][e]);
+                        moved |= f[n][e] != 1.f;
+                        unit_run[n][e] = unit_v;
+                    }
                 if constexpr (TWO) {
 #pragma unroll
                     for (int w = 0; w < VW; ++w) {
-                        float acc[4][4];
+                        float acc[2][NR][4];
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+                        for (int d = 0; d < 2; ++d)
+#pragma unroll
+                            for (int n = 0; n < NR; ++n) acc[d][n][0] = acc[d][n][1] = acc[d][n][2] = acc[d][n][3] = 0.f;
 #pragma unroll
                         for (int kt = 0; kt < KT; ++kt)
-                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int t, uint32_t b0, uint32_t b1) {
-                                mma_f16_16816(acc[t], pa[1][kt], b0, b1);
-                                mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int d, const uint32_t(&v)[4]) {
+#pragma unroll
+                                for (int n = 0; n < NR; ++n) {
+                                    mma_f16_16816(acc[d & 1][n], v, pb[TERMS - 1][kt][n][0], pb[TERMS - 1][kt][n][1]);
+                                    mma_f16_16816(acc[d & 1][n], v, pb[0][kt][n][0], pb[0][kt][n][1]);
+                                }
                             });
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
-                            float(&x)[4] = o[4 * w + t];
-                            x[0] = fmaf(x[0], f0, acc[t][0]), x[1] = fmaf(x[1], f0, acc[t][1]), x[2] = fmaf(x[2], f1, acc[t][2]), x[3] = fmaf(x[3], f1, acc[t][3]);
+                        for (int d = 0; d < 2; ++d) {
+                            if (P::v16 != 0 && w == VW - 1 && d >= 1) break;
+#pragma unroll
+                            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[2 * w + d][n][e] = fmaf(o[2 * w + d][n][e], f[n][e & 1], acc[d][n][e]);
                         }
                     }
                 } else {
-                    if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
+                    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                        for (int t = 0; t < OT; ++t) o[t][0] *= f0, o[t][1] *= f0, o[t][2] *= f1, o[t][3] *= f1;
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[d][n][e] *= f[n][e & 1];
                     }
 #pragma unroll
                     for (int w = 0; w < VW; ++w)
 #pragma unroll
                         for (int kt = 0; kt < KT; ++kt)
-                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int t, uint32_t b0, uint32_t b1) { mma_f16_16816(o[4 * w + t], pa[0][kt], b0, b1); });
+                            word_products(kt, w, [](uint32_t x, int) { return x; }, [&](int d, const uint32_t(&v)[4]) {
+#pragma unroll
+                                for (int n = 0; n < NR; ++n) mma_f16_16816(o[d][n], v, pb[0][kt][n][0], pb[0][kt][n][1]);
+                            });
                 }
             } else {
                 // scales far apart, or a NaN: a unit in which what was there (2^had at most) and what comes (2^comes) both have room, and token by
                 // token, each with the positions that it sees
-                int shift_old[2], shift_new[2];
+                int shift_new[NR][2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float most = 0.f;
+                for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int t = 0; t < OT; ++t) most = fmaxf(most, fmaxf(fabsf(o[t][2 * e]), fabsf(o[t][2 * e + 1])));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)) * corr[e];
-                    const int had = most > 0.f ? unit_run[e] + exponent_of(most) : -1000;
-                    const int comes = unit_v + 30 + (int)fmaxf(m_tile[e] - m_run[e], -800.f);
-                    const int unit_both = max(max(had, comes) - 30, -150);
-                    shift_old[e] = unit_run[e] - unit_both, shift_new[e] = unit_v - unit_both;
-                    unit_run[e] = unit_both;
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        float most = 0.f;
 #pragma unroll
-                for (int t = 0; t < OT; ++t)
+                        for (int d = 0; d < DT; ++d) most = fmaxf(most, fmaxf(fabsf(o[d][n][e]), fabsf(o[d][n][2 + e])));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[t][e] = ldexpf(o[t][e] * corr[e >> 1], shift_old[e >> 1]);
+                        for (int i = 4; i < 32; i <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
+                        most *= corr[n][e];
+                        const int had = most > 0.f ? unit_run[n][e] + exponent_of(most) : -1000;
+                        const int comes = unit_v + 30 + (int)fmaxf(m_tile[n][e] - m_run[n][e], -800.f);
+                        const int unit_both = max(max(had, comes) - 30, -150);
+                        shift_new[n][e] = unit_v - unit_both;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) o[d][n][2 * h + e] = ldexpf(o[d][n][2 * h + e] * corr[n][e], unit_run[n][e] - unit_both);
+                        unit_run[n][e] = unit_both;
+                    }
                 for (int token = t_first; token <= t_last; ++token) {
                     const int upto = t_first == t_last ? first_hi : a.tok_pos[r.begin + token] + 1, from = a.window > 0 ? upto - a.window : 0;
-                    const bool mine[2] = {(row0 + g) / G == token, (row0 + g + 8) / G == token};
 #pragma unroll
                     for (int w = 0; w < VW; ++w) {
-                        float acc[4][4];
+                        float acc[2][NR][4];
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+                        for (int d = 0; d < 2; ++d)
+#pragma unroll
+                            for (int n = 0; n < NR; ++n) acc[d][n][0] = acc[d][n][1] = acc[d][n][2] = acc[d][n][3] = 0.f;
 #pragma unroll
                         for (int kt = 0; kt < KT; ++kt)
-                            word_products(kt, w, [&](uint32_t x, int at) { return key0 + at >= from && key0 + at < upto ? x : 0u; }, [&](int t, uint32_t b0, uint32_t b1) {
-                                if constexpr (TWO) mma_f16_16816(acc[t], pa[1][kt], b0, b1);
-                                mma_f16_16816(acc[t], pa[0][kt], b0, b1);
+                            word_products(kt, w, [&](uint32_t x, int at_key) { return key0 + at_key >= from && key0 + at_key < upto ? x : 0u; }, [&](int d, const uint32_t(&v)[4]) {
+#pragma unroll
+                                for (int n = 0; n < NR; ++n) {
+                                    if constexpr (TWO) mma_f16_16816(acc[d & 1][n], v, pb[TERMS - 1][kt][n][0], pb[TERMS - 1][kt][n][1]);
+                                    mma_f16_16816(acc[d & 1][n], v, pb[0][kt][n][0], pb[0][kt][n][1]);
+                                }
                             });
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            if (P::v16 != 0 && w == VW - 1 && t >= 2) break;
+                        for (int d = 0; d < 2; ++d) {
+                            if (P::v16 != 0 && w == VW - 1 && d >= 1) break;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (mine[e >> 1]) o[4 * w + t][e] += ldexpf(acc[t][e], shift_new[e >> 1]);
+                            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if ((row0 + 8 * n + 2 * c + (e & 1)) / G == token) o[2 * w + d][n][e] += ldexpf(acc[d][n][e], shift_new[n][e & 1]);
                         }
                     }
                 }
             }
         }
 
-        // ---- the warps' results together: the outputs of each alone, under shares of the whole weight
+        // ---- the warps' results together: the outputs of each alone, under shares of the whole weight. An item is four neighbouring components of a row
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
-            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
-            if (c == 0) {
-                m_s[warp][g + 8 * e] = m_run[e];
-                l_s[warp][g + 8 * e] = l_run[e];
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * n + 2 * c + e;
+#pragma unroll
+                for (int i = 4; i < 32; i <<= 1) l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], i);
+                if (g == 0) m_s[warp][row] = m_run[n][e], l_s[warp][row] = l_run[n][e];
+                // (l is 2^14 or more: the division comes first, so that nothing leaves float32's range before the result does)
+                const float inv = l_run[n][e] != 0.f ? 1.f / l_run[n][e] : 0.f;
+                const float u1 = pow2(unit_run[n][e] / 2), u2 = pow2(unit_run[n][e] - unit_run[n][e] / 2);
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    auto value = [&](int d, int h) { return d < DT ? o[d][n][2 * h + e] * inv * u1 * u2 : 0.f; };
+                    *reinterpret_cast<float4*>(&shared_o[(warp * ROWS + row) * LD + (w * 8 + g) * 4]) =
+                        make_float4(value(2 * w, 0), value(2 * w, 1), value(2 * w + 1, 0), value(2 * w + 1, 1));
+                }
             }
-            // (l is 2^14 or more: the division comes first, so that nothing leaves float32's range before the result does)
-            const float inv = l_run[e] != 0.f ? 1.f / l_run[e] : 0.f;
-#pragma unroll
-            for (int t = 0; t < OT; ++t)
-                *reinterpret_cast<float2*>(&shared_o[(warp * EA_ROWS + g + 8 * e) * LD + 8 * t + 8 * (t / 4) + 2 * c]) =
-                    make_float2(scaled(o[t][2 * e] * inv, unit_run[e]), scaled(o[t][2 * e + 1] * inv, unit_run[e]));
-        }
-        __syncthreads();
-        const int live_warps = min(EA_WARPS, p_end - p_begin);   // (the others have seen nothing)
-        if (threadIdx.x < EA_ROWS) {
-            float m = EA_NONE, l = 0.f, part[EA_WARPS];
-            for (int w = 0; w < live_warps; ++w) m = fmaxf(m, m_s[w][threadIdx.x]);
-#pragma unroll
-            for (int w = 0; w < EA_WARPS; ++w) {
-                part[w] = w < live_warps ? fast_exp2(m_s[w][threadIdx.x] - m) * l_s[w][threadIdx.x] : 0.f;
-                l += part[w];
-            }
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll
-            for (int w = 0; w < EA_WARPS; ++w) factor_s[w][threadIdx.x] = part[w] * inv;
-            m_s[0][threadIdx.x] = m;
-            total_s[threadIdx.x] = l;
-        }
         __syncthreads();
         const int first_block = (pair_begin + ahead) / target, runs = (pair_begin + ahead + r.pages - 1) / target - first_block + 1, run = (int)blockIdx.x - first_block;
         // where run k of this pair leaves its results: a block's first pair in the first of its two places
-        auto place_of = [&](int k) { return 2 * (first_block + k) + (pair_begin > (first_block + k) * target ? 1 : 0); };
-        // an item: four products' elements of one column and row, neighbours in the output
-        auto each_item = [&](auto work) {
-            for (int i = threadIdx.x; i < n_rows * VW * 8; i += THREADS) {
-                const int row = i / (VW * 8), w = i / 8 % VW, n = i % 8;
-                work(i, row, w, n, P::v16 != 0 && w == VW - 1 ? 2 : 4);
+        auto place_of = [&](int k) { return place_in(pair_begin, first_block + k, target); };
+        const int items = n_rows * VW * 8;
+        for (int i = threadIdx.x; i < items; i += THREADS) {
+            const int row = i / (VW * 8);
+            float m = EA_NONE, l = 0.f, part[EA_WARPS];
+#pragma unroll
+            for (int k = 0; k < EA_WARPS; ++k) m = fmaxf(m, m_s[k][row]);
+#pragma unroll
+            for (int k = 0; k < EA_WARPS; ++k) l += part[k] = fast_exp2(m_s[k][row] - m) * l_s[k][row];   // (a warp without pages: nothing)
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < EA_WARPS; ++k) {
+                const float f = part[k] * inv;
+                const float4 x = *reinterpret_cast<const float4*>(&shared_o[(k * ROWS + row) * LD + i % (VW * 8) * 4]);
+                v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
             }
-        };
-        auto give_out = [&](const float (&v)[4], int row, int w, int n, int count) {
-            store4(out + row_at(row) + value_component<D>(4 * w, n), v, count);
-        };
-        each_item([&](int i, int row, int w, int n, int count) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < live_warps; ++k) {
-                const float f = factor_s[k][row];
-                const float* from = shared_o + (k * EA_ROWS + row) * LD + 40 * w + n;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < count) v[j] = fmaf(f, from[8 * j], v[j]);
-            }
-            if (runs == 1) give_out(v, row, w, n, count);
-            else *reinterpret_cast<float4*>(a.part_o + (long long)place_of(run) * EA_ROWS * PART + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
-        });
-        if (runs > 1) {
-            // joins the results in `count` places (the k-th: place(k)): their sums in total_s, the output by `done`
-            auto join = [&](int count, auto place, auto done) {
-                __threadfence();
-                const int row = threadIdx.x / EA_SHARE, sub = threadIdx.x % EA_SHARE;   // EA_SHARE lanes a row
-                float2 x[EA_MOST_GROUPS / EA_SHARE];
-                float m = EA_NONE, l = 0.f;
-#pragma unroll
-                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i) {
-                    const int k = sub + i * EA_SHARE;
-                    x[i] = k < count && row < n_rows ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (place(k) * EA_ROWS + row) * 2)) : make_float2(EA_NONE, 0.f);
-                    m = fmaxf(m, x[i].x);
-                }
-#pragma unroll
-                for (int s = 1; s < EA_SHARE; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-#pragma unroll
-                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i) l += x[i].y = fast_exp2(x[i].x - m) * x[i].y;
-#pragma unroll
-                for (int s = 1; s < EA_SHARE; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-                const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll
-                for (int i = 0; i < EA_MOST_GROUPS / EA_SHARE; ++i)
-                    if (sub + i * EA_SHARE < count) factor_s[sub + i * EA_SHARE][row] = x[i].y * inv;
-                if (sub == 0) m_s[0][row] = m, total_s[row] = l;
-                __syncthreads();
-                each_item([&](int i, int row, int w, int n, int items) {
-                    float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                    for (int k = 0; k < count; ++k) {
-                        const float f = factor_s[k][row];
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + (long long)place(k) * EA_ROWS * PART + i * 4));
-                        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
-                    }
-                    done(v, i, row, w, n, items);
-                });
-            };
-            auto leave = [&](int place) {   // maximum and sum
-                if (threadIdx.x < n_rows) *reinterpret_cast<float2*>(a.part_ml + (place * EA_ROWS + threadIdx.x) * 2) = make_float2(m_s[0][threadIdx.x], total_s[threadIdx.x]);
-            };
-            auto last_of = [&](int* ticket, int count) {   // whether all others have left theirs; the counter is then as the next call wants it
-                __threadfence();
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    ticket_s = atomicAdd(ticket, 1);
-                    if (ticket_s == count - 1) *ticket = 0;
-                }
-                __syncthreads();
-                return ticket_s == count - 1;
-            };
-            leave(place_of(run));
-            const int group = run / EA_GROUP, groups = (runs + EA_GROUP - 1) / EA_GROUP, members = min(EA_GROUP, runs - group * EA_GROUP);
-            const int home = place_of(group * EA_GROUP);
-            if (last_of(a.tickets + home, members)) {
-                auto member = [&](int k) { return place_of(group * EA_GROUP + k); };
-                if (groups == 1) {
-                    join(members, member, [&](const float (&v)[4], int, int row, int w, int n, int count) { give_out(v, row, w, n, count); });
-                } else {
-                    join(members, member, [&](const float (&v)[4], int i, int, int, int, int) {
-                        *reinterpret_cast<float4*>(a.part_o + (long long)home * EA_ROWS * PART + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
-                    });
-                    leave(home);
-                    if (last_of(a.tickets + 2 * n_blocks + place_of(0), groups))
-                        join(groups, [&](int k) { return place_of(k * EA_GROUP); },
-                             [&](const float (&v)[4], int, int row, int w, int n, int count) { give_out(v, row, w, n, count); });
-                }
+            if (runs == 1) {
+                give_out<T, D>(out + row_at(row), v, i % (VW * 8));
+            } else {
+                *reinterpret_cast<float4*>(a.part_o + (long long)place_of(run) * ROWS * PART + i * 4) = v;
+                if (i % (VW * 8) == 0) *reinterpret_cast<float2*>(a.part_ml + (place_of(run) * ROWS + row) * 2) = make_float2(m, l);
             }
         }
+        if (runs > 1) {
+            if (threadIdx.x == 0) left_s[n_left] = {pair_begin, first_block, runs, n_rows, row0, kvh, r.begin};
+            ++n_left;   // (two at the most: a block's first pair and its last)
+        }
         __syncthreads();   // (the next pair takes the same shared memory)
+    }
+    // ---- pairs of several blocks: whoever leaves the last of sixteen results joins them, whoever joins the last sixteen joins the sixteens
+    for (int k = 0; k < n_left; ++k) {
+        const Pair pair = left_s[k];
+        const int run = (int)blockIdx.x - pair.first_block, group = run / EA_GROUP, groups = (pair.runs + EA_GROUP - 1) / EA_GROUP;
+        const int home = place_in(pair.begin, pair.first_block + group * EA_GROUP, target);
+        for (int level = 0; level < 2; ++level) {
+            const int count = level == 0 ? min(EA_GROUP, pair.runs - group * EA_GROUP) : groups;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int* ticket = a.tickets + (level == 0 ? home : 2 * n_blocks + place_in(pair.begin, pair.first_block, target));
+                ticket_s = atomicAdd(ticket, 1);
+                if (ticket_s == count - 1) *ticket = 0;   // (as the next call wants it)
+            }
+            __syncthreads();
+            if (ticket_s != count - 1) break;
+            __threadfence();
+            join_parts<T, D, NR>(out, a, pair, target, level == 0 ? group * EA_GROUP : 0, level == 0 ? 1 : EA_GROUP, count, level == 0 && groups > 1 ? home : -1, factor_s);
+            if (groups == 1) break;
+        }
+    }
+    // padding entries: zeros
+    for (int s = n_blocks - 1 - blockIdx.x; s < a.n_seqs; s += n_blocks) {
+        const Sequence x = sequence_of(a, s);
+        if (x.slot < 0)
+            for (int i = threadIdx.x; i < x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
     }
 }
 
 // Blocks that the device holds at once of this shape; 0 where the shape has no kernel.
-template <typename T, int D> static int slots_of() {
+template <typename T, int D, int NR> static int slots_of() {
     static int cached[64];
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
     if (cached[device] == 0) {
         int n = 0;
-        if (cudaFuncSetAttribute(attend_e4m3_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D>::SMEM) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_e4m3_kernel<T, D>, EA_WARPS * 32, Shape<T, D>::SMEM) != cudaSuccess)
+        if (cudaFuncSetAttribute(attend_e4m3_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NR>::SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_e4m3_kernel<T, D, NR>, EA_WARPS * 32, Shape<T, D, NR>::SMEM) != cudaSuccess)
             return 0;
         cached[device] = std::min(n * qf_sm_count(), EA_GROUP * EA_MOST_GROUPS);
     }
     return cached[device];
 }
-template <typename T, int D> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
-    if (a.block_slots <= 0 || a.block_slots != slots_of<T, D>()) return (int)cudaErrorInvalidValue;
-    return (int)launch_pdl(attend_e4m3_kernel<T, D>, dim3(blocks), dim3(EA_WARPS * 32), Shape<T, D>::SMEM, stream, (const T*)q, (T*)out, a);
+template <typename T, int D, int NR> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
+    if (a.block_slots <= 0 || a.block_slots != slots_of<T, D, NR>()) return (int)cudaErrorInvalidValue;
+    return (int)launch_pdl(attend_e4m3_kernel<T, D, NR>, dim3(blocks), dim3(EA_WARPS * 32), Shape<T, D, NR>::SMEM, stream, (const T*)q, (T*)out, a);
 }
 
-#define EA_EVERY(T, CALL)               \
-    switch (head_dim) {                 \
-        case 16: return CALL(T, 16);    \
-        case 32: return CALL(T, 32);    \
-        case 48: return CALL(T, 48);    \
-        case 64: return CALL(T, 64);    \
-        case 80: return CALL(T, 80);    \
-        case 96: return CALL(T, 96);    \
-        case 112: return CALL(T, 112);  \
-        case 128: return CALL(T, 128);  \
+#define EA_EVERY(T, NR, CALL)               \
+    switch (head_dim) {                     \
+        case 16: return CALL(T, 16, NR);    \
+        case 32: return CALL(T, 32, NR);    \
+        case 48: return CALL(T, 48, NR);    \
+        case 64: return CALL(T, 64, NR);    \
+        case 80: return CALL(T, 80, NR);    \
+        case 96: return CALL(T, 96, NR);    \
+        case 112: return CALL(T, 112, NR);  \
+        case 128: return CALL(T, 128, NR);  \
+    }
+#define EA_ALL(CALL)                        \
+    if (is_bf16 && rows == 8) {             \
+        EA_EVERY(bf16, 1, CALL)             \
+    } else if (is_bf16 && rows == 16) {     \
+        EA_EVERY(bf16, 2, CALL)             \
+    } else if (rows == 8) {                 \
+        EA_EVERY(float, 1, CALL)            \
+    } else if (rows == 16) {                \
+        EA_EVERY(float, 2, CALL)            \
     }
 
-// Blocks that the current device holds at once for a head size (0: there is no kernel for it): what the workspaces are sized by.
-QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim) {
-#define EA_SLOTS(T, D) slots_of<T, D>()
-    if (is_bf16) {
-        EA_EVERY(bf16, EA_SLOTS)
-    } else {
-        EA_EVERY(float, EA_SLOTS)
-    }
+// Blocks that the current device holds at once for a head size and blocks of 8 or 16 rows (0: there is no kernel for it): what the workspaces are
+// sized by.
+QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim, int rows) {
+#define EA_SLOTS(T, D, NR) slots_of<T, D, NR>()
+    EA_ALL(EA_SLOTS)
     return 0;
 }
 
-// q, out [tokens][n_heads * head_dim], on 16 bytes; single: every entry has one token; chunks: rows of 16 of the longest span, ceil(tokens * n_heads /
-// kv_heads / 16); most_pages: the most pages that a sequence reads; blocks: n_seqs * kv_heads * chunks * ceil(most_pages / 4), block_slots (of
-// qf_attention_e4m3_slots) at most. part_o [2 * blocks][16][32 * ceil(head_dim / 32)], part_ml [2 * blocks][16][2]; tickets [4 * blocks], zero before the
+// q, out [tokens][n_heads * head_dim], on 16 bytes; single: every entry has one token; rows: of a block, 8 or 16; chunks: of the longest span, ceil(tokens *
+// n_heads / kv_heads / rows); most_pages: the most pages that a sequence reads; blocks: n_seqs * kv_heads * chunks * ceil(most_pages / 4), block_slots (of
+// qf_attention_e4m3_slots) at most. part_o [2 * blocks][rows][32 * ceil(head_dim / 32)], part_ml [2 * blocks][rows][2]; tickets [4 * blocks], zero before the
 // first call and after every call.
 QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int* cu_q, const int* tok_pos, const int* slots, void* codes, float* scales,
                                 const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots, int kv_heads,
-                                int head_dim, int n_heads, int n_seqs, int single, int chunks, int most_pages, int blocks, int block_slots, float scale, int window,
+                                int head_dim, int n_heads, int n_seqs, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window,
                                 float* part_o, float* part_ml, int* tickets, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (head_dim <= 0 || head_dim % 16 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads || chunks <= 0 || most_pages <= 0 || columns <= 0 || n_slots <= 0 ||
@@ -759,11 +844,7 @@ QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int
         return (int)cudaErrorInvalidValue;
     if (n_seqs <= 0) return 0;
     AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_seqs, single, chunks, most_pages, block_slots, window, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
-#define EA_ATTEND(T, D) attend<T, D>(q, out, a, blocks, stream)
-    if (is_bf16) {
-        EA_EVERY(bf16, EA_ATTEND)
-    } else {
-        EA_EVERY(float, EA_ATTEND)
-    }
+#define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
+    EA_ALL(EA_ATTEND)
     return (int)cudaErrorInvalidValue;
 }

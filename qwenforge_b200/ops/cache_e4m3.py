@@ -14,7 +14,7 @@ from .branches import PAGE_TOKENS, _F, _I, _LL, _P, _at, _function, _here, _stre
 from .kernels import KernelError, _check, _dev
 
 E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128)
-E4M3_ROWS = 16     # query rows of a block of the attention (EA_ROWS)
+E4M3_ROWS = 16     # most query rows of a block of the attention: tokens of a span times heads of a group
 E4M3_WARPS = 4     # pages that a block has at work, and takes at the least where a sequence is cut (EA_WARPS)
 
 
@@ -140,8 +140,8 @@ class E4m3Scratch:
         self.device = torch.device(device)
         self.part_o = self.part_ml = self.tickets = None
 
-    def ensure(self, blocks: int, head_dim: int) -> None:
-        rows = 2 * blocks * E4M3_ROWS
+    def ensure(self, blocks: int, head_dim: int, rows: int) -> None:
+        rows *= 2 * blocks
         if self.part_o is None or self.part_o.numel() < rows * -(-head_dim // 32) * 32:
             self.part_o = torch.empty(rows * -(-head_dim // 32) * 32, dtype=torch.float32, device=self.device)
         if self.part_ml is None or self.part_ml.numel() < 2 * rows:
@@ -153,11 +153,11 @@ class E4m3Scratch:
 _block_slots: dict = {}
 
 
-def _slots_of(is_bf16: int, head_dim: int) -> int:
-    key = (torch._C._cuda_getDevice(), is_bf16, head_dim)
+def _slots_of(is_bf16: int, head_dim: int, rows: int) -> int:
+    key = (torch._C._cuda_getDevice(), is_bf16, head_dim, rows)
     n = _block_slots.get(key)
     if n is None:
-        n = _function("attention_e4m3", "qf_attention_e4m3_slots", _I, _I)(is_bf16, head_dim)
+        n = _function("attention_e4m3", "qf_attention_e4m3_slots", _I, _I, _I)(is_bf16, head_dim, rows)
         if n <= 0:
             raise KernelError(f"attention_e4m3: the device has no room for a block of head size {head_dim}")
         _block_slots[key] = n
@@ -194,11 +194,13 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     most = columns if max_kv_len is None else min(columns, -(-int(max_kv_len) // PAGE_TOKENS))
     if window > 0:
         most = min(most, -(-(window + max_q_len - 1) // PAGE_TOKENS) + 1)
-    chunks = -(-min(max_q_len, q.shape[0]) * (n_heads // kv_heads) // E4M3_ROWS)
-    block_slots = _slots_of(is_bf16, d)
+    rows = min(max_q_len, q.shape[0]) * (n_heads // kv_heads)
+    block_rows = 8 if rows <= 8 else E4M3_ROWS
+    chunks = -(-rows // block_rows)
+    block_slots = _slots_of(is_bf16, d, block_rows)
     blocks = min(block_slots, n_seqs * kv_heads * chunks * -(-most // E4M3_WARPS))
-    scratch.ensure(blocks, d)
+    scratch.ensure(blocks, d, block_rows)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
-    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P)(
+    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P)(
         is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.address(), n_heads, n_seqs,
-        max_q_len == 1 and q.shape[0] == n_seqs, chunks, most, blocks, block_slots, scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
+        max_q_len == 1 and q.shape[0] == n_seqs, block_rows, chunks, most, blocks, block_slots, scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
