@@ -14,11 +14,10 @@
 // tiles are the tall side of m16n8k16: S^T = K Q^T (16 positions by 8 rows), O^T = V^T P^T (16 components by 8 rows), so that seven or eight heads
 // of a group fill a tile, where they would be half of one the other way round, with half the products, exponentials and sums to keep.
 // P^T comes out of the first with positions where the second wants rows: eight by eight, the warp transposes it (movmatrix).
-// No shared memory lies on the way of the codes: a lane loads what its fragments hold. For the keys a lane takes D / 4 components of one
-// position in eight, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
+// A warp's tiles come through shared memory of its own, two on their way while it works on the third. For the keys a lane takes D / 4 components
+// of one position in eight, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
 // fragments go through the same). For the values a lane takes D / 8 neighbouring components of the four positions that a step wants
 // of it, and byte t of them is its element of component column t: a byte permutation puts two positions side by side for the conversion.
-// A tile's values are on their way while its scores are formed, the next tile's keys from then on.
 //
 // Work is shared out on the device, from the lengths (a captured graph replays this launch with others): all pages of all (sequence, kv head,
 // rows) in a row, `target` of them to a block, so that one round of blocks does it all. Where every pair's pages can be rounded up to
@@ -33,6 +32,7 @@
 #include "e4m3.cuh"
 
 #define EA_WARPS 4
+#define EA_DEAD 0x7fffffff   // the exponent of a tile that is not there, or that no row sees
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -56,31 +56,10 @@ __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t taken
     const float2 t = floats_of(taken);
     return pack_half(lo - t.x, hi - t.y);
 }
-__device__ __forceinline__ uint4 load16(const void* p) {   // (codes are read once: past L1)
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 load8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load4(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load2(const void* p) {
-    uint16_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
-    return v;
-}
-
 // A row of D components in parts of 128, 64, 32 and 16 that fragments go through one after another.
 template <int D> struct Parts {
-    // keys: a lane's words (four codes, one step of 16 components each) are D / 16; those of part 64 first
-    static constexpr int k64 = D / 64, k32 = (D % 64) / 32, k16 = (D % 32) / 16, k_words = D / 16;
+    // keys: a lane's words (four codes, one step of 16 components each) are D / 16; those of part 128 first
+    static constexpr int k128 = D / 128, k64 = (D % 128) / 64, k32 = (D % 64) / 32, k16 = (D % 32) / 16, k_words = D / 16;
     // values: bytes of a lane from part 128, 64, 32, 16: 16, 8, 4, 2
     static constexpr int v128 = D / 128, v64 = (D % 128) / 64, v32 = (D % 64) / 32, v16 = (D % 32) / 16;
     static constexpr int v_words = 4 * v128 + 2 * v64 + v32 + v16;   // (16 fills half a word)
@@ -88,10 +67,13 @@ template <int D> struct Parts {
 // First component of a lane's key word w (quad column c).
 template <int D> __device__ __forceinline__ constexpr int key_component(int w, int c) {
     using P = Parts<D>;
-    if (w < 4 * P::k64) return 64 * (w / 4) + 16 * c + 4 * (w % 4);
-    w -= 4 * P::k64;
-    if (w < 2 * P::k32) return 64 * P::k64 + 8 * c + 4 * w;
-    return 64 * P::k64 + 32 * P::k32 + 4 * c;
+    int base = 0;
+    if (w < 8 * P::k128) return 32 * c + 4 * w;
+    w -= 8 * P::k128, base += 128 * P::k128;
+    if (w < 4 * P::k64) return base + 16 * c + 4 * w;
+    w -= 4 * P::k64, base += 64 * P::k64;
+    if (w < 2 * P::k32) return base + 8 * c + 4 * w;
+    return base + 32 * P::k32 + 4 * c;
 }
 // The component that product t (of D / 8) has in its column n.
 template <int D> __device__ __forceinline__ int value_component(int t, int n) {
@@ -107,35 +89,42 @@ template <int D> __device__ __forceinline__ int value_component(int t, int n) {
 }
 template <int D> __device__ __forceinline__ void load_key(uint32_t (&w)[D / 16], const unsigned char* row, int c) {
     using P = Parts<D>;
-#pragma unroll
-    for (int i = 0; i < P::k64; ++i) {
-        const uint4 v = load16(row + 64 * i + 16 * c);
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    int at = 0, o = 0;
+    if constexpr (P::k128 != 0) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row + 32 * c), v = *reinterpret_cast<const uint4*>(row + 32 * c + 16);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = v.x, w[5] = v.y, w[6] = v.z, w[7] = v.w;
+        at += 128, o += 8;
+    }
+    if constexpr (P::k64 != 0) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + at + 16 * c);
+        w[o] = v.x, w[o + 1] = v.y, w[o + 2] = v.z, w[o + 3] = v.w;
+        at += 64, o += 4;
     }
     if constexpr (P::k32 != 0) {
-        const uint2 v = load8(row + 64 * P::k64 + 8 * c);
-        w[4 * P::k64] = v.x, w[4 * P::k64 + 1] = v.y;
+        const uint2 v = *reinterpret_cast<const uint2*>(row + at + 8 * c);
+        w[o] = v.x, w[o + 1] = v.y;
+        at += 32, o += 2;
     }
-    if constexpr (P::k16 != 0) w[4 * P::k64 + 2 * P::k32] = load4(row + 64 * P::k64 + 32 * P::k32 + 4 * c);
+    if constexpr (P::k16 != 0) w[o] = *reinterpret_cast<const uint32_t*>(row + at + 4 * c);
 }
 template <int D> __device__ __forceinline__ void load_value(uint32_t (&w)[Parts<D>::v_words], const unsigned char* row, int g) {
     using P = Parts<D>;
     int at = 0, o = 0;
     if constexpr (P::v128 != 0) {
-        const uint4 v = load16(row + 16 * g);
+        const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * g);
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         at += 128, o += 4;
     }
     if constexpr (P::v64 != 0) {
-        const uint2 v = load8(row + at + 8 * g);
+        const uint2 v = *reinterpret_cast<const uint2*>(row + at + 8 * g);
         w[o] = v.x, w[o + 1] = v.y;
         at += 64, o += 2;
     }
     if constexpr (P::v32 != 0) {
-        w[o] = load4(row + at + 4 * g);
+        w[o] = *reinterpret_cast<const uint32_t*>(row + at + 4 * g);
         at += 32, o += 1;
     }
-    if constexpr (P::v16 != 0) w[o] = load2(row + at + 2 * g);
+    if constexpr (P::v16 != 0) w[o] = *reinterpret_cast<const uint16_t*>(row + at + 2 * g);
 }
 __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 
@@ -144,10 +133,13 @@ template <typename T, int D, int NR> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
     static constexpr int ROWS = 8 * NR;
     static constexpr int TILE = D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
-    static constexpr int BLOCKS = NR > 1 ? 2 : 3;                     // of an SM
+    static constexpr int BLOCKS = 2;                                  // of an SM
+    static constexpr int STAGES = 3;                                  // tiles of a warp in shared memory: one at work, the others on their way
+    static constexpr int PITCH = D / 16 % 2 ? D : D + 16;             // bytes of a staged row: an odd number of 16, so that eight rows meet all banks
+    static constexpr int STAGE = 2 * TILE * PITCH;                    // keys, then values
     static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result: items of four
     static constexpr int LD = PART + 4;                               // and where warps leave theirs: rows four banks apart
-    static constexpr int SMEM = EA_WARPS * ROWS * LD * 4;
+    static constexpr int SMEM = EA_WARPS * (STAGES * STAGE > ROWS * LD * 4 ? STAGES * STAGE : ROWS * LD * 4);   // (the outputs take the tiles' place)
     static constexpr int SHARE = EA_WARPS * 32 / ROWS;                // lanes that join a row's maxima and sums
 };
 
@@ -273,7 +265,10 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, DT = D / 16, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS;
     constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32, TERMS = TWO ? 2 : 1;
     grid_chain_entry();
-    extern __shared__ __align__(16) float shared_o[];   // [warps][rows][LD]
+    extern __shared__ __align__(16) unsigned char staged[];   // [warps][STAGES][keys, values][TILE][PITCH]; later the outputs, [warps][rows][LD]
+    float* shared_o = reinterpret_cast<float*>(staged);
+    __shared__ float scale_s[EA_WARPS][S::STAGES];   // of the staged tiles: the keys' scale, the values' exponent
+    __shared__ int unit_s[EA_WARPS][S::STAGES];
     __shared__ float m_s[EA_WARPS][ROWS], l_s[EA_WARPS][ROWS], factor_s[EA_MOST_GROUPS * ROWS];
     __shared__ int ticket_s;
     __shared__ Pair left_s[2];
@@ -371,43 +366,57 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                 lo[n][e] = a.window > 0 ? max(0, hi[n][e] - a.window) : 0;
             }
 
-        // ---- keys of a step: pages p_begin + warp, + EA_WARPS, ..., a tile of one at a time
+        // ---- pages p_begin + warp, + EA_WARPS, ...: a tile of one at a time, through the warp's own stages
         const int steps = my_pages * PER_PAGE;
         const long long plane = (long long)KVH * QF_PAGE * D;
-        int lane_page = -1, lane_unit = 0;   // of 32 of the warp's pages, one a lane: its number, its scales
-        float lane_scale = 0.f;
-        int page_next = -1, unit_next = 0;   // of the step whose keys are loaded
-        float ks_next = 0.f;
-        uint32_t kw[NT][KW];
+        int lane_page = -1, lane_unit = 0, page_next = -1, unit_next = 0;   // of 32 of the warp's pages, one a lane: its number, its scales
+        float lane_scale = 0.f, scale_next = 0.f;
+        unsigned char* stage0 = staged + warp * S::STAGES * S::STAGE;
         auto key0_of = [&](int step) { return (p_begin + warp + step / PER_PAGE * EA_WARPS) * QF_PAGE + step % PER_PAGE * TILE; };
-        auto look_up = [&](int from) {   // pages from .. from + 31 of the warp's
-            lane_page = -1;
-            if (from + lane < my_pages) {
-                lane_page = e4m3_page(site, r.slot, (p_begin + warp + (from + lane) * EA_WARPS) * QF_PAGE);
-                if (lane_page < 0) {
-                    if (y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
-                } else {
-                    const float* scales = site.scales + (long long)lane_page * site.page_scales + kvh;
-                    lane_scale = scales[0];
-                    lane_unit = exponent_of(scales[KVH]);
+        auto fetch = [&](int step) {   // (one group of copies, perhaps an empty one)
+            if (step < steps) {
+                const int key0 = key0_of(step), stage = step % S::STAGES;
+                if (step % PER_PAGE == 0) {
+                    const int i = step / PER_PAGE;
+                    if (i % 32 == 0) {   // the next 32 pages
+                        lane_page = -1;
+                        if (i + lane < my_pages) {
+                            lane_page = e4m3_page(site, r.slot, (p_begin + warp + (i + lane) * EA_WARPS) * QF_PAGE);
+                            if (lane_page < 0) {
+                                if (y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
+                            } else {
+                                const float* scales = site.scales + (long long)lane_page * site.page_scales + kvh;
+                                lane_scale = scales[0];
+                                lane_unit = exponent_of(scales[KVH]);
+                            }
+                        }
+                    }
+                    page_next = __shfl_sync(0xffffffffu, lane_page, i % 32);
+                    scale_next = __shfl_sync(0xffffffffu, lane_scale, i % 32);
+                    unit_next = __shfl_sync(0xffffffffu, lane_unit, i % 32);
+                }
+                const bool live = page_next >= 0 && key0 < some_hi && key0 + TILE > some_lo;
+                if (lane == 0) scale_s[warp][stage] = scale_next, unit_s[warp][stage] = live ? unit_next : EA_DEAD;
+                if (live) {
+                    const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE) * D;
+                    unsigned char* to = stage0 + stage * S::STAGE;
+                    const bool whole = key0 >= some_lo && key0 + TILE <= some_hi;   // (else: zeros where nobody looks, NaN perhaps)
+                    constexpr int CHUNKS = TILE * D / 16;
+#pragma unroll
+                    for (int i = 0; i < (CHUNKS + 31) / 32; ++i) {
+                        const int e = i * 32 + lane, row = e / (D / 16), key = key0 + row;
+                        if (CHUNKS % 32 == 0 || e < CHUNKS) {
+                            const bool valid = whole || (key >= some_lo && key < some_hi);
+                            cp_async_16(to + e * 16 + row * (S::PITCH - D), k + e * 16, valid);
+                            cp_async_16(to + e * 16 + row * (S::PITCH - D) + TILE * S::PITCH, k + plane + e * 16, valid);
+                        }
+                    }
                 }
             }
+            cp_async_commit();
         };
-        auto load_keys = [&](int step) {
-            const int key0 = key0_of(step);
-            if (step % PER_PAGE == 0) {
-                const int i = step / PER_PAGE;
-                if (i % 32 == 0) look_up(i);
-                page_next = __shfl_sync(0xffffffffu, lane_page, i % 32);
-                ks_next = __shfl_sync(0xffffffffu, lane_scale, i % 32);
-                unit_next = __shfl_sync(0xffffffffu, lane_unit, i % 32);
-            }
-            if (page_next < 0 || key0 >= some_hi || key0 + TILE <= some_lo) return;
-            const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + g) * D;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) load_key<D>(kw[t], k + t * 8 * D, c);
-        };
-        if (steps > 0) load_keys(0);
+        for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
 
         // ---- the queries' fragments: lane (g, c) has row g's components of its column
         uint32_t qb[TERMS][NR][KW][2];
@@ -463,38 +472,18 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         bool begun = false;
 
         for (int step = 0; step < steps; ++step) {
-            const int page = page_next, key0 = key0_of(step), unit_v = unit_next;
-            const float ks = ks_next;
-            if (page < 0 || key0 >= some_hi || key0 + TILE <= some_lo) {
-                if (step + 1 < steps) load_keys(step + 1);
-                continue;
-            }
+            cp_async_wait<S::STAGES - 2>();
+            __syncwarp();   // (this tile has come for every lane, and every lane is done with the one before it)
+            fetch(step + S::STAGES - 1);
+            const int stage = step % S::STAGES, key0 = key0_of(step), unit_v = unit_s[warp][stage];
+            const float ks = scale_s[warp][stage];
+            if (unit_v == EA_DEAD) continue;
             if (!begun) {
 #pragma unroll
                 for (int n = 0; n < NR; ++n) unit_run[n][0] = unit_run[n][1] = unit_v;
                 begun = true;
             }
-            // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
-            uint32_t vw[KT][4][VW];
-            {
-                const unsigned char* v = site.codes + (long long)page * site.page_bytes + plane + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE + 2 * c) * D;
-                if (key0 >= some_lo && key0 + TILE <= some_hi) {   // every position is held, and seen by some row
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) load_value<D>(vw[kt][i], v + (16 * kt + (i & 1) + 8 * (i >> 1)) * D, g);
-                } else {
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int at_key = 16 * kt + (i & 1) + 8 * (i >> 1), key = key0 + at_key + 2 * c;
-#pragma unroll
-                            for (int w = 0; w < VW; ++w) vw[kt][i][w] = 0u;   // (what lies elsewhere is nobody's, NaN perhaps)
-                            if (key >= some_lo && key < some_hi) load_value<D>(vw[kt][i], v + at_key * D, g);
-                        }
-                }
-            }
+            const unsigned char* keys = stage0 + stage * S::STAGE + g * S::PITCH;
             // ---- scores: positions 16 t + g (0, 1) and 16 t + 8 + g (2, 3) by rows 2 c, 2 c + 1
             float s[KT][NR][4];
 #pragma unroll
@@ -502,62 +491,77 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
 #pragma unroll
                 for (int n = 0; n < NR; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
 #pragma unroll
-            for (int w = 0; w < KW; ++w)
+            for (int t = 0; t < KT; ++t) {
+                uint32_t kw[2][KW];
+                load_key<D>(kw[0], keys + 16 * t * S::PITCH, c);
+                load_key<D>(kw[1], keys + (16 * t + 8) * S::PITCH, c);
 #pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    const uint32_t x = kw[2 * t][w], z = kw[2 * t + 1][w], k[4] = {half2_of_low(x), half2_of_low(z), half2_of_high(x), half2_of_high(z)};
+                for (int w = 0; w < KW; ++w) {
+                    const uint32_t k[4] = {half2_of_low(kw[0][w]), half2_of_low(kw[1][w]), half2_of_high(kw[0][w]), half2_of_high(kw[1][w])};
 #pragma unroll
                     for (int n = 0; n < NR; ++n) {
                         if constexpr (TWO) mma_f16_16816(s[t][n], k, qb[TERMS - 1][n][w][0], qb[TERMS - 1][n][w][1]);
                         mma_f16_16816(s[t][n], k, qb[0][n][w][0], qb[0][n][w][1]);
                     }
                 }
-            if (step + 1 < steps) load_keys(step + 1);
+            }
+            // ---- this tile's values: positions 16 kt + 2 c, + 1, + 8, + 9
+            uint32_t vw[KT][4][VW];
+            const unsigned char* values = stage0 + stage * S::STAGE + (TILE + 2 * c) * S::PITCH;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load_value<D>(vw[kt][i], values + (16 * kt + (i & 1) + 8 * (i >> 1)) * S::PITCH, g);
             // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none
             const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
-            auto seen = [&](int t, int n, int e) {
-                const int key = key0 + 16 * t + 8 * (e >> 1) + g;
-                return key >= lo[n][e & 1] && key < hi[n][e & 1];
-            };
             float corr[NR][2], m_tile[NR][2];
             uint32_t pb[TERMS][KT][NR][2];
+            auto weigh = [&](auto whole) {
+                auto seen = [&](int t, int n, int e) {
+                    if (decltype(whole)::value) return true;
+                    const int key = key0 + 16 * t + 8 * (e >> 1) + g;
+                    return key >= lo[n][e & 1] && key < hi[n][e & 1];
+                };
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                float top[2] = {EA_NONE, EA_NONE}, shift[2], by_k[2];
+                for (int n = 0; n < NR; ++n) {
+                    float top[2] = {EA_NONE, EA_NONE}, shift[2], by_k[2];
 #pragma unroll
-                for (int t = 0; t < KT; ++t)
+                    for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (full || seen(t, n, e)) top[e & 1] = fmaxf(top[e & 1], s[t][n][e]);
+                        for (int e = 0; e < 4; ++e)
+                            if (seen(t, n, e)) top[e & 1] = fmaxf(top[e & 1], s[t][n][e]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    by_k[e] = by[n][e] * ks;
+                    for (int e = 0; e < 2; ++e) {
+                        by_k[e] = by[n][e] * ks;
 #pragma unroll
-                    for (int i = 4; i < 32; i <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], i));
-                    m_tile[n][e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
-                    const float m = fmaxf(m_run[n][e], m_tile[n][e]);
-                    corr[n][e] = fast_exp2(m_run[n][e] - m);
-                    m_run[n][e] = m;
-                    shift[e] = 14.f - m;
-                    l_run[n][e] *= corr[n][e];
-                }
-#pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    float(&x)[4] = s[t][n];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = fast_exp2(fmaf(x[e], by_k[e & 1], shift[e & 1]));
-                        if (!full && !seen(t, n, e)) x[e] = 0.f;
-                        l_run[n][e & 1] += x[e];
+                        for (int i = 4; i < 32; i <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], i));
+                        m_tile[n][e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
+                        const float m = fmaxf(m_run[n][e], m_tile[n][e]);
+                        corr[n][e] = fast_exp2(m_run[n][e] - m);
+                        m_run[n][e] = m;
+                        shift[e] = 14.f - m;
+                        l_run[n][e] *= corr[n][e];
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t most = pack_half(x[2 * h], x[2 * h + 1]);
-                        pb[0][t][n][h] = transposed(most);
-                        if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
+                    for (int t = 0; t < KT; ++t) {
+                        float(&x)[4] = s[t][n];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = fast_exp2(fmaf(x[e], by_k[e & 1], shift[e & 1]));
+                            if (!seen(t, n, e)) x[e] = 0.f;
+                            l_run[n][e & 1] += x[e];
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t most = pack_half(x[2 * h], x[2 * h + 1]);
+                            pb[0][t][n][h] = transposed(most);
+                            if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
+                        }
                     }
                 }
-            }
+            };
+            if (full) weigh(std::true_type{});
+            else weigh(std::false_type{});
             // ---- values. Word w of the four positions of a step holds their elements of the component columns 4 w .. 4 w + 3
             auto word_products = [&](int kt, int w, auto take, auto add) {
                 uint32_t x[4];
@@ -699,6 +703,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             }
         }
 
+        cp_async_wait<0>();
+        __syncthreads();   // (the outputs take the tiles' place)
         // ---- the warps' results together: the outputs of each alone, under shares of the whole weight. An item is four neighbouring components of a row
 #pragma unroll
         for (int n = 0; n < NR; ++n)
