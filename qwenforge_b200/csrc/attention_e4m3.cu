@@ -126,6 +126,10 @@ template <int D> __device__ __forceinline__ void load_value(uint32_t (&w)[Parts<
     }
     if constexpr (P::v16 != 0) w[o] = *reinterpret_cast<const uint16_t*>(row + at + 2 * g);
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from)); }
+__device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0));
+}
 __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 
 // NR: eights of rows of a block.
@@ -273,7 +277,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     __shared__ int ticket_s;
     __shared__ Pair left_s[2];
     int n_left = 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, c = lane & 3;
     const E4m3Site& site = a.site;
     const int KVH = site.kv_heads, G = a.n_heads / KVH, pairs_each = KVH * a.chunks;
     const int q_width = a.n_heads * D, n_blocks = gridDim.x;
@@ -281,8 +286,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     // ---- this block's share (every warp works it out for itself; a lane keeps its one of the first 32 sequences)
     Sequence first;
     first.pages = 0;
-    if (lane < a.n_seqs) first = sequence_of(a, lane);
-    auto pages_of = [&](int s0) { return s0 == 0 ? first.pages : s0 + lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0; };
+    if ((int)lane < a.n_seqs) first = sequence_of(a, lane);
+    auto pages_of = [&](int s0) { return s0 == 0 ? first.pages : s0 + (int)lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0; };
     int total = 0, pairs = 0, whole = 0, target = EA_WARPS;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
         const int pages = pages_of(s0);
@@ -315,7 +320,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
+                if ((int)lane >= o) upto += v;
             }
             const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > range_begin);
             if (beyond) {
@@ -351,7 +356,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         const int row0 = chunk * ROWS, n_rows = min(ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
         if (n_rows <= 0 || p_begin >= p_end) continue;
         auto row_at = [&](int row) { return row_offset<D>(a, r.begin, kvh, row0 + row); };
-        const int my_pages = p_begin + warp < p_end ? (p_end - p_begin - warp + EA_WARPS - 1) / EA_WARPS : 0;
+        const int my_pages = (p_end - p_begin - (int)warp + EA_WARPS - 1) / EA_WARPS;   // (0 where there are fewer than warps)
         // what the rows see, lo .. hi - 1: this lane's (8 n + 2 c and + 1), all of them together, every one of them
         const int t_first = a.single ? 0 : row0 / G, t_last = a.single ? 0 : (row0 + n_rows - 1) / G;
         const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (a.single ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
@@ -367,21 +372,23 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             }
 
         // ---- pages p_begin + warp, + EA_WARPS, ...: a tile of one at a time, through the warp's own stages
-        const int steps = my_pages * PER_PAGE;
+        const unsigned steps = my_pages * PER_PAGE;
         const long long plane = (long long)KVH * QF_PAGE * D;
         int lane_page = -1, lane_unit = 0, page_next = -1, unit_next = 0;   // of 32 of the warp's pages, one a lane: its number, its scales
         float lane_scale = 0.f, scale_next = 0.f;
-        unsigned char* stage0 = staged + warp * S::STAGES * S::STAGE;
-        auto key0_of = [&](int step) { return (p_begin + warp + step / PER_PAGE * EA_WARPS) * QF_PAGE + step % PER_PAGE * TILE; };
-        auto fetch = [&](int step) {   // (one group of copies, perhaps an empty one)
-            if (step < steps) {
-                const int key0 = key0_of(step), stage = step % S::STAGES;
-                if (step % PER_PAGE == 0) {
-                    const int i = step / PER_PAGE;
+        const unsigned char* stage0 = staged + warp * S::STAGES * S::STAGE;
+        const uint32_t lane_to = smem_addr(stage0) + lane * 16 + lane / (D / 16) * (S::PITCH - D);   // where the lane's first piece of a tile goes
+        auto key0_of = [&](unsigned step) { return (p_begin + (int)warp + (int)(step / PER_PAGE) * EA_WARPS) * QF_PAGE + (int)(step % PER_PAGE) * TILE; };
+        unsigned fetched = 0, fetch_stage = 0;
+        auto fetch = [&]() {   // the next tile (one group of copies, perhaps an empty one)
+            if (fetched < steps) {
+                const int key0 = key0_of(fetched);
+                if (fetched % PER_PAGE == 0) {
+                    const int i = fetched / PER_PAGE;
                     if (i % 32 == 0) {   // the next 32 pages
                         lane_page = -1;
-                        if (i + lane < my_pages) {
-                            lane_page = e4m3_page(site, r.slot, (p_begin + warp + (i + lane) * EA_WARPS) * QF_PAGE);
+                        if (i + (int)lane < my_pages) {
+                            lane_page = e4m3_page(site, r.slot, (p_begin + (int)warp + (i + (int)lane) * EA_WARPS) * QF_PAGE);
                             if (lane_page < 0) {
                                 if (y == 0) atomicOr(a.err, QF_ERR_NO_PAGE);
                             } else {
@@ -396,27 +403,42 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     unit_next = __shfl_sync(0xffffffffu, lane_unit, i % 32);
                 }
                 const bool live = page_next >= 0 && key0 < some_hi && key0 + TILE > some_lo;
-                if (lane == 0) scale_s[warp][stage] = scale_next, unit_s[warp][stage] = live ? unit_next : EA_DEAD;
+                if (lane == 0) scale_s[warp][fetch_stage] = scale_next, unit_s[warp][fetch_stage] = live ? unit_next : EA_DEAD;
                 if (live) {
-                    const unsigned char* k = site.codes + (long long)page_next * site.page_bytes + ((long long)kvh * QF_PAGE + step % PER_PAGE * TILE) * D;
-                    unsigned char* to = stage0 + stage * S::STAGE;
-                    const bool whole = key0 >= some_lo && key0 + TILE <= some_hi;   // (else: zeros where nobody looks, NaN perhaps)
-                    constexpr int CHUNKS = TILE * D / 16;
+                    const unsigned char* k =
+                        site.codes + (long long)page_next * site.page_bytes + (kvh * QF_PAGE + (int)(fetched % PER_PAGE) * TILE) * D + lane * 16;
+                    const unsigned char* v = k + plane;
+                    const uint32_t to = lane_to + fetch_stage * S::STAGE;
+                    constexpr int CHUNKS = TILE * D / 16, ROUNDS = (CHUNKS + 31) / 32;
+                    // piece i * 32 + lane: its row's number and so its place move by constants where a round has whole rows
+                    auto place = [&](int i) -> uint32_t {
+                        if constexpr (32 % (D / 16) == 0) return to + i * (512 + 32 / (D / 16) * (S::PITCH - D));
+                        else return to + i * 512 + ((unsigned)(i * 32 + lane) / (D / 16) - lane / (D / 16)) * (S::PITCH - D);
+                    };
+                    if (key0 >= some_lo && key0 + TILE <= some_hi) {
 #pragma unroll
-                    for (int i = 0; i < (CHUNKS + 31) / 32; ++i) {
-                        const int e = i * 32 + lane, row = e / (D / 16), key = key0 + row;
-                        if (CHUNKS % 32 == 0 || e < CHUNKS) {
-                            const bool valid = whole || (key >= some_lo && key < some_hi);
-                            cp_async_16(to + e * 16 + row * (S::PITCH - D), k + e * 16, valid);
-                            cp_async_16(to + e * 16 + row * (S::PITCH - D) + TILE * S::PITCH, k + plane + e * 16, valid);
-                        }
+                        for (int i = 0; i < ROUNDS; ++i)
+                            if (CHUNKS % 32 == 0 || i * 32 + lane < CHUNKS) {
+                                copy16(place(i), k + i * 512);
+                                copy16(place(i) + TILE * S::PITCH, v + i * 512);
+                            }
+                    } else {   // zeros where nobody looks, NaN perhaps
+#pragma unroll
+                        for (int i = 0; i < ROUNDS; ++i)
+                            if (CHUNKS % 32 == 0 || i * 32 + lane < CHUNKS) {
+                                const int key = key0 + (int)((unsigned)(i * 32 + lane) / (D / 16));
+                                copy16_or_zero(place(i), k + i * 512, key >= some_lo && key < some_hi);
+                                copy16_or_zero(place(i) + TILE * S::PITCH, v + i * 512, key >= some_lo && key < some_hi);
+                            }
                     }
                 }
+                ++fetched;
+                fetch_stage = fetch_stage + 1 == S::STAGES ? 0 : fetch_stage + 1;
             }
             cp_async_commit();
         };
 #pragma unroll
-        for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+        for (int i = 0; i < S::STAGES - 1; ++i) fetch();
 
         // ---- the queries' fragments: lane (g, c) has row g's components of its column
         uint32_t qb[TERMS][NR][KW][2];
@@ -471,11 +493,13 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         for (int n = 0; n < NR; ++n) m_run[n][0] = m_run[n][1] = EA_NONE, l_run[n][0] = l_run[n][1] = 0.f, unit_run[n][0] = unit_run[n][1] = 0;
         bool begun = false;
 
-        for (int step = 0; step < steps; ++step) {
+        unsigned stage = S::STAGES - 1;   // (of the step before the first)
+        for (unsigned step = 0; step < steps; ++step) {
             cp_async_wait<S::STAGES - 2>();
             __syncwarp();   // (this tile has come for every lane, and every lane is done with the one before it)
-            fetch(step + S::STAGES - 1);
-            const int stage = step % S::STAGES, key0 = key0_of(step), unit_v = unit_s[warp][stage];
+            fetch();
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            const int key0 = key0_of(step), unit_v = unit_s[warp][stage];
             const float ks = scale_s[warp][stage];
             if (unit_v == EA_DEAD) continue;
             if (!begun) {
