@@ -9,9 +9,14 @@
 //   new codes = round(x * 2^-e), to nearest even, from float32: one rounding
 // A page that is begun takes its exponent from its new rows alone, whatever an earlier holder left there. Rows behind the new ones stay.
 //
-// A run is a page's new rows. A block takes the runs that begin among its share of the step's tokens, a warp a head at a time over all
-// rows of the run: amax and codes are one warp's business, without a barrier. Sines and cosines are worked out once per run for the
-// heads of the block. A key or value head is read twice (amax, codes), the second time from L1 or L2.
+// A run is a page's new rows. Two kernels, the same in what they write:
+//   write_runs     spans of EW_LONG tokens or more: a block takes the runs that begin among 64 of the step's tokens and some of the heads, all its
+//                  threads one head at a time. A thread has the same one or two pieces (a row, eight pairs of the rotation) of every head, so
+//                  their sines and cosines are worked out once and stay in registers, a key's or value's elements stay there between amax and
+//                  codes, and the next head's are loaded meanwhile.
+//   write_any      single tokens, short spans, and rows or rotations that 16-byte accesses do not fit: a warp a head at a time over all rows of
+//                  a run; amax and codes are one warp's business, without a barrier. Sines and cosines come from shared memory, worked
+//                  out once per run. A key or value head is read twice, the second time from L1 or L2.
 #include "e4m3.cuh"
 
 #define EW_WARPS 8
@@ -60,9 +65,23 @@ __device__ __forceinline__ float finite_size(float v) {
     return a <= 3.402823466e38f ? a : 0.f;
 }
 
+// Codes of rows that a page had, rounded to a larger unit: code * `by`, by <= 1/2 a power of two.
+__device__ __forceinline__ void rescale_codes(uint4* codes, int pieces, float by, int first, int step) {
+    for (int i = first; i < pieces; i += step) {
+        uint4 w = codes[i];
+        uint32_t* words = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 lo = floats_of(half2_of_low(words[e])), hi = floats_of(half2_of_high(words[e]));
+            words[e] = e4m3_four(lo.x * by, lo.y * by, hi.x * by, hi.y * by);
+        }
+        codes[i] = w;
+    }
+}
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(EW_WARPS * 32)
-write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
+write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                   const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
                   T* __restrict__ q_out, E4m3Site site, int write_cache, int n_tokens, int share, int most_rows, int* err) {
     grid_chain_entry();
@@ -149,19 +168,7 @@ write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
             if (at > 0) {
                 const int before = exponent_of(*scale);
                 exp = max(exp, before);
-                if (exp > before) {
-                    const float by = pow2(max(before - exp, -126));
-                    for (int i = lane; i < at * D / 16; i += 32) {
-                        uint4 w = reinterpret_cast<const uint4*>(codes)[i];
-                        uint32_t* words = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 lo = floats_of(half2_of_low(words[e])), hi = floats_of(half2_of_high(words[e]));
-                            words[e] = e4m3_four(lo.x * by, lo.y * by, hi.x * by, hi.y * by);
-                        }
-                        reinterpret_cast<uint4*>(codes)[i] = w;
-                    }
-                }
+                if (exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), lane, 32);
             }
             const float by = pow2(-exp);
             codes += at * D;
@@ -180,6 +187,146 @@ write_e4m3_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     }
 }
 
+#define EW_THREADS 256
+#define EW_PIECES 2   // of a thread: 64 rows of up to eight pieces
+
+template <typename T>
+__global__ void __launch_bounds__(EW_THREADS, 2)
+write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
+                  const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
+                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_tokens, int* err) {
+    grid_chain_entry();
+    constexpr int RAW = 16 * sizeof(T) / 16;   // 16-byte words of a piece: eight elements here, eight there
+    __shared__ float amax_s[2][EW_THREADS / 32];
+    const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2, groups = D / 16;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = n_heads + 2 * KVH;
+    const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
+    const int t0 = blockIdx.x * QF_PAGE;
+    int parity = 0;
+    for (int part = 0; part < QF_PAGE; part += 32) {
+        // tokens at which a run begins
+        bool begins = false;
+        if (t0 + part + lane < n_tokens) begins = tok_pos[t0 + part + lane] % QF_PAGE == 0 || t0 + part + lane == cu_q[tok_seq[t0 + part + lane]];
+        for (uint32_t left = __ballot_sync(0xffffffffu, begins); left; left &= left - 1) {
+            const int t = t0 + part + __ffs(left) - 1, seq = tok_seq[t], first_pos = tok_pos[t], at = first_pos % QF_PAGE;
+            const int slot = write_cache ? slots[seq] : -1, rows = min(cu_q[seq + 1] - t, QF_PAGE - at);
+            const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
+            if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
+            // this thread's pieces: a row, the places of its two eights in a head, and their turn
+            int row[EW_PIECES], a_at[EW_PIECES], b_at[EW_PIECES];
+            bool turns[EW_PIECES];
+            float cosine[EW_PIECES][8], sine[EW_PIECES][8];
+#pragma unroll
+            for (int k = 0; k < EW_PIECES; ++k) {
+                const unsigned i = threadIdx.x + k * EW_THREADS, g = i % (unsigned)groups;
+                row[k] = i / (unsigned)groups;
+                turns[k] = 8 * (int)g < half;
+                a_at[k] = turns[k] ? 8 * g : 16 * g;   // (rot_dim + 16 (g - half / 8) behind the rotated part)
+                b_at[k] = turns[k] ? 8 * g + half : 16 * g + 8;
+                if (row[k] < rows && turns[k]) {
+                    const float p = (float)(first_pos + row[k]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = inv_freq[8 * g + e], angle = p * f, rest = fmaf(p, f, -angle);
+                        float s, c;
+                        sincosf(angle, &s, &c);
+                        cosine[k][e] = fmaf(-s, rest, c);
+                        sine[k][e] = fmaf(c, rest, s);
+                    }
+                }
+            }
+            uint4 raw[EW_PIECES][RAW];
+            auto load = [&](int h) {
+#pragma unroll
+                for (int k = 0; k < EW_PIECES; ++k)
+                    if (row[k] < rows) {
+                        const T* src = qkv + (long long)(t + row[k]) * qkv_stride + (long long)h * D;
+#pragma unroll
+                        for (int i = 0; i < RAW / 2; ++i) {
+                            raw[k][i] = reinterpret_cast<const uint4*>(src + a_at[k])[i];
+                            raw[k][RAW / 2 + i] = reinterpret_cast<const uint4*>(src + b_at[k])[i];
+                        }
+                    }
+            };
+            if (h_begin < h_end) load(h_begin);
+            for (int h = h_begin; h < h_end; ++h) {
+                const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
+                const int kvh = is_v ? h - n_heads - KVH : h - n_heads;
+                float x[EW_PIECES][16], amax = 0.f;
+#pragma unroll
+                for (int k = 0; k < EW_PIECES; ++k) {
+                    if (row[k] >= rows) continue;
+                    const T* v = reinterpret_cast<const T*>(raw[k]);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[k][e] = Num<T>::to_f(v[e]);
+                    if (bias) {
+                        float b[8];
+#pragma unroll
+                        for (int part16 = 0; part16 < 2; ++part16) {
+                            load_values<T, 8>(bias + (long long)h * D + (part16 ? b_at[k] : a_at[k]), nullptr, b);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[k][8 * part16 + e] += b[e];
+                        }
+                    }
+                    if (!is_v && turns[k]) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float u = x[k][e], w = x[k][8 + e];
+                            x[k][e] = u * cosine[k][e] - w * sine[k][e];
+                            x[k][8 + e] = w * cosine[k][e] + u * sine[k][e];
+                        }
+                    }
+                }
+                if (h + 1 < h_end) load(h + 1);
+                if (is_q) {
+#pragma unroll
+                    for (int k = 0; k < EW_PIECES; ++k)
+                        if (row[k] < rows) {
+                            T* dst = q_out + ((long long)(t + row[k]) * n_heads + h) * D;
+                            store_values<T, 8>(dst + a_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][0]));
+                            store_values<T, 8>(dst + b_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][8]));
+                        }
+                    continue;
+                }
+                if (page < 0) continue;
+#pragma unroll
+                for (int k = 0; k < EW_PIECES; ++k)
+                    if (row[k] < rows) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_size(x[k][e]));
+                    }
+                float* scale = site.scales + (long long)page * site.page_scales + (is_v ? KVH : 0) + kvh;
+                const int before = at > 0 ? exponent_of(*scale) : E4M3_LOW;
+                amax = warp_max(amax);
+                if (lane == 0) amax_s[parity][warp] = amax;
+                __syncthreads();   // (every thread has read the old scale, too)
+#pragma unroll
+                for (int w = 0; w < EW_THREADS / 32; ++w) amax = fmaxf(amax, amax_s[parity][w]);
+                parity ^= 1;
+                const int exp = max(e4m3_exponent(amax), before);
+                unsigned char* codes = site.codes + (long long)page * site.page_bytes + (long long)((is_v ? KVH : 0) + kvh) * QF_PAGE * D;
+                if (at > 0 && exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), threadIdx.x, EW_THREADS);
+                const float by = pow2(-exp);
+#pragma unroll
+                for (int k = 0; k < EW_PIECES; ++k)
+                    if (row[k] < rows) {
+                        unsigned char* dst = codes + (at + row[k]) * D;
+                        store_codes<8>(dst + a_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][0]), by);
+                        store_codes<8>(dst + b_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][8]), by);
+                    }
+                if (threadIdx.x == 0) *scale = pow2(exp);
+            }
+        }
+    }
+}
+
+#ifndef EW_HEADS
+#define EW_HEADS 6   // heads of a block of write_runs
+#endif
+#ifndef EW_LONG
+#define EW_LONG 16   // tokens of the longest span from which write_runs is the faster one (@LONG@)
+#endif
+
 template <typename T>
 static int write_launch(const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq, const int* tok_pos, const int* slots,
                         const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int write_cache, int n_tokens, int max_q_len, int* err,
@@ -189,10 +336,15 @@ static int write_launch(const void* qkv, const void* bias, long long qkv_stride,
     const int most_rows = max_q_len < QF_PAGE ? max_q_len : QF_PAGE;
     const size_t smem = (size_t)most_rows * (rot_dim / 2) * sizeof(float2);
     const bool wide = rot_dim % 16 == 0 && qkv_stride % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias) % 16 == 0;
+    if (wide && max_q_len >= EW_LONG) {
+        const int pieces = (heads + EW_HEADS - 1) / EW_HEADS;
+        return (int)launch_pdl(write_runs_kernel<T>, dim3((n_tokens + QF_PAGE - 1) / QF_PAGE, pieces), dim3(EW_THREADS), 0, stream, (const T*)qkv, (const T*)bias, qkv_stride,
+                               cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, err);
+    }
     const dim3 grid((n_tokens + share - 1) / share, slices);
-    return (int)(wide ? launch_pdl(write_e4m3_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
+    return (int)(wide ? launch_pdl(write_any_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
                                    tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err)
-                      : launch_pdl(write_e4m3_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
+                      : launch_pdl(write_any_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
                                    tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err));
 }
 

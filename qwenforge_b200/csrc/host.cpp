@@ -55,6 +55,13 @@ int (*attention_shared)(int, const void*, void*, const int*, const int*, const i
 int (*copy_pages)(void*, int, int, int, long long, long long, int, long long, long long, int, const int*, int, Stream);
 int (*verify_drafts)(const float*, int, int, long long, const float*, long long, const int*, int, const int*, int, const float*, float, unsigned long long,
                      unsigned long long, const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
+int (*write_e4m3)(int, const void*, const void*, long long, const int*, const int*, const int*, const int*, const float*, int, int, void*, void*, float*,
+                  const int*, long long, long long, int, int, int, int, int, int, int, int, int*, Stream);
+int (*read_e4m3)(int, void*, long long, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int, int,
+                 int, int*, Stream);
+int (*attention_e4m3_slots)(int, int, int);
+int (*attention_e4m3)(int, const void*, void*, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int,
+                      int, int, int, int, int, int, int, float, int, float*, float*, int*, int*, Stream);
 PyObject* kernel_error = nullptr;
 
 const struct {
@@ -66,7 +73,9 @@ const struct {
                {"qf_stabilized_gates", (void**)&stabilized_gates}, {"qf_state_chunks", (void**)&state_chunks},
                {"qf_gated_group_norm", (void**)&gated_group_norm}, {"qf_rope_cache_write", (void**)&rope_cache_write}, {"qf_swiglu", (void**)&swiglu},
                {"qf_causal_conv", (void**)&causal_conv}, {"qf_row_chunks", (void**)&row_chunks},
-               {"qf_attention_shared", (void**)&attention_shared}, {"qf_copy_pages", (void**)&copy_pages}, {"qf_verify_drafts", (void**)&verify_drafts}};
+               {"qf_attention_shared", (void**)&attention_shared}, {"qf_copy_pages", (void**)&copy_pages}, {"qf_verify_drafts", (void**)&verify_drafts},
+               {"qf_rope_cache_write_e4m3", (void**)&write_e4m3}, {"qf_cache_read_e4m3", (void**)&read_e4m3}, {"qf_attention_e4m3", (void**)&attention_e4m3},
+               {"qf_attention_e4m3_slots", (void**)&attention_e4m3_slots}};
 
 // setup(KernelError, {name: address}): some of the entries, or more of them later.
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -499,6 +508,119 @@ PyObject* pages_copied(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- a cache in 8 bits: the launches of ops/cache_e4m3.py, in the same manner (host time of a call, microseconds, there / here: @HOST@).
+// A site's place: the tuple (codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim) of its checked tensors.
+struct Place {
+    void* codes;
+    float* scales;
+    const int* table;
+    long long page_bytes, page_scales;
+    int table_stride, columns, n_slots, kv_heads, head_dim;
+};
+bool placed(PyObject* o, Place& p) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 10) return false;
+    long long v[10];
+    for (int i = 0; i < 10; ++i) v[i] = number(PyTuple_GET_ITEM(o, i));
+    p = Place{(void*)v[0], (float*)v[1], (const int*)v[2], v[3], v[4], (int)v[5], (int)v[6], (int)v[7], (int)v[8], (int)v[9]};
+    return true;
+}
+
+// rope_cache_write_e4m3(qkv, bias or None, cu_q, tok_seq, tok_pos, slots, inv_freq or None, q_out, err, storage, place, rot_dim, n_heads, write_cache, max_q_len)
+PyObject* e4m3_written(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 15) return PyErr_Format(PyExc_TypeError, "rope_cache_write_e4m3: 15 arguments");
+    const at::Tensor* t[10];
+    for (int i = 0; i < 10; ++i) t[i] = tensor(args[i]);
+    const at::Tensor *qkv = t[0], *bias = t[1], *cu = t[2], *seq = t[3], *pos = t[4], *slots = t[5], *freq = t[6], *q = t[7], *err = t[8], *storage = t[9];
+    Place p;
+    const bool known = placed(args[10], p);
+    const long long rot = number(args[11]), heads = number(args[12]), writes = number(args[13]), most = number(args[14]);
+    if (PyErr_Occurred()) return nullptr;
+    const int device = c10::cuda::current_device();
+    const at::ScalarType type = qkv ? qkv->scalar_type() : at::kInt;
+    if (!known || !write_e4m3 || (type != at::kBFloat16 && type != at::kFloat) || !on(qkv, type, device) || !dense(q, type, device) || !dense(cu, at::kInt, device) ||
+        !dense(seq, at::kInt, device) || !dense(pos, at::kInt, device) || !dense(slots, at::kInt, device) || !dense(err, at::kInt, device) || !storage ||
+        !storage->is_cuda() || storage->get_device() != device || (args[1] != Py_None && !dense(bias, type, device)) ||
+        (args[6] != Py_None && !dense(freq, at::kFloat, device)) || heads <= 0 || most <= 0 || most > INT_MAX || qkv->dim() != 2 || qkv->stride(1) != 1)
+        Py_RETURN_NONE;
+    const long long rows = qkv->size(0), width = (heads + 2 * p.kv_heads) * p.head_dim;
+    if (rows <= 0 || qkv->size(1) < width || q->dim() != 2 || q->size(0) != rows || q->size(1) != heads * p.head_dim || seq->numel() != rows || pos->numel() != rows ||
+        cu->numel() != slots->numel() + 1 || (bias && bias->numel() != width) || (freq && (rot < 0 || rot > p.head_dim || freq->numel() * 2 != rot)))
+        Py_RETURN_NONE;
+    return code_of([&] {
+        return write_e4m3(type == at::kBFloat16, qkv->data_ptr(), bias ? bias->data_ptr() : nullptr, qkv->stride(0), ints(cu), ints(seq), ints(pos), ints(slots),
+                          freq ? freq->const_data_ptr<float>() : nullptr, (int)rot, (int)heads, q->data_ptr(), p.codes, p.scales, p.table, p.page_bytes, p.page_scales,
+                          p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, writes != 0, (int)rows, (int)most, at_ptr<int>(*err), stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_read_e4m3(out, cu_q, tok_pos, slots, err, storage, place, n_seqs, max_kv_len, window)
+PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "cache_read_e4m3: 10 arguments");
+    const at::Tensor* t[6];
+    for (int i = 0; i < 6; ++i) t[i] = tensor(args[i]);
+    const at::Tensor *out = t[0], *cu = t[1], *pos = t[2], *slots = t[3], *err = t[4], *storage = t[5];
+    Place p;
+    const bool known = placed(args[6], p);
+    const long long seqs = number(args[7]), longest = number(args[8]), window = number(args[9]);
+    if (PyErr_Occurred()) return nullptr;
+    const int device = c10::cuda::current_device();
+    const at::ScalarType type = out ? out->scalar_type() : at::kInt;
+    if (!known || !read_e4m3 || (type != at::kBFloat16 && type != at::kFloat) || !on(out, type, device) || !dense(cu, at::kInt, device) || !dense(pos, at::kInt, device) ||
+        !dense(slots, at::kInt, device) || !dense(err, at::kInt, device) || !storage || !storage->is_cuda() || storage->get_device() != device || seqs <= 0 ||
+        slots->numel() != seqs || cu->numel() != seqs + 1 || longest <= 0 || window < 0 || window > INT_MAX || out->sizes() != storage->sizes() || !on16(*out))
+        Py_RETURN_NONE;
+    const long long d = p.head_dim, page = 2ll * p.kv_heads * 64 * d, step = out->size(0) == 1 ? page : out->stride(0);
+    if (out->stride(4) != 1 || out->stride(3) != d || out->stride(2) != 64 * d || out->stride(1) != p.kv_heads * 64 * d || step < page || step % 8) Py_RETURN_NONE;
+    const long long pages = (longest + 63) / 64;
+    return code_of([&] {
+        return read_e4m3(type == at::kBFloat16, out->data_ptr(), step, ints(cu), ints(pos), ints(slots), p.codes, p.scales, p.table, p.page_bytes, p.page_scales,
+                         p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, (int)seqs, (int)(pages < p.columns ? pages : p.columns), (int)window,
+                         at_ptr<int>(*err), stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_e4m3(q, out, cu_q, tok_pos, slots, err, storage, place, part_o, part_ml, tickets, n_heads, n_seqs, max_q_len, scale, window, max_kv_len)
+PyObject* e4m3_attended(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 17) return PyErr_Format(PyExc_TypeError, "attention_e4m3: 17 arguments");
+    const at::Tensor *q = tensor(args[0]), *out = tensor(args[1]), *cu = tensor(args[2]), *pos = tensor(args[3]), *slots = tensor(args[4]), *err = tensor(args[5]),
+                     *storage = tensor(args[6]), *part_o = tensor(args[8]), *part_ml = tensor(args[9]), *tickets = tensor(args[10]);
+    Place p;
+    const bool known = placed(args[7], p);
+    const long long heads = number(args[11]), seqs = number(args[12]), most_q = number(args[13]);
+    const double scale = PyFloat_AsDouble(args[14]);
+    const long long window = number(args[15]), longest = number(args[16]);
+    if (PyErr_Occurred()) return nullptr;
+    const int device = c10::cuda::current_device();
+    const at::ScalarType type = q ? q->scalar_type() : at::kInt;
+    if (!known || !attention_e4m3 || !attention_e4m3_slots || (type != at::kBFloat16 && type != at::kFloat) || !dense(q, type, device) || !dense(out, type, device) ||
+        !dense(cu, at::kInt, device) || !dense(pos, at::kInt, device) || !dense(slots, at::kInt, device) || !dense(err, at::kInt, device) || !storage ||
+        !storage->is_cuda() || storage->get_device() != device || !on(part_o, at::kFloat, device) || !on(part_ml, at::kFloat, device) || !on(tickets, at::kInt, device) ||
+        seqs <= 0 || slots->numel() != seqs || cu->numel() != seqs + 1 || heads <= 0 || heads % p.kv_heads || most_q <= 0 || window < 0 || window > INT_MAX ||
+        q->dim() != 2 || q->size(0) <= 0 || q->size(1) != heads * p.head_dim || out->sizes() != q->sizes() || pos->numel() != q->size(0) || !on16(*q) || !on16(*out))
+        Py_RETURN_NONE;
+    const long long tokens = q->size(0), rows = (most_q < tokens ? most_q : tokens) * (heads / p.kv_heads), block_rows = rows <= 8 ? 8 : 16;
+    const long long chunks = (rows + block_rows - 1) / block_rows;
+    long long most = (longest + 63) / 64 > p.columns ? p.columns : (longest + 63) / 64;
+    if (window > 0 && (window + most_q + 62) / 64 + 1 < most) most = (window + most_q + 62) / 64 + 1;
+    const long long block_slots = attention_e4m3_slots(type == at::kBFloat16, p.head_dim, (int)block_rows);
+    const long long need = seqs * p.kv_heads * chunks * ((most + 3) / 4), blocks = need < block_slots ? need : block_slots;
+    if (most <= 0 || block_slots <= 0 || chunks > INT_MAX || part_o->numel() < 2 * blocks * block_rows * ((p.head_dim + 31) / 32 * 32) ||
+        part_ml->numel() < 4 * blocks * block_rows || tickets->numel() < 4 * blocks)
+        Py_RETURN_NONE;
+    return code_of([&] {
+        return attention_e4m3(type == at::kBFloat16, q->data_ptr(), out->data_ptr(), ints(cu), ints(pos), ints(slots), p.codes, p.scales, p.table, p.page_bytes,
+                              p.page_scales, p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, (int)heads, (int)seqs, most_q == 1 && tokens == seqs,
+                              (int)block_rows, (int)chunks, (int)most, (int)blocks, (int)block_slots, (float)scale, (int)window, at_ptr<float>(*part_o),
+                              at_ptr<float>(*part_ml), at_ptr<int>(*tickets), at_ptr<int>(*err), stream());
+    });
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {{"setup", (PyCFunction)(void (*)())setup, METH_FASTCALL, nullptr},
                          {"rms_norm", (PyCFunction)(void (*)())rms_norm, METH_FASTCALL, nullptr},
                          {"prompt_attention", (PyCFunction)(void (*)())prompt_attention, METH_FASTCALL, nullptr},
@@ -509,6 +631,9 @@ PyMethodDef methods[] = {{"setup", (PyCFunction)(void (*)())setup, METH_FASTCALL
                          {"attention_shared", (PyCFunction)(void (*)())shared_attention, METH_FASTCALL, nullptr},
                          {"verify_drafts", (PyCFunction)(void (*)())drafts_verified, METH_FASTCALL, nullptr},
                          {"copy_pages", (PyCFunction)(void (*)())pages_copied, METH_FASTCALL, nullptr},
+                         {"rope_cache_write_e4m3", (PyCFunction)(void (*)())e4m3_written, METH_FASTCALL, nullptr},
+                         {"cache_read_e4m3", (PyCFunction)(void (*)())e4m3_read, METH_FASTCALL, nullptr},
+                         {"attention_e4m3", (PyCFunction)(void (*)())e4m3_attended, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

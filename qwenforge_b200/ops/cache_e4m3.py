@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import kernels
-from .branches import PAGE_TOKENS, _F, _I, _LL, _P, _at, _function, _here, _stream
+from .branches import PAGE_TOKENS, _F, _I, _LL, _P, _at, _function, _here, _native, _stream
 from .kernels import KernelError, _check, _dev
 
 E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128)
@@ -21,7 +21,7 @@ E4M3_WARPS = 4     # pages that a block has at work, and takes at the least wher
 class E4m3SiteArgs:
     """What the kernels need to address one schedule entry's keys and values in 8 bits. storage: float8_e4m3fn [pages, 2, kv_heads, 64,
     head_dim], scales: float32 [pages, 2, kv_heads] (a page of each dense, pages at any distance of 16 bytes' multiple), table: int32 [slots, columns]."""
-    __slots__ = ("storage", "scales", "table", "kv_heads", "head_dim")
+    __slots__ = ("storage", "scales", "table", "kv_heads", "head_dim", "place")
 
     def __init__(self, storage: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, kv_heads: int, head_dim: int):
         _dev("cache", storage, torch.float8_e4m3fn, contiguous=False)
@@ -40,14 +40,12 @@ class E4m3SiteArgs:
             raise KernelError("a cache in 8 bits begins on 16 bytes")
         if table.dim() != 2 or table.stride(1) != 1 or table.shape[0] < 1 or table.shape[1] < 1:
             raise KernelError("the page table is [slots, pages] with unit inner stride")
+        if len({t.get_device() for t in (storage, scales, table)}) != 1:
+            raise KernelError("a cache in 8 bits lies on one device")
         self.storage, self.scales, self.table, self.kv_heads, self.head_dim = storage, scales, table, kv_heads, head_dim
-
-    def address(self) -> tuple:
-        """codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim"""
-        s, c, t = self.storage, self.scales, self.table
-        one = s.shape[0] == 1
-        return (s.data_ptr(), c.data_ptr(), t.data_ptr(), 2 * self.kv_heads * PAGE_TOKENS * self.head_dim if one else s.stride(0),
-                2 * self.kv_heads if one else c.stride(0), t.stride(0), t.shape[1], t.shape[0], self.kv_heads, self.head_dim)
+        one = storage.shape[0] == 1   # codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim
+        self.place = (storage.data_ptr(), scales.data_ptr(), table.data_ptr(), 2 * page if one else storage.stride(0), 2 * kv_heads if one else scales.stride(0),
+                      table.stride(0), table.shape[1], table.shape[0], kv_heads, head_dim)
 
 
 _SITE = (_P, _P, _P, _LL, _LL, _I, _I, _I, _I, _I)
@@ -72,6 +70,11 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     to 2^119), and no less than it has if it held rows before the new ones; those rows' codes are then rounded to the larger unit. Rounding is
     to nearest even, once, from float32. Infinities become +-448, NaN stays. Rows behind the new ones stay as they are; a padding
     entry (slot -1) writes its queries only, as does every entry with `write_cache` false."""
+    if qkv.is_cuda:
+        code = _native("rope_cache_write_e4m3", "cache_e4m3")(qkv, bias, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, err, site.storage, site.place, rot_dim,
+                                                              n_heads, write_cache, max_q_len)
+        if code is not None:
+            return _check(code, "rope_cache_write_e4m3")
     dtype = qkv.dtype
     is_bf16 = kernels._is_bf16(dtype)
     kernels._rows("qkv", qkv)
@@ -99,7 +102,7 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
         return
     _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _P, _P)(
         is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
-        n_heads, q_out.data_ptr(), *site.address(), bool(write_cache), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
+        n_heads, q_out.data_ptr(), *site.place, bool(write_cache), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
 
 
 def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_seqs: int, max_kv_len: int,
@@ -108,6 +111,10 @@ def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor
     page numbers of the cache, so that its page table serves both. Of entry s the rows up to its last new token's, from the first that a
     window of `window` positions (0: all) leaves its first one; every other row of `out` stays as it is. `max_kv_len`: an upper bound of any
     sequence's length."""
+    if out.is_cuda:
+        code = _native("cache_read_e4m3", "cache_e4m3")(out, cu_q, tok_pos, slots, err, site.storage, site.place, n_seqs, max_kv_len, window)
+        if code is not None:
+            return _check(code, "cache_read_e4m3")
     is_bf16 = kernels._is_bf16(out.dtype)
     _dev("out", out, contiguous=False)
     _batch("cache_read_e4m3", cu_q, tok_pos, slots, err)
@@ -124,7 +131,7 @@ def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor
     pages = min(-(-int(max_kv_len) // PAGE_TOKENS), site.table.shape[1])
     _check(_function("cache_e4m3", "qf_cache_read_e4m3", _I, _P, _LL, _P, _P, _P, *_SITE, _I, _I, _I, _P, _P)(
         is_bf16, out.data_ptr(), 2 * kv_heads * PAGE_TOKENS * d if out.shape[0] == 1 else out.stride(0), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(),
-        *site.address(), n_seqs, pages, window, err.data_ptr(), _stream()), "cache_read_e4m3")
+        *site.place, n_seqs, pages, window, err.data_ptr(), _stream()), "cache_read_e4m3")
 
 
 def attention_e4m3_pays(max_q_len: int, group: int) -> bool:
@@ -172,6 +179,11 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     (window 0: all up to p). Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at consecutive positions, at most max_q_len; an entry may have none, and a
     padding entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page
     table has room for)."""
+    if q.is_cuda:
+        code = _native("attention_e4m3", "attention_e4m3")(q, out, cu_q, tok_pos, slots, err, site.storage, site.place, scratch.part_o, scratch.part_ml, scratch.tickets,
+                                                           n_heads, n_seqs, max_q_len, scale, window, 1 << 40 if max_kv_len is None else max_kv_len)
+        if code is not None:
+            return _check(code, "attention_e4m3")
     dtype, d, kv_heads = q.dtype, site.head_dim, site.kv_heads
     is_bf16 = kernels._is_bf16(dtype)
     _dev("q", q)
@@ -202,5 +214,5 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     scratch.ensure(blocks, d, block_rows)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
     _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P)(
-        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.address(), n_heads, n_seqs,
+        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.place, n_heads, n_seqs,
         max_q_len == 1 and q.shape[0] == n_seqs, block_rows, chunks, most, blocks, block_slots, scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")

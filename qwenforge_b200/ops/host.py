@@ -20,6 +20,7 @@ _ENTRIES = {"norm": ("qf_add_rms_norm",),
             "tc_gemm": ("qf_tc_gemm_qkv_pairs_pays", "qf_tc_gemm_qkv_pairs", "qf_tc_gemm_is_persistent", "qf_tc_gemm", "qf_tc_gemm_tail"),
             "attention_prefill_tc": ("qf_attention_prefill_tc_ex",), "rope_cache": ("qf_rope_cache_write",), "activation": ("qf_swiglu",), "recurrent": ("qf_stabilized_gates", "qf_gated_group_norm", "qf_causal_conv"),
             "state_chunks": ("qf_state_chunks",), "row_chunks": ("qf_row_chunks",), "attention_shared": ("qf_attention_shared",),
+            "cache_e4m3": ("qf_rope_cache_write_e4m3", "qf_cache_read_e4m3"), "attention_e4m3": ("qf_attention_e4m3", "qf_attention_e4m3_slots"),
             "verify_drafts": ("qf_verify_drafts",), "page_copy": ("qf_copy_pages",)}
 _known: set = set()   # libraries whose entries the module has been told
 _module = None
