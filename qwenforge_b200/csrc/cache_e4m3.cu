@@ -1,8 +1,7 @@
 // Writing a sequence cache of e4m3 codes, and reading it back (the format: e4m3.cuh).
 //
 // ---- Write, behind the q/k/v projection of a step's tokens: x = row + bias; queries and keys rotated (split halves over the first R
-// components, as rope_cache.cu; the product position * frequency with its rounding error, so that an angle of tens of thousands is
-// as exact as a small one); queries written out. For every page that gets new rows, of each plane and kv head:
+// components, as rope_cache.cu, with angles that are as exact at position 30,000 as at 3); queries written out. For every page that gets new rows, of each plane and kv head:
 //   amax = max |x| over the new rows' finite elements,  e = the least exponent with amax <= 448 * 2^e
 //   the page had rows before (the first new one does not begin it): e = max(e, e_old), and where that is more than e_old, those
 //   rows' codes become round(code * 2^(e_old - e))
@@ -79,111 +78,158 @@ __device__ __forceinline__ void rescale_codes(uint4* codes, int pieces, float by
     }
 }
 
+// Cosine and sine of position * frequency. The angle is taken in turns, position * (frequency / 2 pi) with both factors' rounding errors, so that whole
+// turns fall away exactly and an angle of tens of thousands is as good as a small one.
+struct Turns {
+    float most, rest;   // frequency / 2 pi, in two parts
+    __device__ __forceinline__ explicit Turns(float frequency) {
+        const float inv = 0.15915494f, inv_rest = 6.42063824e-09f;   // 1 / 2 pi, in two parts
+        most = frequency * inv;
+        rest = fmaf(frequency, inv, -most) + frequency * inv_rest;
+    }
+    __device__ __forceinline__ float2 at(float position) const {
+        const float whole = rintf(position * most), part = fmaf(position, rest, fmaf(position, most, -whole));
+        float s, c;
+        sincospif(2.f * part, &s, &c);
+        return make_float2(c, s);
+    }
+};
+
+// A run: the rows from token t on, of entry seq, that one page gets.
+struct NewRows {
+    int t, seq, rows, first_pos;
+};
+// The number-th run of a step. `single`: an entry's tokens are one (or none), and every token is a run.
+__device__ __forceinline__ bool run_of(int number, int single, int n_seqs, const int* cu_q, const int* tok_seq, const int* tok_pos, NewRows& r) {
+    if (single) {
+        r = NewRows{number, tok_seq[number], 1, tok_pos[number]};
+        return true;
+    }
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0, before = 0; s0 < n_seqs; s0 += 32) {
+        int begin = 0, count = 0, first = 0, runs = 0;
+        if (s0 + lane < n_seqs) {
+            begin = cu_q[s0 + lane];
+            count = cu_q[s0 + lane + 1] - begin;
+            if (count > 0) {
+                first = tok_pos[begin];
+                runs = (first + count - 1) / QF_PAGE - first / QF_PAGE + 1;
+            }
+        }
+        int upto = runs;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t beyond = __ballot_sync(0xffffffffu, before + upto > number);
+        if (beyond) {
+            const int who = __ffs(beyond) - 1, k = number - before - __shfl_sync(0xffffffffu, upto - runs, who);
+            begin = __shfl_sync(0xffffffffu, begin, who), count = __shfl_sync(0xffffffffu, count, who), first = __shfl_sync(0xffffffffu, first, who);
+            const int from = k == 0 ? 0 : (first / QF_PAGE + k) * QF_PAGE - first;   // tokens of the entry before the run
+            r = NewRows{begin + from, s0 + who, min(count - from, QF_PAGE - (first + from) % QF_PAGE), first + from};
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(EW_WARPS * 32)
 write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
-                  const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
-                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_tokens, int share, int most_rows, int* err) {
+                 const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
+                 T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int single, int most_rows, int* err) {
     grid_chain_entry();
     extern __shared__ float2 turn[];   // [rows of a run][rot_dim / 2] cosine, sine
     const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2, pass = D - rot_dim;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int heads = n_heads + 2 * KVH;
     const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
-    const int t_begin = blockIdx.x * share, t_end = min(t_begin + share, n_tokens);
-    for (int t = t_begin; t < t_end; ++t) {
-        const int seq = tok_seq[t], first_pos = tok_pos[t];
-        if (t != cu_q[seq] && first_pos % QF_PAGE != 0) continue;   // (the run began at an earlier token)
-        const int slot = write_cache ? slots[seq] : -1, at = first_pos % QF_PAGE;
-        int rows = min(cu_q[seq + 1] - t, QF_PAGE - at);
-        if (rows > most_rows) {   // (an entry longer than the call has said: there is no room for its angles)
-            if (threadIdx.x == 0) atomicOr(err, QF_ERR_ROW_RANGE);
-            rows = most_rows;
-        }
-        const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
-        if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
-            const float p = (float)(first_pos + i / half), f = inv_freq[i % half];
-            const float angle = p * f, rest = fmaf(p, f, -angle);
-            float s, c;
-            sincosf(angle, &s, &c);
-            turn[i] = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
-        }
-        __syncthreads();
-        for (int h = h_begin + warp; h < h_end; h += EW_WARPS) {
-            const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
-            if (!is_q && page < 0) continue;
-            const int plane = is_v ? 1 : 0, kvh = is_v ? h - n_heads - KVH : h - n_heads;
-            const T* src = qkv + (long long)t * qkv_stride + (long long)h * D;
-            const T* b = bias ? bias + (long long)h * D : nullptr;
-            unsigned char* codes = is_q ? nullptr : site.codes + (long long)page * site.page_bytes + (long long)(plane * KVH + kvh) * QF_PAGE * D;
-            T* q_dst = q_out + (long long)t * n_heads * D + (long long)h * D;
-            const int turned = is_v ? 0 : half / VEC, plain = is_v ? D / VEC : pass / VEC, plain0 = is_v ? 0 : rot_dim;
-            // one item: VEC pairs of the rotation of a row, then VEC components that pass through
-            auto pairs_of = [&](int i, int& row, int& j, float (&a)[VEC], float (&z)[VEC]) {
-                row = i / turned, j = (i % turned) * VEC;
-                const T* x = src + (long long)row * qkv_stride;
-                float x1[VEC], x2[VEC];
-                load_values<T, VEC>(x + j, b ? b + j : nullptr, x1);
-                load_values<T, VEC>(x + j + half, b ? b + j + half : nullptr, x2);
+    NewRows run;
+    if (!run_of(blockIdx.x, single, n_seqs, cu_q, tok_seq, tok_pos, run)) return;
+    const int t = run.t, first_pos = run.first_pos, at = first_pos % QF_PAGE, slot = write_cache ? slots[run.seq] : -1;
+    int rows = run.rows;
+    if (rows > most_rows || (single && cu_q[run.seq + 1] - cu_q[run.seq] > 1)) {   // (an entry longer than the call has said: there is no room for its angles)
+        if (threadIdx.x == 0) atomicOr(err, QF_ERR_ROW_RANGE);
+        rows = min(rows, most_rows);
+    }
+    const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
+    if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
+    for (int i = threadIdx.x; i < rows * half; i += blockDim.x) turn[i] = Turns(inv_freq[i % half]).at((float)(first_pos + i / half));
+    __syncthreads();
+    for (int h = h_begin + warp; h < h_end; h += EW_WARPS) {
+        const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
+        if (!is_q && page < 0) continue;
+        const int plane = is_v ? 1 : 0, kvh = is_v ? h - n_heads - KVH : h - n_heads;
+        const T* src = qkv + (long long)t * qkv_stride + (long long)h * D;
+        const T* b = bias ? bias + (long long)h * D : nullptr;
+        unsigned char* codes = is_q ? nullptr : site.codes + (long long)page * site.page_bytes + (long long)(plane * KVH + kvh) * QF_PAGE * D;
+        T* q_dst = q_out + (long long)t * n_heads * D + (long long)h * D;
+        const int turned = is_v ? 0 : half / VEC, plain = is_v ? D / VEC : pass / VEC, plain0 = is_v ? 0 : rot_dim;
+        // one item: VEC pairs of the rotation of a row, then VEC components that pass through
+        auto pairs_of = [&](int i, int& row, int& j, float (&a)[VEC], float (&z)[VEC]) {
+            row = i / turned, j = (i % turned) * VEC;
+            const T* x = src + (long long)row * qkv_stride;
+            float x1[VEC], x2[VEC];
+            load_values<T, VEC>(x + j, b ? b + j : nullptr, x1);
+            load_values<T, VEC>(x + j + half, b ? b + j + half : nullptr, x2);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float2 cs = turn[row * half + j + e];
-                    a[e] = x1[e] * cs.x - x2[e] * cs.y;
-                    z[e] = x2[e] * cs.x + x1[e] * cs.y;
-                }
-            };
-            auto plain_of = [&](int i, int& row, int& j, float (&a)[VEC]) {
-                row = i / plain, j = plain0 + (i % plain) * VEC;
-                load_values<T, VEC>(src + (long long)row * qkv_stride + j, b ? b + j : nullptr, a);
-            };
-            int row, j;
-            float a[VEC], z[VEC];
-            if (is_q) {
-                for (int i = lane; i < rows * turned; i += 32) {
-                    pairs_of(i, row, j, a, z);
-                    store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j, a);
-                    store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j + half, z);
-                }
-                for (int i = lane; i < rows * plain; i += 32) {
-                    plain_of(i, row, j, a);
-                    store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j, a);
-                }
-                continue;
+            for (int e = 0; e < VEC; ++e) {
+                const float2 cs = turn[row * half + j + e];
+                a[e] = x1[e] * cs.x - x2[e] * cs.y;
+                z[e] = x2[e] * cs.x + x1[e] * cs.y;
             }
-            float amax = 0.f;
+        };
+        auto plain_of = [&](int i, int& row, int& j, float (&a)[VEC]) {
+            row = i / plain, j = plain0 + (i % plain) * VEC;
+            load_values<T, VEC>(src + (long long)row * qkv_stride + j, b ? b + j : nullptr, a);
+        };
+        int row, j;
+        float a[VEC], z[VEC];
+        if (is_q) {
             for (int i = lane; i < rows * turned; i += 32) {
                 pairs_of(i, row, j, a, z);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, fmaxf(finite_size(a[e]), finite_size(z[e])));
+                store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j, a);
+                store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j + half, z);
             }
             for (int i = lane; i < rows * plain; i += 32) {
                 plain_of(i, row, j, a);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, finite_size(a[e]));
+                store_values<T, VEC>(q_dst + (long long)row * n_heads * D + j, a);
             }
-            float* scale = site.scales + (long long)page * site.page_scales + plane * KVH + kvh;
-            int exp = e4m3_exponent(warp_max(amax));
-            if (at > 0) {
-                const int before = exponent_of(*scale);
-                exp = max(exp, before);
-                if (exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), lane, 32);
-            }
-            const float by = pow2(-exp);
-            codes += at * D;
-            for (int i = lane; i < rows * turned; i += 32) {
-                pairs_of(i, row, j, a, z);
-                store_codes<VEC>(codes + row * D + j, a, by);
-                store_codes<VEC>(codes + row * D + j + half, z, by);
-            }
-            for (int i = lane; i < rows * plain; i += 32) {
-                plain_of(i, row, j, a);
-                store_codes<VEC>(codes + row * D + j, a, by);
-            }
-            __syncwarp();   // (every lane has read the old scale)
-            if (lane == 0) *scale = pow2(exp);
+            continue;
         }
+        float amax = 0.f;
+        for (int i = lane; i < rows * turned; i += 32) {
+            pairs_of(i, row, j, a, z);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, fmaxf(finite_size(a[e]), finite_size(z[e])));
+        }
+        for (int i = lane; i < rows * plain; i += 32) {
+            plain_of(i, row, j, a);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, finite_size(a[e]));
+        }
+        float* scale = site.scales + (long long)page * site.page_scales + plane * KVH + kvh;
+        int exp = e4m3_exponent(warp_max(amax));
+        if (at > 0) {
+            const int before = exponent_of(*scale);
+            exp = max(exp, before);
+            if (exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), lane, 32);
+        }
+        const float by = pow2(-exp);
+        codes += at * D;
+        for (int i = lane; i < rows * turned; i += 32) {
+            pairs_of(i, row, j, a, z);
+            store_codes<VEC>(codes + row * D + j, a, by);
+            store_codes<VEC>(codes + row * D + j + half, z, by);
+        }
+        for (int i = lane; i < rows * plain; i += 32) {
+            plain_of(i, row, j, a);
+            store_codes<VEC>(codes + row * D + j, a, by);
+        }
+        __syncwarp();   // (every lane has read the old scale)
+        if (lane == 0) *scale = pow2(exp);
     }
 }
 
@@ -194,129 +240,129 @@ template <typename T>
 __global__ void __launch_bounds__(EW_THREADS, 2)
 write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                   const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
-                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_tokens, int* err) {
+                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int* err) {
     grid_chain_entry();
-    constexpr int RAW = 16 * sizeof(T) / 16;   // 16-byte words of a piece: eight elements here, eight there
+    constexpr int WORDS = 8 * sizeof(T) / 16;   // of 16 bytes, of eight elements
     __shared__ float amax_s[2][EW_THREADS / 32];
-    const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2, groups = D / 16;
+    const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2;
+    const unsigned groups = D / 16;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = n_heads + 2 * KVH;
     const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
-    const int t0 = blockIdx.x * QF_PAGE;
-    int parity = 0;
-    for (int part = 0; part < QF_PAGE; part += 32) {
-        // tokens at which a run begins
-        bool begins = false;
-        if (t0 + part + lane < n_tokens) begins = tok_pos[t0 + part + lane] % QF_PAGE == 0 || t0 + part + lane == cu_q[tok_seq[t0 + part + lane]];
-        for (uint32_t left = __ballot_sync(0xffffffffu, begins); left; left &= left - 1) {
-            const int t = t0 + part + __ffs(left) - 1, seq = tok_seq[t], first_pos = tok_pos[t], at = first_pos % QF_PAGE;
-            const int slot = write_cache ? slots[seq] : -1, rows = min(cu_q[seq + 1] - t, QF_PAGE - at);
-            const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
-            if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
-            // this thread's pieces: a row, the places of its two eights in a head, and their turn
-            int row[EW_PIECES], a_at[EW_PIECES], b_at[EW_PIECES];
-            bool turns[EW_PIECES];
-            float cosine[EW_PIECES][8], sine[EW_PIECES][8];
+    NewRows run;
+    if (h_begin >= h_end || !run_of(blockIdx.x, 0, n_seqs, cu_q, tok_seq, tok_pos, run)) return;
+    const int at = run.first_pos % QF_PAGE, rows = run.rows, slot = write_cache ? slots[run.seq] : -1;
+    const int page = slot >= 0 ? e4m3_page(site, slot, run.first_pos) : -1;
+    if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
+    // this thread's pieces: a row, the places of its two eights in a head, and their turn
+    bool mine[EW_PIECES], turns[EW_PIECES];
+    int a_at[EW_PIECES], b_off[EW_PIECES], code_at[EW_PIECES];
+    const T* src[EW_PIECES];
+    T* dst[EW_PIECES];
+    float2 turn[EW_PIECES][8];
+    uint4 raw[EW_PIECES][2][WORDS];
+    auto load = [&]() {   // the next head
 #pragma unroll
-            for (int k = 0; k < EW_PIECES; ++k) {
-                const unsigned i = threadIdx.x + k * EW_THREADS, g = i % (unsigned)groups;
-                row[k] = i / (unsigned)groups;
-                turns[k] = 8 * (int)g < half;
-                a_at[k] = turns[k] ? 8 * g : 16 * g;   // (rot_dim + 16 (g - half / 8) behind the rotated part)
-                b_at[k] = turns[k] ? 8 * g + half : 16 * g + 8;
-                if (row[k] < rows && turns[k]) {
-                    const float p = (float)(first_pos + row[k]);
+        for (int k = 0; k < EW_PIECES; ++k)
+            if (mine[k]) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float f = inv_freq[8 * g + e], angle = p * f, rest = fmaf(p, f, -angle);
-                        float s, c;
-                        sincosf(angle, &s, &c);
-                        cosine[k][e] = fmaf(-s, rest, c);
-                        sine[k][e] = fmaf(c, rest, s);
-                    }
+                for (int i = 0; i < WORDS; ++i) {
+                    raw[k][0][i] = reinterpret_cast<const uint4*>(src[k])[i];
+                    raw[k][1][i] = reinterpret_cast<const uint4*>(src[k] + b_off[k])[i];
                 }
+                src[k] += D;
             }
-            uint4 raw[EW_PIECES][RAW];
-            auto load = [&](int h) {
+    };
 #pragma unroll
-                for (int k = 0; k < EW_PIECES; ++k)
-                    if (row[k] < rows) {
-                        const T* src = qkv + (long long)(t + row[k]) * qkv_stride + (long long)h * D;
+    for (int k = 0; k < EW_PIECES; ++k) {
+        const unsigned i = threadIdx.x + k * EW_THREADS;
+        const int g = i % groups, row = i / groups;
+        mine[k] = row < rows;
+        turns[k] = 8 * g < half;
+        a_at[k] = turns[k] ? 8 * g : 16 * g;   // (behind the rotated part: rot_dim + 16 (g - half / 8), and the eight behind that)
+        b_off[k] = turns[k] ? half : 8;
+        code_at[k] = (at + row) * D + a_at[k];
+        src[k] = qkv + (long long)(run.t + row) * qkv_stride + h_begin * D + a_at[k];
+        dst[k] = q_out + ((long long)(run.t + row) * n_heads + h_begin) * D + a_at[k];
+    }
+    load();
 #pragma unroll
-                        for (int i = 0; i < RAW / 2; ++i) {
-                            raw[k][i] = reinterpret_cast<const uint4*>(src + a_at[k])[i];
-                            raw[k][RAW / 2 + i] = reinterpret_cast<const uint4*>(src + b_at[k])[i];
-                        }
-                    }
-            };
-            if (h_begin < h_end) load(h_begin);
-            for (int h = h_begin; h < h_end; ++h) {
-                const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
-                const int kvh = is_v ? h - n_heads - KVH : h - n_heads;
-                float x[EW_PIECES][16], amax = 0.f;
+    for (int k = 0; k < EW_PIECES; ++k)
+        if (mine[k] && turns[k]) {
+            const float position = (float)(run.first_pos + (int)((threadIdx.x + k * EW_THREADS) / groups));
 #pragma unroll
-                for (int k = 0; k < EW_PIECES; ++k) {
-                    if (row[k] >= rows) continue;
-                    const T* v = reinterpret_cast<const T*>(raw[k]);
+            for (int e = 0; e < 8; ++e) turn[k][e] = Turns(inv_freq[a_at[k] + e]).at(position);
+        }
+    int parity = 0;
+    for (int h = h_begin; h < h_end; ++h) {
+        const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
+        float x[EW_PIECES][2][8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[k][e] = Num<T>::to_f(v[e]);
-                    if (bias) {
-                        float b[8];
+        for (int k = 0; k < EW_PIECES; ++k) {
+            if (!mine[k]) continue;
 #pragma unroll
-                        for (int part16 = 0; part16 < 2; ++part16) {
-                            load_values<T, 8>(bias + (long long)h * D + (part16 ? b_at[k] : a_at[k]), nullptr, b);
+            for (int i = 0; i < 2; ++i) {
+                const T* v = reinterpret_cast<const T*>(raw[k][i]);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[k][8 * part16 + e] += b[e];
-                        }
-                    }
-                    if (!is_v && turns[k]) {
+                for (int e = 0; e < 8; ++e) x[k][i][e] = Num<T>::to_f(v[e]);
+                if (bias) {
+                    float b[8];
+                    load_values<T, 8>(bias + h * D + a_at[k] + i * b_off[k], nullptr, b);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float u = x[k][e], w = x[k][8 + e];
-                            x[k][e] = u * cosine[k][e] - w * sine[k][e];
-                            x[k][8 + e] = w * cosine[k][e] + u * sine[k][e];
-                        }
-                    }
+                    for (int e = 0; e < 8; ++e) x[k][i][e] += b[e];
                 }
-                if (h + 1 < h_end) load(h + 1);
-                if (is_q) {
-#pragma unroll
-                    for (int k = 0; k < EW_PIECES; ++k)
-                        if (row[k] < rows) {
-                            T* dst = q_out + ((long long)(t + row[k]) * n_heads + h) * D;
-                            store_values<T, 8>(dst + a_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][0]));
-                            store_values<T, 8>(dst + b_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][8]));
-                        }
-                    continue;
-                }
-                if (page < 0) continue;
-#pragma unroll
-                for (int k = 0; k < EW_PIECES; ++k)
-                    if (row[k] < rows) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_size(x[k][e]));
-                    }
-                float* scale = site.scales + (long long)page * site.page_scales + (is_v ? KVH : 0) + kvh;
-                const int before = at > 0 ? exponent_of(*scale) : E4M3_LOW;
-                amax = warp_max(amax);
-                if (lane == 0) amax_s[parity][warp] = amax;
-                __syncthreads();   // (every thread has read the old scale, too)
-#pragma unroll
-                for (int w = 0; w < EW_THREADS / 32; ++w) amax = fmaxf(amax, amax_s[parity][w]);
-                parity ^= 1;
-                const int exp = max(e4m3_exponent(amax), before);
-                unsigned char* codes = site.codes + (long long)page * site.page_bytes + (long long)((is_v ? KVH : 0) + kvh) * QF_PAGE * D;
-                if (at > 0 && exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), threadIdx.x, EW_THREADS);
-                const float by = pow2(-exp);
-#pragma unroll
-                for (int k = 0; k < EW_PIECES; ++k)
-                    if (row[k] < rows) {
-                        unsigned char* dst = codes + (at + row[k]) * D;
-                        store_codes<8>(dst + a_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][0]), by);
-                        store_codes<8>(dst + b_at[k], *reinterpret_cast<const float(*)[8]>(&x[k][8]), by);
-                    }
-                if (threadIdx.x == 0) *scale = pow2(exp);
             }
         }
+        if (h + 1 < h_end) load();
+        if (!is_v) {
+#pragma unroll
+            for (int k = 0; k < EW_PIECES; ++k)
+                if (mine[k] && turns[k]) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float u = x[k][0][e], w = x[k][1][e];
+                        x[k][0][e] = u * turn[k][e].x - w * turn[k][e].y;
+                        x[k][1][e] = w * turn[k][e].x + u * turn[k][e].y;
+                    }
+                }
+        }
+        if (is_q) {
+#pragma unroll
+            for (int k = 0; k < EW_PIECES; ++k)
+                if (mine[k]) {
+                    store_values<T, 8>(dst[k], x[k][0]);
+                    store_values<T, 8>(dst[k] + b_off[k], x[k][1]);
+                    dst[k] += D;
+                }
+            continue;
+        }
+        if (page < 0) continue;
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < EW_PIECES; ++k)
+            if (mine[k]) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(finite_size(x[k][0][e]), finite_size(x[k][1][e])));
+            }
+        const int place = h - n_heads;   // plane * kv heads + head
+        float* scale = site.scales + (long long)page * site.page_scales + place;
+        const int before = at > 0 ? exponent_of(*scale) : E4M3_LOW;
+        amax = warp_max(amax);
+        if (lane == 0) amax_s[parity][warp] = amax;
+        __syncthreads();   // (every thread has read the old scale, too)
+#pragma unroll
+        for (int w = 0; w < EW_THREADS / 32; ++w) amax = fmaxf(amax, amax_s[parity][w]);
+        parity ^= 1;
+        const int exp = max(e4m3_exponent(amax), before);
+        unsigned char* codes = site.codes + (long long)page * site.page_bytes + place * QF_PAGE * D;
+        if (at > 0 && exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), threadIdx.x, EW_THREADS);
+        const float by = pow2(-exp);
+#pragma unroll
+        for (int k = 0; k < EW_PIECES; ++k)
+            if (mine[k]) {
+                store_codes<8>(codes + code_at[k], x[k][0], by);
+                store_codes<8>(codes + code_at[k] + b_off[k], x[k][1], by);
+            }
+        if (threadIdx.x == 0) *scale = pow2(exp);
     }
 }
 
@@ -329,23 +375,24 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
 
 template <typename T>
 static int write_launch(const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq, const int* tok_pos, const int* slots,
-                        const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int write_cache, int n_tokens, int max_q_len, int* err,
-                        cudaStream_t stream) {
-    const int heads = n_heads + 2 * site.kv_heads, slices = (heads + EW_WARPS - 1) / EW_WARPS;
-    const int share = max_q_len > 1 ? 16 : 1;
-    const int most_rows = max_q_len < QF_PAGE ? max_q_len : QF_PAGE;
-    const size_t smem = (size_t)most_rows * (rot_dim / 2) * sizeof(float2);
+                        const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int write_cache, int n_tokens, int n_seqs, int max_q_len,
+                        int* err, cudaStream_t stream) {
+    const int heads = n_heads + 2 * site.kv_heads, single = max_q_len == 1;
+    // runs: an entry of n tokens has n / 64 + 2 at the most
+    const long long most_runs = n_tokens / QF_PAGE + 2ll * n_seqs;
+    const int runs = single || most_runs > n_tokens ? n_tokens : (int)most_runs;
     const bool wide = rot_dim % 16 == 0 && qkv_stride % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias) % 16 == 0;
     if (wide && max_q_len >= EW_LONG) {
-        const int pieces = (heads + EW_HEADS - 1) / EW_HEADS;
-        return (int)launch_pdl(write_runs_kernel<T>, dim3((n_tokens + QF_PAGE - 1) / QF_PAGE, pieces), dim3(EW_THREADS), 0, stream, (const T*)qkv, (const T*)bias, qkv_stride,
-                               cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, err);
+        return (int)launch_pdl(write_runs_kernel<T>, dim3(runs, (heads + EW_HEADS - 1) / EW_HEADS), dim3(EW_THREADS), 0, stream, (const T*)qkv, (const T*)bias, qkv_stride,
+                               cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, err);
     }
-    const dim3 grid((n_tokens + share - 1) / share, slices);
-    return (int)(wide ? launch_pdl(write_any_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
-                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err)
-                      : launch_pdl(write_any_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq,
-                                   tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_tokens, share, most_rows, err));
+    const int most_rows = max_q_len < QF_PAGE ? max_q_len : QF_PAGE;
+    const size_t smem = (size_t)most_rows * (rot_dim / 2) * sizeof(float2);
+    const dim3 grid(runs, (heads + EW_WARPS - 1) / EW_WARPS);
+    return (int)(wide ? launch_pdl(write_any_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos,
+                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, err)
+                      : launch_pdl(write_any_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos,
+                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, err));
 }
 
 static bool site_fits(const E4m3Site& s) {
@@ -358,13 +405,13 @@ static bool site_fits(const E4m3Site& s) {
 QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq,
                                        const int* tok_pos, const int* slots, const float* inv_freq, int rot_dim, int n_heads, void* q_out, void* codes,
                                        float* scales, const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots,
-                                       int kv_heads, int head_dim, int write_cache, int n_tokens, int max_q_len, int* err, cudaStream_t stream) {
+                                       int kv_heads, int head_dim, int write_cache, int n_tokens, int n_seqs, int max_q_len, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (!inv_freq) rot_dim = 0;
     if (!site_fits(site) || head_dim > 128 || rot_dim < 0 || rot_dim > head_dim || (rot_dim & 1) || n_heads <= 0 || max_q_len <= 0) return (int)cudaErrorInvalidValue;
     if (n_tokens <= 0) return 0;
-    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, max_q_len, err, stream)
-                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, max_q_len, err, stream);
+    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, err, stream)
+                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, err, stream);
 }
 
 // ---- Read back: the rows that a batch's sequences hold (from the first that a window of `window` positions leaves the first new token, 0:

@@ -56,7 +56,7 @@ int (*copy_pages)(void*, int, int, int, long long, long long, int, long long, lo
 int (*verify_drafts)(const float*, int, int, long long, const float*, long long, const int*, int, const int*, int, const float*, float, unsigned long long,
                      unsigned long long, const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
 int (*write_e4m3)(int, const void*, const void*, long long, const int*, const int*, const int*, const int*, const float*, int, int, void*, void*, float*,
-                  const int*, long long, long long, int, int, int, int, int, int, int, int, int*, Stream);
+                  const int*, long long, long long, int, int, int, int, int, int, int, int, int, int*, Stream);
 int (*read_e4m3)(int, void*, long long, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int, int,
                  int, int*, Stream);
 int (*attention_e4m3_slots)(int, int, int);
@@ -550,7 +550,7 @@ PyObject* e4m3_written(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return code_of([&] {
         return write_e4m3(type == at::kBFloat16, qkv->data_ptr(), bias ? bias->data_ptr() : nullptr, qkv->stride(0), ints(cu), ints(seq), ints(pos), ints(slots),
                           freq ? freq->const_data_ptr<float>() : nullptr, (int)rot, (int)heads, q->data_ptr(), p.codes, p.scales, p.table, p.page_bytes, p.page_scales,
-                          p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, writes != 0, (int)rows, (int)most, at_ptr<int>(*err), stream());
+                          p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, writes != 0, (int)rows, (int)slots->numel(), (int)most, at_ptr<int>(*err), stream());
     });
     END_HANDLE_TH_ERRORS
 }

@@ -100,9 +100,9 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     _here("rope_cache_write_e4m3", qkv, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, site.storage, site.scales, site.table, err, bias)
     if n == 0:
         return
-    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _P, _P)(
+    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _I, _P, _P)(
         is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
-        n_heads, q_out.data_ptr(), *site.place, bool(write_cache), n, max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
+        n_heads, q_out.data_ptr(), *site.place, bool(write_cache), n, slots.numel(), max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
 
 
 def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_seqs: int, max_kv_len: int,
