@@ -32,6 +32,9 @@
 #include "e4m3.cuh"
 
 #define EA_WARPS 4
+#ifndef EA_USE_CLUSTERS
+#define EA_USE_CLUSTERS 1
+#endif
 #define EA_DEAD 0x7fffffff   // the exponent of a tile that is not there, or that no row sees
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 
@@ -138,33 +141,35 @@ template <typename T, int D, int NR> struct Shape {
     static constexpr int ROWS = 8 * NR;
     static constexpr int TILE = D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
     static constexpr int BLOCKS = 2;                                  // of an SM
-    static constexpr int STAGES = 3;                                  // tiles of a warp in shared memory: one at work, the others on their way
+    static constexpr int STAGES = D <= 64 ? 2 : 3;                                  // tiles of a warp in shared memory: one at work, the others on their way
     static constexpr int PITCH = D / 16 % 2 ? D : D + 16;             // bytes of a staged row: an odd number of 16, so that eight rows meet all banks
     static constexpr int STAGE = 2 * TILE * PITCH;                    // keys, then values
     static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result: items of four
     static constexpr int LD = PART + 4;                               // and where warps leave theirs: rows four banks apart
-    static constexpr int SMEM = EA_WARPS * (STAGES * STAGE > ROWS * LD * 4 ? STAGES * STAGE : ROWS * LD * 4);   // (the outputs take the tiles' place)
+    // (the outputs, the warps' and the block's with its maxima and sums, take the tiles' place)
+    static constexpr int OUTPUTS = (EA_WARPS + 1) * ROWS * LD * 4 + ROWS * 8, TILES = EA_WARPS * STAGES * STAGE, SMEM = TILES > OUTPUTS ? TILES : OUTPUTS;
     static constexpr int SHARE = EA_WARPS * 32 / ROWS;                // lanes that join a row's maxima and sums
 };
 
 struct AttendArgs {
     const int *cu_q, *tok_pos, *slots;
     E4m3Site site;
-    int n_heads, n_seqs, single, chunks, most_pages, block_slots, window;
+    int n_heads, group, n_seqs, single, chunks, most_pages, block_slots, window, cluster;   // group: query heads of a kv head
     float scale_log2;
     float *part_o, *part_ml;   // [2 * blocks][ROWS][PART], [2 * blocks][ROWS][2]
     int *tickets, *err;        // [4 * blocks]
 };
 
 struct Sequence {
-    int slot, begin, tokens, first_pos, last_pos, page0, pages;
+    int slot, begin, tokens, first_pos, last_pos, page0, pages, pairs;   // pairs: kv heads times blocks of rows
 };
-__device__ __forceinline__ Sequence sequence_of(const AttendArgs& a, int s) {
+template <int ROWS> __device__ __forceinline__ Sequence sequence_of(const AttendArgs& a, int s) {
     Sequence r;
     r.begin = a.single ? s : a.cu_q[s];   // (single: every entry has one token)
     r.tokens = a.single ? 1 : a.cu_q[s + 1] - r.begin;
     r.slot = r.tokens > 0 ? a.slots[s] : -1;
     r.first_pos = r.last_pos = r.page0 = r.pages = 0;
+    r.pairs = a.site.kv_heads * (a.single ? a.chunks : min(a.chunks, (int)((unsigned)(r.tokens * a.group + ROWS - 1) / ROWS)));
     if (r.tokens > 0) {
         r.first_pos = a.tok_pos[r.begin];
         r.last_pos = a.single ? r.first_pos : a.tok_pos[r.begin + r.tokens - 1];
@@ -186,7 +191,7 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     }
 }
 
-#define EA_PAIR_COST 8     // pages whose time a pair's beginning and end take
+#define EA_PAIR_COST 14    // pages whose time a pair's beginning and end take
 #define EA_GROUP 16        // partial results that a block joins at once
 #define EA_MOST_GROUPS 64  // ... and groups of them: enough for 1,024 blocks
 
@@ -194,7 +199,7 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
 __device__ __forceinline__ int place_in(int pair_begin, int block, int target) { return 2 * block + (pair_begin > block * target ? 1 : 0); }
 // Element 0 of the query (and output) of row i (token * group + head of the group) of the kv head kvh.
 template <int D> __device__ __forceinline__ long long row_offset(const AttendArgs& a, int begin, int kvh, int i) {
-    const int G = a.n_heads / a.site.kv_heads, token = a.single ? 0 : i / G;
+    const int G = a.group, token = a.single ? 0 : i / G;
     return (long long)(begin + token) * a.n_heads * D + (long long)(kvh * G + i - token * G) * D;
 }
 // Item i of a row, four neighbouring components (two of a part of 16), to its row of the output.
@@ -260,6 +265,117 @@ __device__ __forceinline__ void join_parts(T* out, const AttendArgs& a, const Pa
     }
 }
 
+// Thread-block clusters: all threads of all blocks arrive (what they wrote is then seen by whoever has waited) and wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Shared memory of block `rank` of the cluster at the place that is `at` in this one's.
+__device__ __forceinline__ uint32_t of_rank(const void* at, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(at)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 remote4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float2 remote2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
+}
+#define EA_CLUSTER 8   // blocks of a cluster
+// The end of a pair whose runs are clusters: a block puts its warps' results together, the cluster its blocks', each block an eighth of the items; of
+// several clusters the last one to leave an eighth joins that. No result takes the way through memory where one cluster has the pair.
+template <typename T, int D, int NR>
+__device__ __forceinline__ void join_cluster(T* out, const AttendArgs& a, float* shared_o, const float* m_s, const float* l_s, int items, int row0, int token0, int kvh,
+                                             int rank, int first, int run, int runs, int* ticket_s) {
+    using S = Shape<T, D, NR>;
+    constexpr int VW = Parts<D>::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS, THREADS = EA_WARPS * 32;
+    float* block_o = shared_o + EA_WARPS * ROWS * LD;   // [rows][LD], behind the warps' own; then maxima and sums
+    float2* block_ml = reinterpret_cast<float2*>(block_o + ROWS * LD);
+    for (int i = threadIdx.x; i < items; i += THREADS) {
+        const int row = i / (VW * 8), at = row * LD + i % (VW * 8) * 4;
+        float m = EA_NONE, l = 0.f, part[EA_WARPS];
+#pragma unroll
+        for (int k = 0; k < EA_WARPS; ++k) m = fmaxf(m, m_s[k * ROWS + row]);
+#pragma unroll
+        for (int k = 0; k < EA_WARPS; ++k) l += part[k] = fast_exp2(m_s[k * ROWS + row] - m) * l_s[k * ROWS + row];
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < EA_WARPS; ++k) {
+            const float f = part[k] * inv;
+            const float4 x = *reinterpret_cast<const float4*>(&shared_o[k * ROWS * LD + at]);
+            v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+        }
+        *reinterpret_cast<float4*>(block_o + at) = v;
+        if (i % (VW * 8) == 0) block_ml[row] = make_float2(m, l);
+    }
+    cluster_arrive();
+    cluster_wait();
+    const int each = (items + EA_CLUSTER - 1) / EA_CLUSTER, begin = rank * each, end = min(begin + each, items);
+    // one of `count` results to the others: their maxima and sums, their items
+    auto join = [&](int count, auto ml_of, auto item_of, float2& ml) {
+        float2 x[16];
+        float4 y[16], v = make_float4(0.f, 0.f, 0.f, 0.f);
+        ml = make_float2(EA_NONE, 0.f);
+        for (int k0 = 0; k0 < count; k0 += 16) {   // (an eighth of a sequence's page table: more than sixteen from 32,768 positions on)
+            float m = ml.x;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (k0 + k < count) x[k] = ml_of(k0 + k), y[k] = item_of(k0 + k), m = fmaxf(m, x[k].x);
+            const float old = fast_exp2(ml.x - m) * ml.y;
+            float l = old;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (k0 + k < count) l += x[k].y = fast_exp2(x[k].x - m) * x[k].y;
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            const float f0 = old * inv;
+            v.x *= f0, v.y *= f0, v.z *= f0, v.w *= f0;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (k0 + k < count) {
+                    const float f = x[k].y * inv;
+                    v.x = fmaf(f, y[k].x, v.x), v.y = fmaf(f, y[k].y, v.y), v.z = fmaf(f, y[k].z, v.z), v.w = fmaf(f, y[k].w, v.w);
+                }
+            ml = make_float2(m, l);
+        }
+        return v;
+    };
+    auto to_out = [&](const float4& v, int i) { give_out<T, D>(out + row_offset<D>(a, token0, kvh, row0 + i / (VW * 8)), v, i % (VW * 8)); };
+    for (int i = begin + threadIdx.x; i < end; i += THREADS) {
+        const int row = i / (VW * 8), at = row * LD + i % (VW * 8) * 4;
+        float2 ml;
+        const float4 v = join(EA_CLUSTER, [&](int k) { return remote2(of_rank(block_ml + row, k)); }, [&](int k) { return remote4(of_rank(block_o + at, k)); }, ml);
+        if (runs == 1) {
+            to_out(v, i);
+        } else {
+            *reinterpret_cast<float4*>(a.part_o + (long long)(first + run) * ROWS * PART + i * 4) = v;
+            // (blocks that share a row leave the same)
+            if (i % (VW * 8) == 0 || i == begin) *reinterpret_cast<float2*>(a.part_ml + ((first + run) * ROWS + row) * 2) = ml;
+        }
+    }
+    if (runs == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* ticket = a.tickets + first * EA_CLUSTER + rank;
+        *ticket_s = atomicAdd(ticket, 1);
+        if (*ticket_s == runs - 1) *ticket = 0;   // (as the next call wants it)
+    }
+    __syncthreads();
+    if (*ticket_s != runs - 1) return;
+    __threadfence();
+    for (int i = begin + threadIdx.x; i < end; i += THREADS) {
+        const int row = i / (VW * 8);
+        float2 ml;
+        to_out(join(runs, [&](int k) { return __ldcg(reinterpret_cast<const float2*>(a.part_ml + ((first + k) * ROWS + row) * 2)); },
+                    [&](int k) { return __ldcg(reinterpret_cast<const float4*>(a.part_o + (long long)(first + k) * ROWS * PART + i * 4)); }, ml),
+               i);
+    }
+}
+
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(EA_WARPS * 32, Shape<T, D, NR>::BLOCKS)
 attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_constant__ AttendArgs a) {
@@ -280,42 +396,60 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
     const E4m3Site& site = a.site;
-    const int KVH = site.kv_heads, G = a.n_heads / KVH, pairs_each = KVH * a.chunks;
+    const int KVH = site.kv_heads, G = a.group;
     const int q_width = a.n_heads * D, n_blocks = gridDim.x;
 
     // ---- this block's share (every warp works it out for itself; a lane keeps its one of the first 32 sequences)
     Sequence first;
-    first.pages = 0;
-    if ((int)lane < a.n_seqs) first = sequence_of(a, lane);
-    auto pages_of = [&](int s0) { return s0 == 0 ? first.pages : s0 + (int)lane < a.n_seqs ? sequence_of(a, s0 + lane).pages : 0; };
-    int total = 0, pairs = 0, whole = 0, target = EA_WARPS;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const int pages = pages_of(s0);
-        total += pages;
-        pairs += pages > 0;
-    }
-    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total) * pairs_each;
-    pairs = (int)__reduce_add_sync(0xffffffffu, (unsigned)pairs) * pairs_each;
-    if (total > target * a.block_slots) target = (total + a.block_slots - 1) / a.block_slots;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) whole += (pages_of(s0) + target - 1) / target;
-    whole = (int)__reduce_add_sync(0xffffffffu, (unsigned)whole) * pairs_each;
-    // pages of a pair are rounded up to whole units; where blocks may have several pairs, each counts EA_PAIR_COST pages more
-    const bool aligned = whole <= a.block_slots;
-    const int ahead = aligned ? 0 : EA_PAIR_COST;
-    if (aligned) {
-        total = whole * target;
+    first.pages = first.pairs = 0;
+    if ((int)lane < a.n_seqs) first = sequence_of<ROWS>(a, lane);
+    auto pages_of = [&](int s0) {   // (pages, pairs) of this lane's one of 32 sequences
+        if (s0 == 0) return make_int2(first.pages, first.pairs);
+        if (s0 + (int)lane >= a.n_seqs) return make_int2(0, 0);
+        const Sequence x = sequence_of<ROWS>(a, s0 + lane);
+        return make_int2(x.pages, x.pairs);
+    };
+    const int rank = a.cluster > 1 ? (int)blockIdx.x % EA_CLUSTER : 0, number = a.cluster > 1 ? (int)blockIdx.x / EA_CLUSTER : (int)blockIdx.x;
+    int total = 0, target = EA_WARPS, ahead = 0;
+    bool aligned = true;
+    if (a.cluster > 1) {   // a cluster takes the part of a block, always whole units; there is one for every pair's every unit
+        target = EA_WARPS * EA_CLUSTER;
+        total = 0x7fffffff;
     } else {
-        total += pairs * ahead;
-        target = max(target, (total + a.block_slots - 1) / a.block_slots);
+        int pairs = 0, whole = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const int2 x = pages_of(s0);
+            total += x.x * x.y;
+            pairs += x.x > 0 ? x.y : 0;
+        }
+        total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+        pairs = (int)__reduce_add_sync(0xffffffffu, (unsigned)pairs);
+        if (total > target * a.block_slots) target = (total + a.block_slots - 1) / a.block_slots;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const int2 x = pages_of(s0);
+            whole += (x.x + target - 1) / target * x.y;
+        }
+        whole = (int)__reduce_add_sync(0xffffffffu, (unsigned)whole);
+        // pages of a pair are rounded up to whole units; where blocks may have several pairs, each counts EA_PAIR_COST pages more
+        aligned = whole <= a.block_slots;
+        if (aligned) {
+            total = whole * target;
+        } else {
+            ahead = EA_PAIR_COST;
+            total += pairs * ahead;
+            target = max(target, (total + a.block_slots - 1) / a.block_slots);
+        }
     }
     auto places_of = [&](int pages) { return pages == 0 ? 0 : aligned ? (pages + target - 1) / target * target : pages + ahead; };
-    const int range_begin = blockIdx.x * target, range_end = min(range_begin + target, total);
+    const int range_begin = number * target;
+    int range_end = min(range_begin + target, total);
     // the sequence in whose pages it begins
     int seq = 0, base = 0;
     Sequence r = first;
     if (range_begin < range_end) {
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            const int mine = places_of(pages_of(s0)) * pairs_each;
+            const int2 x = pages_of(s0);
+            const int mine = places_of(x.x) * x.y;
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -331,32 +465,38 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     r.slot = __shfl_sync(0xffffffffu, first.slot, who), r.begin = __shfl_sync(0xffffffffu, first.begin, who);
                     r.tokens = __shfl_sync(0xffffffffu, first.tokens, who), r.first_pos = __shfl_sync(0xffffffffu, first.first_pos, who);
                     r.last_pos = __shfl_sync(0xffffffffu, first.last_pos, who), r.page0 = __shfl_sync(0xffffffffu, first.page0, who);
-                    r.pages = __shfl_sync(0xffffffffu, first.pages, who);
+                    r.pages = __shfl_sync(0xffffffffu, first.pages, who), r.pairs = __shfl_sync(0xffffffffu, first.pairs, who);
                 } else {
-                    r = sequence_of(a, seq);
+                    r = sequence_of<ROWS>(a, seq);
                 }
                 break;
             }
             base += __shfl_sync(0xffffffffu, upto, 31);
+            if (s0 + 32 >= a.n_seqs) range_end = range_begin;   // (a cluster that nothing is left for)
         }
     }
 
     int padded = places_of(r.pages);
     for (int at = range_begin; at < range_end;) {
-        while (at >= base + padded * pairs_each) {   // (sequences without pages are passed over)
-            base += padded * pairs_each;
-            r = sequence_of(a, ++seq);
+        while (at >= base + padded * r.pairs) {   // (sequences without pages are passed over)
+            base += padded * r.pairs;
+            r = sequence_of<ROWS>(a, ++seq);
             padded = places_of(r.pages);
         }
-        const int y = (at - base) / padded, pair_begin = base + y * padded, kvh = y / a.chunks, chunk = y % a.chunks;
-        const int p_begin = r.page0 + max(at - pair_begin - ahead, 0), p_end = r.page0 + min(min(padded, range_end - pair_begin) - ahead, r.pages);
-        const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin;
+        const int y = (at - base) / padded, pair_begin = base + y * padded, kvh = y % KVH, chunk = y / KVH;
+        int p_begin = r.page0 + max(at - pair_begin - ahead, 0), p_end = r.page0 + min(min(padded, range_end - pair_begin) - ahead, r.pages);
+        const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin && rank == 0;
         at = min(pair_begin + padded, range_end);
         if (reports && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
         const int row0 = chunk * ROWS, n_rows = min(ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
         if (n_rows <= 0 || p_begin >= p_end) continue;
+        if (a.cluster > 1) {   // this block's share, perhaps none
+            const int each = (p_end - p_begin + a.cluster - 1) / a.cluster;
+            p_begin += rank * each;
+            p_end = min(p_begin + each, p_end);
+        }
         auto row_at = [&](int row) { return row_offset<D>(a, r.begin, kvh, row0 + row); };
-        const int my_pages = (p_end - p_begin - (int)warp + EA_WARPS - 1) / EA_WARPS;   // (0 where there are fewer than warps)
+        const int my_pages = max(p_end - p_begin - (int)warp + EA_WARPS - 1, 0) / EA_WARPS;   // (0 where there are fewer than warps)
         // what the rows see, lo .. hi - 1: this lane's (8 n + 2 c and + 1), all of them together, every one of them
         const int t_first = a.single ? 0 : row0 / G, t_last = a.single ? 0 : (row0 + n_rows - 1) / G;
         const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (a.single ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
@@ -749,10 +889,14 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                 }
             }
         __syncthreads();
-        const int first_block = (pair_begin + ahead) / target, runs = (pair_begin + ahead + r.pages - 1) / target - first_block + 1, run = (int)blockIdx.x - first_block;
+        const int first_block = (pair_begin + ahead) / target, runs = (pair_begin + ahead + r.pages - 1) / target - first_block + 1, run = number - first_block;
         // where run k of this pair leaves its results: a block's first pair in the first of its two places
         auto place_of = [&](int k) { return place_in(pair_begin, first_block + k, target); };
         const int items = n_rows * VW * 8;
+        if (a.cluster > 1) {
+            join_cluster<T, D, NR>(out, a, shared_o, &m_s[0][0], &l_s[0][0], items, row0, r.begin, kvh, rank, first_block, run, runs, &ticket_s);
+            break;   // (a cluster has one pair)
+        }
         for (int i = threadIdx.x; i < items; i += THREADS) {
             const int row = i / (VW * 8);
             float m = EA_NONE, l = 0.f, part[EA_WARPS];
@@ -781,6 +925,10 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         }
         __syncthreads();   // (the next pair takes the same shared memory)
     }
+    if (a.cluster > 1) {   // (no block's shared memory goes while another may read it)
+        cluster_arrive();
+        cluster_wait();
+    }
     // ---- pairs of several blocks: whoever leaves the last of sixteen results joins them, whoever joins the last sixteen joins the sixteens
     for (int k = 0; k < n_left; ++k) {
         const Pair pair = left_s[k];
@@ -804,7 +952,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     }
     // padding entries: zeros
     for (int s = n_blocks - 1 - blockIdx.x; s < a.n_seqs; s += n_blocks) {
-        const Sequence x = sequence_of(a, s);
+        const Sequence x = sequence_of<ROWS>(a, s);
         if (x.slot < 0)
             for (int i = threadIdx.x; i < x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
     }
@@ -826,7 +974,20 @@ template <typename T, int D, int NR> static int slots_of() {
 }
 template <typename T, int D, int NR> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
     if (a.block_slots <= 0 || a.block_slots != slots_of<T, D, NR>()) return (int)cudaErrorInvalidValue;
-    return (int)launch_pdl(attend_e4m3_kernel<T, D, NR>, dim3(blocks), dim3(EA_WARPS * 32), Shape<T, D, NR>::SMEM, stream, (const T*)q, (T*)out, a);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(EA_WARPS * 32);
+    config.dynamicSmemBytes = Shape<T, D, NR>::SMEM;
+    config.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = a.cluster > 1 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&config, attend_e4m3_kernel<T, D, NR>, (const T*)q, (T*)out, a);
 }
 
 #define EA_EVERY(T, NR, CALL)               \
@@ -873,7 +1034,11 @@ QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int
         blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
     if (n_seqs <= 0) return 0;
-    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_seqs, single, chunks, most_pages, block_slots, window, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
+    // Where clusters have room for every pair, they take its pages: eight blocks bring their results together without the way through memory (@CLUSTER@).
+    const long long clusters = (long long)n_seqs * kv_heads * chunks * ((most_pages + EA_WARPS * EA_CLUSTER - 1) / (EA_WARPS * EA_CLUSTER));
+    int cluster = 1;
+    if (clusters * EA_CLUSTER <= block_slots && EA_USE_CLUSTERS) cluster = EA_CLUSTER, blocks = (int)clusters * EA_CLUSTER;
+    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, cluster, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
 #define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
     EA_ALL(EA_ATTEND)
     return (int)cudaErrorInvalidValue;
