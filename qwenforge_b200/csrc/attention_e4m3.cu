@@ -32,9 +32,6 @@
 #include "e4m3.cuh"
 
 #define EA_WARPS 4
-#ifndef EA_USE_CLUSTERS
-#define EA_USE_CLUSTERS 1
-#endif
 #define EA_DEAD 0x7fffffff   // the exponent of a tile that is not there, or that no row sees
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 
@@ -139,9 +136,10 @@ __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(cod
 template <typename T, int D, int NR> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
     static constexpr int ROWS = 8 * NR;
-    static constexpr int TILE = D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
-    static constexpr int BLOCKS = 2;                                  // of an SM
-    static constexpr int STAGES = D <= 64 ? 2 : 3;                                  // tiles of a warp in shared memory: one at work, the others on their way
+    static constexpr bool SMALL = D <= 64 && NR == 1;
+    static constexpr int TILE = SMALL ? 32 : D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
+    static constexpr int BLOCKS = SMALL ? 3 : 2;                      // of an SM
+    static constexpr int STAGES = D <= 64 ? 2 : 3;                    // tiles of a warp in shared memory: one at work, the others on their way
     static constexpr int PITCH = D / 16 % 2 ? D : D + 16;             // bytes of a staged row: an odd number of 16, so that eight rows meet all banks
     static constexpr int STAGE = 2 * TILE * PITCH;                    // keys, then values
     static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result: items of four
@@ -154,7 +152,7 @@ template <typename T, int D, int NR> struct Shape {
 struct AttendArgs {
     const int *cu_q, *tok_pos, *slots;
     E4m3Site site;
-    int n_heads, group, n_seqs, single, chunks, most_pages, block_slots, window, cluster;   // group: query heads of a kv head
+    int n_heads, group, n_seqs, single, chunks, most_pages, block_slots, window, cluster, cluster_log;   // group: query heads of a kv head
     float scale_log2;
     float *part_o, *part_ml;   // [2 * blocks][ROWS][PART], [2 * blocks][ROWS][2]
     int *tickets, *err;        // [4 * blocks]
@@ -284,9 +282,8 @@ __device__ __forceinline__ float2 remote2(uint32_t at) {
     asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
     return v;
 }
-#define EA_CLUSTER 8   // blocks of a cluster
-// The end of a pair whose runs are clusters: a block puts its warps' results together, the cluster its blocks', each block an eighth of the items; of
-// several clusters the last one to leave an eighth joins that. No result takes the way through memory where one cluster has the pair.
+// The end of a pair whose runs are clusters: a block puts its warps' results together, the cluster its blocks', each block a share of the items; of
+// several clusters the last one to leave a share joins that. No result takes the way through memory where one cluster has the pair.
 template <typename T, int D, int NR>
 __device__ __forceinline__ void join_cluster(T* out, const AttendArgs& a, float* shared_o, const float* m_s, const float* l_s, int items, int row0, int token0, int kvh,
                                              int rank, int first, int run, int runs, int* ticket_s) {
@@ -314,13 +311,13 @@ __device__ __forceinline__ void join_cluster(T* out, const AttendArgs& a, float*
     }
     cluster_arrive();
     cluster_wait();
-    const int each = (items + EA_CLUSTER - 1) / EA_CLUSTER, begin = rank * each, end = min(begin + each, items);
+    const int each = (items + a.cluster - 1) >> a.cluster_log, begin = rank * each, end = min(begin + each, items);
     // one of `count` results to the others: their maxima and sums, their items
     auto join = [&](int count, auto ml_of, auto item_of, float2& ml) {
         float2 x[16];
         float4 y[16], v = make_float4(0.f, 0.f, 0.f, 0.f);
         ml = make_float2(EA_NONE, 0.f);
-        for (int k0 = 0; k0 < count; k0 += 16) {   // (an eighth of a sequence's page table: more than sixteen from 32,768 positions on)
+        for (int k0 = 0; k0 < count; k0 += 16) {   // (blocks of a cluster, or clusters of a pair)
             float m = ml.x;
 #pragma unroll
             for (int k = 0; k < 16; ++k)
@@ -347,7 +344,7 @@ __device__ __forceinline__ void join_cluster(T* out, const AttendArgs& a, float*
     for (int i = begin + threadIdx.x; i < end; i += THREADS) {
         const int row = i / (VW * 8), at = row * LD + i % (VW * 8) * 4;
         float2 ml;
-        const float4 v = join(EA_CLUSTER, [&](int k) { return remote2(of_rank(block_ml + row, k)); }, [&](int k) { return remote4(of_rank(block_o + at, k)); }, ml);
+        const float4 v = join(a.cluster, [&](int k) { return remote2(of_rank(block_ml + row, k)); }, [&](int k) { return remote4(of_rank(block_o + at, k)); }, ml);
         if (runs == 1) {
             to_out(v, i);
         } else {
@@ -360,7 +357,7 @@ __device__ __forceinline__ void join_cluster(T* out, const AttendArgs& a, float*
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        int* ticket = a.tickets + first * EA_CLUSTER + rank;
+        int* ticket = a.tickets + first * a.cluster + rank;
         *ticket_s = atomicAdd(ticket, 1);
         if (*ticket_s == runs - 1) *ticket = 0;   // (as the next call wants it)
     }
@@ -409,11 +406,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         const Sequence x = sequence_of<ROWS>(a, s0 + lane);
         return make_int2(x.pages, x.pairs);
     };
-    const int rank = a.cluster > 1 ? (int)blockIdx.x % EA_CLUSTER : 0, number = a.cluster > 1 ? (int)blockIdx.x / EA_CLUSTER : (int)blockIdx.x;
+    const int rank = (int)blockIdx.x & (a.cluster - 1), number = (int)blockIdx.x >> a.cluster_log;   // (one of 1, 8 or 16)
     int total = 0, target = EA_WARPS, ahead = 0;
     bool aligned = true;
     if (a.cluster > 1) {   // a cluster takes the part of a block, always whole units; there is one for every pair's every unit
-        target = EA_WARPS * EA_CLUSTER;
+        target = EA_WARPS << a.cluster_log;
         total = 0x7fffffff;
     } else {
         int pairs = 0, whole = 0;
@@ -491,7 +488,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         const int row0 = chunk * ROWS, n_rows = min(ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
         if (n_rows <= 0 || p_begin >= p_end) continue;
         if (a.cluster > 1) {   // this block's share, perhaps none
-            const int each = (p_end - p_begin + a.cluster - 1) / a.cluster;
+            const int each = (p_end - p_begin + a.cluster - 1) >> a.cluster_log;
             p_begin += rank * each;
             p_end = min(p_begin + each, p_end);
         }
@@ -966,14 +963,48 @@ template <typename T, int D, int NR> static int slots_of() {
     if (cached[device] == 0) {
         int n = 0;
         if (cudaFuncSetAttribute(attend_e4m3_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NR>::SMEM) != cudaSuccess ||
+            cudaFuncSetAttribute(attend_e4m3_kernel<T, D, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_e4m3_kernel<T, D, NR>, EA_WARPS * 32, Shape<T, D, NR>::SMEM) != cudaSuccess)
             return 0;
         cached[device] = std::min(n * qf_sm_count(), EA_GROUP * EA_MOST_GROUPS);
     }
     return cached[device];
 }
+// Clusters of 2^log blocks that the device holds at once.
+template <typename T, int D, int NR> static int clusters_of(int log) {
+    static int cached[64][5];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+    int& n = cached[device][log];
+    if (n == 0) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(1 << log);
+        config.blockDim = dim3(EA_WARPS * 32);
+        config.dynamicSmemBytes = Shape<T, D, NR>::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1 << log;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        config.attrs = attr;
+        config.numAttrs = 1;
+        int found = 0;
+        if (cudaOccupancyMaxActiveClusters(&found, attend_e4m3_kernel<T, D, NR>, &config) != cudaSuccess || found <= 0) {
+            (void)cudaGetLastError();   // (none of this size)
+            found = -1;
+        }
+        n = found;
+    }
+    return n;
+}
 template <typename T, int D, int NR> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
     if (a.block_slots <= 0 || a.block_slots != slots_of<T, D, NR>()) return (int)cudaErrorInvalidValue;
+    // Where clusters have room for every pair at once, they take its pages: eight blocks (sixteen, if that is what a pair's pages want) bring their
+    // results together without the way through memory (@CLUSTER@).
+    for (int log = a.most_pages > EA_WARPS * 8 ? 4 : 3; log >= 3 && a.cluster_log == 0; --log) {
+        const long long all = (long long)a.n_seqs * a.site.kv_heads * a.chunks * ((a.most_pages + (EA_WARPS << log) - 1) / (EA_WARPS << log));
+        if (all << log <= a.block_slots && all <= clusters_of<T, D, NR>(log)) a.cluster_log = log, blocks = (int)all << log;
+    }
+    a.cluster = 1 << a.cluster_log;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(blocks);
     config.blockDim = dim3(EA_WARPS * 32);
@@ -1034,11 +1065,7 @@ QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int
         blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
     if (n_seqs <= 0) return 0;
-    // Where clusters have room for every pair, they take its pages: eight blocks bring their results together without the way through memory (@CLUSTER@).
-    const long long clusters = (long long)n_seqs * kv_heads * chunks * ((most_pages + EA_WARPS * EA_CLUSTER - 1) / (EA_WARPS * EA_CLUSTER));
-    int cluster = 1;
-    if (clusters * EA_CLUSTER <= block_slots && EA_USE_CLUSTERS) cluster = EA_CLUSTER, blocks = (int)clusters * EA_CLUSTER;
-    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, cluster, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
+    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, 1, 0, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
 #define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
     EA_ALL(EA_ATTEND)
     return (int)cudaErrorInvalidValue;
