@@ -9,13 +9,17 @@
 // A page that is begun takes its exponent from its new rows alone, whatever an earlier holder left there. Rows behind the new ones stay.
 //
 // A run is a page's new rows. Two kernels, the same in what they write:
-//   write_runs     spans of EW_LONG tokens or more: a block takes the runs that begin among 64 of the step's tokens and some of the heads, all its
-//                  threads one head at a time. A thread has the same one or two pieces (a row, eight pairs of the rotation) of every head, so
-//                  their sines and cosines are worked out once and stay in registers, a key's or value's elements stay there between amax and
-//                  codes, and the next head's are loaded meanwhile.
+//   write_runs     spans of EW_LONG tokens or more: a block takes a run and some of the heads, all its threads one head at a time. A thread has the
+//                  same one or two pieces (a row, eight pairs of the rotation) of every head, so their sines and cosines are worked out once
+//                  and stay in registers, a key's or value's elements stay there between amax and codes, and the next head's are loaded
+//                  meanwhile. One prompt of 8,192 tokens, 28 + 4 + 4 heads of 128 in bfloat16: 37 microseconds, 3.8 TB/s (142 MB, 22 at the
+//                  copy's rate): instructions bound it, two thirds of them the rotation and its angles; twelve float32 prompts of up to 900
+//                  tokens, 16 + 2 + 2 heads of 128: 17.5 microseconds, 3.9 TB/s.
 //   write_any      single tokens, short spans, and rows or rotations that 16-byte accesses do not fit: a warp a head at a time over all rows of
 //                  a run; amax and codes are one warp's business, without a barrier. Sines and cosines come from shared memory, worked
-//                  out once per run. A key or value head is read twice, the second time from L1 or L2.
+//                  out once per run. A key or value head is read twice, the second time from L1 or L2. One token of one sequence: 3.1
+//                  microseconds, of 96 sequences at 28 + 4 + 4 heads of 128 4.4: a chain of loads (position, page, scale), the angle, the
+//                  warp's maximum.
 #include "e4m3.cuh"
 
 #define EW_WARPS 8
@@ -234,9 +238,10 @@ write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lon
 }
 
 #define EW_THREADS 256
-#define EW_PIECES 2   // of a thread: 64 rows of up to eight pieces
 
-template <typename T>
+// PIECES of a thread: two for heads of more than 64 components, one for the others. Threads whose row lies behind the run work on its last row, whose
+// elements change no maximum, and store nothing.
+template <typename T, int PIECES>
 __global__ void __launch_bounds__(EW_THREADS, 2)
 write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                   const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
@@ -245,7 +250,7 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     constexpr int WORDS = 8 * sizeof(T) / 16;   // of 16 bytes, of eight elements
     __shared__ float amax_s[2][EW_THREADS / 32];
     const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2;
-    const unsigned groups = D / 16;
+    const unsigned groups = D / 16, rows_each = EW_THREADS / groups;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = n_heads + 2 * KVH;
     const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
     NewRows run;
@@ -253,96 +258,96 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     const int at = run.first_pos % QF_PAGE, rows = run.rows, slot = write_cache ? slots[run.seq] : -1;
     const int page = slot >= 0 ? e4m3_page(site, slot, run.first_pos) : -1;
     if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
-    // this thread's pieces: a row, the places of its two eights in a head, and their turn
-    bool mine[EW_PIECES], turns[EW_PIECES];
-    int a_at[EW_PIECES], b_off[EW_PIECES], code_at[EW_PIECES];
-    const T* src[EW_PIECES];
-    T* dst[EW_PIECES];
-    float2 turn[EW_PIECES][8];
-    uint4 raw[EW_PIECES][2][WORDS];
+    // this thread's pieces: rows, and of each the same sixteen components, eight here and eight there
+    const int g = threadIdx.x % groups;
+    const bool turns = 8 * g < half;
+    const int a_at = turns ? 8 * g : 16 * g;   // (behind the rotated part: rot_dim + 16 (g - half / 8), and the eight behind that)
+    const int b_off = turns ? half : 8;
+    bool mine[PIECES];
+    int code_at[PIECES];
+    const T* src[PIECES];
+    T* dst[PIECES];
+    float2 turn[PIECES][8];
+    uint4 raw[PIECES][2][WORDS];
     auto load = [&]() {   // the next head
 #pragma unroll
-        for (int k = 0; k < EW_PIECES; ++k)
-            if (mine[k]) {
+        for (int k = 0; k < PIECES; ++k) {
 #pragma unroll
-                for (int i = 0; i < WORDS; ++i) {
-                    raw[k][0][i] = reinterpret_cast<const uint4*>(src[k])[i];
-                    raw[k][1][i] = reinterpret_cast<const uint4*>(src[k] + b_off[k])[i];
-                }
-                src[k] += D;
+            for (int i = 0; i < WORDS; ++i) {
+                raw[k][0][i] = reinterpret_cast<const uint4*>(src[k])[i];
+                raw[k][1][i] = reinterpret_cast<const uint4*>(src[k] + b_off)[i];
             }
+            src[k] += D;
+        }
     };
 #pragma unroll
-    for (int k = 0; k < EW_PIECES; ++k) {
-        const unsigned i = threadIdx.x + k * EW_THREADS;
-        const int g = i % groups, row = i / groups;
-        mine[k] = row < rows;
-        turns[k] = 8 * g < half;
-        a_at[k] = turns[k] ? 8 * g : 16 * g;   // (behind the rotated part: rot_dim + 16 (g - half / 8), and the eight behind that)
-        b_off[k] = turns[k] ? half : 8;
-        code_at[k] = (at + row) * D + a_at[k];
-        src[k] = qkv + (long long)(run.t + row) * qkv_stride + h_begin * D + a_at[k];
-        dst[k] = q_out + ((long long)(run.t + row) * n_heads + h_begin) * D + a_at[k];
+    for (int k = 0; k < PIECES; ++k) {
+        const int place = threadIdx.x / groups + k * rows_each, row = min(place, rows - 1);
+        mine[k] = place < rows && threadIdx.x < groups * rows_each;
+        code_at[k] = (at + row) * D + a_at;
+        src[k] = qkv + (long long)(run.t + row) * qkv_stride + h_begin * D + a_at;
+        dst[k] = q_out + ((long long)(run.t + row) * n_heads + h_begin) * D + a_at;
     }
     load();
+    if (turns) {
 #pragma unroll
-    for (int k = 0; k < EW_PIECES; ++k)
-        if (mine[k] && turns[k]) {
-            const float position = (float)(run.first_pos + (int)((threadIdx.x + k * EW_THREADS) / groups));
+        for (int e = 0; e < 8; ++e) {
+            const Turns f(inv_freq[a_at + e]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) turn[k][e] = Turns(inv_freq[a_at[k] + e]).at(position);
+            for (int k = 0; k < PIECES; ++k) turn[k][e] = f.at((float)(run.first_pos + code_at[k] / D - at));
         }
+    }
     int parity = 0;
     for (int h = h_begin; h < h_end; ++h) {
         const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
-        float x[EW_PIECES][2][8];
+        float x[PIECES][2][8];
 #pragma unroll
-        for (int k = 0; k < EW_PIECES; ++k) {
-            if (!mine[k]) continue;
+        for (int k = 0; k < PIECES; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const T* v = reinterpret_cast<const T*>(raw[k][i]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[k][i][e] = Num<T>::to_f(v[e]);
-                if (bias) {
-                    float b[8];
-                    load_values<T, 8>(bias + h * D + a_at[k] + i * b_off[k], nullptr, b);
+            }
+        if (h + 1 < h_end) load();
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float b[8];
+                load_values<T, 8>(bias + h * D + a_at + i * b_off, nullptr, b);
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[k][i][e] += b[e];
-                }
             }
         }
-        if (h + 1 < h_end) load();
-        if (!is_v) {
+        if (!is_v && turns) {
 #pragma unroll
-            for (int k = 0; k < EW_PIECES; ++k)
-                if (mine[k] && turns[k]) {
+            for (int k = 0; k < PIECES; ++k)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float u = x[k][0][e], w = x[k][1][e];
-                        x[k][0][e] = u * turn[k][e].x - w * turn[k][e].y;
-                        x[k][1][e] = w * turn[k][e].x + u * turn[k][e].y;
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    const float u = x[k][0][e], w = x[k][1][e];
+                    x[k][0][e] = u * turn[k][e].x - w * turn[k][e].y;
+                    x[k][1][e] = w * turn[k][e].x + u * turn[k][e].y;
                 }
         }
         if (is_q) {
 #pragma unroll
-            for (int k = 0; k < EW_PIECES; ++k)
+            for (int k = 0; k < PIECES; ++k) {
                 if (mine[k]) {
                     store_values<T, 8>(dst[k], x[k][0]);
-                    store_values<T, 8>(dst[k] + b_off[k], x[k][1]);
-                    dst[k] += D;
+                    store_values<T, 8>(dst[k] + b_off, x[k][1]);
                 }
+                dst[k] += D;
+            }
             continue;
         }
         if (page < 0) continue;
         float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < EW_PIECES; ++k)
-            if (mine[k]) {
+        for (int k = 0; k < PIECES; ++k)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(finite_size(x[k][0][e]), finite_size(x[k][1][e])));
-            }
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(finite_size(x[k][0][e]), finite_size(x[k][1][e])));
         const int place = h - n_heads;   // plane * kv heads + head
         float* scale = site.scales + (long long)page * site.page_scales + place;
         const int before = at > 0 ? exponent_of(*scale) : E4M3_LOW;
@@ -357,21 +362,22 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
         if (at > 0 && exp > before) rescale_codes(reinterpret_cast<uint4*>(codes), at * D / 16, pow2(max(before - exp, -126)), threadIdx.x, EW_THREADS);
         const float by = pow2(-exp);
 #pragma unroll
-        for (int k = 0; k < EW_PIECES; ++k)
+        for (int k = 0; k < PIECES; ++k)
             if (mine[k]) {
                 store_codes<8>(codes + code_at[k], x[k][0], by);
-                store_codes<8>(codes + code_at[k] + b_off[k], x[k][1], by);
+                store_codes<8>(codes + code_at[k] + b_off, x[k][1], by);
             }
         if (threadIdx.x == 0) *scale = pow2(exp);
     }
 }
 
-#ifndef EW_HEADS
-#define EW_HEADS 6   // heads of a block of write_runs
-#endif
-#ifndef EW_LONG
-#define EW_LONG 16   // tokens of the longest span from which write_runs is the faster one (@LONG@)
-#endif
+// Heads of a block of write_runs, which share its sines and cosines. Microseconds with 3, 4, 5, 6 and 9 of them: twelve float32 prompts of up to 900 tokens,
+// 16 + 2 + 2 heads of 128, 20.0, 21.7, 17.5, 17.5 and 22.0; one of 8,192 in bfloat16, 28 + 4 + 4 heads of 128, 39.3, 36.9, 36.8, 37.4 and 37.3.
+#define EW_HEADS 6
+// Tokens of the longest span from which write_runs is the faster one. Microseconds, write_any / write_runs, bfloat16, spans of 8, 16 and 32 tokens: 14 + 2 + 2
+// heads of 64, 1 sequence 4.0 / 6.6, 5.2 / 6.5, 7.4 / 6.7, 64 sequences 5.9 / 8.4, 8.0 / 8.7, 13.4 / 9.3; 28 + 4 + 4 of 128, 1 sequence 5.8 / 7.2, 8.4 / 7.2,
+// 13.7 / 8.3, 64 sequences 10.1 / 13.2, 16.6 / 14.5, 34 / 22.
+#define EW_LONG 16
 
 template <typename T>
 static int write_launch(const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq, const int* tok_pos, const int* slots,
@@ -383,8 +389,9 @@ static int write_launch(const void* qkv, const void* bias, long long qkv_stride,
     const int runs = single || most_runs > n_tokens ? n_tokens : (int)most_runs;
     const bool wide = rot_dim % 16 == 0 && qkv_stride % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias) % 16 == 0;
     if (wide && max_q_len >= EW_LONG) {
-        return (int)launch_pdl(write_runs_kernel<T>, dim3(runs, (heads + EW_HEADS - 1) / EW_HEADS), dim3(EW_THREADS), 0, stream, (const T*)qkv, (const T*)bias, qkv_stride,
-                               cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, err);
+        return (int)launch_pdl(site.head_dim > 64 ? write_runs_kernel<T, 2> : write_runs_kernel<T, 1>, dim3(runs, (heads + EW_HEADS - 1) / EW_HEADS), dim3(EW_THREADS), 0,
+                               stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache,
+                               n_seqs, err);
     }
     const int most_rows = max_q_len < QF_PAGE ? max_q_len : QF_PAGE;
     const size_t smem = (size_t)most_rows * (rot_dim / 2) * sizeof(float2);
@@ -416,7 +423,8 @@ QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void*
 
 // ---- Read back: the rows that a batch's sequences hold (from the first that a window of `window` positions leaves the first new token, 0:
 // all; up to the last new token) as values, into a storage of the same shape in another type, at the same page numbers: a page table serves
-// both. A block takes one plane and head of a page.
+// both. A block takes one plane and head of a page. Four documents of 68,000 tokens together, 4 heads of 128: 38 microseconds, 5.5 TB/s of the 6.5 that a
+// copy has.
 template <typename T>
 __global__ void __launch_bounds__(256)
 read_e4m3_kernel(T* __restrict__ out, long long out_page, const int* __restrict__ cu_q, const int* __restrict__ tok_pos, const int* __restrict__ slots,

@@ -134,9 +134,17 @@ def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor
         *site.place, n_seqs, pages, window, err.data_ptr(), _stream()), "cache_read_e4m3")
 
 
-def attention_e4m3_pays(max_q_len: int, group: int) -> bool:
-    """Whether a step of up to `max_q_len` tokens per sequence, `group` query heads to a kv head, attends over the codes: its rows fill few tiles."""
-    return max_q_len * group <= 4 * E4M3_ROWS
+# Rows (tokens of a span times heads of a group) up to which `attention_e4m3` is the faster way in bfloat16: a tile of 16 rows reads the cache anew, while
+# `cache_read_e4m3` with the kernels for prompts reads and writes every position once. Microseconds, codes / read back and attended over, seven heads to a
+# group, spans of 4, 16, 32 and 64 tokens: 8 sequences behind 4,000 tokens, 2 kv heads of 64 15 / 42, 28 / 42, 42 / 42, 71 / 42, 4 of 128 30 / 89, 63 / 90,
+# 111 / 91, 194 / 92; behind 300 12 / 11, 13 / 11, 13 / 11, 21 / 12 and 16 / 18, 17 / 18, 29 / 18, 50 / 20. In float32, where the other way is
+# `attention_generic`, codes are faster throughout: one span of 256 behind 4,000 tokens 48 / 228 and 174 / 571, a prompt of 2,000 149 / 246 and 581 / 867.
+E4M3_PAYS_ROWS = 128
+
+
+def attention_e4m3_pays(dtype: torch.dtype, max_q_len: int, group: int) -> bool:
+    """Whether a step of up to `max_q_len` tokens per sequence, `group` query heads to a kv head, is to attend over the codes."""
+    return dtype is torch.float32 or max_q_len * group <= E4M3_PAYS_ROWS
 
 
 class E4m3Scratch:
@@ -173,8 +181,8 @@ def _slots_of(is_bf16: int, head_dim: int, rows: int) -> int:
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_heads: int,
                    n_seqs: int, max_q_len: int, scale: float, window: int, scratch: E4m3Scratch, err: torch.Tensor, max_kv_len: Optional[int] = None) -> None:
-    """Causal grouped-query attention of a step's tokens over a cache in 8 bits: single tokens, and short spans (every 16 rows of tokens times the heads of
-    a group read the cache anew, so a prompt goes by `cache_read_e4m3` and the kernels for many rows). q, out [T, n_heads * head_dim], bfloat16 or
+    """Causal grouped-query attention of a step's tokens over a cache in 8 bits: single tokens, and spans (every 16 rows of tokens times the heads of
+    a group read the cache anew, see `attention_e4m3_pays`). q, out [T, n_heads * head_dim], bfloat16 or
     float32; query head i reads kv head i // (n_heads / kv_heads); key j is visible to a token at p iff max(0, p - window + 1) <= j <= p
     (window 0: all up to p). Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at consecutive positions, at most max_q_len; an entry may have none, and a
     padding entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page

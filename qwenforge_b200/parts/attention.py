@@ -43,7 +43,8 @@ Options that other designs switch on, each a parameter of the spec (all off for 
   out_gate       the concatenated heads are multiplied element by element with sigmoid(G h), a projection [heads * value_dim,
                  hidden] of the same input whose columns follow those of q, k, v in the one product
 A cache in 8 bits (`ctx.cache_dtype`) is taken by the plain form, at the head sizes of its kernels: keys and values are written as codes,
-single tokens and short spans attend over the codes, longer spans over the values that are read back into the group's storage for them.
+single tokens and short spans (in float32 all of them) attend over the codes, longer spans over the values that are read back into the
+group's storage for them.
 The position part may pair components 2j and 2j + 1 (`rotary_interleaved`) instead of j and j + R/2.
 """
 from __future__ import annotations
@@ -555,7 +556,7 @@ class GqaAttention(Mixer):
         ops.rope_cache_write_e4m3(qkv, ctx.cu_q, ctx.tok_seq, ctx.tok_pos, ctx.slots, inv_freq, rot_dim, self.n_heads, q, site.codes(), ctx.max_q_len, ctx.err,
                                   bias=bias, write_cache=writes_cache)
         attended = torch.empty_like(q)
-        if ctx.attention == "auto" and ops.attention_e4m3_pays(ctx.max_q_len, self.n_heads // self.n_kv):
+        if ctx.attention == "auto" and ops.attention_e4m3_pays(qkv.dtype, ctx.max_q_len, self.n_heads // self.n_kv):
             ops.attention_e4m3(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window,
                                ctx.codes_scratch, ctx.err, ctx.max_kv_len)
             return attended

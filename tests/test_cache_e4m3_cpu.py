@@ -86,4 +86,5 @@ def test_what_is_on_the_cpu_is_refused():
 
 
 def test_which_steps_attend_over_codes():
-    assert ops.attention_e4m3_pays(1, 7) and ops.attention_e4m3_pays(8, 8) and not ops.attention_e4m3_pays(2048, 7)
+    assert ops.attention_e4m3_pays(torch.bfloat16, 1, 7) and ops.attention_e4m3_pays(torch.bfloat16, 16, 8)
+    assert not ops.attention_e4m3_pays(torch.bfloat16, 17, 8) and ops.attention_e4m3_pays(torch.float32, 2048, 7)
