@@ -495,6 +495,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         const bool reports = y == 0 && threadIdx.x == 0 && at == pair_begin && rank == 0;
         at = min(pair_begin + padded, range_end);
         if (reports && r.last_pos / QF_PAGE - r.page0 + 1 > r.pages) atomicOr(a.err, QF_ERR_POSITION_RANGE);
+        if (reports && r.tokens * G > a.chunks * ROWS) atomicOr(a.err, QF_ERR_ROW_RANGE);   // (a span longer than the call has said)
         const int row0 = chunk * ROWS, n_rows = min(ROWS, r.tokens * G - row0);   // rows: token * G + head of the group
         if (n_rows <= 0 || p_begin >= p_end) continue;
         if (a.cluster > 1) {   // this block's share, perhaps none
@@ -951,6 +952,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     // padding entries: zeros
     for (int s = n_blocks - 1 - blockIdx.x; s < a.n_seqs; s += n_blocks) {
         const Sequence x = sequence_of<ROWS>(a, s);
+        if (a.single && threadIdx.x == 0 && a.cu_q[s + 1] - a.cu_q[s] != 1) atomicOr(a.err, QF_ERR_ROW_RANGE);   // (an entry of other than one token)
         if (x.slot < 0)
             for (int i = threadIdx.x; i < x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
     }

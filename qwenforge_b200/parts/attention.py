@@ -558,7 +558,7 @@ class GqaAttention(Mixer):
         attended = torch.empty_like(q)
         if ctx.attention == "auto" and ops.attention_e4m3_pays(qkv.dtype, ctx.max_q_len, self.n_heads // self.n_kv):
             ops.attention_e4m3(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window,
-                               ctx.codes_scratch, ctx.err, ctx.max_kv_len)
+                               ctx.codes_scratch or ops.E4m3Scratch(q.device), ctx.err, ctx.max_kv_len)
             return attended
         values = site.group.values
         ops.cache_read_e4m3(values, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), ctx.n_seqs, ctx.max_kv_len, ctx.err, window=self.window)

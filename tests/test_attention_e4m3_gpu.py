@@ -135,7 +135,7 @@ def test_a_token_of_a_span_does_not_see_the_next_ones_nan(dtype):
 @BOTH
 def test_scales_far_apart(dtype):
     """A page of huge values that no query looks at beside one of tiny values that all of them do, and the other way round."""
-    for low, high in ((-100, 20), (20, -100), (-112, 60)):
+    for low, high in ((-100, 20), (20, -100), (-112, 60), (-112, 119), (119, -112)):
         c = Case([(200, 1), (400, 2)], 4, 2, 64, dtype, seed=3, low=-10)
         for s in range(2):
             for p in range(4):
@@ -164,6 +164,29 @@ def test_a_query_that_is_not_finite_stays_alone():
     assert bool(torch.isnan(got[1, 1]).all())
     got[1, 1] = want[1, 1]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+@BOTH
+def test_a_scale_of_zero_or_less(scale, dtype):
+    c = Case(TOKENS[:5], 4, 2, 64, dtype, seed=3)
+    q = query(c)
+    out = torch.empty_like(q, device="cuda")
+    ops.attention_e4m3(q.cuda(), out, c.dev["cu_q"], c.dev["tok_pos"], c.dev["slots"], c.site, 4, c.n, 1, scale, 0, ops.E4m3Scratch("cuda"), c.err)
+    values = c.storage.cpu().double() * c.held_scales.cpu().double()[..., None, None]
+    want, size, far = ref.attend(q, c.cu_q, c.tok_pos, c.slots, values, c.table, 4, scale, 0)
+    assert bool(((out.cpu().double().view(want.shape) - want).abs() <= ref.attend_tolerance(want, size, far.abs(), dtype)).all()) and int(c.err) == 0
+
+
+def test_entries_longer_than_the_call_says():
+    c = Case([(10, 9), (30, 2)], 10, 2, 64, torch.bfloat16, seed=3)
+    c.most = 3
+    run(c, query(c))
+    assert int(c.err) == ops.ERR_ROW_RANGE
+    c = Case([(10, 2), (30, 0)], 10, 2, 64, torch.bfloat16, seed=3)   # two tokens of two entries, but not one each
+    c.most = 1
+    run(c, query(c))
+    assert int(c.err) & ops.ERR_ROW_RANGE
 
 
 def test_pages_that_are_not_held_and_lengths_beyond_the_bound():

@@ -143,3 +143,22 @@ def test_the_simt_kernel_and_the_fast_ones():
             model.step(cache, [(slot, tokens[:130])])
             logits.append(torch.cat([model.step(cache, [(slot, tokens[t:t + 2])]).cpu() for t in range(130, 140, 2)]))
     helpers.assert_logits_close(logits[0], logits[1].double(), torch.float32)
+
+
+def test_a_trace_replayed(tmp_path):
+    """`trace_run --cache-dtype`: logits near those of a cache in the model's own type, and not the same."""
+    import json
+    import numpy as np
+    from qwenforge_b200.engine import replay
+    folder, _ = helpers.make_model_dir(helpers.SMALL_64, 5)
+    lines = [json.dumps({"step": 0, "entries": [{"id": "a", "tokens": helpers.random_tokens(1000, 70, 1), "want": [69]}]}),
+             json.dumps({"step": 1, "entries": [{"id": "a", "tokens": [5], "want": [0]}], "end": ["a"]})]
+    got = {}
+    for dtype in ("auto", "float8_e4m3"):
+        args = replay.parse_args(["--model", str(folder), "--dtype", "float32", "--out", str(tmp_path), "--max-tokens", "128", "--cache-dtype", dtype])
+        with torch.inference_mode():
+            model = Model.from_dir(args.model, args.dtype, args.device, "auto", args.cache_dtype)
+            replay.replay(model, model.new_cache(1024, 4), lines, tmp_path, report=lambda text: None)
+        got[dtype] = np.fromfile(tmp_path / "1.f32", dtype="<f4")
+    off = np.abs(got["auto"] - got["float8_e4m3"]).max()
+    assert 0 < off <= 2.0 ** -3 * np.abs(got["auto"]).max()
