@@ -153,7 +153,7 @@ template <typename T, int D, int NR> struct Shape {
 struct AttendArgs {
     const int *cu_q, *tok_pos, *slots;
     E4m3Site site;
-    int n_heads, group, n_seqs, single, chunks, most_pages, block_slots, window, cluster, cluster_log;   // group: query heads of a kv head
+    int n_heads, group, n_seqs, single, chunks, most_pages, block_slots, window, constants, cluster, cluster_log;   // group: query heads of a kv head
     float scale_log2;
     float *part_o, *part_ml;   // [2 * blocks][ROWS][PART], [2 * blocks][ROWS][2]
     int *tickets, *err;        // [4 * blocks]
@@ -391,7 +391,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     constexpr bool TWO = S::TWO;
     constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, DT = D / 16, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS;
     constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32, TERMS = TWO ? 2 : 1;
-    grid_chain_entry();
+    grid_launch_dependents();
+    // `constants`: lengths, slots, page tables and the pages before an entry's first new one are nobody's output, so the kernel ahead is waited for only
+    // before the rest is read
+    bool waited = !a.constants;
+    if (waited) grid_dependency_wait();
     extern __shared__ __align__(16) unsigned char staged[];   // [warps][STAGES][keys, values][TILE][PITCH]; later the outputs, [warps][rows][LD]
     float* shared_o = reinterpret_cast<float*>(staged);
     __shared__ float scale_s[EA_WARPS][S::STAGES];   // of the staged tiles: the keys' scale, the values' exponent
@@ -585,8 +589,23 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             }
             cp_async_commit();
         };
+        if (waited) {
 #pragma unroll
-        for (int i = 0; i < S::STAGES - 1; ++i) fetch();
+            for (int i = 0; i < S::STAGES - 1; ++i) fetch();
+        }
+#pragma unroll 1
+        for (int i = waited ? S::STAGES : 0; i < S::STAGES; ++i) {
+            if (!waited && (i == S::STAGES - 1 || i >= (int)steps || key0_of(i) / QF_PAGE >= r.first_pos / QF_PAGE)) {
+                grid_dependency_wait();
+                waited = true;
+                if (lane_page >= 0 && p_begin + (int)warp + (int)lane * EA_WARPS >= r.first_pos / QF_PAGE) {   // (scales that were looked up before)
+                    const float* scales = site.scales + (long long)lane_page * site.page_scales + kvh;
+                    lane_scale = scales[0];
+                    lane_unit = exponent_of(scales[KVH]);
+                }
+            }
+            if (i < S::STAGES - 1) fetch();
+        }
 
         // ---- the queries' fragments: lane (g, c) has row g's components of its column
         uint32_t qb[TERMS][NR][KW][2];
@@ -949,6 +968,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             if (groups == 1) break;
         }
     }
+    if (!waited) grid_dependency_wait();
     // padding entries: zeros
     for (int s = n_blocks - 1 - blockIdx.x; s < a.n_seqs; s += n_blocks) {
         const Sequence x = sequence_of<ROWS>(a, s);
@@ -1061,7 +1081,7 @@ QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim, int rows) {
 // first call and after every call.
 QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int* cu_q, const int* tok_pos, const int* slots, void* codes, float* scales,
                                 const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots, int kv_heads,
-                                int head_dim, int n_heads, int n_seqs, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window,
+                                int head_dim, int n_heads, int n_seqs, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window, int constants,
                                 float* part_o, float* part_ml, int* tickets, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (head_dim <= 0 || head_dim % 16 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads || chunks <= 0 || most_pages <= 0 || most_pages >= 1 << 20 || columns <= 0 || n_slots <= 0 ||
@@ -1069,7 +1089,7 @@ QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int
         blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
     if (n_seqs <= 0) return 0;
-    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, 1, 0, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
+    AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, constants, 1, 0, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
 #define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
     EA_ALL(EA_ATTEND)
     return (int)cudaErrorInvalidValue;

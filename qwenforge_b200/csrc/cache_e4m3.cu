@@ -143,15 +143,20 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(EW_WARPS * 32)
 write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                  const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
-                 T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int single, int most_rows, int* err) {
-    grid_chain_entry();
+                 T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int single, int most_rows, int constants,
+                 int* err) {
+    grid_launch_dependents();
+    if (!constants) grid_dependency_wait();
     extern __shared__ float2 turn[];   // [rows of a run][rot_dim / 2] cosine, sine
     const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2, pass = D - rot_dim;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int heads = n_heads + 2 * KVH;
     const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
     NewRows run;
-    if (!run_of(blockIdx.x, single, n_seqs, cu_q, tok_seq, tok_pos, run)) return;
+    if (!run_of(blockIdx.x, single, n_seqs, cu_q, tok_seq, tok_pos, run)) {
+        grid_dependency_wait();
+        return;
+    }
     const int t = run.t, first_pos = run.first_pos, at = first_pos % QF_PAGE, slot = write_cache ? slots[run.seq] : -1;
     int rows = run.rows;
     if (rows > most_rows || (single && cu_q[run.seq + 1] - cu_q[run.seq] > 1)) {   // (an entry longer than the call has said: there is no room for its angles)
@@ -162,6 +167,7 @@ write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lon
     if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
     for (int i = threadIdx.x; i < rows * half; i += blockDim.x) turn[i] = Turns(inv_freq[i % half]).at((float)(first_pos + i / half));
     __syncthreads();
+    if (constants) grid_dependency_wait();   // (what is read from here on may be the output of the kernel ahead)
     for (int h = h_begin + warp; h < h_end; h += EW_WARPS) {
         const bool is_q = h < n_heads, is_v = h >= n_heads + KVH;
         if (!is_q && page < 0) continue;
@@ -245,8 +251,9 @@ template <typename T, int PIECES>
 __global__ void __launch_bounds__(EW_THREADS, 2)
 write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long long qkv_stride, const int* __restrict__ cu_q, const int* __restrict__ tok_seq,
                   const int* __restrict__ tok_pos, const int* __restrict__ slots, const float* __restrict__ inv_freq, int rot_dim, int n_heads,
-                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int* err) {
-    grid_chain_entry();
+                  T* __restrict__ q_out, E4m3Site site, int write_cache, int n_seqs, int constants, int* err) {
+    grid_launch_dependents();
+    if (!constants) grid_dependency_wait();
     constexpr int WORDS = 8 * sizeof(T) / 16;   // of 16 bytes, of eight elements
     __shared__ float amax_s[2][EW_THREADS / 32];
     const int D = site.head_dim, KVH = site.kv_heads, half = rot_dim / 2;
@@ -254,7 +261,10 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = n_heads + 2 * KVH;
     const int h_each = (heads + gridDim.y - 1) / gridDim.y, h_begin = blockIdx.y * h_each, h_end = min(h_begin + h_each, heads);
     NewRows run;
-    if (h_begin >= h_end || !run_of(blockIdx.x, 0, n_seqs, cu_q, tok_seq, tok_pos, run)) return;
+    if (h_begin >= h_end || !run_of(blockIdx.x, 0, n_seqs, cu_q, tok_seq, tok_pos, run)) {
+        grid_dependency_wait();
+        return;
+    }
     const int at = run.first_pos % QF_PAGE, rows = run.rows, slot = write_cache ? slots[run.seq] : -1;
     const int page = slot >= 0 ? e4m3_page(site, slot, run.first_pos) : -1;
     if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
@@ -288,7 +298,7 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
         src[k] = qkv + (long long)(run.t + row) * qkv_stride + h_begin * D + a_at;
         dst[k] = q_out + ((long long)(run.t + row) * n_heads + h_begin) * D + a_at;
     }
-    load();
+    if (!constants) load();
     if (turns) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -296,6 +306,10 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) turn[k][e] = f.at((float)(run.first_pos + code_at[k] / D - at));
         }
+    }
+    if (constants) {
+        grid_dependency_wait();   // (the rows may be the output of the kernel ahead)
+        load();
     }
     int parity = 0;
     for (int h = h_begin; h < h_end; ++h) {
@@ -382,7 +396,7 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
 template <typename T>
 static int write_launch(const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq, const int* tok_pos, const int* slots,
                         const float* inv_freq, int rot_dim, int n_heads, void* q_out, const E4m3Site& site, int write_cache, int n_tokens, int n_seqs, int max_q_len,
-                        int* err, cudaStream_t stream) {
+                        int constants, int* err, cudaStream_t stream) {
     const int heads = n_heads + 2 * site.kv_heads, single = max_q_len == 1;
     // runs: an entry of n tokens has n / 64 + 2 at the most
     const long long most_runs = n_tokens / QF_PAGE + 2ll * n_seqs;
@@ -391,15 +405,15 @@ static int write_launch(const void* qkv, const void* bias, long long qkv_stride,
     if (wide && max_q_len >= EW_LONG) {
         return (int)launch_pdl(site.head_dim > 64 ? write_runs_kernel<T, 2> : write_runs_kernel<T, 1>, dim3(runs, (heads + EW_HEADS - 1) / EW_HEADS), dim3(EW_THREADS), 0,
                                stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache,
-                               n_seqs, err);
+                               n_seqs, constants, err);
     }
     const int most_rows = max_q_len < QF_PAGE ? max_q_len : QF_PAGE;
     const size_t smem = (size_t)most_rows * (rot_dim / 2) * sizeof(float2);
     const dim3 grid(runs, (heads + EW_WARPS - 1) / EW_WARPS);
     return (int)(wide ? launch_pdl(write_any_kernel<T, 8>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos,
-                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, err)
+                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, constants, err)
                       : launch_pdl(write_any_kernel<T, 1>, grid, dim3(EW_WARPS * 32), smem, stream, (const T*)qkv, (const T*)bias, qkv_stride, cu_q, tok_seq, tok_pos,
-                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, err));
+                                   slots, inv_freq, rot_dim, n_heads, (T*)q_out, site, write_cache, n_seqs, single, most_rows, constants, err));
 }
 
 static bool site_fits(const E4m3Site& s) {
@@ -412,13 +426,13 @@ static bool site_fits(const E4m3Site& s) {
 QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq,
                                        const int* tok_pos, const int* slots, const float* inv_freq, int rot_dim, int n_heads, void* q_out, void* codes,
                                        float* scales, const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots,
-                                       int kv_heads, int head_dim, int write_cache, int n_tokens, int n_seqs, int max_q_len, int* err, cudaStream_t stream) {
+                                       int kv_heads, int head_dim, int write_cache, int n_tokens, int n_seqs, int max_q_len, int constants, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (!inv_freq) rot_dim = 0;
     if (!site_fits(site) || head_dim > 128 || rot_dim < 0 || rot_dim > head_dim || (rot_dim & 1) || n_heads <= 0 || max_q_len <= 0) return (int)cudaErrorInvalidValue;
     if (n_tokens <= 0) return 0;
-    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, err, stream)
-                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, err, stream);
+    return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, constants, err, stream)
+                   : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, constants, err, stream);
 }
 
 // ---- Read back: the rows that a batch's sequences hold (from the first that a window of `window` positions leaves the first new token, 0:

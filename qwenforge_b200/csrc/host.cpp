@@ -57,12 +57,12 @@ int (*copy_pages)(void*, int, int, int, long long, long long, int, long long, lo
 int (*verify_drafts)(const float*, int, int, long long, const float*, long long, const int*, int, const int*, int, const float*, float, unsigned long long,
                      unsigned long long, const long long*, const int*, int*, int*, int, double*, void*, void*, int*, Stream);
 int (*write_e4m3)(int, const void*, const void*, long long, const int*, const int*, const int*, const int*, const float*, int, int, void*, void*, float*,
-                  const int*, long long, long long, int, int, int, int, int, int, int, int, int, int*, Stream);
+                  const int*, long long, long long, int, int, int, int, int, int, int, int, int, int, int*, Stream);
 int (*read_e4m3)(int, void*, long long, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int, int,
                  int, int*, Stream);
 int (*attention_e4m3_slots)(int, int, int);
 int (*attention_e4m3)(int, const void*, void*, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int,
-                      int, int, int, int, int, int, int, float, int, float*, float*, int*, int*, Stream);
+                      int, int, int, int, int, int, int, float, int, int, float*, float*, int*, int*, Stream);
 PyObject* kernel_error = nullptr;
 
 const struct {
@@ -526,16 +526,16 @@ bool placed(PyObject* o, Place& p) {
     return true;
 }
 
-// rope_cache_write_e4m3(qkv, bias or None, cu_q, tok_seq, tok_pos, slots, inv_freq or None, q_out, err, storage, place, rot_dim, n_heads, write_cache, max_q_len)
+// rope_cache_write_e4m3(qkv, bias or None, cu_q, tok_seq, tok_pos, slots, inv_freq or None, q_out, err, storage, place, rot_dim, n_heads, write_cache, max_q_len, constants)
 PyObject* e4m3_written(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 15) return PyErr_Format(PyExc_TypeError, "rope_cache_write_e4m3: 15 arguments");
+    if (n != 16) return PyErr_Format(PyExc_TypeError, "rope_cache_write_e4m3: 16 arguments");
     const at::Tensor* t[10];
     for (int i = 0; i < 10; ++i) t[i] = tensor(args[i]);
     const at::Tensor *qkv = t[0], *bias = t[1], *cu = t[2], *seq = t[3], *pos = t[4], *slots = t[5], *freq = t[6], *q = t[7], *err = t[8], *storage = t[9];
     Place p;
     const bool known = placed(args[10], p);
-    const long long rot = number(args[11]), heads = number(args[12]), writes = number(args[13]), most = number(args[14]);
+    const long long rot = number(args[11]), heads = number(args[12]), writes = number(args[13]), most = number(args[14]), constants = number(args[15]);
     if (PyErr_Occurred()) return nullptr;
     const int device = c10::cuda::current_device();
     const at::ScalarType type = qkv ? qkv->scalar_type() : at::kInt;
@@ -551,7 +551,7 @@ PyObject* e4m3_written(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return code_of([&] {
         return write_e4m3(type == at::kBFloat16, qkv->data_ptr(), bias ? bias->data_ptr() : nullptr, qkv->stride(0), ints(cu), ints(seq), ints(pos), ints(slots),
                           freq ? freq->const_data_ptr<float>() : nullptr, (int)rot, (int)heads, q->data_ptr(), p.codes, p.scales, p.table, p.page_bytes, p.page_scales,
-                          p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, writes != 0, (int)rows, (int)slots->numel(), (int)most, at_ptr<int>(*err), stream());
+                          p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, writes != 0, (int)rows, (int)slots->numel(), (int)most, constants != 0, at_ptr<int>(*err), stream());
     });
     END_HANDLE_TH_ERRORS
 }
@@ -584,17 +584,17 @@ PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// attention_e4m3(q, out, cu_q, tok_pos, slots, err, storage, place, part_o, part_ml, tickets, n_heads, n_seqs, max_q_len, scale, window, max_kv_len)
+// attention_e4m3(q, out, cu_q, tok_pos, slots, err, storage, place, part_o, part_ml, tickets, n_heads, n_seqs, max_q_len, scale, window, max_kv_len, constants)
 PyObject* e4m3_attended(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 17) return PyErr_Format(PyExc_TypeError, "attention_e4m3: 17 arguments");
+    if (n != 18) return PyErr_Format(PyExc_TypeError, "attention_e4m3: 18 arguments");
     const at::Tensor *q = tensor(args[0]), *out = tensor(args[1]), *cu = tensor(args[2]), *pos = tensor(args[3]), *slots = tensor(args[4]), *err = tensor(args[5]),
                      *storage = tensor(args[6]), *part_o = tensor(args[8]), *part_ml = tensor(args[9]), *tickets = tensor(args[10]);
     Place p;
     const bool known = placed(args[7], p);
     const long long heads = number(args[11]), seqs = number(args[12]), most_q = number(args[13]);
     const double scale = PyFloat_AsDouble(args[14]);
-    const long long window = number(args[15]), longest = number(args[16]);
+    const long long window = number(args[15]), longest = number(args[16]), constants = number(args[17]);
     if (PyErr_Occurred()) return nullptr;
     const int device = c10::cuda::current_device();
     const at::ScalarType type = q ? q->scalar_type() : at::kInt;
@@ -616,7 +616,7 @@ PyObject* e4m3_attended(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return code_of([&] {
         return attention_e4m3(type == at::kBFloat16, q->data_ptr(), out->data_ptr(), ints(cu), ints(pos), ints(slots), p.codes, p.scales, p.table, p.page_bytes,
                               p.page_scales, p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, (int)heads, (int)seqs, most_q == 1 && tokens == seqs,
-                              (int)block_rows, (int)chunks, (int)most, (int)blocks, (int)block_slots, (float)scale, (int)window, at_ptr<float>(*part_o),
+                              (int)block_rows, (int)chunks, (int)most, (int)blocks, (int)block_slots, (float)scale, (int)window, constants != 0, at_ptr<float>(*part_o),
                               at_ptr<float>(*part_ml), at_ptr<int>(*tickets), at_ptr<int>(*err), stream());
     });
     END_HANDLE_TH_ERRORS

@@ -60,7 +60,7 @@ def _batch(what: str, cu_q, tok_pos, slots, err) -> None:
 
 def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor,
                           inv_freq: Optional[torch.Tensor], rot_dim: int, n_heads: int, q_out: torch.Tensor, site: E4m3SiteArgs, max_q_len: int,
-                          err: torch.Tensor, bias: Optional[torch.Tensor] = None, write_cache: bool = True) -> None:
+                          err: torch.Tensor, bias: Optional[torch.Tensor] = None, write_cache: bool = True, constants: bool = False) -> None:
     """`rope_cache_write` into a cache in 8 bits: qkv [T, (NH + 2 KVH) D] (bfloat16 or float32; perhaps the first columns of wider rows) with its bias, q and
     k heads rotated by position (split halves of the first rot_dim components; inv_freq None: not at all), q to q_out [T, NH D], k and v
     as codes. Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at most max_q_len, at consecutive positions; a slot is in one entry at
@@ -69,10 +69,12 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     A page that gets rows takes, per plane and head, the least power of two under which all their finite elements lie within +-448 (of 2^-112
     to 2^119), and no less than it has if it held rows before the new ones; those rows' codes are then rounded to the larger unit. Rounding is
     to nearest even, once, from float32. Infinities become +-448, NaN stays. Rows behind the new ones stay as they are; a padding
-    entry (slot -1) writes its queries only, as does every entry with `write_cache` false."""
+    entry (slot -1) writes its queries only, as does every entry with `write_cache` false.
+    `constants` promises that no kernel in flight on the stream writes cu_q, tok_seq, tok_pos, slots, inv_freq or the page table (a bound model's step):
+    they are then read while the kernel ahead ends."""
     if qkv.is_cuda:
         code = _native("rope_cache_write_e4m3", "cache_e4m3")(qkv, bias, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, err, site.storage, site.place, rot_dim,
-                                                              n_heads, write_cache, max_q_len)
+                                                              n_heads, write_cache, max_q_len, constants)
         if code is not None:
             return _check(code, "rope_cache_write_e4m3")
     dtype = qkv.dtype
@@ -100,9 +102,9 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     _here("rope_cache_write_e4m3", qkv, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, site.storage, site.scales, site.table, err, bias)
     if n == 0:
         return
-    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _I, _P, _P)(
+    _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _I, _I, _P, _P)(
         is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
-        n_heads, q_out.data_ptr(), *site.place, bool(write_cache), n, slots.numel(), max_q_len, err.data_ptr(), _stream()), "rope_cache_write_e4m3")
+        n_heads, q_out.data_ptr(), *site.place, bool(write_cache), n, slots.numel(), max_q_len, bool(constants), err.data_ptr(), _stream()), "rope_cache_write_e4m3")
 
 
 def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_seqs: int, max_kv_len: int,
@@ -180,16 +182,18 @@ def _slots_of(is_bf16: int, head_dim: int, rows: int) -> int:
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor, slots: torch.Tensor, site: E4m3SiteArgs, n_heads: int,
-                   n_seqs: int, max_q_len: int, scale: float, window: int, scratch: E4m3Scratch, err: torch.Tensor, max_kv_len: Optional[int] = None) -> None:
+                   n_seqs: int, max_q_len: int, scale: float, window: int, scratch: E4m3Scratch, err: torch.Tensor, max_kv_len: Optional[int] = None,
+                   constants: bool = False) -> None:
     """Causal grouped-query attention of a step's tokens over a cache in 8 bits: single tokens, and spans (every 16 rows of tokens times the heads of
     a group read the cache anew, see `attention_e4m3_pays`). q, out [T, n_heads * head_dim], bfloat16 or
     float32; query head i reads kv head i // (n_heads / kv_heads); key j is visible to a token at p iff max(0, p - window + 1) <= j <= p
     (window 0: all up to p). Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at consecutive positions, at most max_q_len; an entry may have none, and a
     padding entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page
-    table has room for)."""
+    table has room for). `constants` promises that no kernel in flight on the stream writes cu_q, tok_pos, slots, the page table or a page before an
+    entry's first new token's (a bound model's step): they are then read while the kernel ahead ends."""
     if q.is_cuda:
         code = _native("attention_e4m3", "attention_e4m3")(q, out, cu_q, tok_pos, slots, err, site.storage, site.place, scratch.part_o, scratch.part_ml, scratch.tickets,
-                                                           n_heads, n_seqs, max_q_len, scale, window, 1 << 40 if max_kv_len is None else max_kv_len)
+                                                           n_heads, n_seqs, max_q_len, scale, window, 1 << 40 if max_kv_len is None else max_kv_len, constants)
         if code is not None:
             return _check(code, "attention_e4m3")
     dtype, d, kv_heads = q.dtype, site.head_dim, site.kv_heads
@@ -221,6 +225,6 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     blocks = min(block_slots, n_seqs * kv_heads * chunks * -(-most // E4M3_WARPS))
     scratch.ensure(blocks, d, block_rows)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
-    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P)(
+    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _P)(
         is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.place, n_heads, n_seqs,
-        max_q_len == 1 and q.shape[0] == n_seqs, block_rows, chunks, most, blocks, block_slots, scale, window, scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
+        max_q_len == 1 and q.shape[0] == n_seqs, block_rows, chunks, most, blocks, block_slots, scale, window, bool(constants), scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")
