@@ -151,20 +151,24 @@ def attention_e4m3_pays(dtype: torch.dtype, max_q_len: int, group: int) -> bool:
 
 class E4m3Scratch:
     """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). One
-    instance serves calls that run one after another on one stream; what is captured into a graph has one of its own."""
+    instance serves calls that run one after another on one stream; what is captured into a graph has one of its own. Should a captured call
+    share one all the same, its replays take their turn like calls: what a call outgrows is kept as long as the instance, because a graph may hold its address."""
+    TICKETS = 4096   # four for each of 1,024 blocks, the most that a launch has; zero from here on, where memory that a capture hands out is not
 
     def __init__(self, device):
         self.device = torch.device(device)
-        self.part_o = self.part_ml = self.tickets = None
+        self.part_o = self.part_ml = None
+        self.tickets = torch.zeros(self.TICKETS, dtype=torch.int32, device=self.device)
+        self.outgrown: list = []
 
     def ensure(self, blocks: int, head_dim: int, rows: int) -> None:
         rows *= 2 * blocks
-        if self.part_o is None or self.part_o.numel() < rows * -(-head_dim // 32) * 32:
-            self.part_o = torch.empty(rows * -(-head_dim // 32) * 32, dtype=torch.float32, device=self.device)
-        if self.part_ml is None or self.part_ml.numel() < 2 * rows:
-            self.part_ml = torch.empty(2 * rows, dtype=torch.float32, device=self.device)
-        if self.tickets is None or self.tickets.numel() < 4 * blocks:
-            self.tickets = torch.zeros(4 * blocks, dtype=torch.int32, device=self.device)
+        for name, size in (("part_o", rows * -(-head_dim // 32) * 32), ("part_ml", 2 * rows)):
+            held = getattr(self, name)
+            if held is None or held.numel() < size:
+                if held is not None:
+                    self.outgrown.append(held)
+                setattr(self, name, torch.empty(size, dtype=torch.float32, device=self.device))
 
 
 _block_slots: dict = {}

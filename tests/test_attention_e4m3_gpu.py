@@ -222,6 +222,37 @@ def test_a_captured_call_replayed_with_other_lengths():
     assert not bool(out[1].any())
 
 
+def test_a_workspace_that_a_captured_call_shares_with_larger_ones():
+    """A larger call replaces buffers whose address the graph holds: the replay finds them still there, and nobody else in them."""
+    small, large = Case([(900, 1), (40, 1)], 4, 2, 64, torch.bfloat16, seed=3), Case([(3000, 1)] * 12, 28, 4, 128, torch.bfloat16, seed=4)
+    q, out, scratch = query(small).cuda(), torch.empty((2, 4 * 64), dtype=torch.bfloat16, device="cuda"), ops.E4m3Scratch("cuda")
+    want = run(small, q, scratch=scratch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_e4m3(q, out, small.dev["cu_q"], small.dev["tok_pos"], small.dev["slots"], small.site, 4, 2, 1, 64 ** -0.5, 0, scratch, small.err)
+    before = scratch.part_o.numel()
+    check(large, query(large), run(large, query(large), scratch=scratch))
+    assert scratch.part_o.numel() > before
+    others = [torch.full((before,), 5.0, device="cuda") for _ in range(8)]   # (would get the buffer, were it given back)
+    graph.replay()
+    assert torch.equal(out, want) and all(bool((o == 5).all()) for o in others)
+    check(large, query(large), run(large, query(large), scratch=scratch))
+
+
+def test_a_workspace_that_grows_under_a_capture():
+    """A call behind the capture and before any replay finds its counters zero."""
+    c = Case([(900, 1), (4000, 1)], 14, 2, 64, torch.bfloat16, seed=3)
+    q = query(c).cuda()
+    want, out, scratch = run(c, q), torch.empty((2, 14 * 64), dtype=torch.bfloat16, device="cuda"), ops.E4m3Scratch("cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_e4m3(q, out, c.dev["cu_q"], c.dev["tok_pos"], c.dev["slots"], c.site, 14, 2, 1, 64 ** -0.5, 0, scratch, c.err)
+    assert torch.equal(run(c, q, scratch=scratch), want)
+    graph.replay()
+    assert torch.equal(out, want)
+    assert torch.equal(run(c, q, scratch=scratch), want)
+
+
 def test_calls_on_two_streams():
     """Each with a scratch of its own, at once."""
     cases = [Case([(3000 + 7 * i, 1), (100, 1)], 14, 2, 64, torch.bfloat16, seed=i) for i in range(2)]
