@@ -15,7 +15,7 @@
 // tiles are the tall side of m16n8k16: S^T = K Q^T (16 positions by 8 rows), O^T = V^T P^T (16 components by 8 rows), so that seven or eight heads
 // of a group fill a tile, where they would be half of one the other way round, with half the products, exponentials and sums to keep.
 // P^T comes out of the first with positions where the second wants rows: eight by eight, the warp transposes it (movmatrix).
-// A warp's tiles come through shared memory of its own, two on their way while it works on the third. For the keys a lane takes D / 4 components
+// A warp's tiles come through shared memory of its own, the next one on its way while it works on one. For the keys a lane takes D / 4 components
 // of one position in eight, 16 bytes at a time (which components a product's steps go through is free, as long as the queries'
 // fragments go through the same). For the values a lane takes D / 8 neighbouring components of the four positions that a step wants
 // of it, and byte t of them is its element of component column t: a byte permutation puts two positions side by side for the conversion.
@@ -25,6 +25,12 @@
 // whole blocks within that round, they are, and a block has one pair; else blocks begin and end anywhere, and lengths that
 // differ leave no SM idle. A pair of several blocks leaves partial results (maximum, sum, output); the block that ends last, by a
 // ticket, joins them in their order, sixteen at a time, and the last of those the sixteens.
+//
+// Microseconds in a row of calls: a chat of 900 tokens, 14 heads over 2 of 64, 7.7; 8 of 4,096 9.2 (8.3 MB); one document of 32,000, 16 over 2 of 128, 14.4 (16.4 MB);
+// 64 of up to 8,000, 28 over 4 of 128, 58.3 (272 MB, 4.7 TB/s; a copy has 6.5); 256 of 8,000 each 340 (2.1 GB, 6.2 TB/s); 12 spans of up to five tokens
+// behind up to 3,000 25.4; float32, 20 of up to 3,500, 16 over 2 of 128, 14.3. Small calls are a chain: the plan from the lengths 2, first loads 1.3, the warps'
+// merge 1.3, bringing blocks together 2 to 4. Large ones are bound by memory where lengths are even; ragged ones and spans by the issue of some 540 instructions
+// a tile of 32 positions, in 8 warps of an SM whose steps wait for their own products, exponentials and conversions.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -133,14 +139,18 @@ __device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bo
 }
 __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 
-// NR: eights of rows of a block.
+// NR: eights of rows of a block. Microseconds of the other choices in bfloat16, this one's first (heads of 64 are 14 over 2, of 128 28 over 4 where it does not say):
+// SMALL's tiles and blocks as of the rest of D <= 64: 8 sequences of 4,096 tokens, heads of 64, 9.2 / 12.0, 64 of up to 8,000 24.5 / 25.0, a chat of 900
+// 7.7 / 7.4; three stages: 64 of up to 8,000, heads of 128, 58.3 / 60.8, one of 32,000, 16 over 2 of 128, 14.3 / 14.6, spans of five tokens, heads of
+// 64, 13.5 / 15.6; tiles of a whole page for heads of 128: 64 of up to 8,000 58.3 / 69, 8 of 2,000 to 4,000 12.0 / 13.7, alone with 2,000 tokens 8.9 / 8.3; three blocks
+// to an SM there (168 registers, some spilled): 58.3 / 61.1, one of 32,000 14.6 / 13.5, alone with 8,000 11.6 / 12.8.
 template <typename T, int D, int NR> struct Shape {
     static constexpr bool TWO = sizeof(T) == 4;                       // float32: queries and weights as two float16 each
     static constexpr int ROWS = 8 * NR;
     static constexpr bool SMALL = D <= 64 && NR == 1;
     static constexpr int TILE = SMALL ? 32 : D <= 64 ? 64 : TWO && NR > 1 ? 16 : 32;   // positions of a step
     static constexpr int BLOCKS = SMALL ? 3 : 2;                      // of an SM
-    static constexpr int STAGES = D <= 64 ? 2 : 3;                    // tiles of a warp in shared memory: one at work, the others on their way
+    static constexpr int STAGES = 2;                                  // tiles of a warp in shared memory: one at work, the others on their way
     static constexpr int PITCH = D / 16 % 2 ? D : D + 16;             // bytes of a staged row: an odd number of 16, so that eight rows meet all banks
     static constexpr int STAGE = 2 * TILE * PITCH;                    // keys, then values
     static constexpr int PART = 32 * Parts<D>::v_words;               // floats of a row of a partial result: items of four
@@ -194,7 +204,9 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     }
 }
 
-#define EA_PAIR_COST 14    // pages whose time a pair's beginning and end take
+// Pages whose time a pair's beginning and end take. Microseconds with 14 / 0: 64 sequences of up to 8,000 tokens, 28 heads over 4 of 128, 61 / 74, 12 spans of up to
+// five tokens 26 / 47.
+#define EA_PAIR_COST 14
 #define EA_GROUP 16        // partial results that a block joins at once
 #define EA_MOST_GROUPS 64  // ... and groups of them: enough for 1,024 blocks
 
@@ -389,7 +401,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     using S = Shape<T, D, NR>;
     using P = Parts<D>;
     constexpr bool TWO = S::TWO;
-    constexpr int TILE = S::TILE, NT = TILE / 8, KT = TILE / 16, DT = D / 16, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS;
+    constexpr int TILE = S::TILE, KT = TILE / 16, DT = D / 16, KW = P::k_words, VW = P::v_words, LD = S::LD, PART = S::PART, ROWS = S::ROWS;
     constexpr int PER_PAGE = QF_PAGE / TILE, THREADS = EA_WARPS * 32, TERMS = TWO ? 2 : 1;
     grid_launch_dependents();
     // `constants`: lengths, slots, page tables and the pages before an entry's first new one are nobody's output, so the kernel ahead is waited for only
@@ -974,7 +986,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         const Sequence x = sequence_of<ROWS>(a, s);
         if (a.single && threadIdx.x == 0 && a.cu_q[s + 1] - a.cu_q[s] != 1) atomicOr(a.err, QF_ERR_ROW_RANGE);   // (an entry of other than one token)
         if (x.slot < 0)
-            for (int i = threadIdx.x; i < x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
+            for (long long i = threadIdx.x; i < (long long)x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
     }
 }
 
@@ -1022,11 +1034,13 @@ template <typename T, int D, int NR> static int clusters_of(int log) {
 template <typename T, int D, int NR> static int attend(const void* q, void* out, AttendArgs& a, int blocks, cudaStream_t stream) {
     if (a.block_slots <= 0 || a.block_slots != slots_of<T, D, NR>()) return (int)cudaErrorInvalidValue;
     // Where clusters have room for every pair at once, they take its pages: eight blocks (sixteen, if that is what a pair's pages want) bring their
-    // results together without the way through memory. Microseconds, without clusters / with: one chat of 900 tokens, 14 heads over 2 of 64, 8.7 / 7.3;
-    // 8 of 4,096 10.9 / 9.1, 16 of up to 2,000 10.2 / 8.5; one document of 32,000, 16 over 2 of 128, 15.7 / 14.8.
+    // results together without the way through memory. Microseconds, without clusters / with: one chat of 900 tokens, 14 heads over 2 of 64, 8.3 / 7.7,
+    // 8 of 4,096 10.4 / 9.2, 20 of 1,000 10.2 / 8.6; 28 over 4 of 128, 7 of 1,000 11.3 / 9.1, one of 8,000 14.2 / 11.6. More than seven ninths of the device's
+    // places are not for clusters, which want theirs side by side: 8 of 300 tokens (256 blocks of 296) 10.6 / 12.3, 4 of 4,000 (256) 12.1 / 15.0, 8 of 1,000 11.5 / 11.5,
+    // heads of 64, 12 of 4,096 (384 of 444) 10.6 / 13.0, 11 of up to 4,096 (352) 9.8 / 10.1.
     for (int log = a.most_pages > EA_WARPS * 8 ? 4 : 3; log >= 3 && a.cluster_log == 0; --log) {
         const long long all = (long long)a.n_seqs * a.site.kv_heads * a.chunks * ((a.most_pages + (EA_WARPS << log) - 1) / (EA_WARPS << log));
-        if (all << log <= a.block_slots && all <= clusters_of<T, D, NR>(log)) a.cluster_log = log, blocks = (int)all << log;
+        if ((all << log) * 9 <= a.block_slots * 7ll && all <= clusters_of<T, D, NR>(log)) a.cluster_log = log, blocks = (int)all << log;
     }
     a.cluster = 1 << a.cluster_log;
     cudaLaunchConfig_t config = {};
