@@ -26,9 +26,9 @@
 // differ leave no SM idle. A pair of several blocks leaves partial results (maximum, sum, output); the block that ends last, by a
 // ticket, joins them in their order, sixteen at a time, and the last of those the sixteens.
 //
-// Microseconds in a row of calls: a chat of 900 tokens, 14 heads over 2 of 64, 7.7; 8 of 4,096 9.2 (8.3 MB); one document of 32,000, 16 over 2 of 128, 14.4 (16.4 MB);
-// 64 of up to 8,000, 28 over 4 of 128, 58.3 (272 MB, 4.7 TB/s; a copy has 6.5); 256 of 8,000 each 340 (2.1 GB, 6.2 TB/s); 12 spans of up to five tokens
-// behind up to 3,000 25.4; float32, 20 of up to 3,500, 16 over 2 of 128, 14.3. Small calls are a chain: the plan from the lengths 2, first loads 1.3, the warps'
+// Microseconds in a row of calls: a chat of 900 tokens, 14 heads over 2 of 64, 7.1; 8 of 4,096 8.9 (8.3 MB); one document of 32,000, 16 over 2 of 128, 14.4 (16.4 MB);
+// 64 of up to 8,000, 28 over 4 of 128, 57.4 (272 MB, 4.7 TB/s; a copy has 6.5); 256 of 8,000 each 340 (2.1 GB, 6.2 TB/s); 12 spans of up to five tokens
+// behind up to 3,000 25.2; float32, 20 of up to 3,500, 16 over 2 of 128, 14.3. Small calls are a chain: the plan from the lengths 2, first loads 1.3, the warps'
 // merge 1.3, bringing blocks together 2 to 4. Large ones are bound by memory where lengths are even; ragged ones and spans by the issue of some 540 instructions
 // a tile of 32 positions, in 8 warps of an SM whose steps wait for their own products, exponentials and conversions.
 #include <cuda_fp16.h>
@@ -174,14 +174,18 @@ struct Sequence {
 };
 template <int ROWS> __device__ __forceinline__ Sequence sequence_of(const AttendArgs& a, int s) {
     Sequence r;
-    r.begin = a.single ? s : a.cu_q[s];   // (single: every entry has one token)
-    r.tokens = a.single ? 1 : a.cu_q[s + 1] - r.begin;
-    r.slot = r.tokens > 0 ? a.slots[s] : -1;
+    const int guess = a.single ? a.tok_pos[s] : 0;   // (single: as many tokens as entries, so most probably one each: all loads at once)
+    r.begin = a.cu_q[s];
+    r.tokens = a.cu_q[s + 1] - r.begin;
+    r.slot = a.slots[s];
+    if (r.tokens <= 0) r.slot = -1;
     r.first_pos = r.last_pos = r.page0 = r.pages = 0;
-    r.pairs = a.site.kv_heads * (a.single ? a.chunks : min(a.chunks, (int)((unsigned)(r.tokens * a.group + ROWS - 1) / ROWS)));
-    if (r.tokens > 0) {
+    r.pairs = a.site.kv_heads * min(a.chunks, (int)((unsigned)(r.tokens * a.group + ROWS - 1) / ROWS));
+    if (a.single && r.begin == s && r.tokens == 1) {
+        r.first_pos = r.last_pos = guess;
+    } else if (r.tokens > 0) {
         r.first_pos = a.tok_pos[r.begin];
-        r.last_pos = a.single ? r.first_pos : a.tok_pos[r.begin + r.tokens - 1];
+        r.last_pos = a.tok_pos[r.begin + r.tokens - 1];
     }
     if (r.slot >= 0) {
         r.page0 = a.window > 0 ? max(0, r.first_pos - a.window + 1) / QF_PAGE : 0;
@@ -214,7 +218,7 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
 __device__ __forceinline__ int place_in(int pair_begin, int block, int target) { return 2 * block + (pair_begin > block * target ? 1 : 0); }
 // Element 0 of the query (and output) of row i (token * group + head of the group) of the kv head kvh.
 template <int D> __device__ __forceinline__ long long row_offset(const AttendArgs& a, int begin, int kvh, int i) {
-    const int G = a.group, token = a.single ? 0 : i / G;
+    const int G = a.group, token = i < G ? 0 : i / G;
     return (long long)(begin + token) * a.n_heads * D + (long long)(kvh * G + i - token * G) * D;
 }
 // Item i of a row, four neighbouring components (two of a part of 16), to its row of the output.
@@ -522,8 +526,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         auto row_at = [&](int row) { return row_offset<D>(a, r.begin, kvh, row0 + row); };
         const int my_pages = max(p_end - p_begin - (int)warp + EA_WARPS - 1, 0) / EA_WARPS;   // (0 where there are fewer than warps)
         // what the rows see, lo .. hi - 1: this lane's (8 n + 2 c and + 1), all of them together, every one of them
-        const int t_first = a.single ? 0 : row0 / G, t_last = a.single ? 0 : (row0 + n_rows - 1) / G;
-        const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (a.single ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
+        const int t_first = r.tokens == 1 ? 0 : row0 / G, t_last = r.tokens == 1 ? 0 : (row0 + n_rows - 1) / G;
+        const int first_hi = (t_first == 0 ? r.first_pos : a.tok_pos[r.begin + t_first]) + 1, some_hi = (t_last == 0 ? r.first_pos : a.tok_pos[r.begin + t_last]) + 1;
         const int some_lo = a.window > 0 ? max(0, first_hi - a.window) : 0, all_lo = a.window > 0 ? max(0, some_hi - a.window) : 0;
         int lo[NR][2], hi[NR][2];
 #pragma unroll
@@ -984,7 +988,6 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
     // padding entries: zeros
     for (int s = n_blocks - 1 - blockIdx.x; s < a.n_seqs; s += n_blocks) {
         const Sequence x = sequence_of<ROWS>(a, s);
-        if (a.single && threadIdx.x == 0 && a.cu_q[s + 1] - a.cu_q[s] != 1) atomicOr(a.err, QF_ERR_ROW_RANGE);   // (an entry of other than one token)
         if (x.slot < 0)
             for (long long i = threadIdx.x; i < (long long)x.tokens * q_width; i += THREADS) out[(long long)x.begin * q_width + i] = Num<T>::from_f(0.f);
     }
@@ -1089,7 +1092,7 @@ QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim, int rows) {
     return 0;
 }
 
-// q, out [tokens][n_heads * head_dim], on 16 bytes; single: every entry has one token; rows: of a block, 8 or 16; chunks: of the longest span, ceil(tokens *
+// q, out [tokens][n_heads * head_dim], on 16 bytes; single: there are as many tokens as entries, and an entry has one at the most; rows: of a block, 8 or 16; chunks: of the longest span, ceil(tokens *
 // n_heads / kv_heads / rows); most_pages: the most pages that a sequence reads; blocks: n_seqs * kv_heads * chunks * ceil(most_pages / 4), block_slots (of
 // qf_attention_e4m3_slots) at most. part_o [2 * blocks][rows][32 * ceil(head_dim / 32)], part_ml [2 * blocks][rows][2]; tickets [4 * blocks], zero before the
 // first call and after every call.
@@ -1098,11 +1101,11 @@ QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int
                                 int head_dim, int n_heads, int n_seqs, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window, int constants,
                                 float* part_o, float* part_ml, int* tickets, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
+    if (n_seqs <= 0) return 0;
     if (head_dim <= 0 || head_dim % 16 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads || chunks <= 0 || most_pages <= 0 || most_pages >= 1 << 20 || columns <= 0 || n_slots <= 0 ||
         page_bytes % 16 || ((uintptr_t)codes | (uintptr_t)q | (uintptr_t)out) % 16 || page_bytes < 2ll * kv_heads * QF_PAGE * head_dim || page_scales < 2ll * kv_heads ||
         blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
-    if (n_seqs <= 0) return 0;
     AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, constants, 1, 0, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
 #define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
     EA_ALL(EA_ATTEND)

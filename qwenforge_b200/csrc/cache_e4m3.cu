@@ -162,15 +162,19 @@ write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lon
         grid_dependency_wait();
         return;
     }
-    const int t = run.t, first_pos = run.first_pos, at = first_pos % QF_PAGE, slot = write_cache ? slots[run.seq] : -1;
+    const int t = run.t, first_pos = run.first_pos, at = first_pos % QF_PAGE, seq = single ? min(max(run.seq, 0), n_seqs - 1) : run.seq;
+    const int entry_begin = cu_q[seq], entry_end = cu_q[seq + 1], held = slots[seq];
+    const bool inside = !single || (seq == run.seq && t >= entry_begin && t < entry_end);   // (or a row behind the last entry's, which nothing becomes of)
+    const int slot = write_cache && inside ? held : -1;
     int rows = run.rows;
-    if (rows > most_rows || (single && cu_q[run.seq + 1] - cu_q[run.seq] > 1)) {   // (an entry longer than the call has said: there is no room for its angles)
+    if (rows > most_rows || (single && inside && entry_end - entry_begin > 1)) {   // (an entry longer than the call has said: there is no room for its angles)
         if (threadIdx.x == 0) atomicOr(err, QF_ERR_ROW_RANGE);
         rows = min(rows, most_rows);
     }
     const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
     if (slot >= 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, QF_ERR_NO_PAGE);
     for (int i = threadIdx.x; i < rows * half; i += blockDim.x) turn[i] = Turns(inv_freq[i % half]).at((float)(first_pos + i / half));
+    if (!inside) rows = 0;
     __syncthreads();
     if (constants) grid_dependency_wait();   // (what is read from here on may be the output of the kernel ahead)
     for (int h = h_begin + warp; h < h_end; h += EW_WARPS) {
@@ -435,7 +439,7 @@ QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void*
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (!inv_freq) rot_dim = 0;
     if (!site_fits(site) || head_dim > 128 || rot_dim < 0 || rot_dim > head_dim || (rot_dim & 1) || n_heads <= 0 || max_q_len <= 0) return (int)cudaErrorInvalidValue;
-    if (n_tokens <= 0) return 0;
+    if (n_tokens <= 0 || n_seqs <= 0) return 0;
     return is_bf16 ? write_launch<bf16>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, constants, err, stream)
                    : write_launch<float>(qkv, bias, qkv_stride, cu_q, tok_seq, tok_pos, slots, inv_freq, rot_dim, n_heads, q_out, site, write_cache, n_tokens, n_seqs, max_q_len, constants, err, stream);
 }

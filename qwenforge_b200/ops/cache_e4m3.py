@@ -100,7 +100,7 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     if n and max_q_len <= 0:
         raise KernelError("rope_cache_write_e4m3: max_q_len is the most tokens of an entry")
     _here("rope_cache_write_e4m3", qkv, cu_q, tok_seq, tok_pos, slots, inv_freq, q_out, site.storage, site.scales, site.table, err, bias)
-    if n == 0:
+    if n == 0 or slots.numel() == 0:
         return
     _check(_function("cache_e4m3", "qf_rope_cache_write_e4m3", _I, _P, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _P, *_SITE, _I, _I, _I, _I, _I, _P, _P)(
         is_bf16, qkv.data_ptr(), _at(bias), qkv.stride(0), cu_q.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), _at(inv_freq), rot_dim,
@@ -216,7 +216,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     if n_seqs and (max_q_len <= 0 or (max_kv_len is not None and max_kv_len <= 0)):
         raise KernelError("attention_e4m3: max_q_len and max_kv_len bound an entry's tokens and its sequence's length")
     _here("attention_e4m3", q, out, cu_q, tok_pos, slots, site.storage, site.scales, site.table, err)
-    if q.shape[0] == 0:
+    if q.shape[0] == 0 or n_seqs == 0:
         return
     columns = site.table.shape[1]
     most = columns if max_kv_len is None else min(columns, -(-int(max_kv_len) // PAGE_TOKENS))

@@ -204,6 +204,18 @@ def test_pages_that_are_not_held_and_lengths_beyond_the_bound():
     assert int(c.err) & (ops.ERR_NO_PAGE | 32)
 
 
+@BOTH
+def test_as_many_rows_as_entries_but_not_one_each(dtype):
+    """An entry without a token, and a row behind the last entry, which stays as it is."""
+    c = Case([(700, 1), (90, 0), (300, 1), (20, 1, True)], 14, 2, 64, dtype, seed=3)
+    q = torch.cat((query(Case([(0, 3)], 14, 2, 64, dtype)), torch.full((1, 14 * 64), 3.0, dtype=dtype)))
+    out = torch.full((4, 14 * 64), 9.0, dtype=dtype, device="cuda")
+    tok_pos = torch.cat((c.dev["tok_pos"], c.dev["tok_pos"].new_tensor([5])))
+    ops.attention_e4m3(q.cuda(), out, c.dev["cu_q"], tok_pos, c.dev["slots"], c.site, 14, 4, 1, 64 ** -0.5, 0, ops.E4m3Scratch("cuda"), c.err)
+    check(c, q[:3], out[:3])
+    assert bool((out[3] == 9).all()) and not bool(out[2].any())
+
+
 def test_a_captured_call_replayed_with_other_lengths():
     """The launch is the same whatever the lengths: runs are cut on the device."""
     c = Case([(900, 1), (40, 1), (3000, 1)], 14, 2, 64, torch.bfloat16, seed=3)

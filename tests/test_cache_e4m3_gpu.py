@@ -247,6 +247,28 @@ def test_no_tokens_and_no_sequences():
     assert torch.equal(c.storage.cpu().view(torch.uint8), c.codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("of", [0, 1, 7], ids=["of the first", "of the last", "of none"])
+def test_a_row_behind_the_last_entry(of):
+    """Whatever it says it is of."""
+    c = Case([(70, 1), (5, 1)], 4, 2, 64, torch.bfloat16)
+    more = lambda x, v: torch.cat((x, x.new_tensor([v])))   # noqa: E731
+    qkv, q_out = torch.cat((c.qkv, c.qkv[:1] + 1)).cuda(), torch.full((3, 4 * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.rope_cache_write_e4m3(qkv, c.dev["cu_q"], more(c.dev["tok_seq"], of), more(c.dev["tok_pos"], 3), c.dev["slots"], c.inv_freq.cuda(), c.rot_dim, 4, q_out, c.site, 1,
+                              c.err, bias=None if c.bias is None else c.bias.cuda())
+    c.check(q_out[:2])
+    assert bool((q_out[2] == 7).all()) and int(c.err) == 0
+
+
+def test_rows_but_no_entry():
+    c = Case([(0, 1)], 4, 2, 64, torch.bfloat16)
+    none, one = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q_out = torch.full((1, 256), 7.0, dtype=torch.bfloat16, device="cuda")
+    for most in (1, 70):
+        ops.rope_cache_write_e4m3(c.qkv.cuda(), one, one, one, none, None, 0, 4, q_out, c.site, most, c.err)
+    ops.attention_e4m3(q_out.clone(), q_out, one, one, none, c.site, 4, 0, 1, 0.125, 0, ops.E4m3Scratch("cuda"), c.err)
+    assert bool((q_out == 7).all()) and torch.equal(c.storage.cpu().view(torch.uint8), c.codes.view(torch.uint8)) and int(c.err) == 0
+
+
 def test_an_entry_longer_than_the_call_says():
     c = Case([(0, 9)], 4, 2, 64, torch.bfloat16)
     c.most = 4
