@@ -221,6 +221,21 @@ def test_read_back(dtype, heads, kv_heads, dim, window):
     assert torch.equal(pages.cpu(), want) and bool((out[:, -16:] == 5).all()) and int(c.err) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("window", [1, 10, 64, 130])
+def test_read_back_of_long_spans_behind_short_windows(dtype, window):
+    """More pages than a window has: a block takes several."""
+    c = Case([(500, 700), (1000, 3), (65, 191), (0, 1)], 4, 2, 48, dtype, seed=5)
+    out = torch.full(c.codes.shape, 5.0, dtype=dtype, device="cuda")
+    ops.cache_read_e4m3(out, c.dev["cu_q"], c.dev["tok_pos"], c.dev["slots"], c.site, c.n, 1200, c.err, window=window)
+    want = torch.full(c.codes.shape, 5.0, dtype=dtype)
+    for s in range(c.n):
+        for p in range(max(0, int(c.tok_pos[c.cu_q[s]]) - window + 1), int(c.tok_pos[c.cu_q[s + 1] - 1]) + 1):
+            page = int(c.table[c.slots[s], p // PAGE])
+            want[page, :, :, p % PAGE] = (c.codes[page, :, :, p % PAGE].double() * c.scales[page].double()[..., None]).to(dtype)
+    assert torch.equal(out.cpu(), want) and int(c.err) == 0
+
+
 def test_read_back_is_exact_in_bfloat16():
     """Every code times scales at both ends of the range: the product has four bits, within bfloat16's exponents."""
     c = Case([(0, 64), (0, 64)], 1, 1, 16, torch.bfloat16, seed=4)
