@@ -212,7 +212,9 @@ class PrefillGraphs:
     multiple of a granule (64 tokens up to 512, then 128, 256 and 512: at most an eighth more work), and the longest
     entry is rounded up likewise (blocks of rows that no entry has end at once). A step whose token count is a
     multiple of the granule already gets no padding entry. The second step of a rounded shape is captured, with its
-    integers in a buffer of the graph's own; every later one copies its integers there and replays. Steps of more
+    integers in a buffer of the graph's own; every later one copies its integers there and replays. With a cache in 8
+    bits the shape has a bound on the lengths, too (a power of two, as the decode graphs' has): the attention over codes
+    reads no further than the bound that it is launched with. Steps of more
     than `MAX_TOKENS` tokens are bound by the GPU and are left alone, as are single-token steps (the decode graphs'
     business). The newest `keep` graphs are kept; they share one memory pool, since no two run at the same time.
     """
@@ -251,6 +253,9 @@ class PrefillGraphs:
         as it is; the second time a rounded shape comes it is captured here and its logits are returned)."""
         step = self.rounded(step, triples, want)
         key = (cache.serial,) + step.shape_key
+        if self.model.cache_dtype is not None:
+            step = dataclasses.replace(step, max_kv_len=length_bound(step.max_kv_len))
+            key += (step.max_kv_len,)
         held = self.graphs.pop(key, None)
         if held is None:
             self.seen[key] = self.seen.get(key, 0) + 1
