@@ -41,6 +41,10 @@
 #define EA_WARPS 4
 #define EA_DEAD 0x7fffffff   // the exponent of a tile that is not there, or that no row sees
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
+// How far (in powers of two) the values' units of a warp's pages may be from the one at which it last measured its outputs before it measures them again. An output is
+// within 2^40 units of one page (2^14 weights, 448, some hundred thousand positions), so that with three times this there is room for float32's 2^127 however
+// the units fall and rise.
+#define EA_APART 10
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
@@ -675,6 +679,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
 #pragma unroll
         for (int n = 0; n < NR; ++n) m_run[n][0] = m_run[n][1] = EA_NONE, l_run[n][0] = l_run[n][1] = 0.f, unit_run[n][0] = unit_run[n][1] = 0;
         bool begun = false;
+        int unit_measured = 0;   // of the values at which the outputs were last measured, or begun; far from all where a row's outputs stand far from it
 
         unsigned stage = S::STAGES - 1;   // (of the step before the first)
         for (unsigned step = 0; step < steps; ++step) {
@@ -688,6 +693,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             if (!begun) {
 #pragma unroll
                 for (int n = 0; n < NR; ++n) unit_run[n][0] = unit_run[n][1] = unit_v;
+                unit_measured = unit_v;
                 begun = true;
             }
             const unsigned char* keys = stage0 + stage * S::STAGE + g * S::PITCH;
@@ -782,15 +788,12 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     add(2 * w + d, f);
                 }
             };
-            bool far = false;   // an output is within 2^40 units (2^14 weights, 448, some thousand pages): there is room for 2^30 more
+            bool far = abs(unit_measured - unit_v) > EA_APART;
             int up[NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    up[n][e] = unit_run[n][e] - unit_v;
-                    far |= abs(up[n][e]) > 30;
-                }
+                for (int e = 0; e < 2; ++e) up[n][e] = unit_run[n][e] - unit_v;
             if (!full && t_first != t_last) {   // a NaN that some of the rows do not see must not reach them: 0 * NaN
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
@@ -858,6 +861,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                 // scales far apart, or a NaN: a unit in which what was there (2^had at most) and what comes (2^comes) both have room, and token by
                 // token, each with the positions that it sees
                 int shift_new[NR][2];
+                bool apart = false;
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -877,7 +881,9 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
 #pragma unroll
                             for (int h = 0; h < 2; ++h) o[d][n][2 * h + e] = ldexpf(o[d][n][2 * h + e] * corr[n][e], unit_run[n][e] - unit_both);
                         unit_run[n][e] = unit_both;
+                        apart |= abs(unit_both - unit_v) > EA_APART;
                     }
+                unit_measured = __any_sync(0xffffffffu, apart) ? 1000 : unit_v;
                 for (int token = t_first; token <= t_last; ++token) {
                     const int upto = t_first == t_last ? first_hi : a.tok_pos[r.begin + token] + 1, from = a.window > 0 ? upto - a.window : 0;
 #pragma unroll
