@@ -725,11 +725,23 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) load_value<D>(vw[kt][i], values + (16 * kt + (i & 1) + 8 * (i >> 1)) * S::PITCH, g);
-            // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none
+            // ---- with care (below): scales far apart, or a NaN that some of the rows do not see and that must not reach them, 0 * NaN
             const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
+            bool care = abs(unit_measured - unit_v) > EA_APART;
+            if (!full && t_first != t_last) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) care |= holds_nan(vw[kt][i][w]);
+            }
+            care = __any_sync(0xffffffffu, care);
+            // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none. With care they are those under the tile's own
+            // maximum, so that float16 keeps them however far below the row's they lie: their values may be as much larger
             float corr[NR][2], m_tile[NR][2];
             uint32_t pb[TERMS][KT][NR][2];
-            auto weigh = [&](auto whole) {
+            auto weigh = [&](auto whole, auto own) {
                 auto seen = [&](int t, int n, int e) {
                     if (decltype(whole)::value) return true;
                     const int key = key0 + 16 * t + 8 * (e >> 1) + g;
@@ -737,7 +749,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                 };
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    float top[2] = {EA_NONE, EA_NONE}, shift[2], by_k[2];
+                    float top[2] = {EA_NONE, EA_NONE}, shift[2], by_k[2], sum[2] = {0.f, 0.f};
 #pragma unroll
                     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -752,7 +764,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         const float m = fmaxf(m_run[n][e], m_tile[n][e]);
                         corr[n][e] = fast_exp2(m_run[n][e] - m);
                         m_run[n][e] = m;
-                        shift[e] = 14.f - m;
+                        shift[e] = 14.f - (decltype(own)::value ? m_tile[n][e] : m);
                         l_run[n][e] *= corr[n][e];
                     }
 #pragma unroll
@@ -762,7 +774,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         for (int e = 0; e < 4; ++e) {
                             x[e] = fast_exp2(fmaf(x[e], by_k[e & 1], shift[e & 1]));
                             if (!seen(t, n, e)) x[e] = 0.f;
-                            l_run[n][e & 1] += x[e];
+                            if (decltype(own)::value) sum[e & 1] += x[e];
+                            else l_run[n][e & 1] += x[e];
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -771,10 +784,15 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                             if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
                         }
                     }
+                    if (decltype(own)::value) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) l_run[n][e] = fmaf(fast_exp2(m_tile[n][e] - m_run[n][e]), sum[e], l_run[n][e]);
+                    }
                 }
             };
-            if (full) weigh(std::true_type{});
-            else weigh(std::false_type{});
+            if (care) weigh(std::false_type{}, std::true_type{});
+            else if (full) weigh(std::true_type{}, std::false_type{});
+            else weigh(std::false_type{}, std::false_type{});
             // ---- values. Word w of the four positions of a step holds their elements of the component columns 4 w .. 4 w + 3
             auto word_products = [&](int kt, int w, auto take, auto add) {
                 uint32_t x[4];
@@ -788,28 +806,14 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     add(2 * w + d, f);
                 }
             };
-            bool far = abs(unit_measured - unit_v) > EA_APART;
-            int up[NR][2];
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) up[n][e] = unit_run[n][e] - unit_v;
-            if (!full && t_first != t_last) {   // a NaN that some of the rows do not see must not reach them: 0 * NaN
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) far |= holds_nan(vw[kt][i][w]);
-            }
-            if (!__any_sync(0xffffffffu, far)) {
+            if (!care) {
                 float f[NR][2];
                 bool moved = false;
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        f[n][e] = corr[n][e] * pow2(up[n][e]);
+                        f[n][e] = corr[n][e] * pow2(unit_run[n][e] - unit_v);
                         moved |= f[n][e] != 1.f;
                         unit_run[n][e] = unit_v;
                     }
@@ -858,9 +862,10 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                             });
                 }
             } else {
-                // scales far apart, or a NaN: a unit in which what was there (2^had at most) and what comes (2^comes) both have room, and token by
-                // token, each with the positions that it sees
+                // a unit in which what was there (2^had at most) and what comes (2^comes) both have room, and token by token, each with the positions that
+                // it sees
                 int shift_new[NR][2];
+                float share[NR][2];   // of the tile's own weights in the row's, with 2^shift_new
                 bool apart = false;
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
@@ -873,9 +878,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         for (int i = 4; i < 32; i <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
                         most *= corr[n][e];
                         const int had = most > 0.f ? unit_run[n][e] + exponent_of(most) : -1000;
-                        const int comes = unit_v + 30 + (int)fmaxf(m_tile[n][e] - m_run[n][e], -800.f);
+                        const float below = fmaxf(m_tile[n][e] - m_run[n][e], -800.f), whole = floorf(below);
+                        share[n][e] = fast_exp2(below - whole);
+                        const int comes = unit_v + 30 + (int)whole;
                         const int unit_both = max(max(had, comes) - 30, -150);
-                        shift_new[n][e] = unit_v - unit_both;
+                        shift_new[n][e] = unit_v + (int)whole - unit_both;
 #pragma unroll
                         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -909,7 +916,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                             for (int n = 0; n < NR; ++n)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
-                                    if ((row0 + 8 * n + 2 * c + (e & 1)) / G == token) o[2 * w + d][n][e] += ldexpf(acc[d][n][e], shift_new[n][e & 1]);
+                                    if ((row0 + 8 * n + 2 * c + (e & 1)) / G == token) o[2 * w + d][n][e] += ldexpf(acc[d][n][e] * share[n][e & 1], shift_new[n][e & 1]);
                         }
                     }
                 }

@@ -146,3 +146,25 @@ def test_values_of_scales_that_fall_and_rise(stairs, heads, kv_heads, dim, token
     b.codes[:, 0] = torch.ones((), device="cuda").to(torch.float8_e4m3fn)
     b.scales[:, 1] = torch.exp2(e.repeat_interleave(4).repeat(2).float()).cuda()[:, None]
     b.check()
+
+
+# A position of group g scores -`fall` g in base 2, its values stand `rise` binary places above those of the group before: what it adds is 2^((rise - fall) g).
+@pytest.mark.parametrize("fall,rise", [(20, 25), (5, 11), (8, 9), (8, 8), (11, 10), (25, 20), (28, 31)])   # (31 * 4 - 8 is within the scales' 119)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens", [(4, 2, 64, 1), (14, 2, 64, 2), (8, 4, 128, 1), (12, 4, 128, 4)])
+@pytest.mark.parametrize("first", [True, False], ids=["largest weight first", "largest weight last"])
+@BOTH
+def test_large_values_of_small_weight(first, heads, kv_heads, dim, tokens, fall, rise, dtype):
+    """Weights down to 2^-112 beside values that outweigh them."""
+    groups = 5
+    n = 512 // kv_heads
+    order = torch.arange(groups) if first else torch.arange(groups).flip(0)
+    per = 4 * groups
+    pages = torch.arange(per) + per * (torch.arange(n) % 2)[:, None]
+    b = Batch(pages, [per * PAGE - 3 * (i % 5) for i in range(n)], [tokens] * n, heads, kv_heads, dim, dtype, pool=2 * per)
+    g = order.repeat_interleave(4).repeat(2).float().cuda()
+    b.codes[:, 0] = (-g).view(-1, 1, 1, 1).expand(b.codes[:, 0].shape).to(torch.float8_e4m3fn)   # (whole numbers up to 16 are codes)
+    b.scales[:, 0] = 1.0
+    b.scales[:, 1] = torch.exp2(rise * g - 8)[:, None]
+    b.q.fill_(1.0)
+    # every score is -g dim scale: exact but for the factor's rounding, so a weight is as exact as its exponential
+    b.check(scale=fall * math.log(2.0) / dim)
