@@ -7,7 +7,8 @@
 // Queries become float16 behind a power of two per row that brings their largest element to 2^7 .. 2^8: bfloat16 queries lose nothing but
 // what lies 2^-31 below that, float32 queries are two such numbers (22 bits) and take two products. Weights are 2^(s - m + 14), at most 2^14
 // for the running maximum m: rounded to float16 (2^-11 of each weight, an eighth of the output's own rounding) where the output is bfloat16,
-// two numbers where it is float32. Maxima, sums and outputs are float32. The tensor cores' additions cut off bits below 2^-23 of a sum; for float32
+// two numbers where it is float32; either ends at 2^-24, so a weight below 2^-28 of the row's largest is kept to 2^-39 of that (where values' scales are far
+// apart, of the tile's largest). Maxima, sums and outputs are float32. The tensor cores' additions cut off bits below 2^-23 of a sum; for float32
 // outputs their sums end with a tile, for bfloat16 they go on over a warp's pages (2^-14 after 8,000 positions).
 //
 // A block takes pages of a (sequence, kv head, 8 or 16 rows), its warps a page each in turn; a warp looks its next 32 pages and their scales up
@@ -45,6 +46,9 @@
 // within 2^40 units of one page (2^14 weights, 448, some hundred thousand positions), so that with three times this there is room for float32's 2^127 however
 // the units fall and rise.
 #define EA_APART 10
+// Scores in base 2 up to which a weight's exponent is score - (maximum - 14), in float32: that is within one of 14 at the most, and off by no more than a score's own
+// rounding. (From 2^25 on the largest weight could be float16's infinity.) Where scores may be larger, the maximum is taken off the rounded score first.
+#define EA_LARGE 8388608.f
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
@@ -630,6 +634,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         // ---- the queries' fragments: lane (g, c) has row g's components of its column
         uint32_t qb[TERMS][NR][KW][2];
         float by[NR][2];   // scores of rows 8 n + 2 c + e in base-2 units: product * key scale * by
+        float most_by = 0.f;   // key scale * this is no less than any score: products of a row lie within D * 2^8 * 448
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             float2 x[KW][2];
@@ -659,6 +664,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             const float mine = pow2(up) * fabsf(a.scale_log2), down = copysignf(pow2(-up), a.scale_log2);
             by[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
             by[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
+            most_by = fmaxf(most_by, mine);
 #pragma unroll
             for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -668,6 +674,8 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     if constexpr (TWO) qb[TERMS - 1][n][w][i] = pack_rest(u, v, qb[0][n][w][i]);
                 }
         }
+
+        most_by = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_by))) * (D * 256.f * 448.f);   // (positive: in their bits' order)
 
         float o[DT][NR][4];   // components of columns 2 d (0, 1) and 2 d + 1 (2, 3) by rows 2 c, 2 c + 1
 #pragma unroll
@@ -725,23 +733,13 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) load_value<D>(vw[kt][i], values + (16 * kt + (i & 1) + 8 * (i >> 1)) * S::PITCH, g);
-            // ---- with care (below): scales far apart, or a NaN that some of the rows do not see and that must not reach them, 0 * NaN
             const bool full = key0 >= all_lo && key0 + TILE <= first_hi;
-            bool care = abs(unit_measured - unit_v) > EA_APART;
-            if (!full && t_first != t_last) {
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) care |= holds_nan(vw[kt][i][w]);
-            }
-            care = __any_sync(0xffffffffu, care);
-            // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none. With care they are those under the tile's own
-            // maximum, so that float16 keeps them however far below the row's they lie: their values may be as much larger
+            // ---- weights. What a row does not see is EA_NONE on the way to the maximum, and has none. Where scales are far apart, or scores may be large, they
+            // are those under the tile's own maximum, so that float16 keeps them however far below the row's they lie: their values may be as much larger
+            const bool own = abs(unit_measured - unit_v) > EA_APART || !(ks * most_by <= EA_LARGE);
             float corr[NR][2], m_tile[NR][2];
             uint32_t pb[TERMS][KT][NR][2];
-            auto weigh = [&](auto whole, auto own) {
+            auto weigh = [&](auto whole, auto under_own) {
                 auto seen = [&](int t, int n, int e) {
                     if (decltype(whole)::value) return true;
                     const int key = key0 + 16 * t + 8 * (e >> 1) + g;
@@ -760,11 +758,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         by_k[e] = by[n][e] * ks;
 #pragma unroll
                         for (int i = 4; i < 32; i <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], i));
-                        m_tile[n][e] = top[e] > EA_NONE ? top[e] * by_k[e] : EA_NONE;
+                        m_tile[n][e] = top[e] > EA_NONE ? __fmul_rn(top[e], by_k[e]) : EA_NONE;
                         const float m = fmaxf(m_run[n][e], m_tile[n][e]);
                         corr[n][e] = fast_exp2(m_run[n][e] - m);
                         m_run[n][e] = m;
-                        shift[e] = 14.f - (decltype(own)::value ? m_tile[n][e] : m);
+                        shift[e] = 14.f - m;
                         l_run[n][e] *= corr[n][e];
                     }
 #pragma unroll
@@ -772,9 +770,11 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         float(&x)[4] = s[t][n];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            x[e] = fast_exp2(fmaf(x[e], by_k[e & 1], shift[e & 1]));
+                            if (decltype(under_own)::value) x[e] = __fadd_rn(__fsub_rn(__fmul_rn(x[e], by_k[e & 1]), m_tile[n][e & 1]), 14.f);
+                            else x[e] = fmaf(x[e], by_k[e & 1], shift[e & 1]);
+                            x[e] = fast_exp2(x[e]);
                             if (!seen(t, n, e)) x[e] = 0.f;
-                            if (decltype(own)::value) sum[e & 1] += x[e];
+                            if (decltype(under_own)::value) sum[e & 1] += x[e];
                             else l_run[n][e & 1] += x[e];
                         }
 #pragma unroll
@@ -784,15 +784,25 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                             if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
                         }
                     }
-                    if (decltype(own)::value) {
+                    if (decltype(under_own)::value) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) l_run[n][e] = fmaf(fast_exp2(m_tile[n][e] - m_run[n][e]), sum[e], l_run[n][e]);
+                        for (int e = 0; e < 2; ++e) l_run[n][e] = fmaf(fast_exp2(__fsub_rn(m_tile[n][e], m_run[n][e])), sum[e], l_run[n][e]);
                     }
                 }
             };
-            if (care) weigh(std::false_type{}, std::true_type{});
+            if (__builtin_expect(own, 0)) weigh(std::false_type{}, std::true_type{});
             else if (full) weigh(std::true_type{}, std::false_type{});
             else weigh(std::false_type{}, std::false_type{});
+            bool by_token = false;   // a NaN that some of the rows do not see must not reach them: 0 * NaN
+            if (!full && t_first != t_last) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) by_token |= holds_nan(vw[kt][i][w]);
+                by_token = __any_sync(0xffffffffu, by_token);
+            }
             // ---- values. Word w of the four positions of a step holds their elements of the component columns 4 w .. 4 w + 3
             auto word_products = [&](int kt, int w, auto take, auto add) {
                 uint32_t x[4];
@@ -806,7 +816,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                     add(2 * w + d, f);
                 }
             };
-            if (!care) {
+            if (__builtin_expect(!own && !by_token, 1)) {
                 float f[NR][2];
                 bool moved = false;
 #pragma unroll
@@ -878,9 +888,9 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         for (int i = 4; i < 32; i <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
                         most *= corr[n][e];
                         const int had = most > 0.f ? unit_run[n][e] + exponent_of(most) : -1000;
-                        const float below = fmaxf(m_tile[n][e] - m_run[n][e], -800.f), whole = floorf(below);
+                        const float below = own ? fmaxf(__fsub_rn(m_tile[n][e], m_run[n][e]), -800.f) : 0.f, whole = floorf(below);
                         share[n][e] = fast_exp2(below - whole);
-                        const int comes = unit_v + 30 + (int)whole;
+                        const int comes = unit_v + 30 + (own ? (int)whole : (int)fmaxf(m_tile[n][e] - m_run[n][e], -800.f));
                         const int unit_both = max(max(had, comes) - 30, -150);
                         shift_new[n][e] = unit_v + (int)whole - unit_both;
 #pragma unroll

@@ -71,9 +71,19 @@ class Batch:
             far[rows] = (reach.amax(-1) * abs(scale)).reshape(t, self.heads, 1)
         return out, size, far
 
-    def check(self, window=0, scale=None):
+    def check(self, window=0, scale=None, same_scores=False, floor=False):
+        """`same_scores`: what differs between scores is so large that it leaves weights of 0, or nothing at all.
+        `floor`: components may come from weights alone that are far below the row's largest, where the others' values are zero. A weight is a float16 number (or two)
+        that is 2^14 where it is the largest; float16's smallest step is 2^-24, so a weight is off by 2^-25 / 2^14 = 2^-39 of the largest one however small it is
+        itself, the largest is at most 1, and the sum of all is no less than it: 2^-39 of every value that a row sees."""
         got, (want, size, far) = self.run(window, scale), self.plain(window, scale)
+        if same_scores:
+            far.zero_()
         off = (got.double().view(want.shape) - want).abs() - ref.attend_tolerance(want, size, far, self.dtype)
+        if floor:
+            values = (self.codes[:, 1].double().abs() * self.scales[:, 1].double()[..., None, None]).amax((0, 2))   # [kv heads, dim]
+            counts = (self.tok_pos + 1).double()[:, None, None]
+            off -= 2.0 ** -39 * counts * values.repeat_interleave(self.heads // self.kv_heads, 0)
         assert bool((off <= 0).all()), f"{float(off.max())} beyond the tolerance"
         assert torch.equal(self.run(window, scale), got)
 
@@ -168,3 +178,50 @@ def test_large_values_of_small_weight(first, heads, kv_heads, dim, tokens, fall,
     b.q.fill_(1.0)
     # every score is -g dim scale: exact but for the factor's rounding, so a weight is as exact as its exponential
     b.check(scale=fall * math.log(2.0) / dim)
+
+
+def large_batch(seqs, heads, kv_heads, dim, tokens, dtype):
+    """Every query and key component 1, in pages of which one has a key scale of 2 and codes of 1/2."""
+    pages, lengths = scattered(seqs, 1500, seed=4)
+    b = Batch(pages, lengths, [min(x, tokens) for x in lengths], heads, kv_heads, dim, dtype)
+    b.q.fill_(1.0)
+    b.codes[:, 0] = torch.ones((), device="cuda").to(torch.float8_e4m3fn)
+    b.codes[::3, 0] = torch.full((), 0.5, device="cuda").to(torch.float8_e4m3fn)
+    b.scales[:, 0] = 1.0
+    b.scales[::3, 0] = 2.0
+    return b
+
+
+LARGE = pytest.mark.parametrize("score", [1e4, 3e4, 3e7, 1e8, -1e8, 1e12, -1e12, 1e30])
+FEW_AND_MANY = pytest.mark.parametrize("seqs,heads,kv_heads,dim,tokens", [(3, 14, 2, 64, 1), (3, 28, 4, 128, 4), (200, 8, 4, 64, 1), (200, 8, 2, 128, 3)])
+
+
+@LARGE
+@FEW_AND_MANY
+@BOTH
+def test_equal_scores_of_any_size(seqs, heads, kv_heads, dim, tokens, score, dtype):
+    """Even weights."""
+    large_batch(seqs, heads, kv_heads, dim, tokens, dtype).check(scale=score / dim, same_scores=True)
+
+
+@LARGE
+@FEW_AND_MANY
+@BOTH
+def test_scores_of_any_size_that_differ(seqs, heads, kv_heads, dim, tokens, score, dtype):
+    """One position of a page scores half of (or, where scores are negative, twice) what the others do: these have weights of exp(-5000) and less, zero in 64 bits too."""
+    b = large_batch(seqs, heads, kv_heads, dim, tokens, dtype)
+    other = b.codes.clone()
+    b.codes[:, 0] = (b.codes[:, 0].float() * (0.5 if score > 0 else 2.0)).to(torch.float8_e4m3fn)
+    b.codes[:, 0, :, 0] = other[:, 0, :, 0]   # the first position of every page, which every token sees
+    b.check(scale=score / dim, same_scores=True)
+
+
+@pytest.mark.parametrize("spread", [1e3, 1e6, 1e20])
+@FEW_AND_MANY
+@BOTH
+def test_random_scores_of_any_size(seqs, heads, kv_heads, dim, tokens, spread, dtype):
+    pages, lengths = scattered(seqs, 1500, seed=5)
+    b = Batch(pages, lengths, [min(x, tokens) for x in lengths], heads, kv_heads, dim, dtype)
+    b.q = (b.q.float() * spread).to(dtype)
+    b.check(floor=True)
+    assert bool((b.run().view(-1, dim) != 0).any(-1).all())   # (so loose a tolerance would let a row of zeros pass)
