@@ -150,7 +150,8 @@ def attention_e4m3_pays(dtype: torch.dtype, max_q_len: int, group: int) -> bool:
 
 
 class E4m3Scratch:
-    """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). One
+    """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). Sized for
+    as many blocks as the device holds at once, whatever the lengths, so that only another head size or more rows of a block ask for more (2 to 10 MB). One
     instance serves calls that run one after another on one stream; what is captured into a graph has one of its own. Should a captured call
     share one all the same, its replays take their turn like calls: what a call outgrows is kept as long as the instance, because a graph may hold its address."""
     TICKETS = 4096   # four for each of 1,024 blocks, the most that a launch has; zero from here on, where memory that a capture hands out is not
@@ -227,7 +228,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     chunks = -(-rows // block_rows)
     block_slots = _slots_of(is_bf16, d, block_rows)
     blocks = min(block_slots, n_seqs * kv_heads * chunks * -(-most // E4M3_WARPS))
-    scratch.ensure(blocks, d, block_rows)
+    scratch.ensure(block_slots, d, block_rows)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
     _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _P)(
         is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.place, n_heads, n_seqs,
