@@ -169,8 +169,8 @@ write_any_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lon
     const bool inside = !single || (seq == run.seq && t >= entry_begin && t < entry_end);   // (or a row behind the last entry's, which nothing becomes of)
     const int slot = write_cache && inside ? held : -1;
     int rows = run.rows;
-    if (rows > most_rows || (single && inside && entry_end - entry_begin > 1)) {   // (an entry longer than the call has said: there is no room for its angles)
-        if (threadIdx.x == 0) atomicOr(err, QF_ERR_ROW_RANGE);
+    if (rows > most_rows || (single && inside && entry_end - entry_begin > 1)) {   // (an entry longer than the call has said: there is no room for its angles.
+        if (threadIdx.x == 0 && held >= 0) atomicOr(err, QF_ERR_ROW_RANGE);          // A padding entry may be: nobody asks for its queries)
         rows = min(rows, most_rows);
     }
     const int page = slot >= 0 ? e4m3_page(site, slot, first_pos) : -1;
@@ -456,7 +456,7 @@ static bool site_fits(const E4m3Site& s) {
 }
 
 // qkv [n_tokens][qkv_stride]: q heads, then k heads, then v heads; bias as a row, or null; inv_freq null: no rotation. Every entry's tokens
-// stand at consecutive positions; max_q_len: the most tokens of an entry. q_out [n_tokens][n_heads * head_dim].
+// stand at consecutive positions; max_q_len: the most tokens of an entry that has a slot. q_out [n_tokens][n_heads * head_dim].
 QF_EXPORT int qf_rope_cache_write_e4m3(int is_bf16, const void* qkv, const void* bias, long long qkv_stride, const int* cu_q, const int* tok_seq,
                                        const int* tok_pos, const int* slots, const float* inv_freq, int rot_dim, int n_heads, void* q_out, void* codes,
                                        float* scales, const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots,

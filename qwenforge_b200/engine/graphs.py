@@ -214,7 +214,9 @@ class PrefillGraphs:
     multiple of the granule already gets no padding entry. The second step of a rounded shape is captured, with its
     integers in a buffer of the graph's own; every later one copies its integers there and replays. With a cache in 8
     bits the shape has a bound on the lengths, too (a power of two, as the decode graphs' has): the attention over codes
-    reads no further than the bound that it is launched with. Steps of more
+    reads no further than the bound that it is launched with; and a bound on the entries that have a slot, apart from the
+    padding entry's tokens (the next even number up to 32, then the longest entry's), so that short spans go the way that is
+    theirs: attended over as codes. Steps of more
     than `MAX_TOKENS` tokens are bound by the GPU and are left alone, as are single-token steps (the decode graphs'
     business). The newest `keep` graphs are kept; they share one memory pool, since no two run at the same time.
     """
@@ -235,6 +237,10 @@ class PrefillGraphs:
     def granule(n_tokens: int) -> int:
         return 64 if n_tokens <= 512 else 128 if n_tokens <= 2048 else 256 if n_tokens <= 4096 else 512
 
+    @staticmethod
+    def span_bound(longest: int, rounded: int) -> int:
+        return longest + longest % 2 if longest <= 32 else rounded
+
     @classmethod
     def rounded(cls, step, triples, want):
         """The step brought to its rounded shape (see the class): the same entries and wanted places, then one padding
@@ -251,11 +257,12 @@ class PrefillGraphs:
     def run(self, cache, step, triples, want) -> Optional[torch.Tensor]:
         """The step's logits by replay, or None if its rounded shape has no graph yet (the caller then runs the step
         as it is; the second time a rounded shape comes it is captured here and its logits are returned)."""
+        longest = step.max_q_len
         step = self.rounded(step, triples, want)
         key = (cache.serial,) + step.shape_key
         if self.model.cache_dtype is not None:
-            step = dataclasses.replace(step, max_kv_len=length_bound(step.max_kv_len))
-            key += (step.max_kv_len,)
+            step = dataclasses.replace(step, max_kv_len=length_bound(step.max_kv_len), max_span=self.span_bound(longest, step.max_q_len))
+            key += (step.max_kv_len, step.max_span)
         held = self.graphs.pop(key, None)
         if held is None:
             self.seen[key] = self.seen.get(key, 0) + 1

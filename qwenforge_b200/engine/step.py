@@ -39,6 +39,8 @@ class StepContext:
     # of the attention over it
     cache_dtype: Optional[torch.dtype] = None
     codes_scratch: Optional[object] = None
+    # the most tokens of an entry that has a slot, where a padding entry has more (None: max_q_len)
+    max_span: Optional[int] = None
     # per-token side inputs named by whoever feeds the step, [T, ...] on the device: what a part needs beyond a
     # token's index in its sequence (positions on several axes, token types). `tok_pos` stays the index that
     # orders the cache and the causal mask.
@@ -73,6 +75,7 @@ class PackedStep:
     host_slots: list
     host_starts: list
     host_q_lens: list
+    max_span: Optional[int] = None
 
     @property
     def shape_key(self) -> tuple:
@@ -127,7 +130,7 @@ def context_of(step: PackedStep, dev: torch.Tensor, err: torch.Tensor, dtype: to
         n_seqs=n, n_tokens=total, max_q_len=step.max_q_len, max_kv_len=step.max_kv_len,
         token_ids=take(total), tok_seq=take(total), tok_pos=take(total), slots=take(n), cu_q=take(n + 1),
         want_rows=take(step.n_rows) if step.n_rows else None, err=err, dtype=dtype, attention=attention,
-        decode_scratch=decode_scratch, codes_scratch=codes_scratch,
+        decode_scratch=decode_scratch, codes_scratch=codes_scratch, max_span=step.max_span,
         host_slots=step.host_slots, host_starts=step.host_starts, host_q_lens=step.host_q_lens,
     )
 

@@ -69,7 +69,8 @@ def rope_cache_write_e4m3(qkv: torch.Tensor, cu_q: torch.Tensor, tok_seq: torch.
     A page that gets rows takes, per plane and head, the least power of two under which all their finite elements lie within +-448 (of 2^-112
     to 2^119), and no less than it has if it held rows before the new ones; those rows' codes are then rounded to the larger unit. Rounding is
     to nearest even, once, from float32. Infinities become +-448, NaN stays. Rows behind the new ones stay as they are; a padding
-    entry (slot -1) writes its queries only, as does every entry with `write_cache` false.
+    entry (slot -1) writes its queries only, as does every entry with `write_cache` false. A padding entry may have more than max_q_len tokens; which of
+    its queries are then written is left open.
     `constants` promises that no kernel in flight on the stream writes cu_q, tok_seq, tok_pos, slots, inv_freq or the page table (a bound model's step):
     they are then read while the kernel ahead ends."""
     if qkv.is_cuda:
@@ -193,7 +194,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     a group read the cache anew, see `attention_e4m3_pays`). q, out [T, n_heads * head_dim], bfloat16 or
     float32; query head i reads kv head i // (n_heads / kv_heads); key j is visible to a token at p iff max(0, p - window + 1) <= j <= p
     (window 0: all up to p). Entry s owns the tokens cu_q[s] .. cu_q[s + 1] - 1, at consecutive positions, at most max_q_len; an entry may have none, and a
-    padding entry (slot -1) gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page
+    padding entry (slot -1), of any number of tokens, gets zeros. `max_kv_len`: an upper bound of any sequence's length after the step (None: as long as the page
     table has room for). `constants` promises that no kernel in flight on the stream writes cu_q, tok_pos, slots, the page table or a page before an
     entry's first new token's (a bound model's step): they are then read while the kernel ahead ends."""
     if q.is_cuda:

@@ -553,11 +553,13 @@ class GqaAttention(Mixer):
         n = qkv.shape[0]
         inv_freq, rot_dim = rotary if rotary is not None else (None, 0)
         q = torch.empty((n, self.q_width), dtype=qkv.dtype, device=qkv.device)
-        ops.rope_cache_write_e4m3(qkv, ctx.cu_q, ctx.tok_seq, ctx.tok_pos, ctx.slots, inv_freq, rot_dim, self.n_heads, q, site.codes(), ctx.max_q_len, ctx.err,
-                                  bias=bias, write_cache=writes_cache, constants=True)
+        span = ctx.max_span or ctx.max_q_len
+        over_codes = ctx.attention == "auto" and ops.attention_e4m3_pays(qkv.dtype, span, self.n_heads // self.n_kv)
+        ops.rope_cache_write_e4m3(qkv, ctx.cu_q, ctx.tok_seq, ctx.tok_pos, ctx.slots, inv_freq, rot_dim, self.n_heads, q, site.codes(),
+                                  span if over_codes else ctx.max_q_len, ctx.err, bias=bias, write_cache=writes_cache, constants=True)
         attended = torch.empty_like(q)
-        if ctx.attention == "auto" and ops.attention_e4m3_pays(qkv.dtype, ctx.max_q_len, self.n_heads // self.n_kv):
-            ops.attention_e4m3(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), self.n_heads, ctx.n_seqs, ctx.max_q_len, self.scale, self.window,
+        if over_codes:
+            ops.attention_e4m3(q, attended, ctx.cu_q, ctx.tok_pos, ctx.slots, site.codes(), self.n_heads, ctx.n_seqs, span, self.scale, self.window,
                                ctx.codes_scratch or ops.E4m3Scratch(q.device), ctx.err, ctx.max_kv_len, constants=True)
             return attended
         values = site.group.values
