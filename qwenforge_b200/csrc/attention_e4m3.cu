@@ -1115,20 +1115,23 @@ QF_EXPORT int qf_attention_e4m3_slots(int is_bf16, int head_dim, int rows) {
     return 0;
 }
 
-// q, out [tokens][n_heads * head_dim], on 16 bytes; single: there are as many tokens as entries, and an entry has one at the most; rows: of a block, 8 or 16; chunks: of the longest span, ceil(tokens *
+// q, out [n_tokens][n_heads * head_dim], on 16 bytes; single: there are as many tokens as entries, and an entry has one at the most; rows: of a block, 8 or 16; chunks: of the longest span, ceil(tokens *
 // n_heads / kv_heads / rows); most_pages: the most pages that a sequence reads; blocks: n_seqs * kv_heads * chunks * ceil(most_pages / 4), block_slots (of
 // qf_attention_e4m3_slots) at most. part_o [2 * blocks][rows][32 * ceil(head_dim / 32)], part_ml [2 * blocks][rows][2]; tickets [4 * blocks], zero before the
 // first call and after every call.
 QF_EXPORT int qf_attention_e4m3(int is_bf16, const void* q, void* out, const int* cu_q, const int* tok_pos, const int* slots, void* codes, float* scales,
                                 const int* table, long long page_bytes, long long page_scales, int table_stride, int columns, int n_slots, int kv_heads,
-                                int head_dim, int n_heads, int n_seqs, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window, int constants,
+                                int head_dim, int n_heads, int n_seqs, int n_tokens, int single, int rows, int chunks, int most_pages, int blocks, int block_slots, float scale, int window, int constants,
                                 float* part_o, float* part_ml, int* tickets, int* err, cudaStream_t stream) {
     const E4m3Site site{(unsigned char*)codes, scales, table, page_bytes, page_scales, table_stride, columns, n_slots, kv_heads, head_dim};
     if (n_seqs <= 0) return 0;
     if (head_dim <= 0 || head_dim % 16 || kv_heads <= 0 || n_heads <= 0 || n_heads % kv_heads || chunks <= 0 || most_pages <= 0 || most_pages >= 1 << 20 || columns <= 0 || n_slots <= 0 ||
         page_bytes % 16 || ((uintptr_t)codes | (uintptr_t)q | (uintptr_t)out) % 16 || page_bytes < 2ll * kv_heads * QF_PAGE * head_dim || page_scales < 2ll * kv_heads ||
-        blocks <= 0 || blocks > block_slots || window < 0 || (long long)n_seqs * kv_heads * chunks * (most_pages + 2ll * block_slots) > 0x7fffffffll)
+        (rows != 8 && rows != 16) || blocks <= 0 || blocks > block_slots || window < 0)
         return (int)cudaErrorInvalidValue;
+    // pages of all (sequence, kv head, rows) are counted in 32 bits: an entry has a block of rows for each `rows` of its own and one that is partly empty
+    const long long row_blocks = std::min((long long)n_seqs * chunks, (long long)n_tokens * (n_heads / kv_heads) / rows + n_seqs);
+    if (row_blocks * kv_heads * (most_pages + 2ll * block_slots) > 0x7fffffffll) return (int)cudaErrorInvalidValue;
     AttendArgs a{cu_q, tok_pos, slots, site, n_heads, n_heads / kv_heads, n_seqs, single, chunks, most_pages, block_slots, window, constants, 1, 0, scale * 1.4426950408889634f, part_o, part_ml, tickets, err};
 #define EA_ATTEND(T, D, NR) attend<T, D, NR>(q, out, a, blocks, stream)
     EA_ALL(EA_ATTEND)

@@ -62,7 +62,7 @@ int (*read_e4m3)(int, void*, long long, const int*, const int*, const int*, void
                  int, int*, Stream);
 int (*attention_e4m3_slots)(int, int, int);
 int (*attention_e4m3)(int, const void*, void*, const int*, const int*, const int*, void*, float*, const int*, long long, long long, int, int, int, int, int, int,
-                      int, int, int, int, int, int, int, float, int, int, float*, float*, int*, int*, Stream);
+                      int, int, int, int, int, int, int, int, float, int, int, float*, float*, int*, int*, Stream);
 PyObject* kernel_error = nullptr;
 
 const struct {
@@ -615,7 +615,7 @@ PyObject* e4m3_attended(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_RETURN_NONE;
     return code_of([&] {
         return attention_e4m3(type == at::kBFloat16, q->data_ptr(), out->data_ptr(), ints(cu), ints(pos), ints(slots), p.codes, p.scales, p.table, p.page_bytes,
-                              p.page_scales, p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, (int)heads, (int)seqs, most_q == 1 && tokens == seqs,
+                              p.page_scales, p.table_stride, p.columns, p.n_slots, p.kv_heads, p.head_dim, (int)heads, (int)seqs, (int)tokens, most_q == 1 && tokens == seqs,
                               (int)block_rows, (int)chunks, (int)most, (int)blocks, (int)block_slots, (float)scale, (int)window, constants != 0, at_ptr<float>(*part_o),
                               at_ptr<float>(*part_ml), at_ptr<int>(*tickets), at_ptr<int>(*err), stream());
     });

@@ -231,6 +231,6 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, tok_p
     blocks = min(block_slots, n_seqs * kv_heads * chunks * -(-most // E4M3_WARPS))
     scratch.ensure(block_slots, d, block_rows)
     _here("attention_e4m3: scratch", scratch.part_o, scratch.tickets)
-    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _P)(
-        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.place, n_heads, n_seqs,
+    _check(_function("attention_e4m3", "qf_attention_e4m3", _I, _P, _P, _P, _P, _P, *_SITE, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _P)(
+        is_bf16, q.data_ptr(), out.data_ptr(), cu_q.data_ptr(), tok_pos.data_ptr(), slots.data_ptr(), *site.place, n_heads, n_seqs, q.shape[0],
         max_q_len == 1 and q.shape[0] == n_seqs, block_rows, chunks, most, blocks, block_slots, scale, window, bool(constants), scratch.part_o.data_ptr(), scratch.part_ml.data_ptr(), scratch.tickets.data_ptr(), err.data_ptr(), _stream()), "attention_e4m3")

@@ -225,3 +225,12 @@ def test_random_scores_of_any_size(seqs, heads, kv_heads, dim, tokens, spread, d
     b.q = (b.q.float() * spread).to(dtype)
     b.check(floor=True)
     assert bool((b.run().view(-1, dim) != 0).any(-1).all())   # (so loose a tolerance would let a row of zeros pass)
+
+
+def test_many_sequences_beside_a_long_prompt():
+    """The largest entry's blocks of rows times all entries are more than 32 bits count; what there is to do is not."""
+    n = 900
+    pages, _ = scattered(n, 1024, seed=6)
+    b = Batch(pages, [1024] + [40] * (n - 1), [1024] + [1] * (n - 1), 64, 2, 16, torch.float32)
+    assert n * 2 * (1024 * 32 // 16) * (16 + 2 * cache_e4m3._slots_of(0, 16, 16)) > 2 ** 31
+    b.check()
