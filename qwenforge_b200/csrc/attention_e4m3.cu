@@ -739,7 +739,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             const bool own = abs(unit_measured - unit_v) > EA_APART || !(ks * most_by <= EA_LARGE);
             float corr[NR][2], m_tile[NR][2];
             uint32_t pb[TERMS][KT][NR][2];
-            auto weigh = [&](auto whole, auto under_own) {
+            auto weigh = [&](auto whole) {   // (whole: every row sees every position, and the maximum is the running one)
                 auto seen = [&](int t, int n, int e) {
                     if (decltype(whole)::value) return true;
                     const int key = key0 + 16 * t + 8 * (e >> 1) + g;
@@ -763,19 +763,16 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                         corr[n][e] = fast_exp2(m_run[n][e] - m);
                         m_run[n][e] = m;
                         shift[e] = 14.f - m;
-                        l_run[n][e] *= corr[n][e];
                     }
 #pragma unroll
                     for (int t = 0; t < KT; ++t) {
                         float(&x)[4] = s[t][n];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            if (decltype(under_own)::value) x[e] = __fadd_rn(__fsub_rn(__fmul_rn(x[e], by_k[e & 1]), m_tile[n][e & 1]), 14.f);
-                            else x[e] = fmaf(x[e], by_k[e & 1], shift[e & 1]);
-                            x[e] = fast_exp2(x[e]);
+                            const float under = __fadd_rn(__fsub_rn(__fmul_rn(x[e], by_k[e & 1]), m_tile[n][e & 1]), 14.f);
+                            x[e] = fast_exp2(!decltype(whole)::value && own ? under : fmaf(x[e], by_k[e & 1], shift[e & 1]));
                             if (!seen(t, n, e)) x[e] = 0.f;
-                            if (decltype(under_own)::value) sum[e & 1] += x[e];
-                            else l_run[n][e & 1] += x[e];
+                            sum[e & 1] += x[e];
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -784,15 +781,15 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                             if constexpr (TWO) pb[TERMS - 1][t][n][h] = transposed(pack_rest(x[2 * h], x[2 * h + 1], most));
                         }
                     }
-                    if (decltype(under_own)::value) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) l_run[n][e] = fmaf(fast_exp2(__fsub_rn(m_tile[n][e], m_run[n][e])), sum[e], l_run[n][e]);
+                    for (int e = 0; e < 2; ++e) {
+                        const float share = !decltype(whole)::value && own ? fast_exp2(__fsub_rn(m_tile[n][e], m_run[n][e])) : 1.f;
+                        l_run[n][e] = fmaf(l_run[n][e], corr[n][e], sum[e] * share);
                     }
                 }
             };
-            if (__builtin_expect(own, 0)) weigh(std::false_type{}, std::true_type{});
-            else if (full) weigh(std::true_type{}, std::false_type{});
-            else weigh(std::false_type{}, std::false_type{});
+            if (full && !own) weigh(std::true_type{});
+            else weigh(std::false_type{});
             bool by_token = false;   // a NaN that some of the rows do not see must not reach them: 0 * NaN
             if (!full && t_first != t_last) {
 #pragma unroll
