@@ -260,7 +260,7 @@ class PrefillGraphs:
         longest = step.max_q_len
         step = self.rounded(step, triples, want)
         key = (cache.serial,) + step.shape_key
-        if self.model.cache_dtype is not None:
+        if getattr(cache, "kv_dtype", None) is not None:
             step = dataclasses.replace(step, max_kv_len=length_bound(step.max_kv_len), max_span=self.span_bound(longest, step.max_q_len))
             key += (step.max_kv_len, step.max_span)
         held = self.graphs.pop(key, None)

@@ -22,11 +22,11 @@ def captured(monkeypatch, cache_dtype, steps):
         return Graph(), torch.zeros(step.packed.size, dtype=torch.int32), None, 0
 
     monkeypatch.setattr(PrefillGraphs, "_capture", capture)
-    graphs = PrefillGraphs(SimpleNamespace(cache_dtype=cache_dtype))
+    graphs = PrefillGraphs(SimpleNamespace())
     for entries in steps:
         triples = [(slot, start, [1] * n) for slot, (start, n) in enumerate(entries)]
         for _ in range(2):
-            graphs.run(SimpleNamespace(serial=1), pack_step(triples, None), triples, None)
+            graphs.run(SimpleNamespace(serial=1, kv_dtype=cache_dtype), pack_step(triples, None), triples, None)
     return seen
 
 
