@@ -27,11 +27,14 @@
 // differ leave no SM idle. A pair of several blocks leaves partial results (maximum, sum, output); the block that ends last, by a
 // ticket, joins them in their order, sixteen at a time, and the last of those the sixteens.
 //
-// Microseconds in a row of calls: a chat of 900 tokens, 14 heads over 2 of 64, 7.1; 8 of 4,096 8.9 (8.3 MB); one document of 32,000, 16 over 2 of 128, 14.4 (16.4 MB);
-// 64 of up to 8,000, 28 over 4 of 128, 57.4 (272 MB, 4.7 TB/s; a copy has 6.5); 256 of 8,000 each 340 (2.1 GB, 6.2 TB/s); 12 spans of up to five tokens
-// behind up to 3,000 25.2; float32, 20 of up to 3,500, 16 over 2 of 128, 14.3. Small calls are a chain: the plan from the lengths 2, first loads 1.3, the warps'
-// merge 1.3, bringing blocks together 2 to 4. Large ones are bound by memory where lengths are even; ragged ones and spans by the issue of some 540 instructions
-// a tile of 32 positions, in 8 warps of an SM whose steps wait for their own products, exponentials and conversions.
+// Microseconds, calls captured one behind another: a chat of 900 tokens, 14 heads over 2 of 64, 7.2; 8 of 4,096 9.0 (8.3 MB); one document of 32,000, 16 over 2 of 128,
+// 14.2 (16.4 MB); 64 of up to 8,000, 28 over 4 of 128, 57.5 (272 MB, 4.7 TB/s; a copy has 6.5); 256 of 8,000 each 345 to 360 (2.1 GB, 6 TB/s); 12 spans of up to five
+// tokens behind up to 3,000 25.0; float32, 20 of up to 3,500, 16 over 2 of 128, 14.5. Small calls are a chain: the plan from the lengths 2, first loads 1.3, the warps'
+// merge 1.3, bringing blocks together 2 to 4. That is no floor: `attention_decode` reads the 16.8 MB of 8 of 4,096 in bfloat16 in 6.8, with a plan that one launch makes
+// for all layers of a step. Here every warp goes through all entries' lengths three times, in 32s: 256 / 600 sequences of up to 300 tokens take 23.5 / 36, 28 over 4 of
+// 128 40 to 44 / 76, where their bytes are 1.6 / 4.0 and 6.5 / 15. Large calls are bound by memory where lengths are even; ragged ones and spans by the issue of some 550
+// instructions a tile of 32 positions, in 8 warps of an SM whose steps wait for their own products, exponentials and conversions. Blocks of 16 rows spill a
+// little for some head sizes (bytes stored a thread: bfloat16 128 16; float32 64 68, 112 112, 128 160).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -147,7 +150,8 @@ __device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bo
 }
 __device__ __forceinline__ bool holds_nan(uint32_t codes) { return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
 
-// NR: eights of rows of a block. Microseconds of the other choices in bfloat16, this one's first (heads of 64 are 14 over 2, of 128 28 over 4 where it does not say):
+// NR: eights of rows of a block. Microseconds of the other choices in bfloat16, this one's first (both sides of a pair in turn, pairs at several states of the kernel: its
+// own figures are at the head of this file; heads of 64 are 14 over 2, of 128 28 over 4 where it does not say):
 // SMALL's tiles and blocks as of the rest of D <= 64: 8 sequences of 4,096 tokens, heads of 64, 9.2 / 12.0, 64 of up to 8,000 24.5 / 25.0, a chat of 900
 // 7.7 / 7.4; three stages: 64 of up to 8,000, heads of 128, 58.3 / 60.8, one of 32,000, 16 over 2 of 128, 14.3 / 14.6, spans of five tokens, heads of
 // 64, 13.5 / 15.6; tiles of a whole page for heads of 128: 64 of up to 8,000 58.3 / 69, 8 of 2,000 to 4,000 12.0 / 13.7, alone with 2,000 tokens 8.9 / 8.3; three blocks
@@ -216,7 +220,7 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     }
 }
 
-// Pages whose time a pair's beginning and end take. Microseconds with 14 / 0: 64 sequences of up to 8,000 tokens, 28 heads over 4 of 128, 61 / 74, 12 spans of up to
+// Pages whose time a pair's beginning and end take. Microseconds with 14 / 0, in turn: 64 sequences of up to 8,000 tokens, 28 heads over 4 of 128, 61 / 74, 12 spans of up to
 // five tokens 26 / 47.
 #define EA_PAIR_COST 14
 #define EA_GROUP 16        // partial results that a block joins at once

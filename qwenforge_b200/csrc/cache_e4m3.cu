@@ -14,13 +14,14 @@
 //                  same one or two pieces (a row, eight pairs of the rotation) of every head, so their sines and cosines are worked out once
 //                  and stay in registers, a key's or value's elements stay there between amax and codes, and the next head's are loaded
 //                  meanwhile. One prompt of 8,192 tokens, 28 + 4 + 4 heads of 128 in bfloat16: 38 microseconds, 3.7 TB/s (142 MB, 22 at the
-//                  copy's rate): instructions bound it, two thirds of them the rotation and its angles; twelve float32 prompts of up to 900
-//                  tokens, 16 + 2 + 2 heads of 128: 17.5 microseconds, 3.9 TB/s.
+//                  copy's rate). It waits for its loads: 128 registers a thread leave four warps to a scheduler, with one head's rows each on their way; half of the
+//                  issue slots are used, and per issue 2.2 warps wait for memory, 0.9 for the instruction before. Twelve float32 prompts of up to
+//                  900 tokens, 16 + 2 + 2 heads of 128: 17.4 microseconds, 3.9 TB/s.
 //   write_any      single tokens, short spans, and rows or rotations that 16-byte accesses do not fit: a warp a head at a time over all rows of
 //                  a run; amax and codes are one warp's business, without a barrier. Sines and cosines come from shared memory, worked
 //                  out once per run. A key or value head is read twice, the second time from L1 or L2. One token of one sequence: 3.1
-//                  microseconds, of 96 sequences at 28 + 4 + 4 heads of 128 4.4: a chain of loads (position, page, scale), the angle, the
-//                  warp's maximum.
+//                  microseconds, of 96 sequences at 28 + 4 + 4 heads of 128 4.5: a chain of loads (position, page, scale), the angle, the
+//                  warp's maximum. Spans of 8 tokens of 64 sequences there: 10.1, for 1.4 of bytes: rows are loaded and turned twice, and a warp has a head alone.
 #include <algorithm>
 
 #include "e4m3.cuh"
@@ -419,7 +420,8 @@ write_runs_kernel(const T* __restrict__ qkv, const T* __restrict__ bias, long lo
     }
 }
 
-// Heads of a block of write_runs, which share its sines and cosines. Microseconds with 3, 4, 5, 6 and 9 of them: twelve float32 prompts of up to 900 tokens,
+// Heads of a block of write_runs, which share its sines and cosines (how many hardly matters to a long prompt: angles are not what it waits for) and make the grid's last
+// wave fuller or emptier, which is what the float32 figures show: other numbers of heads and tokens have it elsewhere. Microseconds with 3, 4, 5, 6 and 9 of them: twelve float32 prompts of up to 900 tokens,
 // 16 + 2 + 2 heads of 128, 20.0, 21.7, 17.5, 17.5 and 22.0; one of 8,192 in bfloat16, 28 + 4 + 4 heads of 128, 39.3, 36.9, 36.8, 37.4 and 37.3.
 #define EW_HEADS 6
 // Tokens of the longest span from which write_runs is the faster one. Microseconds, write_any / write_runs, bfloat16, spans of 8, 16 and 32 tokens: 14 + 2 + 2

@@ -140,8 +140,11 @@ def cache_read_e4m3(out: torch.Tensor, cu_q: torch.Tensor, tok_pos: torch.Tensor
 # Rows (tokens of a span times heads of a group) up to which `attention_e4m3` is the faster way in bfloat16: a tile of 16 rows reads the cache anew, while
 # `cache_read_e4m3` with the kernels for prompts reads and writes every position once. Microseconds, codes / read back and attended over, seven heads to a
 # group, spans of 4, 16, 32 and 64 tokens: 8 sequences behind 4,000 tokens, 2 kv heads of 64 15 / 42, 28 / 42, 42 / 42, 71 / 42, 4 of 128 30 / 89, 63 / 90,
-# 111 / 91, 194 / 92; behind 300 12 / 11, 13 / 11, 13 / 11, 21 / 12 and 16 / 18, 17 / 18, 29 / 18, 50 / 20. In float32, where the other way is
-# `attention_generic`, codes are faster throughout: one span of 256 behind 4,000 tokens 48 / 228 and 174 / 571, a prompt of 2,000 149 / 246 and 581 / 867.
+# 111 / 91, 194 / 92; behind 300 12 / 11, 13 / 11, 13 / 11, 21 / 12 and 16 / 18, 17 / 18, 29 / 18, 50 / 20. Length and number of sequences move the border, and the rule has
+# neither: 32 sequences behind 4,000 tokens 30 / 152, 71 / 153, 126 / 168, 237 / 181 and 74 / 361, 201 / 363, 377 / 366, 725 / 368 (spans of 32 at heads of 64 would gain a
+# quarter from codes), behind 300 13 / 15, 21 / 15, 36 / 17, 59 / 21 and 15 / 48, 52 / 49, 85 / 53, 151 / 60 (spans of 16 there lose a third to them). In float32, where the
+# other way is `attention_generic`, codes were faster at all sizes tried: one span of 256 behind 4,000 tokens 48 / 228 and 174 / 571, a prompt of 2,000 149 / 246 and 581 / 867;
+# longer ones were not tried.
 E4M3_PAYS_ROWS = 128
 
 
@@ -152,7 +155,7 @@ def attention_e4m3_pays(dtype: torch.dtype, max_q_len: int, group: int) -> bool:
 
 class E4m3Scratch:
     """Workspaces of `attention_e4m3`: the runs' sums with their maxima, and ticket counters (kept zero between calls by the kernel itself). Sized for
-    as many blocks as the device holds at once, whatever the lengths, so that only another head size or more rows of a block ask for more (2 to 10 MB). One
+    as many blocks as the device holds at once, whatever the lengths, so that only another head size or more rows of a block ask for more (1 to 5 MB). One
     instance serves calls that run one after another on one stream; what is captured into a graph has one of its own. Should a captured call
     share one all the same, its replays take their turn like calls: what a call outgrows is kept as long as the instance, because a graph may hold its address."""
     TICKETS = 4096   # four for each of 1,024 blocks, the most that a launch has; zero from here on, where memory that a capture hands out is not
