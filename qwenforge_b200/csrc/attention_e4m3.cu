@@ -49,9 +49,10 @@
 // within 2^40 units of one page (2^14 weights, 448, some hundred thousand positions), so that with three times this there is room for float32's 2^127 however
 // the units fall and rise.
 #define EA_APART 10
-// Scores in base 2 up to which a weight's exponent is score - (maximum - 14), in float32: that is within one of 14 at the most, and off by no more than a score's own
-// rounding. (From 2^25 on the largest weight could be float16's infinity.) Where scores may be larger, the maximum is taken off the rounded score first.
-#define EA_LARGE 8388608.f
+// Scores in base 2 up to which a weight's exponent is score - (maximum - 14), in float32: below 2^24 that is within one of 14 at the most, and off by no more than a
+// score's own rounding. (From 2^25 on the largest weight could be float16's infinity.) Where the row's largest query component, the page's scale and 448 allow
+// larger ones, the maximum is taken off the rounded score first.
+#define EA_LARGE 1.6e7f
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
@@ -638,7 +639,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
         // ---- the queries' fragments: lane (g, c) has row g's components of its column
         uint32_t qb[TERMS][NR][KW][2];
         float by[NR][2];   // scores of rows 8 n + 2 c + e in base-2 units: product * key scale * by
-        float most_by = 0.f;   // key scale * this is no less than any score: products of a row lie within D * 2^8 * 448
+        float most_by = 0.f;   // key scale * this is no less than any score: D * 448 * the largest query component * scale
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             float2 x[KW][2];
@@ -668,7 +669,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
             const float mine = pow2(up) * fabsf(a.scale_log2), down = copysignf(pow2(-up), a.scale_log2);
             by[n][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
             by[n][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
-            most_by = fmaxf(most_by, mine);
+            most_by = fmaxf(most_by, top * fabsf(a.scale_log2));
 #pragma unroll
             for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -679,7 +680,7 @@ attend_e4m3_kernel(const T* __restrict__ q, T* __restrict__ out, const __grid_co
                 }
         }
 
-        most_by = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_by))) * (D * 256.f * 448.f);   // (positive: in their bits' order)
+        most_by = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_by))) * (D * 448.f);   // (positive: in their bits' order)
 
         float o[DT][NR][4];   // components of columns 2 d (0, 1) and 2 d + 1 (2, 3) by rows 2 c, 2 c + 1
 #pragma unroll

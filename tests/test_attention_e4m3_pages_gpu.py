@@ -234,3 +234,14 @@ def test_many_sequences_beside_a_long_prompt():
     b = Batch(pages, [1024] + [40] * (n - 1), [1024] + [1] * (n - 1), 64, 2, 16, torch.float32)
     assert n * 2 * (1024 * 32 // 16) * (16 + 2 * cache_e4m3._slots_of(0, 16, 16)) > 2 ** 31
     b.check()
+
+
+@pytest.mark.parametrize("score", [5e6, 1.1e7, 1.2e7, -1.1e7])
+@FEW_AND_MANY
+@BOTH
+def test_equal_scores_as_large_as_their_factors_allow(seqs, heads, kv_heads, dim, tokens, score, dtype):
+    """Key components of 448: what the largest query component and the page's scale allow is what the scores are (1.6e7 and 1.7e7 in base 2)."""
+    b = large_batch(seqs, heads, kv_heads, dim, tokens, dtype)
+    b.codes[:, 0] = torch.full((), 448.0, device="cuda").to(torch.float8_e4m3fn)
+    b.scales[:, 0] = 2.0 ** -9
+    b.check(scale=score / (dim * 448 * 2.0 ** -9), same_scores=True)
