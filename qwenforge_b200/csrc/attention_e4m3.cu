@@ -47,11 +47,12 @@
 #define EA_NONE (-3.0e38f)   // the running maximum of a row that has seen nothing
 // How far (in powers of two) the values' units of a warp's pages may be from the one at which it last measured its outputs before it measures them again. An output is
 // within 2^40 units of one page (2^14 weights, 448, some hundred thousand positions), so that with three times this there is room for float32's 2^127 however
-// the units fall and rise.
+// the units fall and rise, and a weight that float16 keeps to 2^-39 only stays far below what its value can make of it. A model's pages are within a few powers of two;
+// measuring costs: 64 sequences of up to 8,000 tokens, 28 over 4 of 128, take 273 microseconds with values' scales of 2^-20 to 2^20 at random, for 57.
 #define EA_APART 10
 // Scores in base 2 up to which a weight's exponent is score - (maximum - 14), in float32: below 2^24 that is within one of 14 at the most, and off by no more than a
 // score's own rounding. (From 2^25 on the largest weight could be float16's infinity.) Where the row's largest query component, the page's scale and 448 allow
-// larger ones, the maximum is taken off the rounded score first.
+// larger ones, the maximum is taken off the rounded score first, and the tile goes the way of scales that are far apart (289 microseconds).
 #define EA_LARGE 1.6e7f
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
